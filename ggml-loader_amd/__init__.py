@@ -126,9 +126,11 @@ def _declare(core, hip, loader):
     _sig(core, "ggml_mul_mat_id", T, vp, T, T, T)
     _sig(core, "ggml_reshape_2d", T, vp, T, i64, i64)
     _sig(core, "ggml_reshape_3d", T, vp, T, i64, i64, i64)
+    _sig(core, "ggml_reshape_4d", T, vp, T, i64, i64, i64, i64)
     _sig(core, "ggml_view_1d", T, vp, T, i64, sz)
     _sig(core, "ggml_view_2d", T, vp, T, i64, i64, sz, sz)
     _sig(core, "ggml_view_3d", T, vp, T, i64, i64, i64, sz, sz, sz)
+    _sig(core, "ggml_view_4d", T, vp, T, i64, i64, i64, i64, sz, sz, sz, sz)
     _sig(core, "ggml_permute", T, vp, T, i32, i32, i32, i32)
     _sig(core, "ggml_transpose", T, vp, T)
     _sig(core, "ggml_cont", T, vp, T)
@@ -223,6 +225,8 @@ def _declare(core, hip, loader):
     _sig(hip, "ggml_backend_hip_graph_compute_static", i32, vp, vp)
     _sig(hip, "ggml_backend_hip_sample", i32, vp, vp, i64, C.POINTER(ggml_hip_sampler_params), vp, sz,
          C.c_double, C.POINTER(C.c_int32), C.POINTER(C.c_bool))
+    _sig(hip, "ggml_backend_hip_logprobs", i32, vp, vp, i64, i64, vp, C.c_int32, vp, vp, vp, vp)
+    _sig(hip, "ggml_backend_hip_refusal", C.c_char_p, T)
     _sig(hip, "ggml_backend_hip_set_fusion", None, vp, C.c_bool)
     _sig(hip, "ggml_backend_hip_set_profiling", None, vp, C.c_bool)
     _sig(hip, "ggml_backend_hip_set_profile_filter", None, vp, C.c_char_p)
@@ -282,6 +286,28 @@ def hip_sample(backend, logits_tensor, row: int, recent, u: float, *, temp: floa
     if st != 0:
         raise RuntimeError(f"ggml_backend_hip_sample failed ({st})")
     return int(tok.value), bool(used.value)
+
+
+def hip_logprobs(backend, logits_tensor, tokens, *, row: int = 0, n_rows: int | None = None, n_top: int = 0):
+    """ggml_backend_hip_logprobs on rows row .. row + n_rows - 1 of an F32 tensor in the backend's
+    buffer: (log probabilities of tokens, entropies, the n_top likeliest ids and their log
+    probabilities, [n_rows, n_top]). tokens: one id per row, or None (then the first is None)."""
+    import numpy as np
+    if tokens is None and n_rows is None:
+        raise ValueError("hip_logprobs: tokens or n_rows")
+    toks = None if tokens is None else np.ascontiguousarray(np.asarray(tokens, dtype=np.int32))
+    n = len(toks) if n_rows is None else n_rows
+    if toks is not None and toks.shape != (n,):
+        raise ValueError("hip_logprobs: one token per row")
+    ptr = lambda a: None if a is None else a.ctypes.data_as(C.c_void_p)  # noqa: E731
+    logprob = None if toks is None else np.empty(n, np.float32)
+    entropy = np.empty(n, np.float32)
+    ids, top = np.empty((n, max(n_top, 0)), np.int32), np.empty((n, max(n_top, 0)), np.float32)
+    st = libs()["hip"].ggml_backend_hip_logprobs(backend, logits_tensor, row, n, ptr(toks), n_top, ptr(logprob),
+                                                 ptr(entropy), ptr(ids), ptr(top))
+    if st != 0:
+        raise RuntimeError(f"ggml_backend_hip_logprobs failed ({st})")
+    return logprob, entropy, ids, top
 
 
 def hip_backend(device: int = 0):

@@ -486,7 +486,9 @@ struct ggml_tensor * ggml_ssm_conv(struct ggml_context * ctx, struct ggml_tensor
 struct ggml_tensor * ggml_ssm_scan(struct ggml_context * ctx, struct ggml_tensor * s, struct ggml_tensor * x,
         struct ggml_tensor * dt, struct ggml_tensor * A, struct ggml_tensor * B, struct ggml_tensor * C,
         struct ggml_tensor * ids, int version) {
-    ggml_tensor * r = ggml_new_tensor_1d(ctx, GGML_TYPE_F32, ggml_nelements(x) + ggml_nelements(s));
+    // the states of the sequences, not of the whole pool
+    const int64_t n_state = s->ne[0] * s->ne[1] * s->ne[2] * ids->ne[0];
+    ggml_tensor * r = ggml_new_tensor_1d(ctx, GGML_TYPE_F32, ggml_nelements(x) + n_state);
     set_op_param_i32(r, 0, version);
     r->op = GGML_OP_SSM_SCAN;
     r->src[0] = s; r->src[1] = x; r->src[2] = dt; r->src[3] = A; r->src[4] = B; r->src[5] = C; r->src[6] = ids;

@@ -66,6 +66,9 @@ struct hip_device {
     size_t smp_ints = 0;
     uint8_t * smp_ws = nullptr;
     size_t smp_ws_size = 0;
+    // log probabilities: the rows' results, then their tokens
+    int32_t * lp = nullptr;
+    size_t lp_words = 0;
     ggml_backend_buffer_type buft{};
     char name[64] = { 0 };
 };
@@ -423,6 +426,93 @@ int dot_kind(int wtype) {
 }
 
 bool is_2d_contig(const ggml_tensor * t) { return t->ne[2] == 1 && t->ne[3] == 1 && ggml_is_contiguous(t); }
+
+// ---- operands of the state space mixers' ops ----
+
+// a tensor's elements lie inside the memory it is a view of
+bool inside_base(const ggml_tensor * t) {
+    const ggml_tensor * base = t->view_src ? t->view_src : t;
+    unsigned __int128 end = t->view_src ? t->view_offs : 0;
+    for (int i = 0; i < GGML_MAX_DIMS; i++) {
+        if (t->ne[i] <= 0) return true;
+        end += (unsigned __int128) (t->ne[i] - 1) * t->nb[i];
+    }
+    return end + ggml_type_size(t->type) <= ggml_nbytes(base);
+}
+
+// F32 (or another 4-byte type) at strides of whole elements, the innermost extent contiguous
+bool plain_rows(const ggml_tensor * t, int type) {
+    return t && t->type == type && t->nb[0] == 4 && t->nb[1] % 4 == 0 && t->nb[2] % 4 == 0 && t->nb[3] % 4 == 0 && inside_base(t);
+}
+
+bool has_shape(const ggml_tensor * t, int64_t n0, int64_t n1, int64_t n2, int64_t n3) {
+    return t->ne[0] == n0 && t->ne[1] == n1 && t->ne[2] == n2 && t->ne[3] == n3;
+}
+
+const char * ssm_conv_refusal(const ggml_tensor * n) {
+    const ggml_tensor * sx = n->src[0], * c = n->src[1];
+    if (!sx || !c) return "ssm_conv: an operand is missing";
+    if (sx->type != GGML_TYPE_F32 || c->type != GGML_TYPE_F32 || n->type != GGML_TYPE_F32) return "ssm_conv: F32 only";
+    const int64_t K = c->ne[0], T = n->ne[1];
+    if (K < 1 || K > INT_MAX) return "ssm_conv: a filter of no taps";
+    if (c->ne[2] != 1 || c->ne[3] != 1 || sx->ne[3] != 1 || sx->ne[1] != c->ne[1] || sx->ne[0] != K - 1 + T ||
+        !has_shape(n, c->ne[1], T, sx->ne[2], 1)) return "ssm_conv: the operands' extents do not fit";
+    for (const ggml_tensor * t : { sx, c }) {
+        for (int i = 0; i < GGML_MAX_DIMS; i++) {
+            if (t->nb[i] % 4) return "ssm_conv: strides that are not whole elements";
+        }
+        if (!inside_base(t)) return "ssm_conv: an operand reaches past its tensor";
+    }
+    if (!ggml_is_contiguous(n)) return "ssm_conv: the result must be contiguous";
+    return nullptr;
+}
+
+const char * ssm_scan_refusal(const ggml_tensor * n) {
+    const ggml_tensor * s = n->src[0], * x = n->src[1], * dt = n->src[2], * A = n->src[3], * B = n->src[4], * C = n->src[5],
+                      * ids = n->src[6];
+    for (int i = 0; i < 7; i++) {
+        if (!n->src[i]) return "ssm_scan: an operand is missing";
+        if (!plain_rows(n->src[i], i == 6 ? GGML_TYPE_I32 : GGML_TYPE_F32)) {
+            return "ssm_scan: operands are F32 (ids I32) with a contiguous first extent, inside their tensors";
+        }
+    }
+    if (n->op_params[0] != 1) return "ssm_scan: version 1 only";
+    const int64_t N = s->ne[0], P = s->ne[1], H = s->ne[2], G = B->ne[1], T = x->ne[2], S = x->ne[3];
+    if (N < 1 || N > SSM_MAX_STATE) return "ssm_scan: 1 to 256 states per channel";
+    if (P < 1 || H < 1 || P > INT_MAX / H) return "ssm_scan: too many or no channels";
+    if (G < 1 || H % G) return "ssm_scan: the groups do not divide the heads";
+    if (!has_shape(x, P, H, T, S) || !has_shape(dt, H, T, S, 1) || !has_shape(B, N, G, T, S) || !has_shape(C, N, G, T, S) ||
+        (A->ne[0] != 1 && A->ne[0] != N) || !has_shape(A, A->ne[0], H, 1, 1) || !has_shape(ids, S, 1, 1, 1) ||
+        (S > 0 && s->ne[3] < 1)) return "ssm_scan: the operands' extents do not fit";
+    if (n->type != GGML_TYPE_F32 || !ggml_is_contiguous(n) || ggml_nelements(n) != P * H * T * S + N * P * H * S) {
+        return "ssm_scan: the result's extent does not fit";
+    }
+    return nullptr;
+}
+
+// why graph_compute refuses a graph with this node before it queues anything (nullptr: it does not)
+const char * node_refusal(const ggml_tensor * n) {
+    if (n->op == GGML_OP_SSM_CONV) return ssm_conv_refusal(n);
+    if (n->op == GGML_OP_SSM_SCAN) return ssm_scan_refusal(n);
+    return nullptr;
+}
+
+bool graph_refused(const ggml_cgraph * g) {
+    for (int i = 0; i < g->n_nodes; i++) {
+        const ggml_tensor * n = g->nodes[i];
+        const char * why = node_refusal(n);
+        if (!why && (n->op == GGML_OP_SSM_CONV || n->op == GGML_OP_SSM_SCAN)) {
+            for (int s = -1; s < GGML_MAX_SRC; s++) {
+                const ggml_tensor * t = s < 0 ? n : n->src[s];
+                if (t && !t->data && ggml_nelements(t) > 0) why = "an operand is not allocated";
+            }
+        }
+        if (!why) continue;
+        fprintf(stderr, "ggml-hip: %s (node '%s')\n", why, n->name);
+        return true;
+    }
+    return false;
+}
 
 // the nodes of one decode-attention chain (anchored at the K^T Q mul_mat)
 struct attn_match {
@@ -812,9 +902,52 @@ private:
                 }
                 return;
             }
+            case GGML_OP_SSM_CONV: op_ssm_conv(n); return;
+            case GGML_OP_SSM_SCAN: op_ssm_scan(n); return;
             default:
                 HIP_ABORT("op %s is not supported by the hip backend (node '%s')", ggml_op_name(n->op), n->name);
         }
+    }
+
+    // ---- state space mixers (operands checked by node_refusal before the graph ran) ----
+    void op_ssm_conv(ggml_tensor * n) {
+        const ggml_tensor * sx = n->src[0], * c = n->src[1];
+        ssm_conv_launch L{};
+        L.K = (int) c->ne[0];
+        L.D = n->ne[0]; L.T = n->ne[1]; L.S = n->ne[2];
+        L.st_j = L.x_t = (int64_t) sx->nb[0] / 4;
+        L.st_d = L.x_d = (int64_t) sx->nb[1] / 4;
+        L.st_s = L.x_s = (int64_t) sx->nb[2] / 4;
+        L.state = (const float *) sx->data;
+        L.x = L.state + (L.K - 1) * L.st_j;
+        L.w = (const float *) c->data;
+        L.w_k = (int64_t) c->nb[0] / 4;
+        L.w_d = (int64_t) c->nb[1] / 4;
+        L.y = (float *) n->data;
+        prof_scope ps(this, "ssm_conv", (double) (ggml_nbytes(n) * 2 + ggml_nbytes(c)));
+        launch_ssm_conv(L, st_);
+    }
+
+    void op_ssm_scan(ggml_tensor * n) {
+        const ggml_tensor * s = n->src[0], * x = n->src[1], * dt = n->src[2], * A = n->src[3], * B = n->src[4], * C = n->src[5],
+                          * ids = n->src[6];
+        auto f = [](const ggml_tensor * t) { return (const float *) t->data; };
+        auto nb = [](const ggml_tensor * t, int i) { return (int64_t) t->nb[i] / 4; };
+        ssm_scan_launch L{};
+        L.N = (int) s->ne[0]; L.P = (int) s->ne[1]; L.H = (int) s->ne[2]; L.G = (int) B->ne[1];
+        L.T = x->ne[2]; L.S = x->ne[3]; L.pool = s->ne[3];
+        L.s = f(s); L.s_p = nb(s, 1); L.s_h = nb(s, 2); L.s_row = nb(s, 3);
+        L.x = f(x); L.x_h = nb(x, 1); L.x_t = nb(x, 2); L.x_s = nb(x, 3);
+        L.dt = f(dt); L.dt_t = nb(dt, 1); L.dt_s = nb(dt, 2);
+        L.A = f(A); L.a_h = nb(A, 1); L.a_scalar = A->ne[0] == 1;
+        L.B = f(B); L.b_g = nb(B, 1); L.b_t = nb(B, 2); L.b_s = nb(B, 3);
+        L.C = f(C); L.c_g = nb(C, 1); L.c_t = nb(C, 2); L.c_s = nb(C, 3);
+        L.ids = (const int32_t *) ids->data; L.ids_s = nb(ids, 0);
+        L.y = (float *) n->data;
+        L.s_out = L.y + ggml_nelements(x);
+        const double st = (double) L.N * L.P * L.H * L.S * 4;
+        prof_scope ps(this, "ssm_scan", 2 * st + 4.0 * (2 * ggml_nelements(x) + ggml_nelements(dt) + 2 * ggml_nelements(B)));
+        launch_ssm_scan(L, st_);
     }
 
     void op_get_rows(ggml_tensor * n) {
@@ -2260,6 +2393,7 @@ void collect_profile(hip_backend_ctx * c) {
 
 // queues the graph's kernels on the device stream; a timed (profiled) compute also waits for them
 enum ggml_status be_compute_async(ggml_backend_t b, ggml_cgraph * g) {
+    if (graph_refused(g)) return GGML_STATUS_FAILED;
     hip_backend_ctx * c = (hip_backend_ctx *) b->context;
     hip_device & d = dev(c->device);
     c->timing = c->profiling && (c->computes++ % c->profile_every) == 0;
@@ -2308,6 +2442,7 @@ enum ggml_status compute_static(hip_backend_ctx * c, ggml_cgraph * g) {
         fprintf(stderr, "ggml-hip: graph_compute_static: profiling creates events; turn it off first\n");
         return GGML_STATUS_FAILED;
     }
+    if (graph_refused(g)) return GGML_STATUS_FAILED;
     scratch_arena own = std::move(c->scratch);
     c->scratch = scratch_arena{};
     c->scratch.fixed = true;
@@ -2512,6 +2647,78 @@ enum ggml_status ggml_backend_hip_sample(ggml_backend_t backend, const struct gg
     if (res[2] != SMP_OK) return fail("sampling kernel reported an error");
     *token = res[0];
     if (used_draw) *used_draw = res[1] != 0;
+    return GGML_STATUS_SUCCESS;
+}
+
+const char * ggml_backend_hip_refusal(const struct ggml_tensor * node) { return node ? node_refusal(node) : "no node"; }
+
+// (see the declaration for the contract)
+enum ggml_status ggml_backend_hip_logprobs(ggml_backend_t backend, const struct ggml_tensor * logits, int64_t row,
+                                           int64_t n_rows, const int32_t * tokens, int32_t n_top,
+                                           float * logprob, float * entropy, int32_t * top_ids, float * top_logprobs) {
+    auto fail = [](const char * why) {
+        fprintf(stderr, "ggml_backend_hip_logprobs: %s\n", why);
+        return GGML_STATUS_FAILED;
+    };
+    if (!logits) return fail("null argument");
+    if (logits->type != GGML_TYPE_F32 || logits->nb[0] != sizeof(float) || !inside_base(logits)) return fail("logits must be F32 with contiguous rows");
+    for (int i = 1; i < GGML_MAX_DIMS; i++) {
+        if (logits->nb[i] % sizeof(float)) return fail("logits must be F32 with contiguous rows");
+    }
+    const int64_t n = logits->ne[0], rows = ggml_nrows(logits);
+    if (n < 1 || n > INT_MAX / 4) return fail("row length out of range");
+    if (row < 0 || n_rows < 0 || row > rows || n_rows > rows - row) return fail("rows out of range");
+    if (n_top < 0 || n_top > GGML_HIP_LOGPROBS_MAX_TOP || n_top > n) return fail("n_top out of range");
+    if (logprob && !tokens && n_rows > 0) return fail("log probabilities of no tokens");
+    for (int64_t i = 0; tokens && i < n_rows; i++) {
+        if (tokens[i] < 0 || tokens[i] >= n) return fail("token out of range");
+    }
+    if (!ggml_backend_is_hip(backend)) return fail("not a HIP backend");
+    hip_backend_ctx * c = (hip_backend_ctx *) backend->context;
+    if (!logits->data || !logits->buffer || ggml_backend_buffer_get_type(logits->buffer) != ggml_backend_hip_buffer_type(c->device)) {
+        return fail("logits are not in this backend's device buffer");
+    }
+    hip_device & d = dev(c->device);
+    // so many rows at a time: their tokens fit an upload slot and their results the download area
+    const int64_t step = LOGPROBS_ROWS;
+    const int width = 2 + 2 * n_top;
+    for (int64_t r0 = 0; r0 < n_rows; r0 += step) {
+        const int nr = (int) std::min(step, n_rows - r0);
+        const size_t words = (size_t) nr * (width + 1);
+        if (words > d.lp_words) {
+            HIP_CHECK(hipStreamSynchronize(d.stream));
+            drained(d);
+            if (d.lp) HIP_CHECK(hipFree(d.lp));
+            d.lp_words = std::max(words, (size_t) 1 << 16);
+            HIP_CHECK(hipMalloc(&d.lp, d.lp_words * 4));
+        }
+        float * out = (float *) d.lp;
+        int32_t * toks = d.lp + (size_t) nr * width;
+        if (tokens) {
+            uint8_t * slot = upload_slot(d, nr * 4);
+            if (!slot) {
+                HIP_CHECK(hipStreamSynchronize(d.stream));
+                drained(d);
+                slot = upload_slot(d, nr * 4);
+            }
+            memcpy(slot, tokens + r0, nr * 4);
+            HIP_CHECK(hipMemcpyAsync(toks, slot, nr * 4, hipMemcpyHostToDevice, d.stream));
+        }
+        logprobs_launch L{ (const char *) logits->data, logits->ne[1], logits->ne[2], (int64_t) logits->nb[1], (int64_t) logits->nb[2],
+                           (int64_t) logits->nb[3], row + r0, nr, (int) n, n_top, tokens ? toks : nullptr, out };
+        launch_logprobs(L, d.stream);
+        const float * area = (const float *) download_area(d, (size_t) nr * width * 4);
+        HIP_CHECK(hipMemcpyAsync((void *) area, out, (size_t) nr * width * 4, hipMemcpyDeviceToHost, d.stream));
+        HIP_CHECK(hipStreamSynchronize(d.stream));
+        drained(d);
+        for (int i = 0; i < nr; i++) {
+            const float * o = area + (size_t) i * width;
+            if (logprob) logprob[r0 + i] = o[0];
+            if (entropy) entropy[r0 + i] = o[1];
+            if (top_ids && n_top) memcpy(top_ids + (r0 + i) * n_top, o + 2, n_top * 4);
+            if (top_logprobs && n_top) memcpy(top_logprobs + (r0 + i) * n_top, o + 2 + n_top, n_top * 4);
+        }
+    }
     return GGML_STATUS_SUCCESS;
 }
 

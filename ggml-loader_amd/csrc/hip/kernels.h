@@ -554,3 +554,53 @@ void launch_sample(const sample_request & r, hipStream_t st);
 // the sorted path: ws of sample_sorted_ws_bytes(n) bytes
 size_t sample_sorted_ws_bytes(int n);
 void launch_sample_sorted(const sample_request & r, void * ws, size_t ws_bytes, hipStream_t st);
+
+// ---- state space mixers (k_ssm.hip) ----
+// Short causal convolution over a sequence's rows. Row j of sequence s, channel d, is
+// state[j * st_j + d * st_d + s * st_s] for j < K - 1 (the rows before the step) and
+// x[(j - K + 1) * x_t + d * x_d + s * x_s] after them. With r(t, d) those rows,
+//   y[t, d] = sum_k w[k * w_k + d * w_d] * r(t + k, d) (+ bias[d]) (then SiLU)
+// for t < T, contiguous [D, T, S]. Strides in floats.
+struct ssm_conv_launch {
+    const float * state, * x, * w, * bias;
+    float *       y;
+    int64_t       st_j, st_d, st_s, x_t, x_d, x_s, w_k, w_d;
+    int64_t       T, D, S;
+    int           K;
+    int           silu;
+};
+void launch_ssm_conv(const ssm_conv_launch & L, hipStream_t st);
+
+// Selective scan: per sequence s, head h, channel p and state n, with d = softplus(dt[h, t, s]),
+//   state = exp(d * A[n or 0, h]) * state + d * x[p, h, t, s] * B[n, g, t, s]
+//   y[p, h, t, s] = sum_n state * C[n, g, t, s]          g = h / (H / G)
+// from the row ids[s] of the state pool (clamped to its rows); y contiguous [P, H, T, S], the final
+// states contiguous [N, P, H, S]. The innermost extent of every operand is contiguous; the strides
+// are in floats.
+constexpr int SSM_MAX_STATE = 256;
+struct ssm_scan_launch {
+    const float *   s, * x, * dt, * A, * B, * C;
+    const int32_t * ids;
+    float *         y, * s_out;
+    int64_t         s_p, s_h, s_row, x_h, x_t, x_s, dt_t, dt_s, a_h, b_g, b_t, b_s, c_g, c_t, c_s, ids_s;
+    int64_t         T, S, pool;
+    int             N, P, H, G;
+    int             a_scalar;      // one A per head
+};
+void launch_ssm_scan(const ssm_scan_launch & L, hipStream_t st);
+
+// ---- log probabilities (k_logprobs.hip) ----
+// Rows of logits: row r starts at base + off(r), off the byte offset of ggml row r of the tensor
+// (ne and nb over dims 1..3). out rows of 2 + 2k words: the log probability of the row's token
+// (0 where tokens is null), the entropy, k ids (I32), k log probabilities.
+// rows per launch: 64 KiB of tokens, and results of at most 16 MiB (the download area) at 128 alternatives
+constexpr int LOGPROBS_ROWS = 16384;
+struct logprobs_launch {
+    const char *    base;
+    int64_t         ne1, ne2, nb1, nb2, nb3;
+    int64_t         row0;
+    int             n_rows, n, k;
+    const int32_t * tokens;
+    float *         out;
+};
+void launch_logprobs(const logprobs_launch & L, hipStream_t st);

@@ -72,6 +72,34 @@ GGML_API enum ggml_status ggml_backend_hip_sample(ggml_backend_t backend, const 
                                                   const int32_t * recent, size_t n_recent, double u,
                                                   int32_t * token, bool * used_draw);
 
+// Log probabilities of given tokens under rows of logits that stay in device memory, with each
+// row's entropy and its likeliest tokens: what scoring a text or reporting a token's alternatives
+// needs, without reading the rows back. logits: an F32 tensor in this backend's buffer with
+// contiguous rows; rows row .. row + n_rows - 1 (ggml row index over ne[1..3]) are taken as
+// distributions softmax(l). Natural logarithms, in each row:
+//   logprob[i]               log p(tokens[i])
+//   entropy[i]               -sum p log p
+//   top_ids[i * n_top + j]   the j-th likeliest token (equal logits: the lower id first), and
+//   top_logprobs[...]        its log probability
+// A logit of -inf has no weight: its log probability is -inf, and its ids come last in the order.
+// Sums are 32-bit; values are within a few units of 2^-24 of the largest |logit - maximum| involved.
+// NaN stands for every value of a row without a distribution (a NaN logit, a largest logit that is
+// not finite); its ids are still ordered (NaN as -inf). Any of the four outputs may be NULL (not
+// wanted); tokens may be NULL without logprob. n_top is 0 (no alternatives) to
+// GGML_HIP_LOGPROBS_MAX_TOP, at most the row length. Synchronous, on the backend's stream: returns
+// when the outputs are on the host. Fails (GGML_STATUS_FAILED, with a message on stderr, and no
+// output written) for another backend or buffer, rows or tokens out of range, or a bad n_top.
+#define GGML_HIP_LOGPROBS_MAX_TOP 128
+GGML_API enum ggml_status ggml_backend_hip_logprobs(ggml_backend_t backend, const struct ggml_tensor * logits, int64_t row,
+                                                    int64_t n_rows, const int32_t * tokens, int32_t n_top,
+                                                    float * logprob, float * entropy, int32_t * top_ids, float * top_logprobs);
+
+// Why graph_compute refuses a graph that holds this node, before it queues anything, or NULL: the
+// checks of ssm_conv and ssm_scan (types, extents, strides that leave the tensor), whose graphs it
+// answers with GGML_STATUS_FAILED and this message. Needs no device. Other ops' conditions are
+// checked as they run.
+GGML_API const char * ggml_backend_hip_refusal(const struct ggml_tensor * node);
+
 // Graph-level fusion (fused norm+quantize, QKV/gate-up multi-GEMV, rope+KV append, split-KV
 // decode attention). On by default; off runs one kernel per ggml node. Used by the parity tests
 // to check both paths against the oracle.

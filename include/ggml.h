@@ -280,9 +280,18 @@ GGML_API struct ggml_tensor * ggml_l2_norm(struct ggml_context * ctx, struct ggm
 GGML_API struct ggml_tensor * ggml_concat(struct ggml_context * ctx, struct ggml_tensor * a, struct ggml_tensor * b, int dim);
 // silu(a) * b (same shapes)
 GGML_API struct ggml_tensor * ggml_swiglu_split(struct ggml_context * ctx, struct ggml_tensor * a, struct ggml_tensor * b);
-// sx: [d_conv - 1 + n_t, d_inner, n_s], c: [d_conv, d_inner] -> F32 [d_inner, n_t, n_s]
+// Short causal convolution over n_t tokens of n_s sequences: y[d, t, s] = sum_k c[k, d] sx[t + k, d, s].
+// sx: [d_conv - 1 + n_t, d_inner, n_s] (the last d_conv - 1 rows before the step, then the step's),
+// c: [d_conv, d_inner] -> F32 [d_inner, n_t, n_s]
 GGML_API struct ggml_tensor * ggml_ssm_conv(struct ggml_context * ctx, struct ggml_tensor * sx, struct ggml_tensor * c);
-// selective scan: F32 1-D [nelements(x) + nelements(s)], y followed by the new state (model.cpp:1187-1196)
+// Selective scan (model.cpp:1187-1196). With d = softplus(dt[h, t, s]), for every sequence s, head h,
+// channel p and state n, g = h / (n_head / n_group), token by token:
+//   state = exp(d * A[n or 0, h]) * state + d * x[p, h, t, s] * B[n, g, t, s]
+//   y[p, h, t, s] = sum_n C[n, g, t, s] * state
+// s: [d_state, head_dim, n_head, n_rows], a pool in which sequence s starts from row ids[s] (clamped
+// to the pool's rows); x: [head_dim, n_head, n_t, n_s]; dt: [n_head, n_t, n_s]; A: [d_state, n_head],
+// or [1, n_head] for one decay per head; B, C: [d_state, n_group, n_t, n_s]; ids: I32 [n_s]; version: 1.
+// F32 1-D: y [head_dim, n_head, n_t, n_s], then the final states [d_state, head_dim, n_head, n_s]
 GGML_API struct ggml_tensor * ggml_ssm_scan(struct ggml_context * ctx, struct ggml_tensor * s, struct ggml_tensor * x,
         struct ggml_tensor * dt, struct ggml_tensor * A, struct ggml_tensor * B, struct ggml_tensor * C,
         struct ggml_tensor * ids, int version);

@@ -1,0 +1,257 @@
+"""The state space mixers' operators on the HIP backend against float64 (ssm_ref, which carries the
+bound that each value is held to)."""
+import numpy as np
+import pytest
+
+import ssm_ref
+from gl import Graph, gl, ptr
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def hip():
+    b = gl.hip_backend(0)
+    yield b
+    gl.libs()["core"].ggml_backend_free(b)
+
+
+def near(got, want, bound, what=""):
+    """Each value within its bound; where the definition is not finite, the same kind of value."""
+    got, want, bound = got.reshape(want.shape).astype(np.float64), want, np.broadcast_to(bound, want.shape)
+    fine = np.isfinite(want)
+    assert np.array_equal(fine, np.isfinite(got)), what
+    off = np.abs(got - want)[fine] - (bound[fine] + 1e-37)
+    assert off.size == 0 or off.max() <= 0, (what, off.max(), (np.abs(got - want)[fine] / (bound[fine] + 1e-37)).max())
+
+
+def draw(rng, S, T, H, P, N, G, pool, a0, big_dt=False):
+    d = dict(
+        state=rng.standard_normal((pool, H, P, N)).astype(np.float32),
+        x=rng.standard_normal((S, T, H, P)).astype(np.float32),
+        dt=(rng.standard_normal((S, T, H)) * (8 if big_dt else 1) - (0 if big_dt else 3)).astype(np.float32),
+        A=-(0.5 + 8 * rng.random((H, a0))).astype(np.float32),
+        B=rng.standard_normal((S, T, G, N)).astype(np.float32),
+        C=rng.standard_normal((S, T, G, N)).astype(np.float32),
+        ids=rng.permutation(pool)[:S].astype(np.int32))
+    return d
+
+
+def scan_node(g, d):
+    S, T, H, P = d["x"].shape
+    pool, _, _, N = d["state"].shape
+    G = d["B"].shape[2]
+    t = lambda a, *ne: g.tensor(gl.F32, *ne, data=a)  # noqa: E731
+    return g.ssm_scan(t(d["state"], N, P, H, pool), t(d["x"], P, H, T, S), t(d["dt"], H, T, S), t(d["A"], d["A"].shape[1], H),
+                      t(d["B"], N, G, T, S), t(d["C"], N, G, T, S), g.tensor(gl.I32, S, data=d["ids"]), 1)
+
+
+def check_scan(hip, d, what="", clamp=False):
+    S, T, H, P = d["x"].shape
+    N = d["B"].shape[3]
+    with Graph(mem=1 << 20) as g:
+        out = g.compute(hip, scan_node(g, d))
+    ids = np.clip(d["ids"], 0, len(d["state"]) - 1) if clamp else d["ids"]
+    y, h, ye, he = ssm_ref.scan(d["state"][ids], d["x"], d["dt"], d["A"], d["B"], d["C"])
+    n = S * T * H * P
+    near(out[:n], y, ye, ("y", what))
+    near(out[n:], h, he, ("state", what))
+    return out
+
+
+# S, T, H, P, N, G, pool, A's extent
+SCANS = [
+    (1, 1, 1, 1, 1, 1, 1, 1), (1, 1, 5, 3, 7, 1, 1, 1), (3, 1, 6, 64, 128, 2, 5, 1), (2, 2, 4, 64, 128, 1, 2, 1),
+    (1, 17, 3, 5, 13, 3, 2, 1), (2, 63, 2, 64, 128, 1, 2, 1), (1, 64, 4, 64, 128, 2, 1, 1), (1, 65, 2, 64, 128, 2, 1, 1),
+    (2, 130, 2, 32, 16, 1, 3, 1), (1, 200, 3, 80, 96, 1, 1, 1), (1, 129, 2, 128, 256, 2, 1, 1), (1, 333, 2, 64, 64, 1, 1, 1),
+    (1, 90, 1, 33, 100, 1, 1, 1), (1, 70, 2, 48, 200, 1, 1, 1), (5, 7, 3, 64, 128, 3, 9, 1), (1, 1100, 2, 64, 128, 1, 1, 1),
+    # a decay per state: a head per channel, and heads of several channels
+    (1, 1, 300, 1, 16, 1, 1, 16), (2, 50, 130, 1, 16, 1, 3, 16), (1, 257, 67, 1, 8, 1, 1, 8), (3, 3, 65, 1, 32, 1, 3, 32),
+    (1, 40, 6, 1, 5, 2, 1, 5), (1, 33, 3, 4, 16, 1, 2, 16), (1, 25, 2, 2, 129, 2, 1, 129), (1, 1030, 64, 1, 16, 1, 1, 16),
+]
+
+
+@pytest.mark.parametrize("S, T, H, P, N, G, pool, a0", SCANS)
+def test_scan(hip, S, T, H, P, N, G, pool, a0):
+    rng = np.random.default_rng(S * 1000 + T * 7 + H + P + N)
+    check_scan(hip, draw(rng, S, T, H, P, N, G, pool, a0))
+
+
+@pytest.mark.parametrize("P, N, a0", [(64, 128, 1), (1, 16, 16), (5, 7, 1)])
+def test_scan_extreme_steps(hip, P, N, a0):
+    """Time steps from none (dt far below zero) to decays that forget everything."""
+    d = draw(np.random.default_rng(9), 2, 150, 3, P, N, 1, 2, a0, big_dt=True)
+    d["dt"][0, 5:9] = -200
+    d["dt"][0, 80:84] = 60
+    d["dt"][1, 0] = 1e4
+    check_scan(hip, d)
+
+
+@pytest.mark.parametrize("T", [0, 1, 100])
+def test_scan_decay_of_one_and_growth(hip, T):
+    d = draw(np.random.default_rng(10), 1, T, 3, 64, 128, 1, 1, 1)
+    d["A"][0], d["A"][1] = 0, 0.05                    # a state that keeps everything, one that grows
+    out = check_scan(hip, d)
+    if T == 0:
+        assert np.array_equal(out, d["state"].ravel())   # no token: the states as they are
+
+
+@pytest.mark.parametrize("T", [1, 70])
+def test_scan_ids(hip, T):
+    """Two sequences of one row, and ids outside the pool (clamped, never followed)."""
+    d = draw(np.random.default_rng(11), 4, T, 2, 64, 128, 1, 3, 1)
+    d["ids"] = np.array([2, 2, -1, 7], np.int32)
+    check_scan(hip, d, clamp=True)
+
+
+@pytest.mark.parametrize("T, at", [(1, 0), (100, 0), (100, 37), (100, 70), (200, 199)])
+@pytest.mark.parametrize("P, N, a0", [(64, 128, 1), (1, 16, 16)])
+@pytest.mark.parametrize("bad", [np.nan, np.inf])
+def test_scan_keeps_what_came_before_a_bad_value(hip, T, at, P, N, a0, bad):
+    """A value that is not finite reaches its own head's outputs from its token on, and nothing else:
+    earlier tokens, other heads and other sequences keep theirs."""
+    d = draw(np.random.default_rng(12), 2, T, 3, P, N, 1, 2, a0)
+    clean = check_scan(hip, d)
+    d["x"][1, at, 2, 0] = bad
+    with Graph(mem=1 << 20) as g:
+        out = g.compute(hip, scan_node(g, d))
+    n = d["x"].size
+    y, was = out[:n].reshape(d["x"].shape), clean[:n].reshape(d["x"].shape)
+    fine = np.ones(y.shape, bool)
+    fine[1, at:, 2, 0] = False
+    assert not np.isfinite(y[~fine]).any()
+    h, h0 = out[n:].reshape(2, 3, P, N), clean[n:].reshape(2, 3, P, N)
+    hf = np.ones(h.shape, bool)
+    hf[1, 2, 0] = False
+    assert not np.isfinite(h[~hf]).any()
+    y64, h64, ye, he = ssm_ref.scan(d["state"][d["ids"]], np.where(np.isfinite(d["x"]), d["x"], 0), d["dt"], d["A"], d["B"], d["C"])
+    near(y[fine], y64[fine], ye[fine])
+    near(h[hf], h64[hf], he[hf])
+
+
+def test_scan_of_strided_operands(hip):
+    """x, B and C as slices of one projection, dt of another, A of a table, a pool of wider rows."""
+    rng = np.random.default_rng(13)
+    S, T, H, P, N, G = 2, 75, 4, 64, 128, 2
+    d = draw(rng, S, T, H, P, N, G, 3, 1)
+    w = H * P + 2 * G * N + 3
+    rows = rng.standard_normal((S, T, w)).astype(np.float32)
+    steps = np.concatenate([rng.standard_normal((S, T, 5)).astype(np.float32), d["dt"]], 2)
+    d["x"] = rows[:, :, :H * P].reshape(S, T, H, P)
+    d["B"] = rows[:, :, H * P:H * P + G * N].reshape(S, T, G, N)
+    d["C"] = rows[:, :, H * P + G * N:w - 3].reshape(S, T, G, N)
+    with Graph(mem=1 << 20) as g:
+        r = g.tensor(gl.F32, w, T, S, data=rows)
+        x = g.view_4d(r, P, H, T, S, P * 4, w * 4, T * w * 4, 0)
+        B, Cm = (g.view_4d(r, N, G, T, S, N * 4, w * 4, T * w * 4, a * 4) for a in (H * P, H * P + G * N))
+        dt = g.view_3d(g.tensor(gl.F32, H + 5, T, S, data=steps), H, T, S, (H + 5) * 4, T * (H + 5) * 4, 20)
+        table = np.concatenate([d["A"], np.ones((H, 2), np.float32)], 1)
+        A = g.view_2d(g.tensor(gl.F32, 3, H, data=table), 1, H, 12, 0)
+        pool = np.concatenate([d["state"].reshape(3, -1), np.ones((3, 4), np.float32)], 1)
+        s = g.view_4d(g.tensor(gl.F32, pool.shape[1], 3, data=pool), N, P, H, 3, N * 4, N * P * 4, pool.shape[1] * 4, 0)
+        out = g.compute(hip, g.ssm_scan(s, x, dt, A, B, Cm, g.tensor(gl.I32, S, data=d["ids"]), 1))
+    y, h, ye, he = ssm_ref.scan(d["state"][d["ids"]], d["x"], d["dt"], d["A"], d["B"], d["C"])
+    near(out[:y.size], y, ye)
+    near(out[y.size:], h, he)
+
+
+@pytest.mark.parametrize("K, T, D, S", [(4, 1, 1, 1), (4, 1, 300, 5), (1, 9, 5, 1), (2, 5, 64, 1), (4, 2, 33, 2), (4, 100, 129, 1),
+                                       (3, 65, 64, 3), (7, 70, 40, 1), (4, 300, 1024, 1), (4, 0, 8, 1)])
+def test_conv(hip, K, T, D, S):
+    rng = np.random.default_rng(K + T + D)
+    sx = rng.standard_normal((S, D, K - 1 + T)).astype(np.float32)
+    w = rng.standard_normal((D, K)).astype(np.float32)
+    with Graph(mem=1 << 20) as g:
+        out = g.compute(hip, g.ssm_conv(g.tensor(gl.F32, K - 1 + T, D, S, data=sx), g.tensor(gl.F32, K, D, data=w)))
+    near(out, *ssm_ref.conv(sx, w))
+
+
+def test_conv_of_strided_operands(hip):
+    """The rows channel by channel in memory (a transposed view), the filters with a gap between them."""
+    rng = np.random.default_rng(21)
+    K, T, D = 4, 37, 50
+    rows = rng.standard_normal((K - 1 + T, D + 6)).astype(np.float32)
+    w = rng.standard_normal((D, K + 1)).astype(np.float32)
+    with Graph(mem=1 << 20) as g:
+        sx = g.transpose(g.view_2d(g.tensor(gl.F32, D + 6, K - 1 + T, data=rows), D, K - 1 + T, (D + 6) * 4, 8))
+        c = g.view_2d(g.tensor(gl.F32, K + 1, D, data=w), K, D, (K + 1) * 4, 0)
+        out = g.compute(hip, g.ssm_conv(sx, c))
+    near(out, *ssm_ref.conv(rows[:, 2:2 + D].T[None], w[:, :K]))
+
+
+class Mixer:
+    """The convolution with its state, bias and SiLU as a mixer's graph has it. In place: the new rows
+    go back into the state they came from."""
+
+    def __init__(self, g, state, rows, w, bias, in_place, act=True, D=None):
+        S, T, W = rows.shape
+        D, K = w.shape
+        self.st = g.tensor(gl.F32, K - 1, D, S, data=state) if K > 1 else None
+        x = g.view_3d(g.tensor(gl.F32, W, T, S, data=rows), D, T, S, W * 4, T * W * 4, 0)
+        sx = g.concat(self.st, g.transpose(x), 0)
+        nb = sx.contents.nb
+        dest = self.st if in_place else g.tensor(gl.F32, K - 1, D, S, data=np.zeros_like(state))
+        self.new = g.cpy(g.view_3d(sx, K - 1, D, S, nb[1], nb[2], T * 4), dest)
+        y = g.ssm_conv(sx, g.tensor(gl.F32, K, D, data=w))
+        if bias is not None:
+            y = g.add(y, g.tensor(gl.F32, D, data=bias))
+        self.y = g.silu(y) if act else y
+
+
+@pytest.mark.parametrize("fusion", [True, False])
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("K, T, D, S, W, bias, act", [
+    (4, 1, 8, 1, 8, True, True), (4, 1, 260, 7, 300, True, True), (4, 2, 65, 2, 65, True, True), (4, 3, 64, 3, 70, False, True),
+    (4, 64, 64, 1, 128, True, True), (4, 67, 130, 2, 131, True, True), (2, 5, 33, 1, 40, True, True), (3, 200, 512, 1, 1100, False, True),
+    (4, 300, 1000, 1, 1000, True, False), (6, 4, 20, 2, 20, True, True), (4, 21, 44, 1, 44, False, False)])
+def test_conv_with_its_state(hip, fusion, in_place, K, T, D, S, W, bias, act):
+    rng = np.random.default_rng(K * T + D)
+    state = rng.standard_normal((S, D, K - 1)).astype(np.float32)
+    rows = rng.standard_normal((S, T, W)).astype(np.float32)
+    w = rng.standard_normal((D, K)).astype(np.float32)
+    b = rng.standard_normal(D).astype(np.float32) if bias else None
+    sx = np.concatenate([state, rows[:, :, :D].transpose(0, 2, 1)], 2)
+    gl.libs()["hip"].ggml_backend_hip_set_fusion(hip, fusion)
+    try:
+        with Graph(mem=1 << 20) as g:
+            m = Mixer(g, state, rows, w, b, in_place, act)
+            new, y = g.compute(hip, [m.new, m.y])
+    finally:
+        gl.libs()["hip"].ggml_backend_hip_set_fusion(hip, True)
+    assert np.array_equal(new.reshape(S, D, K - 1), sx[:, :, T:])
+    near(y, *ssm_ref.conv(sx, w, b, act))
+
+
+def test_static_compute(hip):
+    d = draw(np.random.default_rng(31), 1, 150, 2, 64, 128, 1, 1, 1)
+    with Graph(mem=1 << 20) as g:
+        n = scan_node(g, d)
+        want = g.compute(hip, n)
+        core = g.core
+        gf = core.ggml_new_graph(g.ctx)
+        core.ggml_build_forward_expand(gf, n)
+        assert gl.libs()["hip"].ggml_backend_hip_graph_compute_static(hip, gf) == 0
+        assert np.array_equal(g.read(n), want)
+
+
+def test_refused_graphs_run_nothing(hip, capfd):
+    """A refused node fails the whole graph before its first kernel: the copy beside it is not made."""
+    with Graph(mem=1 << 20) as g:
+        a = g.tensor(gl.F32, 16, data=np.ones(16, np.float32))
+        b = g.tensor(gl.F32, 16, data=np.zeros(16, np.float32))
+        d = draw(np.random.default_rng(5), 1, 2, 2, 4, 8, 1, 1, 1)
+        s = g.tensor(gl.F32, 8, 4, 2, 1, data=d["state"])
+        x = g.tensor(gl.F32, 4, 2, 2, 1, data=d["x"])
+        dt = g.tensor(gl.F32, 2, 2, 1, data=d["dt"])
+        bc = g.tensor(gl.F32, 8, 1, 2, 1, data=d["B"])
+        n = g.ssm_scan(s, x, dt, g.tensor(gl.F32, 1, 2, data=d["A"]), bc, bc, g.tensor(gl.I32, 1, data=d["ids"]), 3)
+        gf = g.core.ggml_new_graph(g.ctx)
+        for t in (g.cpy(a, b), n):
+            g.core.ggml_build_forward_expand(gf, t)
+        g.buf = g.core.ggml_backend_alloc_ctx_tensors(g.ctx, hip)
+        for t, v in g.inputs:
+            g.core.ggml_backend_tensor_set(t, ptr(v), 0, v.nbytes)
+        assert g.core.ggml_backend_graph_compute(hip, gf) == -1
+        assert gl.libs()["hip"].ggml_backend_hip_graph_compute_static(hip, gf) == -1
+        assert not g.read(b).any()
+    assert "version 1 only" in capfd.readouterr().err
