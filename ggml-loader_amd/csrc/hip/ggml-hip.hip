@@ -376,7 +376,8 @@ enum fuse_bits {
     FUSE_ROUTEG = 1024, // one token's MoE routing inside its routed gate/up GEMV launch
     FUSE_ACCO   = 2048, // one-query attention output accumulated by PV, read as doubles by its GEMVs
     FUSE_WSUMQ  = 4096, // MoE weighted sum also writes the next rms_norm * w as Q8_K (several tokens)
-    FUSE_ALL    = 8191,
+    FUSE_SSM    = 8192, // state rows joined, convolution, bias, SiLU and the new state in one launch
+    FUSE_ALL    = 16383,
 };
 
 struct hip_backend_ctx {
@@ -454,7 +455,7 @@ const char * ssm_conv_refusal(const ggml_tensor * n) {
     if (!sx || !c) return "ssm_conv: an operand is missing";
     if (sx->type != GGML_TYPE_F32 || c->type != GGML_TYPE_F32 || n->type != GGML_TYPE_F32) return "ssm_conv: F32 only";
     const int64_t K = c->ne[0], T = n->ne[1];
-    if (K < 1 || K > INT_MAX) return "ssm_conv: a filter of no taps";
+    if (K < 1 || K > SSM_MAX_TAPS) return "ssm_conv: 1 to 32 taps";
     if (c->ne[2] != 1 || c->ne[3] != 1 || sx->ne[3] != 1 || sx->ne[1] != c->ne[1] || sx->ne[0] != K - 1 + T ||
         !has_shape(n, c->ne[1], T, sx->ne[2], 1)) return "ssm_conv: the operands' extents do not fit";
     for (const ggml_tensor * t : { sx, c }) {
@@ -801,6 +802,10 @@ private:
             case GGML_OP_UNARY:
                 if (fuse(FUSE_SWIGLU) && op_swiglu(i)) return;
                 break;
+            case GGML_OP_CONCAT:
+                if (op_conv_state(i)) return;
+                break;
+            case GGML_OP_SSM_CONV: op_ssm_conv(i); return;
             default: break;
         }
         wrote_.push_back(n);
@@ -902,30 +907,146 @@ private:
                 }
                 return;
             }
-            case GGML_OP_SSM_CONV: op_ssm_conv(n); return;
-            case GGML_OP_SSM_SCAN: op_ssm_scan(n); return;
+                        case GGML_OP_SSM_SCAN: op_ssm_scan(n); return;
             default:
                 HIP_ABORT("op %s is not supported by the hip backend (node '%s')", ggml_op_name(n->op), n->name);
         }
     }
 
     // ---- state space mixers (operands checked by node_refusal before the graph ran) ----
-    void op_ssm_conv(ggml_tensor * n) {
-        const ggml_tensor * sx = n->src[0], * c = n->src[1];
+    // the bytes a tensor's elements span
+    struct span { const char * b, * e; };
+    static span span_of(const ggml_tensor * t) {
+        const char * p = (const char *) t->data;
+        if (ggml_nelements(t) == 0) return { p, p };
+        size_t n = ggml_type_size(t->type) * (size_t) (t->ne[0] / ggml_blck_size(t->type) - 1) + ggml_type_size(t->type);
+        if (!ggml_is_quantized(t->type)) n = (size_t) (t->ne[0] - 1) * t->nb[0] + ggml_type_size(t->type);
+        for (int i = 1; i < GGML_MAX_DIMS; i++) n += (size_t) (t->ne[i] - 1) * t->nb[i];
+        return { p, p + n };
+    }
+    static bool overlap(const ggml_tensor * a, const ggml_tensor * b) {
+        const span x = span_of(a), y = span_of(b);
+        return x.b < y.e && y.b < x.e;
+    }
+    // writing `to` at node `from` instead of at node `at`: no node between the two (fused ones aside)
+    // reads or writes that memory
+    bool may_write_early(int from, int at, const ggml_tensor * to, const std::vector<int> & fused) const {
+        for (int i = from + 1; i < at; i++) {
+            const ggml_tensor * n = g_->nodes[i];
+            if (is_view_op(n->op) || std::find(fused.begin(), fused.end(), i) != fused.end()) continue;
+            if (overlap(n, to)) return false;
+            for (int s = 0; s < GGML_MAX_SRC; s++) {
+                if (n->src[s] && overlap(n->src[s], to)) return false;
+            }
+        }
+        return true;
+    }
+
+    // A convolution's bias and SiLU in its own launch: conv -> add(bias over the channels) -> silu, as far
+    // as each has no other reader. Returns the node that the launch writes.
+    int conv_epilogue(int conv, ssm_conv_launch & L, std::vector<int> & fused) const {
+        int last = conv;
+        if (!fuse(FUSE_SSM) || c_.cb) return last;
+        int u = sole_user(last);
+        if (u >= 0 && g_->nodes[u]->op == GGML_OP_ADD && g_->nodes[u]->src[0] == g_->nodes[last]) {
+            const ggml_tensor * b = g_->nodes[u]->src[1];
+            if (b->type == GGML_TYPE_F32 && has_shape(b, L.D, 1, 1, 1) && b->nb[0] == 4 && b != g_->nodes[last] && ready(b)) {
+                L.bias = (const float *) b->data;
+                fused.push_back(last = u);
+                u = sole_user(last);
+            }
+        }
+        if (u >= 0 && g_->nodes[u]->op == GGML_OP_UNARY && g_->nodes[u]->op_params[0] == GGML_UNARY_OP_SILU) {
+            L.silu = 1;
+            fused.push_back(last = u);
+        }
+        return last;
+    }
+
+    void run_conv(ssm_conv_launch & L, const ggml_tensor * conv, const ggml_tensor * out, const std::vector<int> & fused) {
+        const ggml_tensor * c = conv->src[1];
+        L.w = (const float *) c->data;
+        L.w_k = (int64_t) c->nb[0] / 4;
+        L.w_d = (int64_t) c->nb[1] / 4;
+        L.y = (float *) out->data;
+        for (int i : fused) done_[i] = true;
+        wrote_.push_back(out);
+        prof_scope ps(this, "ssm_conv", 8.0 * (L.D * L.S * (L.T + (L.new_state ? L.K - 1 : 0))));
+        launch_ssm_conv(L, st_);
+    }
+
+    void op_ssm_conv(int i) {
+        const ggml_tensor * n = g_->nodes[i], * sx = n->src[0];
         ssm_conv_launch L{};
-        L.K = (int) c->ne[0];
+        L.K = (int) n->src[1]->ne[0];
         L.D = n->ne[0]; L.T = n->ne[1]; L.S = n->ne[2];
         L.st_j = L.x_t = (int64_t) sx->nb[0] / 4;
         L.st_d = L.x_d = (int64_t) sx->nb[1] / 4;
         L.st_s = L.x_s = (int64_t) sx->nb[2] / 4;
         L.state = (const float *) sx->data;
         L.x = L.state + (L.K - 1) * L.st_j;
-        L.w = (const float *) c->data;
-        L.w_k = (int64_t) c->nb[0] / 4;
-        L.w_d = (int64_t) c->nb[1] / 4;
-        L.y = (float *) n->data;
-        prof_scope ps(this, "ssm_conv", (double) (ggml_nbytes(n) * 2 + ggml_nbytes(c)));
-        launch_ssm_conv(L, st_);
+        std::vector<int> fused;
+        const int out = conv_epilogue(i, L, fused);
+        run_conv(L, n, g_->nodes[out], fused);
+    }
+
+    // concat(state, new rows) -> ssm_conv, with the copy of the last rows into the next state: the rows
+    // are read where they are, the joined tensor is not written
+    bool op_conv_state(int i) {
+        const ggml_tensor * j = g_->nodes[i], * st = j->src[0], * x = j->src[1];
+        if (!fuse(FUSE_SSM) || c_.cb || is_output(i) || j->op_params[0] != 0 || j->type != GGML_TYPE_F32) return false;
+        int conv = -1, view = -1;
+        for (int u : users_[i]) {
+            const ggml_tensor * n = g_->nodes[u];
+            if (n->op == GGML_OP_SSM_CONV && n->src[0] == j && n->src[1] != j && conv < 0) conv = u;
+            else if (n->op == GGML_OP_VIEW && view < 0) view = u;
+            else return false;
+        }
+        if (conv < 0) return false;
+        const ggml_tensor * n = g_->nodes[conv];
+        if (!ready(n->src[1])) return false;
+        ssm_conv_launch L{};
+        L.K = (int) n->src[1]->ne[0];
+        L.D = n->ne[0]; L.T = n->ne[1]; L.S = n->ne[2];
+        if (st->ne[0] != L.K - 1 || L.T < 1) return false;
+        for (const ggml_tensor * t : { st, x }) {
+            for (int k = 0; k < GGML_MAX_DIMS; k++) {
+                if (t->nb[k] % 4) return false;
+            }
+            if (!inside_base(t)) return false;
+        }
+        std::vector<int> fused = { conv };
+        int copy = -1;
+        if (view >= 0) {
+            // the joined tensor's last K - 1 steps, copied in order
+            const ggml_tensor * v = g_->nodes[view];
+            copy = sole_user(view);
+            if (copy < 0 || !has_shape(v, L.K - 1, L.D, L.S, 1) || v->nb[0] != 4 || v->nb[1] != j->nb[1] || v->nb[2] != j->nb[2] ||
+                (const char *) v->data != (const char *) j->data + L.T * 4) return false;
+            const ggml_tensor * cp = g_->nodes[copy];
+            if (cp->op != GGML_OP_CPY || cp->src[0] != v || cp->type != GGML_TYPE_F32 || !ggml_is_contiguous(cp)) return false;
+            fused.push_back(view);
+            fused.push_back(copy);
+        }
+        const int out = conv_epilogue(conv, L, fused);
+        if (copy >= 0) {
+            const ggml_tensor * cp = g_->nodes[copy];
+            const bool same = cp->data == st->data && ggml_is_contiguous(st);
+            if ((!same && overlap(cp, st)) || overlap(cp, x) || overlap(cp, n->src[1]) || overlap(cp, g_->nodes[out])) return false;
+            for (int f : fused) {
+                const ggml_tensor * t = g_->nodes[f];
+                if (t->op == GGML_OP_ADD && overlap(cp, t->src[1])) return false;
+            }
+            if (!may_write_early(i, copy, cp, fused)) return false;
+            L.new_state = (float *) cp->data;
+            wrote_.push_back(cp);
+        }
+        L.state = (const float *) st->data;
+        L.st_j = (int64_t) st->nb[0] / 4; L.st_d = (int64_t) st->nb[1] / 4; L.st_s = (int64_t) st->nb[2] / 4;
+        L.x = (const float *) x->data;
+        L.x_t = (int64_t) x->nb[0] / 4; L.x_d = (int64_t) x->nb[1] / 4; L.x_s = (int64_t) x->nb[2] / 4;
+        run_conv(L, n, g_->nodes[out], fused);
+        return true;
     }
 
     void op_ssm_scan(ggml_tensor * n) {

@@ -18,21 +18,165 @@ __device__ __forceinline__ float softplus(float x) { return x > 20.0f ? x : log1
 // ---------------------------------------------------------------------------------------------
 // short causal convolution
 
-// one thread per output, the channel fastest
-__global__ __launch_bounds__(256) void ssm_conv_kernel(ssm_conv_launch L) {
-    const int64_t i = (int64_t) blockIdx.x * 256 + threadIdx.x;
-    if (i >= L.D * L.T * L.S) return;
-    const int64_t d = i % L.D, t = i / L.D % L.T, s = i / (L.D * L.T);
-    const float * w = L.w + d * L.w_d;
-    const float * sp = L.state + d * L.st_d + s * L.st_s;
-    const float * xp = L.x + d * L.x_d + s * L.x_s;
-    float v = L.bias ? L.bias[d] : 0.0f;
-    for (int k = 0; k < L.K; k++) {
-        const int64_t j = t + k;
-        v = fmaf(w[k * L.w_k], j < L.K - 1 ? sp[j * L.st_j] : xp[(j - L.K + 1) * L.x_t], v);
+// The operator reads each row and writes each output once, so it is bound by memory. Two kernels, by
+// the order of the rows: channels next to each other (a projection's rows, as the executor's fused
+// form has them) need no exchange between lanes; steps next to each other (the joined rows of the
+// plain node) are turned round in LDS. A step of one token is latency: one round of loads.
+
+__device__ __forceinline__ float silu(float v) { return v * __builtin_amdgcn_rcpf(1.0f + exp2_hw(-v * LOG2E)); }
+
+template <int V> struct chunk { float v[V]; };
+template <int V> __device__ __forceinline__ chunk<V> ldv(const float * p) {
+    chunk<V> c;
+    if constexpr (V == 4) {
+        const float4 f = *(const float4 *) p;
+        c.v[0] = f.x; c.v[1] = f.y; c.v[2] = f.z; c.v[3] = f.w;
+    } else {
+        c.v[0] = *p;
     }
-    if (L.silu) v = v / (1.0f + expf(-v));
-    L.y[i] = v;
+    return c;
+}
+template <int V> __device__ __forceinline__ void stv(float * p, const chunk<V> & c) {
+    if constexpr (V == 4) *(float4 *) p = make_float4(c.v[0], c.v[1], c.v[2], c.v[3]);
+    else *p = c.v[0];
+}
+
+// Channels contiguous (x_d == 1), K taps, V channels and TT tokens per thread, all rows of a tile in
+// flight at once. The first tile's threads, the only ones that touch the state, write the new one:
+// it may be the old one's own memory.
+template <int K, int V, int TT>
+__global__ __launch_bounds__(256) void ssm_conv_rows_kernel(ssm_conv_launch L, int blocks) {
+    const int cb = (int) (blockIdx.x % (unsigned) blocks);
+    const int64_t t0 = (int64_t) (blockIdx.x / (unsigned) blocks) * TT;
+    const int64_t d = ((int64_t) cb * blockDim.x + threadIdx.x) * V;
+    if (d >= L.D) return;
+    float w[V][K];
+#pragma unroll
+    for (int i = 0; i < V; i++) {
+#pragma unroll
+        for (int k = 0; k < K; k++) w[i][k] = L.w[(d + i) * L.w_d + k * L.w_k];
+    }
+    chunk<V> b{};
+    if (L.bias) b = ldv<V>(L.bias + d);
+    for (int64_t s = blockIdx.y; s < L.S; s += gridDim.y) {
+        const float * xp = L.x + d + s * L.x_s;
+        const float * sp = L.state + d * L.st_d + s * L.st_s;
+        chunk<V> r[TT + K - 1], last[K > 1 ? K - 1 : 1];
+#pragma unroll
+        for (int j = 0; j < TT + K - 1; j++) {
+            const int64_t t = t0 + j - (K - 1);   // a row past the last is the last again, and not used
+            r[j] = ldv<V>(xp + (t < 0 ? 0 : t < L.T ? t : L.T - 1) * L.x_t);
+        }
+        if (t0 < K - 1) {
+#pragma unroll
+            for (int j = 0; j < K - 1; j++) {
+                if (t0 + j < K - 1) {
+#pragma unroll
+                    for (int i = 0; i < V; i++) r[j].v[i] = sp[i * L.st_d + (t0 + j) * L.st_j];
+                }
+            }
+        }
+        if (L.new_state && t0 == 0) {
+#pragma unroll
+            for (int j = 0; j < K - 1; j++) {
+                const int64_t t = L.T + j - (K - 1);
+                if (t >= 0) {
+                    last[j] = ldv<V>(xp + t * L.x_t);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < V; i++) last[j].v[i] = sp[i * L.st_d + (L.T + j) * L.st_j];
+                }
+            }
+            float * np = L.new_state + (s * L.D + d) * (K - 1);
+#pragma unroll
+            for (int i = 0; i < V; i++) {
+#pragma unroll
+                for (int j = 0; j < K - 1; j++) np[i * (K - 1) + j] = last[j].v[i];
+            }
+        }
+        float * y = L.y + d + L.D * (t0 + L.T * s);
+#pragma unroll
+        for (int j = 0; j < TT; j++) {
+            if (t0 + j >= L.T) break;
+            chunk<V> o;
+#pragma unroll
+            for (int i = 0; i < V; i++) {
+                float v = b.v[i];
+#pragma unroll
+                for (int k = 0; k < K; k++) v = fmaf(w[i][k], r[j + k].v[i], v);
+                o.v[i] = L.silu ? silu(v) : v;
+            }
+            stv<V>(y + j * L.D, o);
+        }
+    }
+}
+
+// Rows in any order: 64 channels by 64 tokens and the K - 1 rows before them through LDS, read with
+// the steps across the lanes and used with the channels across them. An odd row length keeps the
+// lanes' reads on different banks.
+__global__ __launch_bounds__(256) void ssm_conv_tile_kernel(ssm_conv_launch L, int blocks) {
+    extern __shared__ float rows[];
+    const int width = 64 + L.K - 1, stride = width | 1, tid = threadIdx.x;
+    const int64_t d0 = (int64_t) (blockIdx.x % (unsigned) blocks) * 64, t0 = (int64_t) (blockIdx.x / (unsigned) blocks) * 64;
+    const int nd = (int) min((int64_t) 64, L.D - d0), nt = (int) min((int64_t) 64, L.T - t0);
+    for (int64_t s = blockIdx.y; s < L.S; s += gridDim.y) {
+        __syncthreads();
+        for (int i = tid; i < nd * width; i += 256) {
+            const int d = i / width, j = i - d * width;
+            const int64_t r = t0 + j;
+            if (j >= nt + L.K - 1) continue;
+            rows[d * stride + j] = r < L.K - 1 ? L.state[(d0 + d) * L.st_d + r * L.st_j + s * L.st_s]
+                                               : L.x[(d0 + d) * L.x_d + (r - L.K + 1) * L.x_t + s * L.x_s];
+        }
+        if (L.new_state && t0 == 0) {
+            // read before the barrier, written after it, by the one tile that reads the state at all
+            for (int i = tid; i < nd * (L.K - 1); i += 256) {
+                const int d = i / (L.K - 1), j = i - d * (L.K - 1);
+                const int64_t r = L.T + j;
+                rows[64 * stride + i] = r < L.K - 1 ? L.state[(d0 + d) * L.st_d + r * L.st_j + s * L.st_s]
+                                                    : L.x[(d0 + d) * L.x_d + (r - L.K + 1) * L.x_t + s * L.x_s];
+            }
+        }
+        __syncthreads();
+        if (L.new_state && t0 == 0) {
+            for (int i = tid; i < nd * (L.K - 1); i += 256) L.new_state[(s * L.D + d0) * (L.K - 1) + i] = rows[64 * stride + i];
+        }
+        const int d = tid % 64, tw = tid / 64 * 16;
+        if (d < nd) {
+            const float bias = L.bias ? L.bias[d0 + d] : 0.0f;
+            float v[16];
+#pragma unroll
+            for (int j = 0; j < 16; j++) v[j] = bias;
+            for (int k = 0; k < L.K; k++) {
+                const float w = L.w[(d0 + d) * L.w_d + k * L.w_k];
+#pragma unroll
+                for (int j = 0; j < 16; j++) v[j] = fmaf(w, rows[d * stride + tw + j + k], v[j]);
+            }
+            float * y = L.y + d0 + d + L.D * (t0 + L.T * s);
+#pragma unroll
+            for (int j = 0; j < 16; j++) {
+                if (tw + j < nt) y[(tw + j) * L.D] = L.silu ? silu(v[j]) : v[j];
+            }
+        }
+    }
+}
+
+template <int K, int V>
+void launch_conv_rows(const ssm_conv_launch & L, hipStream_t st) {
+    const int64_t groups = (L.D + V - 1) / V;
+    const int threads = (int) std::min<int64_t>(256, (groups + 63) / 64 * 64);
+    const int blocks = (int) ((groups + threads - 1) / threads);
+    const unsigned gy = (unsigned) std::min<int64_t>(L.S, 65535);
+    // eight rows per thread read 11 for 8 outputs (4 taps); one token takes its own rows only
+    if (L.T == 1) launch(ssm_conv_rows_kernel<K, V, 1>, dim3((unsigned) blocks, gy), dim3(threads), 0, st, L, blocks);
+    else launch(ssm_conv_rows_kernel<K, V, 8>, dim3((unsigned) (blocks * ((L.T + 7) / 8)), gy), dim3(threads), 0, st, L, blocks);
+}
+
+template <int K>
+void launch_conv_rows(const ssm_conv_launch & L, hipStream_t st) {
+    const bool wide = L.D % 4 == 0 && L.x_t % 4 == 0 && L.x_s % 4 == 0 && ((uintptr_t) L.x | (uintptr_t) L.y | (uintptr_t) L.bias) % 16 == 0;
+    if (wide) launch_conv_rows<K, 4>(L, st);
+    else launch_conv_rows<K, 1>(L, st);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -98,9 +242,20 @@ void launch_rows(const ssm_scan_launch & L, hipStream_t st) {
 } // namespace
 
 void launch_ssm_conv(const ssm_conv_launch & L, hipStream_t st) {
-    const int64_t n = L.D * L.T * L.S;
-    if (n == 0) return;
-    launch(ssm_conv_kernel, dim3((unsigned) ((n + 255) / 256)), dim3(256), 0, st, L);
+    if (L.D == 0 || L.S == 0) return;
+    if (L.T == 0) return;
+    if (L.x_d == 1 && L.K <= 4) {
+        switch (L.K) {
+            case 1: launch_conv_rows<1>(L, st); return;
+            case 2: launch_conv_rows<2>(L, st); return;
+            case 3: launch_conv_rows<3>(L, st); return;
+            default: launch_conv_rows<4>(L, st); return;
+        }
+    }
+    const int blocks = (int) ((L.D + 63) / 64);
+    const size_t lds = sizeof(float) * (64 * ((64 + L.K - 1) | 1) + 64 * (L.K - 1));
+    launch(ssm_conv_tile_kernel, dim3((unsigned) (blocks * ((L.T + 63) / 64)), (unsigned) std::min<int64_t>(L.S, 65535)), dim3(256), lds, st,
+           L, blocks);
 }
 
 void launch_ssm_scan(const ssm_scan_launch & L, hipStream_t st) {

@@ -560,10 +560,13 @@ void launch_sample_sorted(const sample_request & r, void * ws, size_t ws_bytes, 
 // state[j * st_j + d * st_d + s * st_s] for j < K - 1 (the rows before the step) and
 // x[(j - K + 1) * x_t + d * x_d + s * x_s] after them. With r(t, d) those rows,
 //   y[t, d] = sum_k w[k * w_k + d * w_d] * r(t + k, d) (+ bias[d]) (then SiLU)
-// for t < T, contiguous [D, T, S]. Strides in floats.
+// for t < T, contiguous [D, T, S]. new_state (or null): the rows T .. T + K - 2 in order, contiguous
+// [K - 1, D, S]; it may be the state's own memory where that has the same layout, and is apart from
+// every other operand. Strides in floats.
+constexpr int SSM_MAX_TAPS = 32;    // the tile kernel's LDS: 64 x 95 rows and 64 x 31 of the new state, 32 KiB
 struct ssm_conv_launch {
     const float * state, * x, * w, * bias;
-    float *       y;
+    float *       y, * new_state;
     int64_t       st_j, st_d, st_s, x_t, x_d, x_s, w_k, w_d;
     int64_t       T, D, S;
     int           K;

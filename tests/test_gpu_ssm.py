@@ -156,7 +156,8 @@ def test_scan_of_strided_operands(hip):
 
 
 @pytest.mark.parametrize("K, T, D, S", [(4, 1, 1, 1), (4, 1, 300, 5), (1, 9, 5, 1), (2, 5, 64, 1), (4, 2, 33, 2), (4, 100, 129, 1),
-                                       (3, 65, 64, 3), (7, 70, 40, 1), (4, 300, 1024, 1), (4, 0, 8, 1)])
+                                       (3, 65, 64, 3), (7, 70, 40, 1), (4, 300, 1024, 1), (4, 0, 8, 1), (1, 70, 9, 2), (32, 130, 70, 1),
+                                       (32, 1, 3, 2)])
 def test_conv(hip, K, T, D, S):
     rng = np.random.default_rng(K + T + D)
     sx = rng.standard_normal((S, D, K - 1 + T)).astype(np.float32)
@@ -203,7 +204,8 @@ class Mixer:
 @pytest.mark.parametrize("K, T, D, S, W, bias, act", [
     (4, 1, 8, 1, 8, True, True), (4, 1, 260, 7, 300, True, True), (4, 2, 65, 2, 65, True, True), (4, 3, 64, 3, 70, False, True),
     (4, 64, 64, 1, 128, True, True), (4, 67, 130, 2, 131, True, True), (2, 5, 33, 1, 40, True, True), (3, 200, 512, 1, 1100, False, True),
-    (4, 300, 1000, 1, 1000, True, False), (6, 4, 20, 2, 20, True, True), (4, 21, 44, 1, 44, False, False)])
+    (4, 300, 1000, 1, 1000, True, False), (6, 4, 20, 2, 20, True, True), (9, 70, 70, 2, 71, True, True),
+    (4, 21, 44, 1, 44, False, False)])
 def test_conv_with_its_state(hip, fusion, in_place, K, T, D, S, W, bias, act):
     rng = np.random.default_rng(K * T + D)
     state = rng.standard_normal((S, D, K - 1)).astype(np.float32)
@@ -220,6 +222,39 @@ def test_conv_with_its_state(hip, fusion, in_place, K, T, D, S, W, bias, act):
         gl.libs()["hip"].ggml_backend_hip_set_fusion(hip, True)
     assert np.array_equal(new.reshape(S, D, K - 1), sx[:, :, T:])
     near(y, *ssm_ref.conv(sx, w, b, act))
+
+
+def test_conv_that_others_read(hip):
+    """Graphs that the fused launch must leave alone: the joined rows are an output, the old state is
+    read after the convolution and before the copy over it, the new state goes to another sequence's
+    row of the same memory."""
+    rng = np.random.default_rng(41)
+    K, T, D, S = 4, 2, 24, 1
+    state = rng.standard_normal((2, D, K - 1)).astype(np.float32)
+    rows = rng.standard_normal((S, T, D)).astype(np.float32)
+    w, b = rng.standard_normal((D, K)).astype(np.float32), rng.standard_normal(D).astype(np.float32)
+    sx = np.concatenate([state[:1], rows.transpose(0, 2, 1)], 2)
+    want, bound = ssm_ref.conv(sx, w, b, True)
+    nb1, nb2 = (K - 1) * 4, (K - 1) * D * 4
+    for kind in ("joined", "old", "shift"):
+        with Graph(mem=1 << 20) as g:
+            pool = g.tensor(gl.F32, K - 1, D, 2, data=state)
+            st = g.view_3d(pool, K - 1, D, 1, nb1, nb2, 0)
+            joined = g.concat(st, g.transpose(g.tensor(gl.F32, D, T, S, data=rows)), 0)
+            y = g.silu(g.add(g.ssm_conv(joined, g.tensor(gl.F32, K, D, data=w)), g.tensor(gl.F32, D, data=b)))
+            old = g.scale(g.reshape_2d(st, K - 1, D), 2.0) if kind == "old" else None
+            nb = joined.contents.nb
+            # one step into the pool: the new state lies over the end of the old one and the next row
+            to = g.view_3d(pool, K - 1, D, 1, nb1, nb2, nb1 if kind == "shift" else 0)
+            new = g.cpy(g.view_3d(joined, K - 1, D, S, nb[1], nb[2], T * 4), to)
+            outs = [y] + ([joined] if kind == "joined" else [old] if kind == "old" else []) + [new]
+            got = g.compute(hip, outs)
+            near(got[0], want, bound, kind)
+            assert np.array_equal(got[-1].reshape(D, K - 1), sx[0, :, T:]), kind
+            if kind == "joined":
+                assert np.array_equal(got[1].reshape(sx.shape), sx)
+            if kind == "old":
+                assert np.array_equal(got[1].reshape(D, K - 1), 2 * state[0])
 
 
 def test_static_compute(hip):

@@ -84,6 +84,8 @@ def test_conv_refuses():
         assert "extents" in refusal(g.ssm_conv(g.tensor(gl.F32, 7, 16, 2), g.tensor(gl.F32, 4, 16, 2)))
         assert "extents" in refusal(g.ssm_conv(g.tensor(gl.F32, 7, 16, 2, 2), w))
         wide = g.tensor(gl.F32, 7 * 16)
+        assert refusal(g.ssm_conv(g.tensor(gl.F32, 32, 16), g.tensor(gl.F32, 32, 16))) is None
+        assert "taps" in refusal(g.ssm_conv(g.tensor(gl.F32, 33, 16), g.tensor(gl.F32, 33, 16)))
         assert "past" in refusal(g.ssm_conv(g.view_3d(wide, 7, 16, 1, 32, 448, 0), w))
         assert "whole elements" in refusal(g.ssm_conv(g.view_3d(wide, 5, 16, 1, 22, 352, 0), w))
 
