@@ -66,9 +66,9 @@ struct hip_device {
     size_t smp_ints = 0;
     uint8_t * smp_ws = nullptr;
     size_t smp_ws_size = 0;
-    // log probabilities: the rows' results, then their tokens
-    int32_t * lp = nullptr;
-    size_t lp_words = 0;
+    // log probabilities: the parts of rows that several workgroups read
+    uint8_t * lp = nullptr;
+    size_t lp_size = 0;
     ggml_backend_buffer_type buft{};
     char name[64] = { 0 };
 };
@@ -2800,36 +2800,42 @@ enum ggml_status ggml_backend_hip_logprobs(ggml_backend_t backend, const struct 
         return fail("logits are not in this backend's device buffer");
     }
     hip_device & d = dev(c->device);
-    // so many rows at a time: their tokens fit an upload slot and their results the download area
-    const int64_t step = LOGPROBS_ROWS;
+    // so many rows at a time: their tokens fit an upload slot, their results the download area (the kernels
+    // read and write both in place) and their parts 64 MiB
+    const int64_t part = std::max<int64_t>(logprobs_scratch_bytes((int) n, n_top, 1), 1);
+    const int64_t step = std::min<int64_t>(LOGPROBS_ROWS, std::max<int64_t>(1, ((int64_t) 64 << 20) / part));
     const int width = 2 + 2 * n_top;
     for (int64_t r0 = 0; r0 < n_rows; r0 += step) {
         const int nr = (int) std::min(step, n_rows - r0);
-        const size_t words = (size_t) nr * (width + 1);
-        if (words > d.lp_words) {
+        const size_t ws = (size_t) logprobs_scratch_bytes((int) n, n_top, nr);
+        if (ws > d.lp_size) {
             HIP_CHECK(hipStreamSynchronize(d.stream));
             drained(d);
             if (d.lp) HIP_CHECK(hipFree(d.lp));
-            d.lp_words = std::max(words, (size_t) 1 << 16);
-            HIP_CHECK(hipMalloc(&d.lp, d.lp_words * 4));
+            d.lp_size = std::max(ws, (size_t) 1 << 20);
+            HIP_CHECK(hipMalloc(&d.lp, d.lp_size));
         }
-        float * out = (float *) d.lp;
-        int32_t * toks = d.lp + (size_t) nr * width;
+        uint8_t * slot = nullptr;
         if (tokens) {
-            uint8_t * slot = upload_slot(d, nr * 4);
+            slot = upload_slot(d, nr * 4);
             if (!slot) {
                 HIP_CHECK(hipStreamSynchronize(d.stream));
                 drained(d);
                 slot = upload_slot(d, nr * 4);
             }
             memcpy(slot, tokens + r0, nr * 4);
-            HIP_CHECK(hipMemcpyAsync(toks, slot, nr * 4, hipMemcpyHostToDevice, d.stream));
         }
-        logprobs_launch L{ (const char *) logits->data, logits->ne[1], logits->ne[2], (int64_t) logits->nb[1], (int64_t) logits->nb[2],
-                           (int64_t) logits->nb[3], row + r0, nr, (int) n, n_top, tokens ? toks : nullptr, out };
+        float * area = (float *) download_area(d, (size_t) nr * width * 4);
+        logprobs_launch L{};
+        L.base = (const char *) logits->data;
+        L.ne1 = logits->ne[1]; L.ne2 = logits->ne[2];
+        L.nb1 = (int64_t) logits->nb[1]; L.nb2 = (int64_t) logits->nb[2]; L.nb3 = (int64_t) logits->nb[3];
+        L.row0 = row + r0;
+        L.n_rows = nr; L.n = (int) n; L.k = n_top;
+        L.tokens = (const int32_t *) slot;
+        L.out = area;
+        L.part = d.lp;
         launch_logprobs(L, d.stream);
-        const float * area = (const float *) download_area(d, (size_t) nr * width * 4);
-        HIP_CHECK(hipMemcpyAsync((void *) area, out, (size_t) nr * width * 4, hipMemcpyDeviceToHost, d.stream));
         HIP_CHECK(hipStreamSynchronize(d.stream));
         drained(d);
         for (int i = 0; i < nr; i++) {

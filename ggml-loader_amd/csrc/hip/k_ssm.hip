@@ -44,54 +44,90 @@ template <int V> __device__ __forceinline__ void stv(float * p, const chunk<V> &
 // Channels contiguous (x_d == 1), K taps, V channels and TT tokens per thread, all rows of a tile in
 // flight at once. The first tile's threads, the only ones that touch the state, write the new one:
 // it may be the old one's own memory.
-template <int K, int V, int TT>
+// PACK: filters and states contiguous and 16-byte aligned, so that a thread's four of each are whole
+// float4s (K or K - 1 of them) instead of a dword per value.
+template <int K, int V, int TT, bool PACK>
 __global__ __launch_bounds__(256) void ssm_conv_rows_kernel(ssm_conv_launch L, int blocks) {
     const int cb = (int) (blockIdx.x % (unsigned) blocks);
     const int64_t t0 = (int64_t) (blockIdx.x / (unsigned) blocks) * TT;
     const int64_t d = ((int64_t) cb * blockDim.x + threadIdx.x) * V;
     if (d >= L.D) return;
     float w[V][K];
+    if constexpr (PACK) {
 #pragma unroll
-    for (int i = 0; i < V; i++) {
+        for (int q = 0; q < K; q++) {
+            const chunk<4> c = ldv<4>(L.w + d * K + 4 * q);
 #pragma unroll
-        for (int k = 0; k < K; k++) w[i][k] = L.w[(d + i) * L.w_d + k * L.w_k];
+            for (int i = 0; i < 4; i++) w[(4 * q + i) / K][(4 * q + i) % K] = c.v[i];
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; i++) {
+#pragma unroll
+            for (int k = 0; k < K; k++) w[i][k] = L.w[(d + i) * L.w_d + k * L.w_k];
+        }
     }
     chunk<V> b{};
     if (L.bias) b = ldv<V>(L.bias + d);
     for (int64_t s = blockIdx.y; s < L.S; s += gridDim.y) {
         const float * xp = L.x + d + s * L.x_s;
         const float * sp = L.state + d * L.st_d + s * L.st_s;
-        chunk<V> r[TT + K - 1], last[K > 1 ? K - 1 : 1];
+        chunk<V> r[TT + K - 1];
 #pragma unroll
         for (int j = 0; j < TT + K - 1; j++) {
             const int64_t t = t0 + j - (K - 1);   // a row past the last is the last again, and not used
             r[j] = ldv<V>(xp + (t < 0 ? 0 : t < L.T ? t : L.T - 1) * L.x_t);
         }
-        if (t0 < K - 1) {
+        if (K > 1 && t0 == 0) {
+            float old[V][K > 1 ? K - 1 : 1];      // rows 0 .. K - 2
+            if constexpr (PACK) {
 #pragma unroll
-            for (int j = 0; j < K - 1; j++) {
-                if (t0 + j < K - 1) {
+                for (int q = 0; q < K - 1; q++) {
+                    const chunk<4> c = ldv<4>(sp + 4 * q);
 #pragma unroll
-                    for (int i = 0; i < V; i++) r[j].v[i] = sp[i * L.st_d + (t0 + j) * L.st_j];
+                    for (int i = 0; i < 4; i++) old[(4 * q + i) / (K - 1)][(4 * q + i) % (K - 1)] = c.v[i];
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < V; i++) {
+#pragma unroll
+                    for (int j = 0; j < K - 1; j++) old[i][j] = sp[i * L.st_d + j * L.st_j];
                 }
             }
-        }
-        if (L.new_state && t0 == 0) {
-#pragma unroll
-            for (int j = 0; j < K - 1; j++) {
-                const int64_t t = L.T + j - (K - 1);
-                if (t >= 0) {
-                    last[j] = ldv<V>(xp + t * L.x_t);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < V; i++) last[j].v[i] = sp[i * L.st_d + (L.T + j) * L.st_j];
-                }
-            }
-            float * np = L.new_state + (s * L.D + d) * (K - 1);
 #pragma unroll
             for (int i = 0; i < V; i++) {
 #pragma unroll
-                for (int j = 0; j < K - 1; j++) np[i * (K - 1) + j] = last[j].v[i];
+                for (int j = 0; j < K - 1; j++) r[j].v[i] = old[i][j];
+            }
+            if (L.new_state) {
+                float last[V][K > 1 ? K - 1 : 1];
+#pragma unroll
+                for (int j = 0; j < K - 1; j++) {
+                    const int64_t t = L.T + j - (K - 1);
+                    const chunk<V> c = ldv<V>(xp + (t < 0 ? 0 : t) * L.x_t);
+#pragma unroll
+                    for (int i = 0; i < V; i++) {
+                        last[i][j] = c.v[i];
+#pragma unroll
+                        for (int o = 0; o < K - 1; o++) last[i][j] = L.T + j == o ? old[i][o] : last[i][j];
+                    }
+                }
+                float * np = L.new_state + (s * L.D + d) * (K - 1);
+                if constexpr (PACK) {
+#pragma unroll
+                    for (int q = 0; q < K - 1; q++) {
+                        chunk<4> c;
+#pragma unroll
+                        for (int i = 0; i < 4; i++) c.v[i] = last[(4 * q + i) / (K - 1)][(4 * q + i) % (K - 1)];
+                        stv<4>(np + 4 * q, c);
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < V; i++) {
+#pragma unroll
+                        for (int j = 0; j < K - 1; j++) np[i * (K - 1) + j] = last[i][j];
+                    }
+                }
             }
         }
         float * y = L.y + d + L.D * (t0 + L.T * s);
@@ -161,22 +197,25 @@ __global__ __launch_bounds__(256) void ssm_conv_tile_kernel(ssm_conv_launch L, i
     }
 }
 
-template <int K, int V>
+template <int K, int V, bool PACK>
 void launch_conv_rows(const ssm_conv_launch & L, hipStream_t st) {
     const int64_t groups = (L.D + V - 1) / V;
     const int threads = (int) std::min<int64_t>(256, (groups + 63) / 64 * 64);
     const int blocks = (int) ((groups + threads - 1) / threads);
     const unsigned gy = (unsigned) std::min<int64_t>(L.S, 65535);
     // eight rows per thread read 11 for 8 outputs (4 taps); one token takes its own rows only
-    if (L.T == 1) launch(ssm_conv_rows_kernel<K, V, 1>, dim3((unsigned) blocks, gy), dim3(threads), 0, st, L, blocks);
-    else launch(ssm_conv_rows_kernel<K, V, 8>, dim3((unsigned) (blocks * ((L.T + 7) / 8)), gy), dim3(threads), 0, st, L, blocks);
+    if (L.T == 1) launch(ssm_conv_rows_kernel<K, V, 1, PACK>, dim3((unsigned) blocks, gy), dim3(threads), 0, st, L, blocks);
+    else launch(ssm_conv_rows_kernel<K, V, 8, PACK>, dim3((unsigned) (blocks * ((L.T + 7) / 8)), gy), dim3(threads), 0, st, L, blocks);
 }
 
 template <int K>
 void launch_conv_rows(const ssm_conv_launch & L, hipStream_t st) {
     const bool wide = L.D % 4 == 0 && L.x_t % 4 == 0 && L.x_s % 4 == 0 && ((uintptr_t) L.x | (uintptr_t) L.y | (uintptr_t) L.bias) % 16 == 0;
-    if (wide) launch_conv_rows<K, 4>(L, st);
-    else launch_conv_rows<K, 1>(L, st);
+    const bool pack = wide && L.w_k == 1 && L.w_d == K && (K == 1 || (L.st_j == 1 && L.st_d == K - 1 && L.st_s % 4 == 0)) &&
+                      ((uintptr_t) L.w | (K == 1 ? 0 : (uintptr_t) L.state | (uintptr_t) L.new_state)) % 16 == 0;
+    if (pack) launch_conv_rows<K, 4, true>(L, st);
+    else if (wide) launch_conv_rows<K, 4, false>(L, st);
+    else launch_conv_rows<K, 1, false>(L, st);
 }
 
 // ---------------------------------------------------------------------------------------------

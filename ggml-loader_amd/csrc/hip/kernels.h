@@ -594,8 +594,10 @@ void launch_ssm_scan(const ssm_scan_launch & L, hipStream_t st);
 
 // ---- log probabilities (k_logprobs.hip) ----
 // Rows of logits: row r starts at base + off(r), off the byte offset of ggml row r of the tensor
-// (ne and nb over dims 1..3). out rows of 2 + 2k words: the log probability of the row's token
-// (0 where tokens is null), the entropy, k ids (I32), k log probabilities.
+// (ne and nb over dims 1..3). out (device or host-visible): rows of 2 + 2k words, the log
+// probability of the row's token (0 where tokens is null), the entropy, k ids (I32), k log
+// probabilities. part: logprobs_scratch_bytes. tokens (or null): device or host-visible ids below n.
+constexpr int LOGPROBS_MAX_TOP = 128;
 // rows per launch: 64 KiB of tokens, and results of at most 16 MiB (the download area) at 128 alternatives
 constexpr int LOGPROBS_ROWS = 16384;
 struct logprobs_launch {
@@ -605,5 +607,8 @@ struct logprobs_launch {
     int             n_rows, n, k;
     const int32_t * tokens;
     float *         out;
+    void *          part;
+    int             seg, n_seg, stage;   // set by the launcher
 };
+int64_t logprobs_scratch_bytes(int n, int k, int n_rows);
 void launch_logprobs(const logprobs_launch & L, hipStream_t st);

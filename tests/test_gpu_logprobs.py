@@ -79,7 +79,7 @@ def check(hip, x, tokens, n_top, row=0, t=None):
 
 @pytest.mark.parametrize("n, rows, n_top", [(1, 1, 1), (2, 3, 2), (7, 4, 7), (64, 2, 0), (255, 5, 128), (257, 3, 20), (1000, 33, 5),
                                             (4099, 9, 128), (32064, 37, 20), (151936, 1, 20), (151936, 2, 128), (128256, 300, 1),
-                                            (151936, 1, 0), (50257, 2, 64)])
+                                            (151936, 1, 0), (50257, 2, 64), (8192, 3, 100), (8193, 3, 100), (600001, 1, 128)])
 def test_scores(hip, n, rows, n_top):
     rng = np.random.default_rng(n + rows)
     x = (rng.standard_normal((rows, n)) * 3).astype(np.float32)
@@ -108,6 +108,24 @@ def test_rows_of_every_kind(hip, n, n_top):
     x[10] = np.finfo(np.float32).min
     x[11, :] = np.where(rng.random(n) < 0.5, -0.0, 0.0)
     check(hip, x, rng.integers(0, n, 12), n_top)
+
+
+@pytest.mark.parametrize("n", [4500, 8192, 30000])
+@pytest.mark.parametrize("n_top", [1, 3, 6, 12, 20, 40, 100])
+def test_a_regular_pattern_of_banned_tokens(hip, n, n_top):
+    """Every 1024 ids begin with 256 banned ones, or with 256 of one low value; the rest with and
+    without equal values."""
+    rng = np.random.default_rng(n + n_top)
+    x = rng.standard_normal((6, n)).astype(np.float32)
+    low = np.arange(n) % 1024 < 256
+    x[0, low] = -np.inf
+    x[1, low] = -5
+    x[2] = np.round(x[2])
+    x[2, low] = -np.inf
+    x[3] = np.where(low, -np.inf, 1.0)
+    x[4] = np.where(low, -4.0, np.where(np.arange(n) % 3 == 0, 1.0, 0.5))
+    x[5, ~low] = -np.inf
+    check(hip, x, rng.integers(0, n, 6), n_top)
 
 
 def test_a_banned_token(hip):
