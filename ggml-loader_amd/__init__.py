@@ -299,15 +299,17 @@ def hip_logprobs(backend, logits_tensor, tokens, *, row: int = 0, n_rows: int | 
     n = len(toks) if n_rows is None else n_rows
     if toks is not None and toks.shape != (n,):
         raise ValueError("hip_logprobs: one token per row")
-    ptr = lambda a: None if a is None else a.ctypes.data_as(C.c_void_p)  # noqa: E731
-    logprob = None if toks is None else np.empty(n, np.float32)
-    entropy = np.empty(n, np.float32)
-    ids, top = np.empty((n, max(n_top, 0)), np.int32), np.empty((n, max(n_top, 0)), np.float32)
-    st = libs()["hip"].ggml_backend_hip_logprobs(backend, logits_tensor, row, n, ptr(toks), n_top, ptr(logprob),
-                                                 ptr(entropy), ptr(ids), ptr(top))
+    k = max(n_top, 0)
+    out = np.empty(n * (2 + 2 * k), np.float32)      # the four results one after another
+    logprob, entropy = out[:n], out[n:2 * n]
+    ids, top = out[2 * n:(2 + k) * n].view(np.int32).reshape(n, k), out[(2 + k) * n:].reshape(n, k)
+    at = out.ctypes.data
+    st = libs()["hip"].ggml_backend_hip_logprobs(
+        backend, logits_tensor, row, n, None if toks is None else toks.ctypes.data, n_top,
+        None if toks is None else at, at + 4 * n, at + 8 * n, at + 4 * (2 + k) * n)
     if st != 0:
         raise RuntimeError(f"ggml_backend_hip_logprobs failed ({st})")
-    return logprob, entropy, ids, top
+    return None if toks is None else logprob, entropy, ids, top
 
 
 def hip_backend(device: int = 0):

@@ -23,7 +23,7 @@ constexpr int LP_WAVES = LP_THREADS / WAVE;
 constexpr int LP_PER = 32;                        // logits per thread, in groups of 4
 constexpr int LP_SEG = LP_THREADS * LP_PER;
 constexpr int LP_CAND = 1024;                     // entries a selection sorts
-constexpr float LOG2E = 1.4426950408889634f;
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
 // ascending order key of a float; -0 and +0 share a key
 __device__ __forceinline__ uint32_t okey(float v) {
@@ -45,14 +45,31 @@ __device__ __forceinline__ int wave_sum(int v) {
 }
 
 struct lp_shared {
-    uint64_t key[LP_CAND];
-    float f[2][LP_WAVES];
+    alignas(16) uint64_t key[LP_CAND];
+    float f[2][LP_WAVES], w[LP_WAVES];
     int n[2][LP_WAVES];
-    int count;
 };
 
-// The k best of a workgroup's LP_SEG values (v[4 j + c] is entry j * 1024 + thread * 4 + c), in order,
-// to out(rank, key): every rank below k, key 0 where there are fewer entries.
+// keys[0 .. n) to out(rank, key), every rank below k: each key's rank is the number of keys above it.
+// keys is padded with zeros to a multiple of 4 entries; all threads must call it.
+template <class F>
+__device__ __forceinline__ void rank_keys(const uint64_t * keys, int n, int k, F out) {
+    for (int i = threadIdx.x; i < n; i += LP_THREADS) {
+        const uint64_t mine = keys[i];
+        int rank = 0;
+        const ulonglong2 * kk = (const ulonglong2 *) keys;
+#pragma unroll 4
+        for (int j = 0; j < (n + 3) / 4 * 2; j++) {
+            const ulonglong2 u = kk[j];
+            rank += (u.x > mine ? 1 : 0) + (u.y > mine ? 1 : 0);
+        }
+        if (rank < k) out(rank, mine);
+    }
+}
+
+// The k best of a workgroup's LP_SEG values (v[4 j + c] is entry j * 1024 + thread * 4 + c; the ones
+// from `valid` on are -inf), in order, to out(rank, key): every rank below k, key 0 where there are
+// fewer entries. best: the thread's largest value.
 // A threshold first: M >= k groups of threads each have a largest value, so the smallest of those, t,
 // has at least k entries at or above it (for normally distributed logits and k = 20 about 110 of 8192).
 // The entries above t are listed and each finds its rank by comparing with all; where they are fewer
@@ -60,12 +77,9 @@ struct lp_shared {
 // groups do not share evenly, such as a block of -inf), t becomes the k-th largest value itself, found
 // by bisection: fewer than k entries lie above it.
 template <class F>
-__device__ void select_top(const float (&v)[LP_PER], int valid, int id0, int k, lp_shared & S, F out) {
-    const int tid = threadIdx.x, wave = tid / WAVE;
-    auto index = [&](int i) { return (i / 4) * (LP_THREADS * 4) + tid * 4 + i % 4; };
-    float t = -INFINITY;
-#pragma unroll
-    for (int i = 0; i < LP_PER; i++) t = fmaxf(t, v[i]);
+__device__ __forceinline__ void select_top(const float (&v)[LP_PER], float best, int valid, int id0, int k, lp_shared & S, F out) {
+    const int tid = threadIdx.x, lane = tid % WAVE, wave = tid / WAVE;
+    float t = best;
     if (k > 64) t = group_max<2>(t);
     else if (k > 32) t = group_max<4>(t);
     else if (k > 16) t = group_max<8>(t);
@@ -73,48 +87,52 @@ __device__ void select_top(const float (&v)[LP_PER], int valid, int id0, int k, 
     else if (k > 4) t = group_max<32>(t);
     else t = group_max<64>(t);
     t = -wave_max(-t);
-    if (tid % WAVE == 0) S.f[0][wave] = t;
+    if (lane == 0) S.f[0][wave] = t;
     __syncthreads();
     t = fminf(fminf(S.f[0][0], S.f[0][1]), fminf(S.f[0][2], S.f[0][3]));
-    // entries that satisfy f, over the workgroup; `turn` alternates the words that it uses
+    // entries that satisfy f, of this thread (mine) and of the workgroup; `turn` alternates the words that it uses
+    int mine;
     auto count = [&](int turn, auto f) {
-        int n = 0;
+        mine = 0;
 #pragma unroll
-        for (int i = 0; i < LP_PER; i++) n += index(i) < valid && f(v[i]) ? 1 : 0;
-        n = wave_sum(n);
-        if (tid % WAVE == 0) S.n[turn][wave] = n;
+        for (int i = 0; i < LP_PER; i++) mine += f(v[i]) ? 1 : 0;
+        const int n = wave_sum(mine);
+        if (lane == 0) S.n[turn][wave] = n;
         __syncthreads();
         return S.n[turn][0] + S.n[turn][1] + S.n[turn][2] + S.n[turn][3];
     };
-    int above = count(0, [&](float x) { return x > t; });
+    int turn = 0, above = count(0, [&](float x) { return x > t; });
     if (above > LP_CAND) {
         // the largest value with k entries at or above it; okey(t) has them
         uint32_t lo = okey(t), hi = 0xffffffffu;
-        int turn = 1;
         while (lo < hi) {
             const uint32_t mid = lo + (hi - lo) / 2 + 1;
-            if (count(turn, [&](float x) { return okey(x) >= mid; }) >= k) lo = mid;
+            if (count(turn ^= 1, [&](float x) { return okey(x) >= mid; }) >= k) lo = mid;
             else hi = mid - 1;
-            turn ^= 1;
         }
         t = okey_value(lo);
-        above = count(turn, [&](float x) { return x > t; });
+        above = count(turn ^= 1, [&](float x) { return x > t; });
     }
-    if (tid == 0) S.count = 0;
-    __syncthreads();
+    // the thread's place in the list: those of the waves and lanes before it
+    int scan = mine;
 #pragma unroll
-    for (int i = 0; i < LP_PER; i++) {
-        if (index(i) < valid && v[i] > t) S.key[atomicAdd(&S.count, 1)] = ckey(v[i], id0 + index(i));
+    for (int o = 1; o < WAVE; o *= 2) {
+        const int u = __shfl_up(scan, o, WAVE);
+        scan += lane >= o ? u : 0;
     }
+    int at = scan - mine;
+    for (int w = 0; w < wave; w++) at += S.n[turn][w];
+    if (mine) {
+#pragma unroll
+        for (int i = 0; i < LP_PER; i++) {
+            if (v[i] > t) S.key[at++] = ckey(v[i], id0 + (i / 4) * (LP_THREADS * 4) + tid * 4 + i % 4);
+        }
+    }
+    if (tid < (-above & 3)) S.key[above + tid] = 0;
     __syncthreads();
-    for (int i = tid; i < above; i += LP_THREADS) {
-        const uint64_t mine = S.key[i];
-        int rank = 0;
-        for (int j = 0; j < above; j++) rank += S.key[j] > mine ? 1 : 0;
-        if (rank < k) out(rank, mine);
-    }
+    rank_keys(S.key, above, k, out);
     // entries equal to the threshold, row of 1024 by row in the order of their ids
-    for (int row = 0, at = above; row < LP_PER / 4 && at < k; row++) {
+    for (int row = 0, got = above; row < LP_PER / 4 && got < k; row++) {
         int n = 0, before = 0, all = 0;
         bool eq[4];
 #pragma unroll
@@ -124,22 +142,22 @@ __device__ void select_top(const float (&v)[LP_PER], int valid, int id0, int k, 
             for (int j = 1; j < LP_PER / 4; j++) x = row == j ? v[4 * j + c] : x;
             eq[c] = row * (LP_THREADS * 4) + tid * 4 + c < valid && x == t;
             const uint64_t m = __ballot(eq[c]);
-            before += __popcll(m & ((1ull << (tid % WAVE)) - 1));
+            before += __popcll(m & ((1ull << lane) - 1));
             all += __popcll(m);
         }
         __syncthreads();
-        if (tid % WAVE == 0) S.n[0][wave] = all;
+        if (lane == 0) S.n[0][wave] = all;
         __syncthreads();
         for (int w = 0; w < wave; w++) before += S.n[0][w];
 #pragma unroll
         for (int c = 0; c < 4; c++) {
-            const int rank = at + before + n;
+            const int rank = got + before + n;
             if (eq[c] && rank < k) out(rank, ckey(t, id0 + row * (LP_THREADS * 4) + tid * 4 + c));
             n += eq[c] ? 1 : 0;
         }
-        at += S.n[0][0] + S.n[0][1] + S.n[0][2] + S.n[0][3];
+        got += S.n[0][0] + S.n[0][1] + S.n[0][2] + S.n[0][3];
         if (row == LP_PER / 4 - 1) {
-            for (int i = at + tid; i < k; i += LP_THREADS) out(i, 0);
+            for (int i = got + tid; i < k; i += LP_THREADS) out(i, 0);
         }
     }
 }
@@ -152,6 +170,21 @@ __device__ __forceinline__ const float * row_of(const logprobs_launch & L, int r
 // a segment's (or a row's) maximum, sums and whether it holds a NaN
 struct lp_stats { float m, s, w, bad; };
 
+__device__ __forceinline__ lp_stats join(const lp_stats & a, const lp_stats & b) {
+    lp_stats c{ fmaxf(a.m, b.m), 0.0f, 0.0f, fmaxf(a.bad, b.bad) };
+    if (a.s > 0.0f) {                              // not a part of -inf alone
+        const float z = a.m - c.m, e = __builtin_amdgcn_exp2f(z * LOG2E);
+        c.s = a.s * e;
+        c.w = e > 0.0f ? fmaf(a.s, z, a.w) * e : 0.0f;
+    }
+    if (b.s > 0.0f) {
+        const float z = b.m - c.m, e = __builtin_amdgcn_exp2f(z * LOG2E);
+        c.s = fmaf(b.s, e, c.s);
+        c.w += e > 0.0f ? fmaf(b.s, z, b.w) * e : 0.0f;
+    }
+    return c;
+}
+
 // the log of the sum of a row's exponentials above its maximum: NaN where it has no distribution
 __device__ __forceinline__ float log_sum(const lp_stats & a) { return a.bad != 0.0f || !(fabsf(a.m) < INFINITY) ? NAN : logf(a.s); }
 
@@ -159,8 +192,8 @@ __device__ __forceinline__ float log_sum(const lp_stats & a) { return a.bad != 0
 // memory, where each separate store would be a bus transfer of its own.
 struct lp_out { float w[2 + 2 * LOGPROBS_MAX_TOP]; };
 
-__device__ __forceinline__ void put_scores(const logprobs_launch & L, int r, const float * x, const lp_stats & a, float ls, lp_out & o) {
-    o.w[0] = L.tokens ? x[L.tokens[r]] - a.m - ls : 0.0f;
+__device__ __forceinline__ void put_scores(const logprobs_launch & L, float tok, const lp_stats & a, float ls, lp_out & o) {
+    o.w[0] = tok - a.m - ls;
     o.w[1] = ls - a.w / a.s;
 }
 __device__ __forceinline__ void put_top(const logprobs_launch & L, float m, float ls, lp_out & o, int rank, uint64_t key) {
@@ -178,7 +211,7 @@ template <bool VEC>
 __global__ __launch_bounds__(LP_THREADS) void logprobs_segment_kernel(logprobs_launch L) {
     __shared__ lp_shared S;
     __shared__ lp_out o;
-    const int seg = blockIdx.x, r = blockIdx.y, tid = threadIdx.x, wave = tid / WAVE;
+    const int seg = blockIdx.x, r = blockIdx.y, tid = threadIdx.x, lane = tid % WAVE, wave = tid / WAVE;
     const int id0 = seg * L.seg, valid = min(L.seg, L.n - id0);
     const float * x = row_of(L, r) + id0;
     float v[LP_PER];
@@ -194,89 +227,102 @@ __global__ __launch_bounds__(LP_THREADS) void logprobs_segment_kernel(logprobs_l
         }
     }
     lp_stats a{ -INFINITY, 0.0f, 0.0f, 0.0f };
+    float best = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < LP_PER; i++) {
-        if (v[i] != v[i]) { a.bad = 1.0f; v[i] = -INFINITY; }
-        a.m = fmaxf(a.m, v[i]);
-    }
-    a.m = wave_max(a.m);
-    a.bad = wave_max(a.bad);
-    if (tid % WAVE == 0) { S.f[0][wave] = a.m; S.f[1][wave] = a.bad; }
+    for (int i = 0; i < LP_PER; i++) best = fmaxf(best, v[i]);     // a NaN is never the larger one
+    a.m = wave_max(best);
+    if (lane == 0) S.f[0][wave] = a.m;
     __syncthreads();
     a.m = fmaxf(fmaxf(S.f[0][0], S.f[0][1]), fmaxf(S.f[0][2], S.f[0][3]));
-    a.bad = fmaxf(fmaxf(S.f[1][0], S.f[1][1]), fmaxf(S.f[1][2], S.f[1][3]));
-    __syncthreads();
     // nothing but -inf: every weight is 0, not exp(-inf + inf)
     const float m = a.m == -INFINITY ? 0.0f : a.m;
 #pragma unroll
     for (int i = 0; i < LP_PER; i++) {
-        const float z = v[i] - m, e = __builtin_amdgcn_exp2f(z * LOG2E);
+        const float z = (v[i] - m) * LOG2E, e = __builtin_amdgcn_exp2f(z);
         a.s += e;
         a.w = fmaf(e, fmaxf(z, -3e38f), a.w);     // 0 times -inf is no weight
     }
     a.s = wave_sum(a.s);
     a.w = wave_sum(a.w);
-    if (tid % WAVE == 0) { S.f[0][wave] = a.s; S.f[1][wave] = a.w; }
+    if (lane == 0) { S.f[1][wave] = a.s; S.w[wave] = a.w; }
     __syncthreads();
-    a.s = (S.f[0][0] + S.f[0][1]) + (S.f[0][2] + S.f[0][3]);
-    a.w = (S.f[1][0] + S.f[1][1]) + (S.f[1][2] + S.f[1][3]);
-    __syncthreads();
+    a.s = (S.f[1][0] + S.f[1][1]) + (S.f[1][2] + S.f[1][3]);
+    a.w = ((S.w[0] + S.w[1]) + (S.w[2] + S.w[3])) * LN2;
+    if (a.s != a.s) {
+        // a NaN, or +inf less itself: no distribution. A NaN orders as -inf.
+        a.bad = 1.0f;
+#pragma unroll
+        for (int i = 0; i < LP_PER; i++) v[i] = v[i] != v[i] ? -INFINITY : v[i];
+    }
     if (L.n_seg == 1) {
         const float ls = log_sum(a);
-        if (tid == 0) put_scores(L, r, x, a, ls, o);
-        if (L.k) select_top(v, valid, 0, L.k, S, [&](int rank, uint64_t key) { put_top(L, a.m, ls, o, rank, key); });
+        if (tid == 0) put_scores(L, L.tokens ? x[L.tokens[r]] : 0.0f, a, ls, o);
+        if (L.k) select_top(v, best, valid, 0, L.k, S, [&](int rank, uint64_t key) { put_top(L, a.m, ls, o, rank, key); });
         store_row(L, r, o);
         return;
     }
     const int64_t at = (int64_t) r * L.n_seg + seg;
     if (tid == 0) ((lp_stats *) L.part)[at] = a;
     uint64_t * keys = (uint64_t *) ((lp_stats *) L.part + (int64_t) L.n_rows * L.n_seg) + at * L.k;
-    if (L.k) select_top(v, valid, id0, L.k, S, [&](int rank, uint64_t key) { keys[rank] = key; });
+    if (L.k) select_top(v, best, valid, id0, L.k, S, [&](int rank, uint64_t key) { keys[rank] = key; });
 }
 
-// A row's segments joined. Each segment's list is in descending order, so an entry's rank is its own
-// place plus, for each other segment, the number of entries above it: a bisection per segment.
+// A row's segments joined. Their lists hold n_seg * k entries in descending order; the q best of each,
+// q = ceil(k / n_seg), are at least k, so entries below the smallest of the lists' q-th are out (about
+// 50 of 380 stay for 19 segments and k = 20). What stays is ranked by comparing with all.
 __global__ __launch_bounds__(LP_THREADS) void logprobs_join_kernel(logprobs_launch L) {
-    extern __shared__ uint64_t staged[];
+    extern __shared__ __align__(16) uint64_t kept[];
     __shared__ lp_out o;
+    __shared__ lp_stats all[LP_WAVES];
+    __shared__ uint64_t least[LP_WAVES];
+    __shared__ int count;
     const int r = blockIdx.x, tid = threadIdx.x, total = L.n_seg * L.k;
     const lp_stats * part = (const lp_stats *) L.part + (int64_t) r * L.n_seg;
     const uint64_t * keys = (const uint64_t *) ((const lp_stats *) L.part + (int64_t) L.n_rows * L.n_seg) + (int64_t) r * total;
-    // lists of very long rows stay where they are
-    const uint64_t * list = L.stage ? staged : keys;
-    if (L.stage) {
-        for (int i = tid; i < total; i += LP_THREADS) staged[i] = keys[i];
+    const float tok = L.tokens ? row_of(L, r)[L.tokens[r]] : 0.0f;
+    uint64_t t = ~(uint64_t) 0;
+    if (L.k) {
+        const int q = (L.k + L.n_seg - 1) / L.n_seg;
+        for (int j = tid; j < L.n_seg; j += LP_THREADS) t = min(t, keys[(int64_t) j * L.k + q - 1]);
     }
+    // the sums of this thread's segments, then of the threads' by halves
     lp_stats a{ -INFINITY, 0.0f, 0.0f, 0.0f };
-    for (int j = 0; j < L.n_seg; j++) {
-        a.m = fmaxf(a.m, part[j].m);
-        a.bad = fmaxf(a.bad, part[j].bad);
+    for (int j = tid; j < L.n_seg; j += LP_THREADS) a = join(a, part[j]);
+#pragma unroll
+    for (int h = 1; h < WAVE; h *= 2) {
+        a = join(a, lp_stats{ __shfl_xor(a.m, h, WAVE), __shfl_xor(a.s, h, WAVE), __shfl_xor(a.w, h, WAVE), __shfl_xor(a.bad, h, WAVE) });
+        t = min(t, (uint64_t) __shfl_xor((unsigned long long) t, h, WAVE));
     }
-    for (int j = 0; j < L.n_seg; j++) {
-        if (part[j].s == 0.0f) continue;          // a segment of -inf alone
-        const float z = part[j].m - a.m, e = __builtin_amdgcn_exp2f(z * LOG2E);
-        a.s = fmaf(part[j].s, e, a.s);
-        if (e > 0.0f) a.w = fmaf(fmaf(part[j].s, z, part[j].w), e, a.w);
+    if (tid % WAVE == 0) {
+        all[tid / WAVE] = a;
+        least[tid / WAVE] = t;
     }
-    const float ls = log_sum(a);
-    if (tid == 0) put_scores(L, r, row_of(L, r), a, ls, o);
+    if (tid == 0) count = 0;
     __syncthreads();
-    for (int i = tid; i < total; i += LP_THREADS) {
-        const uint64_t mine = list[i];
-        const int own = i / L.k;
-        int rank = i - own * L.k;
-        for (int s = 0; s < L.n_seg; s++) {
-            if (s == own) continue;
-            const uint64_t * l = list + s * L.k;
-            int lo = 0, hi = L.k;
-            while (lo < hi) {
-                const int mid = (lo + hi) / 2;
-                if (l[mid] > mine) lo = mid + 1;
-                else hi = mid;
-            }
-            rank += lo;
+    a = join(join(all[0], all[1]), join(all[2], all[3]));
+    t = min(min(least[0], least[1]), min(least[2], least[3]));
+    const float ls = log_sum(a);
+    if (tid == 0) put_scores(L, tok, a, ls, o);
+    auto put = [&](int rank, uint64_t key) { put_top(L, a.m, ls, o, rank, key); };
+    if (L.stage) {
+        for (int i = tid; i < total; i += LP_THREADS) {
+            const uint64_t key = keys[i];
+            if (key >= t) kept[atomicAdd(&count, 1)] = key;
         }
-        if (mine && rank < L.k) put_top(L, a.m, ls, o, rank, mine);
+        __syncthreads();
+        const int n = count;
+        if (tid < (-n & 3)) kept[n + tid] = 0;
+        __syncthreads();
+        rank_keys(kept, n, L.k, put);
+    } else {
+        // a very long row: its lists stay where they are
+        for (int i = tid; i < total; i += LP_THREADS) {
+            const uint64_t mine = keys[i];
+            if (mine < t || !mine) continue;
+            int rank = 0;
+            for (int j = 0; j < total; j++) rank += keys[j] > mine ? 1 : 0;
+            if (rank < L.k) put(rank, mine);
+        }
     }
     store_row(L, r, o);
 }
@@ -299,8 +345,8 @@ void launch_logprobs(const logprobs_launch & L0, hipStream_t st) {
     launch(vec ? logprobs_segment_kernel<true> : logprobs_segment_kernel<false>, dim3((unsigned) L.n_seg, (unsigned) L.n_rows),
            dim3(LP_THREADS), 0, st, L);
     if (L.n_seg > 1) {
-        const size_t lds = (size_t) L.n_seg * L.k * 8;
-        L.stage = lds <= 60 << 10;
+        const size_t lds = ((size_t) L.n_seg * L.k + 3) * 8;
+        L.stage = lds <= 48 << 10;
         launch(logprobs_join_kernel, dim3((unsigned) L.n_rows), dim3(LP_THREADS), L.stage ? lds : 0, st, L);
     }
 }
