@@ -591,6 +591,11 @@ struct ssm_scan_launch {
     int             a_scalar;      // one A per head
 };
 void launch_ssm_scan(const ssm_scan_launch & L, hipStream_t st);
+// the same over many tokens with one A per head, as matrix products (k_ssm_mm.hip); ws: 256-byte aligned scratch
+constexpr int SSM_MM_MIN_TOKENS = 16;
+bool ssm_scan_mm_takes(const ssm_scan_launch & L);
+int64_t ssm_scan_mm_scratch_bytes(const ssm_scan_launch & L);
+void launch_ssm_scan_mm(const ssm_scan_launch & L, void * ws, hipStream_t st);
 
 // ---- log probabilities (k_logprobs.hip) ----
 // Rows of logits: row r starts at base + off(r), off the byte offset of ggml row r of the tensor

@@ -64,7 +64,8 @@ SCANS = [
     (1, 1, 1, 1, 1, 1, 1, 1), (1, 1, 5, 3, 7, 1, 1, 1), (3, 1, 6, 64, 128, 2, 5, 1), (2, 2, 4, 64, 128, 1, 2, 1),
     (1, 17, 3, 5, 13, 3, 2, 1), (2, 63, 2, 64, 128, 1, 2, 1), (1, 64, 4, 64, 128, 2, 1, 1), (1, 65, 2, 64, 128, 2, 1, 1),
     (2, 130, 2, 32, 16, 1, 3, 1), (1, 200, 3, 80, 96, 1, 1, 1), (1, 129, 2, 128, 256, 2, 1, 1), (1, 333, 2, 64, 64, 1, 1, 1),
-    (1, 90, 1, 33, 100, 1, 1, 1), (1, 70, 2, 48, 200, 1, 1, 1), (5, 7, 3, 64, 128, 3, 9, 1), (1, 1100, 2, 64, 128, 1, 1, 1),
+    (4, 13000, 1, 16, 128, 1, 4, 1), (1, 64, 3, 130, 128, 1, 1, 1), (1, 300, 16, 64, 128, 8, 1, 1), (2, 150, 9, 16, 32, 3, 2, 1),
+    (1, 200, 40, 32, 64, 8, 1, 1), (1, 2000, 3, 48, 128, 1, 1, 1), (1, 90, 1, 33, 100, 1, 1, 1), (1, 70, 2, 48, 200, 1, 1, 1), (5, 7, 3, 64, 128, 3, 9, 1), (1, 1100, 2, 64, 128, 1, 1, 1),
     # a decay per state: a head per channel, and heads of several channels
     (1, 1, 300, 1, 16, 1, 1, 16), (2, 50, 130, 1, 16, 1, 3, 16), (1, 257, 67, 1, 8, 1, 1, 8), (3, 3, 65, 1, 32, 1, 3, 32),
     (1, 40, 6, 1, 5, 2, 1, 5), (1, 33, 3, 4, 16, 1, 2, 16), (1, 25, 2, 2, 129, 2, 1, 129), (1, 1030, 64, 1, 16, 1, 1, 16),
