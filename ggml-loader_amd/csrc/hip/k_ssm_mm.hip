@@ -37,6 +37,7 @@ typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef float float2v __attribute__((ext_vector_type(2)));
 typedef float float4v __attribute__((ext_vector_type(4)));
+typedef uint32_t uint4v __attribute__((ext_vector_type(4)));
 
 constexpr int Q = 64;                        // tokens per chunk
 constexpr int STEP_WORDS = 5 * Q;            // exp(c), exp(c_63 - c), d, c as two floats
@@ -344,15 +345,15 @@ __global__ __launch_bounds__(256, 2) void ssm_scan_mm_kernel(mm_plan P) {
         }
     }
 
-    uint4 stage[2 * NK];                                       // a thread's share of an operand's planes on their way to LDS
+    uint4v stage[2 * NK];                                      // a thread's share of an operand's planes on their way to LDS
     auto fetch = [&](int c, int which) {
         const char * src = P.ws + P.planes + (((int64_t) s * P.nc + c) * L.G + g) * rec_bytes<NK>() + which * 2 * PLANE + tid * 16;
 #pragma unroll
-        for (int q = 0; q < 2 * NK; q++) stage[q] = *(const uint4 *) (src + q * 4096);
+        for (int q = 0; q < 2 * NK; q++) stage[q] = *(const uint4v *) (src + q * 4096);
     };
     auto put = [&]() {
 #pragma unroll
-        for (int q = 0; q < 2 * NK; q++) *(uint4 *) (buf + tid * 16 + q * 4096) = stage[q];
+        for (int q = 0; q < 2 * NK; q++) *(uint4v *) (buf + tid * 16 + q * 4096) = stage[q];
     };
 
     float decay = 1.0f;                                        // of the segment so far
@@ -362,15 +363,26 @@ __global__ __launch_bounds__(256, 2) void ssm_scan_mm_kernel(mm_plan P) {
         // X's inputs: token 32 ks + 8 grp + i of the wave's channels
         float x[PT][2][8];
         {
+            // one lane offset for all of them: the rest of each address is the wave's
             const float * xp = L.x + h * L.x_h + s * L.x_s + (P.t0 + c * Q) * L.x_t;
-#pragma unroll
-            for (int pt = 0; pt < PT; pt++) {
+            if (left >= Q) {
 #pragma unroll
                 for (int ks = 0; ks < 2; ks++) {
 #pragma unroll
                     for (int i = 0; i < 8; i++) {
-                        const int t = 32 * ks + 8 * grp + i;
-                        x[pt][ks][i] = xp[(int64_t) min(t, left - 1) * L.x_t + pch[pt]];
+                        const float * xi = xp + (32 * ks + i) * L.x_t;
+#pragma unroll
+                        for (int pt = 0; pt < PT; pt++) x[pt][ks][i] = xi[(uint32_t) (8 * grp * (int) L.x_t + pch[pt])];
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int ks = 0; ks < 2; ks++) {
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        const int t = min(32 * ks + 8 * grp + i, left - 1);
+#pragma unroll
+                        for (int pt = 0; pt < PT; pt++) x[pt][ks][i] = xp[(uint32_t) (t * (int) L.x_t + pch[pt])];
                     }
                 }
             }
@@ -518,7 +530,6 @@ __global__ __launch_bounds__(256, 2) void ssm_scan_mm_kernel(mm_plan P) {
             }
             __syncthreads();                                   // C is read, the matrices are written
             put();
-            if (c + 1 < c1) fetch(c + 1, 0);
             if (active) {
                 half8 xh[PT][2], xl[PT][2];
                 float inv_x[PT];
@@ -558,11 +569,12 @@ __global__ __launch_bounds__(256, 2) void ssm_scan_mm_kernel(mm_plan P) {
                             const int t = 16 * tt + 4 * grp + i;
                             float v = fmaf(acc[tt][pt][i] * inv_s[pt], e[i], sum[pt][i] * inv_m * inv_x[pt]);
                             v = t < bad[pt] ? v : NAN;
-                            if (pok[pt] && t < left) y[(int64_t) t * L.P * L.H + pch[pt]] = v;
+                            if (pok[pt] && t < left) (y + (16 * tt + i) * L.P * L.H)[(uint32_t) (4 * grp * L.P * L.H + pch[pt])] = v;
                         }
                     }
                 }
             }
+            if (c + 1 < c1) fetch(c + 1, 0);
             __syncthreads();                                   // B is in place
         } else if (c + 1 < c1) {
             fetch(c + 1, 1);
@@ -728,7 +740,9 @@ void launch_mm(const ssm_scan_launch & L, const mm_sizes & z, void * ws, hipStre
 bool ssm_scan_mm_takes(const ssm_scan_launch & L) {
     // the grids' limits: one dimension each for the sequences and for groups and heads
     return L.a_scalar && L.T >= SSM_MM_MIN_TOKENS && L.S <= 65535 && L.G + (L.H + 15) / 16 <= 65535 &&
-           L.S * (int64_t) L.H * L.P < INT32_MAX;
+           L.S * (int64_t) L.H * L.P < INT32_MAX &&
+           // 32-bit offsets within a chunk
+           L.x_t >= 0 && L.x_t <= 1 << 24 && (int64_t) L.H * L.P <= 1 << 24 && L.P <= 1 << 24;
 }
 
 int64_t ssm_scan_mm_scratch_bytes(const ssm_scan_launch & L) { return mm_size(L).total; }
