@@ -109,161 +109,188 @@ __device__ __forceinline__ void load_perm(const float * row, int n, int N, bool 
     }
 }
 
-__device__ __forceinline__ float block_max(float v, float * s) {
-    v = wave_max(v);
-    if (threadIdx.x % WAVE == 0) s[threadIdx.x / WAVE] = v;
-    __syncthreads();
-    v = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
-    __syncthreads();
-    return v;
-}
-
 template <int NK>
-__device__ void prepare_operands(const mm_plan & P, int s, int c, int g, char * lds) {
+__global__ __launch_bounds__(256) void ssm_operands_kernel(mm_plan P) {
+    extern __shared__ __align__(16) char lds[];                // B's planes: blocks of 16 tokens by 32 states
     const ssm_scan_launch & L = P.L;
+    const int c = blockIdx.x, g = blockIdx.y, s = blockIdx.z;
     const int tid = threadIdx.x, lane = tid % WAVE, wave = tid / WAVE;
     const int left = P.T - c * Q;             // tokens from the chunk's first on
-    float * red = (float *) (lds + 16 * 1024 * NK);
     constexpr int PLANE = 4 * 1024 * NK;
+    float * red = (float *) (lds + 2 * PLANE);
     const int64_t rec = ((int64_t) s * P.nc + c) * L.G + g;
     char * out = P.ws + P.planes + rec * rec_bytes<NK>();
-    const float * src[2] = { L.C + g * L.c_g + s * L.c_s + (P.t0 + c * Q) * L.c_t, L.B + g * L.b_g + s * L.b_s + (P.t0 + c * Q) * L.b_t };
-    const int64_t stride[2] = { L.c_t, L.b_t };
-    float inv[2];
+    // a wave's 16 tokens of both, all states
+    const int t = 16 * wave + lane % 16;
+    const int64_t row = P.t0 + c * Q + min(t, left - 1);
+    const float * cp = L.C + g * L.c_g + s * L.c_s + row * L.c_t, * bp = L.B + g * L.b_g + s * L.b_s + row * L.b_t;
+    float v[2][NK][8], most[2] = { 0.0f, 0.0f };
+#pragma unroll
+    for (int q = 0; q < NK; q++) {
+        load_perm(cp, 32 * q + 4 * (lane / 16), L.N, P.vec_bc, v[0][q]);
+        load_perm(bp, 32 * q + 4 * (lane / 16), L.N, P.vec_bc, v[1][q]);
+    }
 #pragma unroll
     for (int o = 0; o < 2; o++) {
-        float v[NK][8], most = 0.0f;
 #pragma unroll
         for (int q = 0; q < NK; q++) {
-            const int it = tid + 256 * q, tt = it / (64 * NK), ks = it / 64 % NK;
-            const int t = 16 * tt + lane % 16;
-            load_perm(src[o] + (int64_t) min(t, left - 1) * stride[o], 32 * ks + 4 * (lane / 16), L.N, P.vec_bc, v[q]);
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                v[q][i] = t < left ? v[q][i] : 0.0f;
-                most = fmaxf(most, finite_abs(v[q][i]));
+                v[o][q][i] = t < left ? v[o][q][i] : 0.0f;
+                most[o] = fmaxf(most[o], finite_abs(v[o][q][i]));
             }
         }
-        const float sc = scale_of(block_max(most, red));
+        most[o] = wave_max(most[o]);
+        if (lane == 0) red[o * 4 + wave] = most[o];
+    }
+    __syncthreads();
+    float inv[2];
+    half8 ch[NK], cl[NK];
+#pragma unroll
+    for (int o = 0; o < 2; o++) {
+        const float sc = scale_of(fmaxf(fmaxf(red[o * 4], red[o * 4 + 1]), fmaxf(red[o * 4 + 2], red[o * 4 + 3])));
         inv[o] = inverse_of(sc);
 #pragma unroll
         for (int q = 0; q < NK; q++) {
-            const int it = tid + 256 * q;
             half8 hi, lo;
+            const int at = ((wave * NK + q) * 64 + lane) * 16;
 #pragma unroll
-            for (int i = 0; i < 8; i++) v[q][i] *= sc;
-            split8(v[q], hi, lo);
-            char * at = lds + o * 2 * PLANE + it * 16;
-            *(half8 *) at = hi;
-            *(half8 *) (at + PLANE) = lo;
+            for (int i = 0; i < 8; i++) v[o][q][i] = as_f32(v[o][q][i] * sc);
+            split8(v[o][q], hi, lo);
             if (o == 0) {
-                *(half8 *) (out + it * 16) = hi;
-                *(half8 *) (out + PLANE + it * 16) = lo;
+                ch[q] = hi;
+                cl[q] = lo;
+                *(half8 *) (out + at) = hi;
+                *(half8 *) (out + PLANE + at) = lo;
+            } else {
+                *(half8 *) (lds + at) = hi;
+                *(half8 *) (lds + PLANE + at) = lo;
             }
         }
     }
     __syncthreads();
-    // C_t . B_j for the blocks of 16 x 16 on and below the diagonal
-    float * G = (float *) (P.ws + P.gmat) + rec * Q * Q;
-    float most = 0.0f;
-    for (int q = wave; q < 10; q += 4) {
-        const int tt = q < 1 ? 0 : q < 3 ? 1 : q < 6 ? 2 : 3, jt = q - tt * (tt + 1) / 2;
+    // C_t . B_j of the wave's tokens, up to the diagonal
+    float * G = (float *) (P.ws + P.gmat) + rec * Q * Q + (16 * wave + 4 * (lane / 16)) * Q + lane % 16;
+    float top = 0.0f;
+    for (int jt = 0; jt <= wave; jt++) {
         float4v acc = { 0, 0, 0, 0 };
 #pragma unroll
         for (int ks = 0; ks < NK; ks++) {
-            const char * a = lds + ((tt * NK + ks) * 64 + lane) * 16, * b = lds + 2 * PLANE + ((jt * NK + ks) * 64 + lane) * 16;
-            acc = mfma3(*(const half8 *) a, *(const half8 *) (a + PLANE), *(const half8 *) b, *(const half8 *) (b + PLANE), acc);
+            const char * b = lds + ((jt * NK + ks) * 64 + lane) * 16;
+            acc = mfma3(ch[ks], cl[ks], *(const half8 *) b, *(const half8 *) (b + PLANE), acc);
         }
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            const float v = acc[i] * inv[0] * inv[1];
-            G[(16 * tt + 4 * (lane / 16) + i) * Q + 16 * jt + lane % 16] = v;
-            most = fmaxf(most, finite_abs(v));
+            const float w = acc[i] * inv[0] * inv[1];
+            G[i * Q + 16 * jt] = w;
+            top = fmaxf(top, finite_abs(w));
         }
     }
-    most = block_max(most, red);
-    if (tid == 0) {
-        float * sc = (float *) (P.ws + P.scales) + rec * 4;
-        sc[0] = inv[0]; sc[1] = inv[1]; sc[2] = most;
-    }
+    top = wave_max(top);
+    if (lane == 0) red[8 + wave] = top;
     // B with the tokens as its k index: row n, eight tokens per lane
-    const uint16_t * bh = (const uint16_t *) (lds + 2 * PLANE);
+    const uint16_t * bh = (const uint16_t *) lds;
 #pragma unroll
     for (int q = 0; q < NK; q++) {
         const int it = tid + 256 * q, nt = it / 128, ks = it / 64 % 2;
         const int n = 16 * nt + lane % 16, j0 = 32 * ks + 8 * (lane / 16), m = n % 32;
-        const int at = (n / 32 * 64 + 16 * (m % 16 / 4)) * 8 + m / 16 * 4 + m % 4;
+        const int at = ((j0 / 16 * NK + n / 32) * 64 + 16 * (m % 16 / 4) + j0 % 16) * 8 + m / 16 * 4 + m % 4;
         uint32_t w[2][4];
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const int j = j0 + i, k = at + (j / 16 * NK * 64 + j % 16) * 8;
+        for (int p = 0; p < 2; p++) {
 #pragma unroll
-            for (int p = 0; p < 2; p++) {
-                const uint32_t u = bh[k + p * (PLANE / 2)];
-                w[p][i / 2] = i % 2 ? w[p][i / 2] | u << 16 : u;
+            for (int i = 0; i < 4; i++) {
+                const uint32_t a = bh[at + 16 * i + p * (PLANE / 2)], b = bh[at + 16 * i + 8 + p * (PLANE / 2)];
+                w[p][i] = a | b << 16;
             }
         }
 #pragma unroll
-        for (int p = 0; p < 2; p++) *(uint4 *) (out + (2 + p) * PLANE + it * 16) = make_uint4(w[p][0], w[p][1], w[p][2], w[p][3]);
+        for (int p = 0; p < 2; p++) *(uint4v *) (out + (2 + p) * PLANE + it * 16) = uint4v{ w[p][0], w[p][1], w[p][2], w[p][3] };
+    }
+    __syncthreads();
+    if (tid == 0) {
+        float * sc = (float *) (P.ws + P.scales) + rec * 4;
+        sc[0] = inv[0]; sc[1] = inv[1];
+        sc[2] = fmaxf(fmaxf(red[8], red[9]), fmaxf(red[10], red[11]));
     }
 }
 
-// 16 heads' running sums over a chunk: a wave per head, a lane per token
-__device__ void prepare_steps(const mm_plan & P, int s, int c, int h0, float * lds) {
+// 16 heads' running sums over a chunk: a wave per four heads, a lane per token
+__global__ __launch_bounds__(256) void ssm_steps_kernel(mm_plan P) {
+    __shared__ float lds[Q * 17];
     const ssm_scan_launch & L = P.L;
-    const int tid = threadIdx.x, lane = tid % WAVE, left = P.T - c * Q;
+    const int c = blockIdx.x, h0 = blockIdx.y * 16, s = blockIdx.z;
+    const int tid = threadIdx.x, lane = tid % WAVE, wave = tid / WAVE, left = P.T - c * Q;
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         const int t = 16 * i + tid / 16, h = h0 + tid % 16;
         lds[t * 17 + tid % 16] = t < left && h < L.H ? L.dt[h + (P.t0 + c * Q + t) * L.dt_t + s * L.dt_s] : 0.0f;
     }
-    __syncthreads();
-    for (int k = tid / WAVE; k < 16; k += 4) {
-        const int h = h0 + k;
-        if (h >= L.H) break;
-        // a token past the last neither decays nor adds
-        const float d = lane < left ? softplus(lds[lane * 17 + k]) : 0.0f;
-        double sum = (double) d * ((double) L.A[h * L.a_h] * 1.4426950408889634074);
-        if (lane >= left) sum = 0.0;
+    float a[4];
 #pragma unroll
-        for (int o = 1; o < WAVE; o *= 2) {
-            const double u = __shfl_up(sum, o, WAVE);
-            sum += lane >= o ? u : 0.0;
+    for (int k = 0; k < 4; k++) a[k] = L.A[min(h0 + 4 * wave + k, L.H - 1) * L.a_h];
+    __syncthreads();
+    float d[4];
+    double sum[4];
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        // a token past the last neither decays nor adds
+        d[k] = lane < left ? softplus(lds[lane * 17 + 4 * wave + k]) : 0.0f;
+        sum[k] = lane < left ? (double) d[k] * ((double) a[k] * 1.4426950408889634074) : 0.0;
+    }
+#pragma unroll
+    for (int o = 1; o < WAVE; o *= 2) {
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const double u = __shfl_up(sum[k], o, WAVE);
+            sum[k] += lane >= o ? u : 0.0;
         }
-        const double rest = __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(sum), 63),
-                                             __builtin_amdgcn_readlane(__double2loint(sum), 63)) - sum;
-        const float hi = (float) sum, lo = fabsf(hi) < INFINITY ? (float) (sum - (double) hi) : 0.0f;
+    }
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        const int h = h0 + 4 * wave + k;
+        const double rest = __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(sum[k]), 63),
+                                             __builtin_amdgcn_readlane(__double2loint(sum[k]), 63)) - sum[k];
+        const float hi = (float) sum[k], lo = fabsf(hi) < INFINITY ? (float) (sum[k] - (double) hi) : 0.0f;
         const float rh = (float) rest, rl = fabsf(rh) < INFINITY ? (float) (rest - (double) rh) : 0.0f;
+        if (h >= L.H) break;
         float * o = (float *) (P.ws + P.steps) + (((int64_t) s * P.nc + c) * L.H + h) * STEP_WORDS + lane;
         o[0] = exp2_hw(hi) * fmaf(lo, LN2, 1.0f);
         o[Q] = exp2_hw(rh) * fmaf(rl, LN2, 1.0f);
-        o[2 * Q] = d;
+        o[2 * Q] = d[k];
         o[3 * Q] = hi;
         o[4 * Q] = lo;
     }
 }
 
-template <int NK>
-__global__ __launch_bounds__(256) void ssm_prepare_kernel(mm_plan P) {
-    extern __shared__ __align__(16) char lds[];
-    const int c = blockIdx.x, y = blockIdx.y, s = blockIdx.z;
-    if (y < P.L.G) prepare_operands<NK>(P, s, c, y, lds);
-    else prepare_steps(P, s, c, (y - P.L.G) * 16, (float *) lds);
-}
-
 // ---------------------------------------------------------------------------------------------
 // scan
 
-// NK: steps of 32 states; PT: tiles of 16 channels per wave; OUT: outputs and final states, else the
-// segment's state from nothing
-template <int NK, int PT, bool OUT>
-__global__ __launch_bounds__(256, 2) void ssm_scan_mm_kernel(mm_plan P) {
+constexpr int WAVES = 8;                                       // per workgroup, each with 16 channels of a head
+constexpr int THREADS = WAVES * WAVE;
+// B's buffers: the next chunk's beside this one's, where they fit 160 KiB with C's and the matrices
+constexpr int b_slots(int nk) { return nk == 8 ? 1 : 2; }
+
+// most |a[i]|, over the four lanes of a column
+__device__ __forceinline__ float column_max(float m) {
+    m = fmaxf(m, __shfl_xor(m, 16, WAVE));
+    return fmaxf(m, __shfl_xor(m, 32, WAVE));
+}
+
+// NK: steps of 32 states; OUT: outputs and final states, else the segment's state from nothing.
+// Everything a chunk reads is loaded into registers while the chunk before it is computed: its operands'
+// planes (on to LDS at the chunk's end: C's over the last one's, B's beside it), the inputs, C_t . B_j and the
+// heads' exponentials. Two barriers a chunk: LDS is written; C is read and the matrices are written.
+template <int NK, bool OUT>
+__global__ __launch_bounds__(THREADS, 2) void ssm_scan_mm_kernel(mm_plan P) {
     extern __shared__ __align__(16) char lds[];
     const ssm_scan_launch & L = P.L;
-    constexpr int PLANE = 4 * 1024 * NK;
-    char * buf = lds;                                          // C's planes, then B's
-    float * steps = (float *) (lds + 2 * PLANE);               // per head
-    char * mats = (char *) (steps + P.hw * STEP_WORDS);        // per head: the two planes of (C_t . B_j) exp(c_t - c_j)
+    constexpr int PLANE = 4 * 1024 * NK, OPERAND = 2 * PLANE, STAGE = OPERAND / (THREADS * 16), SLOTS = b_slots(NK);
+    static_assert(STAGE >= 1, "a thread moves whole 16-byte pieces");
+    char * cbuf = lds;                                         // C's planes
+    char * bbuf = lds + (OUT ? OPERAND : 0);                   // B's, of this chunk and the next
+    float * steps = (float *) (bbuf + SLOTS * OPERAND);        // per head, of this chunk and the next
+    char * mats = (char *) (steps + 2 * P.hw * STEP_WORDS);    // per head: the two planes of (C_t . B_j) exp(c_t - c_j)
     const int tid = threadIdx.x, lane = tid % WAVE, wave = tid / WAVE, col = lane % 16, grp = lane / 16;
 
     // the workgroups that read the same operands take turns on one XCD (consecutive ids go to different ones)
@@ -278,374 +305,391 @@ __global__ __launch_bounds__(256, 2) void ssm_scan_mm_kernel(mm_plan P) {
         m = (int) blockIdx.x % members;
     }
     const int g = u % L.G, sg = u / L.G % P.n_seg, s = u / (L.G * P.n_seg);
-    const int per = L.H / L.G;
-    const int hl = P.p_blocks > 1 ? 0 : wave / P.slices, slice = P.p_blocks > 1 ? m % P.p_blocks * 4 + wave : wave % P.slices;
     if (!OUT && sg == P.n_seg - 1) return;                     // nobody starts from the last segment's state
+    const int per = L.H / L.G;
+    const int hl = P.p_blocks > 1 ? 0 : wave / P.slices, slice = P.p_blocks > 1 ? m % P.p_blocks * WAVES + wave : wave % P.slices;
     const int hb = m / P.p_blocks * P.hw;
     const int heads = min(P.hw, per - hb);                     // heads of this workgroup
     const bool active = hl < heads && slice < P.slices;
     const int h = g * per + hb + (active ? hl : 0);
     const int c0 = sg * P.seg, c1 = min(P.nc, c0 + P.seg);
+    const bool pok = active && 16 * slice + col < L.P;
+    const int pch = min(16 * slice + col, L.P - 1);
 
-    // the wave's states: tile nt, channel tile pt, i: state 16 nt + 4 grp + i of channel 16 (slice PT + pt) + col
-    float4v S[2 * NK][PT];
-    int pch[PT];
-    bool pok[PT];
+    // the wave's states: tile nt, i: state 16 nt + 4 grp + i of channel 16 slice + col
+    float4v S[2 * NK];
 #pragma unroll
-    for (int pt = 0; pt < PT; pt++) {
-        const int p = 16 * (slice * PT + pt) + col;
-        pok[pt] = active && p < L.P;
-        pch[pt] = min(p, L.P - 1);
-    }
-#pragma unroll
-    for (int nt = 0; nt < 2 * NK; nt++) {
-#pragma unroll
-        for (int pt = 0; pt < PT; pt++) S[nt][pt] = float4v{ 0, 0, 0, 0 };
-    }
+    for (int nt = 0; nt < 2 * NK; nt++) S[nt] = float4v{ 0, 0, 0, 0 };
+    // segments' states: in the order the lanes hold them
+    auto part_at = [&](int k) {
+        return (float4v *) (P.ws + P.parts) + ((((int64_t) s * P.n_seg + k) * L.H + h) * P.slices + slice) * (2 * NK * WAVE) + lane;
+    };
     if (OUT && active) {
         int64_t row = s;
         if (P.pooled) {
             row = L.ids[s * L.ids_s];
             row = row < 0 ? 0 : row >= L.pool ? L.pool - 1 : row;
         }
+        const float * s0 = P.s0 + (P.pooled ? pch * L.s_p + h * L.s_h + row * L.s_row
+                                            : (int64_t) L.N * (pch + (int64_t) L.P * (h + (int64_t) L.H * s)));
 #pragma unroll
-        for (int pt = 0; pt < PT; pt++) {
-            const float * s0 = P.s0 + (P.pooled ? pch[pt] * L.s_p + h * L.s_h + row * L.s_row
-                                                : (int64_t) L.N * (pch[pt] + (int64_t) L.P * (h + (int64_t) L.H * s)));
+        for (int nt = 0; nt < 2 * NK; nt++) {
+            const int n = 16 * nt + 4 * grp;
+            if (P.vec_s0 && n + 3 < L.N) {
+                const float4 f = *(const float4 *) (s0 + n);
+                S[nt] = float4v{ f.x, f.y, f.z, f.w };
+            } else {
 #pragma unroll
-            for (int nt = 0; nt < 2 * NK; nt++) {
-                const int n = 16 * nt + 4 * grp;
-                if (P.vec_s0 && n + 3 < L.N) {
-                    const float4 f = *(const float4 *) (s0 + n);
-                    S[nt][pt] = float4v{ f.x, f.y, f.z, f.w };
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 4; i++) S[nt][pt][i] = n + i < L.N ? s0[n + i] : 0.0f;
-                }
+                for (int i = 0; i < 4; i++) S[nt][i] = n + i < L.N ? s0[n + i] : 0.0f;
             }
         }
-    }
-    // segments' states: in the order the lanes hold them
-    auto part_at = [&](int k) {
-        return (float4v *) (P.ws + P.parts) + ((((int64_t) s * P.n_seg + k) * L.H + h) * P.slices + slice) * (2 * NK * PT * WAVE) + lane;
-    };
-    if (OUT && active) {
         for (int k = 0; k < sg; k++) {
             const float dec = ((const float *) (P.ws + P.decays))[((int64_t) s * P.n_seg + k) * L.H + h];
             const float4v * q = part_at(k);
 #pragma unroll
             for (int nt = 0; nt < 2 * NK; nt++) {
+                const float4v f = q[nt * WAVE];
 #pragma unroll
-                for (int pt = 0; pt < PT; pt++) {
-                    const float4v f = q[(nt * PT + pt) * WAVE];
-#pragma unroll
-                    for (int i = 0; i < 4; i++) S[nt][pt][i] = fmaf(S[nt][pt][i], dec, f[i]);
-                }
+                for (int i = 0; i < 4; i++) S[nt][i] = fmaf(S[nt][i], dec, f[i]);
             }
         }
     }
 
-    uint4v stage[2 * NK];                                      // a thread's share of an operand's planes on their way to LDS
-    auto fetch = [&](int c, int which) {
-        const char * src = P.ws + P.planes + (((int64_t) s * P.nc + c) * L.G + g) * rec_bytes<NK>() + which * 2 * PLANE + tid * 16;
+    // what the next chunk reads
+    uint4v stage_c[OUT ? STAGE : 1], stage_b[STAGE];
+    float x[2][8], gg[2][8], sc_next[3], st_next[(4 * STEP_WORDS + THREADS - 1) / THREADS];
+    // thread's part of a head's matrix: row mt, columns 8 mj .. + 7 and, in the lower half, 32 further on
+    const int mt = tid % 256 / 4, mj = tid % 4;
+    auto fetch = [&](int c) {
+        const int64_t rec = ((int64_t) s * P.nc + c) * L.G + g;
+        const int left = P.T - c * Q;
+        const char * src = P.ws + P.planes + rec * rec_bytes<NK>() + tid * 16;
 #pragma unroll
-        for (int q = 0; q < 2 * NK; q++) stage[q] = *(const uint4v *) (src + q * 4096);
+        for (int q = 0; q < STAGE; q++) {
+            if (OUT) stage_c[q] = *(const uint4v *) (src + q * THREADS * 16);
+            stage_b[q] = *(const uint4v *) (src + OPERAND + q * THREADS * 16);
+        }
+        const float * sp = (const float *) (P.ws + P.steps) + (((int64_t) s * P.nc + c) * L.H + g * per + hb) * STEP_WORDS;
+#pragma unroll
+        for (int q = 0; q < (4 * STEP_WORDS + THREADS - 1) / THREADS; q++) st_next[q] = sp[min(tid + q * THREADS, heads * STEP_WORDS - 1)];
+        const float * sc = (const float *) (P.ws + P.scales) + rec * 4;
+#pragma unroll
+        for (int i = 0; i < 3; i++) sc_next[i] = sc[i];
+        if (OUT) {
+            const float * G = (const float *) (P.ws + P.gmat) + rec * Q * Q + mt * Q + 8 * mj;
+#pragma unroll
+            for (int q = 0; q < 2; q++) {
+                const float4 a = *(const float4 *) (G + 32 * q), b = *(const float4 *) (G + 32 * q + 4);
+                gg[q][0] = a.x; gg[q][1] = a.y; gg[q][2] = a.z; gg[q][3] = a.w;
+                gg[q][4] = b.x; gg[q][5] = b.y; gg[q][6] = b.z; gg[q][7] = b.w;
+            }
+        }
+        // token 32 ks + 8 grp + i of the wave's channels; past the last token it is the last again, and cleared
+        const char * xp = (const char *) (L.x + h * L.x_h + s * L.x_s + (P.t0 + c * Q) * L.x_t);
+        const uint32_t row = 4 * (uint32_t) L.x_t;
+        if (left >= Q) {
+            uint32_t at = 8 * grp * row + 4 * (uint32_t) pch;
+#pragma unroll
+            for (int ks = 0; ks < 2; ks++) {
+#pragma unroll
+                for (int i = 0; i < 8; i++, at += row) x[ks][i] = *(const float *) (xp + at);
+                at += 24 * row;
+            }
+        } else {
+#pragma unroll
+            for (int ks = 0; ks < 2; ks++) {
+#pragma unroll
+                for (int i = 0; i < 8; i++) x[ks][i] = *(const float *) (xp + (min(32 * ks + 8 * grp + i, left - 1) * row + 4 * (uint32_t) pch));
+            }
+        }
     };
-    auto put = [&]() {
+    // and on to LDS
+    auto put = [&](int turn) {
 #pragma unroll
-        for (int q = 0; q < 2 * NK; q++) *(uint4v *) (buf + tid * 16 + q * 4096) = stage[q];
+        for (int q = 0; q < STAGE; q++) {
+            if (OUT) *(uint4v *) (cbuf + (tid + q * THREADS) * 16) = stage_c[q];
+            *(uint4v *) (bbuf + turn % SLOTS * OPERAND + (tid + q * THREADS) * 16) = stage_b[q];
+        }
+#pragma unroll
+        for (int q = 0; q < (4 * STEP_WORDS + THREADS - 1) / THREADS; q++) {
+            const int i = tid + q * THREADS;
+            if (i < heads * STEP_WORDS) steps[turn * P.hw * STEP_WORDS + i] = st_next[q];
+        }
     };
 
     float decay = 1.0f;                                        // of the segment so far
-    fetch(c0, OUT ? 0 : 1);
+    fetch(c0);
+    put(0);
     for (int c = c0; c < c1; c++) {
-        const int left = P.T - c * Q;
-        // X's inputs: token 32 ks + 8 grp + i of the wave's channels
-        float x[PT][2][8];
-        {
-            // one lane offset for all of them: the rest of each address is the wave's
-            const float * xp = L.x + h * L.x_h + s * L.x_s + (P.t0 + c * Q) * L.x_t;
-            if (left >= Q) {
-#pragma unroll
-                for (int ks = 0; ks < 2; ks++) {
-#pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        const float * xi = xp + (32 * ks + i) * L.x_t;
-#pragma unroll
-                        for (int pt = 0; pt < PT; pt++) x[pt][ks][i] = xi[(uint32_t) (8 * grp * (int) L.x_t + pch[pt])];
-                    }
-                }
-            } else {
-#pragma unroll
-                for (int ks = 0; ks < 2; ks++) {
-#pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        const int t = min(32 * ks + 8 * grp + i, left - 1);
-#pragma unroll
-                        for (int pt = 0; pt < PT; pt++) x[pt][ks][i] = xp[(uint32_t) (t * (int) L.x_t + pch[pt])];
-                    }
-                }
-            }
-        }
-        __syncthreads();                                       // the last chunk's reads of LDS are done
-        put();
-        {
-            const float * sp = (const float *) (P.ws + P.steps) + (((int64_t) s * P.nc + c) * L.H + g * per + hb) * STEP_WORDS;
-            for (int i = tid; i < heads * (STEP_WORDS / 4); i += 256) ((float4 *) steps)[i] = ((const float4 *) sp)[i];
-        }
-        const float * scales = (const float *) (P.ws + P.scales) + (((int64_t) s * P.nc + c) * L.G + g) * 4;
-        const float inv_c = scales[0], inv_b = scales[1], gmost = scales[2];
-        if (OUT) fetch(c, 1);
-        __syncthreads();
-        const float * my = steps + (active ? hl : 0) * STEP_WORDS;
+        const int turn = (c - c0) & 1, left = P.T - c * Q;
+        const bool whole = left >= Q && 16 * (slice + 1) <= L.P;   // every lane's tokens and channels
+        const float inv_c = sc_next[0], inv_b = sc_next[1], gmost = sc_next[2];
+        const char * B = bbuf + turn % SLOTS * OPERAND + lane * 16;
+        __syncthreads();                                       // this chunk's LDS is written
+        const float * head_steps = steps + turn * P.hw * STEP_WORDS, * my = head_steps + (active ? hl : 0) * STEP_WORDS;
         const float e_last = my[Q - 1];
         if (OUT) {
-            // (C_t . B_j) exp(c_t - c_j) below the diagonal, split, in the order of the A operand: thread's row t, eight j
-            const float * G = (const float *) (P.ws + P.gmat) + (((int64_t) s * P.nc + c) * L.G + g) * Q * Q;
-            for (int it = tid; it < heads * 384; it += 256) {
-                const int k = it / 384, e = it - k * 384;
-                const int t = e < 128 ? e / 4 : 32 + (e - 128) / 8, jb = e < 128 ? e % 4 : e % 8;
-                const float * st = steps + k * STEP_WORDS;
+            // (C_t . B_j) exp(c_t - c_j) below the diagonal, split, in the order of the A operand
+            for (int k = wave / 4; k < heads; k += WAVES / 4) {
+                const float * st = head_steps + k * STEP_WORDS;
                 const float sm = scale_of(gmost * fmaxf(1.0f, st[Q - 1]));
-                const float ht = st[3 * Q + t], lt = st[4 * Q + t];
-                const float4 g0 = *(const float4 *) (G + t * Q + 8 * jb), g1 = *(const float4 *) (G + t * Q + 8 * jb + 4);
-                const float4 h0 = *(const float4 *) (st + 3 * Q + 8 * jb), h1 = *(const float4 *) (st + 3 * Q + 8 * jb + 4);
-                const float4 l0 = *(const float4 *) (st + 4 * Q + 8 * jb), l1 = *(const float4 *) (st + 4 * Q + 8 * jb + 4);
-                const float gg[8] = { g0.x, g0.y, g0.z, g0.w, g1.x, g1.y, g1.z, g1.w };
-                const float hh[8] = { h0.x, h0.y, h0.z, h0.w, h1.x, h1.y, h1.z, h1.w };
-                const float ll[8] = { l0.x, l0.y, l0.z, l0.w, l1.x, l1.y, l1.z, l1.w };
-                float v[8];
+                const float ht = st[3 * Q + mt], lt = st[4 * Q + mt];
+                const int tt = mt / 16;
+                char * at = mats + k * 2 * M_BYTES + (mt % 16 + 16 * mj) * 16;
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const float w = gg[i] * sm * exp2_hw((ht - hh[i]) + (lt - ll[i]));
-                    v[i] = 8 * jb + i <= t ? w : 0.0f;
+                for (int q = 0; q < 2; q++) {
+                    if (q == 1 && mt < 32) break;
+                    const int j0 = 8 * mj + 32 * q;
+                    const float4 h0 = *(const float4 *) (st + 3 * Q + j0), h1 = *(const float4 *) (st + 3 * Q + j0 + 4);
+                    const float4 l0 = *(const float4 *) (st + 4 * Q + j0), l1 = *(const float4 *) (st + 4 * Q + j0 + 4);
+                    const float hh[8] = { h0.x, h0.y, h0.z, h0.w, h1.x, h1.y, h1.z, h1.w };
+                    const float ll[8] = { l0.x, l0.y, l0.z, l0.w, l1.x, l1.y, l1.z, l1.w };
+                    float v[8];
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        const float w = as_f32(gg[q][i] * sm * exp2_hw((ht - hh[i]) + (lt - ll[i])));
+                        v[i] = j0 + i <= mt ? w : 0.0f;
+                    }
+                    half8 hi, lo;
+                    split8(v, hi, lo);
+                    char * o = at + (tt < 2 ? tt : 2 * tt - 2 + q) * 1024;
+                    *(half8 *) o = hi;
+                    *(half8 *) (o + M_BYTES) = lo;
                 }
-                half8 hi, lo;
-                split8(v, hi, lo);
-                const int tt = t / 16, blk = tt < 2 ? tt : 2 * tt - 2 + jb / 4;
-                char * at = mats + k * 2 * M_BYTES + blk * 1024 + (t % 16 + 16 * (jb % 4)) * 16;
-                *(half8 *) at = hi;
-                *(half8 *) (at + M_BYTES) = lo;
             }
         }
         // X = d x, cleared of tokens past the last and of values that are not finite
-        int bad[PT];                                           // the channel's first token with such a value
-        float sx[PT];
+        int bad = Q;                                           // the channel's first token with such a value
+        bool odd_chunk;
+        float most = 0.0f;
         {
             float odd = 0.0f;
 #pragma unroll
-            for (int pt = 0; pt < PT; pt++) {
-                float most = 0.0f;
-                bad[pt] = Q;
+            for (int ks = 0; ks < 2; ks++) {
+                const float4 d0 = *(const float4 *) (my + 2 * Q + 32 * ks + 8 * grp), d1 = *(const float4 *) (my + 2 * Q + 32 * ks + 8 * grp + 4);
+                const float dd[8] = { d0.x, d0.y, d0.z, d0.w, d1.x, d1.y, d1.z, d1.w };
+#pragma unroll
+                for (int i = 0; i < 8; i++) x[ks][i] *= dd[i];
+            }
+            if (!whole) {
 #pragma unroll
                 for (int ks = 0; ks < 2; ks++) {
-                    const float4 d0 = *(const float4 *) (my + 2 * Q + 32 * ks + 8 * grp), d1 = *(const float4 *) (my + 2 * Q + 32 * ks + 8 * grp + 4);
-                    const float dd[8] = { d0.x, d0.y, d0.z, d0.w, d1.x, d1.y, d1.z, d1.w };
 #pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        const float v = pok[pt] && 32 * ks + 8 * grp + i < left ? x[pt][ks][i] * dd[i] : 0.0f;
-                        x[pt][ks][i] = v;
-                        odd = fmaf(v, 0.0f, odd);
-                        most = fmaxf(most, fabsf(v));
-                    }
-                }
-                sx[pt] = most;
-            }
-            if (__any(odd != 0.0f)) {
-#pragma unroll
-                for (int pt = 0; pt < PT; pt++) {
-                    sx[pt] = 0.0f;
-#pragma unroll
-                    for (int ks = 1; ks >= 0; ks--) {
-#pragma unroll
-                        for (int i = 7; i >= 0; i--) {
-                            const bool fine = fabsf(x[pt][ks][i]) < INFINITY;
-                            if (!fine) bad[pt] = 32 * ks + 8 * grp + i;
-                            x[pt][ks][i] = fine ? x[pt][ks][i] : 0.0f;
-                            sx[pt] = fmaxf(sx[pt], fabsf(x[pt][ks][i]));
-                        }
-                    }
-                    bad[pt] = min(bad[pt], __shfl_xor(bad[pt], 16, WAVE));
-                    bad[pt] = min(bad[pt], __shfl_xor(bad[pt], 32, WAVE));
+                    for (int i = 0; i < 8; i++) x[ks][i] = pok && 32 * ks + 8 * grp + i < left ? x[ks][i] : 0.0f;
                 }
             }
 #pragma unroll
-            for (int pt = 0; pt < PT; pt++) {
-                sx[pt] = fmaxf(sx[pt], __shfl_xor(sx[pt], 16, WAVE));
-                sx[pt] = fmaxf(sx[pt], __shfl_xor(sx[pt], 32, WAVE));
+            for (int ks = 0; ks < 2; ks++) {
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    odd = fmaf(x[ks][i], 0.0f, odd);
+                    most = fmaxf(most, fabsf(x[ks][i]));
+                }
             }
+            odd_chunk = __any(odd != 0.0f);
+            if (odd_chunk) {
+                most = 0.0f;
+#pragma unroll
+                for (int ks = 1; ks >= 0; ks--) {
+#pragma unroll
+                    for (int i = 7; i >= 0; i--) {
+                        const bool fine = fabsf(x[ks][i]) < INFINITY;
+                        if (!fine) bad = 32 * ks + 8 * grp + i;
+                        x[ks][i] = fine ? x[ks][i] : 0.0f;
+                        most = fmaxf(most, fabsf(x[ks][i]));
+                    }
+                }
+                bad = min(bad, __shfl_xor(bad, 16, WAVE));
+                bad = min(bad, __shfl_xor(bad, 32, WAVE));
+            }
+            most = column_max(most);
         }
+        half8 xh[2], xl[2];
         if (OUT) {
-            // exp(c_t) C_t S
-            float4v acc[4][PT];
-            float inv_s[PT];
+            // C_t S
+            float4v acc[4];
+            float inv_s = 1.0f;
             if (active) {
-                float ss[PT];
+                float top = 0.0f;
 #pragma unroll
-                for (int pt = 0; pt < PT; pt++) {
-                    float most = 0.0f;
+                for (int nt = 0; nt < 2 * NK; nt++) {
+#pragma unroll
+                    for (int i = 0; i < 4; i++) top = fmaxf(top, fabsf(S[nt][i]));
+                }
+                top = column_max(top);
+                if (__any(!(top < INFINITY))) {
+                    top = 0.0f;
 #pragma unroll
                     for (int nt = 0; nt < 2 * NK; nt++) {
 #pragma unroll
-                        for (int i = 0; i < 4; i++) most = fmaxf(most, fabsf(S[nt][pt][i]));
+                        for (int i = 0; i < 4; i++) top = fmaxf(top, finite_abs(S[nt][i]));
                     }
-                    most = fmaxf(most, __shfl_xor(most, 16, WAVE));
-                    most = fmaxf(most, __shfl_xor(most, 32, WAVE));
-                    if (__any(!(most < INFINITY))) {
-                        most = 0.0f;
-#pragma unroll
-                        for (int nt = 0; nt < 2 * NK; nt++) {
-#pragma unroll
-                            for (int i = 0; i < 4; i++) most = fmaxf(most, finite_abs(S[nt][pt][i]));
-                        }
-                        most = fmaxf(most, __shfl_xor(most, 16, WAVE));
-                        most = fmaxf(most, __shfl_xor(most, 32, WAVE));
-                    }
-                    ss[pt] = scale_of(most);
-                    inv_s[pt] = inverse_of(ss[pt]) * inv_c;
+                    top = column_max(top);
                 }
+                const float ss = scale_of(top);
+                inv_s = inverse_of(ss) * inv_c;
 #pragma unroll
-                for (int tt = 0; tt < 4; tt++) {
-#pragma unroll
-                    for (int pt = 0; pt < PT; pt++) acc[tt][pt] = float4v{ 0, 0, 0, 0 };
-                }
+                for (int tt = 0; tt < 4; tt++) acc[tt] = float4v{ 0, 0, 0, 0 };
 #pragma unroll
                 for (int ks = 0; ks < NK; ks++) {
-                    half8 bh[PT], bl[PT];
-#pragma unroll
-                    for (int pt = 0; pt < PT; pt++) {
-                        float v[8];
-#pragma unroll
-                        for (int i = 0; i < 8; i++) v[i] = as_f32(S[2 * ks + i / 4][pt][i % 4] * ss[pt]);
-                        split8(v, bh[pt], bl[pt]);
-                    }
+                    half8 ah[4], al[4], bh, bl;
 #pragma unroll
                     for (int tt = 0; tt < 4; tt++) {
-                        const char * a = buf + ((tt * NK + ks) * 64 + lane) * 16;
-                        const half8 ah = *(const half8 *) a, al = *(const half8 *) (a + PLANE);
-#pragma unroll
-                        for (int pt = 0; pt < PT; pt++) acc[tt][pt] = mfma3(ah, al, bh[pt], bl[pt], acc[tt][pt]);
+                        const char * a = cbuf + ((tt * NK + ks) * 64 + lane) * 16;
+                        ah[tt] = *(const half8 *) a;
+                        al[tt] = *(const half8 *) (a + PLANE);
                     }
+                    float v[8];
+#pragma unroll
+                    for (int i = 0; i < 8; i++) v[i] = as_f32(S[2 * ks + i / 4][i % 4] * ss);
+                    split8(v, bh, bl);
+#pragma unroll
+                    for (int tt = 0; tt < 4; tt++) acc[tt] = mfma(al[tt], bh, acc[tt]);
+#pragma unroll
+                    for (int tt = 0; tt < 4; tt++) acc[tt] = mfma(ah[tt], bl, acc[tt]);
+#pragma unroll
+                    for (int tt = 0; tt < 4; tt++) acc[tt] = mfma(ah[tt], bh, acc[tt]);
                 }
             }
             __syncthreads();                                   // C is read, the matrices are written
-            put();
             if (active) {
-                half8 xh[PT][2], xl[PT][2];
-                float inv_x[PT];
-                const float inv_m = inverse_of(scale_of(gmost * fmaxf(1.0f, e_last)));
+                const float sc = scale_of(most);
+                const float inv = inverse_of(scale_of(gmost * fmaxf(1.0f, e_last))) * inverse_of(sc);
 #pragma unroll
-                for (int pt = 0; pt < PT; pt++) {
-                    const float sc = scale_of(sx[pt]);
-                    inv_x[pt] = inverse_of(sc);
+                for (int ks = 0; ks < 2; ks++) {
+                    float v[8];
 #pragma unroll
-                    for (int ks = 0; ks < 2; ks++) {
-                        float v[8];
-#pragma unroll
-                        for (int i = 0; i < 8; i++) v[i] = as_f32(x[pt][ks][i] * sc);
-                        split8(v, xh[pt][ks], xl[pt][ks]);
-                    }
+                    for (int i = 0; i < 8; i++) v[i] = as_f32(x[ks][i] * sc);
+                    split8(v, xh[ks], xl[ks]);
                 }
                 const char * mine = mats + hl * 2 * M_BYTES + lane * 16;
-                float * y = L.y + h * L.P + (int64_t) L.P * L.H * (P.t0 + c * Q + L.T * s);
+                half8 ah[6], al[6];
+#pragma unroll
+                for (int b = 0; b < 6; b++) {
+                    ah[b] = *(const half8 *) (mine + b * 1024);
+                    al[b] = *(const half8 *) (mine + b * 1024 + M_BYTES);
+                }
+                // tiles 0 and 1 end within the first 32 tokens
+                float4v sum[4];
+#pragma unroll
+                for (int tt = 0; tt < 4; tt++) sum[tt] = mfma(al[tt < 2 ? tt : 2 * tt - 2], xh[0], float4v{ 0, 0, 0, 0 });
+#pragma unroll
+                for (int tt = 0; tt < 4; tt++) sum[tt] = mfma(ah[tt < 2 ? tt : 2 * tt - 2], xl[0], sum[tt]);
+#pragma unroll
+                for (int tt = 0; tt < 4; tt++) sum[tt] = mfma(ah[tt < 2 ? tt : 2 * tt - 2], xh[0], sum[tt]);
+#pragma unroll
+                for (int tt = 2; tt < 4; tt++) sum[tt] = mfma(al[2 * tt - 1], xh[1], sum[tt]);
+#pragma unroll
+                for (int tt = 2; tt < 4; tt++) sum[tt] = mfma(ah[2 * tt - 1], xl[1], sum[tt]);
+#pragma unroll
+                for (int tt = 2; tt < 4; tt++) sum[tt] = mfma(ah[2 * tt - 1], xh[1], sum[tt]);
 #pragma unroll
                 for (int tt = 0; tt < 4; tt++) {
-                    float4v sum[PT];
-#pragma unroll
-                    for (int pt = 0; pt < PT; pt++) sum[pt] = float4v{ 0, 0, 0, 0 };
-#pragma unroll
-                    for (int ks = 0; ks <= tt / 2; ks++) {
-                        const char * a = mine + (tt < 2 ? tt : 2 * tt - 2 + ks) * 1024;
-                        const half8 ah = *(const half8 *) a, al = *(const half8 *) (a + M_BYTES);
-#pragma unroll
-                        for (int pt = 0; pt < PT; pt++) sum[pt] = mfma3(ah, al, xh[pt][ks], xl[pt][ks], sum[pt]);
-                    }
                     const float4 e4 = *(const float4 *) (my + 16 * tt + 4 * grp);
                     const float e[4] = { e4.x, e4.y, e4.z, e4.w };
 #pragma unroll
-                    for (int pt = 0; pt < PT; pt++) {
+                    for (int i = 0; i < 4; i++) acc[tt][i] = fmaf(acc[tt][i], inv_s * e[i], sum[tt][i] * inv);
+                }
+                if (odd_chunk) {
 #pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            const int t = 16 * tt + 4 * grp + i;
-                            float v = fmaf(acc[tt][pt][i] * inv_s[pt], e[i], sum[pt][i] * inv_m * inv_x[pt]);
-                            v = t < bad[pt] ? v : NAN;
-                            if (pok[pt] && t < left) (y + (16 * tt + i) * L.P * L.H)[(uint32_t) (4 * grp * L.P * L.H + pch[pt])] = v;
+                    for (int tt = 0; tt < 4; tt++) {
+#pragma unroll
+                        for (int i = 0; i < 4; i++) acc[tt][i] = 16 * tt + 4 * grp + i < bad ? acc[tt][i] : NAN;
+                    }
+                }
+                char * y = (char *) (L.y + h * L.P + (int64_t) L.P * L.H * (P.t0 + c * Q + L.T * s));
+                const uint32_t row = 4 * (uint32_t) L.P * (uint32_t) L.H;
+                uint32_t at = 4 * grp * row + 4 * (uint32_t) pch;
+#pragma unroll
+                for (int tt = 0; tt < 4; tt++) {
+                    if (whole) {
+#pragma unroll
+                        for (int i = 0; i < 4; i++, at += row) *(float *) (y + at) = acc[tt][i];
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 4; i++, at += row) {
+                            if (pok && 16 * tt + 4 * grp + i < left) *(float *) (y + at) = acc[tt][i];
                         }
                     }
+                    at += 12 * row;
                 }
             }
-            if (c + 1 < c1) fetch(c + 1, 0);
-            __syncthreads();                                   // B is in place
-        } else if (c + 1 < c1) {
-            fetch(c + 1, 1);
         }
         // the state at the chunk's end
+        float inv_u = 1.0f;
         if (active) {
-            half8 xh[PT][2], xl[PT][2];
-            float inv_x[PT];
-            const float grow = fmaxf(1.0f, my[Q]);
+            const float sc = scale_of(most * fmaxf(1.0f, my[Q]));
+            inv_u = inverse_of(sc) * inv_b;
 #pragma unroll
-            for (int pt = 0; pt < PT; pt++) {
-                const float sc = scale_of(sx[pt] * grow);
-                inv_x[pt] = inverse_of(sc) * inv_b;
+            for (int ks = 0; ks < 2; ks++) {
+                const float4 w0 = *(const float4 *) (my + Q + 32 * ks + 8 * grp), w1 = *(const float4 *) (my + Q + 32 * ks + 8 * grp + 4);
+                const float ww[8] = { w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w };
+                float v[8];
+#pragma unroll
+                for (int i = 0; i < 8; i++) v[i] = as_f32(x[ks][i] * ww[i] * sc);
+                split8(v, xh[ks], xl[ks]);
+            }
+        }
+        if (c + 1 < c1) fetch(c + 1);
+        if (active) {
+#pragma unroll
+            for (int n0 = 0; n0 < 2 * NK; n0 += 2) {
+                float4v sum[2];
+                half8 ah[2][2], al[2][2];
+#pragma unroll
+                for (int q = 0; q < 2; q++) {
+#pragma unroll
+                    for (int ks = 0; ks < 2; ks++) {
+                        ah[q][ks] = *(const half8 *) (B + ((n0 + q) * 2 + ks) * 1024);
+                        al[q][ks] = *(const half8 *) (B + ((n0 + q) * 2 + ks) * 1024 + PLANE);
+                    }
+                }
+#pragma unroll
+                for (int q = 0; q < 2; q++) sum[q] = mfma(al[q][0], xh[0], float4v{ 0, 0, 0, 0 });
+#pragma unroll
+                for (int q = 0; q < 2; q++) sum[q] = mfma(al[q][1], xh[1], sum[q]);
 #pragma unroll
                 for (int ks = 0; ks < 2; ks++) {
-                    const float4 w0 = *(const float4 *) (my + Q + 32 * ks + 8 * grp), w1 = *(const float4 *) (my + Q + 32 * ks + 8 * grp + 4);
-                    const float ww[8] = { w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w };
-                    float v[8];
 #pragma unroll
-                    for (int i = 0; i < 8; i++) v[i] = as_f32(x[pt][ks][i] * ww[i] * sc);
-                    split8(v, xh[pt][ks], xl[pt][ks]);
+                    for (int q = 0; q < 2; q++) sum[q] = mfma(ah[q][ks], xl[ks], sum[q]);
+#pragma unroll
+                    for (int q = 0; q < 2; q++) sum[q] = mfma(ah[q][ks], xh[ks], sum[q]);
+                }
+#pragma unroll
+                for (int q = 0; q < 2; q++) {
+#pragma unroll
+                    for (int i = 0; i < 4; i++) S[n0 + q][i] = fmaf(S[n0 + q][i], e_last, sum[q][i] * inv_u);
                 }
             }
+            if (odd_chunk) {
 #pragma unroll
-            for (int nt = 0; nt < 2 * NK; nt++) {
-                float4v sum[PT];
+                for (int nt = 0; nt < 2 * NK; nt++) {
 #pragma unroll
-                for (int pt = 0; pt < PT; pt++) sum[pt] = float4v{ 0, 0, 0, 0 };
-#pragma unroll
-                for (int ks = 0; ks < 2; ks++) {
-                    const char * a = buf + ((nt * 2 + ks) * 64 + lane) * 16;
-                    const half8 ah = *(const half8 *) a, al = *(const half8 *) (a + PLANE);
-#pragma unroll
-                    for (int pt = 0; pt < PT; pt++) sum[pt] = mfma3(ah, al, xh[pt][ks], xl[pt][ks], sum[pt]);
-                }
-#pragma unroll
-                for (int pt = 0; pt < PT; pt++) {
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const float v = fmaf(S[nt][pt][i], e_last, sum[pt][i] * inv_x[pt]);
-                        S[nt][pt][i] = bad[pt] < Q ? NAN : v;
-                    }
+                    for (int i = 0; i < 4; i++) S[nt][i] = bad < Q ? NAN : S[nt][i];
                 }
             }
             decay *= e_last;
         }
+        if (SLOTS == 1) __syncthreads();                       // B is read
+        if (c + 1 < c1) put(turn ^ 1);
     }
     if (!active) return;
     if (!OUT) {
         if (lane == 0 && slice == 0) ((float *) (P.ws + P.decays))[((int64_t) s * P.n_seg + sg) * L.H + h] = decay;
         float4v * q = part_at(sg);
 #pragma unroll
+        for (int nt = 0; nt < 2 * NK; nt++) q[nt * WAVE] = S[nt];
+    } else if (c1 == P.nc && pok) {
+        float * s1 = P.s1 + (int64_t) L.N * (pch + (int64_t) L.P * (h + (int64_t) L.H * s));
+#pragma unroll
         for (int nt = 0; nt < 2 * NK; nt++) {
+            const int n = 16 * nt + 4 * grp;
+            if (P.vec_s1 && n + 3 < L.N) {
+                *(float4 *) (s1 + n) = make_float4(S[nt][0], S[nt][1], S[nt][2], S[nt][3]);
+            } else {
 #pragma unroll
-            for (int pt = 0; pt < PT; pt++) q[(nt * PT + pt) * WAVE] = S[nt][pt];
-        }
-    } else if (c1 == P.nc) {
-#pragma unroll
-        for (int pt = 0; pt < PT; pt++) {
-            if (!pok[pt]) continue;
-            float * s1 = P.s1 + (int64_t) L.N * (pch[pt] + (int64_t) L.P * (h + (int64_t) L.H * s));
-#pragma unroll
-            for (int nt = 0; nt < 2 * NK; nt++) {
-                const int n = 16 * nt + 4 * grp;
-                if (P.vec_s1 && n + 3 < L.N) {
-                    *(float4 *) (s1 + n) = make_float4(S[nt][pt][0], S[nt][pt][1], S[nt][pt][2], S[nt][pt][3]);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        if (n + i < L.N) s1[n + i] = S[nt][pt][i];
-                    }
+                for (int i = 0; i < 4; i++) {
+                    if (n + i < L.N) s1[n + i] = S[nt][i];
                 }
             }
         }
@@ -655,11 +699,9 @@ __global__ __launch_bounds__(256, 2) void ssm_scan_mm_kernel(mm_plan P) {
 // ---------------------------------------------------------------------------------------------
 
 int steps_of(int N) { return N <= 32 ? 1 : N <= 64 ? 2 : N <= 128 ? 4 : 8; }
-// two tiles of channels per wave read each operand from LDS once for both; eight steps of states leave no registers for that
-int tiles_of(int N, int P) { return steps_of(N) == 8 || P <= 16 ? 1 : 2; }
 
 struct mm_sizes {
-    int     nk, pt, slices, hw, head_blocks, p_blocks;
+    int     nk, slices, hw, head_blocks, p_blocks;
     int64_t chunks, block, n_seg, seg;      // chunks in all and per block of tokens, segments of a block
     int64_t planes, gmat, scales, steps, parts, decays, state, total;
 };
@@ -667,19 +709,20 @@ struct mm_sizes {
 mm_sizes mm_size(const ssm_scan_launch & L) {
     mm_sizes z;
     z.nk = steps_of(L.N);
-    z.pt = tiles_of(L.N, L.P);
-    z.slices = (L.P + 16 * z.pt - 1) / (16 * z.pt);
-    z.hw = z.slices == 1 ? 4 : z.slices == 2 ? 2 : 1;
-    z.p_blocks = (z.slices + 3) / 4;
+    z.slices = (L.P + 15) / 16;
+    z.p_blocks = (z.slices + WAVES - 1) / WAVES;
+    // heads of a workgroup: as its waves allow, and their matrices' 15 KiB each beside the operands
+    z.hw = z.p_blocks > 1 ? 1 : std::min(WAVES / z.slices, z.nk == 8 ? 2 : 4);
     z.head_blocks = (L.H / L.G + z.hw - 1) / z.hw;
     z.chunks = (L.T + Q - 1) / Q;
     const int64_t rec = (int64_t) z.nk * 16384 + Q * Q * 4 + 16, per = L.S * (L.G * rec + (int64_t) L.H * STEP_WORDS * 4);
     // prepared operands of at most 64 MiB: the tokens go through in blocks
     z.block = std::max<int64_t>(1, std::min<int64_t>({ z.chunks, ((int64_t) 64 << 20) / per, 65535 }));
-    // segments until two workgroups of every CU have work, of at least two chunks
+    // segments until every CU has a workgroup
     const int64_t base = L.S * L.G * z.head_blocks * z.p_blocks;
-    const int64_t part = L.S * L.H * (int64_t) z.slices * (2 * z.nk * z.pt * WAVE * 16 + 4);
-    z.n_seg = std::max<int64_t>(1, std::min<int64_t>({ (512 + base - 1) / base, z.block / 2, ((int64_t) 32 << 20) / part }));
+    const int64_t part = L.S * L.H * (int64_t) z.slices * (2 * z.nk * WAVE * 16) + L.S * L.H * 4;
+    static const int segmin = getenv("SEGMIN") ? atoi(getenv("SEGMIN")) : 2;
+    z.n_seg = std::max<int64_t>(1, std::min<int64_t>({ 256 / base, z.block / segmin, ((int64_t) 32 << 20) / part }));
     z.seg = (z.block + z.n_seg - 1) / z.n_seg;
     z.n_seg = (z.block + z.seg - 1) / z.seg;
     int64_t at = 0;
@@ -688,7 +731,7 @@ mm_sizes mm_size(const ssm_scan_launch & L) {
     z.gmat = take(L.S * z.block * L.G * Q * Q * 4);
     z.scales = take(L.S * z.block * L.G * 16);
     z.steps = take(L.S * z.block * (int64_t) L.H * STEP_WORDS * 4);
-    z.parts = take(z.n_seg > 1 ? L.S * z.n_seg * (int64_t) L.H * z.slices * 2 * z.nk * z.pt * WAVE * 16 : 0);
+    z.parts = take(z.n_seg > 1 ? L.S * z.n_seg * (int64_t) L.H * z.slices * 2 * z.nk * WAVE * 16 : 0);
     z.decays = take(z.n_seg > 1 ? L.S * z.n_seg * (int64_t) L.H * 4 : 0);
     // states between blocks of tokens, one read while the next is written
     z.state = take(z.block < z.chunks ? 2 * L.S * (int64_t) L.N * L.P * L.H * 4 : 0);
@@ -696,17 +739,22 @@ mm_sizes mm_size(const ssm_scan_launch & L) {
     return z;
 }
 
-template <int NK, int PT>
+template <int NK>
 void launch_mm(const ssm_scan_launch & L, const mm_sizes & z, void * ws, hipStream_t st) {
     mm_plan P{};
     P.L = L;
     P.ws = (char *) ws;
     P.planes = z.planes; P.gmat = z.gmat; P.scales = z.scales; P.steps = z.steps; P.parts = z.parts; P.decays = z.decays;
     P.hw = z.hw; P.slices = z.slices; P.head_blocks = z.head_blocks; P.p_blocks = z.p_blocks;
-    static const bool lds_set = [] {
-        HIP_CHECK(hipFuncSetAttribute((const void *) ssm_prepare_kernel<NK>, hipFuncAttributeMaxDynamicSharedMemorySize, NK * 16384 + 64));
-        HIP_CHECK(hipFuncSetAttribute((const void *) ssm_scan_mm_kernel<NK, PT, true>, hipFuncAttributeMaxDynamicSharedMemorySize,
-                                      NK * 8192 + 4 * (STEP_WORDS * 4 + 2 * M_BYTES)));
+    constexpr int OPERAND = NK * 8192;
+    auto lds_of = [](int hw, bool out) {
+        return (size_t) OPERAND * (b_slots(NK) + (out ? 1 : 0)) + (size_t) hw * (2 * STEP_WORDS * 4 + (out ? 2 * M_BYTES : 0));
+    };
+    static const bool lds_set = [&] {
+        const int hw = NK == 8 ? 2 : 4;
+        HIP_CHECK(hipFuncSetAttribute((const void *) ssm_operands_kernel<NK>, hipFuncAttributeMaxDynamicSharedMemorySize, OPERAND + 64));
+        HIP_CHECK(hipFuncSetAttribute((const void *) ssm_scan_mm_kernel<NK, false>, hipFuncAttributeMaxDynamicSharedMemorySize, (int) lds_of(hw, false)));
+        HIP_CHECK(hipFuncSetAttribute((const void *) ssm_scan_mm_kernel<NK, true>, hipFuncAttributeMaxDynamicSharedMemorySize, (int) lds_of(hw, true)));
         return true;
     }();
     (void) lds_set;
@@ -725,13 +773,11 @@ void launch_mm(const ssm_scan_launch & L, const mm_sizes & z, void * ws, hipStre
         P.s1 = c + z.block < z.chunks ? hold + turn * states : L.s_out;
         P.vec_s0 = c == 0 ? rows16(L.s, L.s_p, L.s_h, L.s_row) : L.N % 4 == 0 && (uintptr_t) P.s0 % 16 == 0;
         P.vec_s1 = L.N % 4 == 0 && (uintptr_t) P.s1 % 16 == 0;
-        const size_t planes = (size_t) NK * 8192;
-        launch(ssm_prepare_kernel<NK>, dim3((unsigned) P.nc, (unsigned) (L.G + (L.H + 15) / 16), (unsigned) L.S), dim3(256),
-               std::max<size_t>(2 * planes + 64, Q * 17 * 4), st, P);
-        const size_t lds = planes + (size_t) z.hw * STEP_WORDS * 4;
-        const unsigned members = (unsigned) (z.head_blocks * z.p_blocks);
-        if (P.n_seg > 1) launch(ssm_scan_mm_kernel<NK, PT, false>, dim3((unsigned) (L.S * L.G * P.n_seg) * members), dim3(256), lds, st, P);
-        launch(ssm_scan_mm_kernel<NK, PT, true>, dim3((unsigned) (L.S * L.G * P.n_seg) * members), dim3(256), lds + (size_t) z.hw * 2 * M_BYTES, st, P);
+        launch(ssm_steps_kernel, dim3((unsigned) P.nc, (unsigned) ((L.H + 15) / 16), (unsigned) L.S), dim3(256), 0, st, P);
+        launch(ssm_operands_kernel<NK>, dim3((unsigned) P.nc, (unsigned) L.G, (unsigned) L.S), dim3(256), OPERAND + 64, st, P);
+        const dim3 grid((unsigned) (L.S * L.G * P.n_seg * z.head_blocks * z.p_blocks));
+        if (P.n_seg > 1) launch(ssm_scan_mm_kernel<NK, false>, grid, dim3(THREADS), lds_of(z.hw, false), st, P);
+        launch(ssm_scan_mm_kernel<NK, true>, grid, dim3(THREADS), lds_of(z.hw, true), st, P);
     }
 }
 
@@ -739,7 +785,7 @@ void launch_mm(const ssm_scan_launch & L, const mm_sizes & z, void * ws, hipStre
 
 bool ssm_scan_mm_takes(const ssm_scan_launch & L) {
     // the grids' limits: one dimension each for the sequences and for groups and heads
-    return L.a_scalar && L.T >= SSM_MM_MIN_TOKENS && L.S <= 65535 && L.G + (L.H + 15) / 16 <= 65535 &&
+    return L.a_scalar && L.T >= SSM_MM_MIN_TOKENS && L.S <= 65535 && L.G <= 65535 && L.H <= 16 * 65535 &&
            L.S * (int64_t) L.H * L.P < INT32_MAX &&
            // 32-bit offsets within a chunk
            L.x_t >= 0 && L.x_t <= 1 << 24 && (int64_t) L.H * L.P <= 1 << 24 && L.P <= 1 << 24;
@@ -749,8 +795,8 @@ int64_t ssm_scan_mm_scratch_bytes(const ssm_scan_launch & L) { return mm_size(L)
 
 void launch_ssm_scan_mm(const ssm_scan_launch & L, void * ws, hipStream_t st) {
     const mm_sizes z = mm_size(L);
-    if (z.nk == 8) launch_mm<8, 1>(L, z, ws, st);
-    else if (z.nk == 4) z.pt == 2 ? launch_mm<4, 2>(L, z, ws, st) : launch_mm<4, 1>(L, z, ws, st);
-    else if (z.nk == 2) z.pt == 2 ? launch_mm<2, 2>(L, z, ws, st) : launch_mm<2, 1>(L, z, ws, st);
-    else z.pt == 2 ? launch_mm<1, 2>(L, z, ws, st) : launch_mm<1, 1>(L, z, ws, st);
+    if (z.nk == 8) launch_mm<8>(L, z, ws, st);
+    else if (z.nk == 4) launch_mm<4>(L, z, ws, st);
+    else if (z.nk == 2) launch_mm<2>(L, z, ws, st);
+    else launch_mm<1>(L, z, ws, st);
 }
