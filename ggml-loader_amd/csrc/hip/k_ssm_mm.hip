@@ -114,7 +114,7 @@ __global__ __launch_bounds__(256) void ssm_operands_kernel(mm_plan P) {
     extern __shared__ __align__(16) char lds[];                // B's planes: blocks of 16 tokens by 32 states
     const ssm_scan_launch & L = P.L;
     const int c = blockIdx.x, g = blockIdx.y, s = blockIdx.z;
-    const int tid = threadIdx.x, lane = tid % WAVE, wave = tid / WAVE;
+    const int tid = threadIdx.x, lane = tid % WAVE, wave = __builtin_amdgcn_readfirstlane(tid / WAVE);
     const int left = P.T - c * Q;             // tokens from the chunk's first on
     constexpr int PLANE = 4 * 1024 * NK;
     float * red = (float *) (lds + 2 * PLANE);
@@ -220,7 +220,7 @@ __global__ __launch_bounds__(256) void ssm_steps_kernel(mm_plan P) {
     __shared__ float lds[Q * 17];
     const ssm_scan_launch & L = P.L;
     const int c = blockIdx.x, h0 = blockIdx.y * 16, s = blockIdx.z;
-    const int tid = threadIdx.x, lane = tid % WAVE, wave = tid / WAVE, left = P.T - c * Q;
+    const int tid = threadIdx.x, lane = tid % WAVE, wave = __builtin_amdgcn_readfirstlane(tid / WAVE), left = P.T - c * Q;
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         const int t = 16 * i + tid / 16, h = h0 + tid % 16;
@@ -271,6 +271,13 @@ constexpr int THREADS = WAVES * WAVE;
 // B's buffers: the next chunk's beside this one's, where they fit 160 KiB with C's and the matrices
 constexpr int b_slots(int nk) { return nk == 8 ? 1 : 2; }
 
+// An offset that is formed where it is used: kept for the whole loop, with the fifteen that follow from it,
+// it would take the registers that the loop is short of.
+__device__ __forceinline__ uint32_t here(uint32_t x) {
+    asm volatile("" : "+v"(x));
+    return x;
+}
+
 // most |a[i]|, over the four lanes of a column
 __device__ __forceinline__ float column_max(float m) {
     m = fmaxf(m, __shfl_xor(m, 16, WAVE));
@@ -291,7 +298,8 @@ __global__ __launch_bounds__(THREADS, 2) void ssm_scan_mm_kernel(mm_plan P) {
     char * bbuf = lds + (OUT ? OPERAND : 0);                   // B's, of this chunk and the next
     float * steps = (float *) (bbuf + SLOTS * OPERAND);        // per head, of this chunk and the next
     char * mats = (char *) (steps + 2 * P.hw * STEP_WORDS);    // per head: the two planes of (C_t . B_j) exp(c_t - c_j)
-    const int tid = threadIdx.x, lane = tid % WAVE, wave = tid / WAVE, col = lane % 16, grp = lane / 16;
+    // the wave's number as the scalar that it is: what depends on it alone stays out of the vector registers
+    const int tid = threadIdx.x, lane = tid % WAVE, wave = __builtin_amdgcn_readfirstlane(tid / WAVE), col = lane % 16, grp = lane / 16;
 
     // the workgroups that read the same operands take turns on one XCD (consecutive ids go to different ones)
     const int members = P.head_blocks * P.p_blocks, units = (int) (gridDim.x / (unsigned) members);
@@ -388,7 +396,7 @@ __global__ __launch_bounds__(THREADS, 2) void ssm_scan_mm_kernel(mm_plan P) {
         const char * xp = (const char *) (L.x + h * L.x_h + s * L.x_s + (P.t0 + c * Q) * L.x_t);
         const uint32_t row = 4 * (uint32_t) L.x_t;
         if (left >= Q) {
-            uint32_t at = 8 * grp * row + 4 * (uint32_t) pch;
+            uint32_t at = here(8 * grp * row + 4 * (uint32_t) pch);
 #pragma unroll
             for (int ks = 0; ks < 2; ks++) {
 #pragma unroll
@@ -599,7 +607,7 @@ __global__ __launch_bounds__(THREADS, 2) void ssm_scan_mm_kernel(mm_plan P) {
                 }
                 char * y = (char *) (L.y + h * L.P + (int64_t) L.P * L.H * (P.t0 + c * Q + L.T * s));
                 const uint32_t row = 4 * (uint32_t) L.P * (uint32_t) L.H;
-                uint32_t at = 4 * grp * row + 4 * (uint32_t) pch;
+                uint32_t at = here(4 * grp * row + 4 * (uint32_t) pch);
 #pragma unroll
                 for (int tt = 0; tt < 4; tt++) {
                     if (whole) {
