@@ -1068,17 +1068,13 @@ private:
         L.s_out = L.y + ggml_nelements(x);
         const double st = (double) L.N * L.P * L.H * L.S * 4;
         prof_scope ps(this, "ssm_scan", 2 * st + 4.0 * (2 * ggml_nelements(x) + ggml_nelements(dt) + 2 * ggml_nelements(B)));
-        if (!ssm_scan_mm_takes(L)) {
-            launch_ssm_scan(L, st_);
-            return;
-        }
         // one buffer for the graph's scans, which the stream runs one after another
-        const int64_t bytes = ssm_scan_mm_scratch_bytes(L);
+        const int64_t bytes = ssm_scan_scratch_bytes(L);
         if (bytes > ssm_bytes_) {
             ssm_buf_ = c_.scratch.alloc((size_t) bytes);
             ssm_bytes_ = bytes;
         }
-        launch_ssm_scan_mm(L, ssm_buf_, st_);
+        launch_ssm_scan(L, ssm_buf_, st_);
     }
     void * ssm_buf_ = nullptr;
     int64_t ssm_bytes_ = 0;

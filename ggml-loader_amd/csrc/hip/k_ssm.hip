@@ -2,18 +2,11 @@
 // (model.cpp:1156-1196).
 #include "hip_common.h"
 #include "kernels.h"
+#include "ssm_ops.h"
 
 #include <algorithm>
 
 namespace {
-
-// e^x by the hardware's 2^x: x * log2(e) rounds once (2^-24 of it) and v_exp_f32 is off by one unit
-constexpr float LOG2E = 1.4426950408889634f;
-
-__device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
-
-// log(1 + e^x); above 20 the sum rounds to e^x, so x itself (the unary op's rule)
-__device__ __forceinline__ float softplus(float x) { return x > 20.0f ? x : log1pf(expf(x)); }
 
 // ---------------------------------------------------------------------------------------------
 // short causal convolution
@@ -221,7 +214,13 @@ void launch_conv_rows(const ssm_conv_launch & L, hipStream_t st) {
 // ---------------------------------------------------------------------------------------------
 // selective scan
 
-// One row (sequence, head, channel) per group of LANES lanes, R states per lane, the tokens in order.
+__device__ __forceinline__ int64_t pool_row(const ssm_scan_launch & L, int64_t s) {
+    const int64_t id = L.ids[s * L.ids_s];
+    return id < 0 ? 0 : id >= L.pool ? L.pool - 1 : id;
+}
+
+// Any operands: one row (sequence, head, channel) per group of LANES lanes, R states per lane, the tokens
+// in order.
 template <int LANES, int R>
 __global__ __launch_bounds__(256) void ssm_scan_rows_kernel(ssm_scan_launch L) {
     const int64_t row = ((int64_t) blockIdx.x * 256 + threadIdx.x) / LANES;
@@ -233,9 +232,7 @@ __global__ __launch_bounds__(256) void ssm_scan_rows_kernel(ssm_scan_launch L) {
     const int p = (int) (r % L.P), h = (int) (r / L.P % L.H);
     const int64_t s = r / ((int64_t) L.P * L.H);
     const int g = h / (L.H / L.G);
-    int64_t id = L.ids[s * L.ids_s];
-    id = id < 0 ? 0 : id >= L.pool ? L.pool - 1 : id;
-    const float * s0 = L.s + p * L.s_p + h * L.s_h + id * L.s_row;
+    const float * s0 = L.s + p * L.s_p + h * L.s_h + pool_row(L, s) * L.s_row;
     const float * A = L.A + h * L.a_h;
     float st[R], a[R];
 #pragma unroll
@@ -278,6 +275,216 @@ void launch_rows(const ssm_scan_launch & L, hipStream_t st) {
     launch(ssm_scan_rows_kernel<LANES, R>, dim3((unsigned) ((rows + per - 1) / per)), dim3(256), 0, st, L);
 }
 
+// A few tokens (decoding): the states are most of what is read and written, so a lane takes them 16 bytes
+// at a time and STEP_ROWS channels at once. LANES lanes hold a channel's 4 LANES states; the group's channels
+// share B and C, and (ONE_HEAD) the time step and the decay.
+constexpr int STEP_ROWS = 4;
+
+template <int LANES, bool ONE_HEAD>
+__global__ __launch_bounds__(256) void ssm_scan_step_kernel(ssm_scan_launch L, int64_t groups) {
+    const int64_t group = ((int64_t) blockIdx.x * 256 + threadIdx.x) / LANES;
+    const int lane = threadIdx.x % LANES, n = 4 * lane;
+    if (group >= groups) return;                               // whole groups only
+    const int64_t r0 = group * STEP_ROWS, per = (int64_t) L.P * L.H, s = r0 / per;
+    const int q0 = (int) (r0 - s * per);
+    const bool on = n < L.N;
+    int p[STEP_ROWS], h[STEP_ROWS];
+#pragma unroll
+    for (int k = 0; k < STEP_ROWS; k++) {
+        h[k] = ONE_HEAD ? q0 / L.P : (q0 + k) / L.P;
+        p[k] = q0 + k - h[k] * L.P;
+    }
+    const int g = h[0] / (L.H / L.G);
+    const int64_t id = pool_row(L, s);
+    const float4 zero = make_float4(0, 0, 0, 0);
+    float4 st[STEP_ROWS], a[ONE_HEAD ? 1 : STEP_ROWS];
+#pragma unroll
+    for (int k = 0; k < STEP_ROWS; k++) st[k] = on ? *(const float4 *) (L.s + p[k] * L.s_p + h[k] * L.s_h + id * L.s_row + n) : zero;
+#pragma unroll
+    for (int k = 0; k < (ONE_HEAD ? 1 : STEP_ROWS); k++) {
+        const float * A = L.A + h[k] * L.a_h;
+        if (L.a_scalar) a[k] = make_float4(A[0], A[0], A[0], A[0]);
+        else a[k] = on ? make_float4(A[n], A[n + 1], A[n + 2], A[n + 3]) : zero;
+        a[k] = make_float4(a[k].x * LOG2E, a[k].y * LOG2E, a[k].z * LOG2E, a[k].w * LOG2E);
+    }
+    const float * B = L.B + g * L.b_g + s * L.b_s + n, * C = L.C + g * L.c_g + s * L.c_s + n;
+    float * y = L.y + q0 + per * L.T * s;
+    for (int64_t t = 0; t < L.T; t++) {
+        float d[ONE_HEAD ? 1 : STEP_ROWS], x[STEP_ROWS], v[STEP_ROWS];
+#pragma unroll
+        for (int k = 0; k < (ONE_HEAD ? 1 : STEP_ROWS); k++) d[k] = L.dt[h[k] + t * L.dt_t + s * L.dt_s];
+#pragma unroll
+        for (int k = 0; k < STEP_ROWS; k++) x[k] = L.x[p[k] + h[k] * L.x_h + t * L.x_t + s * L.x_s];
+        const float4 b = on ? *(const float4 *) (B + t * L.b_t) : zero, c = on ? *(const float4 *) (C + t * L.c_t) : zero;
+        float4 e = zero;
+#pragma unroll
+        for (int k = 0; k < STEP_ROWS; k++) {
+            if (!ONE_HEAD || k == 0) {
+                float & dk = d[ONE_HEAD ? 0 : k];
+                const float4 ak = a[ONE_HEAD ? 0 : k];
+                dk = softplus(dk);
+                e.x = exp2_hw(dk * ak.x);
+                if (ONE_HEAD && L.a_scalar) e.y = e.z = e.w = e.x;
+                else { e.y = exp2_hw(dk * ak.y); e.z = exp2_hw(dk * ak.z); e.w = exp2_hw(dk * ak.w); }
+            }
+            const float dx = d[ONE_HEAD ? 0 : k] * x[k];
+            st[k].x = fmaf(st[k].x, e.x, dx * b.x);
+            st[k].y = fmaf(st[k].y, e.y, dx * b.y);
+            st[k].z = fmaf(st[k].z, e.z, dx * b.z);
+            st[k].w = fmaf(st[k].w, e.w, dx * b.w);
+            v[k] = group_sum<LANES>(fmaf(st[k].x, c.x, st[k].y * c.y) + fmaf(st[k].z, c.z, st[k].w * c.w));
+        }
+#pragma unroll
+        for (int k = 0; k < STEP_ROWS; k++) {
+            if (lane == k % LANES) y[t * per + k] = v[k];
+        }
+    }
+    if (!on) return;
+#pragma unroll
+    for (int k = 0; k < STEP_ROWS; k++) *(float4 *) (L.s_out + (int64_t) L.N * (r0 + k) + n) = st[k];
+}
+
+bool rows16(const void * p, int64_t a, int64_t b, int64_t c) { return (uintptr_t) p % 16 == 0 && a % 4 == 0 && b % 4 == 0 && c % 4 == 0; }
+
+bool step_takes(const ssm_scan_launch & L) {
+    return L.N % 4 == 0 && ((int64_t) L.H / L.G * L.P) % STEP_ROWS == 0 && rows16(L.s, L.s_p, L.s_h, L.s_row) && rows16(L.B, L.b_g, L.b_t, L.b_s) &&
+           rows16(L.C, L.c_g, L.c_t, L.c_s) && (uintptr_t) L.s_out % 16 == 0;
+}
+
+template <int LANES>
+void launch_step(const ssm_scan_launch & L, hipStream_t st) {
+    const int64_t groups = (int64_t) L.P * L.H * L.S / STEP_ROWS, per = 256 / LANES;
+    const dim3 grid((unsigned) ((groups + per - 1) / per));
+    if (L.P % STEP_ROWS == 0) launch(ssm_scan_step_kernel<LANES, true>, grid, dim3(256), 0, st, L, groups);
+    else launch(ssm_scan_step_kernel<LANES, false>, grid, dim3(256), 0, st, L, groups);
+}
+
+// Heads of one channel over many tokens: a lane per channel with all of its N states in registers, so that no
+// sum crosses lanes and B and C, the same for the wave's 64 channels, are scalar operands. Every state takes
+// an exponential and four more operations per token, which bounds it: 16 states at 4 + 4 cycles. The tokens are
+// split into segments, since channels alone are too few waves: `local` finds each segment's final state from
+// nothing and its sum of time steps, `join` the state that each begins with, and the last launch the outputs.
+// The first pass repeats 7/8 of the work; carrying its outputs over would take as many exponentials again.
+struct chan_plan {
+    ssm_scan_launch L;
+    float * part;          // [S, n_seg, N, H]: segments' states, then what each begins with
+    float * sums;          // [S, n_seg, H]
+    int     seg, n_seg;    // tokens per segment, segments
+};
+
+typedef const __attribute__((address_space(4))) float * scalar_ptr;
+
+template <int N, bool OUT>
+__global__ __launch_bounds__(64) void ssm_scan_channels_kernel(chan_plan P) {
+    const ssm_scan_launch & L = P.L;
+    const int h = blockIdx.x * 64 + threadIdx.x, hc = min(h, L.H - 1), sg = blockIdx.y;
+    const int64_t s = blockIdx.z;
+    const int g = (int) (blockIdx.x * 64) / (L.H / L.G);
+    const int64_t t0 = (int64_t) sg * P.seg, t1 = min(L.T, t0 + P.seg);
+    float a[N], st[N];
+    const float * A = L.A + hc * L.a_h;
+#pragma unroll
+    for (int n = 0; n < N; n++) a[n] = A[L.a_scalar ? 0 : n] * LOG2E;
+    if (OUT) {
+        if (P.n_seg == 1) {
+            const float * s0 = L.s + hc * L.s_h + pool_row(L, s) * L.s_row;
+#pragma unroll
+            for (int n = 0; n < N; n++) st[n] = s0[n];
+        } else {
+            const float * q = P.part + ((s * P.n_seg + sg) * N) * L.H + hc;
+#pragma unroll
+            for (int n = 0; n < N; n++) st[n] = q[(int64_t) n * L.H];
+        }
+    } else {
+#pragma unroll
+        for (int n = 0; n < N; n++) st[n] = 0.0f;
+    }
+    const float * x = L.x + hc * L.x_h + s * L.x_s + t0 * L.x_t, * dt = L.dt + hc + s * L.dt_s + t0 * L.dt_t;
+    scalar_ptr B = (scalar_ptr) (uintptr_t) (L.B + g * L.b_g + s * L.b_s + t0 * L.b_t);
+    scalar_ptr C = (scalar_ptr) (uintptr_t) (L.C + g * L.c_g + s * L.c_s + t0 * L.c_t);
+    float * y = L.y + hc + (int64_t) L.H * (t0 + L.T * s);
+    float sum = 0.0f;
+    // the next token's inputs are on their way while this one is computed
+    float xn = x[0], dn = dt[0];
+    for (int64_t t = t0; t < t1; t++) {
+        const float xt = xn, raw = dn;
+        if (t + 1 < t1) {
+            x += L.x_t;
+            dt += L.dt_t;
+        }
+        xn = *x;
+        dn = *dt;
+        const float d = softplus(raw), dx = d * xt;
+        float v = 0.0f;
+#pragma unroll
+        for (int n = 0; n < N; n++) {
+            st[n] = fmaf(st[n], exp2_hw(d * a[n]), dx * B[n]);
+            if (OUT) v = fmaf(st[n], C[n], v);
+        }
+        sum += d;
+        if (OUT) {
+            if (h < L.H) *y = v;
+            y += L.H;
+            C += L.c_t;
+        }
+        B += L.b_t;
+    }
+    if (h >= L.H) return;
+    if (OUT) {
+        if (sg != P.n_seg - 1) return;
+        float * so = L.s_out + (int64_t) N * (h + (int64_t) L.H * s);
+#pragma unroll
+        for (int n = 0; n < N; n++) so[n] = st[n];
+    } else {
+        float * q = P.part + ((s * P.n_seg + sg) * N) * L.H + h;
+#pragma unroll
+        for (int n = 0; n < N; n++) q[(int64_t) n * L.H] = st[n];
+        P.sums[(s * P.n_seg + sg) * L.H + h] = sum;
+    }
+}
+
+// a thread per channel and state: the segments in order
+__global__ __launch_bounds__(256) void ssm_scan_join_kernel(chan_plan P) {
+    const ssm_scan_launch & L = P.L;
+    const int h = blockIdx.x * 256 + threadIdx.x, n = blockIdx.y;
+    const int64_t s = blockIdx.z;
+    if (h >= L.H) return;
+    const float a = L.A[h * L.a_h + (L.a_scalar ? 0 : n)] * LOG2E;
+    float st = L.s[n + h * L.s_h + pool_row(L, s) * L.s_row];
+    float * q = P.part + (s * P.n_seg * L.N + n) * L.H + h;
+    const float * sum = P.sums + s * P.n_seg * L.H + h;
+    const int64_t step = (int64_t) L.N * L.H;
+#pragma unroll 8
+    for (int k = 0; k < P.n_seg; k++) {
+        const float own = q[k * step], e = exp2_hw(sum[(int64_t) k * L.H] * a);
+        q[k * step] = st;
+        st = fmaf(st, e, own);
+    }
+}
+
+bool channels_take(const ssm_scan_launch & L) {
+    return L.P == 1 && (L.N == 8 || L.N == 16 || L.N == 32) && L.T > SSM_STEP_TOKENS && (L.G == 1 || L.H / L.G % 64 == 0) && L.S <= 65535;
+}
+
+// Segments for four waves of every SIMD, of 32 tokens at least and 4096 segments at most.
+void chan_segments(const ssm_scan_launch & L, chan_plan & P) {
+    const int64_t waves = (L.H + 63) / 64 * L.S, want = (4096 + waves - 1) / waves;
+    const int64_t n = std::max<int64_t>(1, std::min<int64_t>({ want, L.T / 32, 4096 }));
+    P.seg = (int) ((L.T + n - 1) / n);
+    P.n_seg = (int) ((L.T + P.seg - 1) / P.seg);
+}
+
+template <int N>
+void launch_channels(const chan_plan & P, hipStream_t st) {
+    const ssm_scan_launch & L = P.L;
+    const unsigned hx = (unsigned) ((L.H + 63) / 64);
+    if (P.n_seg > 1) {
+        launch(ssm_scan_channels_kernel<N, false>, dim3(hx, (unsigned) P.n_seg - 1, (unsigned) L.S), dim3(64), 0, st, P);
+        launch(ssm_scan_join_kernel, dim3((unsigned) ((L.H + 255) / 256), (unsigned) N, (unsigned) L.S), dim3(256), 0, st, P);
+    }
+    launch(ssm_scan_channels_kernel<N, true>, dim3(hx, (unsigned) P.n_seg, (unsigned) L.S), dim3(64), 0, st, P);
+}
+
 } // namespace
 
 void launch_ssm_conv(const ssm_conv_launch & L, hipStream_t st) {
@@ -297,8 +504,38 @@ void launch_ssm_conv(const ssm_conv_launch & L, hipStream_t st) {
            L, blocks);
 }
 
-void launch_ssm_scan(const ssm_scan_launch & L, hipStream_t st) {
+int64_t ssm_scan_scratch_bytes(const ssm_scan_launch & L) {
+    if (!channels_take(L)) return ssm_scan_mm_takes(L) ? ssm_scan_mm_scratch_bytes(L) : 0;
+    chan_plan P{};
+    chan_segments(L, P);
+    return P.n_seg == 1 ? 0 : L.S * P.n_seg * (int64_t) L.H * (L.N + 1) * 4;
+}
+
+void launch_ssm_scan(const ssm_scan_launch & L, void * ws, hipStream_t st) {
     if ((int64_t) L.P * L.H * L.S == 0) return;
+    if (channels_take(L)) {
+        chan_plan P{};
+        P.L = L;
+        chan_segments(L, P);
+        P.part = (float *) ws;
+        P.sums = P.part + L.S * P.n_seg * (int64_t) L.H * L.N;
+        if (L.N == 8) launch_channels<8>(P, st);
+        else if (L.N == 16) launch_channels<16>(P, st);
+        else launch_channels<32>(P, st);
+        return;
+    }
+    if (ssm_scan_mm_takes(L)) {
+        launch_ssm_scan_mm(L, ws, st);
+        return;
+    }
+    if (step_takes(L)) {
+        if (L.N <= 16) launch_step<4>(L, st);
+        else if (L.N <= 32) launch_step<8>(L, st);
+        else if (L.N <= 64) launch_step<16>(L, st);
+        else if (L.N <= 128) launch_step<32>(L, st);
+        else launch_step<64>(L, st);
+        return;
+    }
     if (L.N <= 16) launch_rows<16, 1>(L, st);
     else if (L.N <= 32) launch_rows<32, 1>(L, st);
     else if (L.N <= 64) launch_rows<64, 1>(L, st);

@@ -28,6 +28,7 @@
 // and dt enter rows and columns of their own only.)
 #include "hip_common.h"
 #include "kernels.h"
+#include "ssm_ops.h"
 
 #include <algorithm>
 
@@ -42,9 +43,6 @@ typedef uint32_t uint4v __attribute__((ext_vector_type(4)));
 constexpr int Q = 64;                        // tokens per chunk
 constexpr int STEP_WORDS = 5 * Q;            // exp(c), exp(c_63 - c), d, c as two floats
 constexpr int M_BYTES = 6 * 1024;            // one plane of a head's 64 x 64 lower triangle, in 16 x 32 blocks
-constexpr float LN2 = 0.6931471805599453f;
-
-__device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // the power of two that takes a largest magnitude to 2^12 .. 2^13, and its inverse
 __device__ __forceinline__ float scale_of(float most) {
@@ -69,9 +67,6 @@ __device__ __forceinline__ float4v mfma(half8 a, half8 b, float4v c) { return __
 __device__ __forceinline__ float4v mfma3(half8 ah, half8 al, half8 bh, half8 bl, float4v c) {
     return mfma(ah, bh, mfma(ah, bl, mfma(al, bh, c)));
 }
-
-// log(1 + e^x); above 20 the sum rounds to e^x, so x itself (the unary op's rule)
-__device__ __forceinline__ float softplus(float x) { return x > 20.0f ? x : log1pf(expf(x)); }
 
 // what the launches share; offsets into the scratch in bytes
 struct mm_plan {
@@ -726,11 +721,11 @@ mm_sizes mm_size(const ssm_scan_launch & L) {
     const int64_t rec = (int64_t) z.nk * 16384 + Q * Q * 4 + 16, per = L.S * (L.G * rec + (int64_t) L.H * STEP_WORDS * 4);
     // prepared operands of at most 64 MiB: the tokens go through in blocks
     z.block = std::max<int64_t>(1, std::min<int64_t>({ z.chunks, ((int64_t) 64 << 20) / per, 65535 }));
-    // segments until every CU has a workgroup
+    // segments until every CU has a workgroup, of one chunk if need be (333 tokens of 24 heads: 41 us with two
+    // chunks at least, 37 with one)
     const int64_t base = L.S * L.G * z.head_blocks * z.p_blocks;
     const int64_t part = L.S * L.H * (int64_t) z.slices * (2 * z.nk * WAVE * 16) + L.S * L.H * 4;
-    static const int segmin = getenv("SEGMIN") ? atoi(getenv("SEGMIN")) : 2;
-    z.n_seg = std::max<int64_t>(1, std::min<int64_t>({ 256 / base, z.block / segmin, ((int64_t) 32 << 20) / part }));
+    z.n_seg = std::max<int64_t>(1, std::min<int64_t>({ 256 / base, z.block, ((int64_t) 32 << 20) / part }));
     z.seg = (z.block + z.n_seg - 1) / z.n_seg;
     z.n_seg = (z.block + z.seg - 1) / z.seg;
     int64_t at = 0;
@@ -793,7 +788,7 @@ void launch_mm(const ssm_scan_launch & L, const mm_sizes & z, void * ws, hipStre
 
 bool ssm_scan_mm_takes(const ssm_scan_launch & L) {
     // the grids' limits: one dimension each for the sequences and for groups and heads
-    return L.a_scalar && L.T >= SSM_MM_MIN_TOKENS && L.S <= 65535 && L.G <= 65535 && L.H <= 16 * 65535 &&
+    return L.a_scalar && L.T > SSM_STEP_TOKENS && L.S <= 65535 && L.G <= 65535 && L.H <= 16 * 65535 &&
            L.S * (int64_t) L.H * L.P < INT32_MAX &&
            // 32-bit offsets within a chunk
            L.x_t >= 0 && L.x_t <= 1 << 24 && (int64_t) L.H * L.P <= 1 << 24 && L.P <= 1 << 24;

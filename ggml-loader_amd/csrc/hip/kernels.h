@@ -590,9 +590,11 @@ struct ssm_scan_launch {
     int             N, P, H, G;
     int             a_scalar;      // one A per head
 };
-void launch_ssm_scan(const ssm_scan_launch & L, hipStream_t st);
-// the same over many tokens with one A per head, as matrix products (k_ssm_mm.hip); ws: 256-byte aligned scratch
-constexpr int SSM_MM_MIN_TOKENS = 16;
+constexpr int SSM_STEP_TOKENS = 16;    // up to so many tokens the states are what a step reads and writes
+// ws: 256-byte aligned scratch of ssm_scan_scratch_bytes (0: none)
+int64_t ssm_scan_scratch_bytes(const ssm_scan_launch & L);
+void launch_ssm_scan(const ssm_scan_launch & L, void * ws, hipStream_t st);
+// over many tokens with one A per head: matrix products (k_ssm_mm.hip)
 bool ssm_scan_mm_takes(const ssm_scan_launch & L);
 int64_t ssm_scan_mm_scratch_bytes(const ssm_scan_launch & L);
 void launch_ssm_scan_mm(const ssm_scan_launch & L, void * ws, hipStream_t st);

@@ -68,7 +68,8 @@ SCANS = [
     (1, 200, 40, 32, 64, 8, 1, 1), (1, 2000, 3, 48, 128, 1, 1, 1), (1, 90, 1, 33, 100, 1, 1, 1), (1, 70, 2, 48, 200, 1, 1, 1), (5, 7, 3, 64, 128, 3, 9, 1), (1, 1100, 2, 64, 128, 1, 1, 1),
     # a decay per state: a head per channel, and heads of several channels
     (1, 1, 300, 1, 16, 1, 1, 16), (2, 50, 130, 1, 16, 1, 3, 16), (1, 257, 67, 1, 8, 1, 1, 8), (3, 3, 65, 1, 32, 1, 3, 32),
-    (1, 40, 6, 1, 5, 2, 1, 5), (1, 33, 3, 4, 16, 1, 2, 16), (1, 25, 2, 2, 129, 2, 1, 129), (1, 1030, 64, 1, 16, 1, 1, 16),
+    (2, 100, 128, 1, 16, 2, 2, 16), (1, 40, 70, 1, 16, 1, 1, 1), (1, 17, 64, 1, 32, 1, 1, 32), (1, 9, 12, 1, 8, 3, 1, 8),
+    (2, 16, 5, 4, 4, 1, 2, 1), (3, 2, 8, 8, 256, 2, 3, 256), (1, 5, 4, 2, 64, 2, 1, 1), (1, 40, 6, 1, 5, 2, 1, 5), (1, 33, 3, 4, 16, 1, 2, 16), (1, 25, 2, 2, 129, 2, 1, 129), (1, 1030, 64, 1, 16, 1, 1, 16),
 ]
 
 
