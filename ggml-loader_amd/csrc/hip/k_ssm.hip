@@ -404,31 +404,46 @@ __global__ __launch_bounds__(64) void ssm_scan_channels_kernel(chan_plan P) {
     scalar_ptr C = (scalar_ptr) (uintptr_t) (L.C + g * L.c_g + s * L.c_s + t0 * L.c_t);
     float * y = L.y + hc + (int64_t) L.H * (t0 + L.T * s);
     float sum = 0.0f;
-    // the next token's inputs are on their way while this one is computed
-    float xn = x[0], dn = dt[0];
-    for (int64_t t = t0; t < t1; t++) {
-        const float xt = xn, raw = dn;
-        if (t + 1 < t1) {
-            x += L.x_t;
-            dt += L.dt_t;
-        }
-        xn = *x;
-        dn = *dt;
+    auto token = [&](float raw, float xt) {
         const float d = softplus(raw), dx = d * xt;
         float v = 0.0f;
 #pragma unroll
         for (int n = 0; n < N; n++) {
-            st[n] = fmaf(st[n], exp2_hw(d * a[n]), dx * B[n]);
+            st[n] = fmaf(dx, B[n], st[n] * exp2_hw(d * a[n]));
             if (OUT) v = fmaf(st[n], C[n], v);
         }
         sum += d;
         if (OUT) {
-            if (h < L.H) *y = v;
+            *y = v;                                            // lanes past the last channel store its value again
             y += L.H;
             C += L.c_t;
         }
         B += L.b_t;
+    };
+    // four tokens at a time, the next four's inputs on their way (past the segment, its last token's)
+    float xn[4], dn[4];
+    auto fetch = [&](int64_t t) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int64_t k = min(t + i, t1 - 1) - t0;
+            xn[i] = x[k * L.x_t];
+            dn[i] = dt[k * L.dt_t];
+        }
+    };
+    fetch(t0);
+    int64_t t = t0;
+    for (; t + 4 <= t1; t += 4) {
+        float xt[4], raw[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            xt[i] = xn[i];
+            raw[i] = dn[i];
+        }
+        fetch(t + 4);
+#pragma unroll
+        for (int i = 0; i < 4; i++) token(raw[i], xt[i]);
     }
+    for (int i = 0; t + i < t1; i++) token(i == 0 ? dn[0] : i == 1 ? dn[1] : dn[2], i == 0 ? xn[0] : i == 1 ? xn[1] : xn[2]);
     if (h >= L.H) return;
     if (OUT) {
         if (sg != P.n_seg - 1) return;
@@ -454,11 +469,20 @@ __global__ __launch_bounds__(256) void ssm_scan_join_kernel(chan_plan P) {
     float * q = P.part + (s * P.n_seg * L.N + n) * L.H + h;
     const float * sum = P.sums + s * P.n_seg * L.H + h;
     const int64_t step = (int64_t) L.N * L.H;
-#pragma unroll 8
-    for (int k = 0; k < P.n_seg; k++) {
-        const float own = q[k * step], e = exp2_hw(sum[(int64_t) k * L.H] * a);
-        q[k * step] = st;
-        st = fmaf(st, e, own);
+    // sixteen segments' loads in flight
+    for (int k0 = 0; k0 < P.n_seg; k0 += 16) {
+        float own[16], d[16];
+#pragma unroll
+        for (int k = 0; k < 16; k++) {
+            const int64_t c = min(k0 + k, P.n_seg - 1);
+            own[k] = q[c * step];
+            d[k] = sum[c * L.H];
+        }
+#pragma unroll
+        for (int k = 0; k < 16; k++) {
+            if (k0 + k < P.n_seg) q[(k0 + k) * step] = st;
+            st = fmaf(st, exp2_hw(d[k] * a), own[k]);
+        }
     }
 }
 
