@@ -41,7 +41,11 @@ typedef float float4v __attribute__((ext_vector_type(4)));
 typedef uint32_t uint4v __attribute__((ext_vector_type(4)));
 
 constexpr int Q = 64;                        // tokens per chunk
-constexpr int STEP_WORDS = 5 * Q;            // exp(c), exp(c_63 - c), d, c as two floats
+// exp(c), exp(c_63 - c), d, c as two floats, exp(c at the end of its 16 tokens - c)
+constexpr int STEP_WORDS = 6 * Q;
+// C_t . B_j of a chunk: ten tiles of 16 x 16, the diagonal's and then, row by row, those below it, each as the
+// matrices' lanes load it: two parts of 32 lanes (row + 16 (column / 8)) by four columns
+constexpr int G_WORDS = 10 * 256;
 constexpr int M_BYTES = 6 * 1024;            // one plane of a head's 64 x 64 lower triangle, in 16 x 32 blocks
 
 // the power of two that takes a largest magnitude to 2^12 .. 2^13, and its inverse
@@ -52,13 +56,14 @@ __device__ __forceinline__ float scale_of(float most) {
 __device__ __forceinline__ float inverse_of(float scale) { return __uint_as_float((254u - (__float_as_uint(scale) >> 23)) << 23); }
 __device__ __forceinline__ float finite_abs(float x) { return fabsf(x) < INFINITY ? fabsf(x) : 0.0f; }
 
-// eight scaled values as hi + lo
-__device__ __forceinline__ void split8(const float (&v)[8], half8 & hi, half8 & lo) {
+// eight values times a power of two as hi + lo. The product is exact, so hi comes from one mixed-precision
+// multiply-add and the rest from another: two and a half operations a value.
+__device__ __forceinline__ void split8(const float (&v)[8], float scale, half8 & hi, half8 & lo) {
 #pragma unroll
     for (int i = 0; i < 8; i += 2) {
-        const half2v h = __builtin_convertvector(float2v{ v[i], v[i + 1] }, half2v);
-        const half2v l = __builtin_convertvector(float2v{ fmaf((float) h[0], -1.0f, v[i]), fmaf((float) h[1], -1.0f, v[i + 1]) }, half2v);
-        hi[i] = h[0]; hi[i + 1] = h[1];
+        const _Float16 h0 = (_Float16) fmaf(v[i], scale, 0.0f), h1 = (_Float16) fmaf(v[i + 1], scale, 0.0f);
+        const half2v l = __builtin_convertvector(float2v{ fmaf(v[i], scale, -(float) h0), fmaf(v[i + 1], scale, -(float) h1) }, half2v);
+        hi[i] = h0; hi[i + 1] = h1;
         lo[i] = l[0]; lo[i + 1] = l[1];
     }
 }
@@ -105,10 +110,8 @@ __device__ __forceinline__ void load_perm(const float * row, int n, int N, bool 
 }
 
 template <int NK>
-__global__ __launch_bounds__(256) void ssm_operands_kernel(mm_plan P) {
-    extern __shared__ __align__(16) char lds[];                // B's planes: blocks of 16 tokens by 32 states
-    const ssm_scan_launch & L = P.L;
-    const int c = blockIdx.x, g = blockIdx.y, s = blockIdx.z;
+__device__ __forceinline__ void prepare_operands(const mm_plan & P, int c, int g, int s, char * lds) {
+    const ssm_scan_launch & L = P.L;                           // lds: B's planes, blocks of 16 tokens by 32 states
     const int tid = threadIdx.x, lane = tid % WAVE, wave = __builtin_amdgcn_readfirstlane(tid / WAVE);
     const int left = P.T - c * Q;             // tokens from the chunk's first on
     constexpr int PLANE = 4 * 1024 * NK;
@@ -149,9 +152,7 @@ __global__ __launch_bounds__(256) void ssm_operands_kernel(mm_plan P) {
         for (int q = 0; q < NK; q++) {
             half8 hi, lo;
             const int at = ((wave * NK + q) * 64 + lane) * 16;
-#pragma unroll
-            for (int i = 0; i < 8; i++) v[o][q][i] = as_f32(v[o][q][i] * sc);
-            split8(v[o][q], hi, lo);
+            split8(v[o][q], sc, hi, lo);
             if (o == 0) {
                 ch[q] = hi;
                 cl[q] = lo;
@@ -165,7 +166,8 @@ __global__ __launch_bounds__(256) void ssm_operands_kernel(mm_plan P) {
     }
     __syncthreads();
     // C_t . B_j of the wave's tokens, up to the diagonal
-    float * G = (float *) (P.ws + P.gmat) + rec * Q * Q + (16 * wave + 4 * (lane / 16)) * Q + lane % 16;
+    const int gcol = lane % 16;
+    float * G = (float *) (P.ws + P.gmat) + rec * G_WORDS + (gcol % 8 / 4) * 128 + (gcol / 8 * 16 + 4 * (lane / 16)) * 4 + gcol % 4;
     float top = 0.0f;
     for (int jt = 0; jt <= wave; jt++) {
         float4v acc = { 0, 0, 0, 0 };
@@ -177,7 +179,7 @@ __global__ __launch_bounds__(256) void ssm_operands_kernel(mm_plan P) {
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const float w = acc[i] * inv[0] * inv[1];
-            G[i * Q + 16 * jt] = w;
+            G[(jt == wave ? wave : 4 + wave * (wave - 1) / 2 + jt) * 256 + 4 * i] = w;
             top = fmaxf(top, finite_abs(w));
         }
     }
@@ -211,10 +213,8 @@ __global__ __launch_bounds__(256) void ssm_operands_kernel(mm_plan P) {
 }
 
 // 16 heads' running sums over a chunk: a wave per four heads, a lane per token
-__global__ __launch_bounds__(256) void ssm_steps_kernel(mm_plan P) {
-    __shared__ float lds[Q * 17];
+__device__ __forceinline__ void prepare_steps(const mm_plan & P, int c, int h0, int s, float * lds) {
     const ssm_scan_launch & L = P.L;
-    const int c = blockIdx.x, h0 = blockIdx.y * 16, s = blockIdx.z;
     const int tid = threadIdx.x, lane = tid % WAVE, wave = __builtin_amdgcn_readfirstlane(tid / WAVE), left = P.T - c * Q;
 #pragma unroll
     for (int i = 0; i < 4; i++) {
@@ -244,10 +244,12 @@ __global__ __launch_bounds__(256) void ssm_steps_kernel(mm_plan P) {
 #pragma unroll
     for (int k = 0; k < 4; k++) {
         const int h = h0 + 4 * wave + k;
+        const double tile = __shfl(sum[k], lane | 15, WAVE) - sum[k];
         const double rest = __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(sum[k]), 63),
                                              __builtin_amdgcn_readlane(__double2loint(sum[k]), 63)) - sum[k];
         const float hi = (float) sum[k], lo = fabsf(hi) < INFINITY ? (float) (sum[k] - (double) hi) : 0.0f;
         const float rh = (float) rest, rl = fabsf(rh) < INFINITY ? (float) (rest - (double) rh) : 0.0f;
+        const float th = (float) tile, tl = fabsf(th) < INFINITY ? (float) (tile - (double) th) : 0.0f;
         if (h >= L.H) break;
         float * o = (float *) (P.ws + P.steps) + (((int64_t) s * P.nc + c) * L.H + h) * STEP_WORDS + lane;
         o[0] = exp2_hw(hi) * fmaf(lo, LN2, 1.0f);
@@ -255,7 +257,16 @@ __global__ __launch_bounds__(256) void ssm_steps_kernel(mm_plan P) {
         o[2 * Q] = d[k];
         o[3 * Q] = hi;
         o[4 * Q] = lo;
+        o[5 * Q] = exp2_hw(th) * fmaf(tl, LN2, 1.0f);
     }
+}
+
+template <int NK>
+__global__ __launch_bounds__(256) void ssm_prepare_kernel(mm_plan P) {
+    extern __shared__ __align__(16) char lds[];
+    const int y = blockIdx.y;
+    if (y < P.L.G) prepare_operands<NK>(P, blockIdx.x, y, blockIdx.z, lds);
+    else prepare_steps(P, blockIdx.x, (y - P.L.G) * 16, blockIdx.z, (float *) lds);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -346,65 +357,122 @@ __global__ __launch_bounds__(THREADS, 2) void ssm_scan_mm_kernel(mm_plan P) {
                 for (int i = 0; i < 4; i++) S[nt][i] = n + i < L.N ? s0[n + i] : 0.0f;
             }
         }
-        for (int k = 0; k < sg; k++) {
-            const float dec = ((const float *) (P.ws + P.decays))[((int64_t) s * P.n_seg + k) * L.H + h];
-            const float4v * q = part_at(k);
+        // two segments' loads in flight
+        for (int k = 0; k < sg; k += 2) {
+            const int k1 = min(k + 1, sg - 1);
+            const float * dp = (const float *) (P.ws + P.decays) + (int64_t) s * P.n_seg * L.H + h;
+            const float d0 = dp[(int64_t) k * L.H], d1 = dp[(int64_t) k1 * L.H];
+            const float4v * q0 = part_at(k), * q1 = part_at(k1);
+            float4v f0[2 * NK], f1[2 * NK];
 #pragma unroll
             for (int nt = 0; nt < 2 * NK; nt++) {
-                const float4v f = q[nt * WAVE];
+                f0[nt] = q0[nt * WAVE];
+                f1[nt] = q1[nt * WAVE];
+            }
 #pragma unroll
-                for (int i = 0; i < 4; i++) S[nt][i] = fmaf(S[nt][i], dec, f[i]);
+            for (int nt = 0; nt < 2 * NK; nt++) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) S[nt][i] = fmaf(S[nt][i], d0, f0[nt][i]);
+            }
+            if (k + 1 < sg) {
+#pragma unroll
+                for (int nt = 0; nt < 2 * NK; nt++) {
+#pragma unroll
+                    for (int i = 0; i < 4; i++) S[nt][i] = fmaf(S[nt][i], d1, f1[nt][i]);
+                }
             }
         }
     }
 
     // what the next chunk reads
     uint4v stage_c[OUT ? STAGE : 1], stage_b[STAGE];
-    float x[2][8], gg[2][8], sc_next[3], st_next[(4 * STEP_WORDS + THREADS - 1) / THREADS];
-    // thread's part of a head's matrix: row mt, columns 8 mj .. + 7 and, in the lower half, 32 further on
-    const int mt = tid % 256 / 4, mj = tid % 4;
+    float4 gg[2][2];
+    float x[2][8], sc_next[3], st_next[(4 * STEP_WORDS + THREADS - 1) / THREADS];
+    // The matrices' tiles of 16 x 16, two per wave and turn: a head has four on the diagonal, which need an
+    // exponential per element, and six below it, where exp(c_t - c_j) is exp(c_t - c_b) exp(c_b - c_j), b the last
+    // of the tile's columns: one exponential per row beside prepared ones. A turn is (head, pair of tiles); the
+    // diagonal ones come first, and a second turn goes to the waves that had the cheaper first.
+    const int turns = 5 * heads;
+    struct tile_place { int k, tt, jt; };
+    auto place = [&](int turn) {
+        tile_place w;
+        if (turn < 2 * heads) {
+            w.k = turn / 2;
+            w.tt = w.jt = turn % 2 * 2 + lane / 32;
+        } else {
+            const int q = turn - 2 * heads, i = q % 3 * 2 + lane / 32;
+            w.k = q / 3;
+            w.tt = i < 1 ? 1 : i < 3 ? 2 : 3;
+            w.jt = i < 1 ? 0 : i < 3 ? i - 1 : i - 3;
+        }
+        return w;
+    };
+    auto turn_of = [&](int r) { return WAVES * r + (wave + WAVES / 2 * r) % WAVES; };
+    // the lane's row of a tile and its eight columns
+    const int tr = lane % 16, th = lane / 16 % 2;
+    auto load_g = [&](const char * G, int turn, float4 (&v)[2]) {
+        const int pair = turn < 2 * heads ? turn % 2 : 2 + (turn - 2 * heads) % 3;
+        const uint32_t at = here(lane / 32 * 1024 + lane % 32 * 16);
+        v[0] = *(const float4 *) (G + pair * 2048 + at);
+        v[1] = *(const float4 *) (G + pair * 2048 + 512 + at);
+    };
+    if (OUT) {
+        // the tiles above the diagonal that the products read: blocks 0 and 3, columns 16 to 31
+        for (int i = tid; i < heads * 2 * 2 * 32; i += THREADS)
+            *(uint4v *) (mats + i / 64 * M_BYTES + (i / 32 % 2 ? 3 : 0) * 1024 + (32 + i % 32) * 16) = uint4v{ 0, 0, 0, 0 };
+    }
+    // where the next chunk's are, and how far on each lies in the chunk after
+    const char * at_planes, * at_steps, * at_scales, * at_g, * at_x;
+    {
+        const int64_t rec = ((int64_t) s * P.nc + c0) * L.G + g;
+        at_planes = P.ws + P.planes + rec * rec_bytes<NK>();
+        at_scales = P.ws + P.scales + rec * 16;
+        at_g = P.ws + P.gmat + rec * (G_WORDS * 4);
+        at_steps = P.ws + P.steps + (((int64_t) s * P.nc + c0) * L.H + g * per + hb) * (STEP_WORDS * 4);
+        at_x = (const char *) (L.x + h * L.x_h + s * L.x_s + (P.t0 + c0 * Q) * L.x_t);
+    }
+    const int64_t x_on = Q * 4 * L.x_t, steps_on = (int64_t) L.H * (STEP_WORDS * 4);
     auto fetch = [&](int c) {
-        const int64_t rec = ((int64_t) s * P.nc + c) * L.G + g;
         const int left = P.T - c * Q;
-        const char * src = P.ws + P.planes + rec * rec_bytes<NK>() + tid * 16;
+        const uint32_t piece = here(tid * 16);
 #pragma unroll
         for (int q = 0; q < STAGE; q++) {
-            if (OUT) stage_c[q] = *(const uint4v *) (src + q * THREADS * 16);
-            stage_b[q] = *(const uint4v *) (src + OPERAND + q * THREADS * 16);
+            if (OUT) stage_c[q] = *(const uint4v *) (at_planes + q * THREADS * 16 + piece);
+            stage_b[q] = *(const uint4v *) (at_planes + OPERAND + q * THREADS * 16 + piece);
         }
-        const float * sp = (const float *) (P.ws + P.steps) + (((int64_t) s * P.nc + c) * L.H + g * per + hb) * STEP_WORDS;
 #pragma unroll
-        for (int q = 0; q < (4 * STEP_WORDS + THREADS - 1) / THREADS; q++) st_next[q] = sp[min(tid + q * THREADS, heads * STEP_WORDS - 1)];
-        const float * sc = (const float *) (P.ws + P.scales) + rec * 4;
+        for (int q = 0; q < (4 * STEP_WORDS + THREADS - 1) / THREADS; q++)
+            st_next[q] = *(const float *) (at_steps + 4 * (uint32_t) min(tid + q * THREADS, heads * STEP_WORDS - 1));
 #pragma unroll
-        for (int i = 0; i < 3; i++) sc_next[i] = sc[i];
+        for (int i = 0; i < 3; i++) sc_next[i] = ((const float *) at_scales)[i];
         if (OUT) {
-            const float * G = (const float *) (P.ws + P.gmat) + rec * Q * Q + mt * Q + 8 * mj;
 #pragma unroll
-            for (int q = 0; q < 2; q++) {
-                const float4 a = *(const float4 *) (G + 32 * q), b = *(const float4 *) (G + 32 * q + 4);
-                gg[q][0] = a.x; gg[q][1] = a.y; gg[q][2] = a.z; gg[q][3] = a.w;
-                gg[q][4] = b.x; gg[q][5] = b.y; gg[q][6] = b.z; gg[q][7] = b.w;
+            for (int r = 0; r < 2; r++) {
+                if (turn_of(r) < turns) load_g(at_g, turn_of(r), gg[r]);
             }
         }
         // token 32 ks + 8 grp + i of the wave's channels; past the last token it is the last again, and cleared
-        const char * xp = (const char *) (L.x + h * L.x_h + s * L.x_s + (P.t0 + c * Q) * L.x_t);
         const uint32_t row = 4 * (uint32_t) L.x_t;
         if (left >= Q) {
             uint32_t at = here(8 * grp * row + 4 * (uint32_t) pch);
 #pragma unroll
             for (int ks = 0; ks < 2; ks++) {
 #pragma unroll
-                for (int i = 0; i < 8; i++, at += row) x[ks][i] = *(const float *) (xp + at);
+                for (int i = 0; i < 8; i++, at += row) x[ks][i] = *(const float *) (at_x + at);
                 at += 24 * row;
             }
         } else {
 #pragma unroll
             for (int ks = 0; ks < 2; ks++) {
 #pragma unroll
-                for (int i = 0; i < 8; i++) x[ks][i] = *(const float *) (xp + (min(32 * ks + 8 * grp + i, left - 1) * row + 4 * (uint32_t) pch));
+                for (int i = 0; i < 8; i++) x[ks][i] = *(const float *) (at_x + (min(32 * ks + 8 * grp + i, left - 1) * row + 4 * (uint32_t) pch));
             }
         }
+        at_planes += L.G * rec_bytes<NK>();
+        at_scales += L.G * 16;
+        at_g += L.G * (G_WORDS * 4);
+        at_steps += steps_on;
+        at_x += x_on;
     };
     // and on to LDS
     auto put = [&](int turn) {
@@ -433,80 +501,70 @@ __global__ __launch_bounds__(THREADS, 2) void ssm_scan_mm_kernel(mm_plan P) {
         const float e_last = my[Q - 1];
         if (OUT) {
             // (C_t . B_j) exp(c_t - c_j) below the diagonal, split, in the order of the A operand
-            for (int k = wave / 4; k < heads; k += WAVES / 4) {
-                const float * st = head_steps + k * STEP_WORDS;
+#pragma unroll 1
+            for (int r = 0; turn_of(r) < turns; r++) {
+                const int now = turn_of(r);
+                const tile_place w = place(now);
+                if (r == 1) {
+                    gg[0][0] = gg[1][0];
+                    gg[0][1] = gg[1][1];
+                } else if (r > 1) {
+                    load_g(P.ws + P.gmat + (((int64_t) s * P.nc + c) * L.G + g) * (G_WORDS * 4), now, gg[0]);
+                }
+                const float g8[8] = { gg[0][0].x, gg[0][0].y, gg[0][0].z, gg[0][0].w, gg[0][1].x, gg[0][1].y, gg[0][1].z, gg[0][1].w };
+                const float * st = head_steps + w.k * STEP_WORDS;
                 const float sm = scale_of(gmost * fmaxf(1.0f, st[Q - 1]));
-                const float ht = st[3 * Q + mt], lt = st[4 * Q + mt];
-                const int tt = mt / 16;
-                char * at = mats + k * 2 * M_BYTES + (mt % 16 + 16 * mj) * 16;
-#pragma unroll
-                for (int q = 0; q < 2; q++) {
-                    if (q == 1 && mt < 32) break;
-                    const int j0 = 8 * mj + 32 * q;
+                const int t = 16 * w.tt + tr, j0 = 16 * w.jt + 8 * th;
+                float v[8], scale = sm;
+                if (now < 2 * heads) {
+                    const float ht = st[3 * Q + t], lt = st[4 * Q + t];
                     const float4 h0 = *(const float4 *) (st + 3 * Q + j0), h1 = *(const float4 *) (st + 3 * Q + j0 + 4);
                     const float4 l0 = *(const float4 *) (st + 4 * Q + j0), l1 = *(const float4 *) (st + 4 * Q + j0 + 4);
                     const float hh[8] = { h0.x, h0.y, h0.z, h0.w, h1.x, h1.y, h1.z, h1.w };
                     const float ll[8] = { l0.x, l0.y, l0.z, l0.w, l1.x, l1.y, l1.z, l1.w };
-                    float v[8];
 #pragma unroll
                     for (int i = 0; i < 8; i++) {
-                        const float w = as_f32(gg[q][i] * sm * exp2_hw((ht - hh[i]) + (lt - ll[i])));
-                        v[i] = j0 + i <= mt ? w : 0.0f;
+                        const float e = g8[i] * exp2_hw((ht - hh[i]) + (lt - ll[i]));
+                        v[i] = 8 * th + i <= tr ? e : 0.0f;
                     }
-                    half8 hi, lo;
-                    split8(v, hi, lo);
-                    char * o = at + (tt < 2 ? tt : 2 * tt - 2 + q) * 1024;
-                    *(half8 *) o = hi;
-                    *(half8 *) (o + M_BYTES) = lo;
+                } else {
+                    const int b = 16 * w.jt + 15;
+                    const float row = exp2_hw((st[3 * Q + t] - st[3 * Q + b]) + (st[4 * Q + t] - st[4 * Q + b]));
+                    const float4 f0 = *(const float4 *) (st + 5 * Q + j0), f1 = *(const float4 *) (st + 5 * Q + j0 + 4);
+                    const float ff[8] = { f0.x, f0.y, f0.z, f0.w, f1.x, f1.y, f1.z, f1.w };
+#pragma unroll
+                    for (int i = 0; i < 8; i++) v[i] = g8[i] * ff[i] * row;
                 }
+                half8 hi, lo;
+                split8(v, scale, hi, lo);
+                char * o = mats + w.k * 2 * M_BYTES + (w.tt < 2 ? w.tt : 2 * w.tt - 2 + w.jt / 2) * 1024 + (tr + 16 * (w.jt % 2 * 2 + th)) * 16;
+                *(half8 *) o = hi;
+                *(half8 *) (o + M_BYTES) = lo;
             }
         }
-        // X = d x, cleared of tokens past the last and of values that are not finite
-        int bad = Q;                                           // the channel's first token with such a value
-        bool odd_chunk;
+        // X = d x, cleared of tokens past the last
         float most = 0.0f;
-        {
-            float odd = 0.0f;
 #pragma unroll
-            for (int ks = 0; ks < 2; ks++) {
-                const float4 d0 = *(const float4 *) (my + 2 * Q + 32 * ks + 8 * grp), d1 = *(const float4 *) (my + 2 * Q + 32 * ks + 8 * grp + 4);
-                const float dd[8] = { d0.x, d0.y, d0.z, d0.w, d1.x, d1.y, d1.z, d1.w };
+        for (int ks = 0; ks < 2; ks++) {
+            const float4 d0 = *(const float4 *) (my + 2 * Q + 32 * ks + 8 * grp), d1 = *(const float4 *) (my + 2 * Q + 32 * ks + 8 * grp + 4);
+            const float dd[8] = { d0.x, d0.y, d0.z, d0.w, d1.x, d1.y, d1.z, d1.w };
 #pragma unroll
-                for (int i = 0; i < 8; i++) x[ks][i] *= dd[i];
-            }
-            if (!whole) {
-#pragma unroll
-                for (int ks = 0; ks < 2; ks++) {
-#pragma unroll
-                    for (int i = 0; i < 8; i++) x[ks][i] = pok && 32 * ks + 8 * grp + i < left ? x[ks][i] : 0.0f;
-                }
-            }
-#pragma unroll
-            for (int ks = 0; ks < 2; ks++) {
-#pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    odd = fmaf(x[ks][i], 0.0f, odd);
-                    most = fmaxf(most, fabsf(x[ks][i]));
-                }
-            }
-            odd_chunk = __any(odd != 0.0f);
-            if (odd_chunk) {
-                most = 0.0f;
-#pragma unroll
-                for (int ks = 1; ks >= 0; ks--) {
-#pragma unroll
-                    for (int i = 7; i >= 0; i--) {
-                        const bool fine = fabsf(x[ks][i]) < INFINITY;
-                        if (!fine) bad = 32 * ks + 8 * grp + i;
-                        x[ks][i] = fine ? x[ks][i] : 0.0f;
-                        most = fmaxf(most, fabsf(x[ks][i]));
-                    }
-                }
-                bad = min(bad, __shfl_xor(bad, 16, WAVE));
-                bad = min(bad, __shfl_xor(bad, 32, WAVE));
-            }
-            most = column_max(most);
+            for (int i = 0; i < 8; i++) x[ks][i] *= dd[i];
         }
+        if (!whole) {
+#pragma unroll
+            for (int ks = 0; ks < 2; ks++) {
+#pragma unroll
+                for (int i = 0; i < 8; i++) x[ks][i] = pok && 32 * ks + 8 * grp + i < left ? x[ks][i] : 0.0f;
+            }
+        }
+#pragma unroll
+        for (int ks = 0; ks < 2; ks++) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) most = fmaxf(most, fabsf(x[ks][i]));
+        }
+        most = column_max(most);
+        int bad = Q;                                           // the channel's first token whose X is not finite
         half8 xh[2], xl[2];
         if (OUT) {
             // C_t S
@@ -544,8 +602,8 @@ __global__ __launch_bounds__(THREADS, 2) void ssm_scan_mm_kernel(mm_plan P) {
                     }
                     float v[8];
 #pragma unroll
-                    for (int i = 0; i < 8; i++) v[i] = as_f32(S[2 * ks + i / 4][i % 4] * ss);
-                    split8(v, bh, bl);
+                    for (int i = 0; i < 8; i++) v[i] = S[2 * ks + i / 4][i % 4];
+                    split8(v, ss, bh, bl);
 #pragma unroll
                     for (int tt = 0; tt < 4; tt++) acc[tt] = mfma(al[tt], bh, acc[tt]);
 #pragma unroll
@@ -556,36 +614,65 @@ __global__ __launch_bounds__(THREADS, 2) void ssm_scan_mm_kernel(mm_plan P) {
             }
             __syncthreads();                                   // C is read, the matrices are written
             if (active) {
-                const float sc = scale_of(most);
-                const float inv = inverse_of(scale_of(gmost * fmaxf(1.0f, e_last))) * inverse_of(sc);
-#pragma unroll
-                for (int ks = 0; ks < 2; ks++) {
-                    float v[8];
-#pragma unroll
-                    for (int i = 0; i < 8; i++) v[i] = as_f32(x[ks][i] * sc);
-                    split8(v, xh[ks], xl[ks]);
-                }
+                const float inv_m = inverse_of(scale_of(gmost * fmaxf(1.0f, e_last)));
                 const char * mine = mats + hl * 2 * M_BYTES + lane * 16;
-                half8 ah[6], al[6];
-#pragma unroll
-                for (int b = 0; b < 6; b++) {
-                    ah[b] = *(const half8 *) (mine + b * 1024);
-                    al[b] = *(const half8 *) (mine + b * 1024 + M_BYTES);
-                }
-                // tiles 0 and 1 end within the first 32 tokens
                 float4v sum[4];
+                float inv_x = 1.0f;
+                auto products = [&]() {
+                    const float sc = scale_of(most);
+                    inv_x = inverse_of(sc);
 #pragma unroll
-                for (int tt = 0; tt < 4; tt++) sum[tt] = mfma(al[tt < 2 ? tt : 2 * tt - 2], xh[0], float4v{ 0, 0, 0, 0 });
+                    for (int ks = 0; ks < 2; ks++) split8(x[ks], sc, xh[ks], xl[ks]);
 #pragma unroll
-                for (int tt = 0; tt < 4; tt++) sum[tt] = mfma(ah[tt < 2 ? tt : 2 * tt - 2], xl[0], sum[tt]);
+                    for (int t2 = 0; t2 < 4; t2 += 2) {
+                        // tiles 0 and 1 end within the first 32 tokens
+                        half8 ah[2][2], al[2][2];
 #pragma unroll
-                for (int tt = 0; tt < 4; tt++) sum[tt] = mfma(ah[tt < 2 ? tt : 2 * tt - 2], xh[0], sum[tt]);
+                        for (int ks = 0; ks <= t2 / 2; ks++) {
 #pragma unroll
-                for (int tt = 2; tt < 4; tt++) sum[tt] = mfma(al[2 * tt - 1], xh[1], sum[tt]);
+                            for (int q = 0; q < 2; q++) {
+                                const char * a = mine + (t2 == 0 ? q : 2 + 2 * q + ks) * 1024;
+                                ah[q][ks] = *(const half8 *) a;
+                                al[q][ks] = *(const half8 *) (a + M_BYTES);
+                            }
+                        }
 #pragma unroll
-                for (int tt = 2; tt < 4; tt++) sum[tt] = mfma(ah[2 * tt - 1], xl[1], sum[tt]);
+                        for (int q = 0; q < 2; q++) sum[t2 + q] = mfma(al[q][0], xh[0], float4v{ 0, 0, 0, 0 });
 #pragma unroll
-                for (int tt = 2; tt < 4; tt++) sum[tt] = mfma(ah[2 * tt - 1], xh[1], sum[tt]);
+                        for (int q = 0; q < 2; q++) sum[t2 + q] = mfma(ah[q][0], xl[0], sum[t2 + q]);
+#pragma unroll
+                        for (int q = 0; q < 2; q++) sum[t2 + q] = mfma(ah[q][0], xh[0], sum[t2 + q]);
+                        if (t2) {
+#pragma unroll
+                            for (int q = 0; q < 2; q++) sum[t2 + q] = mfma(al[q][1], xh[1], sum[t2 + q]);
+#pragma unroll
+                            for (int q = 0; q < 2; q++) sum[t2 + q] = mfma(ah[q][1], xl[1], sum[t2 + q]);
+#pragma unroll
+                            for (int q = 0; q < 2; q++) sum[t2 + q] = mfma(ah[q][1], xh[1], sum[t2 + q]);
+                        }
+                    }
+                };
+                products();
+                // Every row of the last tile takes all of a channel's tokens, so an X that is not finite shows there (as
+                // may a value of B, C or dt, which stays as it is): again without it.
+                if (__any(!(fabsf(sum[3][3]) < INFINITY))) {
+                    most = 0.0f;
+#pragma unroll
+                    for (int ks = 1; ks >= 0; ks--) {
+#pragma unroll
+                        for (int i = 7; i >= 0; i--) {
+                            const bool fine = fabsf(x[ks][i]) < INFINITY;
+                            if (!fine) bad = 32 * ks + 8 * grp + i;
+                            x[ks][i] = fine ? x[ks][i] : 0.0f;
+                            most = fmaxf(most, fabsf(x[ks][i]));
+                        }
+                    }
+                    bad = min(bad, __shfl_xor(bad, 16, WAVE));
+                    bad = min(bad, __shfl_xor(bad, 32, WAVE));
+                    most = column_max(most);
+                    products();
+                }
+                const float inv = inv_m * inv_x;
 #pragma unroll
                 for (int tt = 0; tt < 4; tt++) {
                     const float4 e4 = *(const float4 *) (my + 16 * tt + 4 * grp);
@@ -593,7 +680,7 @@ __global__ __launch_bounds__(THREADS, 2) void ssm_scan_mm_kernel(mm_plan P) {
 #pragma unroll
                     for (int i = 0; i < 4; i++) acc[tt][i] = fmaf(acc[tt][i], inv_s * e[i], sum[tt][i] * inv);
                 }
-                if (odd_chunk) {
+                if (__any(bad < Q)) {
 #pragma unroll
                     for (int tt = 0; tt < 4; tt++) {
 #pragma unroll
@@ -629,8 +716,8 @@ __global__ __launch_bounds__(THREADS, 2) void ssm_scan_mm_kernel(mm_plan P) {
                 const float ww[8] = { w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w };
                 float v[8];
 #pragma unroll
-                for (int i = 0; i < 8; i++) v[i] = as_f32(x[ks][i] * ww[i] * sc);
-                split8(v, xh[ks], xl[ks]);
+                for (int i = 0; i < 8; i++) v[i] = x[ks][i] * ww[i];
+                split8(v, sc, xh[ks], xl[ks]);
             }
         }
         if (c + 1 < c1) fetch(c + 1);
@@ -664,7 +751,7 @@ __global__ __launch_bounds__(THREADS, 2) void ssm_scan_mm_kernel(mm_plan P) {
                     for (int i = 0; i < 4; i++) S[n0 + q][i] = fmaf(S[n0 + q][i], e_last, sum[q][i] * inv_u);
                 }
             }
-            if (odd_chunk) {
+            if (OUT && __any(bad < Q)) {
 #pragma unroll
                 for (int nt = 0; nt < 2 * NK; nt++) {
 #pragma unroll
@@ -718,7 +805,7 @@ mm_sizes mm_size(const ssm_scan_launch & L) {
     z.hw = z.p_blocks > 1 ? 1 : std::min(WAVES / z.slices, z.nk == 8 ? 2 : 4);
     z.head_blocks = (L.H / L.G + z.hw - 1) / z.hw;
     z.chunks = (L.T + Q - 1) / Q;
-    const int64_t rec = (int64_t) z.nk * 16384 + Q * Q * 4 + 16, per = L.S * (L.G * rec + (int64_t) L.H * STEP_WORDS * 4);
+    const int64_t rec = (int64_t) z.nk * 16384 + G_WORDS * 4 + 16, per = L.S * (L.G * rec + (int64_t) L.H * STEP_WORDS * 4);
     // prepared operands of at most 64 MiB: the tokens go through in blocks
     z.block = std::max<int64_t>(1, std::min<int64_t>({ z.chunks, ((int64_t) 64 << 20) / per, 65535 }));
     // segments until every CU has a workgroup, of one chunk if need be (333 tokens of 24 heads: 41 us with two
@@ -731,7 +818,7 @@ mm_sizes mm_size(const ssm_scan_launch & L) {
     int64_t at = 0;
     auto take = [&](int64_t bytes) { const int64_t r = at; at += (bytes + 255) / 256 * 256; return r; };
     z.planes = take(L.S * z.block * L.G * (int64_t) z.nk * 16384);
-    z.gmat = take(L.S * z.block * L.G * Q * Q * 4);
+    z.gmat = take(L.S * z.block * L.G * G_WORDS * 4);
     z.scales = take(L.S * z.block * L.G * 16);
     z.steps = take(L.S * z.block * (int64_t) L.H * STEP_WORDS * 4);
     z.parts = take(z.n_seg > 1 ? L.S * z.n_seg * (int64_t) L.H * z.slices * 2 * z.nk * WAVE * 16 : 0);
@@ -755,7 +842,7 @@ void launch_mm(const ssm_scan_launch & L, const mm_sizes & z, void * ws, hipStre
     };
     static const bool lds_set = [&] {
         const int hw = NK == 8 ? 2 : 4;
-        HIP_CHECK(hipFuncSetAttribute((const void *) ssm_operands_kernel<NK>, hipFuncAttributeMaxDynamicSharedMemorySize, OPERAND + 64));
+        HIP_CHECK(hipFuncSetAttribute((const void *) ssm_prepare_kernel<NK>, hipFuncAttributeMaxDynamicSharedMemorySize, OPERAND + 64));
         HIP_CHECK(hipFuncSetAttribute((const void *) ssm_scan_mm_kernel<NK, false>, hipFuncAttributeMaxDynamicSharedMemorySize, (int) lds_of(hw, false)));
         HIP_CHECK(hipFuncSetAttribute((const void *) ssm_scan_mm_kernel<NK, true>, hipFuncAttributeMaxDynamicSharedMemorySize, (int) lds_of(hw, true)));
         return true;
@@ -776,8 +863,8 @@ void launch_mm(const ssm_scan_launch & L, const mm_sizes & z, void * ws, hipStre
         P.s1 = c + z.block < z.chunks ? hold + turn * states : L.s_out;
         P.vec_s0 = c == 0 ? rows16(L.s, L.s_p, L.s_h, L.s_row) : L.N % 4 == 0 && (uintptr_t) P.s0 % 16 == 0;
         P.vec_s1 = L.N % 4 == 0 && (uintptr_t) P.s1 % 16 == 0;
-        launch(ssm_steps_kernel, dim3((unsigned) P.nc, (unsigned) ((L.H + 15) / 16), (unsigned) L.S), dim3(256), 0, st, P);
-        launch(ssm_operands_kernel<NK>, dim3((unsigned) P.nc, (unsigned) L.G, (unsigned) L.S), dim3(256), OPERAND + 64, st, P);
+        launch(ssm_prepare_kernel<NK>, dim3((unsigned) P.nc, (unsigned) (L.G + (L.H + 15) / 16), (unsigned) L.S), dim3(256),
+               std::max<size_t>(OPERAND + 64, Q * 17 * 4), st, P);
         const dim3 grid((unsigned) (L.S * L.G * P.n_seg * z.head_blocks * z.p_blocks));
         if (P.n_seg > 1) launch(ssm_scan_mm_kernel<NK, false>, grid, dim3(THREADS), lds_of(z.hw, false), st, P);
         launch(ssm_scan_mm_kernel<NK, true>, grid, dim3(THREADS), lds_of(z.hw, true), st, P);
@@ -788,7 +875,7 @@ void launch_mm(const ssm_scan_launch & L, const mm_sizes & z, void * ws, hipStre
 
 bool ssm_scan_mm_takes(const ssm_scan_launch & L) {
     // the grids' limits: one dimension each for the sequences and for groups and heads
-    return L.a_scalar && L.T > SSM_STEP_TOKENS && L.S <= 65535 && L.G <= 65535 && L.H <= 16 * 65535 &&
+    return L.a_scalar && L.T > SSM_STEP_TOKENS && L.S <= 65535 && L.G + (L.H + 15) / 16 <= 65535 &&
            L.S * (int64_t) L.H * L.P < INT32_MAX &&
            // 32-bit offsets within a chunk
            L.x_t >= 0 && L.x_t <= 1 << 24 && (int64_t) L.H * L.P <= 1 << 24 && L.P <= 1 << 24;
