@@ -280,42 +280,56 @@ void launch_rows(const ssm_scan_launch & L, hipStream_t st) {
 // share B and C, and (ONE_HEAD) the time step and the decay.
 constexpr int STEP_ROWS = 4;
 
+// 16 bytes at any float's address
+__device__ __forceinline__ float4 load4(const float * p) {
+    typedef float v4 __attribute__((ext_vector_type(4), aligned(4)));
+    const v4 v = *(const v4 *) p;
+    return make_float4(v[0], v[1], v[2], v[3]);
+}
+__device__ __forceinline__ void store4(float * p, float4 f) {
+    typedef float v4 __attribute__((ext_vector_type(4), aligned(4)));
+    const v4 v = { f.x, f.y, f.z, f.w };
+    *(v4 *) p = v;
+}
+
 template <int LANES, bool ONE_HEAD>
 __global__ __launch_bounds__(256) void ssm_scan_step_kernel(ssm_scan_launch L, int64_t groups) {
     const int64_t group = ((int64_t) blockIdx.x * 256 + threadIdx.x) / LANES;
     const int lane = threadIdx.x % LANES, n = 4 * lane;
     if (group >= groups) return;                               // whole groups only
-    const int64_t r0 = group * STEP_ROWS, per = (int64_t) L.P * L.H, s = r0 / per;
-    const int q0 = (int) (r0 - s * per);
+    const int64_t per = (int64_t) L.P * L.H, in_seq = (per + STEP_ROWS - 1) / STEP_ROWS, s = group / in_seq;
+    const int q0 = (int) (group - s * in_seq) * STEP_ROWS;
     const bool on = n < L.N;
-    int p[STEP_ROWS], h[STEP_ROWS];
+    // past a sequence's last channel that one again: its values are stored twice
+    int q[STEP_ROWS], p[STEP_ROWS], h[STEP_ROWS];
 #pragma unroll
     for (int k = 0; k < STEP_ROWS; k++) {
-        h[k] = ONE_HEAD ? q0 / L.P : (q0 + k) / L.P;
-        p[k] = q0 + k - h[k] * L.P;
+        q[k] = ONE_HEAD ? q0 + k : min(q0 + k, (int) per - 1);
+        h[k] = ONE_HEAD ? q0 / L.P : q[k] / L.P;
+        p[k] = q[k] - h[k] * L.P;
     }
     const int g = h[0] / (L.H / L.G);
     const int64_t id = pool_row(L, s);
     const float4 zero = make_float4(0, 0, 0, 0);
     float4 st[STEP_ROWS], a[ONE_HEAD ? 1 : STEP_ROWS];
 #pragma unroll
-    for (int k = 0; k < STEP_ROWS; k++) st[k] = on ? *(const float4 *) (L.s + p[k] * L.s_p + h[k] * L.s_h + id * L.s_row + n) : zero;
+    for (int k = 0; k < STEP_ROWS; k++) st[k] = on ? load4(L.s + p[k] * L.s_p + h[k] * L.s_h + id * L.s_row + n) : zero;
 #pragma unroll
     for (int k = 0; k < (ONE_HEAD ? 1 : STEP_ROWS); k++) {
         const float * A = L.A + h[k] * L.a_h;
         if (L.a_scalar) a[k] = make_float4(A[0], A[0], A[0], A[0]);
-        else a[k] = on ? make_float4(A[n], A[n + 1], A[n + 2], A[n + 3]) : zero;
+        else a[k] = on ? load4(A + n) : zero;
         a[k] = make_float4(a[k].x * LOG2E, a[k].y * LOG2E, a[k].z * LOG2E, a[k].w * LOG2E);
     }
     const float * B = L.B + g * L.b_g + s * L.b_s + n, * C = L.C + g * L.c_g + s * L.c_s + n;
-    float * y = L.y + q0 + per * L.T * s;
+    float * y = L.y + per * L.T * s;
     for (int64_t t = 0; t < L.T; t++) {
         float d[ONE_HEAD ? 1 : STEP_ROWS], x[STEP_ROWS], v[STEP_ROWS];
 #pragma unroll
         for (int k = 0; k < (ONE_HEAD ? 1 : STEP_ROWS); k++) d[k] = L.dt[h[k] + t * L.dt_t + s * L.dt_s];
 #pragma unroll
         for (int k = 0; k < STEP_ROWS; k++) x[k] = L.x[p[k] + h[k] * L.x_h + t * L.x_t + s * L.x_s];
-        const float4 b = on ? *(const float4 *) (B + t * L.b_t) : zero, c = on ? *(const float4 *) (C + t * L.c_t) : zero;
+        const float4 b = on ? load4(B + t * L.b_t) : zero, c = on ? load4(C + t * L.c_t) : zero;
         float4 e = zero;
 #pragma unroll
         for (int k = 0; k < STEP_ROWS; k++) {
@@ -336,38 +350,38 @@ __global__ __launch_bounds__(256) void ssm_scan_step_kernel(ssm_scan_launch L, i
         }
 #pragma unroll
         for (int k = 0; k < STEP_ROWS; k++) {
-            if (lane == k % LANES) y[t * per + k] = v[k];
+            if (lane == k % LANES) y[t * per + q[k]] = v[k];
         }
     }
     if (!on) return;
 #pragma unroll
-    for (int k = 0; k < STEP_ROWS; k++) *(float4 *) (L.s_out + (int64_t) L.N * (r0 + k) + n) = st[k];
+    for (int k = 0; k < STEP_ROWS; k++) store4(L.s_out + (int64_t) L.N * (q[k] + per * s) + n, st[k]);
 }
 
-bool rows16(const void * p, int64_t a, int64_t b, int64_t c) { return (uintptr_t) p % 16 == 0 && a % 4 == 0 && b % 4 == 0 && c % 4 == 0; }
-
 bool step_takes(const ssm_scan_launch & L) {
-    return L.N % 4 == 0 && ((int64_t) L.H / L.G * L.P) % STEP_ROWS == 0 && rows16(L.s, L.s_p, L.s_h, L.s_row) && rows16(L.B, L.b_g, L.b_t, L.b_s) &&
-           rows16(L.C, L.c_g, L.c_t, L.c_s) && (uintptr_t) L.s_out % 16 == 0;
+    return L.N % 4 == 0 && (L.G == 1 || ((int64_t) L.H / L.G * L.P) % STEP_ROWS == 0);
 }
 
 template <int LANES>
 void launch_step(const ssm_scan_launch & L, hipStream_t st) {
-    const int64_t groups = (int64_t) L.P * L.H * L.S / STEP_ROWS, per = 256 / LANES;
+    const int64_t groups = ((int64_t) L.P * L.H + STEP_ROWS - 1) / STEP_ROWS * L.S, per = 256 / LANES;
     const dim3 grid((unsigned) ((groups + per - 1) / per));
     if (L.P % STEP_ROWS == 0) launch(ssm_scan_step_kernel<LANES, true>, grid, dim3(256), 0, st, L, groups);
     else launch(ssm_scan_step_kernel<LANES, false>, grid, dim3(256), 0, st, L, groups);
 }
 
-// Heads of one channel over many tokens: a lane per channel with all of its N states in registers, so that no
-// sum crosses lanes and B and C, the same for the wave's 64 channels, are scalar operands. Every state takes
-// an exponential and four more operations per token, which bounds it: 16 states at 4 + 4 cycles. The tokens are
-// split into segments, since channels alone are too few waves: `local` finds each segment's final state from
-// nothing and its sum of time steps, `join` the state that each begins with, and the last launch the outputs.
-// The first pass repeats 7/8 of the work; carrying its outputs over would take as many exponentials again.
+// Heads of one channel: a lane per channel with all of its N states in registers, so that no sum crosses lanes
+// and B and C, the same for the wave's 64 channels, are scalar operands. Every state takes an exponential and
+// four more operations per token, which bounds it over many tokens; the states' bytes do over few, and they go
+// through LDS so that lanes next to each other read 16 bytes next to each other (without it 81 sequences of 5120
+// channels and 16 states took 32 us a token, with it 12.1, 4.8 TB/s; the kernel for few tokens took 15.7).
+// Where channels alone are too few waves the tokens are split into segments: `local` finds each segment's final
+// state from nothing and its sum of time steps, `join` the state that each begins with, and the last launch the
+// outputs (72 us at 1500 tokens of 5120 channels: 28, 5 and 36). The first pass repeats 7/8 of the work;
+// carrying its outputs over would take as many exponentials again.
 struct chan_plan {
     ssm_scan_launch L;
-    float * part;          // [S, n_seg, N, H]: segments' states, then what each begins with
+    float * part;          // [S, n_seg, H, N]: segments' states, then what each begins with
     float * sums;          // [S, n_seg, H]
     int     seg, n_seg;    // tokens per segment, segments
 };
@@ -377,27 +391,50 @@ typedef const __attribute__((address_space(4))) float * scalar_ptr;
 template <int N, bool OUT>
 __global__ __launch_bounds__(64) void ssm_scan_channels_kernel(chan_plan P) {
     const ssm_scan_launch & L = P.L;
-    const int h = blockIdx.x * 64 + threadIdx.x, hc = min(h, L.H - 1), sg = blockIdx.y;
+    // decays and states lie by channels in memory: LANES lanes read a channel's, and LDS turns them
+    constexpr int LANES = N / 4, PITCH = N + 4;
+    __shared__ __align__(16) float turn[64 * PITCH];
+    const int h0 = blockIdx.x * 64, h = h0 + threadIdx.x, hc = min(h, L.H - 1), sg = blockIdx.y;
+    const int c0 = threadIdx.x / LANES, n4 = threadIdx.x % LANES * 4;
     const int64_t s = blockIdx.z;
-    const int g = (int) (blockIdx.x * 64) / (L.H / L.G);
+    const int g = h0 / (L.H / L.G);
     const int64_t t0 = (int64_t) sg * P.seg, t1 = min(L.T, t0 + P.seg);
     float a[N], st[N];
-    const float * A = L.A + hc * L.a_h;
+    float4 part[LANES];
+    auto rows = [&](const float * p, int64_t step) {
 #pragma unroll
-    for (int n = 0; n < N; n++) a[n] = A[L.a_scalar ? 0 : n] * LOG2E;
-    if (OUT) {
-        if (P.n_seg == 1) {
-            const float * s0 = L.s + hc * L.s_h + pool_row(L, s) * L.s_row;
+        for (int i = 0; i < LANES; i++) part[i] = load4(p + min(h0 + c0 + i * (64 / LANES), L.H - 1) * step + n4);
+    };
+    auto turned = [&](float (&v)[N]) {
 #pragma unroll
-            for (int n = 0; n < N; n++) st[n] = s0[n];
-        } else {
-            const float * q = P.part + ((s * P.n_seg + sg) * N) * L.H + hc;
+        for (int i = 0; i < LANES; i++) *(float4 *) (turn + (c0 + i * (64 / LANES)) * PITCH + n4) = part[i];
+        __syncthreads();
 #pragma unroll
-            for (int n = 0; n < N; n++) st[n] = q[(int64_t) n * L.H];
+        for (int n = 0; n < N; n += 4) {
+            const float4 f = *(const float4 *) (turn + threadIdx.x * PITCH + n);
+            v[n] = f.x; v[n + 1] = f.y; v[n + 2] = f.z; v[n + 3] = f.w;
         }
+        __syncthreads();
+    };
+    if (L.a_scalar) {
+        const float a0 = L.A[hc * L.a_h];
+#pragma unroll
+        for (int n = 0; n < N; n++) a[n] = a0;
     } else {
+        rows(L.A, L.a_h);
+        turned(a);
+    }
+#pragma unroll
+    for (int n = 0; n < N; n++) a[n] *= LOG2E;
+    if (!OUT) {
 #pragma unroll
         for (int n = 0; n < N; n++) st[n] = 0.0f;
+    } else if (P.n_seg == 1) {
+        rows(L.s + pool_row(L, s) * L.s_row, L.s_h);
+        turned(st);
+    } else {
+        rows(P.part + (s * P.n_seg + sg) * N * L.H, N);
+        turned(st);
     }
     const float * x = L.x + hc * L.x_h + s * L.x_s + t0 * L.x_t, * dt = L.dt + hc + s * L.dt_s + t0 * L.dt_t;
     scalar_ptr B = (scalar_ptr) (uintptr_t) (L.B + g * L.b_g + s * L.b_s + t0 * L.b_t);
@@ -444,56 +481,60 @@ __global__ __launch_bounds__(64) void ssm_scan_channels_kernel(chan_plan P) {
         for (int i = 0; i < 4; i++) token(raw[i], xt[i]);
     }
     for (int i = 0; t + i < t1; i++) token(i == 0 ? dn[0] : i == 1 ? dn[1] : dn[2], i == 0 ? xn[0] : i == 1 ? xn[1] : xn[2]);
-    if (h >= L.H) return;
-    if (OUT) {
-        if (sg != P.n_seg - 1) return;
-        float * so = L.s_out + (int64_t) N * (h + (int64_t) L.H * s);
+    if (OUT && sg != P.n_seg - 1) return;
+    float * q = OUT ? L.s_out + (int64_t) N * L.H * s : P.part + (s * P.n_seg + sg) * N * L.H;
 #pragma unroll
-        for (int n = 0; n < N; n++) so[n] = st[n];
-    } else {
-        float * q = P.part + ((s * P.n_seg + sg) * N) * L.H + h;
+    for (int n = 0; n < N; n += 4) *(float4 *) (turn + threadIdx.x * PITCH + n) = make_float4(st[n], st[n + 1], st[n + 2], st[n + 3]);
+    __syncthreads();
 #pragma unroll
-        for (int n = 0; n < N; n++) q[(int64_t) n * L.H] = st[n];
-        P.sums[(s * P.n_seg + sg) * L.H + h] = sum;
+    for (int i = 0; i < LANES; i++) {
+        const int c = c0 + i * (64 / LANES);
+        if (h0 + c < L.H) store4(q + (int64_t) N * (h0 + c) + n4, *(const float4 *) (turn + c * PITCH + n4));
     }
+    if (!OUT && h < L.H) P.sums[(s * P.n_seg + sg) * L.H + h] = sum;
 }
 
 // a thread per channel and state: the segments in order
 __global__ __launch_bounds__(256) void ssm_scan_join_kernel(chan_plan P) {
     const ssm_scan_launch & L = P.L;
-    const int h = blockIdx.x * 256 + threadIdx.x, n = blockIdx.y;
-    const int64_t s = blockIdx.z;
-    if (h >= L.H) return;
+    const int64_t i = (int64_t) blockIdx.x * 256 + threadIdx.x, step = (int64_t) L.N * L.H, s = blockIdx.y;
+    if (i >= step) return;
+    const int h = (int) (i / L.N), n = (int) (i - (int64_t) h * L.N);
     const float a = L.A[h * L.a_h + (L.a_scalar ? 0 : n)] * LOG2E;
     float st = L.s[n + h * L.s_h + pool_row(L, s) * L.s_row];
-    float * q = P.part + (s * P.n_seg * L.N + n) * L.H + h;
+    float * q = P.part + s * P.n_seg * step + i;
     const float * sum = P.sums + s * P.n_seg * L.H + h;
-    const int64_t step = (int64_t) L.N * L.H;
     // sixteen segments' loads in flight
     for (int k0 = 0; k0 < P.n_seg; k0 += 16) {
         float own[16], d[16];
 #pragma unroll
         for (int k = 0; k < 16; k++) {
-            const int64_t c = min(k0 + k, P.n_seg - 1);
-            own[k] = q[c * step];
-            d[k] = sum[c * L.H];
+            if (k0 + k < P.n_seg - 1) {
+                own[k] = q[(k0 + k) * step];
+                d[k] = sum[(int64_t) (k0 + k) * L.H];
+            }
         }
 #pragma unroll
         for (int k = 0; k < 16; k++) {
-            if (k0 + k < P.n_seg) q[(k0 + k) * step] = st;
+            if (k0 + k >= P.n_seg) break;
+            q[(k0 + k) * step] = st;
             st = fmaf(st, exp2_hw(d[k] * a), own[k]);
         }
     }
 }
 
 bool channels_take(const ssm_scan_launch & L) {
-    return L.P == 1 && (L.N == 8 || L.N == 16 || L.N == 32) && L.T > SSM_STEP_TOKENS && (L.G == 1 || L.H / L.G % 64 == 0) && L.S <= 65535;
+    return L.P == 1 && (L.N == 8 || L.N == 16 || L.N == 32) && L.T >= 1 && (L.G == 1 || L.H / L.G % 64 == 0) && L.S <= 65535;
 }
 
-// Segments for four waves of every SIMD, of 32 tokens at least and 4096 segments at most.
+// One segment, or enough for four waves of every SIMD, of 8 tokens at least. With w waves of channels a token
+// takes 0.4 us in one piece (up to a wave per SIMD); split, about w / 820 of that, the first pass's work included,
+// and 12 us more. 80 waves (5120 channels): 32 tokens 15.7 us in one piece and 17.0 split, 48 tokens 21.9 and
+// 17.5; 640 waves: 54 tokens 26.6 and 40.1.
 void chan_segments(const ssm_scan_launch & L, chan_plan & P) {
-    const int64_t waves = (L.H + 63) / 64 * L.S, want = (4096 + waves - 1) / waves;
-    const int64_t n = std::max<int64_t>(1, std::min<int64_t>({ want, L.T / 32, 4096 }));
+    const int64_t waves = (L.H + 63) / 64 * L.S;
+    int64_t n = 1;
+    if (L.T * (820 - waves) > 32 * 820) n = std::min<int64_t>({ (4096 + waves - 1) / waves, L.T / 8, 4096 });
     P.seg = (int) ((L.T + n - 1) / n);
     P.n_seg = (int) ((L.T + P.seg - 1) / P.seg);
 }
@@ -504,7 +545,7 @@ void launch_channels(const chan_plan & P, hipStream_t st) {
     const unsigned hx = (unsigned) ((L.H + 63) / 64);
     if (P.n_seg > 1) {
         launch(ssm_scan_channels_kernel<N, false>, dim3(hx, (unsigned) P.n_seg - 1, (unsigned) L.S), dim3(64), 0, st, P);
-        launch(ssm_scan_join_kernel, dim3((unsigned) ((L.H + 255) / 256), (unsigned) N, (unsigned) L.S), dim3(256), 0, st, P);
+        launch(ssm_scan_join_kernel, dim3((unsigned) (((int64_t) N * L.H + 255) / 256), (unsigned) L.S), dim3(256), 0, st, P);
     }
     launch(ssm_scan_channels_kernel<N, true>, dim3(hx, (unsigned) P.n_seg, (unsigned) L.S), dim3(64), 0, st, P);
 }

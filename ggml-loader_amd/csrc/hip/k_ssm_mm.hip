@@ -871,11 +871,21 @@ void launch_mm(const ssm_scan_launch & L, const mm_sizes & z, void * ws, hipStre
     }
 }
 
+// Up to so many tokens the recurrence itself is faster: products need an operand and a chunk's latency, 12 us with
+// 32 states, 20 with 128 and 36 with 256, and a step takes 0.5 to 0.6 us. 80 heads of 64 channels and 128 states: 16
+// tokens 13.1 us by steps and 20.6 by products, 24 17.8 and 20.8, 32 22.5 and 20.8; 24 heads of 32 states 16 tokens
+// 11.2 and 12.6, 24 15.3 and 12.6; of 256 states 48 tokens 36.4 and 36.6. Where channels fill the chip a step takes
+// longer and the latency doesn't count: 163840 channels of 128 states 16 tokens 75.7 and 80.6, 24 106.8 and 80.8.
+int step_tokens(const ssm_scan_launch & L) {
+    const int few = L.N <= 64 ? 16 : L.N <= 128 ? 24 : 48;
+    return L.S * (int64_t) L.H * L.P > 65536 ? few * 2 / 3 : few;
+}
+
 } // namespace
 
 bool ssm_scan_mm_takes(const ssm_scan_launch & L) {
     // the grids' limits: one dimension each for the sequences and for groups and heads
-    return L.a_scalar && L.T > SSM_STEP_TOKENS && L.S <= 65535 && L.G + (L.H + 15) / 16 <= 65535 &&
+    return L.a_scalar && L.T > step_tokens(L) && L.S <= 65535 && L.G + (L.H + 15) / 16 <= 65535 &&
            L.S * (int64_t) L.H * L.P < INT32_MAX &&
            // 32-bit offsets within a chunk
            L.x_t >= 0 && L.x_t <= 1 << 24 && (int64_t) L.H * L.P <= 1 << 24 && L.P <= 1 << 24;

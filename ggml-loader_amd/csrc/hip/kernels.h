@@ -590,7 +590,6 @@ struct ssm_scan_launch {
     int             N, P, H, G;
     int             a_scalar;      // one A per head
 };
-constexpr int SSM_STEP_TOKENS = 16;    // up to so many tokens the states are what a step reads and writes
 // ws: 256-byte aligned scratch of ssm_scan_scratch_bytes (0: none)
 int64_t ssm_scan_scratch_bytes(const ssm_scan_launch & L);
 void launch_ssm_scan(const ssm_scan_launch & L, void * ws, hipStream_t st);

@@ -1,12 +1,13 @@
 """The state space mixers' operators in float64, each with a bound on the error of a float32
 evaluation that is carried through the same recurrence (u = 2^-24, half a step of float32).
 
-scan: a step forms exp(d A) from a softplus (expf and log1pf: 3 u of it, 4 u with the product by A
-and by log2 e, so 8 u |d A| with both) and the 2^x instruction (2 u), multiplies and adds (2 u), and
-adds d x B (4 u). Decays over up to 128 tokens may be formed from one running sum of their exponents,
-whose rounding (8 u of the sum of |d A| over them) every such decay inherits. The output adds N
-products: at most (2 + 8 + N / 8) u of their absolute sum, for lanes that hold up to N / 8 of them;
-a state that matrix products form adds up to 64 products per pass, 64 u of the absolute state.
+scan: a step forms exp(d A) from a softplus (a series and a 2^x instruction: 4 u of it, 4 u with the
+product by A and by log2 e, so 8 u |d A| with both) and another 2^x (2 u), multiplies and adds (2 u),
+and adds d x B (4 u). Decays over up to 128 tokens may be formed from one running sum of their
+exponents, whose rounding (8 u of the sum of |d A| over them) every such decay inherits. The output
+adds N products: at most (2 + 8 + N / 8) u of their absolute sum, for lanes that hold up to N / 8 of
+them, or 32 u where one lane holds up to 32; a state that matrix products form adds up to 64 products
+per pass, 64 u of the absolute state, which covers that too.
 """
 import numpy as np
 

@@ -131,6 +131,41 @@ def test_scan_keeps_what_came_before_a_bad_value(hip, T, at, P, N, a0, bad):
     near(h[hf], h64[hf], he[hf])
 
 
+# few tokens, channels and states at the edges of what a lane, a wave or a group of rows takes
+FEW = [
+    (3, 1, 67, 1, 16, 1, 3, 16), (2, 1, 64, 1, 8, 1, 2, 8), (3, 2, 130, 1, 32, 1, 3, 32), (2, 5, 129, 1, 16, 1, 2, 16), (1, 8, 1, 1, 16, 1, 1, 1),
+    (2, 4, 192, 1, 8, 3, 2, 8), (1, 3, 96, 1, 16, 3, 1, 16), (2, 39, 65, 1, 16, 1, 2, 16), (2, 48, 65, 1, 16, 1, 2, 16), (3, 41, 200, 1, 32, 1, 3, 32),
+    (5, 3, 7, 3, 20, 1, 5, 1), (3, 1, 5, 1, 64, 1, 3, 64), (4, 2, 3, 3, 12, 1, 4, 12), (3, 4, 3, 6, 128, 1, 3, 1), (2, 24, 3, 64, 128, 1, 2, 1),
+    (2, 25, 3, 64, 128, 1, 2, 1), (1, 48, 2, 4, 256, 1, 1, 1), (1, 49, 2, 4, 256, 1, 1, 1), (33, 17, 32, 64, 20, 1, 33, 1), (2, 7, 6, 2, 36, 3, 2, 1),
+]
+
+
+@pytest.mark.parametrize("S, T, H, P, N, G, pool, a0", FEW)
+@pytest.mark.parametrize("odd", [False, True])
+def test_scan_of_few_tokens(hip, S, T, H, P, N, G, pool, a0, odd):
+    """Whole tensors, and slices of rows whose addresses and strides are no multiple of 16 bytes."""
+    d = draw(np.random.default_rng(S + T * 3 + H + P * N), S, T, H, P, N, G, pool, a0)
+    if not odd:
+        check_scan(hip, d)
+        return
+    rows = lambda a, n: a.reshape(-1, n)  # noqa: E731
+    wide = np.concatenate([np.zeros((S * T, 1), np.float32), rows(d["x"], H * P), rows(d["B"], G * N), rows(d["C"], G * N)], 1)
+    w = wide.shape[1] + 1 if wide.shape[1] % 2 == 0 else wide.shape[1]
+    wide = np.pad(wide, ((0, 0), (0, w - wide.shape[1])))
+    per = H * P * N + 1
+    states = np.pad(rows(d["state"], H * P * N), ((0, 0), (0, 1)))
+    with Graph(mem=1 << 20) as g:
+        r = g.tensor(gl.F32, w, T, S, data=wide)
+        x = g.view_4d(r, P, H, T, S, P * 4, w * 4, T * w * 4, 4)
+        B, Cm = (g.view_4d(r, N, G, T, S, N * 4, w * 4, T * w * 4, 4 * a) for a in (1 + H * P, 1 + H * P + G * N))
+        s = g.view_4d(g.tensor(gl.F32, per, pool, data=states), N, P, H, pool, N * 4, N * P * 4, per * 4, 0)
+        dt, A = g.tensor(gl.F32, H, T, S, data=d["dt"]), g.tensor(gl.F32, a0, H, data=d["A"])
+        out = g.compute(hip, g.ssm_scan(s, x, dt, A, B, Cm, g.tensor(gl.I32, S, data=d["ids"]), 1))
+    y, h, ye, he = ssm_ref.scan(d["state"][d["ids"]], d["x"], d["dt"], d["A"], d["B"], d["C"])
+    near(out[:y.size], y, ye)
+    near(out[y.size:], h, he)
+
+
 def test_scan_of_strided_operands(hip):
     """x, B and C as slices of one projection, dt of another, A of a table, a pool of wider rows."""
     rng = np.random.default_rng(13)
