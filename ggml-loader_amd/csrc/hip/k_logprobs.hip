@@ -46,6 +46,7 @@ __device__ __forceinline__ int wave_sum(int v) {
 
 struct lp_shared {
     alignas(16) uint64_t key[LP_CAND];
+    alignas(16) float best[LP_THREADS];
     float f[2][LP_WAVES], w[LP_WAVES];
     int n[2][LP_WAVES];
 };
@@ -70,26 +71,48 @@ __device__ __forceinline__ void rank_keys(const uint64_t * keys, int n, int k, F
 // The k best of a workgroup's LP_SEG values (v[4 j + c] is entry j * 1024 + thread * 4 + c; the ones
 // from `valid` on are -inf), in order, to out(rank, key): every rank below k, key 0 where there are
 // fewer entries. best: the thread's largest value.
-// A threshold first: M >= k groups of threads each have a largest value, so the smallest of those, t,
-// has at least k entries at or above it (for normally distributed logits and k = 20 about 110 of 8192).
-// The entries above t are listed and each finds its rank by comparing with all; where they are fewer
-// than k, entries equal to t follow in the order of their ids. Were the list too long (values that the
-// groups do not share evenly, such as a block of -inf), t becomes the k-th largest value itself, found
-// by bisection: fewer than k entries lie above it.
+// A threshold first: of M >= 2 k groups of threads, each with its largest value, the k-th largest, t, has k
+// entries at or above it and few more (with evenly spread values and k = 20 of 64 groups about 24). The entries
+// from t on are listed and each finds its rank by comparing with all. Were the list too long (values that the
+// groups do not share evenly, such as a block of -inf, or many equal ones), t becomes the k-th largest value
+// itself, found by bisection: fewer than k entries lie above it, and ones equal to it follow in the order of
+// their ids. (With the least of M >= k groups' values for t, as it was, 110 entries were listed for k = 20,
+// and ranking them took as long as a third of the pass: 65 us at 512 rows of 128256 instead of XX.)
 template <class F>
 __device__ __forceinline__ void select_top(const float (&v)[LP_PER], float best, int valid, int id0, int k, lp_shared & S, F out) {
     const int tid = threadIdx.x, lane = tid % WAVE, wave = tid / WAVE;
-    float t = best;
-    if (k > 64) t = group_max<2>(t);
-    else if (k > 32) t = group_max<4>(t);
-    else if (k > 16) t = group_max<8>(t);
-    else if (k > 8) t = group_max<16>(t);
-    else if (k > 4) t = group_max<32>(t);
-    else t = group_max<64>(t);
-    t = -wave_max(-t);
-    if (lane == 0) S.f[0][wave] = t;
-    __syncthreads();
-    t = fminf(fminf(S.f[0][0], S.f[0][1]), fminf(S.f[0][2], S.f[0][3]));
+    float t;
+    // `groups` values lie in S.best; of those with fewer than k above them the least one
+    auto kth = [&](float own, int groups) {
+        int above = 0;
+#pragma unroll 16
+        for (int i = 0; i < groups; i += 4) {
+            const float4 g = *(const float4 *) (S.best + i);
+            above += (g.x > own ? 1 : 0) + (g.y > own ? 1 : 0) + (g.z > own ? 1 : 0) + (g.w > own ? 1 : 0);
+        }
+        return -wave_max(above < k ? -own : -INFINITY);
+    };
+    // the least of a value per wave
+    auto least = [&](float v) {
+        if (lane == 0) S.f[0][wave] = v;
+        __syncthreads();
+        return fminf(fminf(S.f[0][0], S.f[0][1]), fminf(S.f[0][2], S.f[0][3]));
+    };
+    if (k <= 8) {
+        // 8 or 4 groups and the least of all: about 22 or 8 entries
+        t = k > 4 ? group_max<32>(best) : group_max<64>(best);
+        t = least(-wave_max(-t));
+    } else if (k <= 32) {
+        // every wave for itself
+        const float g = group_max<4>(best);
+        if (lane % 4 == 0) S.best[tid / 4] = g;
+        __syncthreads();
+        t = kth(S.best[lane], 64);
+    } else {
+        S.best[tid] = best;
+        __syncthreads();
+        t = least(kth(best, LP_THREADS));
+    }
     // entries that satisfy f, of this thread (mine) and of the workgroup; `turn` alternates the words that it uses
     int mine;
     auto count = [&](int turn, auto f) {
@@ -101,10 +124,14 @@ __device__ __forceinline__ void select_top(const float (&v)[LP_PER], float best,
         __syncthreads();
         return S.n[turn][0] + S.n[turn][1] + S.n[turn][2] + S.n[turn][3];
     };
+    // entries above `t` are listed: with the float before t that is t's too, but for the -inf that also fill a segment
+    const float kt = t;
+    bool ties = t == -INFINITY;
+    if (!ties) t = okey_value(okey(t) - (t == 0.0f ? 2 : 1));     // -0 is no less than 0
     int turn = 0, above = count(0, [&](float x) { return x > t; });
     if (above > LP_CAND) {
-        // the largest value with k entries at or above it; okey(t) has them
-        uint32_t lo = okey(t), hi = 0xffffffffu;
+        // the largest value with k entries at or above it; kt has them
+        uint32_t lo = okey(kt), hi = 0xffffffffu;
         while (lo < hi) {
             const uint32_t mid = lo + (hi - lo) / 2 + 1;
             if (count(turn ^= 1, [&](float x) { return okey(x) >= mid; }) >= k) lo = mid;
@@ -112,6 +139,7 @@ __device__ __forceinline__ void select_top(const float (&v)[LP_PER], float best,
         }
         t = okey_value(lo);
         above = count(turn ^= 1, [&](float x) { return x > t; });
+        ties = true;
     }
     // the thread's place in the list: those of the waves and lanes before it
     int scan = mine;
@@ -131,6 +159,7 @@ __device__ __forceinline__ void select_top(const float (&v)[LP_PER], float best,
     if (tid < (-above & 3)) S.key[above + tid] = 0;
     __syncthreads();
     rank_keys(S.key, above, k, out);
+    if (!ties) return;
     // entries equal to the threshold, row of 1024 by row in the order of their ids
     for (int row = 0, got = above; row < LP_PER / 4 && got < k; row++) {
         int n = 0, before = 0, all = 0;
@@ -280,6 +309,10 @@ __global__ __launch_bounds__(LP_THREADS) void logprobs_join_kernel(logprobs_laun
     const lp_stats * part = (const lp_stats *) L.part + (int64_t) r * L.n_seg;
     const uint64_t * keys = (const uint64_t *) ((const lp_stats *) L.part + (int64_t) L.n_rows * L.n_seg) + (int64_t) r * total;
     const float tok = L.tokens ? row_of(L, r)[L.tokens[r]] : 0.0f;
+    // the thread's first entries, on their way while the sums join
+    uint64_t first[2];
+#pragma unroll
+    for (int i = 0; i < 2; i++) first[i] = tid + i * LP_THREADS < total ? keys[tid + i * LP_THREADS] : 0;
     uint64_t t = ~(uint64_t) 0;
     if (L.k) {
         const int q = (L.k + L.n_seg - 1) / L.n_seg;
@@ -305,10 +338,12 @@ __global__ __launch_bounds__(LP_THREADS) void logprobs_join_kernel(logprobs_laun
     if (tid == 0) put_scores(L, tok, a, ls, o);
     auto put = [&](int rank, uint64_t key) { put_top(L, a.m, ls, o, rank, key); };
     if (L.stage) {
-        for (int i = tid; i < total; i += LP_THREADS) {
-            const uint64_t key = keys[i];
+        auto keep = [&](uint64_t key) {
             if (key >= t) kept[atomicAdd(&count, 1)] = key;
-        }
+        };
+        if (tid < total) keep(first[0]);
+        if (tid + LP_THREADS < total) keep(first[1]);
+        for (int i = tid + 2 * LP_THREADS; i < total; i += LP_THREADS) keep(keys[i]);
         __syncthreads();
         const int n = count;
         if (tid < (-n & 3)) kept[n + tid] = 0;

@@ -128,6 +128,28 @@ def test_a_regular_pattern_of_banned_tokens(hip, n, n_top):
     check(hip, x, rng.integers(0, n, 6), n_top)
 
 
+@pytest.mark.parametrize("n", [700, 5000, 30000])
+@pytest.mark.parametrize("n_top", [2, 7, 20, 33, 128])
+def test_the_last_of_the_likeliest_among_equals(hip, n, n_top):
+    """The n_top-th entry is one of many equal ones, of a sign that 0 has two of, next to the smallest
+    floats or at the range's end; equal ones go by their ids."""
+    rng = np.random.default_rng(n + n_top)
+    x = -1 - rng.random((6, n), dtype=np.float32)
+    some = [rng.permutation(n) for _ in range(6)]
+    x[0, some[0][:200]] = np.where(rng.random(200) < 0.5, 0.0, -0.0)
+    x[1, some[1][:200]] = np.where(rng.random(200) < 0.5, 1e-45, -1e-45)
+    x[2] = -np.inf
+    x[2, some[2][:300]] = -np.finfo(np.float32).max
+    x[3] = rng.integers(0, 4, n)
+    x[4] = 0
+    x[5, some[5][:100]] = 1e-45
+    x[5, some[5][100:200]] = 0.0
+    for r in range(6):
+        if r != 4:
+            x[r, some[r][300:300 + n_top // 2]] = 3.0        # some above them
+    check(hip, x, rng.integers(0, n, 6), n_top)
+
+
 def test_a_banned_token(hip):
     x = np.array([[0, -np.inf, 1]], np.float32)
     got = check(hip, x, np.array([1]), 3)
