@@ -172,6 +172,7 @@ def _declare(core, hip, loader):
     _sig(core, "ggml_backend_tensor_set", None, T, vp, sz, sz)
     _sig(core, "ggml_backend_tensor_get", None, T, vp, sz, sz)
     _sig(core, "ggml_backend_graph_compute", i32, vp, vp)
+    _sig(core, "ggml_backend_graph_compute_async", i32, vp, vp)
     _sig(core, "ggml_backend_free", None, vp)
     _sig(core, "ggml_backend_name", C.c_char_p, vp)
     _sig(core, "ggml_backend_get_default_buffer_type", vp, vp)

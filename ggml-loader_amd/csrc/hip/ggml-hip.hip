@@ -465,6 +465,9 @@ const char * ssm_conv_refusal(const ggml_tensor * n) {
         if (!inside_base(t)) return "ssm_conv: an operand reaches past its tensor";
     }
     if (!ggml_is_contiguous(n)) return "ssm_conv: the result must be contiguous";
+    // a launch has up to 2^32 threads, of a channel and eight tokens each, and no fewer than 256 a block
+    const int64_t D = std::max<int64_t>(c->ne[1], 256);
+    if (D > INT_MAX || (T > 0 && D > ((int64_t) 1 << 34) / T)) return "ssm_conv: too many channels and tokens";
     return nullptr;
 }
 
@@ -485,6 +488,8 @@ const char * ssm_scan_refusal(const ggml_tensor * n) {
     if (!has_shape(x, P, H, T, S) || !has_shape(dt, H, T, S, 1) || !has_shape(B, N, G, T, S) || !has_shape(C, N, G, T, S) ||
         (A->ne[0] != 1 && A->ne[0] != N) || !has_shape(A, A->ne[0], H, 1, 1) || !has_shape(ids, S, 1, 1, 1) ||
         (S > 0 && s->ne[3] < 1)) return "ssm_scan: the operands' extents do not fit";
+    // up to 64 threads a channel, 2^32 a launch
+    if (S > ((int64_t) 1 << 25) / (P * H)) return "ssm_scan: too many channels";
     if (n->type != GGML_TYPE_F32 || !ggml_is_contiguous(n) || ggml_nelements(n) != P * H * T * S + N * P * H * S) {
         return "ssm_scan: the result's extent does not fit";
     }

@@ -14,14 +14,22 @@
 // 16/3 times the rate of the float32 matrix instructions. Sums and states are float32. The running
 // sums c are formed in double and kept as two floats, so that their differences keep 24 bits.
 //
-// Three launches. `prepare`, per (sequence, chunk, group): C and B split into the order in which the
-// lanes of a matrix instruction hold them, and the products C_t . B_j, which the group's heads share;
-// per (sequence, chunk, 16 heads): c and its exponentials. `scan<false>`, where the tokens are split
-// into segments for want of heads: each segment's state from nothing. `scan<true>`: the segments
-// before joined, then the chunks one after another. A wave holds the states of 16 or 32 channels of a
-// head in registers for its whole segment: the instruction that updates them leaves state n of
-// channel p in the lane that the next chunk's product reads it from, when the k index of that product
-// runs n = 4 g + i, then 16 + 4 g + i over lane group g, the order that C is prepared in.
+// Three launches. ssm_prepare_kernel, per (sequence, chunk, group): C and B split into the order in which the
+// lanes of a matrix instruction hold them, and the products C_t . B_j, which the group's heads share; per
+// (sequence, chunk, 16 heads): c and its exponentials. ssm_scan_mm_kernel<NK, false>, where the tokens are split
+// into segments for want of heads: each segment's state from nothing. ssm_scan_mm_kernel<NK, true>: the segments
+// before joined, then the chunks one after another. A wave holds the states of 16 channels of a head in registers
+// for its whole segment: the instruction that updates them leaves state n of channel p in the lane that the next
+// chunk's product reads it from, when the k index of that product runs n = 4 g + i, then 16 + 4 g + i over lane
+// group g, the order that C is prepared in. Eight waves share a chunk's operands, loaded a chunk ahead.
+//
+// 4096 tokens of 128 heads x 64 x 128, 8 groups: 177 us (1.76 TB/s of what must be read and written, whose floor
+// is 61 us; 22 + 43 + 126 in a trace), 333 tokens of 24 heads 32. Nothing is saturated: the matrix cores are busy
+// for a fifth of the time, the vector units for two fifths and LDS for a quarter, and leaving any one part out
+// (the loads of x or of the operands, the update of the state, the stores) saves a tenth each, so a chunk's
+// barriers and the latency between its parts are what is left. Two tiles of channels a wave (166 us for the last
+// launch), workgroups of four waves (159), four waves a SIMD with one buffer (spills), and half the waves a step
+// ahead of the others (149) were all slower than its 126.
 //
 // A value that is not finite must not reach earlier tokens of its chunk through 0 times it: X is
 // cleared of such values, and the channel's outputs from that token on, and its state, are NaN. (B, C
@@ -31,6 +39,7 @@
 #include "ssm_ops.h"
 
 #include <algorithm>
+#include <atomic>
 
 namespace {
 
@@ -840,14 +849,16 @@ void launch_mm(const ssm_scan_launch & L, const mm_sizes & z, void * ws, hipStre
     auto lds_of = [](int hw, bool out) {
         return (size_t) OPERAND * (b_slots(NK) + (out ? 1 : 0)) + (size_t) hw * (2 * STEP_WORDS * 4 + (out ? 2 * M_BYTES : 0));
     };
-    static const bool lds_set = [&] {
+    static std::atomic<uint64_t> lds_set{ 0 };                 // devices, a bit each
+    int device = 0;
+    HIP_CHECK(hipGetDevice(&device));
+    if (device > 63 || !(lds_set.load(std::memory_order_relaxed) >> device & 1)) {
         const int hw = NK == 8 ? 2 : 4;
         HIP_CHECK(hipFuncSetAttribute((const void *) ssm_prepare_kernel<NK>, hipFuncAttributeMaxDynamicSharedMemorySize, OPERAND + 64));
         HIP_CHECK(hipFuncSetAttribute((const void *) ssm_scan_mm_kernel<NK, false>, hipFuncAttributeMaxDynamicSharedMemorySize, (int) lds_of(hw, false)));
         HIP_CHECK(hipFuncSetAttribute((const void *) ssm_scan_mm_kernel<NK, true>, hipFuncAttributeMaxDynamicSharedMemorySize, (int) lds_of(hw, true)));
-        return true;
-    }();
-    (void) lds_set;
+        if (device < 64) lds_set.fetch_or(1ull << device, std::memory_order_relaxed);
+    }
     auto rows16 = [](const void * p, int64_t a, int64_t b, int64_t c) { return (uintptr_t) p % 16 == 0 && a % 4 == 0 && b % 4 == 0 && c % 4 == 0; };
     P.vec_bc = rows16(L.B, L.b_g, L.b_t, L.b_s) && rows16(L.C, L.c_g, L.c_t, L.c_s);
     float * hold = (float *) ((char *) ws + z.state);
@@ -884,9 +895,9 @@ int step_tokens(const ssm_scan_launch & L) {
 } // namespace
 
 bool ssm_scan_mm_takes(const ssm_scan_launch & L) {
-    // the grids' limits: one dimension each for the sequences and for groups and heads
+    // the grids' limits: one dimension each for the sequences and for groups and heads, 2^32 threads in all
     return L.a_scalar && L.T > step_tokens(L) && L.S <= 65535 && L.G + (L.H + 15) / 16 <= 65535 &&
-           L.S * (int64_t) L.H * L.P < INT32_MAX &&
+           L.S * (int64_t) L.H * ((L.P + 127) / 128) < 1 << 22 &&
            // 32-bit offsets within a chunk
            L.x_t >= 0 && L.x_t <= 1 << 24 && (int64_t) L.H * L.P <= 1 << 24 && L.P <= 1 << 24;
 }

@@ -90,6 +90,16 @@ def test_conv_refuses():
         assert "whole elements" in refusal(g.ssm_conv(g.view_3d(wide, 5, 16, 1, 22, 352, 0), w))
 
 
+def test_refuses_what_no_launch_takes():
+    with Graph(mem=1 << 20) as g:
+        conv = lambda D, T: refusal(g.ssm_conv(g.tensor(gl.F32, 3 + T, D), g.tensor(gl.F32, 4, D)))  # noqa: E731
+        assert conv(10240, 1 << 20) is None and conv(1, 1 << 26) is None and conv(1 << 30, 1) is None
+        assert "too many" in conv(10240, 1 << 21) and "too many" in conv(1, (1 << 26) + 1) and "too many" in conv(1 << 31, 0)
+        many = lambda S, H, P: refusal(scan(g, **scan_operands(g, S=S, H=H, P=P, T=1, G=1, pool=1)))  # noqa: E731
+        assert many(4096, 128, 64) is None and many(1, 1 << 25, 1) is None
+        assert "channels" in many(4097, 128, 64) and "channels" in many(1, (1 << 25) + 1, 1) and "channels" in many(1, 1 << 20, 1 << 12)
+
+
 def test_other_nodes_are_not_refused():
     with Graph(mem=1 << 20) as g:
         a = g.tensor(gl.F32, 8, 3)
