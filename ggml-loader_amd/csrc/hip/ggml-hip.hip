@@ -968,6 +968,20 @@ private:
         return last;
     }
 
+    // the launch at node `from` may write node `out`'s memory, where the graph lets memory serve twice: its own
+    // operands lie elsewhere, and so does all that nodes before `out` still read or write
+    bool conv_may_write(int from, int out, std::initializer_list<const ggml_tensor *> reads, const std::vector<int> & fused) const {
+        const ggml_tensor * to = g_->nodes[out];
+        for (const ggml_tensor * t : reads) {
+            if (overlap(t, to)) return false;
+        }
+        for (int f : fused) {
+            const ggml_tensor * t = g_->nodes[f];
+            if (t->op == GGML_OP_ADD && overlap(t->src[1], to)) return false;
+        }
+        return may_write_early(from, out, to, fused);
+    }
+
     void run_conv(ssm_conv_launch & L, const ggml_tensor * conv, const ggml_tensor * out, const std::vector<int> & fused) {
         const ggml_tensor * c = conv->src[1];
         L.w = (const float *) c->data;
@@ -991,7 +1005,13 @@ private:
         L.state = (const float *) sx->data;
         L.x = L.state + (L.K - 1) * L.st_j;
         std::vector<int> fused;
-        const int out = conv_epilogue(i, L, fused);
+        int out = conv_epilogue(i, L, fused);
+        if (out != i && !conv_may_write(i, out, { sx, n->src[1] }, fused)) {
+            L.bias = nullptr;
+            L.silu = 0;
+            fused.clear();
+            out = i;
+        }
         run_conv(L, n, g_->nodes[out], fused);
     }
 
@@ -1034,6 +1054,7 @@ private:
             fused.push_back(copy);
         }
         const int out = conv_epilogue(conv, L, fused);
+        if (!conv_may_write(i, out, { st, x, n->src[1] }, fused)) return false;
         if (copy >= 0) {
             const ggml_tensor * cp = g_->nodes[copy];
             const bool same = cp->data == st->data && ggml_is_contiguous(st);

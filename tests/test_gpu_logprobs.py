@@ -77,7 +77,7 @@ def check(hip, x, tokens, n_top, row=0, t=None):
     return got
 
 
-@pytest.mark.parametrize("n, rows, n_top", [(1, 1, 1), (2, 3, 2), (7, 4, 7), (64, 2, 0), (255, 5, 128), (257, 3, 20), (1000, 33, 5),
+@pytest.mark.parametrize("n, rows, n_top", [(1, 1, 1), (2, 3, 2), (7, 4, 7), (64, 2, 0), (255, 5, 128), (257, 3, 20), (1000, 33, 5), (57345, 2, 20), (57345, 1, 128),
                                             (4099, 9, 128), (32064, 37, 20), (151936, 1, 20), (151936, 2, 128), (128256, 300, 1),
                                             (151936, 1, 0), (50257, 2, 64), (8192, 3, 100), (8193, 3, 100), (600001, 1, 128)])
 def test_scores(hip, n, rows, n_top):

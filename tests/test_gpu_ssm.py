@@ -294,6 +294,38 @@ def test_conv_that_others_read(hip):
                 assert np.array_equal(got[1].reshape(D, K - 1), 2 * state[0])
 
 
+@pytest.mark.parametrize("what", ["rows", "joined", "between"])
+def test_conv_whose_result_takes_used_memory(hip, what):
+    """A result that lies in memory which is free by its place in the graph, and not before: the new
+    rows', the joined rows', that of another node's value."""
+    rng = np.random.default_rng(43)
+    K, T, D = 4, 300, 96
+    state = rng.standard_normal((1, D, K - 1)).astype(np.float32)
+    rows = rng.standard_normal((1, T, D)).astype(np.float32)
+    w, b = rng.standard_normal((D, K)).astype(np.float32), rng.standard_normal(D).astype(np.float32)
+    want, bound = ssm_ref.conv(np.concatenate([state, 2 * rows.transpose(0, 2, 1)], 2), w, b, True)
+    with Graph(mem=1 << 20) as g:
+        r = g.tensor(gl.F32, D, T, data=rows)
+        x = g.scale(r, 2.0)
+        joined = g.concat(g.tensor(gl.F32, K - 1, D, 1, data=state), g.transpose(x), 0)
+        conv = g.ssm_conv(joined, g.tensor(gl.F32, K, D, data=w))
+        between = g.scale(r, 3.0)
+        used = g.scale(between, 0.5)
+        y = g.silu(g.add(conv, g.tensor(gl.F32, D, data=b)))
+        gf = g.core.ggml_new_graph(g.ctx)
+        for t in (conv, used, y):
+            g.core.ggml_build_forward_expand(gf, t)
+        for t in (used, y):
+            g.core.ggml_set_output(t)
+        g.buf = g.core.ggml_backend_alloc_ctx_tensors(g.ctx, hip)
+        for t, v in g.inputs:
+            g.core.ggml_backend_tensor_set(t, ptr(v), 0, v.nbytes)
+        y.contents.data = {"rows": x, "joined": joined, "between": between}[what].contents.data
+        assert g.core.ggml_backend_graph_compute(hip, gf) == 0
+        near(g.read(y), want, bound, what)
+        assert np.array_equal(g.read(used), (rows * np.float32(3) * np.float32(0.5)).ravel())
+
+
 def test_static_compute(hip):
     d = draw(np.random.default_rng(31), 1, 150, 2, 64, 128, 1, 1, 1)
     with Graph(mem=1 << 20) as g:
