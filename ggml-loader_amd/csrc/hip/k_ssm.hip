@@ -280,18 +280,6 @@ void launch_rows(const ssm_scan_launch & L, hipStream_t st) {
 // share B and C, and (ONE_HEAD) the time step and the decay.
 constexpr int STEP_ROWS = 4;
 
-// 16 bytes at any float's address
-__device__ __forceinline__ float4 load4(const float * p) {
-    typedef float v4 __attribute__((ext_vector_type(4), aligned(4)));
-    const v4 v = *(const v4 *) p;
-    return make_float4(v[0], v[1], v[2], v[3]);
-}
-__device__ __forceinline__ void store4(float * p, float4 f) {
-    typedef float v4 __attribute__((ext_vector_type(4), aligned(4)));
-    const v4 v = { f.x, f.y, f.z, f.w };
-    *(v4 *) p = v;
-}
-
 template <int LANES, bool ONE_HEAD>
 __global__ __launch_bounds__(256) void ssm_scan_step_kernel(ssm_scan_launch L, int64_t groups) {
     const int64_t group = ((int64_t) blockIdx.x * 256 + threadIdx.x) / LANES;

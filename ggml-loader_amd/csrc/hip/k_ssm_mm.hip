@@ -94,7 +94,6 @@ struct mm_plan {
     int             nc;           // chunks
     int             n_seg, seg;   // segments, chunks per segment
     int             pooled;       // s0 is the pool
-    int             vec_bc, vec_s0, vec_s1;
     int             hw, slices, head_blocks, p_blocks;   // heads per workgroup, waves per head, ...
 };
 
@@ -104,12 +103,12 @@ template <int NK> constexpr int64_t rec_bytes() { return (int64_t) NK * 16 * 102
 // prepare
 
 // eight states of a token in the order of the products' k index: 4 from n, 4 from n + 16
-__device__ __forceinline__ void load_perm(const float * row, int n, int N, bool vec, float (&v)[8]) {
+__device__ __forceinline__ void load_perm(const float * row, int n, int N, float (&v)[8]) {
 #pragma unroll
     for (int q = 0; q < 2; q++) {
         const int k = n + 16 * q;
-        if (vec && k + 3 < N) {
-            const float4 f = *(const float4 *) (row + k);
+        if (k + 3 < N) {
+            const float4 f = load4(row + k);
             v[4 * q] = f.x; v[4 * q + 1] = f.y; v[4 * q + 2] = f.z; v[4 * q + 3] = f.w;
         } else {
 #pragma unroll
@@ -134,8 +133,8 @@ __device__ __forceinline__ void prepare_operands(const mm_plan & P, int c, int g
     float v[2][NK][8], most[2] = { 0.0f, 0.0f };
 #pragma unroll
     for (int q = 0; q < NK; q++) {
-        load_perm(cp, 32 * q + 4 * (lane / 16), L.N, P.vec_bc, v[0][q]);
-        load_perm(bp, 32 * q + 4 * (lane / 16), L.N, P.vec_bc, v[1][q]);
+        load_perm(cp, 32 * q + 4 * (lane / 16), L.N, v[0][q]);
+        load_perm(bp, 32 * q + 4 * (lane / 16), L.N, v[1][q]);
     }
 #pragma unroll
     for (int o = 0; o < 2; o++) {
@@ -358,8 +357,8 @@ __global__ __launch_bounds__(THREADS, 2) void ssm_scan_mm_kernel(mm_plan P) {
 #pragma unroll
         for (int nt = 0; nt < 2 * NK; nt++) {
             const int n = 16 * nt + 4 * grp;
-            if (P.vec_s0 && n + 3 < L.N) {
-                const float4 f = *(const float4 *) (s0 + n);
+            if (n + 3 < L.N) {
+                const float4 f = load4(s0 + n);
                 S[nt] = float4v{ f.x, f.y, f.z, f.w };
             } else {
 #pragma unroll
@@ -395,7 +394,7 @@ __global__ __launch_bounds__(THREADS, 2) void ssm_scan_mm_kernel(mm_plan P) {
 
     // what the next chunk reads
     uint4v stage_c[OUT ? STAGE : 1], stage_b[STAGE];
-    float4 gg[2][2];
+    float4v gg[2][2];
     float x[2][8], sc_next[3], st_next[(4 * STEP_WORDS + THREADS - 1) / THREADS];
     // The matrices' tiles of 16 x 16, two per wave and turn: a head has four on the diagonal, which need an
     // exponential per element, and six below it, where exp(c_t - c_j) is exp(c_t - c_b) exp(c_b - c_j), b the last
@@ -419,11 +418,11 @@ __global__ __launch_bounds__(THREADS, 2) void ssm_scan_mm_kernel(mm_plan P) {
     auto turn_of = [&](int r) { return WAVES * r + (wave + WAVES / 2 * r) % WAVES; };
     // the lane's row of a tile and its eight columns
     const int tr = lane % 16, th = lane / 16 % 2;
-    auto load_g = [&](const char * G, int turn, float4 (&v)[2]) {
+    auto load_g = [&](const char * G, int turn, float4v (&v)[2]) {
         const int pair = turn < 2 * heads ? turn % 2 : 2 + (turn - 2 * heads) % 3;
         const uint32_t at = here(lane / 32 * 1024 + lane % 32 * 16);
-        v[0] = *(const float4 *) (G + pair * 2048 + at);
-        v[1] = *(const float4 *) (G + pair * 2048 + 512 + at);
+        v[0] = *(const float4v *) (G + pair * 2048 + at);
+        v[1] = *(const float4v *) (G + pair * 2048 + 512 + at);
     };
     if (OUT) {
         // the tiles above the diagonal that the products read: blocks 0 and 3, columns 16 to 31
@@ -520,7 +519,7 @@ __global__ __launch_bounds__(THREADS, 2) void ssm_scan_mm_kernel(mm_plan P) {
                 } else if (r > 1) {
                     load_g(P.ws + P.gmat + (((int64_t) s * P.nc + c) * L.G + g) * (G_WORDS * 4), now, gg[0]);
                 }
-                const float g8[8] = { gg[0][0].x, gg[0][0].y, gg[0][0].z, gg[0][0].w, gg[0][1].x, gg[0][1].y, gg[0][1].z, gg[0][1].w };
+                const float g8[8] = { gg[0][0][0], gg[0][0][1], gg[0][0][2], gg[0][0][3], gg[0][1][0], gg[0][1][1], gg[0][1][2], gg[0][1][3] };
                 const float * st = head_steps + w.k * STEP_WORDS;
                 const float sm = scale_of(gmost * fmaxf(1.0f, st[Q - 1]));
                 const int t = 16 * w.tt + tr, j0 = 16 * w.jt + 8 * th;
@@ -783,8 +782,8 @@ __global__ __launch_bounds__(THREADS, 2) void ssm_scan_mm_kernel(mm_plan P) {
 #pragma unroll
         for (int nt = 0; nt < 2 * NK; nt++) {
             const int n = 16 * nt + 4 * grp;
-            if (P.vec_s1 && n + 3 < L.N) {
-                *(float4 *) (s1 + n) = make_float4(S[nt][0], S[nt][1], S[nt][2], S[nt][3]);
+            if (n + 3 < L.N) {
+                store4(s1 + n, make_float4(S[nt][0], S[nt][1], S[nt][2], S[nt][3]));
             } else {
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
@@ -859,8 +858,6 @@ void launch_mm(const ssm_scan_launch & L, const mm_sizes & z, void * ws, hipStre
         HIP_CHECK(hipFuncSetAttribute((const void *) ssm_scan_mm_kernel<NK, true>, hipFuncAttributeMaxDynamicSharedMemorySize, (int) lds_of(hw, true)));
         if (device < 64) lds_set.fetch_or(1ull << device, std::memory_order_relaxed);
     }
-    auto rows16 = [](const void * p, int64_t a, int64_t b, int64_t c) { return (uintptr_t) p % 16 == 0 && a % 4 == 0 && b % 4 == 0 && c % 4 == 0; };
-    P.vec_bc = rows16(L.B, L.b_g, L.b_t, L.b_s) && rows16(L.C, L.c_g, L.c_t, L.c_s);
     float * hold = (float *) ((char *) ws + z.state);
     const int64_t states = L.S * (int64_t) L.N * L.P * L.H;
     for (int64_t c = 0, turn = 0; c < z.chunks; c += z.block, turn ^= 1) {
@@ -872,8 +869,6 @@ void launch_mm(const ssm_scan_launch & L, const mm_sizes & z, void * ws, hipStre
         P.pooled = c == 0;
         P.s0 = c == 0 ? L.s : hold + (turn ^ 1) * states;
         P.s1 = c + z.block < z.chunks ? hold + turn * states : L.s_out;
-        P.vec_s0 = c == 0 ? rows16(L.s, L.s_p, L.s_h, L.s_row) : L.N % 4 == 0 && (uintptr_t) P.s0 % 16 == 0;
-        P.vec_s1 = L.N % 4 == 0 && (uintptr_t) P.s1 % 16 == 0;
         launch(ssm_prepare_kernel<NK>, dim3((unsigned) P.nc, (unsigned) (L.G + (L.H + 15) / 16), (unsigned) L.S), dim3(256),
                std::max<size_t>(OPERAND + 64, Q * 17 * 4), st, P);
         const dim3 grid((unsigned) (L.S * L.G * P.n_seg * z.head_blocks * z.p_blocks));
