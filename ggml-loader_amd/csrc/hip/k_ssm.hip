@@ -14,7 +14,8 @@ namespace {
 // The operator reads each row and writes each output once, so it is bound by memory. Two kernels, by
 // the order of the rows: channels next to each other (a projection's rows, as the executor's fused
 // form has them) need no exchange between lanes; steps next to each other (the joined rows of the
-// plain node) are turned round in LDS. A step of one token is latency: one round of loads.
+// plain node) are turned round in LDS. A step of one token is latency: one round of loads. 4096 tokens of 10240
+// channels and 4 taps: 62.9 us by rows (5.3 TB/s), 146 by tiles.
 
 __device__ __forceinline__ float silu(float v) { return v * __builtin_amdgcn_rcpf(1.0f + exp2_hw(-v * LOG2E)); }
 
@@ -22,7 +23,7 @@ template <int V> struct chunk { float v[V]; };
 template <int V> __device__ __forceinline__ chunk<V> ldv(const float * p) {
     chunk<V> c;
     if constexpr (V == 4) {
-        const float4 f = *(const float4 *) p;
+        const float4 f = load4(p);
         c.v[0] = f.x; c.v[1] = f.y; c.v[2] = f.z; c.v[3] = f.w;
     } else {
         c.v[0] = *p;
@@ -30,21 +31,18 @@ template <int V> __device__ __forceinline__ chunk<V> ldv(const float * p) {
     return c;
 }
 template <int V> __device__ __forceinline__ void stv(float * p, const chunk<V> & c) {
-    if constexpr (V == 4) *(float4 *) p = make_float4(c.v[0], c.v[1], c.v[2], c.v[3]);
+    if constexpr (V == 4) store4(p, make_float4(c.v[0], c.v[1], c.v[2], c.v[3]));
     else *p = c.v[0];
 }
 
 // Channels contiguous (x_d == 1), K taps, V channels and TT tokens per thread, all rows of a tile in
 // flight at once. The first tile's threads, the only ones that touch the state, write the new one:
 // it may be the old one's own memory.
-// PACK: filters and states contiguous and 16-byte aligned, so that a thread's four of each are whole
-// float4s (K or K - 1 of them) instead of a dword per value.
+// PACK: filters and a sequence's states contiguous, so that a thread's four of each are K or K - 1 float4s. Four
+// channels a thread only where they are: 64 tokens of 5120 channels take 5.2 us so, 5.5 with a channel each,
+// and 8.9 with four of which each loads its filter and state by dwords; 4096 tokens of 10240 62.9, 73.4 and 76.1.
 template <int K, int V, int TT, bool PACK>
-__global__ __launch_bounds__(256) void ssm_conv_rows_kernel(ssm_conv_launch L, int blocks) {
-    const int cb = (int) (blockIdx.x % (unsigned) blocks);
-    const int64_t t0 = (int64_t) (blockIdx.x / (unsigned) blocks) * TT;
-    const int64_t d = ((int64_t) cb * blockDim.x + threadIdx.x) * V;
-    if (d >= L.D) return;
+__device__ __forceinline__ void conv_rows(const ssm_conv_launch & L, int64_t t0, int64_t d) {
     float w[V][K];
     if constexpr (PACK) {
 #pragma unroll
@@ -140,6 +138,16 @@ __global__ __launch_bounds__(256) void ssm_conv_rows_kernel(ssm_conv_launch L, i
     }
 }
 
+// V channels a thread; the ones that are left over have a thread each, in a wave of their own: in the last
+// wave of the others they would wait for those (777 tokens of 2558 channels 7.9 us, and 7.0 with a thread a channel)
+template <int K, int V, int TT, bool PACK>
+__global__ __launch_bounds__(256) void ssm_conv_rows_kernel(ssm_conv_launch L, int blocks) {
+    const int64_t t0 = (int64_t) (blockIdx.x / (unsigned) blocks) * TT;
+    const int64_t i = (int64_t) (blockIdx.x % (unsigned) blocks) * blockDim.x + threadIdx.x, whole = L.D / V, rest = (whole + 63) / 64 * 64;
+    if (i < whole) conv_rows<K, V, TT, PACK>(L, t0, i * V);
+    else if (V > 1 && i >= rest && i < rest + L.D % V) conv_rows<K, 1, TT, false>(L, t0, i - rest + whole * V);
+}
+
 // Rows in any order: 64 channels by 64 tokens and the K - 1 rows before them through LDS, read with
 // the steps across the lanes and used with the channels across them. An odd row length keeps the
 // lanes' reads on different banks.
@@ -192,7 +200,7 @@ __global__ __launch_bounds__(256) void ssm_conv_tile_kernel(ssm_conv_launch L, i
 
 template <int K, int V, bool PACK>
 void launch_conv_rows(const ssm_conv_launch & L, hipStream_t st) {
-    const int64_t groups = (L.D + V - 1) / V;
+    const int64_t groups = L.D % V ? (L.D / V + 63) / 64 * 64 + L.D % V : L.D / V;
     const int threads = (int) std::min<int64_t>(256, (groups + 63) / 64 * 64);
     const int blocks = (int) ((groups + threads - 1) / threads);
     const unsigned gy = (unsigned) std::min<int64_t>(L.S, 65535);
@@ -203,11 +211,8 @@ void launch_conv_rows(const ssm_conv_launch & L, hipStream_t st) {
 
 template <int K>
 void launch_conv_rows(const ssm_conv_launch & L, hipStream_t st) {
-    const bool wide = L.D % 4 == 0 && L.x_t % 4 == 0 && L.x_s % 4 == 0 && ((uintptr_t) L.x | (uintptr_t) L.y | (uintptr_t) L.bias) % 16 == 0;
-    const bool pack = wide && L.w_k == 1 && L.w_d == K && (K == 1 || (L.st_j == 1 && L.st_d == K - 1 && L.st_s % 4 == 0)) &&
-                      ((uintptr_t) L.w | (K == 1 ? 0 : (uintptr_t) L.state | (uintptr_t) L.new_state)) % 16 == 0;
+    const bool pack = L.w_k == 1 && L.w_d == K && (K == 1 || (L.st_j == 1 && L.st_d == K - 1));
     if (pack) launch_conv_rows<K, 4, true>(L, st);
-    else if (wide) launch_conv_rows<K, 4, false>(L, st);
     else launch_conv_rows<K, 1, false>(L, st);
 }
 
@@ -277,7 +282,8 @@ void launch_rows(const ssm_scan_launch & L, hipStream_t st) {
 
 // A few tokens (decoding): the states are most of what is read and written, so a lane takes them 16 bytes
 // at a time and STEP_ROWS channels at once. LANES lanes hold a channel's 4 LANES states; the group's channels
-// share B and C, and (ONE_HEAD) the time step and the decay.
+// share B and C, and (ONE_HEAD) the time step and the decay. 32 sequences of 80 heads of 64 channels and 128
+// states: 35 us a token, 4.8 TB/s of states; on the same states again 26.6, and 75 by the kernel for any operands.
 constexpr int STEP_ROWS = 4;
 
 template <int LANES, bool ONE_HEAD>
@@ -365,7 +371,7 @@ void launch_step(const ssm_scan_launch & L, hipStream_t st) {
 // channels and 16 states took 32 us a token, with it 12.1, 4.8 TB/s; the kernel for few tokens took 15.7).
 // Where channels alone are too few waves the tokens are split into segments: `local` finds each segment's final
 // state from nothing and its sum of time steps, `join` the state that each begins with, and the last launch the
-// outputs (72 us at 1500 tokens of 5120 channels: 28, 5 and 36). The first pass repeats 7/8 of the work;
+// outputs (74 us at 1500 tokens of 5120 channels: 29, 10 and 38). The first pass repeats 7/8 of the work;
 // carrying its outputs over would take as many exponentials again.
 struct chan_plan {
     ssm_scan_launch L;

@@ -31,7 +31,8 @@ GGML_API ggml_backend_buffer_type_t ggml_backend_hip_buffer_type(int device);
 
 // ggml_backend_graph_compute without any device allocation: no counterpart in the reference; for
 // callers that cannot allocate (serving loops, harnesses that forbid hipMalloc). The kernels'
-// scratch (attention scores and partials, quantized activations, expert groups, argmax parts)
+// scratch (attention scores and partials, quantized activations, expert groups, argmax parts, scans'
+// prepared operands and segment states: up to 96 MiB and two copies of the sequences' states)
 // comes from a file-scope device array of GGML_HIP_STATIC_SCRATCH_BYTES that every GPU the
 // library runs on holds until the process ends; the graph's tensors are the caller's as with
 // ggml_backend_graph_compute, and the result is the same. Like ggml_backend_graph_compute it
@@ -87,7 +88,8 @@ GGML_API enum ggml_status ggml_backend_hip_sample(ggml_backend_t backend, const 
 // not finite); its ids are still ordered (NaN as -inf). Any of the four outputs may be NULL (not
 // wanted); tokens may be NULL without logprob. n_top is 0 (no alternatives) to
 // GGML_HIP_LOGPROBS_MAX_TOP, at most the row length. Synchronous, on the backend's stream: returns
-// when the outputs are on the host. Fails (GGML_STATUS_FAILED, with a message on stderr, and no
+// when the outputs are on the host; calls on one device share its scratch (not from two threads at
+// once). Fails (GGML_STATUS_FAILED, with a message on stderr, and no
 // output written) for another backend or buffer, rows or tokens out of range, or a bad n_top.
 #define GGML_HIP_LOGPROBS_MAX_TOP 128
 GGML_API enum ggml_status ggml_backend_hip_logprobs(ggml_backend_t backend, const struct ggml_tensor * logits, int64_t row,

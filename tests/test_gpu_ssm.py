@@ -239,6 +239,7 @@ class Mixer:
 @pytest.mark.parametrize("fusion", [True, False])
 @pytest.mark.parametrize("in_place", [False, True])
 @pytest.mark.parametrize("K, T, D, S, W, bias, act", [
+    (4, 1, 21, 3, 25, True, True), (3, 40, 259, 2, 261, True, True), (4, 9, 2, 1, 7, True, False), (2, 3, 1027, 2, 1027, False, True),
     (4, 1, 8, 1, 8, True, True), (4, 1, 260, 7, 300, True, True), (4, 2, 65, 2, 65, True, True), (4, 3, 64, 3, 70, False, True),
     (4, 64, 64, 1, 128, True, True), (4, 67, 130, 2, 131, True, True), (2, 5, 33, 1, 40, True, True), (3, 200, 512, 1, 1100, False, True),
     (4, 300, 1000, 1, 1000, True, False), (6, 4, 20, 2, 20, True, True), (9, 70, 70, 2, 71, True, True),
