@@ -503,14 +503,17 @@ const char * node_refusal(const ggml_tensor * n) {
     return nullptr;
 }
 
-bool graph_refused(const ggml_cgraph * g) {
+bool graph_refused(const ggml_cgraph * g, int device) {
     for (int i = 0; i < g->n_nodes; i++) {
         const ggml_tensor * n = g->nodes[i];
         const char * why = node_refusal(n);
         if (!why && (n->op == GGML_OP_SSM_CONV || n->op == GGML_OP_SSM_SCAN)) {
             for (int s = -1; s < GGML_MAX_SRC; s++) {
                 const ggml_tensor * t = s < 0 ? n : n->src[s];
-                if (t && !t->data && ggml_nelements(t) > 0) why = "an operand is not allocated";
+                if (!t || ggml_nelements(t) == 0) continue;
+                const ggml_backend_buffer_t buf = t->view_src ? t->view_src->buffer : t->buffer;
+                if (!t->data) why = "an operand is not allocated";
+                else if (buf && ggml_backend_buffer_get_type(buf) != ggml_backend_hip_buffer_type(device)) why = "an operand is not in this device's memory";
             }
         }
         if (!why) continue;
@@ -2548,8 +2551,8 @@ void collect_profile(hip_backend_ctx * c) {
 
 // queues the graph's kernels on the device stream; a timed (profiled) compute also waits for them
 enum ggml_status be_compute_async(ggml_backend_t b, ggml_cgraph * g) {
-    if (graph_refused(g)) return GGML_STATUS_FAILED;
     hip_backend_ctx * c = (hip_backend_ctx *) b->context;
+    if (graph_refused(g, c->device)) return GGML_STATUS_FAILED;
     hip_device & d = dev(c->device);
     c->timing = c->profiling && (c->computes++ % c->profile_every) == 0;
     const auto t0 = std::chrono::steady_clock::now();
@@ -2597,7 +2600,7 @@ enum ggml_status compute_static(hip_backend_ctx * c, ggml_cgraph * g) {
         fprintf(stderr, "ggml-hip: graph_compute_static: profiling creates events; turn it off first\n");
         return GGML_STATUS_FAILED;
     }
-    if (graph_refused(g)) return GGML_STATUS_FAILED;
+    if (graph_refused(g, c->device)) return GGML_STATUS_FAILED;
     scratch_arena own = std::move(c->scratch);
     c->scratch = scratch_arena{};
     c->scratch.fixed = true;

@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 
 import ssm_ref
-from gl import Graph, gl, ptr
+from gl import Graph, cpu_backend, gl, ptr
 
 pytestmark = pytest.mark.gpu
 
@@ -360,3 +360,18 @@ def test_refused_graphs_run_nothing(hip, capfd):
         assert gl.libs()["hip"].ggml_backend_hip_graph_compute_static(hip, gf) == -1
         assert not g.read(b).any()
     assert "version 1 only" in capfd.readouterr().err
+
+
+def test_refuses_memory_of_another_backend(hip, capfd):
+    """Operands in host memory are named, not read."""
+    cpu = cpu_backend(1)
+    d = draw(np.random.default_rng(6), 1, 2, 2, 4, 8, 1, 1, 1)
+    with Graph(mem=1 << 20) as g:
+        n = scan_node(g, d)
+        gf = g.core.ggml_new_graph(g.ctx)
+        g.core.ggml_build_forward_expand(gf, n)
+        g.buf = g.core.ggml_backend_alloc_ctx_tensors(g.ctx, cpu)
+        assert g.core.ggml_backend_graph_compute(hip, gf) == -1
+        assert gl.libs()["hip"].ggml_backend_hip_graph_compute_static(hip, gf) == -1
+    gl.libs()["core"].ggml_backend_free(cpu)
+    assert "not in this device's memory" in capfd.readouterr().err
