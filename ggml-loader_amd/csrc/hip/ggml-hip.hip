@@ -376,7 +376,7 @@ enum fuse_bits {
     FUSE_ROUTEG = 1024, // one token's MoE routing inside its routed gate/up GEMV launch
     FUSE_ACCO   = 2048, // one-query attention output accumulated by PV, read as doubles by its GEMVs
     FUSE_WSUMQ  = 4096, // MoE weighted sum also writes the next rms_norm * w as Q8_K (several tokens)
-    FUSE_SSM    = 8192, // state rows joined, convolution, bias, SiLU and the new state in one launch
+    FUSE_SSM    = 8192, // state rows joined, convolution, bias, SiLU and the new state in one launch; a scan and its states' copy
     FUSE_ALL    = 16383,
 };
 
@@ -1078,6 +1078,49 @@ private:
         return true;
     }
 
+    // no view of node i's value, or of a view of it, reaches past `end`
+    bool views_below(int i, const char * end) const {
+        for (int u : users_[i]) {
+            if (is_view_op(g_->nodes[u]->op) && (span_of(g_->nodes[u]).e > end || !views_below(u, end))) return false;
+        }
+        return true;
+    }
+
+    // The copy of a scan's final states, all of them in order, that the scan's launch makes by writing them where
+    // the copy goes (the view and the copy are then done), or nullptr. The pool's own memory can take them where the
+    // pool is one sequence's only row and each state is written by the thread that read it or in a later
+    // launch: not by products, whose segments all read the first states.
+    const ggml_tensor * scan_state_copy(const ggml_tensor * n, const ssm_scan_launch & L) {
+        const int i = node_index(n);
+        if (!fuse(FUSE_SSM) || c_.cb || i < 0 || is_output(i)) return nullptr;
+        const ggml_tensor * s = n->src[0];
+        const char * from = (const char *) L.s_out;
+        int view = -1;
+        for (int u : users_[i]) {
+            const ggml_tensor * t = g_->nodes[u];
+            if (t->op != GGML_OP_VIEW) return nullptr;
+            if (span_of(t).e <= from) {
+                if (!views_below(u, from)) return nullptr;
+            } else if (view < 0 && t->data == (const void *) from && t->type == GGML_TYPE_F32 && ggml_is_contiguous(t) &&
+                       ggml_nelements(t) == L.S * L.N * L.P * L.H) {
+                view = u;
+            } else {
+                return nullptr;
+            }
+        }
+        const int copy = sole_user(view);
+        if (copy < 0) return nullptr;
+        const ggml_tensor * cp = g_->nodes[copy];
+        if (cp->op != GGML_OP_CPY || cp->src[0] != g_->nodes[view] || cp->type != GGML_TYPE_F32 || !ggml_is_contiguous(cp) || overlap(cp, n)) return nullptr;
+        for (int k = 1; k < 7; k++) {
+            if (overlap(cp, n->src[k])) return nullptr;
+        }
+        if (overlap(cp, s) && !(L.S == 1 && L.pool == 1 && cp->data == s->data && ggml_is_contiguous(s) && !ssm_scan_mm_takes(L))) return nullptr;
+        if (!may_write_early(i, copy, cp, { view, copy })) return nullptr;
+        done_[view] = done_[copy] = true;
+        return cp;
+    }
+
     void op_ssm_scan(ggml_tensor * n) {
         const ggml_tensor * s = n->src[0], * x = n->src[1], * dt = n->src[2], * A = n->src[3], * B = n->src[4], * C = n->src[5],
                           * ids = n->src[6];
@@ -1095,6 +1138,10 @@ private:
         L.ids = (const int32_t *) ids->data; L.ids_s = nb(ids, 0);
         L.y = (float *) n->data;
         L.s_out = L.y + ggml_nelements(x);
+        if (const ggml_tensor * cp = scan_state_copy(n, L)) {
+            L.s_out = (float *) cp->data;
+            wrote_.push_back(cp);
+        }
         const double st = (double) L.N * L.P * L.H * L.S * 4;
         prof_scope ps(this, "ssm_scan", 2 * st + 4.0 * (2 * ggml_nelements(x) + ggml_nelements(dt) + 2 * ggml_nelements(B)));
         // one buffer for the graph's scans, which the stream runs one after another

@@ -524,7 +524,8 @@ bool channels_take(const ssm_scan_launch & L) {
 // One segment, or enough for four waves of every SIMD, of 8 tokens at least. With w waves of channels a token
 // takes 0.4 us in one piece (up to a wave per SIMD); split, about w / 820 of that, the first pass's work included,
 // and 12 us more. 80 waves (5120 channels): 32 tokens 15.7 us in one piece and 17.0 split, 48 tokens 21.9 and
-// 17.5; 640 waves: 54 tokens 26.6 and 40.1.
+// 17.5; 640 waves: 54 tokens 26.6 and 40.1. Two, three, four and six waves of every SIMD: 1500 tokens of 5120 channels
+// 82, 73.5, 75 and 79 us, of 8192 117, 104, 99 and 102.
 void chan_segments(const ssm_scan_launch & L, chan_plan & P) {
     const int64_t waves = (L.H + 63) / 64 * L.S;
     int64_t n = 1;

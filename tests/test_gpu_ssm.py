@@ -362,6 +362,57 @@ def test_refused_graphs_run_nothing(hip, capfd):
     assert "version 1 only" in capfd.readouterr().err
 
 
+def run_with_state_copy(hip, d, kind, fusion):
+    """y and the memory the final states are copied to; `kind`: what else the graph does with either."""
+    S, T, H, P = d["x"].shape
+    pool, _, _, N = d["state"].shape
+    one = H * P * N
+    gl.libs()["hip"].ggml_backend_hip_set_fusion(hip, fusion)
+    try:
+        with Graph(mem=1 << 20) as g:
+            n = scan_node(g, d)
+            s = n.contents.src[0]
+            y = g.view_1d(n, S * T * H * P, 0)
+            states = g.view_1d(n, S * one, S * T * H * P * 4)
+            other = g.tensor(gl.F32, S * one, data=np.zeros(S * one, np.float32))
+            to = {"apart": other, "read_between": other}.get(kind)
+            if to is None:
+                to = g.view_1d(s, S * one, 0)
+            outs = [g.scale(y, 1.0)]
+            if kind == "old":
+                outs.append(g.scale(g.reshape_2d(s, N * P, H * pool), 2.0))       # the pool's old rows, read after the scan
+            if kind == "read_between":
+                outs.append(g.scale(other, 2.0))
+            if kind == "states":
+                outs.append(g.scale(states, 3.0))
+            if kind == "across":
+                outs.append(g.scale(g.view_1d(n, 2 * H * P, max(S * T * H * P - H * P, 0) * 4), 2.0))
+            copy = g.cpy(states, to)
+            got = g.compute(hip, outs + [copy])
+            return got, g.read(s)
+    finally:
+        gl.libs()["hip"].ggml_backend_hip_set_fusion(hip, True)
+
+
+@pytest.mark.parametrize("kind", ["pool", "apart", "old", "read_between", "states", "across"])
+@pytest.mark.parametrize("S, T, H, P, N, G, pool, a0", [
+    (1, 1, 4, 64, 128, 2, 1, 1), (1, 5, 3, 3, 20, 1, 1, 20), (1, 100, 4, 64, 128, 1, 1, 1), (1, 1000, 4, 64, 128, 1, 1, 1),
+    (1, 1, 130, 1, 16, 1, 1, 16), (1, 300, 130, 1, 16, 1, 1, 16), (1, 3, 5, 2, 7, 1, 1, 1), (3, 1, 4, 64, 128, 2, 3, 1),
+    (3, 2, 65, 1, 16, 1, 4, 16), (2, 200, 4, 32, 64, 1, 2, 1)])
+def test_scan_with_its_state_copied(hip, S, T, H, P, N, G, pool, a0, kind):
+    """The copy of the final states into the pool or elsewhere, with and without fusion: the same values,
+    whatever else reads the states, the old ones, or the memory that they go to."""
+    d = draw(np.random.default_rng(S + T + H + N), S, T, H, P, N, G, pool, a0)
+    want, pool_want = run_with_state_copy(hip, d, kind, False)
+    got, pool_got = run_with_state_copy(hip, d, kind, True)
+    for a, b in zip(got, want):
+        assert np.array_equal(a, b)
+    assert np.array_equal(pool_got, pool_want)
+    y, h, ye, he = ssm_ref.scan(d["state"][d["ids"]], d["x"], d["dt"], d["A"], d["B"], d["C"])
+    near(got[0], y, ye)
+    near(got[-1], h, he)
+
+
 def test_refuses_memory_of_another_backend(hip, capfd):
     """Operands in host memory are named, not read."""
     cpu = cpu_backend(1)
