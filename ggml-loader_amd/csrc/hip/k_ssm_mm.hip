@@ -21,7 +21,7 @@
 // before joined, then the chunks one after another. A wave holds the states of 16 channels of a head in registers
 // for its whole segment: the instruction that updates them leaves state n of channel p in the lane that the next
 // chunk's product reads it from, when the k index of that product runs n = 4 g + i, then 16 + 4 g + i over lane
-// group g, the order that C is prepared in. Eight waves share a chunk's operands, loaded a chunk ahead.
+// group g, the order that C is prepared in. Eight waves share a chunk's operands.
 //
 // 4096 tokens of 128 heads x 64 x 128, 8 groups: 180 us (1.73 TB/s of what must be read and written, whose floor
 // is 61 us; 22 + 41 + 122 in a trace), 333 tokens of 24 heads 32. Nothing is saturated: the matrix cores are busy
@@ -299,8 +299,8 @@ __device__ __forceinline__ float column_max(float m) {
 }
 
 // NK: steps of 32 states; OUT: outputs and final states, else the segment's state from nothing.
-// Everything a chunk reads is loaded into registers while the chunk before it is computed: its operands'
-// planes (on to LDS at the chunk's end: C's over the last one's, B's beside it), the inputs, C_t . B_j and the
+// What a chunk reads is loaded into registers while the chunk before it is computed: its operands'
+// planes (EARLY; on to LDS at the chunk's end: C's over the last one's, B's beside it), the inputs, C_t . B_j and the
 // heads' exponentials. Two barriers a chunk: LDS is written; C is read and the matrices are written.
 template <int NK, bool OUT>
 __global__ __launch_bounds__(THREADS, 2) void ssm_scan_mm_kernel(mm_plan P) {
@@ -393,7 +393,11 @@ __global__ __launch_bounds__(THREADS, 2) void ssm_scan_mm_kernel(mm_plan P) {
     }
 
     // what the next chunk reads
-    uint4v stage_c[OUT ? STAGE : 1], stage_b[STAGE];
+    // The operands' planes a chunk ahead too, or only once the chunk before is done: the registers that hold them are
+    // those that outputs of 128 and more states lack. 3 x 1625 tokens of 36 x 64 x 64 63.7 us ahead and 66.8 late;
+    // 1402 of 64 x 80 x 128 67.5 and 66.1; 3 x 586 of 30 x 128 x 256 128 (94 registers spilled) and 96.
+    constexpr bool EARLY = !OUT || NK < 4;
+    uint4v stage_c[OUT && EARLY ? STAGE : 1], stage_b[EARLY ? STAGE : 1];
     float4v gg[2][2];
     float x[2][8], sc_next[3], st_next[(4 * STEP_WORDS + THREADS - 1) / THREADS];
     // The matrices' tiles of 16 x 16, two per wave and turn: a head has four on the diagonal, which need an
@@ -442,11 +446,13 @@ __global__ __launch_bounds__(THREADS, 2) void ssm_scan_mm_kernel(mm_plan P) {
     const int64_t x_on = Q * 4 * L.x_t, steps_on = (int64_t) L.H * (STEP_WORDS * 4);
     auto fetch = [&](int c) {
         const int left = P.T - c * Q;
-        const uint32_t piece = here(tid * 16);
+        if constexpr (EARLY) {
+            const uint32_t piece = here(tid * 16);
 #pragma unroll
-        for (int q = 0; q < STAGE; q++) {
-            if (OUT) stage_c[q] = *(const uint4v *) (at_planes + q * THREADS * 16 + piece);
-            stage_b[q] = *(const uint4v *) (at_planes + OPERAND + q * THREADS * 16 + piece);
+            for (int q = 0; q < STAGE; q++) {
+                if (OUT) stage_c[q] = *(const uint4v *) (at_planes + q * THREADS * 16 + piece);
+                stage_b[q] = *(const uint4v *) (at_planes + OPERAND + q * THREADS * 16 + piece);
+            }
         }
 #pragma unroll
         for (int q = 0; q < (4 * STEP_WORDS + THREADS - 1) / THREADS; q++)
@@ -484,10 +490,24 @@ __global__ __launch_bounds__(THREADS, 2) void ssm_scan_mm_kernel(mm_plan P) {
     };
     // and on to LDS
     auto put = [&](int turn) {
+        if constexpr (EARLY) {
 #pragma unroll
-        for (int q = 0; q < STAGE; q++) {
-            if (OUT) *(uint4v *) (cbuf + (tid + q * THREADS) * 16) = stage_c[q];
-            *(uint4v *) (bbuf + turn % SLOTS * OPERAND + (tid + q * THREADS) * 16) = stage_b[q];
+            for (int q = 0; q < STAGE; q++) {
+                if (OUT) *(uint4v *) (cbuf + (tid + q * THREADS) * 16) = stage_c[q];
+                *(uint4v *) (bbuf + turn % SLOTS * OPERAND + (tid + q * THREADS) * 16) = stage_b[q];
+            }
+        } else {
+            // C's planes, then B's, in the record
+            const char * planes = at_planes - L.G * rec_bytes<NK>() + tid * 16;
+            char * to[2] = { cbuf + tid * 16, bbuf + turn % SLOTS * OPERAND - OPERAND + tid * 16 };
+#pragma unroll
+            for (int q0 = 0; q0 < 2 * STAGE; q0 += 8) {
+                uint4v piece[8];
+#pragma unroll
+                for (int q = 0; q < 8; q++) piece[q] = *(const uint4v *) (planes + (q0 + q) * THREADS * 16);
+#pragma unroll
+                for (int q = 0; q < 8; q++) *(uint4v *) (to[q0 + q >= STAGE] + (q0 + q) * THREADS * 16) = piece[q];
+            }
         }
 #pragma unroll
         for (int q = 0; q < (4 * STEP_WORDS + THREADS - 1) / THREADS; q++) {
@@ -878,12 +898,12 @@ void launch_mm(const ssm_scan_launch & L, const mm_sizes & z, void * ws, hipStre
 }
 
 // Up to so many tokens the recurrence itself is faster: products need an operand and a chunk's latency, 12 us with
-// 32 states, 20 with 128 and 36 with 256, and a step takes 0.5 to 0.6 us. 80 heads of 64 channels and 128 states: 16
+// 32 states, 20 with 128 and 31 with 256, and a step takes 0.5 to 0.6 us. 80 heads of 64 channels and 128 states: 16
 // tokens 13.1 us by steps and 20.6 by products, 24 17.8 and 20.8, 32 22.5 and 20.8; 24 heads of 32 states 16 tokens
-// 11.2 and 12.6, 24 15.3 and 12.6; of 256 states 48 tokens 36.4 and 36.6. Where channels fill the chip a step takes
+// 11.2 and 12.6, 24 15.3 and 12.6; of 256 states 32 tokens 25.6 and 31.2, 48 36.3 and 31.6. Where channels fill the chip a step takes
 // longer and the latency doesn't count: 163840 channels of 128 states 16 tokens 75.7 and 80.6, 24 106.8 and 80.8.
 int step_tokens(const ssm_scan_launch & L) {
-    const int few = L.N <= 64 ? 16 : L.N <= 128 ? 24 : 48;
+    const int few = L.N <= 64 ? 16 : L.N <= 128 ? 24 : 40;
     return L.S * (int64_t) L.H * L.P > 65536 ? few * 2 / 3 : few;
 }
 
