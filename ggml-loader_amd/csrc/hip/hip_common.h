@@ -114,6 +114,18 @@ __device__ __forceinline__ float group_sum(float v) {
     return v;
 }
 
+// 16 bytes at any float's address
+__device__ __forceinline__ float4 load4(const float * p) {
+    typedef float v4 __attribute__((ext_vector_type(4), aligned(4)));
+    const v4 v = *(const v4 *) p;
+    return make_float4(v[0], v[1], v[2], v[3]);
+}
+__device__ __forceinline__ void store4(float * p, float4 f) {
+    typedef float v4 __attribute__((ext_vector_type(4), aligned(4)));
+    const v4 v = { f.x, f.y, f.z, f.w };
+    *(v4 *) p = v;
+}
+
 template <int G>
 __device__ __forceinline__ float group_max(float v) {
     if (G >= 2) v = fmaxf(v, dpp_f<0xB1>(v));

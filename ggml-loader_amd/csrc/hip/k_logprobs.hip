@@ -238,7 +238,6 @@ __device__ __forceinline__ void store_row(const logprobs_launch & L, int r, cons
 }
 
 // One segment of one row. Where it is the whole row the results are final, else they go to the scratch.
-template <bool VEC>
 __global__ __launch_bounds__(LP_THREADS) void logprobs_segment_kernel(logprobs_launch L) {
     __shared__ lp_shared S;
     __shared__ lp_out o;
@@ -249,8 +248,8 @@ __global__ __launch_bounds__(LP_THREADS) void logprobs_segment_kernel(logprobs_l
 #pragma unroll
     for (int j = 0; j < LP_PER / 4; j++) {
         const int i = j * (LP_THREADS * 4) + tid * 4;
-        if (VEC && i + 3 < valid) {
-            const float4 f = *(const float4 *) (x + i);
+        if (i + 3 < valid) {
+            const float4 f = load4(x + i);
             v[4 * j] = f.x; v[4 * j + 1] = f.y; v[4 * j + 2] = f.z; v[4 * j + 3] = f.w;
         } else {
 #pragma unroll
@@ -375,11 +374,11 @@ int64_t logprobs_scratch_bytes(int n, int k, int n_rows) {
 void launch_logprobs(const logprobs_launch & L0, hipStream_t st) {
     logprobs_launch L = L0;
     L.n_seg = segments(L.n);
-    // even segments, of whole rows of 1024 entries
-    L.seg = std::min(LP_SEG, ((L.n + L.n_seg - 1) / L.n_seg + LP_THREADS * 4 - 1) / (LP_THREADS * 4) * (LP_THREADS * 4));
+    // even segments: a short one's best entries would let the join keep most of the others' lists (5 rows of 132883,
+    // 42 entries: 40 us, and 33 so)
+    L.seg = ((L.n + L.n_seg - 1) / L.n_seg + 3) / 4 * 4;
     L.n_seg = (L.n + L.seg - 1) / L.seg;
-    const bool vec = ((uintptr_t) L.base | (uintptr_t) L.nb1 | (uintptr_t) L.nb2 | (uintptr_t) L.nb3) % 16 == 0;
-    launch(vec ? logprobs_segment_kernel<true> : logprobs_segment_kernel<false>, dim3((unsigned) L.n_seg, (unsigned) L.n_rows),
+    launch(logprobs_segment_kernel, dim3((unsigned) L.n_seg, (unsigned) L.n_rows),
            dim3(LP_THREADS), 0, st, L);
     if (L.n_seg > 1) {
         const size_t lds = ((size_t) L.n_seg * L.k + 3) * 8;

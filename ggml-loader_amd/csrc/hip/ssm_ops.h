@@ -8,18 +8,6 @@ constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 // 2^x by the hardware's instruction, off by at most one unit
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// 16 bytes at any float's address
-__device__ __forceinline__ float4 load4(const float * p) {
-    typedef float v4 __attribute__((ext_vector_type(4), aligned(4)));
-    const v4 v = *(const v4 *) p;
-    return make_float4(v[0], v[1], v[2], v[3]);
-}
-__device__ __forceinline__ void store4(float * p, float4 f) {
-    typedef float v4 __attribute__((ext_vector_type(4), aligned(4)));
-    const v4 v = { f.x, f.y, f.z, f.w };
-    *(v4 *) p = v;
-}
-
 // log(1 + e^x) = max(x, 0) + log1p(u), u = e^-|x|, with log1p(u) = 2 atanh(s), s = u / (2 + u) <= 1/3, as
 // its series: nine terms leave 3^-19 / 19 < 2^-34 of s. u keeps the rounding of |x| log2(e) as a factor.
 // Within four units over all x, and below -88, where u underflows, 0.
