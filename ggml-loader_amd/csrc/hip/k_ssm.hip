@@ -371,7 +371,7 @@ void launch_step(const ssm_scan_launch & L, hipStream_t st) {
 // channels and 16 states took 32 us a token, with it 12.1, 4.8 TB/s; the kernel for few tokens took 15.7).
 // Where channels alone are too few waves the tokens are split into segments: `local` finds each segment's final
 // state from nothing and its sum of time steps, `join` the state that each begins with, and the last launch the
-// outputs (74 us at 1500 tokens of 5120 channels: 29, 10 and 38). The first pass repeats 7/8 of the work;
+// outputs (73.5 us at 1500 tokens of 5120 channels: 28, 10 and 37). The first pass repeats 7/8 of the work;
 // carrying its outputs over would take as many exponentials again.
 struct chan_plan {
     ssm_scan_launch L;

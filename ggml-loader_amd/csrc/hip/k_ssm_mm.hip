@@ -23,13 +23,13 @@
 // chunk's product reads it from, when the k index of that product runs n = 4 g + i, then 16 + 4 g + i over lane
 // group g, the order that C is prepared in. Eight waves share a chunk's operands.
 //
-// 4096 tokens of 128 heads x 64 x 128, 8 groups: 180 us (1.73 TB/s of what must be read and written, whose floor
-// is 61 us; 22 + 41 + 122 in a trace), 333 tokens of 24 heads 32. Nothing is saturated: the matrix cores are busy
+// 4096 tokens of 128 heads x 64 x 128, 8 groups: 178 us (1.76 TB/s of what must be read and written, whose floor
+// is 61 us; 22 + 40 + 119 in a trace), 333 tokens of 24 heads 32. Nothing is saturated: the matrix cores are busy
 // for a fifth of the time, the vector units for two fifths and LDS for a quarter, and leaving any one part out
 // (the loads of x or of the operands, the update of the state, the stores) saves a tenth each, so a chunk's
 // barriers and the latency between its parts are what is left. Two tiles of channels a wave (166 us for the last
 // launch), workgroups of four waves (159), four waves a SIMD with one buffer (spills), and half the waves a step
-// ahead of the others (149) were all slower than its 122 to 126.
+// ahead of the others (149) were all slower than its 119 to 126.
 //
 // A value that is not finite must not reach earlier tokens of its chunk through 0 times it: X is
 // cleared of such values, and the channel's outputs from that token on, and its state, are NaN. (B, C
