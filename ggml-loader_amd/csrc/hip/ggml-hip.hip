@@ -2885,9 +2885,11 @@ enum ggml_status ggml_backend_hip_logprobs(ggml_backend_t backend, const struct 
     }
     hip_device & d = dev(c->device);
     // so many rows at a time: their tokens fit an upload slot, their results the download area (the kernels
-    // read and write both in place) and their parts 64 MiB
-    const int64_t part = std::max<int64_t>(logprobs_scratch_bytes((int) n, n_top, 1), 1);
-    const int64_t step = std::min<int64_t>(LOGPROBS_ROWS, std::max<int64_t>(1, ((int64_t) 64 << 20) / part));
+    // read and write both in place) and their parts LOGPROBS_PART
+    static_assert(logprobs_rows(0, 0, DOWN_MAX) == LOGPROBS_ROWS && LOGPROBS_ROWS * sizeof(int32_t) <= UP_SMALL, "tokens fit a slot");
+    static_assert(logprobs_rows(0, LOGPROBS_MAX_TOP, DOWN_MAX) * (2 + 2 * LOGPROBS_MAX_TOP) * 4 <= DOWN_MAX, "results fit the area");
+    static_assert(LOGPROBS_MAX_TOP == GGML_HIP_LOGPROBS_MAX_TOP, "one limit");
+    const int64_t step = logprobs_rows(logprobs_scratch_bytes((int) n, n_top, 1), n_top, DOWN_MAX);
     const int width = 2 + 2 * n_top;
     for (int64_t r0 = 0; r0 < n_rows; r0 += step) {
         const int nr = (int) std::min(step, n_rows - r0);
@@ -2907,9 +2909,10 @@ enum ggml_status ggml_backend_hip_logprobs(ggml_backend_t backend, const struct 
                 drained(d);
                 slot = upload_slot(d, nr * 4);
             }
-            memcpy(slot, tokens + r0, nr * 4);
+            if (slot) memcpy(slot, tokens + r0, nr * 4);
         }
         float * area = (float *) download_area(d, (size_t) nr * width * 4);
+        if ((tokens && !slot) || !area) return fail("no room for a launch's tokens and results");
         logprobs_launch L{};
         L.base = (const char *) logits->data;
         L.ne1 = logits->ne[1]; L.ne2 = logits->ne[2];

@@ -604,8 +604,14 @@ void launch_ssm_scan_mm(const ssm_scan_launch & L, void * ws, hipStream_t st);
 // probability of the row's token (0 where tokens is null), the entropy, k ids (I32), k log
 // probabilities. part: logprobs_scratch_bytes. tokens (or null): device or host-visible ids below n.
 constexpr int LOGPROBS_MAX_TOP = 128;
-// rows per launch: 64 KiB of tokens, and results of at most 16 MiB (the download area) at 128 alternatives
-constexpr int LOGPROBS_ROWS = 16384;
+constexpr int LOGPROBS_ROWS = 16384;                         // rows per launch, for 64 KiB of tokens
+constexpr int64_t LOGPROBS_PART = (int64_t) 64 << 20;        // their parts
+// rows per launch: `part` bytes of scratch a row, and results of 2 + 2 k words a row in an area of `area` bytes
+constexpr int64_t logprobs_rows(int64_t part, int k, int64_t area) {
+    const int64_t scratch = part > 0 ? LOGPROBS_PART / part : LOGPROBS_ROWS, results = area / ((2 + 2 * (int64_t) k) * 4);
+    const int64_t rows = scratch < results ? scratch : results;
+    return rows < 1 ? 1 : rows < LOGPROBS_ROWS ? rows : LOGPROBS_ROWS;
+}
 struct logprobs_launch {
     const char *    base;
     int64_t         ne1, ne2, nb1, nb2, nb3;

@@ -194,6 +194,13 @@ def test_more_rows_than_a_launch_takes(hip):
     check(hip, x, rng.integers(0, 12, len(x)), 2)
 
 
+def test_more_alternatives_than_the_download_area_holds(hip):
+    """128 alternatives of each of 16384 + 70 rows are more than the pinned area's 16 MiB."""
+    rng = np.random.default_rng(7)
+    x = rng.standard_normal((16384 + 70, 130)).astype(np.float32)
+    check(hip, x, rng.integers(0, 130, len(x)), 128)
+
+
 def test_refuses_another_buffer(hip, capfd):
     with Graph(mem=1 << 20) as g:
         with pytest.raises(RuntimeError):
