@@ -239,7 +239,10 @@ __device__ __forceinline__ void prepare_steps(const mm_plan & P, int c, int h0, 
     for (int k = 0; k < 4; k++) {
         // a token past the last neither decays nor adds
         d[k] = lane < left ? softplus(lds[lane * 17 + 4 * wave + k]) : 0.0f;
-        sum[k] = lane < left ? (double) d[k] * ((double) a[k] * 1.4426950408889634074) : 0.0;
+        // 2^-1024 leaves nothing of a float and 2^1024 overflows, so a step beyond either is as good as that one; the
+        // sums stay below 2^16 and the differences over other tokens keep their bits
+        const double e = (double) d[k] * ((double) a[k] * 1.4426950408889634074);
+        sum[k] = lane >= left ? 0.0 : e < -1024.0 ? -1024.0 : e > 1024.0 ? 1024.0 : e;   // a NaN stays one
     }
 #pragma unroll
     for (int o = 1; o < WAVE; o *= 2) {

@@ -89,6 +89,26 @@ def test_scan_extreme_steps(hip, P, N, a0):
     check_scan(hip, d)
 
 
+@pytest.mark.parametrize("P, N, a0", [(64, 128, 1), (1, 16, 16), (5, 7, 1)])
+@pytest.mark.parametrize("big", [1e12, 2e38])
+def test_scan_steps_that_forget_everything(hip, P, N, a0, big):
+    """A time step of any size that leaves nothing of the state is as good as a step of 60 (e^-240) with the
+    same d x: neither its own token nor the later ones lose bits to its exponent, or become NaN where that
+    leaves the range. (60 x / d rounds once: u of d x B, within the 4 u that the bound has for it.)"""
+    d = draw(np.random.default_rng(8), 2, 150, 3, P, N, 1, 2, a0)
+    d["A"] = (d["A"] / 2 - 4).astype(np.float32)
+    same = {k: v.copy() for k, v in d.items()}
+    for at in (3, 4, 70, 71, 72, 149):
+        d["dt"][:, at] = np.float32(big)
+        same["dt"][:, at] = 60
+        d["x"][:, at] = (d["x"][:, at].astype(np.float64) * (60 / float(np.float32(big)))).astype(np.float32)
+    with Graph(mem=1 << 20) as g:
+        out = g.compute(hip, scan_node(g, d))
+    y, h, ye, he = ssm_ref.scan(same["state"][same["ids"]], same["x"], same["dt"], same["A"], same["B"], same["C"])
+    near(out[:y.size], y, ye, "y")
+    near(out[y.size:], h, he, "state")
+
+
 @pytest.mark.parametrize("T", [0, 1, 100])
 def test_scan_decay_of_one_and_growth(hip, T):
     d = draw(np.random.default_rng(10), 1, T, 3, 64, 128, 1, 1, 1)
