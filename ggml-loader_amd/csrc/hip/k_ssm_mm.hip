@@ -9,10 +9,22 @@
 // 128 at the vector rate, which no layout can go below).
 //
 // The products run on the F16 matrix cores. Every operand is scaled by a power of two that puts its
-// largest magnitude at 2^12 and split as x = hi + lo, two halves: 22 bits, and values down to 2^-26 of
-// the largest lose none of them. hi hi + hi lo + lo hi is then a float32 product to within 2^-22, at
-// 16/3 times the rate of the float32 matrix instructions. Sums and states are float32. The running
-// sums c are formed in double and kept as two floats, so that their differences keep 24 bits.
+// largest magnitude at 2^14 and split as x = hi + 2^-12 lo, two halves: 22 bits down to 2^-30 of the
+// largest, and below that an error of 2^-52 of the largest (2^-25 and 2^-12 of it: half a step of the
+// smallest halves). hi hi + 2^-12 (hi lo + lo hi), two sums of matrix products, is then a float32
+// product to within 2^-21, at 16/3 times the rate of the float32 matrix instructions. Sums and states are
+// float32. The running sums c are formed in double and kept as two floats, so that their differences
+// keep 24 bits.
+//
+// One power serves a chunk's C, one its B, one a row of the decayed products C_t . B_j, one a channel's X, its
+// states, and its decayed X. So values that differ by more than 2^33 within one of these would lose bits to
+// the largest, earlier tokens' outputs to later ones among them: a chunk in which they do, or in which one is
+// not finite, is done by its recurrence instead (by_tokens), by the waves of its group for C and B, of its 16 channels
+// for X and the states. Of the decayed products, which reach any depth, it is the row's largest against its own
+// token's that counts, with the spread of X: outputs are wrong by 2^-52 of the largest |C_t . B_j| |X_j| before
+// decay at most, which shows only where all inputs but zeros have decayed by more than 2^30.
+// (With one sum for all three products and 2^12 for the largest, halves held 22 bits down to 2^-15 and a later
+// value of 1e8 put the outputs before it off by 1e-3; that took 180 us instead of 200 at the first size below.)
 //
 // Three launches. ssm_prepare_kernel, per (sequence, chunk, group): C and B split into the order in which the
 // lanes of a matrix instruction hold them, and the products C_t . B_j, which the group's heads share; per
@@ -23,17 +35,13 @@
 // chunk's product reads it from, when the k index of that product runs n = 4 g + i, then 16 + 4 g + i over lane
 // group g, the order that C is prepared in. Eight waves share a chunk's operands.
 //
-// 4096 tokens of 128 heads x 64 x 128, 8 groups: 178 us (1.76 TB/s of what must be read and written, whose floor
-// is 61 us; 22 + 40 + 119 in a trace), 333 tokens of 24 heads 32. Nothing is saturated: the matrix cores are busy
-// for a fifth of the time, the vector units for two fifths and LDS for a quarter, and leaving any one part out
-// (the loads of x or of the operands, the update of the state, the stores) saves a tenth each, so a chunk's
-// barriers and the latency between its parts are what is left. Two tiles of channels a wave (166 us for the last
-// launch), workgroups of four waves (159), four waves a SIMD with one buffer (spills), and half the waves a step
-// ahead of the others (149) were all slower than its 119 to 126.
-//
-// A value that is not finite must not reach earlier tokens of its chunk through 0 times it: X is
-// cleared of such values, and the channel's outputs from that token on, and its state, are NaN. (B, C
-// and dt enter rows and columns of their own only.)
+// 4096 tokens of 128 heads x 64 x 128, 8 groups: 200 us (1.56 TB/s of what must be read and written, whose floor
+// is 61 us; 23 + 51 + 141 in a trace), 333 tokens of 24 heads 35. Before the halves' range was widened these were 180
+// and 32, and then nothing was saturated: the matrix cores were busy for a fifth of the time, the vector units for two
+// fifths and LDS for a quarter, and leaving any one part out (the loads of x or of the operands, the update of the
+// state, the stores) saved a tenth each, so a chunk's barriers and the latency between its parts were what was left.
+// Against 119 to 126 us of the last launch then, two tiles of channels a wave took 166, workgroups of four waves 159,
+// half the waves a step ahead of the others 149; four waves a SIMD with one buffer spilled.
 #include "hip_common.h"
 #include "kernels.h"
 #include "ssm_ops.h"
@@ -52,34 +60,49 @@ typedef uint32_t uint4v __attribute__((ext_vector_type(4)));
 constexpr int Q = 64;                        // tokens per chunk
 // exp(c), exp(c_63 - c), d, c as two floats, exp(c at the end of its 16 tokens - c)
 constexpr int STEP_WORDS = 6 * Q;
+// per (sequence, chunk, group): the exponents of C's and B's powers of two; how far a row's largest |C_t . B_j|
+// exceeds what its own token adds, at most (infinite where C, B or a product is out of range); the largest |C_t . B_j|;
+// that of each row
+constexpr int SCALE_WORDS = 4 + Q;
 // C_t . B_j of a chunk: ten tiles of 16 x 16, the diagonal's and then, row by row, those below it, each as the
 // matrices' lanes load it: two parts of 32 lanes (row + 16 (column / 8)) by four columns
 constexpr int G_WORDS = 10 * 256;
 constexpr int M_BYTES = 6 * 1024;            // one plane of a head's 64 x 64 lower triangle, in 16 x 32 blocks
 
-// the power of two that takes a largest magnitude to 2^12 .. 2^13, and its inverse
-__device__ __forceinline__ float scale_of(float most) {
-    const int e = (int) (__float_as_uint(most) >> 23 & 255);
-    return __uint_as_float((uint32_t) min(266 - e, 247) << 23);
-}
-__device__ __forceinline__ float inverse_of(float scale) { return __uint_as_float((254u - (__float_as_uint(scale) >> 23)) << 23); }
+// the exponent of the power of two that takes a largest magnitude to 2^14 .. 2^15, and that power
+__device__ __forceinline__ int shift_of(float most) { return min(141 - (int) (__float_as_uint(most) >> 23 & 255), 126); }
+__device__ __forceinline__ float power_of(int shift) { return __uint_as_float((uint32_t) (shift + 127) << 23); }
 __device__ __forceinline__ float finite_abs(float x) { return fabsf(x) < INFINITY ? fabsf(x) : 0.0f; }
+// The smallest magnitude other than 0 is that of the least key, a NaN where there is none (and less a unit).
+__device__ __forceinline__ uint32_t least_key(float x) { return (__float_as_uint(x) << 1) - 1; }
+__device__ __forceinline__ float least_value(uint32_t key) { return __uint_as_float(key >> 1); }
+// and the largest that of the largest of these, where a NaN is above an infinity
+__device__ __forceinline__ int most_key(float x) { return (int) (__float_as_uint(x) & 0x7fffffffu); }
+// whether values are finite and the smallest other than 0 so near the largest that halves hold each to 2^-19
+__device__ __forceinline__ bool in_range(float least, float most) { return most < INFINITY && !(least * 0x1p33f < most); }
 
-// eight values times a power of two as hi + lo. The product is exact, so hi comes from one mixed-precision
-// multiply-add and the rest from another: two and a half operations a value.
+// eight values times a power of two as hi + 2^-12 lo. The product is exact, so hi comes from one mixed-precision
+// multiply-add, the rest from another and lo from a third.
 __device__ __forceinline__ void split8(const float (&v)[8], float scale, half8 & hi, half8 & lo) {
 #pragma unroll
-    for (int i = 0; i < 8; i += 2) {
-        const _Float16 h0 = (_Float16) fmaf(v[i], scale, 0.0f), h1 = (_Float16) fmaf(v[i + 1], scale, 0.0f);
-        const half2v l = __builtin_convertvector(float2v{ fmaf(v[i], scale, -(float) h0), fmaf(v[i + 1], scale, -(float) h1) }, half2v);
-        hi[i] = h0; hi[i + 1] = h1;
-        lo[i] = l[0]; lo[i + 1] = l[1];
+    for (int i = 0; i < 8; i++) {
+        const _Float16 h = (_Float16) fmaf(v[i], scale, 0.0f);
+        hi[i] = h;
+        lo[i] = (_Float16) fmaf(fmaf(v[i], scale, -(float) h), 0x1p12f, 0.0f);
     }
 }
 
 __device__ __forceinline__ float4v mfma(half8 a, half8 b, float4v c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
-__device__ __forceinline__ float4v mfma3(half8 ah, half8 al, half8 bh, half8 bl, float4v c) {
-    return mfma(ah, bh, mfma(ah, bl, mfma(al, bh, c)));
+// a sum of products hi hi and the one of hi lo + lo hi, which stands 2^12 above it
+__device__ __forceinline__ void mfma3(half8 ah, half8 al, half8 bh, half8 bl, float4v & sum, float4v & cross) {
+    cross = mfma(al, bh, cross);
+    sum = mfma(ah, bh, sum);
+    cross = mfma(ah, bl, cross);
+}
+__device__ __forceinline__ float4v joined(float4v sum, float4v cross) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) sum[i] = fmaf(cross[i], 0x1p-12f, sum[i]);
+    return sum;
 }
 
 // what the launches share; offsets into the scratch in bytes
@@ -117,20 +140,22 @@ __device__ __forceinline__ void load_perm(const float * row, int n, int N, float
     }
 }
 
+constexpr int PREPARE_WORDS = 16 + 2 * Q;    // of LDS beside B's planes
+
 template <int NK>
 __device__ __forceinline__ void prepare_operands(const mm_plan & P, int c, int g, int s, char * lds) {
     const ssm_scan_launch & L = P.L;                           // lds: B's planes, blocks of 16 tokens by 32 states
     const int tid = threadIdx.x, lane = tid % WAVE, wave = __builtin_amdgcn_readfirstlane(tid / WAVE);
     const int left = P.T - c * Q;             // tokens from the chunk's first on
     constexpr int PLANE = 4 * 1024 * NK;
-    float * red = (float *) (lds + 2 * PLANE);
+    float * red = (float *) (lds + 2 * PLANE), * row_most = red + 16, * row_own = red + 16 + Q;
     const int64_t rec = ((int64_t) s * P.nc + c) * L.G + g;
     char * out = P.ws + P.planes + rec * rec_bytes<NK>();
     // a wave's 16 tokens of both, all states
     const int t = 16 * wave + lane % 16;
     const int64_t row = P.t0 + c * Q + min(t, left - 1);
     const float * cp = L.C + g * L.c_g + s * L.c_s + row * L.c_t, * bp = L.B + g * L.b_g + s * L.b_s + row * L.b_t;
-    float v[2][NK][8], most[2] = { 0.0f, 0.0f };
+    float v[2][NK][8], own = 0.0f;
 #pragma unroll
     for (int q = 0; q < NK; q++) {
         load_perm(cp, 32 * q + 4 * (lane / 16), L.N, v[0][q]);
@@ -138,24 +163,43 @@ __device__ __forceinline__ void prepare_operands(const mm_plan & P, int c, int g
     }
 #pragma unroll
     for (int o = 0; o < 2; o++) {
+        uint32_t key = ~0u;
+        int top = 0;
 #pragma unroll
         for (int q = 0; q < NK; q++) {
 #pragma unroll
             for (int i = 0; i < 8; i++) {
                 v[o][q][i] = t < left ? v[o][q][i] : 0.0f;
-                most[o] = fmaxf(most[o], finite_abs(v[o][q][i]));
+                top = max(top, most_key(v[o][q][i]));
+                key = min(key, least_key(v[o][q][i]));
             }
         }
-        most[o] = wave_max(most[o]);
-        if (lane == 0) red[o * 4 + wave] = most[o];
+        const float m = __int_as_float(top), most = wave_max(m < INFINITY ? m : INFINITY), least = -wave_max(-least_value(key));
+        if (lane == 0) {
+            red[o * 4 + wave] = most;
+            red[8 + o * 4 + wave] = least;
+        }
     }
+    // what a token's row adds to its own output, at most
+#pragma unroll
+    for (int q = 0; q < NK; q++) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) own += fabsf(v[0][q][i] * v[1][q][i]);
+    }
+    own += __shfl_xor(own, 16, WAVE);
+    own += __shfl_xor(own, 32, WAVE);
+    if (lane < 16) row_own[t] = own;
     __syncthreads();
-    float inv[2];
+    int shift[2];
+    bool fine = true;
     half8 ch[NK], cl[NK];
 #pragma unroll
     for (int o = 0; o < 2; o++) {
-        const float sc = scale_of(fmaxf(fmaxf(red[o * 4], red[o * 4 + 1]), fmaxf(red[o * 4 + 2], red[o * 4 + 3])));
-        inv[o] = inverse_of(sc);
+        const float * r = red + o * 4;
+        const float most = fmaxf(fmaxf(r[0], r[1]), fmaxf(r[2], r[3]));
+        fine = fine && in_range(fminf(fminf(r[8], r[9]), fminf(r[10], r[11])), most);
+        shift[o] = shift_of(most);
+        const float sc = power_of(shift[o]);
 #pragma unroll
         for (int q = 0; q < NK; q++) {
             half8 hi, lo;
@@ -176,23 +220,28 @@ __device__ __forceinline__ void prepare_operands(const mm_plan & P, int c, int g
     // C_t . B_j of the wave's tokens, up to the diagonal
     const int gcol = lane % 16;
     float * G = (float *) (P.ws + P.gmat) + rec * G_WORDS + (gcol % 8 / 4) * 128 + (gcol / 8 * 16 + 4 * (lane / 16)) * 4 + gcol % 4;
-    float top = 0.0f;
+    float top[4] = { 0.0f, 0.0f, 0.0f, 0.0f };
     for (int jt = 0; jt <= wave; jt++) {
-        float4v acc = { 0, 0, 0, 0 };
+        float4v acc = { 0, 0, 0, 0 }, cross = { 0, 0, 0, 0 };
 #pragma unroll
         for (int ks = 0; ks < NK; ks++) {
             const char * b = lds + ((jt * NK + ks) * 64 + lane) * 16;
-            acc = mfma3(ch[ks], cl[ks], *(const half8 *) b, *(const half8 *) (b + PLANE), acc);
+            mfma3(ch[ks], cl[ks], *(const half8 *) b, *(const half8 *) (b + PLANE), acc, cross);
         }
+        acc = joined(acc, cross);
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            const float w = acc[i] * inv[0] * inv[1];
+            const float w = ldexpf(acc[i], -(shift[0] + shift[1]));
             G[(jt == wave ? wave : 4 + wave * (wave - 1) / 2 + jt) * 256 + 4 * i] = w;
-            top = fmaxf(top, finite_abs(w));
+            // no later token's
+            if (jt < wave || gcol <= 4 * (lane / 16) + i) top[i] = fmaxf(top[i], fabsf(w) < INFINITY ? fabsf(w) : INFINITY);
         }
     }
-    top = wave_max(top);
-    if (lane == 0) red[8 + wave] = top;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        top[i] = group_max<16>(top[i]);
+        if (gcol == 0) row_most[16 * wave + 4 * (lane / 16) + i] = top[i];
+    }
     // B with the tokens as its k index: row n, eight tokens per lane
     const uint16_t * bh = (const uint16_t *) lds;
 #pragma unroll
@@ -213,10 +262,18 @@ __device__ __forceinline__ void prepare_operands(const mm_plan & P, int c, int g
         for (int p = 0; p < 2; p++) *(uint4v *) (out + (2 + p) * PLANE + it * 16) = uint4v{ w[p][0], w[p][1], w[p][2], w[p][3] };
     }
     __syncthreads();
-    if (tid == 0) {
-        float * sc = (float *) (P.ws + P.scales) + rec * 4;
-        sc[0] = inv[0]; sc[1] = inv[1];
-        sc[2] = fmaxf(fmaxf(red[8], red[9]), fmaxf(red[10], red[11]));
+    if (wave == 0) {
+        const float row = row_most[lane], mine = row_own[lane];
+        const float ratio = row < INFINITY ? (row > 0.0f && mine > 0.0f ? row / mine : 0.0f) : INFINITY;
+        const float spread = fmaxf(wave_max(ratio), 1.0f), all = wave_max(row);
+        float * sc = (float *) (P.ws + P.scales) + rec * SCALE_WORDS;
+        sc[4 + lane] = row;
+        if (lane == 0) {
+            sc[0] = __int_as_float(shift[0]);
+            sc[1] = __int_as_float(shift[1]);
+            sc[2] = fine ? spread : INFINITY;
+            sc[3] = all;
+        }
     }
 }
 
@@ -294,8 +351,32 @@ __device__ __forceinline__ uint32_t here(uint32_t x) {
     asm volatile("" : "+v"(x));
     return x;
 }
+__device__ __forceinline__ int here_s(int x) {
+    asm volatile("" : "+s"(x));
+    return x;
+}
+// likewise the arguments, read again from where the launch put them
+typedef const __attribute__((address_space(4))) mm_plan * plan_ptr;
+__device__ __forceinline__ plan_ptr plan_here() {
+    plan_ptr p = (plan_ptr) __builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(p));
+    return p;
+}
 
-// most |a[i]|, over the four lanes of a column
+// states n .. n + 3 of a row of N
+__device__ __forceinline__ float4v states4(const float * row, int n, int N) {
+    float4v v;
+    if (n + 3 < N) {
+        const float4 f = load4(row + n);
+        v = float4v{ f.x, f.y, f.z, f.w };
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++) v[i] = n + i < N ? row[n + i] : 0.0f;
+    }
+    return v;
+}
+
+// the largest value of a column's four lanes
 __device__ __forceinline__ float column_max(float m) {
     m = fmaxf(m, __shfl_xor(m, 16, WAVE));
     return fmaxf(m, __shfl_xor(m, 32, WAVE));
@@ -315,6 +396,7 @@ __global__ __launch_bounds__(THREADS, 2) void ssm_scan_mm_kernel(mm_plan P) {
     char * bbuf = lds + (OUT ? OPERAND : 0);                   // B's, of this chunk and the next
     float * steps = (float *) (bbuf + SLOTS * OPERAND);        // per head, of this chunk and the next
     char * mats = (char *) (steps + 2 * P.hw * STEP_WORDS);    // per head: the two planes of (C_t . B_j) exp(c_t - c_j)
+    int * row_shift = (int *) (mats + P.hw * 2 * M_BYTES);     // per head: the exponents of their rows' powers of two
     // the wave's number as the scalar that it is: what depends on it alone stays out of the vector registers
     const int tid = threadIdx.x, lane = tid % WAVE, wave = __builtin_amdgcn_readfirstlane(tid / WAVE), col = lane % 16, grp = lane / 16;
 
@@ -358,16 +440,7 @@ __global__ __launch_bounds__(THREADS, 2) void ssm_scan_mm_kernel(mm_plan P) {
         const float * s0 = P.s0 + (P.pooled ? pch * L.s_p + h * L.s_h + row * L.s_row
                                             : (int64_t) L.N * (pch + (int64_t) L.P * (h + (int64_t) L.H * s)));
 #pragma unroll
-        for (int nt = 0; nt < 2 * NK; nt++) {
-            const int n = 16 * nt + 4 * grp;
-            if (n + 3 < L.N) {
-                const float4 f = load4(s0 + n);
-                S[nt] = float4v{ f.x, f.y, f.z, f.w };
-            } else {
-#pragma unroll
-                for (int i = 0; i < 4; i++) S[nt][i] = n + i < L.N ? s0[n + i] : 0.0f;
-            }
-        }
+        for (int nt = 0; nt < 2 * NK; nt++) S[nt] = states4(s0, 16 * nt + 4 * grp, L.N);
         // two segments' loads in flight
         for (int k = 0; k < sg; k += 2) {
             const int k1 = min(k + 1, sg - 1);
@@ -402,7 +475,7 @@ __global__ __launch_bounds__(THREADS, 2) void ssm_scan_mm_kernel(mm_plan P) {
     constexpr bool EARLY = !OUT || NK < 4;
     uint4v stage_c[OUT && EARLY ? STAGE : 1], stage_b[EARLY ? STAGE : 1];
     float4v gg[2][2];
-    float x[2][8], sc_next[3], st_next[(4 * STEP_WORDS + THREADS - 1) / THREADS];
+    float gr[2], x[2][8], sc_next[4], st_next[(4 * STEP_WORDS + THREADS - 1) / THREADS];
     // The matrices' tiles of 16 x 16, two per wave and turn: a head has four on the diagonal, which need an
     // exponential per element, and six below it, where exp(c_t - c_j) is exp(c_t - c_b) exp(c_b - c_j), b the last
     // of the tile's columns: one exponential per row beside prepared ones. A turn is (head, pair of tiles); the
@@ -425,7 +498,8 @@ __global__ __launch_bounds__(THREADS, 2) void ssm_scan_mm_kernel(mm_plan P) {
     auto turn_of = [&](int r) { return WAVES * r + (wave + WAVES / 2 * r) % WAVES; };
     // the lane's row of a tile and its eight columns
     const int tr = lane % 16, th = lane / 16 % 2;
-    auto load_g = [&](const char * G, int turn, float4v (&v)[2]) {
+    auto load_g = [&](const char * G, const char * scales, int turn, float4v (&v)[2], float & most) {
+        most = ((const float *) scales)[4 + 16 * place(turn).tt + tr];
         const int pair = turn < 2 * heads ? turn % 2 : 2 + (turn - 2 * heads) % 3;
         const uint32_t at = here(lane / 32 * 1024 + lane % 32 * 16);
         v[0] = *(const float4v *) (G + pair * 2048 + at);
@@ -441,7 +515,7 @@ __global__ __launch_bounds__(THREADS, 2) void ssm_scan_mm_kernel(mm_plan P) {
     {
         const int64_t rec = ((int64_t) s * P.nc + c0) * L.G + g;
         at_planes = P.ws + P.planes + rec * rec_bytes<NK>();
-        at_scales = P.ws + P.scales + rec * 16;
+        at_scales = P.ws + P.scales + rec * (SCALE_WORDS * 4);
         at_g = P.ws + P.gmat + rec * (G_WORDS * 4);
         at_steps = P.ws + P.steps + (((int64_t) s * P.nc + c0) * L.H + g * per + hb) * (STEP_WORDS * 4);
         at_x = (const char *) (L.x + h * L.x_h + s * L.x_s + (P.t0 + c0 * Q) * L.x_t);
@@ -461,11 +535,11 @@ __global__ __launch_bounds__(THREADS, 2) void ssm_scan_mm_kernel(mm_plan P) {
         for (int q = 0; q < (4 * STEP_WORDS + THREADS - 1) / THREADS; q++)
             st_next[q] = *(const float *) (at_steps + 4 * (uint32_t) min(tid + q * THREADS, heads * STEP_WORDS - 1));
 #pragma unroll
-        for (int i = 0; i < 3; i++) sc_next[i] = ((const float *) at_scales)[i];
+        for (int i = 0; i < 4; i++) sc_next[i] = ((const float *) at_scales)[i];
         if (OUT) {
 #pragma unroll
             for (int r = 0; r < 2; r++) {
-                if (turn_of(r) < turns) load_g(at_g, turn_of(r), gg[r]);
+                if (turn_of(r) < turns) load_g(at_g, at_scales, turn_of(r), gg[r], gr[r]);
             }
         }
         // token 32 ks + 8 grp + i of the wave's channels; past the last token it is the last again, and cleared
@@ -486,7 +560,7 @@ __global__ __launch_bounds__(THREADS, 2) void ssm_scan_mm_kernel(mm_plan P) {
             }
         }
         at_planes += L.G * rec_bytes<NK>();
-        at_scales += L.G * 16;
+        at_scales += L.G * (SCALE_WORDS * 4);
         at_g += L.G * (G_WORDS * 4);
         at_steps += steps_on;
         at_x += x_on;
@@ -519,13 +593,48 @@ __global__ __launch_bounds__(THREADS, 2) void ssm_scan_mm_kernel(mm_plan P) {
         }
     };
 
+    // The chunk by its recurrence, in float32 throughout: for operands whose halves would lose a value beside a larger
+    // one. 16 states after another go through all tokens, which takes few registers beside the main path's: a lane's
+    // four of its channel, whose output so far stays in memory.
+    auto by_tokens = [&](int c, const float * my) {
+        const plan_ptr K = plan_here();
+        const uint32_t n0 = here(4 * grp), p0 = here(pch);
+        const int h1 = here_s(h), s1 = here_s(s), g1 = here_s(g);
+        const float a = K->L.A[h1 * K->L.a_h] * LOG2E;
+        const int64_t row = K->t0 + c * Q;
+        const int n_t = min(Q, K->T - c * Q);
+#pragma unroll
+        for (int nt = 0; nt < 2 * NK; nt++) {
+            if (16 * nt >= K->L.N) break;
+            const float * xp = K->L.x + h1 * K->L.x_h + s1 * K->L.x_s + row * K->L.x_t;
+            const float * bp = K->L.B + g1 * K->L.b_g + s1 * K->L.b_s + row * K->L.b_t + 16 * nt;
+            const float * cp = K->L.C + g1 * K->L.c_g + s1 * K->L.c_s + row * K->L.c_t + 16 * nt;
+            float * y = K->L.y + (int64_t) K->L.P * (h1 + (int64_t) K->L.H * (row + K->L.T * s1));
+            const int left = K->L.N - 16 * nt;
+#pragma unroll 1
+            for (int t = 0; t < n_t; t++, xp += K->L.x_t, bp += K->L.b_t, cp += K->L.c_t, y += (int64_t) K->L.P * K->L.H) {
+                const float d = my[2 * Q + t], e = exp2_hw(d * a), dx = d * xp[p0];
+                const float4v b = states4(bp, (int) n0, left), f = OUT ? states4(cp, (int) n0, left) : b;
+#pragma unroll
+                for (int i = 0; i < 4; i++) S[nt][i] = fmaf(S[nt][i], e, dx * b[i]);
+                if (OUT) {
+                    float v = fmaf(S[nt][0], f[0], S[nt][1] * f[1]) + fmaf(S[nt][2], f[2], S[nt][3] * f[3]);
+                    v += __shfl_xor(v, 16, WAVE);
+                    v += __shfl_xor(v, 32, WAVE);
+                    if (pok && grp == 0) y[p0] = nt == 0 ? v : y[p0] + v;
+                }
+            }
+        }
+    };
+
     float decay = 1.0f;                                        // of the segment so far
     fetch(c0);
     put(0);
     for (int c = c0; c < c1; c++) {
         const int turn = (c - c0) & 1, left = P.T - c * Q;
         const bool whole = left >= Q && 16 * (slice + 1) <= L.P;   // every lane's tokens and channels
-        const float inv_c = sc_next[0], inv_b = sc_next[1], gmost = sc_next[2];
+        const int shift_c = __float_as_int(sc_next[0]), shift_b = __float_as_int(sc_next[1]);
+        const float spread = sc_next[2], gmost = sc_next[3];
         const char * B = bbuf + turn % SLOTS * OPERAND + lane * 16;
         __syncthreads();                                       // this chunk's LDS is written
         const float * head_steps = steps + turn * P.hw * STEP_WORDS, * my = head_steps + (active ? hl : 0) * STEP_WORDS;
@@ -539,15 +648,19 @@ __global__ __launch_bounds__(THREADS, 2) void ssm_scan_mm_kernel(mm_plan P) {
                 if (r == 1) {
                     gg[0][0] = gg[1][0];
                     gg[0][1] = gg[1][1];
+                    gr[0] = gr[1];
                 } else if (r > 1) {
-                    load_g(P.ws + P.gmat + (((int64_t) s * P.nc + c) * L.G + g) * (G_WORDS * 4), now, gg[0]);
+                    const int64_t rec = ((int64_t) s * P.nc + c) * L.G + g;
+                    load_g(P.ws + P.gmat + rec * (G_WORDS * 4), P.ws + P.scales + rec * (SCALE_WORDS * 4), now, gg[0], gr[0]);
                 }
                 const float g8[8] = { gg[0][0][0], gg[0][0][1], gg[0][0][2], gg[0][0][3], gg[0][1][0], gg[0][1][1], gg[0][1][2], gg[0][1][3] };
                 const float * st = head_steps + w.k * STEP_WORDS;
-                const float sm = scale_of(gmost * fmaxf(1.0f, st[Q - 1]));
                 const int t = 16 * w.tt + tr, j0 = 16 * w.jt + 8 * th;
-                float v[8], scale = sm;
+                // no element of the row is larger, and what later tokens hold does not matter to it
+                const int shift = shift_of(gr[0] * fmaxf(1.0f, st[t]));
+                float v[8];
                 if (now < 2 * heads) {
+                    if (th == 0) row_shift[w.k * Q + t] = shift;
                     const float ht = st[3 * Q + t], lt = st[4 * Q + t];
                     const float4 h0 = *(const float4 *) (st + 3 * Q + j0), h1 = *(const float4 *) (st + 3 * Q + j0 + 4);
                     const float4 l0 = *(const float4 *) (st + 4 * Q + j0), l1 = *(const float4 *) (st + 4 * Q + j0 + 4);
@@ -567,14 +680,13 @@ __global__ __launch_bounds__(THREADS, 2) void ssm_scan_mm_kernel(mm_plan P) {
                     for (int i = 0; i < 8; i++) v[i] = g8[i] * ff[i] * row;
                 }
                 half8 hi, lo;
-                split8(v, scale, hi, lo);
+                split8(v, power_of(shift), hi, lo);
                 char * o = mats + w.k * 2 * M_BYTES + (w.tt < 2 ? w.tt : 2 * w.tt - 2 + w.jt / 2) * 1024 + (tr + 16 * (w.jt % 2 * 2 + th)) * 16;
                 *(half8 *) o = hi;
                 *(half8 *) (o + M_BYTES) = lo;
             }
         }
         // X = d x, cleared of tokens past the last
-        float most = 0.0f;
 #pragma unroll
         for (int ks = 0; ks < 2; ks++) {
             const float4 d0 = *(const float4 *) (my + 2 * Q + 32 * ks + 8 * grp), d1 = *(const float4 *) (my + 2 * Q + 32 * ks + 8 * grp + 4);
@@ -589,39 +701,56 @@ __global__ __launch_bounds__(THREADS, 2) void ssm_scan_mm_kernel(mm_plan P) {
                 for (int i = 0; i < 8; i++) x[ks][i] = pok && 32 * ks + 8 * grp + i < left ? x[ks][i] : 0.0f;
             }
         }
+        // whether halves do for the wave's channels
+        int top = 0;
+        uint32_t key = ~0u;
 #pragma unroll
         for (int ks = 0; ks < 2; ks++) {
 #pragma unroll
-            for (int i = 0; i < 8; i++) most = fmaxf(most, fabsf(x[ks][i]));
+            for (int i = 0; i < 8; i++) {
+                top = max(top, most_key(x[ks][i]));
+                key = min(key, least_key(x[ks][i]));
+            }
         }
-        most = column_max(most);
-        int bad = Q;                                           // the channel's first token whose X is not finite
+        const float own = __int_as_float(top), most = column_max(own < INFINITY ? own : INFINITY);
+        const float growth = fmaxf(1.0f, e_last);              // a decay above 1 grows all through a chunk
+        bool fine = in_range(least_value(key), most * (spread * growth)) && gmost * growth < INFINITY;
         half8 xh[2], xl[2];
         if (OUT) {
             // C_t S
             float4v acc[4];
-            float inv_s = 1.0f;
+            int shift_s = 0;
+            float stop = 0.0f;
             if (active) {
-                float top = 0.0f;
+                uint32_t skey = ~0u;
 #pragma unroll
                 for (int nt = 0; nt < 2 * NK; nt++) {
 #pragma unroll
-                    for (int i = 0; i < 4; i++) top = fmaxf(top, fabsf(S[nt][i]));
+                    for (int i = 0; i < 4; i++) {
+                        stop = fmaxf(stop, fabsf(S[nt][i]));
+                        skey = min(skey, least_key(S[nt][i]));
+                    }
                 }
-                top = column_max(top);
-                if (__any(!(top < INFINITY))) {
-                    top = 0.0f;
+                stop = column_max(stop);
+                if (__any(!(stop < INFINITY))) {
+                    // a state that is not finite: its channel's outputs are not either, and no other's are touched
+                    stop = 0.0f;
 #pragma unroll
                     for (int nt = 0; nt < 2 * NK; nt++) {
 #pragma unroll
-                        for (int i = 0; i < 4; i++) top = fmaxf(top, finite_abs(S[nt][i]));
+                        for (int i = 0; i < 4; i++) stop = fmaxf(stop, finite_abs(S[nt][i]));
                     }
-                    top = column_max(top);
+                    stop = column_max(stop);
                 }
-                const float ss = scale_of(top);
-                inv_s = inverse_of(ss) * inv_c;
+                fine = fine && in_range(least_value(skey), stop);
+            }
+            fine = !__any(!fine);
+            if (active && fine) {
+                shift_s = shift_of(stop);
+                const float ss = power_of(shift_s);
+                float4v cross[4];
 #pragma unroll
-                for (int tt = 0; tt < 4; tt++) acc[tt] = float4v{ 0, 0, 0, 0 };
+                for (int tt = 0; tt < 4; tt++) acc[tt] = cross[tt] = float4v{ 0, 0, 0, 0 };
 #pragma unroll
                 for (int ks = 0; ks < NK; ks++) {
                     half8 ah[4], al[4], bh, bl;
@@ -636,87 +765,54 @@ __global__ __launch_bounds__(THREADS, 2) void ssm_scan_mm_kernel(mm_plan P) {
                     for (int i = 0; i < 8; i++) v[i] = S[2 * ks + i / 4][i % 4];
                     split8(v, ss, bh, bl);
 #pragma unroll
-                    for (int tt = 0; tt < 4; tt++) acc[tt] = mfma(al[tt], bh, acc[tt]);
-#pragma unroll
-                    for (int tt = 0; tt < 4; tt++) acc[tt] = mfma(ah[tt], bl, acc[tt]);
+                    for (int tt = 0; tt < 4; tt++) cross[tt] = mfma(al[tt], bh, cross[tt]);
 #pragma unroll
                     for (int tt = 0; tt < 4; tt++) acc[tt] = mfma(ah[tt], bh, acc[tt]);
+#pragma unroll
+                    for (int tt = 0; tt < 4; tt++) cross[tt] = mfma(ah[tt], bl, cross[tt]);
                 }
+#pragma unroll
+                for (int tt = 0; tt < 4; tt++) acc[tt] = joined(acc[tt], cross[tt]);
             }
             __syncthreads();                                   // C is read, the matrices are written
-            if (active) {
-                const float inv_m = inverse_of(scale_of(gmost * fmaxf(1.0f, e_last)));
+            if (active && fine) {
                 const char * mine = mats + hl * 2 * M_BYTES + lane * 16;
+                const int shift_x = shift_of(most);
                 float4v sum[4];
-                float inv_x = 1.0f;
-                auto products = [&]() {
-                    const float sc = scale_of(most);
-                    inv_x = inverse_of(sc);
 #pragma unroll
-                    for (int ks = 0; ks < 2; ks++) split8(x[ks], sc, xh[ks], xl[ks]);
+                for (int ks = 0; ks < 2; ks++) split8(x[ks], power_of(shift_x), xh[ks], xl[ks]);
 #pragma unroll
-                    for (int t2 = 0; t2 < 4; t2 += 2) {
-                        // tiles 0 and 1 end within the first 32 tokens
-                        half8 ah[2][2], al[2][2];
+                for (int t2 = 0; t2 < 4; t2 += 2) {
+                    // tiles 0 and 1 end within the first 32 tokens
+                    half8 ah[2][2], al[2][2];
 #pragma unroll
-                        for (int ks = 0; ks <= t2 / 2; ks++) {
+                    for (int ks = 0; ks <= t2 / 2; ks++) {
 #pragma unroll
-                            for (int q = 0; q < 2; q++) {
-                                const char * a = mine + (t2 == 0 ? q : 2 + 2 * q + ks) * 1024;
-                                ah[q][ks] = *(const half8 *) a;
-                                al[q][ks] = *(const half8 *) (a + M_BYTES);
-                            }
-                        }
-#pragma unroll
-                        for (int q = 0; q < 2; q++) sum[t2 + q] = mfma(al[q][0], xh[0], float4v{ 0, 0, 0, 0 });
-#pragma unroll
-                        for (int q = 0; q < 2; q++) sum[t2 + q] = mfma(ah[q][0], xl[0], sum[t2 + q]);
-#pragma unroll
-                        for (int q = 0; q < 2; q++) sum[t2 + q] = mfma(ah[q][0], xh[0], sum[t2 + q]);
-                        if (t2) {
-#pragma unroll
-                            for (int q = 0; q < 2; q++) sum[t2 + q] = mfma(al[q][1], xh[1], sum[t2 + q]);
-#pragma unroll
-                            for (int q = 0; q < 2; q++) sum[t2 + q] = mfma(ah[q][1], xl[1], sum[t2 + q]);
-#pragma unroll
-                            for (int q = 0; q < 2; q++) sum[t2 + q] = mfma(ah[q][1], xh[1], sum[t2 + q]);
+                        for (int q = 0; q < 2; q++) {
+                            const char * a = mine + (t2 == 0 ? q : 2 + 2 * q + ks) * 1024;
+                            ah[q][ks] = *(const half8 *) a;
+                            al[q][ks] = *(const half8 *) (a + M_BYTES);
                         }
                     }
-                };
-                products();
-                // Every row of the last tile takes all of a channel's tokens, so an X that is not finite shows there (as
-                // may a value of B, C or dt, which stays as it is): again without it.
-                if (__any(!(fabsf(sum[3][3]) < INFINITY))) {
-                    most = 0.0f;
+                    float4v own[2], cross[2];
 #pragma unroll
-                    for (int ks = 1; ks >= 0; ks--) {
+                    for (int q = 0; q < 2; q++) own[q] = cross[q] = float4v{ 0, 0, 0, 0 };
 #pragma unroll
-                        for (int i = 7; i >= 0; i--) {
-                            const bool fine = fabsf(x[ks][i]) < INFINITY;
-                            if (!fine) bad = 32 * ks + 8 * grp + i;
-                            x[ks][i] = fine ? x[ks][i] : 0.0f;
-                            most = fmaxf(most, fabsf(x[ks][i]));
-                        }
+                    for (int ks = 0; ks <= t2 / 2; ks++) {
+#pragma unroll
+                        for (int q = 0; q < 2; q++) mfma3(ah[q][ks], al[q][ks], xh[ks], xl[ks], own[q], cross[q]);
                     }
-                    bad = min(bad, __shfl_xor(bad, 16, WAVE));
-                    bad = min(bad, __shfl_xor(bad, 32, WAVE));
-                    most = column_max(most);
-                    products();
+#pragma unroll
+                    for (int q = 0; q < 2; q++) sum[t2 + q] = joined(own[q], cross[q]);
                 }
-                const float inv = inv_m * inv_x;
 #pragma unroll
                 for (int tt = 0; tt < 4; tt++) {
                     const float4 e4 = *(const float4 *) (my + 16 * tt + 4 * grp);
+                    const int4 r4 = *(const int4 *) (row_shift + (active ? hl : 0) * Q + 16 * tt + 4 * grp);
                     const float e[4] = { e4.x, e4.y, e4.z, e4.w };
+                    const int rs[4] = { r4.x, r4.y, r4.z, r4.w };
 #pragma unroll
-                    for (int i = 0; i < 4; i++) acc[tt][i] = fmaf(acc[tt][i], inv_s * e[i], sum[tt][i] * inv);
-                }
-                if (__any(bad < Q)) {
-#pragma unroll
-                    for (int tt = 0; tt < 4; tt++) {
-#pragma unroll
-                        for (int i = 0; i < 4; i++) acc[tt][i] = 16 * tt + 4 * grp + i < bad ? acc[tt][i] : NAN;
-                    }
+                    for (int i = 0; i < 4; i++) acc[tt][i] = ldexpf(acc[tt][i] * e[i], -(shift_s + shift_c)) + ldexpf(sum[tt][i], -(shift_x + rs[i]));
                 }
                 char * y = (char *) (L.y + h * L.P + (int64_t) L.P * L.H * (P.t0 + c * Q + L.T * s));
                 const uint32_t row = 4 * (uint32_t) L.P * (uint32_t) L.H;
@@ -735,27 +831,35 @@ __global__ __launch_bounds__(THREADS, 2) void ssm_scan_mm_kernel(mm_plan P) {
                     at += 12 * row;
                 }
             }
+        } else {
+            fine = !__any(!fine);
         }
         // the state at the chunk's end
-        float inv_u = 1.0f;
-        if (active) {
-            const float sc = scale_of(most * fmaxf(1.0f, my[Q]));
-            inv_u = inverse_of(sc) * inv_b;
+        int shift_u = 0;
+        if (active && fine) {
+            float v[2][8], wmost = 0.0f;
 #pragma unroll
             for (int ks = 0; ks < 2; ks++) {
                 const float4 w0 = *(const float4 *) (my + Q + 32 * ks + 8 * grp), w1 = *(const float4 *) (my + Q + 32 * ks + 8 * grp + 4);
                 const float ww[8] = { w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w };
-                float v[8];
 #pragma unroll
-                for (int i = 0; i < 8; i++) v[i] = x[ks][i] * ww[i];
-                split8(v, sc, xh[ks], xl[ks]);
+                for (int i = 0; i < 8; i++) {
+                    v[ks][i] = x[ks][i] * ww[i];
+                    wmost = fmaxf(wmost, fabsf(v[ks][i]));
+                }
             }
+            // by the largest that the decays leave, not by one that they have taken away
+            const int shift_w = shift_of(column_max(wmost));
+            shift_u = shift_w + shift_b;
+#pragma unroll
+            for (int ks = 0; ks < 2; ks++) split8(v[ks], power_of(shift_w), xh[ks], xl[ks]);
         }
+        if (active && !fine) by_tokens(c, my);
         if (c + 1 < c1) fetch(c + 1);
-        if (active) {
+        if (active && fine) {
 #pragma unroll
             for (int n0 = 0; n0 < 2 * NK; n0 += 2) {
-                float4v sum[2];
+                float4v sum[2], cross[2];
                 half8 ah[2][2], al[2][2];
 #pragma unroll
                 for (int q = 0; q < 2; q++) {
@@ -766,31 +870,21 @@ __global__ __launch_bounds__(THREADS, 2) void ssm_scan_mm_kernel(mm_plan P) {
                     }
                 }
 #pragma unroll
-                for (int q = 0; q < 2; q++) sum[q] = mfma(al[q][0], xh[0], float4v{ 0, 0, 0, 0 });
-#pragma unroll
-                for (int q = 0; q < 2; q++) sum[q] = mfma(al[q][1], xh[1], sum[q]);
+                for (int q = 0; q < 2; q++) sum[q] = cross[q] = float4v{ 0, 0, 0, 0 };
 #pragma unroll
                 for (int ks = 0; ks < 2; ks++) {
 #pragma unroll
-                    for (int q = 0; q < 2; q++) sum[q] = mfma(ah[q][ks], xl[ks], sum[q]);
-#pragma unroll
-                    for (int q = 0; q < 2; q++) sum[q] = mfma(ah[q][ks], xh[ks], sum[q]);
+                    for (int q = 0; q < 2; q++) mfma3(ah[q][ks], al[q][ks], xh[ks], xl[ks], sum[q], cross[q]);
                 }
 #pragma unroll
                 for (int q = 0; q < 2; q++) {
+                    sum[q] = joined(sum[q], cross[q]);
 #pragma unroll
-                    for (int i = 0; i < 4; i++) S[n0 + q][i] = fmaf(S[n0 + q][i], e_last, sum[q][i] * inv_u);
+                    for (int i = 0; i < 4; i++) S[n0 + q][i] = fmaf(S[n0 + q][i], e_last, ldexpf(sum[q][i], -shift_u));
                 }
             }
-            if (OUT && __any(bad < Q)) {
-#pragma unroll
-                for (int nt = 0; nt < 2 * NK; nt++) {
-#pragma unroll
-                    for (int i = 0; i < 4; i++) S[nt][i] = bad < Q ? NAN : S[nt][i];
-                }
-            }
-            decay *= e_last;
         }
+        decay *= e_last;
         if (SLOTS == 1) __syncthreads();                       // B is read
         if (c + 1 < c1) put(turn ^ 1);
     }
@@ -836,7 +930,7 @@ mm_sizes mm_size(const ssm_scan_launch & L) {
     z.hw = z.p_blocks > 1 ? 1 : std::min(WAVES / z.slices, z.nk == 8 ? 2 : 4);
     z.head_blocks = (L.H / L.G + z.hw - 1) / z.hw;
     z.chunks = (L.T + Q - 1) / Q;
-    const int64_t rec = (int64_t) z.nk * 16384 + G_WORDS * 4 + 16, per = L.S * (L.G * rec + (int64_t) L.H * STEP_WORDS * 4);
+    const int64_t rec = (int64_t) z.nk * 16384 + (G_WORDS + SCALE_WORDS) * 4, per = L.S * (L.G * rec + (int64_t) L.H * STEP_WORDS * 4);
     // prepared operands of at most 64 MiB: the tokens go through in blocks
     z.block = std::max<int64_t>(1, std::min<int64_t>({ z.chunks, ((int64_t) 64 << 20) / per, 65535 }));
     // segments until every CU has a workgroup, of one chunk if need be (333 tokens of 24 heads: 41 us with two
@@ -850,7 +944,7 @@ mm_sizes mm_size(const ssm_scan_launch & L) {
     auto take = [&](int64_t bytes) { const int64_t r = at; at += (bytes + 255) / 256 * 256; return r; };
     z.planes = take(L.S * z.block * L.G * (int64_t) z.nk * 16384);
     z.gmat = take(L.S * z.block * L.G * G_WORDS * 4);
-    z.scales = take(L.S * z.block * L.G * 16);
+    z.scales = take(L.S * z.block * L.G * SCALE_WORDS * 4);
     z.steps = take(L.S * z.block * (int64_t) L.H * STEP_WORDS * 4);
     z.parts = take(z.n_seg > 1 ? L.S * z.n_seg * (int64_t) L.H * z.slices * 2 * z.nk * WAVE * 16 : 0);
     z.decays = take(z.n_seg > 1 ? L.S * z.n_seg * (int64_t) L.H * 4 : 0);
@@ -869,14 +963,14 @@ void launch_mm(const ssm_scan_launch & L, const mm_sizes & z, void * ws, hipStre
     P.hw = z.hw; P.slices = z.slices; P.head_blocks = z.head_blocks; P.p_blocks = z.p_blocks;
     constexpr int OPERAND = NK * 8192;
     auto lds_of = [](int hw, bool out) {
-        return (size_t) OPERAND * (b_slots(NK) + (out ? 1 : 0)) + (size_t) hw * (2 * STEP_WORDS * 4 + (out ? 2 * M_BYTES : 0));
+        return (size_t) OPERAND * (b_slots(NK) + (out ? 1 : 0)) + (size_t) hw * (2 * STEP_WORDS * 4 + (out ? 2 * M_BYTES + Q * 4 : 0));
     };
     static std::atomic<uint64_t> lds_set{ 0 };                 // devices, a bit each
     int device = 0;
     HIP_CHECK(hipGetDevice(&device));
     if (device > 63 || !(lds_set.load(std::memory_order_relaxed) >> device & 1)) {
         const int hw = NK == 8 ? 2 : 4;
-        HIP_CHECK(hipFuncSetAttribute((const void *) ssm_prepare_kernel<NK>, hipFuncAttributeMaxDynamicSharedMemorySize, OPERAND + 64));
+        HIP_CHECK(hipFuncSetAttribute((const void *) ssm_prepare_kernel<NK>, hipFuncAttributeMaxDynamicSharedMemorySize, OPERAND + PREPARE_WORDS * 4));
         HIP_CHECK(hipFuncSetAttribute((const void *) ssm_scan_mm_kernel<NK, false>, hipFuncAttributeMaxDynamicSharedMemorySize, (int) lds_of(hw, false)));
         HIP_CHECK(hipFuncSetAttribute((const void *) ssm_scan_mm_kernel<NK, true>, hipFuncAttributeMaxDynamicSharedMemorySize, (int) lds_of(hw, true)));
         if (device < 64) lds_set.fetch_or(1ull << device, std::memory_order_relaxed);
@@ -893,7 +987,7 @@ void launch_mm(const ssm_scan_launch & L, const mm_sizes & z, void * ws, hipStre
         P.s0 = c == 0 ? L.s : hold + (turn ^ 1) * states;
         P.s1 = c + z.block < z.chunks ? hold + turn * states : L.s_out;
         launch(ssm_prepare_kernel<NK>, dim3((unsigned) P.nc, (unsigned) (L.G + (L.H + 15) / 16), (unsigned) L.S), dim3(256),
-               std::max<size_t>(OPERAND + 64, Q * 17 * 4), st, P);
+               std::max<size_t>(OPERAND + PREPARE_WORDS * 4, Q * 17 * 4), st, P);
         const dim3 grid((unsigned) (L.S * L.G * P.n_seg * z.head_blocks * z.p_blocks));
         if (P.n_seg > 1) launch(ssm_scan_mm_kernel<NK, false>, grid, dim3(THREADS), lds_of(z.hw, false), st, P);
         launch(ssm_scan_mm_kernel<NK, true>, grid, dim3(THREADS), lds_of(z.hw, true), st, P);

@@ -151,6 +151,56 @@ def test_scan_keeps_what_came_before_a_bad_value(hip, T, at, P, N, a0, bad):
     near(h[hf], h64[hf], he[hf])
 
 
+def with_outliers(d, kind, size):
+    """Operands of unequal size: values of one token, of one state, or of an input and a token."""
+    H, P, N, G = d["x"].shape[2], d["x"].shape[3], d["B"].shape[3], d["B"].shape[2]
+    h, p, n, g = H // 2, P // 3, N // 3, G - 1
+    if kind in ("late x", "early x"):
+        d["x"][0, 50 if kind == "late x" else 3, h, p] *= size
+    if kind == "x of all channels":
+        d["x"][0, 50] *= size
+    if kind in ("B", "C"):
+        d[kind][0, 50, g, n] *= size
+    if kind in ("row of B", "row of C"):
+        d[kind[-1]][0, 50] *= size
+    if kind in ("state of B", "state of C"):
+        d["B"][..., n] *= size if kind[-1] == "B" else 1 / size
+        d["C"][..., n] *= size if kind[-1] == "C" else 1 / size
+    if kind == "first state":
+        d["state"][:, h, p, n] *= size
+    if kind == "small inputs first":
+        d["state"][:] = 0
+        d["x"][:, :40] /= size
+    if kind == "x and B":
+        d["x"][0, 20, h, p] *= size
+        d["B"][0, 45, g, n] *= size
+    if kind == "every eighth x":
+        d["state"][:] = 0
+        d["x"][:, 7::8] *= size
+    return d
+
+
+@pytest.mark.parametrize("size", [1e5, 1e6, 1e8, 1e11, 1e18])
+@pytest.mark.parametrize("kind", ["late x", "early x", "x of all channels", "B", "C", "row of B", "row of C", "state of B", "state of C",
+                                  "first state", "small inputs first", "x and B", "every eighth x"])
+@pytest.mark.parametrize("S, T, H, P, N, G, a0", [(2, 150, 2, 64, 128, 1, 1), (1, 400, 2, 20, 30, 2, 1), (1, 70, 3, 5, 256, 1, 1), (1, 150, 66, 1, 16, 1, 16)])
+def test_scan_of_operands_of_unequal_size(hip, S, T, H, P, N, G, a0, kind, size):
+    """A value far larger than the others, finite, takes bits from no other token, channel or state: each
+    output is held to the bound of its own terms."""
+    rng = np.random.default_rng(T + P + N)
+    d = draw(rng, S, T, H, P, N, G, S, a0)
+    check_scan(hip, with_outliers(d, kind, np.float32(size)))
+
+
+@pytest.mark.parametrize("T, a", [(150, 2.0), (70, 15.0), (200, 0.3), (64, 20.0)])
+def test_scan_that_grows(hip, T, a):
+    """Decays above 1: a chunk's last tokens are far larger than its first, which keep their bits."""
+    d = draw(np.random.default_rng(14), 1, T, 3, 64, 128, 1, 1, 1)
+    d["A"][:] = np.float32(a) * np.array([[1.0], [0.5], [-1.0]], np.float32)
+    d["dt"][:] = np.minimum(d["dt"], -2.5)
+    check_scan(hip, d)
+
+
 # few tokens, channels and states at the edges of what a lane, a wave or a group of rows takes
 FEW = [
     (3, 1, 67, 1, 16, 1, 3, 16), (2, 1, 64, 1, 8, 1, 2, 8), (3, 2, 130, 1, 32, 1, 3, 32), (2, 5, 129, 1, 16, 1, 2, 16), (1, 8, 1, 1, 16, 1, 1, 1),
