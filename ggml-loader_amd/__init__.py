@@ -228,6 +228,7 @@ def _declare(core, hip, loader):
          C.c_double, C.POINTER(C.c_int32), C.POINTER(C.c_bool))
     _sig(hip, "ggml_backend_hip_logprobs", i32, vp, vp, i64, i64, vp, C.c_int32, vp, vp, vp, vp)
     _sig(hip, "ggml_backend_hip_refusal", C.c_char_p, T)
+    _sig(hip, "ggml_backend_hip_scan_scratch", sz, T)
     _sig(hip, "ggml_backend_hip_set_fusion", None, vp, C.c_bool)
     _sig(hip, "ggml_backend_hip_set_profiling", None, vp, C.c_bool)
     _sig(hip, "ggml_backend_hip_set_profile_filter", None, vp, C.c_char_p)

@@ -496,6 +496,27 @@ const char * ssm_scan_refusal(const ggml_tensor * n) {
     return nullptr;
 }
 
+// a scan's launch, its states behind y
+ssm_scan_launch scan_launch_of(const ggml_tensor * n) {
+    const ggml_tensor * s = n->src[0], * x = n->src[1], * dt = n->src[2], * A = n->src[3], * B = n->src[4], * C = n->src[5],
+                      * ids = n->src[6];
+    auto f = [](const ggml_tensor * t) { return (const float *) t->data; };
+    auto nb = [](const ggml_tensor * t, int i) { return (int64_t) t->nb[i] / 4; };
+    ssm_scan_launch L{};
+    L.N = (int) s->ne[0]; L.P = (int) s->ne[1]; L.H = (int) s->ne[2]; L.G = (int) B->ne[1];
+    L.T = x->ne[2]; L.S = x->ne[3]; L.pool = s->ne[3];
+    L.s = f(s); L.s_p = nb(s, 1); L.s_h = nb(s, 2); L.s_row = nb(s, 3);
+    L.x = f(x); L.x_h = nb(x, 1); L.x_t = nb(x, 2); L.x_s = nb(x, 3);
+    L.dt = f(dt); L.dt_t = nb(dt, 1); L.dt_s = nb(dt, 2);
+    L.A = f(A); L.a_h = nb(A, 1); L.a_scalar = A->ne[0] == 1;
+    L.B = f(B); L.b_g = nb(B, 1); L.b_t = nb(B, 2); L.b_s = nb(B, 3);
+    L.C = f(C); L.c_g = nb(C, 1); L.c_t = nb(C, 2); L.c_s = nb(C, 3);
+    L.ids = (const int32_t *) ids->data; L.ids_s = nb(ids, 0);
+    L.y = (float *) n->data;
+    L.s_out = L.y + ggml_nelements(x);
+    return L;
+}
+
 // why graph_compute refuses a graph with this node before it queues anything (nullptr: it does not)
 const char * node_refusal(const ggml_tensor * n) {
     if (n->op == GGML_OP_SSM_CONV) return ssm_conv_refusal(n);
@@ -1122,38 +1143,27 @@ private:
     }
 
     void op_ssm_scan(ggml_tensor * n) {
-        const ggml_tensor * s = n->src[0], * x = n->src[1], * dt = n->src[2], * A = n->src[3], * B = n->src[4], * C = n->src[5],
-                          * ids = n->src[6];
-        auto f = [](const ggml_tensor * t) { return (const float *) t->data; };
-        auto nb = [](const ggml_tensor * t, int i) { return (int64_t) t->nb[i] / 4; };
-        ssm_scan_launch L{};
-        L.N = (int) s->ne[0]; L.P = (int) s->ne[1]; L.H = (int) s->ne[2]; L.G = (int) B->ne[1];
-        L.T = x->ne[2]; L.S = x->ne[3]; L.pool = s->ne[3];
-        L.s = f(s); L.s_p = nb(s, 1); L.s_h = nb(s, 2); L.s_row = nb(s, 3);
-        L.x = f(x); L.x_h = nb(x, 1); L.x_t = nb(x, 2); L.x_s = nb(x, 3);
-        L.dt = f(dt); L.dt_t = nb(dt, 1); L.dt_s = nb(dt, 2);
-        L.A = f(A); L.a_h = nb(A, 1); L.a_scalar = A->ne[0] == 1;
-        L.B = f(B); L.b_g = nb(B, 1); L.b_t = nb(B, 2); L.b_s = nb(B, 3);
-        L.C = f(C); L.c_g = nb(C, 1); L.c_t = nb(C, 2); L.c_s = nb(C, 3);
-        L.ids = (const int32_t *) ids->data; L.ids_s = nb(ids, 0);
-        L.y = (float *) n->data;
-        L.s_out = L.y + ggml_nelements(x);
+        const ggml_tensor * x = n->src[1], * dt = n->src[2], * B = n->src[4];
+        ssm_scan_launch L = scan_launch_of(n);
         if (const ggml_tensor * cp = scan_state_copy(n, L)) {
             L.s_out = (float *) cp->data;
             wrote_.push_back(cp);
         }
         const double st = (double) L.N * L.P * L.H * L.S * 4;
         prof_scope ps(this, "ssm_scan", 2 * st + 4.0 * (2 * ggml_nelements(x) + ggml_nelements(dt) + 2 * ggml_nelements(B)));
-        // one buffer for the graph's scans, which the stream runs one after another
-        const int64_t bytes = ssm_scan_scratch_bytes(L);
-        if (bytes > ssm_bytes_) {
-            ssm_buf_ = c_.scratch.alloc((size_t) bytes);
-            ssm_bytes_ = bytes;
+        if (!ssm_sized_) {
+            // one buffer for the graph's scans, which the stream runs one after another
+            int64_t bytes = 0;
+            for (int i = 0; i < g_->n_nodes; i++) {
+                if (g_->nodes[i]->op == GGML_OP_SSM_SCAN) bytes = std::max(bytes, ssm_scan_scratch_bytes(scan_launch_of(g_->nodes[i])));
+            }
+            if (bytes) ssm_buf_ = c_.scratch.alloc((size_t) bytes);
+            ssm_sized_ = true;
         }
         launch_ssm_scan(L, ssm_buf_, st_);
     }
     void * ssm_buf_ = nullptr;
-    int64_t ssm_bytes_ = 0;
+    bool ssm_sized_ = false;
 
     void op_get_rows(ggml_tensor * n) {
         const ggml_tensor * a = n->src[0];
@@ -2856,6 +2866,10 @@ enum ggml_status ggml_backend_hip_sample(ggml_backend_t backend, const struct gg
 }
 
 const char * ggml_backend_hip_refusal(const struct ggml_tensor * node) { return node ? node_refusal(node) : "no node"; }
+
+size_t ggml_backend_hip_scan_scratch(const struct ggml_tensor * node) {
+    return node && node->op == GGML_OP_SSM_SCAN && !node_refusal(node) ? (size_t) ssm_scan_scratch_bytes(scan_launch_of(node)) : 0;
+}
 
 // (see the declaration for the contract)
 enum ggml_status ggml_backend_hip_logprobs(ggml_backend_t backend, const struct ggml_tensor * logits, int64_t row,

@@ -917,9 +917,18 @@ int steps_of(int N) { return N <= 32 ? 1 : N <= 64 ? 2 : N <= 128 ? 4 : 8; }
 
 struct mm_sizes {
     int     nk, slices, hw, head_blocks, p_blocks;
-    int64_t chunks, block, n_seg, seg;      // chunks in all and per block of tokens, segments of a block
+    int64_t seqs, chunks, block, n_seg, seg;   // sequences at once, chunks in all and per block of tokens, segments of a block
     int64_t planes, gmat, scales, steps, parts, decays, state, total;
 };
+
+// prepared operands (with the rounding of their offsets) and segments' states of at most so many bytes: sequences and
+// tokens go through in blocks
+constexpr int64_t MOST_OPERANDS = ((int64_t) 64 << 20) - 4096, MOST_PARTS = (int64_t) 32 << 20;
+
+// those of one chunk of one sequence
+int64_t chunk_bytes(const ssm_scan_launch & L) {
+    return L.G * ((int64_t) steps_of(L.N) * 16384 + (G_WORDS + SCALE_WORDS) * 4) + (int64_t) L.H * STEP_WORDS * 4;
+}
 
 mm_sizes mm_size(const ssm_scan_launch & L) {
     mm_sizes z;
@@ -930,26 +939,27 @@ mm_sizes mm_size(const ssm_scan_launch & L) {
     z.hw = z.p_blocks > 1 ? 1 : std::min(WAVES / z.slices, z.nk == 8 ? 2 : 4);
     z.head_blocks = (L.H / L.G + z.hw - 1) / z.hw;
     z.chunks = (L.T + Q - 1) / Q;
-    const int64_t rec = (int64_t) z.nk * 16384 + (G_WORDS + SCALE_WORDS) * 4, per = L.S * (L.G * rec + (int64_t) L.H * STEP_WORDS * 4);
-    // prepared operands of at most 64 MiB: the tokens go through in blocks
-    z.block = std::max<int64_t>(1, std::min<int64_t>({ z.chunks, ((int64_t) 64 << 20) / per, 65535 }));
+    // as many sequences at once as one chunk of each leaves room for, in even passes
+    const int64_t fit = std::max<int64_t>(1, std::min<int64_t>(L.S, MOST_OPERANDS / chunk_bytes(L))), passes = (L.S + fit - 1) / fit;
+    z.seqs = (L.S + passes - 1) / passes;
+    z.block = std::max<int64_t>(1, std::min<int64_t>({ z.chunks, MOST_OPERANDS / (z.seqs * chunk_bytes(L)), 65535 }));
     // segments until every CU has a workgroup, of one chunk if need be (333 tokens of 24 heads: 41 us with two
     // chunks at least, 37 with one)
-    const int64_t base = L.S * L.G * z.head_blocks * z.p_blocks;
-    const int64_t part = L.S * L.H * (int64_t) z.slices * (2 * z.nk * WAVE * 16) + L.S * L.H * 4;
-    z.n_seg = std::max<int64_t>(1, std::min<int64_t>({ 256 / base, z.block, ((int64_t) 32 << 20) / part }));
+    const int64_t base = z.seqs * L.G * z.head_blocks * z.p_blocks;
+    const int64_t part = z.seqs * L.H * (int64_t) z.slices * (2 * z.nk * WAVE * 16) + z.seqs * L.H * 4;
+    z.n_seg = std::max<int64_t>(1, std::min<int64_t>({ 256 / base, z.block, MOST_PARTS / part }));
     z.seg = (z.block + z.n_seg - 1) / z.n_seg;
     z.n_seg = (z.block + z.seg - 1) / z.seg;
     int64_t at = 0;
     auto take = [&](int64_t bytes) { const int64_t r = at; at += (bytes + 255) / 256 * 256; return r; };
-    z.planes = take(L.S * z.block * L.G * (int64_t) z.nk * 16384);
-    z.gmat = take(L.S * z.block * L.G * G_WORDS * 4);
-    z.scales = take(L.S * z.block * L.G * SCALE_WORDS * 4);
-    z.steps = take(L.S * z.block * (int64_t) L.H * STEP_WORDS * 4);
-    z.parts = take(z.n_seg > 1 ? L.S * z.n_seg * (int64_t) L.H * z.slices * 2 * z.nk * WAVE * 16 : 0);
-    z.decays = take(z.n_seg > 1 ? L.S * z.n_seg * (int64_t) L.H * 4 : 0);
+    z.planes = take(z.seqs * z.block * L.G * (int64_t) z.nk * 16384);
+    z.gmat = take(z.seqs * z.block * L.G * G_WORDS * 4);
+    z.scales = take(z.seqs * z.block * L.G * SCALE_WORDS * 4);
+    z.steps = take(z.seqs * z.block * (int64_t) L.H * STEP_WORDS * 4);
+    z.parts = take(z.n_seg > 1 ? z.seqs * z.n_seg * (int64_t) L.H * z.slices * 2 * z.nk * WAVE * 16 : 0);
+    z.decays = take(z.n_seg > 1 ? z.seqs * z.n_seg * (int64_t) L.H * 4 : 0);
     // states between blocks of tokens, one read while the next is written
-    z.state = take(z.block < z.chunks ? 2 * L.S * (int64_t) L.N * L.P * L.H * 4 : 0);
+    z.state = take(z.block < z.chunks ? 2 * z.seqs * (int64_t) L.N * L.P * L.H * 4 : 0);
     z.total = at;
     return z;
 }
@@ -976,7 +986,7 @@ void launch_mm(const ssm_scan_launch & L, const mm_sizes & z, void * ws, hipStre
         if (device < 64) lds_set.fetch_or(1ull << device, std::memory_order_relaxed);
     }
     float * hold = (float *) ((char *) ws + z.state);
-    const int64_t states = L.S * (int64_t) L.N * L.P * L.H;
+    const int64_t states = z.seqs * (int64_t) L.N * L.P * L.H;
     for (int64_t c = 0, turn = 0; c < z.chunks; c += z.block, turn ^= 1) {
         P.nc = (int) std::min(z.block, z.chunks - c);
         P.t0 = c * Q;
@@ -1010,16 +1020,25 @@ bool ssm_scan_mm_takes(const ssm_scan_launch & L) {
     // the grids' limits: one dimension each for the sequences and for groups and heads, 2^32 threads in all
     return L.a_scalar && L.T > step_tokens(L) && L.S <= 65535 && L.G + (L.H + 15) / 16 <= 65535 &&
            L.S * (int64_t) L.H * ((L.P + 127) / 128) < 1 << 22 &&
+           // one sequence's chunk fits the scratch (512 groups of 256 states do not)
+           chunk_bytes(L) <= MOST_OPERANDS &&
            // 32-bit offsets within a chunk
            L.x_t >= 0 && L.x_t <= 1 << 24 && (int64_t) L.H * L.P <= 1 << 24 && L.P <= 1 << 24;
 }
 
 int64_t ssm_scan_mm_scratch_bytes(const ssm_scan_launch & L) { return mm_size(L).total; }
 
-void launch_ssm_scan_mm(const ssm_scan_launch & L, void * ws, hipStream_t st) {
-    const mm_sizes z = mm_size(L);
-    if (z.nk == 8) launch_mm<8>(L, z, ws, st);
-    else if (z.nk == 4) launch_mm<4>(L, z, ws, st);
-    else if (z.nk == 2) launch_mm<2>(L, z, ws, st);
-    else launch_mm<1>(L, z, ws, st);
+void launch_ssm_scan_mm(const ssm_scan_launch & L0, void * ws, hipStream_t st) {
+    const mm_sizes z = mm_size(L0);
+    const int64_t channels = (int64_t) L0.P * L0.H;
+    for (int64_t s = 0; s < L0.S; s += z.seqs) {
+        ssm_scan_launch L = L0;
+        L.S = std::min(z.seqs, L0.S - s);
+        L.x += s * L.x_s; L.dt += s * L.dt_s; L.B += s * L.b_s; L.C += s * L.c_s; L.ids += s * L.ids_s;
+        L.y += s * channels * L.T; L.s_out += s * channels * L.N;
+        if (z.nk == 8) launch_mm<8>(L, z, ws, st);
+        else if (z.nk == 4) launch_mm<4>(L, z, ws, st);
+        else if (z.nk == 2) launch_mm<2>(L, z, ws, st);
+        else launch_mm<1>(L, z, ws, st);
+    }
 }

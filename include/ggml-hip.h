@@ -32,7 +32,7 @@ GGML_API ggml_backend_buffer_type_t ggml_backend_hip_buffer_type(int device);
 // ggml_backend_graph_compute without any device allocation: no counterpart in the reference; for
 // callers that cannot allocate (serving loops, harnesses that forbid hipMalloc). The kernels'
 // scratch (attention scores and partials, quantized activations, expert groups, argmax parts, scans'
-// prepared operands and segment states: up to 96 MiB and two copies of the sequences' states)
+// prepared operands and segment states: ggml_backend_hip_scan_scratch of the largest scan)
 // comes from a file-scope device array of GGML_HIP_STATIC_SCRATCH_BYTES that every GPU the
 // library runs on holds until the process ends; the graph's tensors are the caller's as with
 // ggml_backend_graph_compute, and the result is the same. Like ggml_backend_graph_compute it
@@ -101,6 +101,12 @@ GGML_API enum ggml_status ggml_backend_hip_logprobs(ggml_backend_t backend, cons
 // answers with GGML_STATUS_FAILED and this message. Needs no device. Other ops' conditions are
 // checked as they run.
 GGML_API const char * ggml_backend_hip_refusal(const struct ggml_tensor * node);
+
+// The device scratch that a graph with this ssm_scan node takes for it, in bytes (its scans share one
+// such area, the largest's): at most 96 MiB, and, where a sequence's tokens take more than that in
+// prepared operands, two copies of the states of the sequences that go through at once. 0 for other
+// nodes and for one that is refused. Needs no device.
+GGML_API size_t ggml_backend_hip_scan_scratch(const struct ggml_tensor * node);
 
 // Graph-level fusion (fused norm+quantize, QKV/gate-up multi-GEMV, rope+KV append, split-KV
 // decode attention). On by default; off runs one kernel per ggml node. Used by the parity tests

@@ -409,6 +409,46 @@ def test_static_compute(hip):
         assert np.array_equal(g.read(n), want)
 
 
+def static(g, hip, *nodes):
+    gf = g.core.ggml_new_graph(g.ctx)
+    for n in nodes:
+        g.core.ggml_build_forward_expand(gf, n)
+    return gl.libs()["hip"].ggml_backend_hip_graph_compute_static(hip, gf)
+
+
+@pytest.mark.parametrize("S, T, H, P, N, G, pool, a0", [(150, 41, 8, 4, 256, 8, 150, 1), (150, 130, 8, 4, 200, 8, 150, 1), (61, 70, 16, 5, 100, 16, 64, 1)])
+def test_static_compute_of_many_sequences(hip, S, T, H, P, N, G, pool, a0):
+    """One chunk of all sequences is more than the prepared operands' 64 MiB: they go through in passes, in the
+    caller's scratch too, and each has its own operands, states and results."""
+    d = draw(np.random.default_rng(33), S, T, H, P, N, G, pool, a0)
+    want = check_scan(hip, d)
+    with Graph(mem=1 << 20) as g:
+        n = scan_node(g, d)
+        g.buf = g.core.ggml_backend_alloc_ctx_tensors(g.ctx, hip)
+        for t, v in g.inputs:
+            g.core.ggml_backend_tensor_set(t, ptr(v), 0, v.nbytes)
+        assert static(g, hip, n) == 0
+        assert np.array_equal(g.read(n), want)
+
+
+def test_scans_of_a_graph_share_their_scratch(hip):
+    """Scans whose scratch would not fit the static area together, the larger ones later."""
+    ds = [draw(np.random.default_rng(34 + S), S, 41, 8, 4, 256, 8, S, 1) for S in (20, 40, 50, 56)]
+    with Graph(mem=1 << 20) as g:
+        nodes = [scan_node(g, d) for d in ds]
+        sizes = [gl.libs()["hip"].ggml_backend_hip_scan_scratch(n) for n in nodes]
+        assert sum(sizes) > 136 << 20 and max(sizes) <= 96 << 20
+        g.buf = g.core.ggml_backend_alloc_ctx_tensors(g.ctx, hip)
+        for t, v in g.inputs:
+            g.core.ggml_backend_tensor_set(t, ptr(v), 0, v.nbytes)
+        assert static(g, hip, *nodes) == 0
+        for n, d in zip(nodes, ds):
+            y, h, ye, he = ssm_ref.scan(d["state"][d["ids"]], d["x"], d["dt"], d["A"], d["B"], d["C"])
+            out = g.read(n)
+            near(out[:y.size], y, ye)
+            near(out[y.size:], h, he)
+
+
 def test_refused_graphs_run_nothing(hip, capfd):
     """A refused node fails the whole graph before its first kernel: the copy beside it is not made."""
     with Graph(mem=1 << 20) as g:

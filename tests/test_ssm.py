@@ -100,6 +100,33 @@ def test_refuses_what_no_launch_takes():
         assert "channels" in many(4097, 128, 64) and "channels" in many(1, (1 << 25) + 1, 1) and "channels" in many(1, 1 << 20, 1 << 12)
 
 
+@pytest.mark.parametrize("T", [1, 17, 64, 65, 4096, 1 << 17])
+@pytest.mark.parametrize("S", [1, 2, 33, 96, 512, 4095, 70000])
+@pytest.mark.parametrize("N, P, H, G, a0", [(128, 64, 128, 8, 1), (256, 64, 16, 16, 1), (256, 1, 600, 600, 1), (16, 1, 512, 1, 16), (32, 1, 64, 1, 32),
+                                            (64, 1000, 8, 2, 1), (1, 1, 1, 1, 1)])
+def test_scan_scratch_is_bounded(S, T, N, P, H, G, a0):
+    """96 MiB, and for more than a block of tokens two copies of the states, whatever the number of sequences."""
+    with Graph(mem=1 << 20) as g:
+        n = scan(g, **scan_operands(g, N=N, P=P, H=H, T=T, S=S, G=G, pool=1, a0=a0))
+        got = gl.libs()["hip"].ggml_backend_hip_scan_scratch(n)
+        if refusal(n):
+            assert got == 0
+        elif T <= 64:
+            assert got <= 96 << 20
+        else:
+            assert got <= (96 << 20) + 2 * S * N * P * H * 4
+
+
+def test_scan_scratch_of_other_nodes():
+    with Graph(mem=1 << 20) as g:
+        lib = gl.libs()["hip"]
+        assert lib.ggml_backend_hip_scan_scratch(None) == 0
+        assert lib.ggml_backend_hip_scan_scratch(g.silu(g.tensor(gl.F32, 8))) == 0
+        assert lib.ggml_backend_hip_scan_scratch(scan(g, version=2, **scan_operands(g, T=100))) == 0
+        assert lib.ggml_backend_hip_scan_scratch(scan(g, **scan_operands(g, T=1))) == 0
+        assert lib.ggml_backend_hip_scan_scratch(scan(g, **scan_operands(g, T=100))) > 0
+
+
 def test_other_nodes_are_not_refused():
     with Graph(mem=1 << 20) as g:
         a = g.tensor(gl.F32, 8, 3)
