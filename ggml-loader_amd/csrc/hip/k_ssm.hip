@@ -565,6 +565,7 @@ void launch_ssm_conv(const ssm_conv_launch & L, hipStream_t st) {
 }
 
 int64_t ssm_scan_scratch_bytes(const ssm_scan_launch & L) {
+    if (L.S == 0) return 0;                                    // nothing to launch, and no workgroups to share segments
     if (!channels_take(L)) return ssm_scan_mm_takes(L) ? ssm_scan_mm_scratch_bytes(L) : 0;
     chan_plan P{};
     chan_segments(L, P);

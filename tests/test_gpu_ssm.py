@@ -110,6 +110,22 @@ def test_scan_steps_that_forget_everything(hip, P, N, a0, big):
 
 
 @pytest.mark.parametrize("T", [0, 1, 100])
+@pytest.mark.parametrize("P, N, a0", [(64, 128, 1), (1, 16, 16), (5, 7, 7)])
+def test_scan_of_no_sequences(hip, T, P, N, a0):
+    """A graph whose batch is empty runs, beside one that is not."""
+    d = draw(np.random.default_rng(15), 1, T, 3, P, N, 1, 1, a0)
+    none = dict(d, **{k: d[k][:0] for k in ("x", "dt", "B", "C", "ids")})
+    with Graph(mem=1 << 20) as g:
+        empty, one = scan_node(g, none), scan_node(g, d)
+        assert empty.contents.ne[0] == 0
+        got = g.compute(hip, [empty, one])
+        assert got[0].size == 0
+    y, h, ye, he = ssm_ref.scan(d["state"][d["ids"]], d["x"], d["dt"], d["A"], d["B"], d["C"])
+    near(got[1][:y.size], y, ye)
+    near(got[1][y.size:], h, he)
+
+
+@pytest.mark.parametrize("T", [0, 1, 100])
 def test_scan_decay_of_one_and_growth(hip, T):
     d = draw(np.random.default_rng(10), 1, T, 3, 64, 128, 1, 1, 1)
     d["A"][0], d["A"][1] = 0, 0.05                    # a state that keeps everything, one that grows

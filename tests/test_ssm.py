@@ -117,6 +117,13 @@ def test_scan_scratch_is_bounded(S, T, N, P, H, G, a0):
             assert got <= (96 << 20) + 2 * S * N * P * H * 4
 
 
+@pytest.mark.parametrize("P, a0", [(4, 1), (1, 16)])
+def test_scan_of_no_sequences_takes_no_scratch(P, a0):
+    with Graph(mem=1 << 20) as g:
+        n = scan(g, **scan_operands(g, S=0, T=100, P=P, H=64, G=1, a0=a0))
+        assert refusal(n) is None and gl.libs()["hip"].ggml_backend_hip_scan_scratch(n) == 0
+
+
 def test_scan_scratch_of_other_nodes():
     with Graph(mem=1 << 20) as g:
         lib = gl.libs()["hip"]
