@@ -971,6 +971,15 @@ private:
         return true;
     }
 
+    // reading `t` at node `from` instead of at node `at`: no node between the two (fused ones aside) writes that memory
+    bool may_read_early(int from, int at, const ggml_tensor * t, const std::vector<int> & fused) const {
+        for (int i = from + 1; i < at; i++) {
+            const ggml_tensor * n = g_->nodes[i];
+            if (!is_view_op(n->op) && std::find(fused.begin(), fused.end(), i) == fused.end() && overlap(n, t)) return false;
+        }
+        return true;
+    }
+
     // A convolution's bias and SiLU in its own launch: conv -> add(bias over the channels) -> silu, as far
     // as each has no other reader. Returns the node that the launch writes.
     int conv_epilogue(int conv, ssm_conv_launch & L, std::vector<int> & fused) const {
@@ -993,7 +1002,8 @@ private:
     }
 
     // the launch at node `from` may write node `out`'s memory, where the graph lets memory serve twice: its own
-    // operands lie elsewhere, and so does all that nodes before `out` still read or write
+    // operands lie elsewhere, and so does all that nodes before `out` still read or write; and the bias is by then what
+    // it is at its sum
     bool conv_may_write(int from, int out, std::initializer_list<const ggml_tensor *> reads, const std::vector<int> & fused) const {
         const ggml_tensor * to = g_->nodes[out];
         for (const ggml_tensor * t : reads) {
@@ -1001,7 +1011,7 @@ private:
         }
         for (int f : fused) {
             const ggml_tensor * t = g_->nodes[f];
-            if (t->op == GGML_OP_ADD && overlap(t->src[1], to)) return false;
+            if (t->op == GGML_OP_ADD && (overlap(t->src[1], to) || !may_read_early(from, f, t->src[1], fused))) return false;
         }
         return may_write_early(from, out, to, fused);
     }
@@ -1078,7 +1088,7 @@ private:
             fused.push_back(copy);
         }
         const int out = conv_epilogue(conv, L, fused);
-        if (!conv_may_write(i, out, { st, x, n->src[1] }, fused)) return false;
+        if (!conv_may_write(i, out, { st, x, n->src[1] }, fused) || !may_read_early(i, conv, n->src[1], fused)) return false;
         if (copy >= 0) {
             const ggml_tensor * cp = g_->nodes[copy];
             const bool same = cp->data == st->data && ggml_is_contiguous(st);

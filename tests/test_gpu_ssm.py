@@ -425,6 +425,42 @@ def test_static_compute(hip):
         assert np.array_equal(g.read(n), want)
 
 
+@pytest.mark.parametrize("fusion", [True, False])
+@pytest.mark.parametrize("what", ["bias", "bias of the plain node", "filters"])
+def test_conv_whose_operands_are_written_before_their_use(hip, what, fusion):
+    """A copy into the bias between the convolution and its sum, or into the filters between the joined rows and
+    the convolution, is seen."""
+    rng = np.random.default_rng(44)
+    K, T, D = 4, 30, 96
+    state = rng.standard_normal((1, D, K - 1)).astype(np.float32)
+    rows = rng.standard_normal((1, T, D)).astype(np.float32)
+    w, b, w2, b2 = (rng.standard_normal(s).astype(np.float32) for s in ((D, K), D, (D, K), D))
+    sx = np.concatenate([state, rows.transpose(0, 2, 1)], 2)
+    gl.libs()["hip"].ggml_backend_hip_set_fusion(hip, fusion)
+    try:
+        with Graph(mem=1 << 20) as g:
+            if what == "bias of the plain node":
+                joined = g.tensor(gl.F32, K - 1 + T, D, 1, data=sx)
+            else:
+                joined = g.concat(g.tensor(gl.F32, K - 1, D, 1, data=state), g.transpose(g.tensor(gl.F32, D, T, data=rows)), 0)
+            wt, bt = g.tensor(gl.F32, K, D, data=w), g.tensor(gl.F32, D, data=b)
+            conv = g.ssm_conv(joined, wt)
+            copy = g.cpy(g.tensor(gl.F32, K, D, data=w2), wt) if what == "filters" else g.cpy(g.tensor(gl.F32, D, data=b2), bt)
+            y = g.silu(g.add(conv, bt))
+            gf = g.core.ggml_new_graph(g.ctx)
+            for t in (joined, copy, conv, y) if what == "filters" else (conv, copy, y):
+                g.core.ggml_build_forward_expand(gf, t)
+            g.core.ggml_set_output(y)
+            g.buf = g.core.ggml_backend_alloc_ctx_tensors(g.ctx, hip)
+            for t, v in g.inputs:
+                g.core.ggml_backend_tensor_set(t, ptr(v), 0, v.nbytes)
+            assert g.core.ggml_backend_graph_compute(hip, gf) == 0
+            y = g.read(y)
+    finally:
+        gl.libs()["hip"].ggml_backend_hip_set_fusion(hip, True)
+    near(y, *ssm_ref.conv(sx, w2 if what == "filters" else w, b if what == "filters" else b2, True))
+
+
 def static(g, hip, *nodes):
     gf = g.core.ggml_new_graph(g.ctx)
     for n in nodes:
