@@ -297,7 +297,13 @@ def hip_logprobs(backend, logits_tensor, tokens, *, row: int = 0, n_rows: int | 
     import numpy as np
     if tokens is None and n_rows is None:
         raise ValueError("hip_logprobs: tokens or n_rows")
-    toks = None if tokens is None else np.ascontiguousarray(np.asarray(tokens, dtype=np.int32))
+    if tokens is None:
+        toks = None
+    else:
+        toks = np.asarray(tokens)
+        if toks.size and (toks.dtype.kind not in "iu" or toks.min() < -2 ** 31 or toks.max() >= 2 ** 31):
+            raise ValueError("hip_logprobs: tokens are 32-bit integers")   # not cut to such
+        toks = np.ascontiguousarray(toks, dtype=np.int32)
     n = len(toks) if n_rows is None else n_rows
     if toks is not None and toks.shape != (n,):
         raise ValueError("hip_logprobs: one token per row")

@@ -55,3 +55,20 @@ def test_python_wrapper_checks():
             gl.hip_logprobs(None, t, [1, 2], n_rows=3)
         with pytest.raises(RuntimeError):
             gl.hip_logprobs(None, t, [1, 2])
+
+
+@pytest.mark.parametrize("tokens", [[2 ** 32 + 1], np.array([2 ** 32 + 1]), np.array([-2 ** 32], np.int64), np.array([2 ** 32 - 1], np.uint32),
+                                    [1.5], np.array([1.0], F), [True], ["1"], [[1]], np.array([2 ** 64 - 1], np.uint64)])
+def test_python_wrapper_takes_no_token_for_another(tokens):
+    """A token that is no 32-bit integer is refused, not cut to one that is in range."""
+    with Graph(mem=1 << 20) as g:
+        with pytest.raises(ValueError):
+            gl.hip_logprobs(None, g.tensor(gl.F32, 8, 3), tokens)
+
+
+@pytest.mark.parametrize("tokens", [[1], (1,), np.array([1], np.int64), np.array([1], np.uint8), []])
+def test_python_wrapper_takes_integers_of_any_kind(tokens, capfd):
+    with Graph(mem=1 << 20) as g:
+        with pytest.raises(RuntimeError):
+            gl.hip_logprobs(None, g.tensor(gl.F32, 8, 3), tokens)
+    assert "not a HIP backend" in capfd.readouterr().err
