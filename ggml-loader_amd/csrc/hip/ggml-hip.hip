@@ -524,6 +524,16 @@ const char * node_refusal(const ggml_tensor * n) {
     return nullptr;
 }
 
+// memory that the device's kernels can read and write: for tensors that a caller placed without a buffer
+bool on_device(const void * p, int device) {
+    hipPointerAttribute_t a{};
+    if (hipPointerGetAttributes(&a, p) != hipSuccess) {
+        (void) hipGetLastError();
+        return false;
+    }
+    return a.type == hipMemoryTypeDevice ? a.device == device : a.type == hipMemoryTypeManaged || a.type == hipMemoryTypeHost;
+}
+
 bool graph_refused(const ggml_cgraph * g, int device) {
     for (int i = 0; i < g->n_nodes; i++) {
         const ggml_tensor * n = g->nodes[i];
@@ -534,7 +544,9 @@ bool graph_refused(const ggml_cgraph * g, int device) {
                 if (!t || ggml_nelements(t) == 0) continue;
                 const ggml_backend_buffer_t buf = t->view_src ? t->view_src->buffer : t->buffer;
                 if (!t->data) why = "an operand is not allocated";
-                else if (buf && ggml_backend_buffer_get_type(buf) != ggml_backend_hip_buffer_type(device)) why = "an operand is not in this device's memory";
+                else if (buf ? ggml_backend_buffer_get_type(buf) != ggml_backend_hip_buffer_type(device) : !on_device(t->data, device)) {
+                    why = "an operand is not in this device's memory";
+                }
             }
         }
         if (!why) continue;

@@ -588,3 +588,26 @@ def test_refuses_memory_of_another_backend(hip, capfd):
         assert gl.libs()["hip"].ggml_backend_hip_graph_compute_static(hip, gf) == -1
     gl.libs()["core"].ggml_backend_free(cpu)
     assert "not in this device's memory" in capfd.readouterr().err
+
+
+@pytest.mark.parametrize("which", ["x", "result"])
+def test_refuses_host_memory_without_a_buffer(hip, which, capfd):
+    """A tensor that the caller placed itself has no buffer to tell its memory by: a context's own memory is
+    named, not read or written; device memory runs."""
+    d = draw(np.random.default_rng(7), 1, 2, 2, 4, 8, 1, 1, 1)
+    host = np.zeros(4096, np.float32)
+    with Graph(mem=1 << 20) as g:
+        n = scan_node(g, d)
+        want = g.compute(hip, n)
+        gf = g.core.ggml_new_graph(g.ctx)
+        g.core.ggml_build_forward_expand(gf, n)
+        t = n if which == "result" else n.contents.src[1]
+        held, at = t.contents.buffer, t.contents.data
+        t.contents.buffer = None
+        assert g.core.ggml_backend_graph_compute(hip, gf) == 0
+        t.contents.data = host.ctypes.data
+        assert g.core.ggml_backend_graph_compute(hip, gf) == -1
+        assert gl.libs()["hip"].ggml_backend_hip_graph_compute_static(hip, gf) == -1
+        t.contents.buffer, t.contents.data = held, at
+        assert np.array_equal(g.read(n), want) and not host.any()
+    assert capfd.readouterr().err.count("not in this device's memory") == 2
