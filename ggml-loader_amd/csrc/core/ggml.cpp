@@ -486,8 +486,8 @@ struct ggml_tensor * ggml_ssm_conv(struct ggml_context * ctx, struct ggml_tensor
 struct ggml_tensor * ggml_ssm_scan(struct ggml_context * ctx, struct ggml_tensor * s, struct ggml_tensor * x,
         struct ggml_tensor * dt, struct ggml_tensor * A, struct ggml_tensor * B, struct ggml_tensor * C,
         struct ggml_tensor * ids, int version) {
-    // the states of the sequences, not of the whole pool
-    const int64_t n_state = s->ne[0] * s->ne[1] * s->ne[2] * ids->ne[0];
+    // the states of the sequences, not of the whole pool; a node without ids is built, and refused at compute
+    const int64_t n_state = ids ? s->ne[0] * s->ne[1] * s->ne[2] * ids->ne[0] : ggml_nelements(s);
     ggml_tensor * r = ggml_new_tensor_1d(ctx, GGML_TYPE_F32, ggml_nelements(x) + n_state);
     set_op_param_i32(r, 0, version);
     r->op = GGML_OP_SSM_SCAN;

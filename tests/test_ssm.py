@@ -60,6 +60,14 @@ def test_scan_refuses_an_operand(name, ne, t):
         assert refusal(scan(g, **o))
 
 
+def test_scan_without_ids_is_built_and_refused():
+    with Graph(mem=1 << 20) as g:
+        o = dict(scan_operands(g), ids=None)
+        n = scan(g, **o)
+        assert n.contents.ne[0] == 4 * 6 * 5 * 2 + 16 * 4 * 6 * 3
+        assert "missing" in refusal(n)
+
+
 def test_scan_refuses_strides_it_cannot_read():
     with Graph(mem=1 << 20) as g:
         o = scan_operands(g)
