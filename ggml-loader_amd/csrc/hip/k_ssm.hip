@@ -434,7 +434,8 @@ __global__ __launch_bounds__(64) void ssm_scan_channels_kernel(chan_plan P) {
     scalar_ptr B = (scalar_ptr) (uintptr_t) (L.B + g * L.b_g + s * L.b_s + t0 * L.b_t);
     scalar_ptr C = (scalar_ptr) (uintptr_t) (L.C + g * L.c_g + s * L.c_s + t0 * L.c_t);
     float * y = L.y + hc + (int64_t) L.H * (t0 + L.T * s);
-    float sum = 0.0f;
+    // the segment's time steps, added with what each sum rounds away: a decay over many tokens rounds as one over few
+    float sum = 0.0f, lost = 0.0f, plain = 0.0f;
     auto token = [&](float raw, float xt) {
         const float d = softplus(raw), dx = d * xt;
         float v = 0.0f;
@@ -443,7 +444,12 @@ __global__ __launch_bounds__(64) void ssm_scan_channels_kernel(chan_plan P) {
             st[n] = fmaf(dx, B[n], st[n] * exp2_hw(d * a[n]));
             if (OUT) v = fmaf(st[n], C[n], v);
         }
-        sum += d;
+        if (!OUT) {
+            const float part = d - lost, next = sum + part;
+            lost = (next - sum) - part;
+            sum = next;
+            plain += d;
+        }
         if (OUT) {
             *y = v;                                            // lanes past the last channel store its value again
             y += L.H;
@@ -485,7 +491,7 @@ __global__ __launch_bounds__(64) void ssm_scan_channels_kernel(chan_plan P) {
         const int c = c0 + i * (64 / LANES);
         if (h0 + c < L.H) store4(q + (int64_t) N * (h0 + c) + n4, *(const float4 *) (turn + c * PITCH + n4));
     }
-    if (!OUT && h < L.H) P.sums[(s * P.n_seg + sg) * L.H + h] = sum;
+    if (!OUT && h < L.H) P.sums[(s * P.n_seg + sg) * L.H + h] = plain < INFINITY ? sum : plain;   // past float's range nothing is lost but all
 }
 
 // a thread per channel and state: the segments in order

@@ -217,6 +217,34 @@ def test_scan_that_grows(hip, T, a):
     check_scan(hip, d)
 
 
+@pytest.mark.parametrize("N", [8, 16])
+@pytest.mark.parametrize("inputs", [False, True])
+def test_scan_of_long_segments(hip, N, inputs):
+    """Many channels of one each take few segments of some 200 tokens, whose decays are one sum of time steps: what
+    that rounds may not grow with the tokens, also where they are all alike (the same dt for every token, by a stride
+    of none, so that every rounding may go the same way). A sample of the channels against the recurrence."""
+    rng = np.random.default_rng(N)
+    H, T = 40960, 1400
+    dt = (rng.standard_normal((1, 1, H)) * 0.5 - 2).astype(np.float32)
+    A = -(0.5 + 1.5 * rng.random((H, N))).astype(np.float32)
+    state = rng.standard_normal((1, H, 1, N)).astype(np.float32)
+    x = (rng.standard_normal((1, T, 1, 1)) * inputs).astype(np.float32)
+    B, Cm = (rng.standard_normal((1, T, 1, N)).astype(np.float32) for _ in range(2))
+    with Graph(mem=1 << 20) as g:
+        xt = g.view_4d(g.tensor(gl.F32, T, data=x), 1, 1, T, 1, 4, 4, 4 * T, 0)
+        dtt = g.view_3d(g.tensor(gl.F32, H, data=dt), H, 1, 1, 4 * H, 4 * H, 0)
+        for t, many in ((xt, H), (dtt, T)):
+            t.contents.ne[1], t.contents.nb[1] = many, 0
+        out = g.compute(hip, g.ssm_scan(g.tensor(gl.F32, N, 1, H, 1, data=state), xt, dtt, g.tensor(gl.F32, N, H, data=A),
+                                        g.tensor(gl.F32, N, 1, T, 1, data=B), g.tensor(gl.F32, N, 1, T, 1, data=Cm),
+                                        g.tensor(gl.I32, 1, data=np.zeros(1, np.int32)), 1))
+    some = np.sort(rng.permutation(H)[:256])
+    y, h, ye, he = ssm_ref.scan(state[:, some], np.broadcast_to(x, (1, T, 256, 1)), np.broadcast_to(dt[:, :, some], (1, T, 256)),
+                                A[some], B, Cm)
+    near(out[:T * H].reshape(1, T, H, 1)[:, :, some], y, ye, "y")
+    near(out[T * H:].reshape(1, H, 1, N)[:, some], h, he, "state")
+
+
 # few tokens, channels and states at the edges of what a lane, a wave or a group of rows takes
 FEW = [
     (3, 1, 67, 1, 16, 1, 3, 16), (2, 1, 64, 1, 8, 1, 2, 8), (3, 2, 130, 1, 32, 1, 3, 32), (2, 5, 129, 1, 16, 1, 2, 16), (1, 8, 1, 1, 16, 1, 1, 1),
