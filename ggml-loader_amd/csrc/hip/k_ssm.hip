@@ -154,7 +154,9 @@ __global__ __launch_bounds__(256) void ssm_conv_rows_kernel(ssm_conv_launch L, i
 __global__ __launch_bounds__(256) void ssm_conv_tile_kernel(ssm_conv_launch L, int blocks) {
     extern __shared__ float rows[];
     const int width = 64 + L.K - 1, stride = width | 1, tid = threadIdx.x;
-    const int64_t d0 = (int64_t) (blockIdx.x % (unsigned) blocks) * 64, t0 = (int64_t) (blockIdx.x / (unsigned) blocks) * 64;
+    const unsigned tile = blockIdx.z * gridDim.x + blockIdx.x;
+    const int64_t d0 = (int64_t) (tile % (unsigned) blocks) * 64, t0 = (int64_t) (tile / (unsigned) blocks) * 64;
+    if (t0 >= L.T) return;                                     // past the last tile
     const int nd = (int) min((int64_t) 64, L.D - d0), nt = (int) min((int64_t) 64, L.T - t0);
     for (int64_t s = blockIdx.y; s < L.S; s += gridDim.y) {
         __syncthreads();
@@ -566,8 +568,10 @@ void launch_ssm_conv(const ssm_conv_launch & L, hipStream_t st) {
     }
     const int blocks = (int) ((L.D + 63) / 64);
     const size_t lds = sizeof(float) * (64 * ((64 + L.K - 1) | 1) + 64 * (L.K - 1));
-    launch(ssm_conv_tile_kernel, dim3((unsigned) (blocks * ((L.T + 63) / 64)), (unsigned) std::min<int64_t>(L.S, 65535)), dim3(256), lds, st,
-           L, blocks);
+    // up to 2^25 tiles; a dimension of the grid has less than 2^32 threads
+    const int64_t tiles = blocks * ((L.T + 63) / 64), across = std::min<int64_t>(tiles, 1 << 22);
+    launch(ssm_conv_tile_kernel, dim3((unsigned) across, (unsigned) std::min<int64_t>(L.S, 65535), (unsigned) ((tiles + across - 1) / across)),
+           dim3(256), lds, st, L, blocks);
 }
 
 int64_t ssm_scan_scratch_bytes(const ssm_scan_launch & L) {

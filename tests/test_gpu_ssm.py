@@ -331,6 +331,32 @@ def test_conv_of_strided_operands(hip):
     near(out, *ssm_ref.conv(rows[:, 2:2 + D].T[None], w[:, :K]))
 
 
+def test_conv_of_most_channels(hip):
+    """2^30 + 5 channels of one token are more tiles than one dimension of a launch has; every channel reads the same
+    rows and the same filter, by strides of none. The ends and a sample are read back."""
+    K, T, D = 5, 1, (1 << 30) + 5
+    rng = np.random.default_rng(22)
+    sx, w = rng.standard_normal((1, 1, K - 1 + T)).astype(np.float32), rng.standard_normal((1, K)).astype(np.float32)
+    with Graph(mem=1 << 20) as g:
+        sxt = g.view_3d(g.tensor(gl.F32, K - 1 + T, data=sx), K - 1 + T, 1, 1, 4 * (K - 1 + T), 4 * (K - 1 + T), 0)
+        wt = g.view_2d(g.tensor(gl.F32, K, data=w), K, 1, 4 * K, 0)
+        for t in (sxt, wt):
+            t.contents.ne[1], t.contents.nb[1] = D, 0
+        n = g.ssm_conv(sxt, wt)
+        gf = g.core.ggml_new_graph(g.ctx)
+        g.core.ggml_build_forward_expand(gf, n)
+        g.buf = g.core.ggml_backend_alloc_ctx_tensors(g.ctx, hip)
+        assert g.buf
+        for t, v in g.inputs:
+            g.core.ggml_backend_tensor_set(t, ptr(v), 0, v.nbytes)
+        assert g.core.ggml_backend_graph_compute(hip, gf) == 0
+        y, bound = ssm_ref.conv(sx, w)
+        for at in (0, (1 << 28) - 500, (1 << 28) + 64, 3 << 28, D - 1000):
+            got = np.zeros(1000, np.float32)
+            g.core.ggml_backend_tensor_get(n, ptr(got), 4 * at, got.nbytes)
+            near(got, np.full(1000, y[0, 0, 0]), bound[0, 0, 0], at)
+
+
 class Mixer:
     """The convolution with its state, bias and SiLU as a mixer's graph has it. In place: the new rows
     go back into the state they came from."""
