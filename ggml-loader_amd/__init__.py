@@ -297,13 +297,13 @@ def hip_logprobs(backend, logits_tensor, tokens, *, row: int = 0, n_rows: int | 
     import numpy as np
     if tokens is None and n_rows is None:
         raise ValueError("hip_logprobs: tokens or n_rows")
-    if tokens is None:
-        toks = None
-    else:
-        toks = np.asarray(tokens)
+    toks = None if tokens is None else np.asarray(tokens)
+    if toks is not None and toks.dtype != np.int32:
         if toks.size and (toks.dtype.kind not in "iu" or toks.min() < -2 ** 31 or toks.max() >= 2 ** 31):
             raise ValueError("hip_logprobs: tokens are 32-bit integers")   # not cut to such
-        toks = np.ascontiguousarray(toks, dtype=np.int32)
+        toks = toks.astype(np.int32)
+    if toks is not None:
+        toks = np.ascontiguousarray(toks)
     n = len(toks) if n_rows is None else n_rows
     if toks is not None and toks.shape != (n,):
         raise ValueError("hip_logprobs: one token per row")
