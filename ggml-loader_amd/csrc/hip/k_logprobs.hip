@@ -25,6 +25,7 @@ constexpr int LP_WAVES = LP_THREADS / WAVE;
 constexpr int LP_PER = 32;                        // logits per thread, in groups of 4
 constexpr int LP_SEG = LP_THREADS * LP_PER;
 constexpr int LP_CAND = 1024;                     // entries a selection sorts
+constexpr int LP_KEPT = 6144;                     // entries a join sorts: 48 KiB
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
 // ascending order key of a float; -0 and +0 share a key
@@ -338,28 +339,41 @@ __global__ __launch_bounds__(LP_THREADS) void logprobs_join_kernel(logprobs_laun
     const float ls = log_sum(a);
     if (tid == 0) put_scores(L, tok, a, ls, o);
     auto put = [&](int rank, uint64_t key) { put_top(L, a.m, ls, o, rank, key); };
-    if (L.stage) {
-        auto keep = [&](uint64_t key) {
-            if (key >= t) kept[atomicAdd(&count, 1)] = key;
-        };
-        if (tid < total) keep(first[0]);
-        if (tid + LP_THREADS < total) keep(first[1]);
-        for (int i = tid + 2 * LP_THREADS; i < total; i += LP_THREADS) keep(keys[i]);
-        __syncthreads();
-        const int n = count;
-        if (tid < (-n & 3)) kept[n + tid] = 0;
-        __syncthreads();
-        rank_keys(kept, n, L.k, put);
-    } else {
-        // a very long row: its lists stay where they are
-        for (int i = tid; i < total; i += LP_THREADS) {
-            const uint64_t mine = keys[i];
-            if (mine < t || !mine) continue;
-            int rank = 0;
-            for (int j = 0; j < total; j++) rank += keys[j] > mine ? 1 : 0;
-            if (rank < L.k) put(rank, mine);
+    auto keep = [&](uint64_t key) {
+        if (key < t) return;
+        const int i = atomicAdd(&count, 1);
+        if (i < LP_KEPT) kept[i] = key;
+    };
+    if (tid < total) keep(first[0]);
+    if (tid + LP_THREADS < total) keep(first[1]);
+    for (int i = tid + 2 * LP_THREADS; i < total; i += LP_THREADS) keep(keys[i]);
+    __syncthreads();
+    if (count > LP_KEPT) {
+        // too many to compare each with all (a very long row, or one of whose segments nothing is left): t becomes the
+        // k-th largest, by bisection; the entries differ by their ids, so k are kept
+        uint64_t hi = ~(uint64_t) 0;
+        int * parts = (int *) kept;
+        for (int turn = 0; t < hi; turn ^= LP_WAVES) {
+            const uint64_t mid = t + (hi - t) / 2 + 1;
+            int n = 0;
+            for (int i = tid; i < total; i += LP_THREADS) n += keys[i] >= mid ? 1 : 0;
+            n = wave_sum(n);
+            if (tid % WAVE == 0) parts[turn + tid / WAVE] = n;
+            __syncthreads();
+            n = (parts[turn] + parts[turn + 1]) + (parts[turn + 2] + parts[turn + 3]);
+            if (n >= L.k) t = mid;
+            else hi = mid - 1;
         }
+        __syncthreads();
+        if (tid == 0) count = 0;
+        __syncthreads();
+        for (int i = tid; i < total; i += LP_THREADS) keep(keys[i]);
+        __syncthreads();
     }
+    const int n = count;
+    if (tid < (-n & 3)) kept[n + tid] = 0;
+    __syncthreads();
+    rank_keys(kept, n, L.k, put);
     store_row(L, r, o);
 }
 
@@ -381,8 +395,7 @@ void launch_logprobs(const logprobs_launch & L0, hipStream_t st) {
     launch(logprobs_segment_kernel, dim3((unsigned) L.n_seg, (unsigned) L.n_rows),
            dim3(LP_THREADS), 0, st, L);
     if (L.n_seg > 1) {
-        const size_t lds = ((size_t) L.n_seg * L.k + 3) * 8;
-        L.stage = lds <= 48 << 10;
-        launch(logprobs_join_kernel, dim3((unsigned) L.n_rows), dim3(LP_THREADS), L.stage ? lds : 0, st, L);
+        const size_t lds = (std::min<size_t>((size_t) L.n_seg * L.k, LP_KEPT) + 3) * 8;
+        launch(logprobs_join_kernel, dim3((unsigned) L.n_rows), dim3(LP_THREADS), lds, st, L);
     }
 }

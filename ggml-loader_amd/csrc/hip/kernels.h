@@ -620,7 +620,7 @@ struct logprobs_launch {
     const int32_t * tokens;
     float *         out;
     void *          part;
-    int             seg, n_seg, stage;   // set by the launcher
+    int             seg, n_seg;   // set by the launcher
 };
 int64_t logprobs_scratch_bytes(int n, int k, int n_rows);
 void launch_logprobs(const logprobs_launch & L, hipStream_t st);

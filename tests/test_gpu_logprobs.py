@@ -150,6 +150,20 @@ def test_the_last_of_the_likeliest_among_equals(hip, n, n_top):
     check(hip, x, rng.integers(0, n, 6), n_top)
 
 
+@pytest.mark.parametrize("n_top", [1, 20, 128])
+def test_very_long_rows(hip, n_top):
+    """Rows of so many segments that their lists are too long to compare each entry with all: an ordinary row, one
+    with segments that hold nothing, one with few values that are all equal, and equal values throughout."""
+    n = 4_200_001
+    rng = np.random.default_rng(n_top)
+    x = (rng.standard_normal((4, n), dtype=np.float32) * 3)
+    x[1, 100_000:150_000] = -np.inf
+    x[2] = -np.inf
+    x[2, rng.permutation(n)[:n_top // 2 + 1]] = 1.0
+    x[3] = np.round(x[3])
+    check(hip, x, rng.integers(0, n, 4), n_top)
+
+
 def test_a_banned_token(hip):
     x = np.array([[0, -np.inf, 1]], np.float32)
     got = check(hip, x, np.array([1]), 3)
