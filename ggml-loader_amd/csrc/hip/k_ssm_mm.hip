@@ -24,7 +24,7 @@
 // token's that counts, with the spread of X: outputs are wrong by 2^-52 of the largest |C_t . B_j| |X_j| before
 // decay at most, which shows only where all inputs but zeros have decayed by more than 2^30.
 // (With one sum for all three products and 2^12 for the largest, halves held 22 bits down to 2^-15 and a later
-// value of 1e8 put the outputs before it off by 1e-3; that took 180 us instead of 200 at the first size below.)
+// value of 1e8 put the outputs before it off by 1e-3; that took 180 us instead of 196 at the first size below.)
 //
 // Three launches. ssm_prepare_kernel, per (sequence, chunk, group): C and B split into the order in which the
 // lanes of a matrix instruction hold them, and the products C_t . B_j, which the group's heads share; per
@@ -35,8 +35,8 @@
 // chunk's product reads it from, when the k index of that product runs n = 4 g + i, then 16 + 4 g + i over lane
 // group g, the order that C is prepared in. Eight waves share a chunk's operands.
 //
-// 4096 tokens of 128 heads x 64 x 128, 8 groups: 200 us (1.56 TB/s of what must be read and written, whose floor
-// is 61 us; 23 + 51 + 141 in a trace), 333 tokens of 24 heads 35. Before the halves' range was widened these were 180
+// 4096 tokens of 128 heads x 64 x 128, 8 groups: 196 us (1.59 TB/s of what must be read and written, whose floor
+// is 61 us; 22 + 48 + 130 in a trace), 333 tokens of 24 heads 35. Before the halves' range was widened these were 180
 // and 32, and then nothing was saturated: the matrix cores were busy for a fifth of the time, the vector units for two
 // fifths and LDS for a quarter, and leaving any one part out (the loads of x or of the operands, the update of the
 // state, the stores) saved a tenth each, so a chunk's barriers and the latency between its parts were what was left.
@@ -76,8 +76,8 @@ __device__ __forceinline__ float finite_abs(float x) { return fabsf(x) < INFINIT
 // The smallest magnitude other than 0 is that of the least key, a NaN where there is none (and less a unit).
 __device__ __forceinline__ uint32_t least_key(float x) { return (__float_as_uint(x) << 1) - 1; }
 __device__ __forceinline__ float least_value(uint32_t key) { return __uint_as_float(key >> 1); }
-// and the largest that of the largest of these, where a NaN is above an infinity
-__device__ __forceinline__ int most_key(float x) { return (int) (__float_as_uint(x) & 0x7fffffffu); }
+// the larger one of a magnitude so far and another, and a NaN where there is one
+__device__ __forceinline__ float most_of(float most, float x) { return __builtin_elementwise_maximum(most, fabsf(x)); }
 // whether values are finite and the smallest other than 0 so near the largest that halves hold each to 2^-19
 __device__ __forceinline__ bool in_range(float least, float most) { return most < INFINITY && !(least * 0x1p33f < most); }
 
@@ -164,17 +164,17 @@ __device__ __forceinline__ void prepare_operands(const mm_plan & P, int c, int g
 #pragma unroll
     for (int o = 0; o < 2; o++) {
         uint32_t key = ~0u;
-        int top = 0;
+        float m = 0.0f;
 #pragma unroll
         for (int q = 0; q < NK; q++) {
 #pragma unroll
             for (int i = 0; i < 8; i++) {
                 v[o][q][i] = t < left ? v[o][q][i] : 0.0f;
-                top = max(top, most_key(v[o][q][i]));
+                m = most_of(m, v[o][q][i]);
                 key = min(key, least_key(v[o][q][i]));
             }
         }
-        const float m = __int_as_float(top), most = wave_max(m < INFINITY ? m : INFINITY), least = -wave_max(-least_value(key));
+        const float most = wave_max(m < INFINITY ? m : INFINITY), least = -wave_max(-least_value(key));
         if (lane == 0) {
             red[o * 4 + wave] = most;
             red[8 + o * 4 + wave] = least;
@@ -470,8 +470,9 @@ __global__ __launch_bounds__(THREADS, 2) void ssm_scan_mm_kernel(mm_plan P) {
 
     // what the next chunk reads
     // The operands' planes a chunk ahead too, or only once the chunk before is done: the registers that hold them are
-    // those that outputs of 128 and more states lack. 3 x 1625 tokens of 36 x 64 x 64 63.7 us ahead and 66.8 late;
-    // 1402 of 64 x 80 x 128 67.5 and 66.1; 3 x 586 of 30 x 128 x 256 128 (94 registers spilled) and 96.
+    // those that outputs of 256 states lack: 4096 tokens of 128 x 64 x 256 464 us late and 702 ahead, 3 x 586 of 30 x
+    // 128 x 256 110 and 152. 128 states don't care (196 and 198 us; 77 both at 1402 of 64 x 80), 64 and fewer have
+    // the registers.
     constexpr bool EARLY = !OUT || NK < 4;
     uint4v stage_c[OUT && EARLY ? STAGE : 1], stage_b[EARLY ? STAGE : 1];
     float4v gg[2][2];
@@ -575,6 +576,7 @@ __global__ __launch_bounds__(THREADS, 2) void ssm_scan_mm_kernel(mm_plan P) {
             }
         } else {
             // C's planes, then B's, in the record
+            static_assert(2 * STAGE % 8 == 0, "eight pieces at a time");
             const char * planes = at_planes - L.G * rec_bytes<NK>() + tid * 16;
             char * to[2] = { cbuf + tid * 16, bbuf + turn % SLOTS * OPERAND - OPERAND + tid * 16 };
 #pragma unroll
@@ -594,8 +596,10 @@ __global__ __launch_bounds__(THREADS, 2) void ssm_scan_mm_kernel(mm_plan P) {
     };
 
     // The chunk by its recurrence, in float32 throughout: for operands whose halves would lose a value beside a larger
-    // one. 16 states after another go through all tokens, which takes few registers beside the main path's: a lane's
-    // four of its channel, whose output so far stays in memory.
+    // one. 16 states after another go through all tokens, a lane's four of its channel, whose output so far stays in
+    // memory; the next ones take their registers' place, so that this takes one loop's code and few registers beside
+    // the main path's. Where every chunk comes here, 4096 tokens of 128 x 64 x 128 take 8.1 ms, as the kernel for
+    // any operands does.
     auto by_tokens = [&](int c, const float * my) {
         const plan_ptr K = plan_here();
         const uint32_t n0 = here(4 * grp), p0 = here(pch);
@@ -603,27 +607,30 @@ __global__ __launch_bounds__(THREADS, 2) void ssm_scan_mm_kernel(mm_plan P) {
         const float a = K->L.A[h1 * K->L.a_h] * LOG2E;
         const int64_t row = K->t0 + c * Q;
         const int n_t = min(Q, K->T - c * Q);
-#pragma unroll
+#pragma unroll 1
         for (int nt = 0; nt < 2 * NK; nt++) {
-            if (16 * nt >= K->L.N) break;
+            float4v st = S[0];
             const float * xp = K->L.x + h1 * K->L.x_h + s1 * K->L.x_s + row * K->L.x_t;
             const float * bp = K->L.B + g1 * K->L.b_g + s1 * K->L.b_s + row * K->L.b_t + 16 * nt;
             const float * cp = K->L.C + g1 * K->L.c_g + s1 * K->L.c_s + row * K->L.c_t + 16 * nt;
             float * y = K->L.y + (int64_t) K->L.P * (h1 + (int64_t) K->L.H * (row + K->L.T * s1));
             const int left = K->L.N - 16 * nt;
 #pragma unroll 1
-            for (int t = 0; t < n_t; t++, xp += K->L.x_t, bp += K->L.b_t, cp += K->L.c_t, y += (int64_t) K->L.P * K->L.H) {
+            for (int t = 0; t < n_t && left > 0; t++, xp += K->L.x_t, bp += K->L.b_t, cp += K->L.c_t, y += (int64_t) K->L.P * K->L.H) {
                 const float d = my[2 * Q + t], e = exp2_hw(d * a), dx = d * xp[p0];
                 const float4v b = states4(bp, (int) n0, left), f = OUT ? states4(cp, (int) n0, left) : b;
 #pragma unroll
-                for (int i = 0; i < 4; i++) S[nt][i] = fmaf(S[nt][i], e, dx * b[i]);
+                for (int i = 0; i < 4; i++) st[i] = fmaf(st[i], e, dx * b[i]);
                 if (OUT) {
-                    float v = fmaf(S[nt][0], f[0], S[nt][1] * f[1]) + fmaf(S[nt][2], f[2], S[nt][3] * f[3]);
+                    float v = fmaf(st[0], f[0], st[1] * f[1]) + fmaf(st[2], f[2], st[3] * f[3]);
                     v += __shfl_xor(v, 16, WAVE);
                     v += __shfl_xor(v, 32, WAVE);
                     if (pok && grp == 0) y[p0] = nt == 0 ? v : y[p0] + v;
                 }
             }
+#pragma unroll
+            for (int i = 0; i + 1 < 2 * NK; i++) S[i] = S[i + 1];
+            S[2 * NK - 1] = st;
         }
     };
 
@@ -702,17 +709,17 @@ __global__ __launch_bounds__(THREADS, 2) void ssm_scan_mm_kernel(mm_plan P) {
             }
         }
         // whether halves do for the wave's channels
-        int top = 0;
+        float own = 0.0f;
         uint32_t key = ~0u;
 #pragma unroll
         for (int ks = 0; ks < 2; ks++) {
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                top = max(top, most_key(x[ks][i]));
+                own = most_of(own, x[ks][i]);
                 key = min(key, least_key(x[ks][i]));
             }
         }
-        const float own = __int_as_float(top), most = column_max(own < INFINITY ? own : INFINITY);
+        const float most = column_max(own < INFINITY ? own : INFINITY);
         const float growth = fmaxf(1.0f, e_last);              // a decay above 1 grows all through a chunk
         bool fine = in_range(least_value(key), most * (spread * growth)) && gmost * growth < INFINITY;
         half8 xh[2], xl[2];
