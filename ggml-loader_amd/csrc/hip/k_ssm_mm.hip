@@ -598,7 +598,7 @@ __global__ __launch_bounds__(THREADS, 2) void ssm_scan_mm_kernel(mm_plan P) {
     // The chunk by its recurrence, in float32 throughout: for operands whose halves would lose a value beside a larger
     // one. 16 states after another go through all tokens, a lane's four of its channel, whose output so far stays in
     // memory; the next ones take their registers' place, so that this takes one loop's code and few registers beside
-    // the main path's. Where every chunk comes here, 4096 tokens of 128 x 64 x 128 take 8.1 ms, as the kernel for
+    // the main path's. Where every chunk comes here, 4096 tokens of 128 x 64 x 128 take 8.3 ms, as the kernel for
     // any operands does.
     auto by_tokens = [&](int c, const float * my) {
         const plan_ptr K = plan_here();
@@ -1011,14 +1011,15 @@ void launch_mm(const ssm_scan_launch & L, const mm_sizes & z, void * ws, hipStre
     }
 }
 
-// Up to so many tokens the recurrence itself is faster: products need an operand and a chunk's latency, 12 us with
-// 32 states, 20 with 128 and 31 with 256, and a step takes 0.5 to 0.6 us. 80 heads of 64 channels and 128 states: 16
-// tokens 13.1 us by steps and 20.6 by products, 24 17.8 and 20.8, 32 22.5 and 20.8; 24 heads of 32 states 16 tokens
-// 11.2 and 12.6, 24 15.3 and 12.6; of 256 states 32 tokens 25.6 and 31.2, 48 36.3 and 31.6. Where channels fill the chip a step takes
-// longer and the latency doesn't count: 163840 channels of 128 states 16 tokens 75.7 and 80.6, 24 106.8 and 80.8.
+// Up to so many tokens the recurrence itself is faster: products need an operand's preparation and a chunk's latency, 14
+// us with 32 states, 17 with 64, 22 with 128 and 38 with 256, and a step takes 0.5 to 0.7 us (24 heads of 64 channels and 32
+// states: 20 tokens 13.1 us by steps and 14.1 by products, 22 14.2 both; 80 heads of 64 states 24 15.9 and 17.0, 28 18.0
+// and 17.1; of 128 28 20.3 and 22.1, 32 22.5 and 22.3; of 256 44 36.4 and 38.0, 48 39.1 and 37.6). Where channels fill the
+// chip a step takes longer and the latency doesn't count, whatever the states: 163840 channels of 128 states 18 tokens
+// 94.5 and 97.8, 20 99.8 and 97.7; of 64 16 52 and 65 with 2.4 a step; 81920 of 256 26 127.5 and 99.9 with 4.
 int step_tokens(const ssm_scan_launch & L) {
-    const int few = L.N <= 64 ? 16 : L.N <= 128 ? 24 : 40;
-    return L.S * (int64_t) L.H * L.P > 65536 ? few * 2 / 3 : few;
+    const int few = L.N <= 32 ? 21 : L.N <= 64 ? 26 : L.N <= 128 ? 31 : 46;
+    return L.S * (int64_t) L.H * L.P > 65536 ? std::min(few, 19) : few;
 }
 
 } // namespace

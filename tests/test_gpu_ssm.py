@@ -522,7 +522,7 @@ def static(g, hip, *nodes):
     return gl.libs()["hip"].ggml_backend_hip_graph_compute_static(hip, gf)
 
 
-@pytest.mark.parametrize("S, T, H, P, N, G, pool, a0", [(150, 41, 8, 4, 256, 8, 150, 1), (150, 130, 8, 4, 200, 8, 150, 1), (61, 70, 16, 5, 100, 16, 64, 1)])
+@pytest.mark.parametrize("S, T, H, P, N, G, pool, a0", [(150, 50, 8, 4, 256, 8, 150, 1), (150, 130, 8, 4, 200, 8, 150, 1), (61, 70, 16, 5, 100, 16, 64, 1)])
 def test_static_compute_of_many_sequences(hip, S, T, H, P, N, G, pool, a0):
     """One chunk of all sequences is more than the prepared operands' 64 MiB: they go through in passes, in the
     caller's scratch too, and each has its own operands, states and results."""
@@ -539,7 +539,7 @@ def test_static_compute_of_many_sequences(hip, S, T, H, P, N, G, pool, a0):
 
 def test_scans_of_a_graph_share_their_scratch(hip):
     """Scans whose scratch would not fit the static area together, the larger ones later."""
-    ds = [draw(np.random.default_rng(34 + S), S, 41, 8, 4, 256, 8, S, 1) for S in (20, 40, 50, 56)]
+    ds = [draw(np.random.default_rng(34 + S), S, 50, 8, 4, 256, 8, S, 1) for S in (20, 40, 50, 56)]
     with Graph(mem=1 << 20) as g:
         nodes = [scan_node(g, d) for d in ds]
         sizes = [gl.libs()["hip"].ggml_backend_hip_scan_scratch(n) for n in nodes]
