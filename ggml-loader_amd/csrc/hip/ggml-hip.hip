@@ -948,7 +948,7 @@ private:
                 }
                 return;
             }
-                        case GGML_OP_SSM_SCAN: op_ssm_scan(n); return;
+            case GGML_OP_SSM_SCAN: op_ssm_scan(n); return;
             default:
                 HIP_ABORT("op %s is not supported by the hip backend (node '%s')", ggml_op_name(n->op), n->name);
         }

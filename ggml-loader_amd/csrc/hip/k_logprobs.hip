@@ -74,8 +74,9 @@ __device__ __forceinline__ void rank_keys(const uint64_t * keys, int n, int k, F
 // The k best of a workgroup's LP_SEG values (v[4 j + c] is entry j * 1024 + thread * 4 + c; the ones
 // from `valid` on are -inf), in order, to out(rank, key): every rank below k, key 0 where there are
 // fewer entries. best: the thread's largest value.
-// A threshold first: of M >= 2 k groups of threads, each with its largest value, the k-th largest, t, has k
-// entries at or above it and few more (with evenly spread values and k = 20 of 64 groups about 24). The entries
+// A threshold first: of M groups of threads, each with its largest value, the k-th largest, t, has k entries at or
+// above it and few more (with evenly spread values and k = 20 of 64 groups about 24). M is 64 up to k = 32 and 256
+// above; up to k = 8 it is 8 or 4, at least k, and t the least of all, which takes no comparing. The entries
 // from t on are listed and each finds its rank by comparing with all. Were the list too long (values that the
 // groups do not share evenly, such as a block of -inf, or many equal ones), t becomes the k-th largest value
 // itself, found by bisection: fewer than k entries lie above it, and ones equal to it follow in the order of
@@ -224,7 +225,7 @@ __device__ __forceinline__ float log_sum(const lp_stats & a) { return a.bad != 0
 // memory, where each separate store would be a bus transfer of its own.
 struct lp_out { float w[2 + 2 * LOGPROBS_MAX_TOP]; };
 
-__device__ __forceinline__ void put_scores(const logprobs_launch & L, float tok, const lp_stats & a, float ls, lp_out & o) {
+__device__ __forceinline__ void put_scores(float tok, const lp_stats & a, float ls, lp_out & o) {
     o.w[0] = tok - a.m - ls;
     o.w[1] = ls - a.w / a.s;
 }
@@ -287,7 +288,7 @@ __global__ __launch_bounds__(LP_THREADS) void logprobs_segment_kernel(logprobs_l
     }
     if (L.n_seg == 1) {
         const float ls = log_sum(a);
-        if (tid == 0) put_scores(L, L.tokens ? x[L.tokens[r]] : 0.0f, a, ls, o);
+        if (tid == 0) put_scores(L.tokens ? x[L.tokens[r]] : 0.0f, a, ls, o);
         if (L.k) select_top(v, best, valid, 0, L.k, S, [&](int rank, uint64_t key) { put_top(L, a.m, ls, o, rank, key); });
         store_row(L, r, o);
         return;
@@ -300,7 +301,7 @@ __global__ __launch_bounds__(LP_THREADS) void logprobs_segment_kernel(logprobs_l
 
 // A row's segments joined. Their lists hold n_seg * k entries in descending order; the q best of each,
 // q = ceil(k / n_seg), are at least k, so entries below the smallest of the lists' q-th are out (about
-// 50 of 380 stay for 19 segments and k = 20). What stays is ranked by comparing with all.
+// 50 of 380 stay for 19 segments and k = 20). What stays is ranked by comparing each with all.
 __global__ __launch_bounds__(LP_THREADS) void logprobs_join_kernel(logprobs_launch L) {
     extern __shared__ __align__(16) uint64_t kept[];
     __shared__ lp_out o;
@@ -337,7 +338,7 @@ __global__ __launch_bounds__(LP_THREADS) void logprobs_join_kernel(logprobs_laun
     a = join(join(all[0], all[1]), join(all[2], all[3]));
     t = min(min(least[0], least[1]), min(least[2], least[3]));
     const float ls = log_sum(a);
-    if (tid == 0) put_scores(L, tok, a, ls, o);
+    if (tid == 0) put_scores(tok, a, ls, o);
     auto put = [&](int rank, uint64_t key) { put_top(L, a.m, ls, o, rank, key); };
     auto keep = [&](uint64_t key) {
         if (key < t) return;

@@ -15,7 +15,8 @@ namespace {
 // the order of the rows: channels next to each other (a projection's rows, as the executor's fused
 // form has them) need no exchange between lanes; steps next to each other (the joined rows of the
 // plain node) are turned round in LDS. A step of one token is latency: one round of loads. 4096 tokens of 10240
-// channels and 4 taps: 62.9 us by rows (5.3 TB/s), 146 by tiles.
+// channels and 4 taps, which are read and written once: 66.3 us by rows (5.06 TB/s; 63 on the same rows again), 146
+// by tiles, which divide by the rows' width for each value and load four bytes at a time.
 
 __device__ __forceinline__ float silu(float v) { return v * __builtin_amdgcn_rcpf(1.0f + exp2_hw(-v * LOG2E)); }
 
@@ -40,7 +41,8 @@ template <int V> __device__ __forceinline__ void stv(float * p, const chunk<V> &
 // it may be the old one's own memory.
 // PACK: filters and a sequence's states contiguous, so that a thread's four of each are K or K - 1 float4s. Four
 // channels a thread only where they are: 64 tokens of 5120 channels take 5.2 us so, 5.5 with a channel each,
-// and 8.9 with four of which each loads its filter and state by dwords; 4096 tokens of 10240 62.9, 73.4 and 76.1.
+// and 8.9 with four of which each loads its filter and state by dwords; 4096 tokens of 10240 62.9, 73.4
+// and 76.1, each on the same rows again.
 template <int K, int V, int TT, bool PACK>
 __device__ __forceinline__ void conv_rows(const ssm_conv_launch & L, int64_t t0, int64_t d) {
     float w[V][K];
@@ -373,7 +375,7 @@ void launch_step(const ssm_scan_launch & L, hipStream_t st) {
 // channels and 16 states took 32 us a token, with it 12.1, 4.8 TB/s; the kernel for few tokens took 15.7).
 // Where channels alone are too few waves the tokens are split into segments: `local` finds each segment's final
 // state from nothing and its sum of time steps, `join` the state that each begins with, and the last launch the
-// outputs (73.5 us at 1500 tokens of 5120 channels: 28, 10 and 37). The first pass repeats 7/8 of the work;
+// outputs (74.7 us at 1500 tokens of 5120 channels: 29, 10 and 37). The first pass repeats 7/8 of the work;
 // carrying its outputs over would take as many exponentials again.
 struct chan_plan {
     ssm_scan_launch L;

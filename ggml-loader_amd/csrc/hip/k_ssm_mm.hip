@@ -36,7 +36,7 @@
 // group g, the order that C is prepared in. Eight waves share a chunk's operands.
 //
 // 4096 tokens of 128 heads x 64 x 128, 8 groups: 196 us (1.59 TB/s of what must be read and written, whose floor
-// is 61 us; 22 + 48 + 130 in a trace), 333 tokens of 24 heads 35. Before the halves' range was widened these were 180
+// is 61 us; 22 + 46 + 130 in a trace), 333 tokens of 24 heads 35. Before the halves' range was widened these were 180
 // and 32, and then nothing was saturated: the matrix cores were busy for a fifth of the time, the vector units for two
 // fifths and LDS for a quarter, and leaving any one part out (the loads of x or of the operands, the update of the
 // state, the stores) saved a tenth each, so a chunk's barriers and the latency between its parts were what was left.
