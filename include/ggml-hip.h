@@ -40,7 +40,8 @@ GGML_API ggml_backend_buffer_type_t ggml_backend_hip_buffer_type(int device);
 // recorded by a caller's HIP graph capture. A graph needing more scratch is rejected with
 // GGML_STATUS_ALLOC_FAILED and a message, but only at the node where the array ran out: the
 // kernels queued before that node have run, including any KV-cache append folded into an earlier
-// attention, so cache rows of the step may already be written; the outputs are undefined. Calls
+// attention and any copy into a mixer's states, so cache rows of the step and states may already be
+// written; the outputs are undefined. Calls
 // share their GPU's array and keep its last contents (no kernel relies on it starting at zero):
 // calls that overlap on one GPU (several threads or backends) race. Fails with profiling on (it
 // creates events).
