@@ -22,7 +22,9 @@ BIN_DIR = os.path.join(PKG_DIR, "bin")
 
 # ggml type ids (GGUF on-disk ids)
 F32, F16, Q4_0, Q8_0, Q4_K, Q5_K, Q6_K, Q8_K, I32, BF16 = 0, 1, 2, 8, 12, 13, 14, 15, 26, 30
+I64 = 27
 ROPE_NORMAL, ROPE_NEOX = 0, 2
+ROPE_MROPE, ROPE_VISION, ROPE_IMROPE = 8, 24, 40
 SORT_ASC, SORT_DESC = 0, 1
 UNARY_SILU = 1
 
@@ -154,6 +156,9 @@ def _declare(core, hip, loader):
     _sig(core, "ggml_ssm_conv", T, vp, T, T)
     _sig(core, "ggml_ssm_scan", T, vp, T, T, T, T, T, T, T, i32)
     _sig(core, "ggml_gated_delta_net", T, vp, T, T, T, T, T, T, i32)
+    _sig(core, "ggml_rope_multi", T, vp, T, T, T, i32, C.POINTER(i32), i32, i32, f32, f32, f32, f32, f32, f32)
+    _sig(core, "ggml_set_rows", T, vp, T, T, T)
+    _sig(core, "ggml_flash_attn_paged", T, vp, T, T, T, T, T, T, f32)
     _sig(core, "ggml_sum_rows", T, vp, T)
     _sig(core, "ggml_argsort", T, vp, T, i32)
     _sig(core, "ggml_top_k", T, vp, T, i32)
@@ -227,6 +232,7 @@ def _declare(core, hip, loader):
     _sig(hip, "ggml_backend_hip_sample", i32, vp, vp, i64, C.POINTER(ggml_hip_sampler_params), vp, sz,
          C.c_double, C.POINTER(C.c_int32), C.POINTER(C.c_bool))
     _sig(hip, "ggml_backend_hip_logprobs", i32, vp, vp, i64, i64, vp, C.c_int32, vp, vp, vp, vp)
+    _sig(hip, "ggml_backend_hip_verify", i32, vp, vp, vp, i64, vp, vp, vp, vp, vp)
     _sig(hip, "ggml_backend_hip_refusal", C.c_char_p, T)
     _sig(hip, "ggml_backend_hip_scan_scratch", sz, T)
     _sig(hip, "ggml_backend_hip_set_fusion", None, vp, C.c_bool)
@@ -318,6 +324,32 @@ def hip_logprobs(backend, logits_tensor, tokens, *, row: int = 0, n_rows: int | 
     if st != 0:
         raise RuntimeError(f"ggml_backend_hip_logprobs failed ({st})")
     return None if toks is None else logprob, entropy, ids, top
+
+
+def hip_verify(backend, probs, n_drafted, tokens, u, *, draft_probs=None):
+    """ggml_backend_hip_verify: (accepted tokens, the token behind them) of each sequence. n_drafted: drafted tokens of
+    each sequence; tokens: all of them; u: a number in [0, 1) for each, and one more a sequence behind its own."""
+    import numpy as np
+
+    def ints(a, name):
+        a = np.asarray(a)
+        if a.dtype != np.int32:
+            if a.size and (a.dtype.kind not in "iu" or a.min() < -2 ** 31 or a.max() >= 2 ** 31):
+                raise ValueError(f"hip_verify: {name} are 32-bit integers")   # not cut to such
+            a = a.astype(np.int32)
+        return np.ascontiguousarray(a)
+
+    n, toks = ints(n_drafted, "n_drafted"), ints(tokens, "tokens")
+    u = np.ascontiguousarray(u, dtype=np.float64)
+    total = int(n.sum(dtype=np.int64))
+    if n.ndim != 1 or (n < 0).any() or toks.shape != (total,) or u.shape != (total + len(n),):
+        raise ValueError("hip_verify: a token for each draft, a number for each and one more a sequence")
+    out = np.empty((2, len(n)), np.int32)
+    st = libs()["hip"].ggml_backend_hip_verify(backend, probs, draft_probs, len(n), n.ctypes.data, toks.ctypes.data, u.ctypes.data,
+                                               out[0].ctypes.data, out[1].ctypes.data)
+    if st != 0:
+        raise RuntimeError(f"ggml_backend_hip_verify failed ({st})")
+    return out[0], out[1]
 
 
 def hip_backend(device: int = 0):

@@ -87,7 +87,7 @@ const char * ggml_op_name(enum ggml_op op) {
         "NONE", "DUP", "ADD", "MUL", "SCALE", "SQR", "RMS_NORM", "MUL_MAT", "MUL_MAT_ID", "CPY", "CONT",
         "RESHAPE", "VIEW", "PERMUTE", "TRANSPOSE", "GET_ROWS", "SOFT_MAX", "ROPE", "FLASH_ATTN_EXT",
         "ARGMAX", "UNARY", "DIV", "SUM_ROWS", "ARGSORT", "SUB", "CONCAT", "L2_NORM", "GLU", "SSM_CONV",
-        "SSM_SCAN", "GATED_DELTA_NET",
+        "SSM_SCAN", "GATED_DELTA_NET", "ROPE_MULTI", "SET_ROWS", "FLASH_ATTN_PAGED",
     };
     return ((int) op >= 0 && op < GGML_OP_COUNT) ? names[op] : "?";
 }
@@ -755,6 +755,52 @@ struct ggml_tensor * ggml_flash_attn_ext(struct ggml_context * ctx, struct ggml_
     r->src[1] = k;
     r->src[2] = v;
     r->src[3] = mask;
+    return r;
+}
+
+// The operands of the three below are checked when a backend computes the node (ggml_backend_hip_refusal says
+// what it refuses); a result's extents are those of the operands that are there.
+struct ggml_tensor * ggml_rope_multi(struct ggml_context * ctx, struct ggml_tensor * a, struct ggml_tensor * b,
+        struct ggml_tensor * c, int n_dims, int sections[GGML_MROPE_SECTIONS], int mode, int n_ctx_orig, float freq_base,
+        float freq_scale, float ext_factor, float attn_factor, float beta_fast, float beta_slow) {
+    ggml_tensor * r = ggml_dup_tensor(ctx, a);
+    int32_t params[15] = { 0, n_dims, mode, 0, n_ctx_orig };
+    memcpy(params + 5,  &freq_base,   4);
+    memcpy(params + 6,  &freq_scale,  4);
+    memcpy(params + 7,  &ext_factor,  4);
+    memcpy(params + 8,  &attn_factor, 4);
+    memcpy(params + 9,  &beta_fast,   4);
+    memcpy(params + 10, &beta_slow,   4);
+    if (sections) memcpy(params + 11, sections, GGML_MROPE_SECTIONS * sizeof(int32_t));
+    set_op_params(r, params, sizeof(params));
+    r->op = GGML_OP_ROPE_MULTI;
+    r->src[0] = a;
+    r->src[1] = b;
+    r->src[2] = c;
+    return r;
+}
+
+struct ggml_tensor * ggml_set_rows(struct ggml_context * ctx, struct ggml_tensor * a, struct ggml_tensor * b, struct ggml_tensor * c) {
+    ggml_tensor * r = ggml_view_tensor(ctx, a);
+    format_name(r, "%s (rows set)", a->name);
+    r->op = GGML_OP_SET_ROWS;
+    r->src[0] = b;
+    r->src[1] = c;
+    r->src[2] = a;
+    return r;
+}
+
+struct ggml_tensor * ggml_flash_attn_paged(struct ggml_context * ctx, struct ggml_tensor * q, struct ggml_tensor * k,
+        struct ggml_tensor * v, struct ggml_tensor * pages, struct ggml_tensor * q_start, struct ggml_tensor * kv_len, float scale) {
+    ggml_tensor * r = ggml_new_tensor_4d(ctx, GGML_TYPE_F32, q->ne[0], q->ne[1], q->ne[2], q->ne[3]);
+    set_op_param_f32(r, 0, scale);
+    r->op = GGML_OP_FLASH_ATTN_PAGED;
+    r->src[0] = q;
+    r->src[1] = k;
+    r->src[2] = v;
+    r->src[3] = pages;
+    r->src[4] = q_start;
+    r->src[5] = kv_len;
     return r;
 }
 

@@ -517,11 +517,158 @@ ssm_scan_launch scan_launch_of(const ggml_tensor * n) {
     return L;
 }
 
+// ---- operands of the paged cache's ops ----
+
+// a tensor of whole blocks in rows without gaps, inside the memory it is a view of, at whole blocks of it
+bool block_rows(const ggml_tensor * t) {
+    const size_t bs = ggml_type_size(t->type);
+    const int64_t blck = ggml_blck_size(t->type);
+    if (blck < 1 || t->ne[0] % blck || t->nb[0] != bs || (t->view_src && (t->view_src->type != t->type || t->view_offs % bs))) return false;
+    unsigned __int128 end = (t->view_src ? t->view_offs : 0) + (unsigned __int128) (t->ne[0] / blck) * bs;
+    for (int i = 0; i < GGML_MAX_DIMS; i++) {
+        if (t->ne[i] <= 0) return true;
+        if (i > 0 && t->nb[i] % bs) return false;
+        if (i > 0) end += (unsigned __int128) (t->ne[i] - 1) * t->nb[i];
+    }
+    return end <= ggml_nbytes(t->view_src ? t->view_src : t);
+}
+
+// no two rows of t share memory (rows of contiguous blocks at strides of any order)
+bool rows_apart(const ggml_tensor * t) {
+    int order[3] = { 1, 2, 3 };
+    std::sort(order, order + 3, [&](int a, int b) { return t->nb[a] < t->nb[b]; });
+    unsigned __int128 size = (unsigned __int128) (t->ne[0] / ggml_blck_size(t->type)) * t->nb[0];
+    for (int d : order) {
+        if (t->ne[d] <= 1) continue;
+        if (t->nb[d] < size) return false;
+        size += (unsigned __int128) (t->ne[d] - 1) * t->nb[d];
+    }
+    return true;
+}
+
+bool i32_vector(const ggml_tensor * t, int64_t n) { return plain_rows(t, GGML_TYPE_I32) && has_shape(t, n, 1, 1, 1); }
+
+// pairs that a rope_multi node turns, and the distance between a pair's values
+int rope_multi_pairs(const ggml_tensor * n) { return n->op_params[2] == GGML_ROPE_TYPE_VISION ? n->op_params[1] : n->op_params[1] / 2; }
+
+const char * rope_multi_refusal(const ggml_tensor * n) {
+    const ggml_tensor * a = n->src[0], * b = n->src[1], * c = n->src[2];
+    if (!a || !b) return "rope_multi: an operand is missing";
+    if (!plain_rows(a, GGML_TYPE_F32) || n->type != GGML_TYPE_F32 || !ggml_is_contiguous(n) || !ggml_are_same_shape(n, a)) {
+        return "rope_multi: F32 rows of contiguous values, inside their tensor";
+    }
+    if (!i32_vector(b, 4 * a->ne[2])) return "rope_multi: four I32 positions a token, one axis after another";
+    const int n_dims = n->op_params[1], mode = n->op_params[2];
+    if (mode != GGML_ROPE_TYPE_MROPE && mode != GGML_ROPE_TYPE_IMROPE && mode != GGML_ROPE_TYPE_VISION) return "rope_multi: unknown mode";
+    if (n_dims < 2 || n_dims % 2 || (mode == GGML_ROPE_TYPE_VISION ? (int64_t) n_dims * 2 != a->ne[0] : n_dims > a->ne[0]) ||
+        rope_multi_pairs(n) > ROWS_MAX_PAIRS) return "rope_multi: n_dims does not fit";
+    int64_t sum = 0;
+    for (int i = 0; i < GGML_MROPE_SECTIONS; i++) {
+        if (n->op_params[11 + i] < 0) return "rope_multi: a negative section";
+        sum += n->op_params[11 + i];
+    }
+    if (sum == 0) return "rope_multi: no sections";
+    float base;
+    memcpy(&base, n->op_params + 5, 4);
+    if (!(base > 0.0f) || std::isinf(base)) return "rope_multi: freq_base must be positive";
+    if (c && (!plain_rows(c, GGML_TYPE_F32) || !has_shape(c, c->ne[0], 1, 1, 1) || c->ne[0] < rope_multi_pairs(n))) return "rope_multi: a frequency factor for each pair, F32";
+    if (a->ne[0] > INT_MAX / 4 || a->ne[1] > INT_MAX / 4 / std::max<int64_t>(a->ne[0], 1) || a->ne[3] > 65535) return "rope_multi: rows are too wide or too many";
+    return nullptr;
+}
+
+const char * set_rows_refusal(const ggml_tensor * n) {
+    const ggml_tensor * b = n->src[0], * c = n->src[1], * a = n->src[2];
+    if (!a || !b || !c) return "set_rows: an operand is missing";
+    if (a->type != GGML_TYPE_F32 && a->type != GGML_TYPE_F16 && a->type != GGML_TYPE_BF16 && a->type != GGML_TYPE_Q8_0 &&
+        a->type != GGML_TYPE_Q4_0) return "set_rows: rows of F32, F16, BF16, Q8_0 or Q4_0";
+    if (!block_rows(a) || !rows_apart(a)) return "set_rows: the rows must be contiguous, apart, inside their tensor";
+    if (!plain_rows(b, GGML_TYPE_F32)) return "set_rows: F32 rows of contiguous values, inside their tensor";
+    const size_t is = c->type == GGML_TYPE_I64 ? 8 : 4;
+    if ((c->type != GGML_TYPE_I32 && c->type != GGML_TYPE_I64) || c->nb[0] != is || c->nb[1] % is || c->nb[2] % is || !inside_base(c)) {
+        return "set_rows: I32 or I64 indices in contiguous rows, inside their tensor";
+    }
+    if (!has_shape(b, a->ne[0], c->ne[0], a->ne[2], a->ne[3]) || c->ne[3] != 1 || c->ne[1] < 1 || c->ne[2] < 1 ||
+        a->ne[2] % c->ne[1] || a->ne[3] % c->ne[2]) return "set_rows: the operands' extents do not fit";
+    if (a->ne[0] > INT_MAX / 4 || a->ne[2] > 65535 || a->ne[3] > 65535) return "set_rows: rows are too wide or too many";
+    return nullptr;
+}
+
+const char * flash_attn_paged_refusal(const ggml_tensor * n) {
+    const ggml_tensor * q = n->src[0], * k = n->src[1], * v = n->src[2], * pages = n->src[3], * start = n->src[4], * len = n->src[5];
+    for (int i = 0; i < 6; i++) if (!n->src[i]) return "flash_attn_paged: an operand is missing";
+    if (!plain_rows(q, GGML_TYPE_F32) || q->ne[3] != 1) return "flash_attn_paged: F32 queries of contiguous values, inside their tensor";
+    if (k->type != GGML_TYPE_Q4_0 || v->type != GGML_TYPE_Q4_0 || !block_rows(k) || !block_rows(v)) {
+        return "flash_attn_paged: a Q4_0 cache of contiguous heads, inside its tensor";
+    }
+    const int64_t D = q->ne[0], H = q->ne[1], T = q->ne[2], KV = k->ne[1], P = k->ne[2], S = pages->ne[1];
+    if (D != 64 && D != 96 && D != 128) return "flash_attn_paged: heads of 64, 96 or 128 values";
+    if (k->ne[0] != D || !ggml_are_same_shape(k, v) || KV < 1 || H % KV || P < 1) return "flash_attn_paged: the cache's extents do not fit";
+    if (!plain_rows(pages, GGML_TYPE_I32) || pages->ne[2] != 1 || pages->ne[3] != 1 || !i32_vector(start, S + 1) || !i32_vector(len, S)) {
+        return "flash_attn_paged: I32 pages of each sequence, starts (one more than sequences) and lengths";
+    }
+    if (n->type != GGML_TYPE_F32 || !ggml_is_contiguous(n) || !has_shape(n, D, H, T, 1)) return "flash_attn_paged: the result's extent does not fit";
+    if (S > PAGED_MAX_SEQS || T > PAGED_MAX_TOKENS || H > PAGED_MAX_HEADS || P > INT_MAX / 2 || pages->ne[0] > INT_MAX / 2 / P) {
+        return "flash_attn_paged: too many sequences, tokens, heads or positions";
+    }
+    return nullptr;
+}
+
+paged_attn paged_attn_of(const ggml_tensor * n) {
+    const ggml_tensor * q = n->src[0], * k = n->src[1], * v = n->src[2], * pages = n->src[3];
+    paged_attn A{};
+    A.q = (const float *) q->data;
+    A.q_h = (int64_t) q->nb[1] / 4; A.q_t = (int64_t) q->nb[2] / 4;
+    A.out = (float *) n->data;
+    auto cache = [](const ggml_tensor * t, const uint8_t *& qs, const __half *& d, int64_t & head, int64_t & pos, int64_t & page) {
+        const planes p = planes_of(t);
+        const int64_t bs = (int64_t) ggml_type_size(t->type);
+        qs = p.qs + p.first_block * Q4_0_QS;
+        d = p.d + p.first_block;
+        head = (int64_t) t->nb[1] / bs; pos = (int64_t) t->nb[2] / bs; page = (int64_t) t->nb[3] / bs;
+    };
+    cache(k, A.kq, A.kd, A.k_head, A.k_pos, A.k_page);
+    cache(v, A.vq, A.vd, A.v_head, A.v_pos, A.v_page);
+    A.pages = (const int32_t *) pages->data;
+    A.pages_s = (int64_t) pages->nb[1] / 4;
+    A.q_start = (const int32_t *) n->src[4]->data;
+    A.kv_len = (const int32_t *) n->src[5]->data;
+    A.n_pages = k->ne[3];
+    A.D = (int) q->ne[0]; A.n_head = (int) q->ne[1]; A.n_head_kv = (int) k->ne[1];
+    A.n_tokens = (int) q->ne[2]; A.n_seqs = (int) pages->ne[1];
+    A.page = (int) k->ne[2]; A.max_pages = (int) pages->ne[0];
+    memcpy(&A.scale, n->op_params, 4);
+    return A;
+}
+
 // why graph_compute refuses a graph with this node before it queues anything (nullptr: it does not)
 const char * node_refusal(const ggml_tensor * n) {
     if (n->op == GGML_OP_SSM_CONV) return ssm_conv_refusal(n);
     if (n->op == GGML_OP_SSM_SCAN) return ssm_scan_refusal(n);
+    if (n->op == GGML_OP_ROPE_MULTI) return rope_multi_refusal(n);
+    if (n->op == GGML_OP_SET_ROWS) return set_rows_refusal(n);
+    if (n->op == GGML_OP_FLASH_ATTN_PAGED) return flash_attn_paged_refusal(n);
     return nullptr;
+}
+
+// ops whose operands graph_refused looks for in the device's memory
+bool checked_op(int op) {
+    return op == GGML_OP_SSM_CONV || op == GGML_OP_SSM_SCAN || op == GGML_OP_ROPE_MULTI || op == GGML_OP_SET_ROWS ||
+           op == GGML_OP_FLASH_ATTN_PAGED;
+}
+
+// the bytes a tensor's elements span
+struct span { const char * b, * e; };
+span span_of(const ggml_tensor * t) {
+    const char * p = (const char *) t->data;
+    if (ggml_nelements(t) == 0) return { p, p };
+    size_t n = ggml_type_size(t->type) * (size_t) (t->ne[0] / ggml_blck_size(t->type) - 1) + ggml_type_size(t->type);
+    if (!ggml_is_quantized(t->type)) n = (size_t) (t->ne[0] - 1) * t->nb[0] + ggml_type_size(t->type);
+    for (int i = 1; i < GGML_MAX_DIMS; i++) n += (size_t) (t->ne[i] - 1) * t->nb[i];
+    return { p, p + n };
+}
+bool overlap(const ggml_tensor * a, const ggml_tensor * b) {
+    const span x = span_of(a), y = span_of(b);
+    return x.b < y.e && y.b < x.e;
 }
 
 // memory that the device's kernels can read and write: for tensors that a caller placed without a buffer
@@ -538,7 +685,7 @@ bool graph_refused(const ggml_cgraph * g, int device) {
     for (int i = 0; i < g->n_nodes; i++) {
         const ggml_tensor * n = g->nodes[i];
         const char * why = node_refusal(n);
-        if (!why && (n->op == GGML_OP_SSM_CONV || n->op == GGML_OP_SSM_SCAN)) {
+        if (!why && checked_op(n->op)) {
             for (int s = -1; s < GGML_MAX_SRC; s++) {
                 const ggml_tensor * t = s < 0 ? n : n->src[s];
                 if (!t || ggml_nelements(t) == 0) continue;
@@ -547,6 +694,10 @@ bool graph_refused(const ggml_cgraph * g, int device) {
                 else if (buf ? ggml_backend_buffer_get_type(buf) != ggml_backend_hip_buffer_type(device) : !on_device(t->data, device)) {
                     why = "an operand is not in this device's memory";
                 }
+            }
+            // stored while others are still read
+            if (!why && n->op == GGML_OP_SET_ROWS && (overlap(n->src[2], n->src[0]) || overlap(n->src[2], n->src[1]))) {
+                why = "set_rows: the rows share memory with what is stored into them";
             }
         }
         if (!why) continue;
@@ -825,7 +976,8 @@ private:
             case GGML_OP_NONE: case GGML_OP_RESHAPE: case GGML_OP_VIEW: case GGML_OP_PERMUTE: case GGML_OP_TRANSPOSE:
                 return;
             case GGML_OP_RMS_NORM: op_rms_norm(i); return;
-            case GGML_OP_ROPE: op_rope(i); return;
+            case GGML_OP_ROPE: if (!op_rows(i)) op_rope(i); return;
+            case GGML_OP_ROPE_MULTI: case GGML_OP_SET_ROWS: op_rows(i); return;
             case GGML_OP_MUL_MAT: op_mul_mat(i); return;
             case GGML_OP_MUL_MAT_ID:
                 if (!gemv_capable(n)) HIP_ABORT("mul_mat_id '%s': unsupported operands", n->name);
@@ -916,6 +1068,7 @@ private:
                 return;
             }
             case GGML_OP_FLASH_ATTN_EXT: op_flash_attn(n); return;
+            case GGML_OP_FLASH_ATTN_PAGED: op_flash_attn_paged(n); return;
             case GGML_OP_ARGMAX: {
                 prof_scope ps(this, "argmax", 0);
                 const tview a = tv(n->src[0]);
@@ -955,20 +1108,6 @@ private:
     }
 
     // ---- state space mixers (operands checked by node_refusal before the graph ran) ----
-    // the bytes a tensor's elements span
-    struct span { const char * b, * e; };
-    static span span_of(const ggml_tensor * t) {
-        const char * p = (const char *) t->data;
-        if (ggml_nelements(t) == 0) return { p, p };
-        size_t n = ggml_type_size(t->type) * (size_t) (t->ne[0] / ggml_blck_size(t->type) - 1) + ggml_type_size(t->type);
-        if (!ggml_is_quantized(t->type)) n = (size_t) (t->ne[0] - 1) * t->nb[0] + ggml_type_size(t->type);
-        for (int i = 1; i < GGML_MAX_DIMS; i++) n += (size_t) (t->ne[i] - 1) * t->nb[i];
-        return { p, p + n };
-    }
-    static bool overlap(const ggml_tensor * a, const ggml_tensor * b) {
-        const span x = span_of(a), y = span_of(b);
-        return x.b < y.e && y.b < x.e;
-    }
     // writing `to` at node `from` instead of at node `at`: no node between the two (fused ones aside)
     // reads or writes that memory
     bool may_write_early(int from, int at, const ggml_tensor * to, const std::vector<int> & fused) const {
@@ -1366,6 +1505,217 @@ private:
             launch_rope_batch(B, st_);
         }
         for (int j : members) done_[j] = true;
+    }
+
+    // ---- rows stored by index, rotations of several axes (operands checked by node_refusal) ----
+    // the stored rows as a job's destination
+    static void rows_into(rows_job & J, const ggml_tensor * n) {
+        const ggml_tensor * c = n->src[1], * a = n->src[2];
+        const size_t bs = ggml_type_size(a->type);
+        J.type = a->type;
+        J.to_rows = a->ne[1];
+        J.idx = c->data;
+        J.idx64 = c->type == GGML_TYPE_I64;
+        J.c_n2 = c->ne[1]; J.c_n3 = c->ne[2];
+        J.c2 = (int64_t) (c->nb[1] / c->nb[0]); J.c3 = (int64_t) (c->nb[2] / c->nb[0]);
+        J.d1 = (int64_t) a->nb[1]; J.d2 = (int64_t) a->nb[2]; J.d3 = (int64_t) a->nb[3];
+        if (!is_repacked(a->type)) {
+            J.dst = (char *) a->data;
+            return;
+        }
+        const planes p = planes_of(a);
+        J.qs = p.qs;
+        J.d = p.d;
+        J.first_block = p.first_block;
+        J.d1 /= bs; J.d2 /= bs; J.d3 /= bs;
+    }
+    static rows_job rows_of(const ggml_tensor * b) {
+        rows_job J{};
+        J.src = (const char *) b->data;
+        J.s1 = (int64_t) b->nb[1]; J.s2 = (int64_t) b->nb[2]; J.s3 = (int64_t) b->nb[3];
+        J.rows = b->ne[1]; J.n2 = b->ne[2]; J.n3 = b->ne[3];
+        J.width = J.head = (int) b->ne[0];
+        return J;
+    }
+    // a rotation's tokens as rows of all their heads; false where the batch's other rotations have other parameters
+    bool rows_rotated(rows_batch & B, rows_job & J, const ggml_tensor * r, bool & multi, bool & ext) {
+        const ggml_tensor * a = r->src[0];
+        J = rows_job{};
+        J.src = (const char *) a->data;
+        J.s_head = (int64_t) a->nb[1]; J.s1 = (int64_t) a->nb[2]; J.s3 = (int64_t) a->nb[3];
+        J.rows = a->ne[2]; J.n2 = 1; J.n3 = a->ne[3];
+        J.head = (int) a->ne[0];
+        J.width = (int) (a->ne[0] * a->ne[1]);
+        J.pos = (const int32_t *) r->src[1]->data;
+        J.n_pos = a->ne[2];
+        J.ff = r->src[2] ? (const float *) r->src[2]->data : nullptr;
+        J.type = GGML_TYPE_F32;
+        J.dst = (char *) r->data;
+        J.d1 = (int64_t) r->nb[2]; J.d3 = (int64_t) r->nb[3];
+        if (r->op == GGML_OP_ROPE) {
+            rows_batch X{};
+            X.p = rope_params_of(r);
+            if (ext && memcmp(&X.p, &B.p, sizeof(rope_params)) != 0) return false;
+            B.p = X.p;
+            ext = true;
+            J.rope = ROWS_ROPE_EXT;
+            J.pairs = B.p.n_dims / 2;
+            J.dist = B.p.mode & GGML_ROPE_TYPE_NEOX ? J.pairs : 1;
+            return true;
+        }
+        double scale, turns[ROWS_MAX_PAIRS];
+        uint8_t axis[ROWS_MAX_PAIRS];
+        J.rope = ROWS_ROPE_MULTI;
+        J.pairs = J.dist = rope_multi_table(r, scale, turns, axis);
+        if (multi && (scale != B.scale || memcmp(turns, B.turns, J.pairs * sizeof(double)) != 0 || memcmp(axis, B.axis, J.pairs) != 0)) return false;
+        multi = true;
+        B.scale = scale;
+        memcpy(B.turns, turns, J.pairs * sizeof(double));
+        memcpy(B.axis, axis, J.pairs);
+        return true;
+    }
+
+    // each pair's turns per position (in 64 bits, frequency factors aside) and the axis it takes positions of
+    static int rope_multi_table(const ggml_tensor * n, double & mscale, double * turns, uint8_t * axis) {
+        const rope_params p = rope_params_of(n);
+        const int32_t * sec = n->op_params + 11;
+        float base;
+        memcpy(&base, n->op_params + 5, 4);
+        const int pairs = rope_multi_pairs(n);
+        const int64_t sum = (int64_t) sec[0] + sec[1] + sec[2] + sec[3];
+        mscale = p.attn_factor;
+        if (p.ext_factor != 0.0f) mscale *= 1.0 + 0.1 * std::log(1.0 / (double) p.freq_scale);
+        for (int i = 0; i < pairs; i++) {
+            const int64_t sector = i % sum;
+            int k = 0;
+            int64_t start = 0;
+            if (p.mode == GGML_ROPE_TYPE_IMROPE) {
+                k = (int) (sector % 3);
+                if (sector >= 3 * (int64_t) sec[k]) k = 3;
+            } else {
+                while (k < 3 && sector >= start + sec[k]) start += sec[k++];
+            }
+            const double e = p.mode == GGML_ROPE_TYPE_VISION ? (double) (sector - start) : (double) i;
+            double m = p.freq_scale;
+            if (p.ext_factor != 0.0f) {
+                const double y = (i - p.corr_dims[0]) / std::max(0.001, (double) p.corr_dims[1] - p.corr_dims[0]);
+                const double mix = (1.0 - std::min(1.0, std::max(0.0, y))) * p.ext_factor;
+                m = m * (1.0 - mix) + mix;
+            }
+            turns[i] = std::pow((double) base, -2.0 * e / p.n_dims) * m / 6.283185307179586476925;
+            axis[i] = (uint8_t) k;
+        }
+        return pairs;
+    }
+
+    // the set_rows node that alone reads rotation i, whole tokens as rows, or -1
+    int rows_stored(int i) const {
+        if (!fuse(FUSE_ROPE) || c_.cb) return -1;
+        const ggml_tensor * r = g_->nodes[i];
+        if (r->ne[3] != 1) return -1;
+        int u = sole_user(i);
+        while (u >= 0 && (g_->nodes[u]->op == GGML_OP_RESHAPE || g_->nodes[u]->op == GGML_OP_VIEW) && g_->nodes[u]->data == r->data) u = sole_user(u);
+        if (u < 0 || g_->nodes[u]->op != GGML_OP_SET_ROWS) return -1;
+        const ggml_tensor * n = g_->nodes[u], * b = n->src[0];
+        if (b->data != r->data || !ggml_is_contiguous(b) || !has_shape(b, r->ne[0] * r->ne[1], r->ne[2], 1, 1)) return -1;
+        return u;
+    }
+
+    // Rotations of several axes and rows stored by index from node i on, with the rotations between them, as one
+    // launch: nodes whose inputs are final and none of which touches another's memory; a rotation that only a set_rows
+    // reads is stored by it. False where node i is a rope_ext that no such node goes with.
+    bool op_rows(int i) {
+        rows_batch B{};
+        std::vector<int> members;
+        std::vector<const ggml_tensor *> in, out;
+        bool multi = false, ext = false, ours = false;
+        auto clear_of = [&](const std::vector<const ggml_tensor *> & reads, const ggml_tensor * writes) {
+            for (const ggml_tensor * t : reads) for (const ggml_tensor * o : out) if (overlap(t, o)) return false;
+            for (const ggml_tensor * t : in) if (overlap(t, writes)) return false;
+            for (const ggml_tensor * t : out) if (overlap(t, writes)) return false;
+            return true;
+        };
+        auto add = [&](int j) {
+            const ggml_tensor * n = g_->nodes[j];
+            rows_job J;
+            std::vector<const ggml_tensor *> reads;
+            const ggml_tensor * writes = n;
+            int stored = -1;
+            if (n->op == GGML_OP_SET_ROWS) {
+                if (!ready(n->src[0]) || !ready(n->src[1]) || !ready(n->src[2])) return false;
+                J = rows_of(n->src[0]);
+                rows_into(J, n);
+                reads = { n->src[0], n->src[1] };
+            } else {
+                if (n->src[0]->type != GGML_TYPE_F32 || n->type != GGML_TYPE_F32 || n->src[0]->nb[0] != 4) return false;
+                for (int k = 0; k < 3; k++) {
+                    if (!n->src[k]) continue;
+                    if (!ready(n->src[k])) return false;
+                    reads.push_back(n->src[k]);
+                }
+                rows_batch was = B;
+                const bool wm = multi, we = ext;
+                if (!rows_rotated(B, J, n, multi, ext)) return false;
+                stored = rows_stored(j);
+                if (stored >= 0) {
+                    const ggml_tensor * r = g_->nodes[stored];
+                    std::vector<int> inside = members;
+                    inside.push_back(j);
+                    inside.push_back(stored);
+                    if (!ready(r->src[1]) || !ready(r->src[2]) || !may_write_early(i, stored, r, inside) || !may_read_early(i, stored, r->src[1], inside)) {
+                        stored = -1;
+                    } else {
+                        J.dst = nullptr;
+                        J.d2 = J.d3 = 0;
+                        rows_into(J, r);
+                        reads.push_back(r->src[1]);
+                        writes = r;
+                    }
+                }
+                if (!members.empty() && !clear_of(reads, writes)) { B = was; multi = wm; ext = we; return false; }
+            }
+            if (!members.empty() && !clear_of(reads, writes)) return false;
+            if (stored >= 0) members.push_back(stored);
+            if (stored >= 0 || n->op != GGML_OP_ROPE) ours = true;
+            members.push_back(j);
+            in.insert(in.end(), reads.begin(), reads.end());
+            out.push_back(writes);
+            B.job[B.n_jobs++] = J;
+            return true;
+        };
+        const bool start = g_->nodes[i]->op == GGML_OP_ROPE;
+        if (!add(i)) {
+            if (start) return false;
+            HIP_ABORT("rows '%s': operands that are not final", g_->nodes[i]->name);
+        }
+        if (fuse(FUSE_ROPE) && !c_.cb) {
+            for (int j = i + 1; j < g_->n_nodes && B.n_jobs < ROWS_MAX_JOBS; j++) {
+                const ggml_tensor * m = g_->nodes[j];
+                if (done_[j] || std::find(members.begin(), members.end(), j) != members.end() || is_view_op(m->op)) continue;
+                if (m->op != GGML_OP_ROPE && m->op != GGML_OP_ROPE_MULTI && m->op != GGML_OP_SET_ROWS) break;
+                if (!add(j)) break;
+            }
+        }
+        if (!ours) return false;
+        for (int j : members) {
+            if (g_->nodes[j]->op == GGML_OP_ROPE) materialize_norm(g_->nodes[j]->src[0]);
+        }
+        for (int k = 0; k < B.n_jobs; k++) {
+            rows_job & J = B.job[k];
+            if (J.rope != ROWS_ROPE_EXT || J.rows < ROPE_TABLE_MIN_TOKENS) continue;
+            rope_job R{};
+            R.pos = J.pos;
+            R.ff = J.ff;
+            R.p = B.p;
+            J.cs = rope_table_of(R, J.rows);
+        }
+        double bytes = 0;
+        for (const ggml_tensor * t : in) bytes += (double) ggml_nbytes(t);
+        for (const ggml_tensor * t : out) wrote_.push_back(t);
+        for (int j : members) done_[j] = true;
+        prof_scope ps(this, "rows", bytes);
+        launch_rows(B, st_);
+        return true;
     }
 
     // A RoPE batch of exactly {Q rotation, K rotation copied into the K cache, V copy into the V
@@ -2541,6 +2891,24 @@ private:
         wrote_.push_back(ctn);
     }
 
+    void op_flash_attn_paged(ggml_tensor * n) {
+        paged_attn A = paged_attn_of(n);
+        if (const int64_t bytes = paged_attn_scratch_bytes(A)) {
+            // one buffer for the graph's layers, which the stream runs one after another
+            if (bytes > paged_size_) {
+                paged_buf_ = c_.scratch.alloc((size_t) bytes);
+                paged_size_ = bytes;
+            }
+            A.scratch = paged_buf_;
+        }
+        // the lengths are the device's: the bytes of full tables, at most the whole cache
+        const double rows = std::min((double) A.n_pages, (double) A.max_pages * A.n_seqs) * A.page;
+        prof_scope ps(this, "attn_paged", rows * A.n_head_kv * (A.D / 32) * 36 + 8.0 * A.n_tokens * A.n_head * A.D);
+        launch_paged_attn(A, st_);
+    }
+    void * paged_buf_ = nullptr;
+    int64_t paged_size_ = 0;
+
     void op_flash_attn(ggml_tensor * n) {
         const ggml_tensor * q = n->src[0], * k = n->src[1], * v = n->src[2], * mask = n->src[3];
         float scale, max_bias, softcap;
@@ -2968,6 +3336,104 @@ enum ggml_status ggml_backend_hip_logprobs(ggml_backend_t backend, const struct 
             if (top_ids && n_top) memcpy(top_ids + (r0 + i) * n_top, o + 2, n_top * 4);
             if (top_logprobs && n_top) memcpy(top_logprobs + (r0 + i) * n_top, o + 2 + n_top, n_top * 4);
         }
+    }
+    return GGML_STATUS_SUCCESS;
+}
+
+// (see the declaration for the contract)
+enum ggml_status ggml_backend_hip_verify(ggml_backend_t backend, const struct ggml_tensor * probs, const struct ggml_tensor * draft_probs,
+                                         int64_t n_seqs, const int32_t * n_drafted, const int32_t * tokens, const double * u,
+                                         int32_t * n_accepted, int32_t * token) {
+    auto fail = [](const char * why) {
+        fprintf(stderr, "ggml_backend_hip_verify: %s\n", why);
+        return GGML_STATUS_FAILED;
+    };
+    if (!probs || n_seqs < 0 || (n_seqs > 0 && (!n_drafted || !u || !n_accepted || !token))) return fail("null argument");
+    for (const ggml_tensor * t : { probs, draft_probs }) {
+        if (!t) continue;
+        if (t->type != GGML_TYPE_F32 || t->nb[0] != sizeof(float) || t->nb[1] % 4 || t->nb[2] % 4 || t->nb[3] % 4 || !inside_base(t)) {
+            return fail("probabilities must be F32 with contiguous rows");
+        }
+    }
+    const int64_t n = probs->ne[0];
+    if (n < 1 || n > INT_MAX / 4) return fail("row length out of range");
+    if (draft_probs && draft_probs->ne[0] != n) return fail("rows of different lengths");
+    int64_t drafts = 0;
+    for (int64_t s = 0; s < n_seqs; s++) {
+        if (n_drafted[s] < 0 || n_drafted[s] > GGML_HIP_VERIFY_MAX_DRAFT) return fail("number of drafted tokens out of range");
+        drafts += n_drafted[s];
+    }
+    if (drafts > 0 && !tokens) return fail("null argument");
+    if (ggml_nrows(probs) < drafts + n_seqs || (draft_probs && ggml_nrows(draft_probs) < drafts)) return fail("too few rows");
+    for (int64_t i = 0; i < drafts; i++) {
+        if (tokens[i] < 0 || tokens[i] >= n) return fail("token out of range");
+    }
+    for (int64_t i = 0; i < drafts + n_seqs; i++) {
+        if (!(u[i] >= 0.0 && u[i] < 1.0)) return fail("random number out of range");
+    }
+    if (!ggml_backend_is_hip(backend)) return fail("not a HIP backend");
+    hip_backend_ctx * c = (hip_backend_ctx *) backend->context;
+    for (const ggml_tensor * t : { probs, draft_probs }) {
+        if (!t || ggml_nelements(t) == 0) continue;
+        const ggml_backend_buffer_t buf = t->view_src ? t->view_src->buffer : t->buffer;
+        if (!t->data || !buf || ggml_backend_buffer_get_type(buf) != ggml_backend_hip_buffer_type(c->device)) {
+            return fail("probabilities are not in this backend's device buffer");
+        }
+    }
+    hip_device & d = dev(c->device);
+    auto rows = [](const ggml_tensor * t) {
+        return verify_rows{ (const char *) t->data, t->ne[1], t->ne[2], (int64_t) t->nb[1], (int64_t) t->nb[2], (int64_t) t->nb[3] };
+    };
+    // so many sequences at a time: their numbers fit an upload slot, their parts 32 MiB
+    const int64_t segments = (n + VERIFY_SEGMENT - 1) / VERIFY_SEGMENT;
+    const int64_t most = std::min<int64_t>(4096, std::max<int64_t>(1, ((int64_t) 32 << 20) / (segments * (int64_t) sizeof(double2))));
+    static_assert((2 * GGML_HIP_VERIFY_MAX_DRAFT + 2) * 8 + 64 <= UP_SMALL, "a sequence fits a slot");
+    static_assert(4096 * 2 * sizeof(int32_t) <= DOWN_MAX, "results fit the area");
+    int64_t at = 0;                                        // drafted tokens before sequence s0
+    for (int64_t s0 = 0; s0 < n_seqs;) {
+        int64_t ns = 0, nd = 0;
+        auto bytes = [](int64_t ns, int64_t nd) { return (size_t) ((nd + ns) * 8 + (ns + 1 + nd) * 4); };
+        while (s0 + ns < n_seqs && ns < most && bytes(ns + 1, nd + n_drafted[s0 + ns]) <= UP_SMALL) nd += n_drafted[s0 + ns++];
+        const size_t parts = (size_t) (ns * segments) * sizeof(double2);
+        if (parts > d.lp_size) {
+            HIP_CHECK(hipStreamSynchronize(d.stream));
+            drained(d);
+            if (d.lp) HIP_CHECK(hipFree(d.lp));
+            d.lp_size = std::max(parts, (size_t) 1 << 20);
+            HIP_CHECK(hipMalloc(&d.lp, d.lp_size));
+        }
+        uint8_t * slot = upload_slot(d, bytes(ns, nd));
+        if (!slot) {
+            HIP_CHECK(hipStreamSynchronize(d.stream));
+            drained(d);
+            slot = upload_slot(d, bytes(ns, nd));
+        }
+        int32_t * area = (int32_t *) download_area(d, (size_t) ns * 8);
+        if (!slot || !area) return fail("no room for a launch's numbers and results");
+        double * su = (double *) slot;
+        int32_t * first = (int32_t *) (su + nd + ns), * st = first + ns + 1;
+        memcpy(su, u + at + s0, (size_t) (nd + ns) * 8);
+        first[0] = 0;
+        for (int64_t s = 0; s < ns; s++) first[s + 1] = first[s] + n_drafted[s0 + s];
+        if (nd) memcpy(st, tokens + at, (size_t) nd * 4);
+        verify_launch L{};
+        L.p = rows(probs);
+        if (draft_probs) L.q = rows(draft_probs);
+        L.row0 = at;
+        L.seq0 = s0;
+        L.n = (int) n; L.n_seqs = (int) ns; L.segments = (int) segments;
+        L.first = first; L.tokens = st; L.u = su;
+        L.parts = (double2 *) d.lp;
+        L.out = area;
+        launch_verify(L, d.stream);
+        HIP_CHECK(hipStreamSynchronize(d.stream));
+        drained(d);
+        for (int64_t s = 0; s < ns; s++) {
+            n_accepted[s0 + s] = area[2 * s];
+            token[s0 + s] = area[2 * s + 1];
+        }
+        at += nd;
+        s0 += ns;
     }
     return GGML_STATUS_SUCCESS;
 }

@@ -374,6 +374,80 @@ constexpr int64_t ROPE_TABLE_MIN_TOKENS = 16;   // RoPE jobs over at least this 
 // layer), formed once
 void launch_rope_table(const int32_t * pos, int64_t n_pos, const rope_params & p, const float * ff, float2 * out, hipStream_t st);
 
+// Rows of F32 values, rotated or not, into rows of dst (F32, F16, BF16, or the planes of Q8_0 / Q4_0): row r into row
+// idx[r], where that lies in [0, to_rows), or into row r without idx. A row is `width` values, heads of `head` at s_head.
+constexpr int ROWS_MAX_JOBS = 4;
+constexpr int ROWS_MAX_PAIRS = 128;
+constexpr int64_t ROWS_PASS = 8192;
+enum { ROWS_ROPE_NONE = 0, ROWS_ROPE_MULTI = 1, ROWS_ROPE_EXT = 2 };
+struct rows_job {
+    const char * src;
+    int64_t s_head, s1, s2, s3;      // bytes
+    int64_t row0, rows, n2, n3;
+    int width, head;
+    // rotation of the row's heads: pairs (i, i + dist), or of neighbours with dist 1; token = row
+    int rope, pairs, dist;
+    const int32_t * pos;             // axis by axis, n_pos each
+    int64_t n_pos;
+    const float * ff;
+    const float2 * cs;               // ROWS_ROPE_EXT: an optional table (launch_rope_table)
+    const void * idx;                // I32, or I64 with idx64; strides in elements over c_n2 x c_n3 sets of indices
+    int idx64;
+    int64_t c2, c3, c_n2, c_n3, to_rows;
+    int type;                        // ggml_type of dst
+    char * dst;                      // with strides d1, d2, d3 in bytes, or
+    uint8_t * qs;                    // planes, strides in blocks
+    __half * d;
+    int64_t first_block, d1, d2, d3;
+    // set by launch_rows
+    int chunks, threads, per_wg, quads, wide;
+    int64_t first_wg;
+};
+struct rows_batch {
+    rows_job job[ROWS_MAX_JOBS];
+    int n_jobs;
+    rope_params p;                   // ROWS_ROPE_EXT
+    // ROWS_ROPE_MULTI: each pair's turns per position and axis; what cosines and sines are multiplied by
+    double scale;
+    double turns[ROWS_MAX_PAIRS];
+    uint8_t axis[ROWS_MAX_PAIRS];
+};
+void launch_rows(rows_batch & B, hipStream_t st);
+
+// Attention of several sequences' tokens over a 4-bit cache on pages (ggml_flash_attn_paged)
+constexpr int64_t PAGED_MAX_SEQS = 4096, PAGED_MAX_TOKENS = 1 << 20, PAGED_MAX_HEADS = 1024;
+struct paged_attn {
+    const float * q;                 // strides in floats
+    int64_t q_t, q_h;
+    float * out;                     // [token][head][D]
+    const uint8_t * kq, * vq;        // planes from the cache's first block on, strides in blocks
+    const __half * kd, * vd;
+    int64_t k_head, k_pos, k_page, v_head, v_pos, v_page;
+    const int32_t * pages, * q_start, * kv_len;
+    int64_t pages_s;                 // I32s between sequences
+    int64_t n_pages;
+    int D, n_head, n_head_kv, n_tokens, n_seqs, page, max_pages;
+    float scale;
+    void * scratch;
+};
+// Drafted tokens against probabilities (ggml_backend_hip_verify): rows as ggml row indices over ne[1..3]
+constexpr int VERIFY_SEGMENT = 2048;
+struct verify_rows { const char * base; int64_t ne1, ne2, nb1, nb2, nb3; };
+struct verify_launch {
+    verify_rows p, q;                // q.base: nullptr for drafts that are certain
+    int64_t row0, seq0;              // drafted tokens and sequences before the launch's: q's row of token i is row0 + i
+    int n, n_seqs, segments;
+    const int32_t * first;           // [n_seqs + 1] the launch's drafted tokens before each sequence's
+    const int32_t * tokens;
+    const double * u;
+    double2 * parts;                 // [n_seqs][segments]
+    int32_t * out;                   // (accepted, token) a sequence
+};
+void launch_verify(const verify_launch & L, hipStream_t st);
+
+int64_t paged_attn_scratch_bytes(const paged_attn & A);
+void launch_paged_attn(const paged_attn & A, hipStream_t st);
+
 void launch_soft_max(const tview & a, const tview * mask, const tview & dst, float scale, float max_bias, hipStream_t st);
 // dst = silu(gate) * up (2-D f32 views), with its Q8_0 (q) or Q8_K (qk) quantization when set; without
 // keep only that quantization may be written

@@ -97,9 +97,31 @@ GGML_API enum ggml_status ggml_backend_hip_logprobs(ggml_backend_t backend, cons
                                                     int64_t n_rows, const int32_t * tokens, int32_t n_top,
                                                     float * logprob, float * entropy, int32_t * top_ids, float * top_logprobs);
 
+// Verifies drafted tokens against the target's probabilities, from given random numbers, for n_seqs
+// sequences: each has n_drafted[s] tokens (0 to GGML_HIP_VERIFY_MAX_DRAFT), as many rows of
+// draft_probs and numbers of u, and one more row of probs and number of u, all packed sequence after
+// sequence. probs, draft_probs: F32 tensors in this backend's buffer with contiguous rows of n values
+// (ggml row index over ne[1..3]), each a distribution; draft_probs may be NULL for drafts made without
+// probabilities (then each is certain of its token). tokens: ids below n; u: numbers in [0, 1).
+//   n_accepted[s]  the first tokens x_i with u_i q_i(x_i) < p_i(x_i), up to the first without
+//   token[s]       the token behind them: drawn with the sequence's last u from the weights
+//                  max(p_i - q_i, 0) at the first that is not accepted (from p_i where all are 0), or
+//                  from the last row of probs: the first id at which the running sum of weights
+//                  exceeds u times their sum. -1 where that sum is not a positive number
+// So accepted and drawn tokens are distributed as the target's own. Sums are 64-bit. Synchronous, on the
+// backend's stream: returns when the outputs are on the host, and waits for the graph that computes the
+// probabilities, which it may follow at once. Calls on one device share its scratch with
+// ggml_backend_hip_logprobs (not from two threads at once). Fails (GGML_STATUS_FAILED, with a message
+// on stderr, and no output written) for another backend or buffer, too few rows, or numbers out of range.
+#define GGML_HIP_VERIFY_MAX_DRAFT 1024
+GGML_API enum ggml_status ggml_backend_hip_verify(ggml_backend_t backend, const struct ggml_tensor * probs,
+                                                  const struct ggml_tensor * draft_probs, int64_t n_seqs,
+                                                  const int32_t * n_drafted, const int32_t * tokens, const double * u,
+                                                  int32_t * n_accepted, int32_t * token);
+
 // Why graph_compute refuses a graph that holds this node, before it queues anything, or NULL: the
-// checks of ssm_conv and ssm_scan (types, extents, strides that leave the tensor), whose graphs it
-// answers with GGML_STATUS_FAILED and this message. Needs no device. Other ops' conditions are
+// checks of ssm_conv, ssm_scan, rope_multi, set_rows and flash_attn_paged (types, extents, strides that
+// leave the tensor), whose graphs it answers with GGML_STATUS_FAILED and this message. Needs no device. Other ops' conditions are
 // checked as they run.
 GGML_API const char * ggml_backend_hip_refusal(const struct ggml_tensor * node);
 

@@ -39,6 +39,11 @@ extern "C" {
 // RoPE modes used by build_graph (model.cpp:1395)
 #define GGML_ROPE_TYPE_NORMAL 0
 #define GGML_ROPE_TYPE_NEOX   2
+// RoPE modes of ggml_rope_multi (ggml's values)
+#define GGML_ROPE_TYPE_MROPE  8
+#define GGML_ROPE_TYPE_VISION 24
+#define GGML_ROPE_TYPE_IMROPE 40
+#define GGML_MROPE_SECTIONS   4
 
 typedef uint16_t ggml_fp16_t;
 typedef struct { uint16_t bits; } ggml_bf16_t;
@@ -106,6 +111,10 @@ enum ggml_op {
     GGML_OP_SSM_CONV,
     GGML_OP_SSM_SCAN,
     GGML_OP_GATED_DELTA_NET,
+    // serving several sequences from a paged cache
+    GGML_OP_ROPE_MULTI,
+    GGML_OP_SET_ROWS,
+    GGML_OP_FLASH_ATTN_PAGED,
     GGML_OP_COUNT,
 };
 
@@ -299,6 +308,33 @@ GGML_API struct ggml_tensor * ggml_ssm_scan(struct ggml_context * ctx, struct gg
 // (model.cpp:1273-1281)
 GGML_API struct ggml_tensor * ggml_gated_delta_net(struct ggml_context * ctx, struct ggml_tensor * q, struct ggml_tensor * k,
         struct ggml_tensor * v, struct ggml_tensor * g, struct ggml_tensor * beta, struct ggml_tensor * state, int version);
+
+// ---- serving several sequences from a paged cache ----
+// RoPE by positions of up to four axes (time, height, width, another). a: F32 [d, n_head, n_tokens, n3], the rows'
+// values contiguous; b: I32 [4 * n_tokens], axis by axis; c: optional F32 frequency factors, one a pair. Pair i is
+// (x[i], x[i + n_pairs]); it turns by b[axis, token] * freq_base^(-2 e / n_dims) / c[i], scaled as ggml_rope_ext scales
+// (freq_scale, ext_factor, attn_factor, beta_fast, beta_slow). sections: pairs of each axis; sector = i modulo their sum.
+//   MROPE:  n_pairs = n_dims / 2, e = i; the axis whose section holds the sector
+//   IMROPE: as MROPE with the axes in turns: axis k where sector % 3 == k and sector < 3 sections[k], else the fourth
+//   VISION: n_dims = d / 2, n_pairs = n_dims; as MROPE with e counted from the section's start
+// Values past the pairs are copied. Angles are formed in 64 bits and each value is rounded once.
+GGML_API struct ggml_tensor * ggml_rope_multi(struct ggml_context * ctx, struct ggml_tensor * a, struct ggml_tensor * b,
+        struct ggml_tensor * c, int n_dims, int sections[GGML_MROPE_SECTIONS], int mode, int n_ctx_orig, float freq_base,
+        float freq_scale, float ext_factor, float attn_factor, float beta_fast, float beta_slow);
+// Row r of b into row c[r] of a, converted to a's type (F32, F16, BF16, Q8_0, Q4_0: blocks as ggml_quantize_chunk forms
+// them); returns a view of a. b: F32 [a->ne[0], n, a->ne[2], a->ne[3]]; c: I32 or I64 [n, c2, c3], c2 dividing a->ne[2] and
+// c3 a->ne[3] (used again over them). A row whose index is outside [0, a->ne[1]) is not stored; of rows with one index the
+// last is. A Q4_0 block that holds a NaN gets a NaN scale.
+GGML_API struct ggml_tensor * ggml_set_rows(struct ggml_context * ctx, struct ggml_tensor * a, struct ggml_tensor * b, struct ggml_tensor * c);
+// Causal attention of the new tokens of several sequences over a cache on pages. q: F32 [d, n_head, n_tokens], rotated, the
+// sequences' tokens one after another: sequence s has tokens q_start[s] .. q_start[s + 1] - 1 (q_start: I32 [n_seqs + 1]), the
+// last of the kv_len[s] positions (I32 [n_seqs]) that it has in the cache. k, v: Q4_0 [d, n_head_kv, page_size, n_pages];
+// position j of sequence s is row j % page_size of page pages[j / page_size, s] (pages: I32 [max_pages, n_seqs]). Head h reads
+// KV head h / (n_head / n_head_kv). Result: F32 [d, n_head, n_tokens], o = sum_j softmax_j(scale q . k_j) v_j over the positions
+// up to the token's own. A token without positions gets zeros. Tokens of no sequence keep what the result's memory held.
+// Positions on a page outside [0, n_pages) do not exist; kv_len is cut to the table, q_start to the tokens.
+GGML_API struct ggml_tensor * ggml_flash_attn_paged(struct ggml_context * ctx, struct ggml_tensor * q, struct ggml_tensor * k,
+        struct ggml_tensor * v, struct ggml_tensor * pages, struct ggml_tensor * q_start, struct ggml_tensor * kv_len, float scale);
 
 // ---- MoE routing (the router of qwen_model.c:551-606 as graph ops) ----
 enum ggml_sort_order {
