@@ -633,7 +633,7 @@ paged_attn paged_attn_of(const ggml_tensor * n) {
     A.q_start = (const int32_t *) n->src[4]->data;
     A.kv_len = (const int32_t *) n->src[5]->data;
     A.n_pages = k->ne[3];
-    A.D = (int) q->ne[0]; A.n_head = (int) q->ne[1]; A.n_head_kv = (int) k->ne[1];
+    A.D = (int) q->ne[0]; A.n_head = (int) q->ne[1]; A.n_head_kv = (int) k->ne[1]; A.group = A.n_head / A.n_head_kv;
     A.n_tokens = (int) q->ne[2]; A.n_seqs = (int) pages->ne[1];
     A.page = (int) k->ne[2]; A.max_pages = (int) pages->ne[0];
     memcpy(&A.scale, n->op_params, 4);

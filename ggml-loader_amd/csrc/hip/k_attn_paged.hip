@@ -3,86 +3,681 @@
 // Token t of sequence s, the i-th of its n, sees positions 0 .. p = kv_len[s] - n + i:
 //   o = sum_j e^(z_j - m) v_j / sum_j e^(z_j - m),  z_j = scale q . k_j,  m = max_j z_j,
 // with k_j = d (c - 8) for each block of 32 codes c under one scale d, and v_j likewise.
+//
+// Both products run on the F16 matrix cores without losing bits of the 32-bit operands: the codes are
+// small integers, exact in F16, and the other operand goes in as two halves (22 bits, two products).
+//   z: A = codes - 8 of 16 positions, B = 16 rows (query, head) of one KV head, a block of 32 values at a time;
+//      the block's sum times the block's scale, in 32 bits.
+//   o: A = codes - 8 of 16 values' columns at 32 positions, B = p d, with the scale of each position's block.
+// The rows of z land in the registers as o's operand B wants them, so p never leaves its lane.
+// K's dwords are exchanged between lanes so that a lane has the four values of a block that its k-index
+// wants; V passes through LDS, whose transposing read gives a lane one value's codes at 16 positions.
 #include "kernels.h"
 #include "ssm_ops.h"
 
+#include <algorithm>
+
 namespace {
 
-// the sequence that token t belongs to, or -1, and its range of tokens
-__device__ __forceinline__ int sequence_of(const paged_attn & A, int t, int & first, int & n) {
-    for (int s = 0; s < A.n_seqs; s++) {
-        const int a = min(max(A.q_start[s], 0), A.n_tokens), b = min(max(A.q_start[s + 1], a), A.n_tokens);
-        if (t >= a && t < b) { first = a; n = b - a; return s; }
-    }
-    return -1;
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef int i2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+
+constexpr int STEP = 64;               // positions of a step
+constexpr int SPLIT_WG = 256;
+constexpr int MIN_STEPS = 2;           // steps a team takes at least
+constexpr float M_NONE = -1.7e38f;     // the maximum of no scores: finite, so that differences are no NaN
+
+// ---- what each sequence asks for ----
+struct seq_info { int first, n, len, last; };   // tokens, positions in the table; the last token sees up to `last`
+
+__device__ __forceinline__ seq_info seq_of(const paged_attn & A, int s) {
+    seq_info q;
+    q.first = min(max(A.q_start[s], 0), A.n_tokens);
+    q.n = min(max(A.q_start[s + 1], q.first), A.n_tokens) - q.first;
+    const int kv = max(A.kv_len[s], 0);
+    q.len = min(kv, A.max_pages * A.page);
+    q.last = A.kv_len[s] - 1;
+    return q;
 }
 
-template <int D>
-__global__ __launch_bounds__(64) void attn_paged_kernel(const paged_attn A) {
-    const int t = blockIdx.x, h = blockIdx.y, lane = threadIdx.x;
-    const int kvh = h / (A.n_head / A.n_head_kv);
-    int first, n;
-    const int s = sequence_of(A, t, first, n);
-    if (s < 0) return;
-    const int len = min(A.kv_len[s], A.max_pages * A.page);
-    const int see = min(A.kv_len[s] - n + (t - first) + 1, len);
-    __shared__ float q[D];
-    for (int i = lane; i < D; i += 64) q[i] = A.q[t * A.q_t + h * A.q_h + i] * A.scale;
-    __syncthreads();
-    float m = -INFINITY, l = 0.0f, o[(D + 63) / 64] = {};
-    for (int j0 = 0; j0 < see; j0 += 64) {
-        const int j = j0 + lane;
-        int64_t page = -1;
-        if (j < see) page = A.pages[s * A.pages_s + j / A.page];
-        float z = -INFINITY;
-        const bool there = page >= 0 && page < A.n_pages;
-        const int64_t row = there ? page : 0;
-        if (there) {
-            const int64_t b0 = page * A.k_page + (j % A.page) * A.k_pos + kvh * A.k_head;
-            z = 0.0f;
-            for (int b = 0; b < D / 32; b++) {
-                float part = 0.0f;
-                for (int i = 0; i < 16; i++) {
-                    const int c = A.kq[(b0 + b) * 16 + i];
-                    part += q[32 * b + i] * (float) ((c & 15) - 8) + q[32 * b + 16 + i] * (float) ((c >> 4) - 8);
+__device__ __forceinline__ int64_t seq_units(const paged_attn & A, const seq_info & q, int tiles_of) {
+    const int tiles = (q.n * A.group + tiles_of - 1) / tiles_of;
+    return (int64_t) tiles * A.head_teams * max((q.len + STEP - 1) / STEP, 1);
+}
+
+// a step is one unit of work; teams (of A.team waves, a KV head each) take equal runs of them
+struct plan {
+    int64_t units, base, rem;
+    int teams;
+    __device__ __forceinline__ int64_t begin(int64_t t) const { return t * base + min(t, rem); }
+    __device__ __forceinline__ int64_t team_of(int64_t u) const {
+        const int64_t big = rem * (base + 1);
+        const int64_t v = u < big ? u : u - big, d = u < big ? base + 1 : base;
+        const int64_t q = v < ((int64_t) 1 << 31) && d < ((int64_t) 1 << 31) ? (int64_t) ((uint32_t) v / (uint32_t) d) : v / d;
+        return u < big ? q : rem + q;
+    }
+};
+
+// a value that every lane holds, as a scalar
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ int64_t uniform(int64_t v) {
+    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t) v), hi = __builtin_amdgcn_readfirstlane((uint32_t) (v >> 32));
+    return (int64_t) (((uint64_t) hi << 32) | lo);
+}
+
+__device__ __forceinline__ int64_t wave_scan(int64_t v) {
+    const int lane = threadIdx.x % WAVE;
+#pragma unroll
+    for (int k = 1; k < WAVE; k *= 2) {
+        const int64_t o = __shfl_up(v, k);
+        if (lane >= k) v += o;
+    }
+    return v;
+}
+
+// the plan, and where the units of sequence `seq` start (seq < 0: not asked)
+__device__ __forceinline__ plan make_plan(const paged_attn & A, int tiles_of, int seq, int64_t & seq_begin) {
+    const int lane = threadIdx.x % WAVE;
+    int64_t all = 0;
+    for (int s0 = 0; s0 < A.n_seqs; s0 += WAVE) {
+        const int s = s0 + lane;
+        const int64_t u = s < A.n_seqs ? seq_units(A, seq_of(A, s), tiles_of) : 0;
+        const int64_t up = wave_scan(u);
+        if (seq >= s0 && seq < s0 + WAVE) seq_begin = uniform(all + __shfl(up - u, seq - s0));
+        all += uniform(__shfl(up, WAVE - 1));
+    }
+    plan P;
+    P.units = all;
+    const int64_t want = (all + MIN_STEPS - 1) / MIN_STEPS;
+    P.teams = (int) max((int64_t) 1, min((int64_t) A.teams, want));
+    if (all < ((int64_t) 1 << 31)) {
+        P.base = uniform((int) ((uint32_t) all / (uint32_t) P.teams));
+        P.rem = (uint32_t) all - (uint32_t) P.base * (uint32_t) P.teams;
+    } else {
+        P.base = all / P.teams;
+        P.rem = all % P.teams;
+    }
+    return P;
+}
+
+// the sequence that unit u falls into, and the first unit of it
+__device__ __forceinline__ int find_unit(const paged_attn & A, int tiles_of, int64_t u, int64_t & begin) {
+    const int lane = threadIdx.x % WAVE;
+    int64_t all = 0;
+    for (int s0 = 0; s0 < A.n_seqs; s0 += WAVE) {
+        const int s = s0 + lane;
+        const int64_t n = s < A.n_seqs ? seq_units(A, seq_of(A, s), tiles_of) : 0;
+        const int64_t up = all + wave_scan(n);
+        const uint64_t past = __ballot(up > u);
+        if (past) {
+            const int l = __builtin_ctzll(past);
+            begin = uniform(__shfl(up - n, l));
+            return s0 + l;
+        }
+        all = uniform(__shfl(up, WAVE - 1));
+    }
+    return A.n_seqs;
+}
+
+__device__ __forceinline__ int page_index(const paged_attn & A, int pos) {
+    return A.page_mul ? (int) (__umulhi((uint32_t) pos, A.page_mul) >> A.page_shift) : pos >> A.page_shift;
+}
+
+// ---- operands ----
+__device__ __forceinline__ h8 as_h8(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    const uint4 v = make_uint4(a, b, c, d);
+    return __builtin_bit_cast(h8, v);
+}
+
+// codes - 8, nibbles (0, 4), (1, 5), (2, 6), (3, 7): 1024 + c or 64 + c in F16, less 1032 or 72. (The codes as F16
+// subnormals, with a term for the 8, would take half as many instructions, but the matrix cores' sums of
+// subnormals are exact to 1e-5 only.)
+struct code_bits {
+    uint32_t low = 0x64006400u, high = 0x54005400u;
+    // in registers, not literals: an instruction takes a mask or them from elsewhere, not both
+    __device__ __forceinline__ code_bits() { asm("" : "+v"(low), "+v"(high)); }
+};
+__device__ __forceinline__ h8 signed_of(uint32_t x, const code_bits & K) {
+    const uint32_t y = x >> 8;
+    auto low = [&](uint32_t v) { return __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2, (v & 0x000F000Fu) | K.low) - h2{ 1032, 1032 }); };
+    auto high = [&](uint32_t v) { return __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2, (v & 0x00F000F0u) | K.high) - h2{ 72, 72 }); };
+    return as_h8(low(x), high(x), low(y), high(y));
+}
+
+// dword c of row k's four to lane group k's register c and back: r[k] in lane group c = r[c] of group k
+__device__ __forceinline__ void transpose4(uint32_t (&r)[4]) {
+#define SWAP(op, a, b)                                              \
+    do {                                                            \
+        const auto v = __builtin_amdgcn_##op(a, b, false, false);   \
+        a = v[0];                                                   \
+        b = v[1];                                                   \
+    } while (0)
+    SWAP(permlane32_swap, r[0], r[2]);
+    SWAP(permlane32_swap, r[1], r[3]);
+    SWAP(permlane16_swap, r[0], r[1]);
+    SWAP(permlane16_swap, r[2], r[3]);
+#undef SWAP
+}
+
+// over the four lane groups of one column
+__device__ __forceinline__ float column_max(float v) {
+    v = fmaxf(v, __shfl_xor(v, 16));
+    return fmaxf(v, __shfl_xor(v, 32));
+}
+__device__ __forceinline__ float column_sum(float v) {
+    v += __shfl_xor(v, 16);
+    return v + __shfl_xor(v, 32);
+}
+
+template <int NB> struct halves { _Float16 v[NB]; };
+template <bool B> struct flag { static constexpr bool value = B; };
+
+__device__ __forceinline__ float half_at(const uint32_t * w, int k) { return (float) __builtin_bit_cast(h2, w[k / 2])[k % 2]; }
+
+// the value of the lane n further in its row of 16, cyclically
+template <int N> __device__ __forceinline__ float row_ror(float v) { return dpp_f<0x120 + N>(v); }
+
+// Few rows a sequence: a wave takes steps of one KV head by itself.
+//
+// Wide: the 16 columns of a tile are 16 rows (query, head), RT tiles of them. Narrow, for up to 16 / NB rows (4 for
+// heads of 96): a column is a row and a block, B holds that block's values and zeros elsewhere, and one tile
+// of sums holds every block's: a lane scales its own block's and sums by neighbours, and forms p d for its own
+// block only, which serves all blocks' products (a quarter of the work where a KV head has four query heads).
+//
+// P16: pages of whole sixteens of rows, so that a load's 16 positions are on one page, found by scalar loads.
+template <int NB, int RT, bool NARROW, bool P16>
+__global__ __launch_bounds__(SPLIT_WG, 2) void paged_split_kernel(const paged_attn A) {
+    constexpr int D = NB * 32, COLS = NARROW ? (NB == 2 ? 8 : 4) : 16, ROWS = COLS * RT;
+    constexpr int LOADS = NB == 2 ? 2 : 4;            // 16-byte loads a lane of a step's K or V
+    constexpr int SROW = STEP + 8;                    // scales of a block over a step's positions
+    static_assert(!NARROW || RT == 1, "one tile");
+    __shared__ __align__(16) uint8_t s_v[SPLIT_WG / WAVE][STEP * NB * 16];
+    __shared__ __align__(16) _Float16 s_kd[SPLIT_WG / WAVE][NB * SROW], s_vd[SPLIT_WG / WAVE][NB * SROW];
+    const int lane = threadIdx.x % WAVE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
+    const int col = lane % 16, c = lane / 16;         // the lane's column of a tile, its lane group
+    const int own = NARROW ? min(col / COLS, NB - 1) : 0;                  // narrow: the column's block
+    const bool spare = NARROW && col / COLS >= NB;
+    const int per_wg = (SPLIT_WG / WAVE) / A.team;
+    const int64_t team = (int64_t) blockIdx.x * per_wg + wave / A.team;   // (a team is 1, 2 or 4 waves)
+    const int in_team = wave & (A.team - 1);
+    const code_bits K;
+
+    int64_t none = 0;
+    const plan P = make_plan(A, ROWS, -1, none);
+    if (team >= P.teams) return;
+    int64_t u = P.begin(team);
+    const int64_t end = P.begin(team + 1);
+    if (u >= end) return;
+    int64_t begin = 0;
+    int seq = uniform(find_unit(A, ROWS, u, begin));
+    u -= begin;                                       // within the sequence
+    int64_t left = end - begin - u;
+
+    while (left > 0 && seq < A.n_seqs) {
+        const seq_info Q = seq_of(A, seq);
+        const int steps = max((Q.len + STEP - 1) / STEP, 1);
+        const int tiles = (Q.n * A.group + ROWS - 1) / ROWS;
+        if (u >= (int64_t) tiles * A.head_teams * steps) { seq++; u = 0; continue; }
+        const int item = uniform(u < ((int64_t) 1 << 32) ? (int) ((uint32_t) u / (uint32_t) steps) : (int) (u / steps));
+        const int step0 = (int) (u - (int64_t) item * steps);
+        const int tile = uniform((int) ((uint32_t) item / (uint32_t) A.head_teams)), head = (item - tile * A.head_teams) * A.team + in_team;
+        const int step1 = (int) min((int64_t) steps, step0 + left);
+        u += step1 - step0;
+        left -= step1 - step0;
+
+        // ---- the rows: two halves of each value, scaled so that a row's largest is near 2^14 ----
+        h8 qh[RT][NB], ql[RT][NB];
+        float fac[RT], m[RT], l[RT];
+        int lim[RT];
+        f4 o[RT][NB][2];
+#pragma unroll
+        for (int t = 0; t < RT; t++) {
+            const int row = tile * ROWS + t * 16 + (NARROW ? col % COLS : col);
+            const bool real = row < Q.n * A.group;
+            const int i = real ? row / A.group : 0, g = real ? row - i * A.group : 0;
+            const float * q = A.q + (int64_t) (Q.first + i) * A.q_t + (int64_t) (head * A.group + g) * A.q_h;
+            // rows that are not there see what the last one sees
+            lim[t] = min(Q.last - (Q.n - 1) + (real ? i : Q.n - 1), Q.len - 1);
+            float big = 0.0f;
+            auto values = [&](int b, float (&v)[8]) {
+                const float4 lo = load4(q + 32 * b + 4 * c), hi = load4(q + 32 * b + 16 + 4 * c);
+                const float w[8] = { lo.x, lo.z, hi.x, hi.z, lo.y, lo.w, hi.y, hi.w };
+#pragma unroll
+                for (int k = 0; k < 8; k++) v[k] = real && !spare ? w[k] : 0.0f;
+            };
+            // the row's largest value: of its own block in each column, narrow
+            float v[8];
+#pragma unroll
+            for (int b = 0; b < (NARROW ? 1 : NB); b++) {
+                values(NARROW ? own : b, v);
+#pragma unroll
+                for (int k = 0; k < 8; k++) big = fmaxf(big, fabsf(v[k]));
+            }
+            if (NARROW) {
+                big = fmaxf(big, row_ror<8>(big));
+                if (NB > 2) big = fmaxf(big, row_ror<4>(big));
+            }
+            big = column_max(big);
+            const int e = big > 0.0f && big < INFINITY ? 14 - __builtin_amdgcn_frexp_expf(big) : 0;
+#pragma unroll
+            for (int b = 0; b < NB; b++) {
+                if (!NARROW) values(b, v);
+#pragma unroll
+                for (int k = 0; k < 8; k++) {
+                    const float x = NARROW && b != own ? 0.0f : __builtin_amdgcn_ldexpf(v[k], e);
+                    qh[t][b][k] = (_Float16) x;
+                    ql[t][b][k] = (_Float16) (x - (float) qh[t][b][k]);
                 }
-                z += part * __half2float(A.kd[b0 + b]);
             }
+            fac[t] = A.scale * LOG2E * __builtin_amdgcn_ldexpf(1.0f, -e);
+            m[t] = M_NONE;
+            l[t] = 0.0f;
+#pragma unroll
+            for (int b = 0; b < NB; b++) o[t][b][0] = o[t][b][1] = f4{ 0, 0, 0, 0 };
         }
-        const float big = fmaxf(m, wave_max(z));
-        if (big == -INFINITY) continue;
-        const float p = there ? exp2_hw((z - big) * LOG2E) : 0.0f, keep = exp2_hw((m - big) * LOG2E);
-        l = l * keep + group_sum<64>(p);
-        m = big;
-        for (int k = 0; k < (D + 63) / 64; k++) o[k] *= keep;
-        for (int i = 0; i < 64; i++) {
-            const float w = lane_f(p, i);
-            if (w == 0.0f) continue;
-            const int64_t pg = __shfl(row, i);
-            const int64_t b0 = pg * A.v_page + ((j0 + i) % A.page) * A.v_pos + kvh * A.v_head;
-            for (int k = 0; k < (D + 63) / 64; k++) {
-                const int e = lane + 64 * k;
-                if (e >= D) continue;
-                const int c = A.vq[(b0 + e / 32) * 16 + e % 16], code = e % 32 < 16 ? c & 15 : c >> 4;
-                o[k] += w * (float) (code - 8) * __half2float(A.vd[b0 + e / 32]);
+        // p d is formed times 2^shift, so that the largest scale seen gives 2^14 to 2^15
+        int shift = 38;
+        const int sure = Q.last - (Q.n - 1) + tile * ROWS / A.group;        // positions up to here are seen by all rows
+
+        // ---- a step's operands: the rows of its positions, their bytes and scales ----
+        const int32_t * table = A.pages + (int64_t) seq * A.pages_s;
+        const uint8_t * kq = A.kq + (int64_t) head * A.k_head * 16, * vq = A.vq + (int64_t) head * A.v_head * 16;
+        const _Float16 * kdp = (const _Float16 *) A.kd + (int64_t) head * A.k_head, * vdp = (const _Float16 *) A.vd + (int64_t) head * A.v_head;
+        auto lane_of = [&](int j) { return NB == 2 ? 32 * j + 16 * (c >> 1) + col : 16 * j + col; };
+        const int blk = NB == 2 ? (c & 1) : min(c, NB - 1);
+        // P16: pages of the step's four sixteens (scalars); else of the lane's position
+        int page[4];
+        auto pages_of = [&](int step) {
+#pragma unroll
+            for (int j = 0; j < (P16 ? 4 : 1); j++) {
+                const int pos = step * STEP + (P16 ? 16 * j : lane);
+                page[j] = pos < Q.len && step < step1 ? table[page_index(A, pos)] : -1;
             }
+        };
+        int64_t krow[P16 ? 4 : 1], vrow[P16 ? 4 : 1];    // first block of a sixteen's rows, or of the lane's
+        bool there;                                      // the lane's position is in the cache
+        uint64_t missing_next;                           // positions whose page is not there
+        auto locate = [&](int step) {
+            const int pos = step * STEP + lane;
+            uint64_t bad = 0;
+            there = pos < Q.len;
+#pragma unroll
+            for (int j = 0; j < (P16 ? 4 : 1); j++) {
+                const int p0 = step * STEP + (P16 ? 16 * j : lane);
+                const bool ok = page[j] >= 0 && page[j] < A.n_pages;
+                const int off = p0 - page_index(A, p0) * A.page;
+                krow[j] = ok ? (int64_t) page[j] * A.k_page + (int64_t) off * A.k_pos : 0;
+                vrow[j] = ok ? (int64_t) page[j] * A.v_page + (int64_t) off * A.v_pos : 0;
+                if (P16) {
+                    if (!ok) bad |= 0xFFFFull << (16 * j);
+                } else {
+                    bad = __ballot(there && !ok);
+                    there = there && ok;
+                }
+            }
+            if (P16) {
+                there = there && !((bad >> lane) & 1);
+                bad &= Q.len - step * STEP >= STEP ? ~0ull : (1ull << max(Q.len - step * STEP, 0)) - 1;
+            }
+            missing_next = bad;
+        };
+        // the 16 bytes of load j, and the lane's own position's first block
+        auto bytes_of = [&](const uint8_t * base, const int64_t * row, int64_t per_pos, int j) -> const uint8_t * {
+            if (!P16) return base + (__shfl(row[0], lane_of(j)) + blk) * 16;
+            int64_t r = row[NB == 2 ? 2 * j : j];
+            if (NB == 2) r += (c >> 1) * (row[2 * j + 1] - r);
+            return base + r * 16 + (uint32_t) ((col * (int) per_pos + blk) * 16);
+        };
+        auto scales_of = [&](const _Float16 * base, const int64_t * row, int64_t per_pos) {
+            if (!P16) return base + row[0];
+            const int64_t r = row[0] + (c & 1) * (row[1] - row[0]), r2 = row[2] + (c & 1) * (row[3] - row[2]);
+            return base + r + (c >> 1) * (r2 - r) + col * (int) per_pos;
+        };
+        u4 kraw[LOADS], vraw[LOADS];
+        halves<NB> kd, vd;
+        auto load_v = [&]() {
+#pragma unroll
+            for (int j = 0; j < LOADS; j++) vraw[j] = *(const u4 *) bytes_of(vq, vrow, A.v_pos, j);
+            const _Float16 * kp = scales_of(kdp, krow, A.k_pos), * vp = scales_of(vdp, vrow, A.v_pos);
+#pragma unroll
+            for (int b = 0; b < NB; b++) {
+                kd.v[b] = kp[b];
+                vd.v[b] = vp[b];
+            }
+        };
+        auto load_k = [&]() {
+#pragma unroll
+            for (int j = 0; j < LOADS; j++) kraw[j] = *(const u4 *) bytes_of(kq, krow, A.k_pos, j);
+        };
+        pages_of(step0);
+        locate(step0);
+        load_k();
+        load_v();
+        pages_of(step0 + 1);
+
+        for (int step = step0; step < step1; step++) {
+            const bool more = step + 1 < step1;
+            const uint64_t missing = missing_next;
+            // ---- V and the scales into LDS, the next ones on their way ----
+#pragma unroll
+            for (int j = 0; j < LOADS; j++) *(u4 *) &s_v[wave][(lane_of(j) * NB + blk) * 16] = vraw[j];
+            float dmax = 0.0f;
+#pragma unroll
+            for (int b = 0; b < NB; b++) {
+                s_kd[wave][b * SROW + lane] = kd.v[b];
+                if (!there) vd.v[b] = 0;
+                s_vd[wave][b * SROW + lane] = vd.v[b];
+                dmax = fmaxf(dmax, fabsf((float) vd.v[b]));
+            }
+            if (more) {
+                locate(step + 1);
+                load_v();
+            }
+
+            // ---- scores ----
+            f4 s[RT][4];
+#pragma unroll
+            for (int j = 0; j < LOADS; j++) {
+                __builtin_amdgcn_sched_barrier(0);
+                uint32_t r[4] = { kraw[j].x, kraw[j].y, kraw[j].z, kraw[j].w };
+                transpose4(r);
+#pragma unroll
+                for (int half = 0; half < 4 / LOADS; half++) {
+                    const int t = 4 / LOADS * j + half;
+                    f4 acc[RT];
+#pragma unroll
+                    for (int b = 0; b < NB; b++) {
+                        const h8 a = signed_of(r[half * 2 + b], K);
+                        if (!NARROW || b == 0) {
+#pragma unroll
+                            for (int x = 0; x < RT; x++) acc[x] = f4{ 0, 0, 0, 0 };
+                        }
+#pragma unroll
+                        for (int x = 0; x < RT; x++) {
+                            acc[x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, qh[x][b], acc[x], 0, 0, 0);
+                            acc[x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, ql[x][b], acc[x], 0, 0, 0);
+                        }
+                        if (NARROW && b < NB - 1) continue;
+                        const uint2 d = *(const uint2 *) &s_kd[wave][(NARROW ? own : b) * SROW + 16 * t + 4 * c];
+                        const uint32_t w[2] = { d.x, d.y };
+#pragma unroll
+                        for (int x = 0; x < RT; x++) {
+#pragma unroll
+                            for (int i = 0; i < 4; i++) s[x][t][i] = fmaf(acc[x][i], half_at(w, i), NARROW || b == 0 ? 0.0f : s[x][t][i]);
+                        }
+                    }
+                    if (NARROW) {
+                        // a spare column's sums are 0 times a scale: 0, or a NaN as that block's own column has it
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            s[0][t][i] += row_ror<8>(s[0][t][i]);
+                            if (NB > 2) s[0][t][i] += row_ror<4>(s[0][t][i]);
+                        }
+                    }
+                }
+            }
+            if (more) load_k();
+            pages_of(step + 2);
+            // the largest scale of V so far
+            if (__any(dmax >= __builtin_amdgcn_ldexpf(1.0f, 15 - shift))) {
+                const float big = wave_max(dmax);
+                const int now = min(shift, 14 - min(max(__builtin_amdgcn_frexp_expf(big < 65536.0f ? big : 65504.0f), -24), 16));
+                const float keep = __builtin_amdgcn_ldexpf(1.0f, now - shift);
+                shift = now;
+#pragma unroll
+                for (int x = 0; x < RT; x++) {
+                    l[x] *= keep;
+#pragma unroll
+                    for (int b = 0; b < NB; b++) { o[x][b][0] *= keep; o[x][b][1] *= keep; }
+                }
+            }
+            const bool edge = step * STEP + STEP - 1 > sure || missing;
+            uint32_t hidden[RT];
+#pragma unroll
+            for (int x = 0; x < RT; x++) {
+                hidden[x] = 0;
+                if (edge) {
+#pragma unroll
+                    for (int t = 0; t < 4; t++) {
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            const int k = 16 * t + 4 * c + i;
+                            if (step * STEP + k > lim[x] || ((missing >> k) & 1)) {
+                                // (fac may be negative or 0)
+                                s[x][t][i] = 0.0f;
+                                hidden[x] |= 1u << (4 * t + i);
+                            }
+                        }
+                    }
+                }
+                float top = -INFINITY;
+#pragma unroll
+                for (int t = 0; t < 4; t++) {
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        s[x][t][i] *= fac[x];
+                        if (edge && ((hidden[x] >> (4 * t + i)) & 1)) s[x][t][i] = -INFINITY;
+                        top = fmaxf(top, s[x][t][i]);
+                    }
+                }
+                top = column_max(top);
+                if (__any(top > m[x])) {
+                    const float now = fmaxf(m[x], top), keep = exp2_hw(m[x] - now);
+                    m[x] = now;
+                    l[x] *= keep;
+#pragma unroll
+                    for (int b = 0; b < NB; b++) { o[x][b][0] *= keep; o[x][b][1] *= keep; }
+                }
+                const float at = m[x] - (float) shift;
+                float sum = 0.0f;
+#pragma unroll
+                for (int t = 0; t < 4; t++) {
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        s[x][t][i] = exp2_hw(s[x][t][i] - at);
+                        sum += s[x][t][i];
+                    }
+                }
+                l[x] += sum;
+            }
+
+            // ---- o += p d (codes - 8), 32 positions of a block at a time ----
+            // lane (col, c) reads the transposed codes of row 16 (col / 4) + 4 c + col % 4
+            const uint8_t * vrow16 = &s_v[wave][(16 * (col >> 2) + 4 * c + (col & 3)) * NB * 16];
+            auto products = [&](auto at_edge) {
+                constexpr bool EDGE = decltype(at_edge)::value;
+#pragma unroll
+                for (int k = 0; k < 2; k++) {
+                    h8 ph[RT], pl[RT];
+                    auto weights = [&](int b) {
+                        const uint2 d0 = *(const uint2 *) &s_vd[wave][b * SROW + 32 * k + 4 * c], d1 = *(const uint2 *) &s_vd[wave][b * SROW + 32 * k + 16 + 4 * c];
+                        const uint32_t w[4] = { d0.x, d0.y, d1.x, d1.y };
+#pragma unroll
+                        for (int x = 0; x < RT; x++) {
+#pragma unroll
+                            for (int i = 0; i < 4; i++) {
+#pragma unroll
+                                for (int t = 0; t < 2; t++) {
+                                    const float p = s[x][2 * k + t][i];
+                                    float d = half_at(w, 4 * t + i);
+                                    if (EDGE) d = (hidden[x] >> (4 * (2 * k + t) + i)) & 1 ? 0.0f : d;
+                                    const _Float16 hi = (_Float16) fmaf(p, d, 0.0f);
+                                    ph[x][2 * i + t] = hi;
+                                    pl[x][2 * i + t] = (_Float16) fmaf(p, d, -(float) hi);
+                                }
+                            }
+                        }
+                    };
+                    if (NARROW) weights(own);
+#pragma unroll
+                    for (int b = 0; b < NB; b++) {
+                        __builtin_amdgcn_sched_barrier(0);
+                        if (!NARROW) weights(b);
+#pragma unroll
+                        for (int h = 0; h < 2; h++) {
+                            const i2 codes = __builtin_amdgcn_ds_read_tr4_b64_v2i32((__attribute__((address_space(3))) i2 *) (vrow16 + b * 16 + h * 8));
+                            const h8 a = signed_of(codes[k], K);
+#pragma unroll
+                            for (int x = 0; x < RT; x++) {
+                                o[x][b][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, ph[x], o[x][b][h], 0, 0, 0);
+                                o[x][b][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, pl[x], o[x][b][h], 0, 0, 0);
+                            }
+                        }
+                    }
+                }
+            };
+            if (edge) products(flag<true>());
+            else products(flag<false>());
+        }
+
+        // ---- the rows' results, or this run's part of them ----
+        const bool whole = step0 == 0 && step1 == steps;
+        const int64_t slot = ((team * 2 + (step0 == 0)) * A.team + in_team) * ROWS;
+#pragma unroll
+        for (int x = 0; x < RT; x++) {
+            const int at_row = x * 16 + (NARROW ? col % COLS : col), row = tile * ROWS + at_row;
+            const float sum = column_sum(l[x]);
+            if (row >= Q.n * A.group || spare) continue;
+            const int i = row / A.group, g = row - i * A.group;
+            // no positions: 0; a NaN stays one
+            const float inv = whole ? (sum > 0.0f ? 1.0f / sum : sum == 0.0f ? 0.0f : sum) : 1.0f;
+            float * out = whole ? A.out + ((int64_t) (Q.first + i) * A.n_head + head * A.group + g) * D
+                                : A.part + (slot + at_row) * D;
+#pragma unroll
+            for (int b = 0; b < NB; b++) {
+                if (NARROW && b != own) continue;
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    // the codes' column 4 c + r of eight bytes: value (4 c + r) / 2 of them, or 16 further
+                    float * at = out + 32 * b + 8 * h + 2 * c;
+                    *(float2 *) at = make_float2(o[x][b][h][0] * inv, o[x][b][h][2] * inv);
+                    *(float2 *) (at + 16) = make_float2(o[x][b][h][1] * inv, o[x][b][h][3] * inv);
+                }
+            }
+            if (!whole && c == 0 && own == 0) A.part_ml[slot + at_row] = make_float2(m[x] - (float) shift, sum);
         }
     }
-    for (int k = 0; k < (D + 63) / 64; k++) {
-        const int e = lane + 64 * k;
-        if (e < D) A.out[((int64_t) t * A.n_head + h) * D + e] = l > 0.0f ? o[k] / l : l == 0.0f ? 0.0f : l;
+}
+
+// Rows whose steps several teams took: their parts joined, a workgroup a row, D / 4 threads a part.
+template <int NB, int ROWS>
+__global__ __launch_bounds__(256) void paged_join_kernel(const paged_attn A) {
+    constexpr int D = NB * 32, PER = D / 4, GROUPS = 256 / PER;
+    __shared__ float4 s_o[GROUPS][PER];
+    __shared__ float2 s_ml[GROUPS];
+    const int token = blockIdx.x, head = blockIdx.y, t = threadIdx.x, lane = t % WAVE;
+    // the token's sequence
+    int seq = -1;
+    for (int s0 = 0; s0 < A.n_seqs && seq < 0; s0 += WAVE) {
+        const int s = s0 + lane;
+        bool mine = false;
+        if (s < A.n_seqs) {
+            const seq_info q = seq_of(A, s);
+            mine = token >= q.first && token < q.first + q.n;
+        }
+        const uint64_t b = __ballot(mine);
+        if (b) seq = s0 + __builtin_ctzll(b);
     }
+    if (seq < 0) return;
+    const seq_info Q = seq_of(A, seq);
+    int64_t begin = 0;
+    const plan P = make_plan(A, ROWS, seq, begin);
+    const int kvh = head / A.group, row = (token - Q.first) * A.group + head - kvh * A.group;
+    const int tile = row / ROWS, steps = max((Q.len + STEP - 1) / STEP, 1);
+    const int64_t a = begin + ((int64_t) tile * A.head_teams + kvh / A.team) * steps;
+    const int64_t t0 = P.team_of(a), t1 = P.team_of(a + steps - 1);
+    if (t0 == t1) return;                               // written whole
+    const int group = t / PER, e = t % PER;
+    float m = M_NONE, l = 0.0f;
+    float4 o = make_float4(0, 0, 0, 0);
+    if (group < GROUPS) {
+        for (int64_t k = t0 + group; k <= t1; k += GROUPS) {
+            const int64_t at = ((k * 2 + (k == t0)) * A.team + kvh % A.team) * ROWS + row - tile * ROWS;
+            const float2 ml = A.part_ml[at];
+            const float4 v = *(const float4 *) (A.part + at * D + 4 * e);
+            const float now = fmaxf(m, ml.x), was = exp2_hw(m - now), is = exp2_hw(ml.x - now);
+            l = l * was + ml.y * is;
+            o.x = o.x * was + v.x * is;
+            o.y = o.y * was + v.y * is;
+            o.z = o.z * was + v.z * is;
+            o.w = o.w * was + v.w * is;
+            m = now;
+        }
+        s_o[group][e] = o;
+        if (e == 0) s_ml[group] = make_float2(m, l);
+    }
+    __syncthreads();
+    if (t >= PER) return;
+    float top = M_NONE;
+    for (int k = 0; k < GROUPS; k++) top = fmaxf(top, s_ml[k].x);
+    l = 0.0f;
+    o = make_float4(0, 0, 0, 0);
+    for (int k = 0; k < GROUPS; k++) {
+        const float w = exp2_hw(s_ml[k].x - top);
+        const float4 v = s_o[k][t];
+        l += s_ml[k].y * w;
+        o.x += v.x * w;
+        o.y += v.y * w;
+        o.z += v.z * w;
+        o.w += v.w * w;
+    }
+    const float inv = l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : l;
+    *(float4 *) (A.out + ((int64_t) token * A.n_head + head) * D + 4 * t) = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+}
+
+constexpr int SPLIT_WGS = 512;         // two workgroups of four waves a CU
+
+// rows of a tile: narrow, one or two of 16
+int split_rows(const paged_attn & A) {
+    const int narrow = A.D == 64 ? 8 : 4;
+    const int64_t rows = (int64_t) A.n_tokens * A.group, per = A.n_seqs;
+    return rows <= narrow * per && A.group <= narrow ? narrow : rows <= 16 * per ? 16 : 32;
+}
+
+template <int NB, int RT, bool NARROW>
+void split(const paged_attn & A, hipStream_t st) {
+    constexpr int ROWS = NARROW ? (NB == 2 ? 8 : 4) : 16 * RT;
+    // a sixteen of positions on one page, its rows within 32-bit offsets
+    const int64_t reach = 16 * 16 * std::max(A.k_pos, A.v_pos);
+    if (A.page % 16 == 0 && reach <= INT32_MAX) launch(paged_split_kernel<NB, RT, NARROW, true>, dim3(SPLIT_WGS), dim3(SPLIT_WG), 0, st, A);
+    else launch(paged_split_kernel<NB, RT, NARROW, false>, dim3(SPLIT_WGS), dim3(SPLIT_WG), 0, st, A);
+    launch(paged_join_kernel<NB, ROWS>, dim3(A.n_tokens, A.n_head), dim3(256), 0, st, A);
+}
+
+template <int NB>
+void split_by_rows(const paged_attn & A, int rows, hipStream_t st) {
+    if (rows < 16) split<NB, 1, true>(A, st);
+    else if (rows == 16) split<NB, 1, false>(A, st);
+    else split<NB, 2, false>(A, st);
 }
 
 } // namespace
 
-int64_t paged_attn_scratch_bytes(const paged_attn & A) { (void) A; return 0; }
+// parts: two a wave
+int64_t paged_attn_scratch_bytes(const paged_attn & A) {
+    if (A.n_tokens == 0 || A.n_seqs == 0 || A.n_head == 0) return 0;
+    const int64_t rows = (int64_t) SPLIT_WGS * (SPLIT_WG / WAVE) * 2 * split_rows(A);
+    return rows * (A.D * 4 + 8);
+}
 
-void launch_paged_attn(const paged_attn & A, hipStream_t st) {
+void launch_paged_attn(paged_attn A, hipStream_t st) {
     if (A.n_tokens == 0 || A.n_seqs == 0 || A.n_head == 0) return;
-    const dim3 grid(A.n_tokens, A.n_head);
-    if (A.D == 64) launch(attn_paged_kernel<64>, grid, dim3(64), 0, st, A);
-    else if (A.D == 96) launch(attn_paged_kernel<96>, grid, dim3(64), 0, st, A);
-    else if (A.D == 128) launch(attn_paged_kernel<128>, grid, dim3(64), 0, st, A);
+    A.team = A.n_head_kv % 4 == 0 ? 4 : A.n_head_kv % 2 == 0 ? 2 : 1;
+    A.head_teams = A.n_head_kv / A.team;
+    A.teams = SPLIT_WGS * (SPLIT_WG / WAVE) / A.team;
+    // pos / page as a product: exact below 2^31 (the multiplier is rounded up, by less than 2^-31 of it)
+    int bits = 0;
+    while ((1ll << bits) < A.page) bits++;
+    A.page_shift = (1ll << bits) == A.page ? bits : bits - 1;
+    A.page_mul = (1ll << bits) == A.page ? 0 : (uint32_t) (((uint64_t) 1 << (31 + bits)) / A.page + 1);
+    const int rows = split_rows(A);
+    A.part = (float *) A.scratch;
+    A.part_ml = (float2 *) (A.part + (int64_t) A.teams * A.team * 2 * rows * A.D);
+    if (A.D == 64) split_by_rows<2>(A, rows, st);
+    else if (A.D == 96) split_by_rows<3>(A, rows, st);
+    else if (A.D == 128) split_by_rows<4>(A, rows, st);
     else HIP_ABORT("flash_attn_paged: heads of %d values", A.D);
 }

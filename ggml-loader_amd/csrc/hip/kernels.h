@@ -426,9 +426,14 @@ struct paged_attn {
     const int32_t * pages, * q_start, * kv_len;
     int64_t pages_s;                 // I32s between sequences
     int64_t n_pages;
-    int D, n_head, n_head_kv, n_tokens, n_seqs, page, max_pages;
+    int D, n_head, n_head_kv, group, n_tokens, n_seqs, page, max_pages;
     float scale;
-    void * scratch;
+    void * scratch;                  // paged_attn_scratch_bytes
+    // set by launch_paged_attn
+    int team, head_teams, teams, page_shift;
+    uint32_t page_mul;
+    float * part;
+    float2 * part_ml;
 };
 // Drafted tokens against probabilities (ggml_backend_hip_verify): rows as ggml row indices over ne[1..3]
 constexpr int VERIFY_SEGMENT = 2048;
@@ -446,7 +451,7 @@ struct verify_launch {
 void launch_verify(const verify_launch & L, hipStream_t st);
 
 int64_t paged_attn_scratch_bytes(const paged_attn & A);
-void launch_paged_attn(const paged_attn & A, hipStream_t st);
+void launch_paged_attn(paged_attn A, hipStream_t st);
 
 void launch_soft_max(const tview & a, const tview * mask, const tview & dst, float scale, float max_bias, hipStream_t st);
 // dst = silu(gate) * up (2-D f32 views), with its Q8_0 (q) or Q8_K (qk) quantization when set; without
