@@ -25,47 +25,38 @@ typedef float f4 __attribute__((ext_vector_type(4)));
 typedef int i2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
-constexpr int STEP = 64;               // positions of a step
+constexpr int STEP = 32;               // positions of a step
 constexpr int SPLIT_WG = 256;
-constexpr int MIN_STEPS = 2;           // steps a team takes at least
 constexpr float M_NONE = -1.7e38f;     // the maximum of no scores: finite, so that differences are no NaN
-
-// ---- what each sequence asks for ----
-struct seq_info { int first, n, len, last; };   // tokens, positions in the table; the last token sees up to `last`
-
-__device__ __forceinline__ seq_info seq_of(const paged_attn & A, int s) {
-    seq_info q;
-    q.first = min(max(A.q_start[s], 0), A.n_tokens);
-    q.n = min(max(A.q_start[s + 1], q.first), A.n_tokens) - q.first;
-    const int kv = max(A.kv_len[s], 0);
-    q.len = min(kv, A.max_pages * A.page);
-    q.last = A.kv_len[s] - 1;
-    return q;
-}
-
-__device__ __forceinline__ int64_t seq_units(const paged_attn & A, const seq_info & q, int tiles_of) {
-    const int tiles = (q.n * A.group + tiles_of - 1) / tiles_of;
-    return (int64_t) tiles * A.head_teams * max((q.len + STEP - 1) / STEP, 1);
-}
-
-// a step is one unit of work; teams (of A.team waves, a KV head each) take equal runs of them
-struct plan {
-    int64_t units, base, rem;
-    int teams;
-    __device__ __forceinline__ int64_t begin(int64_t t) const { return t * base + min(t, rem); }
-    __device__ __forceinline__ int64_t team_of(int64_t u) const {
-        const int64_t big = rem * (base + 1);
-        const int64_t v = u < big ? u : u - big, d = u < big ? base + 1 : base;
-        const int64_t q = v < ((int64_t) 1 << 31) && d < ((int64_t) 1 << 31) ? (int64_t) ((uint32_t) v / (uint32_t) d) : v / d;
-        return u < big ? q : rem + q;
-    }
-};
 
 // a value that every lane holds, as a scalar
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 __device__ __forceinline__ int64_t uniform(int64_t v) {
     const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t) v), hi = __builtin_amdgcn_readfirstlane((uint32_t) (v >> 32));
     return (int64_t) (((uint64_t) hi << 32) | lo);
+}
+__device__ __forceinline__ int64_t from_lane(int64_t v, int l) {
+    const uint32_t lo = __builtin_amdgcn_readlane((uint32_t) v, l), hi = __builtin_amdgcn_readlane((uint32_t) (v >> 32), l);
+    return (int64_t) (((uint64_t) hi << 32) | lo);
+}
+
+// ---- what each sequence asks for ----
+struct seq_info { int first, n, len, last; };   // tokens, positions in the table; the last token sees up to `last`
+
+__device__ __forceinline__ seq_info seq_of(const paged_attn & A, int s) {
+    seq_info q;
+    const int a = A.q_start[s], b = A.q_start[s + 1], kv = A.kv_len[s];
+    q.first = min(max(a, 0), A.n_tokens);
+    q.n = min(max(b, q.first), A.n_tokens) - q.first;
+    q.len = min(max(kv, 0), A.max_pages * A.page);
+    q.last = kv - 1;
+    return q;
+}
+
+__device__ __forceinline__ int steps_of(const seq_info & q) { return max((q.len + STEP - 1) / STEP, 1); }
+
+__device__ __forceinline__ int64_t seq_units(const paged_attn & A, const seq_info & q, int rows) {
+    return (int64_t) ((q.n * A.group + rows - 1) / rows) * A.head_teams * steps_of(q);
 }
 
 __device__ __forceinline__ int64_t wave_scan(int64_t v) {
@@ -78,49 +69,30 @@ __device__ __forceinline__ int64_t wave_scan(int64_t v) {
     return v;
 }
 
-// the plan, and where the units of sequence `seq` start (seq < 0: not asked)
-__device__ __forceinline__ plan make_plan(const paged_attn & A, int tiles_of, int seq, int64_t & seq_begin) {
-    const int lane = threadIdx.x % WAVE;
-    int64_t all = 0;
-    for (int s0 = 0; s0 < A.n_seqs; s0 += WAVE) {
-        const int s = s0 + lane;
-        const int64_t u = s < A.n_seqs ? seq_units(A, seq_of(A, s), tiles_of) : 0;
-        const int64_t up = wave_scan(u);
-        if (seq >= s0 && seq < s0 + WAVE) seq_begin = uniform(all + __shfl(up - u, seq - s0));
-        all += uniform(__shfl(up, WAVE - 1));
-    }
-    plan P;
-    P.units = all;
-    const int64_t want = (all + MIN_STEPS - 1) / MIN_STEPS;
-    P.teams = (int) max((int64_t) 1, min((int64_t) A.teams, want));
-    if (all < ((int64_t) 1 << 31)) {
-        P.base = uniform((int) ((uint32_t) all / (uint32_t) P.teams));
-        P.rem = (uint32_t) all - (uint32_t) P.base * (uint32_t) P.teams;
-    } else {
-        P.base = all / P.teams;
-        P.rem = all % P.teams;
-    }
-    return P;
-}
-
-// the sequence that unit u falls into, and the first unit of it
-__device__ __forceinline__ int find_unit(const paged_attn & A, int tiles_of, int64_t u, int64_t & begin) {
-    const int lane = threadIdx.x % WAVE;
-    int64_t all = 0;
-    for (int s0 = 0; s0 < A.n_seqs; s0 += WAVE) {
-        const int s = s0 + lane;
-        const int64_t n = s < A.n_seqs ? seq_units(A, seq_of(A, s), tiles_of) : 0;
-        const int64_t up = all + wave_scan(n);
-        const uint64_t past = __ballot(up > u);
-        if (past) {
-            const int l = __builtin_ctzll(past);
-            begin = uniform(__shfl(up - n, l));
-            return s0 + l;
+// All sequences' tiles, heads and steps in one line of units; teams (of A.team waves, a KV head each) take equal
+// runs of it, so that no mixture of lengths leaves a wave idle.
+struct plan {
+    int64_t units, base, rem;
+    int teams;
+    __device__ __forceinline__ void deal(int64_t all, int most) {
+        units = all;
+        teams = (int) max((int64_t) 1, min((int64_t) most, all));
+        if (all < ((int64_t) 1 << 31)) {
+            base = uniform((int) ((uint32_t) all / (uint32_t) teams));
+            rem = (uint32_t) all - (uint32_t) base * (uint32_t) teams;
+        } else {
+            base = all / teams;
+            rem = all % teams;
         }
-        all = uniform(__shfl(up, WAVE - 1));
     }
-    return A.n_seqs;
-}
+    __device__ __forceinline__ int64_t begin(int64_t t) const { return t * base + min(t, rem); }
+    __device__ __forceinline__ int64_t team_of(int64_t u) const {
+        const int64_t big = rem * (base + 1);
+        const int64_t v = u < big ? u : u - big, d = u < big ? base + 1 : base;
+        const int64_t q = v < ((int64_t) 1 << 31) && d < ((int64_t) 1 << 31) ? (int64_t) ((uint32_t) v / (uint32_t) d) : v / d;
+        return u < big ? q : rem + q;
+    }
+};
 
 __device__ __forceinline__ int page_index(const paged_attn & A, int pos) {
     return A.page_mul ? (int) (__umulhi((uint32_t) pos, A.page_mul) >> A.page_shift) : pos >> A.page_shift;
@@ -128,7 +100,7 @@ __device__ __forceinline__ int page_index(const paged_attn & A, int pos) {
 
 // ---- operands ----
 __device__ __forceinline__ h8 as_h8(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
-    const uint4 v = make_uint4(a, b, c, d);
+    const u4 v = { a, b, c, d };
     return __builtin_bit_cast(h8, v);
 }
 
@@ -147,30 +119,33 @@ __device__ __forceinline__ h8 signed_of(uint32_t x, const code_bits & K) {
     return as_h8(low(x), high(x), low(y), high(y));
 }
 
-// dword c of row k's four to lane group k's register c and back: r[k] in lane group c = r[c] of group k
-__device__ __forceinline__ void transpose4(uint32_t (&r)[4]) {
-#define SWAP(op, a, b)                                              \
+#define LANE_SWAP(op, a, b)                                         \
     do {                                                            \
-        const auto v = __builtin_amdgcn_##op(a, b, false, false);   \
-        a = v[0];                                                   \
-        b = v[1];                                                   \
+        const auto v_ = __builtin_amdgcn_##op(a, b, false, false);  \
+        a = v_[0];                                                  \
+        b = v_[1];                                                  \
     } while (0)
-    SWAP(permlane32_swap, r[0], r[2]);
-    SWAP(permlane32_swap, r[1], r[3]);
-    SWAP(permlane16_swap, r[0], r[1]);
-    SWAP(permlane16_swap, r[2], r[3]);
-#undef SWAP
+
+// register k of lane group c to register c of lane group k
+__device__ __forceinline__ void transpose4(uint32_t (&r)[4]) {
+    LANE_SWAP(permlane32_swap, r[0], r[2]);
+    LANE_SWAP(permlane32_swap, r[1], r[3]);
+    LANE_SWAP(permlane16_swap, r[0], r[1]);
+    LANE_SWAP(permlane16_swap, r[2], r[3]);
 }
 
 // over the four lane groups of one column
-__device__ __forceinline__ float column_max(float v) {
-    v = fmaxf(v, __shfl_xor(v, 16));
-    return fmaxf(v, __shfl_xor(v, 32));
+template <typename F>
+__device__ __forceinline__ float over_groups(float v, F f) {
+    uint32_t a = __float_as_uint(v), b = a;
+    LANE_SWAP(permlane32_swap, a, b);
+    v = f(__uint_as_float(a), __uint_as_float(b));
+    a = b = __float_as_uint(v);
+    LANE_SWAP(permlane16_swap, a, b);
+    return f(__uint_as_float(a), __uint_as_float(b));
 }
-__device__ __forceinline__ float column_sum(float v) {
-    v += __shfl_xor(v, 16);
-    return v + __shfl_xor(v, 32);
-}
+__device__ __forceinline__ float column_max(float v) { return over_groups(v, [](float a, float b) { return fmaxf(a, b); }); }
+__device__ __forceinline__ float column_sum(float v) { return over_groups(v, [](float a, float b) { return a + b; }); }
 
 template <int NB> struct halves { _Float16 v[NB]; };
 template <bool B> struct flag { static constexpr bool value = B; };
@@ -189,36 +164,56 @@ template <int N> __device__ __forceinline__ float row_ror(float v) { return dpp_
 //
 // P16: pages of whole sixteens of rows, so that a load's 16 positions are on one page, found by scalar loads.
 template <int NB, int RT, bool NARROW, bool P16>
-__global__ __launch_bounds__(SPLIT_WG, 2) void paged_split_kernel(const paged_attn A) {
+__global__ __launch_bounds__(SPLIT_WG, RT == 2 ? 2 : 3) void paged_split_kernel(const paged_attn args) {
     constexpr int D = NB * 32, COLS = NARROW ? (NB == 2 ? 8 : 4) : 16, ROWS = COLS * RT;
-    constexpr int LOADS = NB == 2 ? 2 : 4;            // 16-byte loads a lane of a step's K or V
-    constexpr int SROW = STEP + 8;                    // scales of a block over a step's positions
+    constexpr int LOADS = NB == 2 ? 1 : 2;            // 16-byte loads a lane of a step's K or V
+    constexpr int SROW = STEP + 4;                    // scales of a block over a step's positions
     static_assert(!NARROW || RT == 1, "one tile");
     __shared__ __align__(16) uint8_t s_v[SPLIT_WG / WAVE][STEP * NB * 16];
-    __shared__ __align__(16) _Float16 s_kd[SPLIT_WG / WAVE][NB * SROW], s_vd[SPLIT_WG / WAVE][NB * SROW];
+    __shared__ __align__(16) _Float16 s_d[SPLIT_WG / WAVE][2][NB * SROW];
+    const paged_attn & A = kernargs_prefetched(args);
     const int lane = threadIdx.x % WAVE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
     const int col = lane % 16, c = lane / 16;         // the lane's column of a tile, its lane group
     const int own = NARROW ? min(col / COLS, NB - 1) : 0;                  // narrow: the column's block
     const bool spare = NARROW && col / COLS >= NB;
-    const int per_wg = (SPLIT_WG / WAVE) / A.team;
-    const int64_t team = (int64_t) blockIdx.x * per_wg + wave / A.team;   // (a team is 1, 2 or 4 waves)
+    const int team = (int) blockIdx.x * ((SPLIT_WG / WAVE) >> A.team_bits) + (wave >> A.team_bits);
     const int in_team = wave & (A.team - 1);
     const code_bits K;
 
-    int64_t none = 0;
-    const plan P = make_plan(A, ROWS, -1, none);
-    if (team >= P.teams) return;
-    int64_t u = P.begin(team);
-    const int64_t end = P.begin(team + 1);
-    if (u >= end) return;
-    int64_t begin = 0;
-    int seq = uniform(find_unit(A, ROWS, u, begin));
-    u -= begin;                                       // within the sequence
-    int64_t left = end - begin - u;
+    // ---- the team's run: from unit u of sequence seq on, `left` units ----
+    plan P;
+    int seq = 0;
+    int64_t u = 0, left;
+    {
+        // sequences by lanes, 64 at a time; of few, one look is enough
+        int64_t n = lane < A.n_seqs ? seq_units(A, seq_of(A, lane), ROWS) : 0, up = wave_scan(n), all = from_lane(up, WAVE - 1);
+        for (int s0 = WAVE; s0 < A.n_seqs; s0 += WAVE) {
+            const int s = s0 + lane;
+            all += from_lane(wave_scan(s < A.n_seqs ? seq_units(A, seq_of(A, s), ROWS) : 0), WAVE - 1);
+        }
+        P.deal(all, A.teams);
+        if (team >= P.teams) return;
+        u = P.begin(team);
+        left = P.begin(team + 1) - u;
+        if (left <= 0) return;
+        int64_t before = 0;
+        uint64_t past = __ballot(up > u);
+        for (int s0 = WAVE; !past && s0 < A.n_seqs; s0 += WAVE) {
+            before = from_lane(up, WAVE - 1);
+            const int s = s0 + lane;
+            n = s < A.n_seqs ? seq_units(A, seq_of(A, s), ROWS) : 0;
+            up = before + wave_scan(n);
+            past = __ballot(up > u);
+            seq = s0;
+        }
+        const int l = past ? __builtin_ctzll(past) : 0;
+        seq += l;
+        u -= from_lane(up - n, l);
+    }
 
     while (left > 0 && seq < A.n_seqs) {
         const seq_info Q = seq_of(A, seq);
-        const int steps = max((Q.len + STEP - 1) / STEP, 1);
+        const int steps = steps_of(Q);
         const int tiles = (Q.n * A.group + ROWS - 1) / ROWS;
         if (u >= (int64_t) tiles * A.head_teams * steps) { seq++; u = 0; continue; }
         const int item = uniform(u < ((int64_t) 1 << 32) ? (int) ((uint32_t) u / (uint32_t) steps) : (int) (u / steps));
@@ -227,6 +222,76 @@ __global__ __launch_bounds__(SPLIT_WG, 2) void paged_split_kernel(const paged_at
         const int step1 = (int) min((int64_t) steps, step0 + left);
         u += step1 - step0;
         left -= step1 - step0;
+
+        // ---- a step's operands: the rows of its positions, their bytes and scales ----
+        const int32_t * table = A.pages + (int64_t) seq * A.pages_s;
+        const uint8_t * kq = A.kq + (int64_t) head * A.k_head * 16, * vq = A.vq + (int64_t) head * A.v_head * 16;
+        const _Float16 * kdp = (const _Float16 *) A.kd + (int64_t) head * A.k_head, * vdp = (const _Float16 *) A.vd + (int64_t) head * A.v_head;
+        // K and V: lane (col, c) loads block c of position 16 j + col (of two blocks, 16 (c / 2) + col and c % 2)
+        auto lane_of = [&](int j) { return NB == 2 ? 16 * (c >> 1) + col : 16 * j + col; };
+        const int blk = NB == 2 ? (c & 1) : min(c, NB - 1);
+        // scales: K's of position lane, V's of position lane - 32
+        const int dpos = lane % STEP;
+        const bool dv = lane >= STEP;
+        int page[2];                 // P16: of the step's two sixteens (scalars); else of position lane % 32
+        auto pages_of = [&](int step) {
+#pragma unroll
+            for (int j = 0; j < (P16 ? 2 : 1); j++) {
+                const int pos = step * STEP + (P16 ? 16 * j : dpos);
+                page[j] = pos < Q.len && step < step1 ? table[page_index(A, pos)] : -1;
+            }
+        };
+        int64_t krow[2], vrow[2];    // first block of a sixteen's rows, or of the lane's
+        bool there;                  // the lane's scales' position is in the cache
+        uint32_t missing_next;       // positions whose page is not there
+        auto locate = [&](int step) {
+            const int live = Q.len - step * STEP;        // positions of the step
+            uint32_t bad = 0;
+            there = dpos < live;
+#pragma unroll
+            for (int j = 0; j < (P16 ? 2 : 1); j++) {
+                const int p0 = step * STEP + (P16 ? 16 * j : dpos);
+                const bool ok = page[j] >= 0 && page[j] < A.n_pages;
+                const int off = p0 - page_index(A, p0) * A.page;
+                krow[j] = ok ? (int64_t) page[j] * A.k_page + (int64_t) off * A.k_pos : 0;
+                vrow[j] = ok ? (int64_t) page[j] * A.v_page + (int64_t) off * A.v_pos : 0;
+                if (P16) {
+                    if (!ok) bad |= 0xFFFFu << (16 * j);
+                } else {
+                    bad = (uint32_t) __ballot(there && !ok);
+                    there = there && ok;
+                }
+            }
+            if (P16) {
+                there = there && !((bad >> dpos) & 1);
+                if (live < STEP) bad &= (1u << max(live, 0)) - 1;
+            }
+            missing_next = bad;
+        };
+        auto bytes_of = [&](const uint8_t * base, const int64_t (&row)[2], int64_t per_pos, int j) -> const uint8_t * {
+            if (!P16) return base + (__shfl(row[0], lane_of(j)) + blk) * 16;
+            int64_t r = row[j];
+            if (NB == 2) r += (c >> 1) * (row[1] - r);
+            return base + r * 16 + (uint32_t) ((col * (int) per_pos + blk) * 16);
+        };
+        auto scales_of = [&](const _Float16 * base, const int64_t (&row)[2], int64_t per_pos) {
+            if (!P16) return base + row[0];
+            return base + row[0] + (c & 1) * (row[1] - row[0]) + col * (int) per_pos;
+        };
+        u4 kraw[LOADS], vraw[LOADS];
+        halves<NB> sd;
+        auto load_v = [&]() {
+#pragma unroll
+            for (int j = 0; j < LOADS; j++) vraw[j] = *(const u4 *) bytes_of(vq, vrow, A.v_pos, j);
+            const _Float16 * p = dv ? scales_of(vdp, vrow, A.v_pos) : scales_of(kdp, krow, A.k_pos);
+#pragma unroll
+            for (int b = 0; b < NB; b++) sd.v[b] = p[b];
+        };
+        auto load_k = [&]() {
+#pragma unroll
+            for (int j = 0; j < LOADS; j++) kraw[j] = *(const u4 *) bytes_of(kq, krow, A.k_pos, j);
+        };
+        pages_of(step0);
 
         // ---- the rows: two halves of each value, scaled so that a row's largest is near 2^14 ----
         h8 qh[RT][NB], ql[RT][NB];
@@ -256,23 +321,31 @@ __global__ __launch_bounds__(SPLIT_WG, 2) void paged_split_kernel(const paged_at
 #pragma unroll
                 for (int k = 0; k < 8; k++) big = fmaxf(big, fabsf(v[k]));
             }
+            if (t == 0) {
+                // (behind the queries' loads)
+                locate(step0);
+                load_k();
+                load_v();
+                pages_of(step0 + 1);
+            }
             if (NARROW) {
                 big = fmaxf(big, row_ror<8>(big));
                 if (NB > 2) big = fmaxf(big, row_ror<4>(big));
             }
             big = column_max(big);
             const int e = big > 0.0f && big < INFINITY ? 14 - __builtin_amdgcn_frexp_expf(big) : 0;
+            const float sign = A.scale < 0.0f ? -1.0f : 1.0f;       // the factor of the sums is not negative
 #pragma unroll
             for (int b = 0; b < NB; b++) {
                 if (!NARROW) values(b, v);
 #pragma unroll
                 for (int k = 0; k < 8; k++) {
-                    const float x = NARROW && b != own ? 0.0f : __builtin_amdgcn_ldexpf(v[k], e);
+                    const float x = NARROW && b != own ? 0.0f : __builtin_amdgcn_ldexpf(v[k] * sign, e);
                     qh[t][b][k] = (_Float16) x;
                     ql[t][b][k] = (_Float16) (x - (float) qh[t][b][k]);
                 }
             }
-            fac[t] = A.scale * LOG2E * __builtin_amdgcn_ldexpf(1.0f, -e);
+            fac[t] = fabsf(A.scale) * LOG2E * __builtin_amdgcn_ldexpf(1.0f, -e);
             m[t] = M_NONE;
             l[t] = 0.0f;
 #pragma unroll
@@ -282,95 +355,18 @@ __global__ __launch_bounds__(SPLIT_WG, 2) void paged_split_kernel(const paged_at
         int shift = 38;
         const int sure = Q.last - (Q.n - 1) + tile * ROWS / A.group;        // positions up to here are seen by all rows
 
-        // ---- a step's operands: the rows of its positions, their bytes and scales ----
-        const int32_t * table = A.pages + (int64_t) seq * A.pages_s;
-        const uint8_t * kq = A.kq + (int64_t) head * A.k_head * 16, * vq = A.vq + (int64_t) head * A.v_head * 16;
-        const _Float16 * kdp = (const _Float16 *) A.kd + (int64_t) head * A.k_head, * vdp = (const _Float16 *) A.vd + (int64_t) head * A.v_head;
-        auto lane_of = [&](int j) { return NB == 2 ? 32 * j + 16 * (c >> 1) + col : 16 * j + col; };
-        const int blk = NB == 2 ? (c & 1) : min(c, NB - 1);
-        // P16: pages of the step's four sixteens (scalars); else of the lane's position
-        int page[4];
-        auto pages_of = [&](int step) {
-#pragma unroll
-            for (int j = 0; j < (P16 ? 4 : 1); j++) {
-                const int pos = step * STEP + (P16 ? 16 * j : lane);
-                page[j] = pos < Q.len && step < step1 ? table[page_index(A, pos)] : -1;
-            }
-        };
-        int64_t krow[P16 ? 4 : 1], vrow[P16 ? 4 : 1];    // first block of a sixteen's rows, or of the lane's
-        bool there;                                      // the lane's position is in the cache
-        uint64_t missing_next;                           // positions whose page is not there
-        auto locate = [&](int step) {
-            const int pos = step * STEP + lane;
-            uint64_t bad = 0;
-            there = pos < Q.len;
-#pragma unroll
-            for (int j = 0; j < (P16 ? 4 : 1); j++) {
-                const int p0 = step * STEP + (P16 ? 16 * j : lane);
-                const bool ok = page[j] >= 0 && page[j] < A.n_pages;
-                const int off = p0 - page_index(A, p0) * A.page;
-                krow[j] = ok ? (int64_t) page[j] * A.k_page + (int64_t) off * A.k_pos : 0;
-                vrow[j] = ok ? (int64_t) page[j] * A.v_page + (int64_t) off * A.v_pos : 0;
-                if (P16) {
-                    if (!ok) bad |= 0xFFFFull << (16 * j);
-                } else {
-                    bad = __ballot(there && !ok);
-                    there = there && ok;
-                }
-            }
-            if (P16) {
-                there = there && !((bad >> lane) & 1);
-                bad &= Q.len - step * STEP >= STEP ? ~0ull : (1ull << max(Q.len - step * STEP, 0)) - 1;
-            }
-            missing_next = bad;
-        };
-        // the 16 bytes of load j, and the lane's own position's first block
-        auto bytes_of = [&](const uint8_t * base, const int64_t * row, int64_t per_pos, int j) -> const uint8_t * {
-            if (!P16) return base + (__shfl(row[0], lane_of(j)) + blk) * 16;
-            int64_t r = row[NB == 2 ? 2 * j : j];
-            if (NB == 2) r += (c >> 1) * (row[2 * j + 1] - r);
-            return base + r * 16 + (uint32_t) ((col * (int) per_pos + blk) * 16);
-        };
-        auto scales_of = [&](const _Float16 * base, const int64_t * row, int64_t per_pos) {
-            if (!P16) return base + row[0];
-            const int64_t r = row[0] + (c & 1) * (row[1] - row[0]), r2 = row[2] + (c & 1) * (row[3] - row[2]);
-            return base + r + (c >> 1) * (r2 - r) + col * (int) per_pos;
-        };
-        u4 kraw[LOADS], vraw[LOADS];
-        halves<NB> kd, vd;
-        auto load_v = [&]() {
-#pragma unroll
-            for (int j = 0; j < LOADS; j++) vraw[j] = *(const u4 *) bytes_of(vq, vrow, A.v_pos, j);
-            const _Float16 * kp = scales_of(kdp, krow, A.k_pos), * vp = scales_of(vdp, vrow, A.v_pos);
-#pragma unroll
-            for (int b = 0; b < NB; b++) {
-                kd.v[b] = kp[b];
-                vd.v[b] = vp[b];
-            }
-        };
-        auto load_k = [&]() {
-#pragma unroll
-            for (int j = 0; j < LOADS; j++) kraw[j] = *(const u4 *) bytes_of(kq, krow, A.k_pos, j);
-        };
-        pages_of(step0);
-        locate(step0);
-        load_k();
-        load_v();
-        pages_of(step0 + 1);
-
         for (int step = step0; step < step1; step++) {
             const bool more = step + 1 < step1;
-            const uint64_t missing = missing_next;
+            const uint32_t missing = missing_next;
             // ---- V and the scales into LDS, the next ones on their way ----
 #pragma unroll
             for (int j = 0; j < LOADS; j++) *(u4 *) &s_v[wave][(lane_of(j) * NB + blk) * 16] = vraw[j];
             float dmax = 0.0f;
 #pragma unroll
             for (int b = 0; b < NB; b++) {
-                s_kd[wave][b * SROW + lane] = kd.v[b];
-                if (!there) vd.v[b] = 0;
-                s_vd[wave][b * SROW + lane] = vd.v[b];
-                dmax = fmaxf(dmax, fabsf((float) vd.v[b]));
+                if (!there) sd.v[b] = 0;
+                s_d[wave][dv][b * SROW + dpos] = sd.v[b];
+                if (dv) dmax = fmaxf(dmax, fabsf((float) sd.v[b]));
             }
             if (more) {
                 locate(step + 1);
@@ -378,15 +374,14 @@ __global__ __launch_bounds__(SPLIT_WG, 2) void paged_split_kernel(const paged_at
             }
 
             // ---- scores ----
-            f4 s[RT][4];
+            f4 s[RT][2];
 #pragma unroll
             for (int j = 0; j < LOADS; j++) {
-                __builtin_amdgcn_sched_barrier(0);
                 uint32_t r[4] = { kraw[j].x, kraw[j].y, kraw[j].z, kraw[j].w };
                 transpose4(r);
 #pragma unroll
-                for (int half = 0; half < 4 / LOADS; half++) {
-                    const int t = 4 / LOADS * j + half;
+                for (int half = 0; half < 2 / LOADS; half++) {
+                    const int t = 2 / LOADS * j + half;
                     f4 acc[RT];
 #pragma unroll
                     for (int b = 0; b < NB; b++) {
@@ -401,7 +396,7 @@ __global__ __launch_bounds__(SPLIT_WG, 2) void paged_split_kernel(const paged_at
                             acc[x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, ql[x][b], acc[x], 0, 0, 0);
                         }
                         if (NARROW && b < NB - 1) continue;
-                        const uint2 d = *(const uint2 *) &s_kd[wave][(NARROW ? own : b) * SROW + 16 * t + 4 * c];
+                        const uint2 d = *(const uint2 *) &s_d[wave][0][(NARROW ? own : b) * SROW + 16 * t + 4 * c];
                         const uint32_t w[2] = { d.x, d.y };
 #pragma unroll
                         for (int x = 0; x < RT; x++) {
@@ -441,13 +436,12 @@ __global__ __launch_bounds__(SPLIT_WG, 2) void paged_split_kernel(const paged_at
                 hidden[x] = 0;
                 if (edge) {
 #pragma unroll
-                    for (int t = 0; t < 4; t++) {
+                    for (int t = 0; t < 2; t++) {
 #pragma unroll
                         for (int i = 0; i < 4; i++) {
                             const int k = 16 * t + 4 * c + i;
                             if (step * STEP + k > lim[x] || ((missing >> k) & 1)) {
-                                // (fac may be negative or 0)
-                                s[x][t][i] = 0.0f;
+                                s[x][t][i] = -INFINITY;
                                 hidden[x] |= 1u << (4 * t + i);
                             }
                         }
@@ -455,15 +449,11 @@ __global__ __launch_bounds__(SPLIT_WG, 2) void paged_split_kernel(const paged_at
                 }
                 float top = -INFINITY;
 #pragma unroll
-                for (int t = 0; t < 4; t++) {
+                for (int t = 0; t < 2; t++) {
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        s[x][t][i] *= fac[x];
-                        if (edge && ((hidden[x] >> (4 * t + i)) & 1)) s[x][t][i] = -INFINITY;
-                        top = fmaxf(top, s[x][t][i]);
-                    }
+                    for (int i = 0; i < 4; i++) top = fmaxf(top, s[x][t][i]);
                 }
-                top = column_max(top);
+                top = column_max(top) * fac[x];
                 if (__any(top > m[x])) {
                     const float now = fmaxf(m[x], top), keep = exp2_hw(m[x] - now);
                     m[x] = now;
@@ -471,60 +461,60 @@ __global__ __launch_bounds__(SPLIT_WG, 2) void paged_split_kernel(const paged_at
 #pragma unroll
                     for (int b = 0; b < NB; b++) { o[x][b][0] *= keep; o[x][b][1] *= keep; }
                 }
-                const float at = m[x] - (float) shift;
-                float sum = 0.0f;
+                const float at = (float) shift - m[x];
 #pragma unroll
-                for (int t = 0; t < 4; t++) {
+                for (int t = 0; t < 2; t++) {
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        s[x][t][i] = exp2_hw(s[x][t][i] - at);
-                        sum += s[x][t][i];
+                    for (int i = 0; i < 4; i++) s[x][t][i] = exp2_hw(fmaf(s[x][t][i], fac[x], at));
+                }
+                if (edge) {
+#pragma unroll
+                    for (int t = 0; t < 2; t++) {
+#pragma unroll
+                        for (int i = 0; i < 4; i++) if ((hidden[x] >> (4 * t + i)) & 1) s[x][t][i] = 0.0f;
                     }
                 }
-                l[x] += sum;
+                l[x] += ((s[x][0][0] + s[x][0][1]) + (s[x][0][2] + s[x][0][3])) + ((s[x][1][0] + s[x][1][1]) + (s[x][1][2] + s[x][1][3]));
             }
 
-            // ---- o += p d (codes - 8), 32 positions of a block at a time ----
-            // lane (col, c) reads the transposed codes of row 16 (col / 4) + 4 c + col % 4
-            const uint8_t * vrow16 = &s_v[wave][(16 * (col >> 2) + 4 * c + (col & 3)) * NB * 16];
+            // ---- o += p d (codes - 8), a block at a time ----
+            // The transposing read takes 16 rows of 8 bytes from a lane group: its 8 positions' first halves of a
+            // block, then their second; register h is half h's column of the lane at those positions.
+            const uint8_t * vrow16 = &s_v[wave][(16 * ((col >> 2) & 1) + 4 * c + (col & 3)) * NB * 16 + (col >> 3) * 8];
             auto products = [&](auto at_edge) {
                 constexpr bool EDGE = decltype(at_edge)::value;
+                h8 ph[RT], pl[RT];
+                auto weights = [&](int b) {
+                    const uint2 d0 = *(const uint2 *) &s_d[wave][1][b * SROW + 4 * c], d1 = *(const uint2 *) &s_d[wave][1][b * SROW + 16 + 4 * c];
+                    const uint32_t w[4] = { d0.x, d0.y, d1.x, d1.y };
 #pragma unroll
-                for (int k = 0; k < 2; k++) {
-                    h8 ph[RT], pl[RT];
-                    auto weights = [&](int b) {
-                        const uint2 d0 = *(const uint2 *) &s_vd[wave][b * SROW + 32 * k + 4 * c], d1 = *(const uint2 *) &s_vd[wave][b * SROW + 32 * k + 16 + 4 * c];
-                        const uint32_t w[4] = { d0.x, d0.y, d1.x, d1.y };
+                    for (int x = 0; x < RT; x++) {
 #pragma unroll
-                        for (int x = 0; x < RT; x++) {
+                        for (int i = 0; i < 4; i++) {
 #pragma unroll
-                            for (int i = 0; i < 4; i++) {
-#pragma unroll
-                                for (int t = 0; t < 2; t++) {
-                                    const float p = s[x][2 * k + t][i];
-                                    float d = half_at(w, 4 * t + i);
-                                    if (EDGE) d = (hidden[x] >> (4 * (2 * k + t) + i)) & 1 ? 0.0f : d;
-                                    const _Float16 hi = (_Float16) fmaf(p, d, 0.0f);
-                                    ph[x][2 * i + t] = hi;
-                                    pl[x][2 * i + t] = (_Float16) fmaf(p, d, -(float) hi);
-                                }
+                            for (int t = 0; t < 2; t++) {
+                                const float p = s[x][t][i];
+                                float d = half_at(w, 4 * t + i);
+                                if (EDGE) d = (hidden[x] >> (4 * t + i)) & 1 ? 0.0f : d;
+                                const _Float16 hi = (_Float16) fmaf(p, d, 0.0f);
+                                ph[x][2 * i + t] = hi;
+                                pl[x][2 * i + t] = (_Float16) fmaf(p, d, -(float) hi);
                             }
                         }
-                    };
-                    if (NARROW) weights(own);
+                    }
+                };
+                if (NARROW) weights(own);
 #pragma unroll
-                    for (int b = 0; b < NB; b++) {
-                        __builtin_amdgcn_sched_barrier(0);
-                        if (!NARROW) weights(b);
+                for (int b = 0; b < NB; b++) {
+                    if (!NARROW) weights(b);
+                    const i2 codes = __builtin_amdgcn_ds_read_tr4_b64_v2i32((__attribute__((address_space(3))) i2 *) (vrow16 + b * 16));
 #pragma unroll
-                        for (int h = 0; h < 2; h++) {
-                            const i2 codes = __builtin_amdgcn_ds_read_tr4_b64_v2i32((__attribute__((address_space(3))) i2 *) (vrow16 + b * 16 + h * 8));
-                            const h8 a = signed_of(codes[k], K);
+                    for (int h = 0; h < 2; h++) {
+                        const h8 a = signed_of(codes[h], K);
 #pragma unroll
-                            for (int x = 0; x < RT; x++) {
-                                o[x][b][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, ph[x], o[x][b][h], 0, 0, 0);
-                                o[x][b][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, pl[x], o[x][b][h], 0, 0, 0);
-                            }
+                        for (int x = 0; x < RT; x++) {
+                            o[x][b][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, ph[x], o[x][b][h], 0, 0, 0);
+                            o[x][b][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, pl[x], o[x][b][h], 0, 0, 0);
                         }
                     }
                 }
@@ -535,7 +525,7 @@ __global__ __launch_bounds__(SPLIT_WG, 2) void paged_split_kernel(const paged_at
 
         // ---- the rows' results, or this run's part of them ----
         const bool whole = step0 == 0 && step1 == steps;
-        const int64_t slot = ((team * 2 + (step0 == 0)) * A.team + in_team) * ROWS;
+        const int64_t slot = (((int64_t) team * 2 + (step0 == 0)) * A.team + in_team) * ROWS;
 #pragma unroll
         for (int x = 0; x < RT; x++) {
             const int at_row = x * 16 + (NARROW ? col % COLS : col), row = tile * ROWS + at_row;
@@ -564,29 +554,39 @@ __global__ __launch_bounds__(SPLIT_WG, 2) void paged_split_kernel(const paged_at
 
 // Rows whose steps several teams took: their parts joined, a workgroup a row, D / 4 threads a part.
 template <int NB, int ROWS>
-__global__ __launch_bounds__(256) void paged_join_kernel(const paged_attn A) {
+__global__ __launch_bounds__(256) void paged_join_kernel(const paged_attn args) {
+    const paged_attn & A = kernargs_prefetched(args);
     constexpr int D = NB * 32, PER = D / 4, GROUPS = 256 / PER;
     __shared__ float4 s_o[GROUPS][PER];
     __shared__ float2 s_ml[GROUPS];
     const int token = blockIdx.x, head = blockIdx.y, t = threadIdx.x, lane = t % WAVE;
-    // the token's sequence
+    // the token's sequence, and the units before it
     int seq = -1;
-    for (int s0 = 0; s0 < A.n_seqs && seq < 0; s0 += WAVE) {
+    int64_t all = 0, begin = 0;
+    for (int s0 = 0; s0 < A.n_seqs; s0 += WAVE) {
         const int s = s0 + lane;
         bool mine = false;
+        int64_t n = 0;
         if (s < A.n_seqs) {
             const seq_info q = seq_of(A, s);
             mine = token >= q.first && token < q.first + q.n;
+            n = seq_units(A, q, ROWS);
         }
         const uint64_t b = __ballot(mine);
-        if (b) seq = s0 + __builtin_ctzll(b);
+        const int64_t up = wave_scan(n);
+        if (b && seq < 0) {
+            const int l = __builtin_ctzll(b);
+            seq = s0 + l;
+            begin = all + from_lane(up - n, l);
+        }
+        all += from_lane(up, WAVE - 1);
     }
     if (seq < 0) return;
     const seq_info Q = seq_of(A, seq);
-    int64_t begin = 0;
-    const plan P = make_plan(A, ROWS, seq, begin);
+    plan P;
+    P.deal(all, A.teams);
     const int kvh = head / A.group, row = (token - Q.first) * A.group + head - kvh * A.group;
-    const int tile = row / ROWS, steps = max((Q.len + STEP - 1) / STEP, 1);
+    const int tile = row / ROWS, steps = steps_of(Q);
     const int64_t a = begin + ((int64_t) tile * A.head_teams + kvh / A.team) * steps;
     const int64_t t0 = P.team_of(a), t1 = P.team_of(a + steps - 1);
     if (t0 == t1) return;                               // written whole
@@ -628,7 +628,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const paged_attn A) {
     *(float4 *) (A.out + ((int64_t) token * A.n_head + head) * D + 4 * t) = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
 }
 
-constexpr int SPLIT_WGS = 512;         // two workgroups of four waves a CU
+constexpr int SPLIT_WGS = 768;         // three workgroups of four waves a CU
 
 // rows of a tile: narrow, one or two of 16
 int split_rows(const paged_attn & A) {
@@ -666,6 +666,7 @@ int64_t paged_attn_scratch_bytes(const paged_attn & A) {
 void launch_paged_attn(paged_attn A, hipStream_t st) {
     if (A.n_tokens == 0 || A.n_seqs == 0 || A.n_head == 0) return;
     A.team = A.n_head_kv % 4 == 0 ? 4 : A.n_head_kv % 2 == 0 ? 2 : 1;
+    A.team_bits = A.team / 2;
     A.head_teams = A.n_head_kv / A.team;
     A.teams = SPLIT_WGS * (SPLIT_WG / WAVE) / A.team;
     // pos / page as a product: exact below 2^31 (the multiplier is rounded up, by less than 2^-31 of it)

@@ -430,7 +430,7 @@ struct paged_attn {
     float scale;
     void * scratch;                  // paged_attn_scratch_bytes
     // set by launch_paged_attn
-    int team, head_teams, teams, page_shift;
+    int team, team_bits, head_teams, teams, page_shift;
     uint32_t page_mul;
     float * part;
     float2 * part_ml;
