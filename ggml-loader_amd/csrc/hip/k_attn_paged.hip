@@ -158,14 +158,15 @@ template <int N> __device__ __forceinline__ float row_ror(float v) { return dpp_
 // Few rows a sequence: a wave takes steps of one KV head by itself.
 //
 // Wide: the 16 columns of a tile are 16 rows (query, head), RT tiles of them. Narrow, for up to 16 / NB rows (4 for
-// heads of 96): a column is a row and a block, B holds that block's values and zeros elsewhere, and one tile
-// of sums holds every block's: a lane scales its own block's and sums by neighbours, and forms p d for its own
-// block only, which serves all blocks' products (a quarter of the work where a KV head has four query heads).
+// heads of 96): a column is a row and a block. A lane takes its own block's sums of each product, scales them and
+// adds its neighbours', and forms p d for its own block only, which serves all blocks' products (a quarter of that
+// work where a KV head has four query heads).
 //
 // P16: pages of whole sixteens of rows, so that a load's 16 positions are on one page, found by scalar loads.
 template <int NB, int RT, bool NARROW, bool P16>
-__global__ __launch_bounds__(SPLIT_WG, RT == 2 ? 2 : 3) void paged_split_kernel(const paged_attn args) {
+__global__ __launch_bounds__(SPLIT_WG, NARROW ? 3 : 2) void paged_split_kernel(const paged_attn args) {
     constexpr int D = NB * 32, COLS = NARROW ? (NB == 2 ? 8 : 4) : 16, ROWS = COLS * RT;
+    constexpr int QB = NARROW ? 1 : NB;               // blocks of a column's values: narrow, its own
     constexpr int LOADS = NB == 2 ? 1 : 2;            // 16-byte loads a lane of a step's K or V
     constexpr int SROW = STEP + 4;                    // scales of a block over a step's positions
     static_assert(!NARROW || RT == 1, "one tile");
@@ -233,13 +234,17 @@ __global__ __launch_bounds__(SPLIT_WG, RT == 2 ? 2 : 3) void paged_split_kernel(
         // scales: K's of position lane, V's of position lane - 32
         const int dpos = lane % STEP;
         const bool dv = lane >= STEP;
-        int page[2];                 // P16: of the step's two sixteens (scalars); else of position lane % 32
-        auto pages_of = [&](int step) {
-#pragma unroll
-            for (int j = 0; j < (P16 ? 2 : 1); j++) {
-                const int pos = step * STEP + (P16 ? 16 * j : dpos);
-                page[j] = pos < Q.len && step < step1 ? table[page_index(A, pos)] : -1;
-            }
+        // Pages. P16: 64 table entries at a time in a register, one a lane; the next sixteen's place in the table and
+        // in its page go along as scalars. Else each lane looks up its scales' position, two steps ahead.
+        int held = 0, at_page = 0, at_row = 0, first_held = 0, page = -1;
+        const int sixteens = A.page >> 4, entries = (Q.len + A.page - 1) / A.page;
+        auto hold = [&](int from) {
+            first_held = from;
+            held = from + lane < entries ? table[from + lane] : -1;
+        };
+        auto page_of = [&](int step) {
+            const int pos = step * STEP + dpos;
+            page = pos < Q.len && step < step1 ? table[page_index(A, pos)] : -1;
         };
         int64_t krow[2], vrow[2];    // first block of a sixteen's rows, or of the lane's
         bool there;                  // the lane's scales' position is in the cache
@@ -248,23 +253,29 @@ __global__ __launch_bounds__(SPLIT_WG, RT == 2 ? 2 : 3) void paged_split_kernel(
             const int live = Q.len - step * STEP;        // positions of the step
             uint32_t bad = 0;
             there = dpos < live;
-#pragma unroll
-            for (int j = 0; j < (P16 ? 2 : 1); j++) {
-                const int p0 = step * STEP + (P16 ? 16 * j : dpos);
-                const bool ok = page[j] >= 0 && page[j] < A.n_pages;
-                const int off = p0 - page_index(A, p0) * A.page;
-                krow[j] = ok ? (int64_t) page[j] * A.k_page + (int64_t) off * A.k_pos : 0;
-                vrow[j] = ok ? (int64_t) page[j] * A.v_page + (int64_t) off * A.v_pos : 0;
-                if (P16) {
-                    if (!ok) bad |= 0xFFFFu << (16 * j);
-                } else {
-                    bad = (uint32_t) __ballot(there && !ok);
-                    there = there && ok;
-                }
-            }
             if (P16) {
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    if (at_page - first_held == WAVE) hold(at_page);
+                    const int id = __builtin_amdgcn_readlane(held, at_page - first_held);
+                    const bool ok = (uint32_t) id < (uint32_t) A.n_pages;
+                    if (!ok) bad |= 0xFFFFu << (16 * j);
+                    const uint32_t pg = ok ? id : 0, off = ok ? at_row : 0;
+                    krow[j] = (int64_t) ((uint64_t) pg * (uint32_t) A.k_page + (uint64_t) off * (uint32_t) A.k_pos);
+                    vrow[j] = (int64_t) ((uint64_t) pg * (uint32_t) A.v_page + (uint64_t) off * (uint32_t) A.v_pos);
+                    at_row += 16;
+                    if (at_row == A.page) { at_row = 0; at_page++; }
+                }
                 there = there && !((bad >> dpos) & 1);
                 if (live < STEP) bad &= (1u << max(live, 0)) - 1;
+            } else {
+                const int p0 = step * STEP + dpos;
+                const bool ok = page >= 0 && page < A.n_pages;
+                const int off = p0 - page_index(A, p0) * A.page;
+                krow[0] = ok ? (int64_t) page * A.k_page + (int64_t) off * A.k_pos : 0;
+                vrow[0] = ok ? (int64_t) page * A.v_page + (int64_t) off * A.v_pos : 0;
+                bad = (uint32_t) __ballot(there && !ok);
+                there = there && ok;
             }
             missing_next = bad;
         };
@@ -291,10 +302,17 @@ __global__ __launch_bounds__(SPLIT_WG, RT == 2 ? 2 : 3) void paged_split_kernel(
 #pragma unroll
             for (int j = 0; j < LOADS; j++) kraw[j] = *(const u4 *) bytes_of(kq, krow, A.k_pos, j);
         };
-        pages_of(step0);
+        if (P16) {
+            const int first = step0 * (STEP / 16);
+            at_page = uniform((int) ((uint32_t) first / (uint32_t) sixteens));
+            at_row = (first - at_page * sixteens) * 16;
+            hold(at_page);
+        } else {
+            page_of(step0);
+        }
 
         // ---- the rows: two halves of each value, scaled so that a row's largest is near 2^14 ----
-        h8 qh[RT][NB], ql[RT][NB];
+        h8 qh[RT][QB], ql[RT][QB];
         float fac[RT], m[RT], l[RT];
         int lim[RT];
         f4 o[RT][NB][2];
@@ -316,7 +334,7 @@ __global__ __launch_bounds__(SPLIT_WG, RT == 2 ? 2 : 3) void paged_split_kernel(
             // the row's largest value: of its own block in each column, narrow
             float v[8];
 #pragma unroll
-            for (int b = 0; b < (NARROW ? 1 : NB); b++) {
+            for (int b = 0; b < QB; b++) {
                 values(NARROW ? own : b, v);
 #pragma unroll
                 for (int k = 0; k < 8; k++) big = fmaxf(big, fabsf(v[k]));
@@ -326,7 +344,7 @@ __global__ __launch_bounds__(SPLIT_WG, RT == 2 ? 2 : 3) void paged_split_kernel(
                 locate(step0);
                 load_k();
                 load_v();
-                pages_of(step0 + 1);
+                if (!P16) page_of(step0 + 1);
             }
             if (NARROW) {
                 big = fmaxf(big, row_ror<8>(big));
@@ -336,11 +354,11 @@ __global__ __launch_bounds__(SPLIT_WG, RT == 2 ? 2 : 3) void paged_split_kernel(
             const int e = big > 0.0f && big < INFINITY ? 14 - __builtin_amdgcn_frexp_expf(big) : 0;
             const float sign = A.scale < 0.0f ? -1.0f : 1.0f;       // the factor of the sums is not negative
 #pragma unroll
-            for (int b = 0; b < NB; b++) {
+            for (int b = 0; b < QB; b++) {
                 if (!NARROW) values(b, v);
 #pragma unroll
                 for (int k = 0; k < 8; k++) {
-                    const float x = NARROW && b != own ? 0.0f : __builtin_amdgcn_ldexpf(v[k] * sign, e);
+                    const float x = __builtin_amdgcn_ldexpf(v[k] * sign, e);
                     qh[t][b][k] = (_Float16) x;
                     ql[t][b][k] = (_Float16) (x - (float) qh[t][b][k]);
                 }
@@ -382,27 +400,33 @@ __global__ __launch_bounds__(SPLIT_WG, RT == 2 ? 2 : 3) void paged_split_kernel(
 #pragma unroll
                 for (int half = 0; half < 2 / LOADS; half++) {
                     const int t = 2 / LOADS * j + half;
-                    f4 acc[RT];
+                    f4 mine = { 0, 0, 0, 0 };
 #pragma unroll
                     for (int b = 0; b < NB; b++) {
                         const h8 a = signed_of(r[half * 2 + b], K);
-                        if (!NARROW || b == 0) {
-#pragma unroll
-                            for (int x = 0; x < RT; x++) acc[x] = f4{ 0, 0, 0, 0 };
+                        uint32_t w[2];
+                        if (!NARROW) {
+                            const uint2 d = *(const uint2 *) &s_d[wave][0][b * SROW + 16 * t + 4 * c];
+                            w[0] = d.x;
+                            w[1] = d.y;
                         }
 #pragma unroll
                         for (int x = 0; x < RT; x++) {
-                            acc[x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, qh[x][b], acc[x], 0, 0, 0);
-                            acc[x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, ql[x][b], acc[x], 0, 0, 0);
+                            f4 acc = { 0, 0, 0, 0 };
+                            acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, qh[x][NARROW ? 0 : b], acc, 0, 0, 0);
+                            acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, ql[x][NARROW ? 0 : b], acc, 0, 0, 0);
+#pragma unroll
+                            for (int i = 0; i < 4; i++) {
+                                if (NARROW) mine[i] = b == own ? acc[i] : mine[i];
+                                else s[x][t][i] = fmaf(acc[i], half_at(w, i), b == 0 ? 0.0f : s[x][t][i]);
+                            }
                         }
-                        if (NARROW && b < NB - 1) continue;
-                        const uint2 d = *(const uint2 *) &s_d[wave][0][(NARROW ? own : b) * SROW + 16 * t + 4 * c];
+                    }
+                    if (NARROW) {
+                        const uint2 d = *(const uint2 *) &s_d[wave][0][own * SROW + 16 * t + 4 * c];
                         const uint32_t w[2] = { d.x, d.y };
 #pragma unroll
-                        for (int x = 0; x < RT; x++) {
-#pragma unroll
-                            for (int i = 0; i < 4; i++) s[x][t][i] = fmaf(acc[x][i], half_at(w, i), NARROW || b == 0 ? 0.0f : s[x][t][i]);
-                        }
+                        for (int i = 0; i < 4; i++) s[0][t][i] = fmaf(mine[i], half_at(w, i), 0.0f);
                     }
                     if (NARROW) {
                         // a spare column's sums are 0 times a scale: 0, or a NaN as that block's own column has it
@@ -415,7 +439,7 @@ __global__ __launch_bounds__(SPLIT_WG, RT == 2 ? 2 : 3) void paged_split_kernel(
                 }
             }
             if (more) load_k();
-            pages_of(step + 2);
+            if (!P16) page_of(step + 2);
             // the largest scale of V so far
             if (__any(dmax >= __builtin_amdgcn_ldexpf(1.0f, 15 - shift))) {
                 const float big = wave_max(dmax);
@@ -641,7 +665,7 @@ template <int NB, int RT, bool NARROW>
 void split(const paged_attn & A, hipStream_t st) {
     constexpr int ROWS = NARROW ? (NB == 2 ? 8 : 4) : 16 * RT;
     // a sixteen of positions on one page, its rows within 32-bit offsets
-    const int64_t reach = 16 * 16 * std::max(A.k_pos, A.v_pos);
+    const int64_t reach = std::max(16 * 16 * std::max(A.k_pos, A.v_pos), std::max(A.k_page, A.v_page));
     if (A.page % 16 == 0 && reach <= INT32_MAX) launch(paged_split_kernel<NB, RT, NARROW, true>, dim3(SPLIT_WGS), dim3(SPLIT_WG), 0, st, A);
     else launch(paged_split_kernel<NB, RT, NARROW, false>, dim3(SPLIT_WGS), dim3(SPLIT_WG), 0, st, A);
     launch(paged_join_kernel<NB, ROWS>, dim3(A.n_tokens, A.n_head), dim3(256), 0, st, A);
