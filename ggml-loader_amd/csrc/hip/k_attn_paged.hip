@@ -147,13 +147,32 @@ __device__ __forceinline__ float over_groups(float v, F f) {
 __device__ __forceinline__ float column_max(float v) { return over_groups(v, [](float a, float b) { return fmaxf(a, b); }); }
 __device__ __forceinline__ float column_sum(float v) { return over_groups(v, [](float a, float b) { return a + b; }); }
 
-template <int NB> struct halves { _Float16 v[NB]; };
+// the scales of a position's blocks, as loaded
+template <int NB> struct scales {
+    typedef uint32_t u1 __attribute__((aligned(2)));
+    typedef uint32_t u2 __attribute__((ext_vector_type(2), aligned(2)));
+    uint32_t w[2];
+    __device__ __forceinline__ void load(const _Float16 * p) {
+        if (NB == 4) {
+            const u2 v = *(const u2 *) p;
+            w[0] = v[0];
+            w[1] = v[1];
+        } else {
+            w[0] = *(const u1 *) p;
+            if (NB == 3) w[1] = ((const uint16_t *) p)[2];
+        }
+    }
+    __device__ __forceinline__ float at(int b) const { return (float) __builtin_bit_cast(h2, w[b / 2])[b % 2]; }
+};
 template <bool B> struct flag { static constexpr bool value = B; };
 
-__device__ __forceinline__ float half_at(const uint32_t * w, int k) { return (float) __builtin_bit_cast(h2, w[k / 2])[k % 2]; }
+// nothing in particular, for what is not used again
+template <typename T> __device__ __forceinline__ void forget(T & v) { asm volatile("" : "=v"(v)); }
 
-// the value of the lane n further in its row of 16, cyclically
-template <int N> __device__ __forceinline__ float row_ror(float v) { return dpp_f<0x120 + N>(v); }
+// the value of the lane N further in its row of 16, cyclically
+template <int N> __device__ __forceinline__ float row_ror(float v) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x120 + N, 0xF, 0xF, true));
+}
 
 // Few rows a sequence: a wave takes steps of one KV head by itself.
 //
@@ -168,10 +187,10 @@ __global__ __launch_bounds__(SPLIT_WG, NARROW ? 3 : 2) void paged_split_kernel(c
     constexpr int D = NB * 32, COLS = NARROW ? (NB == 2 ? 8 : 4) : 16, ROWS = COLS * RT;
     constexpr int QB = NARROW ? 1 : NB;               // blocks of a column's values: narrow, its own
     constexpr int LOADS = NB == 2 ? 1 : 2;            // 16-byte loads a lane of a step's K or V
-    constexpr int SROW = STEP + 4;                    // scales of a block over a step's positions
+    constexpr int SROW = STEP + 4;                    // scales of a block over a step's positions, in 32 bits
     static_assert(!NARROW || RT == 1, "one tile");
     __shared__ __align__(16) uint8_t s_v[SPLIT_WG / WAVE][STEP * NB * 16];
-    __shared__ __align__(16) _Float16 s_d[SPLIT_WG / WAVE][2][NB * SROW];
+    __shared__ __align__(16) float s_d[SPLIT_WG / WAVE][2][NB * SROW];
     const paged_attn & A = kernargs_prefetched(args);
     const int lane = threadIdx.x % WAVE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
     const int col = lane % 16, c = lane / 16;         // the lane's column of a tile, its lane group
@@ -227,17 +246,22 @@ __global__ __launch_bounds__(SPLIT_WG, NARROW ? 3 : 2) void paged_split_kernel(c
         // ---- a step's operands: the rows of its positions, their bytes and scales ----
         const int32_t * table = A.pages + (int64_t) seq * A.pages_s;
         const uint8_t * kq = A.kq + (int64_t) head * A.k_head * 16, * vq = A.vq + (int64_t) head * A.v_head * 16;
-        const _Float16 * kdp = (const _Float16 *) A.kd + (int64_t) head * A.k_head, * vdp = (const _Float16 *) A.vd + (int64_t) head * A.v_head;
         // K and V: lane (col, c) loads block c of position 16 j + col (of two blocks, 16 (c / 2) + col and c % 2)
         auto lane_of = [&](int j) { return NB == 2 ? 16 * (c >> 1) + col : 16 * j + col; };
         const int blk = NB == 2 ? (c & 1) : min(c, NB - 1);
         // scales: K's of position lane, V's of position lane - 32
         const int dpos = lane % STEP;
         const bool dv = lane >= STEP;
+        const _Float16 * dp = dv ? (const _Float16 *) A.vd + (int64_t) head * A.v_head : (const _Float16 *) A.kd + (int64_t) head * A.k_head;
+        const int64_t n_pages = A.n_pages, k_page = A.k_page, k_pos = A.k_pos, v_page = A.v_page, v_pos = A.v_pos;
+        const int rows_page = A.page;
+        // P16: a lane's place in a sixteen
+        const uint32_t k_off = (uint32_t) (col * (int) k_pos + blk) * 16, v_off = (uint32_t) (col * (int) v_pos + blk) * 16;
+        if (P16) dp += col * (int) (dv ? v_pos : k_pos);
         // Pages. P16: 64 table entries at a time in a register, one a lane; the next sixteen's place in the table and
         // in its page go along as scalars. Else each lane looks up its scales' position, two steps ahead.
         int held = 0, at_page = 0, at_row = 0, first_held = 0, page = -1;
-        const int sixteens = A.page >> 4, entries = (Q.len + A.page - 1) / A.page;
+        const int sixteens = rows_page >> 4, entries = (Q.len + rows_page - 1) / rows_page;
         auto hold = [&](int from) {
             first_held = from;
             held = from + lane < entries ? table[from + lane] : -1;
@@ -258,49 +282,52 @@ __global__ __launch_bounds__(SPLIT_WG, NARROW ? 3 : 2) void paged_split_kernel(c
                 for (int j = 0; j < 2; j++) {
                     if (at_page - first_held == WAVE) hold(at_page);
                     const int id = __builtin_amdgcn_readlane(held, at_page - first_held);
-                    const bool ok = (uint32_t) id < (uint32_t) A.n_pages;
+                    const bool ok = (uint32_t) id < (uint32_t) n_pages;
                     if (!ok) bad |= 0xFFFFu << (16 * j);
                     const uint32_t pg = ok ? id : 0, off = ok ? at_row : 0;
-                    krow[j] = (int64_t) ((uint64_t) pg * (uint32_t) A.k_page + (uint64_t) off * (uint32_t) A.k_pos);
-                    vrow[j] = (int64_t) ((uint64_t) pg * (uint32_t) A.v_page + (uint64_t) off * (uint32_t) A.v_pos);
+                    krow[j] = (int64_t) ((uint64_t) pg * (uint32_t) k_page + (uint64_t) off * (uint32_t) k_pos);
+                    vrow[j] = (int64_t) ((uint64_t) pg * (uint32_t) v_page + (uint64_t) off * (uint32_t) v_pos);
                     at_row += 16;
-                    if (at_row == A.page) { at_row = 0; at_page++; }
+                    if (at_row == rows_page) { at_row = 0; at_page++; }
                 }
                 there = there && !((bad >> dpos) & 1);
                 if (live < STEP) bad &= (1u << max(live, 0)) - 1;
             } else {
                 const int p0 = step * STEP + dpos;
-                const bool ok = page >= 0 && page < A.n_pages;
-                const int off = p0 - page_index(A, p0) * A.page;
-                krow[0] = ok ? (int64_t) page * A.k_page + (int64_t) off * A.k_pos : 0;
-                vrow[0] = ok ? (int64_t) page * A.v_page + (int64_t) off * A.v_pos : 0;
+                const bool ok = page >= 0 && page < n_pages;
+                const int off = p0 - page_index(A, p0) * rows_page;
+                krow[0] = ok ? (int64_t) page * k_page + (int64_t) off * k_pos : 0;
+                vrow[0] = ok ? (int64_t) page * v_page + (int64_t) off * v_pos : 0;
                 bad = (uint32_t) __ballot(there && !ok);
                 there = there && ok;
             }
             missing_next = bad;
         };
-        auto bytes_of = [&](const uint8_t * base, const int64_t (&row)[2], int64_t per_pos, int j) -> const uint8_t * {
+        auto bytes_of = [&](const uint8_t * base, const int64_t (&row)[2], uint32_t off, int j) -> const uint8_t * {
             if (!P16) return base + (__shfl(row[0], lane_of(j)) + blk) * 16;
-            int64_t r = row[j];
-            if (NB == 2) r += (c >> 1) * (row[1] - r);
-            return base + r * 16 + (uint32_t) ((col * (int) per_pos + blk) * 16);
-        };
-        auto scales_of = [&](const _Float16 * base, const int64_t (&row)[2], int64_t per_pos) {
-            if (!P16) return base + row[0];
-            return base + row[0] + (c & 1) * (row[1] - row[0]) + col * (int) per_pos;
+            if (NB == 2) {
+                const int64_t r0 = uniform(row[0]), r1 = uniform(row[1]);
+                return base + ((c >> 1) ? r1 : r0) * 16 + off;
+            }
+            return base + row[j] * 16 + off;
         };
         u4 kraw[LOADS], vraw[LOADS];
-        halves<NB> sd;
+        scales<NB> sd;
         auto load_v = [&]() {
 #pragma unroll
-            for (int j = 0; j < LOADS; j++) vraw[j] = *(const u4 *) bytes_of(vq, vrow, A.v_pos, j);
-            const _Float16 * p = dv ? scales_of(vdp, vrow, A.v_pos) : scales_of(kdp, krow, A.k_pos);
-#pragma unroll
-            for (int b = 0; b < NB; b++) sd.v[b] = p[b];
+            for (int j = 0; j < LOADS; j++) vraw[j] = *(const u4 *) bytes_of(vq, vrow, v_off, j);
+            if (P16) {
+                // (rows of scales are within 32 bits)
+                const uint32_t k0 = uniform((int) krow[0]), k1 = uniform((int) krow[1]), v0 = uniform((int) vrow[0]), v1 = uniform((int) vrow[1]);
+                const uint32_t k = (c & 1) ? k1 : k0, v = (c & 1) ? v1 : v0;
+                sd.load(dp + (dv ? v : k));
+            } else {
+                sd.load(dp + (dv ? vrow[0] : krow[0]));
+            }
         };
         auto load_k = [&]() {
 #pragma unroll
-            for (int j = 0; j < LOADS; j++) kraw[j] = *(const u4 *) bytes_of(kq, krow, A.k_pos, j);
+            for (int j = 0; j < LOADS; j++) kraw[j] = *(const u4 *) bytes_of(kq, krow, k_off, j);
         };
         if (P16) {
             const int first = step0 * (STEP / 16);
@@ -382,13 +409,19 @@ __global__ __launch_bounds__(SPLIT_WG, NARROW ? 3 : 2) void paged_split_kernel(c
             float dmax = 0.0f;
 #pragma unroll
             for (int b = 0; b < NB; b++) {
-                if (!there) sd.v[b] = 0;
-                s_d[wave][dv][b * SROW + dpos] = sd.v[b];
-                if (dv) dmax = fmaxf(dmax, fabsf((float) sd.v[b]));
+                const float d = there ? sd.at(b) : 0.0f;
+                s_d[wave][dv][b * SROW + dpos] = d;
+                dmax = fmaxf(dmax, fabsf(d));
             }
+            if (!dv) dmax = 0.0f;
             if (more) {
                 locate(step + 1);
                 load_v();
+            } else {
+#pragma unroll
+                for (int j = 0; j < LOADS; j++) forget(vraw[j]);
+                forget(sd.w[0]);
+                forget(sd.w[1]);
             }
 
             // ---- scores ----
@@ -404,12 +437,8 @@ __global__ __launch_bounds__(SPLIT_WG, NARROW ? 3 : 2) void paged_split_kernel(c
 #pragma unroll
                     for (int b = 0; b < NB; b++) {
                         const h8 a = signed_of(r[half * 2 + b], K);
-                        uint32_t w[2];
-                        if (!NARROW) {
-                            const uint2 d = *(const uint2 *) &s_d[wave][0][b * SROW + 16 * t + 4 * c];
-                            w[0] = d.x;
-                            w[1] = d.y;
-                        }
+                        f4 d;
+                        if (!NARROW) d = *(const f4 *) &s_d[wave][0][b * SROW + 16 * t + 4 * c];
 #pragma unroll
                         for (int x = 0; x < RT; x++) {
                             f4 acc = { 0, 0, 0, 0 };
@@ -417,19 +446,17 @@ __global__ __launch_bounds__(SPLIT_WG, NARROW ? 3 : 2) void paged_split_kernel(c
                             acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, ql[x][NARROW ? 0 : b], acc, 0, 0, 0);
 #pragma unroll
                             for (int i = 0; i < 4; i++) {
-                                if (NARROW) mine[i] = b == own ? acc[i] : mine[i];
-                                else s[x][t][i] = fmaf(acc[i], half_at(w, i), b == 0 ? 0.0f : s[x][t][i]);
+                                if (NARROW) mine[i] = b == 0 || b == own ? acc[i] : mine[i];
+                                else s[x][t][i] = b == 0 ? acc[i] * d[i] : fmaf(acc[i], d[i], s[x][t][i]);
                             }
                         }
                     }
                     if (NARROW) {
-                        const uint2 d = *(const uint2 *) &s_d[wave][0][own * SROW + 16 * t + 4 * c];
-                        const uint32_t w[2] = { d.x, d.y };
+                        const f4 d = *(const f4 *) &s_d[wave][0][own * SROW + 16 * t + 4 * c];
 #pragma unroll
-                        for (int i = 0; i < 4; i++) s[0][t][i] = fmaf(mine[i], half_at(w, i), 0.0f);
+                        for (int i = 0; i < 4; i++) s[0][t][i] = spare ? 0.0f : mine[i] * d[i];
                     }
                     if (NARROW) {
-                        // a spare column's sums are 0 times a scale: 0, or a NaN as that block's own column has it
 #pragma unroll
                         for (int i = 0; i < 4; i++) {
                             s[0][t][i] += row_ror<8>(s[0][t][i]);
@@ -438,7 +465,12 @@ __global__ __launch_bounds__(SPLIT_WG, NARROW ? 3 : 2) void paged_split_kernel(c
                     }
                 }
             }
-            if (more) load_k();
+            if (more) {
+                load_k();
+            } else {
+#pragma unroll
+                for (int j = 0; j < LOADS; j++) forget(kraw[j]);
+            }
             if (!P16) page_of(step + 2);
             // the largest scale of V so far
             if (__any(dmax >= __builtin_amdgcn_ldexpf(1.0f, 15 - shift))) {
@@ -509,20 +541,19 @@ __global__ __launch_bounds__(SPLIT_WG, NARROW ? 3 : 2) void paged_split_kernel(c
                 constexpr bool EDGE = decltype(at_edge)::value;
                 h8 ph[RT], pl[RT];
                 auto weights = [&](int b) {
-                    const uint2 d0 = *(const uint2 *) &s_d[wave][1][b * SROW + 4 * c], d1 = *(const uint2 *) &s_d[wave][1][b * SROW + 16 + 4 * c];
-                    const uint32_t w[4] = { d0.x, d0.y, d1.x, d1.y };
+                    const f4 d0 = *(const f4 *) &s_d[wave][1][b * SROW + 4 * c], d1 = *(const f4 *) &s_d[wave][1][b * SROW + 16 + 4 * c];
 #pragma unroll
                     for (int x = 0; x < RT; x++) {
 #pragma unroll
                         for (int i = 0; i < 4; i++) {
 #pragma unroll
                             for (int t = 0; t < 2; t++) {
-                                const float p = s[x][t][i];
-                                float d = half_at(w, 4 * t + i);
+                                float d = t ? d1[i] : d0[i];
                                 if (EDGE) d = (hidden[x] >> (4 * t + i)) & 1 ? 0.0f : d;
-                                const _Float16 hi = (_Float16) fmaf(p, d, 0.0f);
-                                ph[x][2 * i + t] = hi;
-                                pl[x][2 * i + t] = (_Float16) fmaf(p, d, -(float) hi);
+                                // (one product for both halves: see as_f32)
+                                const float w = as_f32(s[x][t][i] * d);
+                                ph[x][2 * i + t] = (_Float16) w;
+                                pl[x][2 * i + t] = (_Float16) fmaf(s[x][t][i], d, -(float) ph[x][2 * i + t]);
                             }
                         }
                     }
@@ -664,8 +695,8 @@ int split_rows(const paged_attn & A) {
 template <int NB, int RT, bool NARROW>
 void split(const paged_attn & A, hipStream_t st) {
     constexpr int ROWS = NARROW ? (NB == 2 ? 8 : 4) : 16 * RT;
-    // a sixteen of positions on one page, its rows within 32-bit offsets
-    const int64_t reach = std::max(16 * 16 * std::max(A.k_pos, A.v_pos), std::max(A.k_page, A.v_page));
+    // a sixteen of positions on one page, its rows within 32-bit offsets, and a row's number within 32 bits
+    const int64_t reach = std::max(std::max(16 * 16 * std::max(A.k_pos, A.v_pos), std::max(A.k_page, A.v_page)), (A.n_pages * std::max(A.k_page, A.v_page) + 1) / 2);
     if (A.page % 16 == 0 && reach <= INT32_MAX) launch(paged_split_kernel<NB, RT, NARROW, true>, dim3(SPLIT_WGS), dim3(SPLIT_WG), 0, st, A);
     else launch(paged_split_kernel<NB, RT, NARROW, false>, dim3(SPLIT_WGS), dim3(SPLIT_WG), 0, st, A);
     launch(paged_join_kernel<NB, ROWS>, dim3(A.n_tokens, A.n_head), dim3(256), 0, st, A);
