@@ -25,8 +25,9 @@ typedef float f4 __attribute__((ext_vector_type(4)));
 typedef int i2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
-constexpr int STEP = 32;               // positions of a step
-constexpr int SPLIT_WG = 256;
+constexpr int STEP = 32;               // positions of a step, few rows
+constexpr int TILE_STEP = 64;          // and many
+constexpr int SPLIT_WG = 256, TILE_WG = 256;
 constexpr float M_NONE = -1.7e38f;     // the maximum of no scores: finite, so that differences are no NaN
 
 // a value that every lane holds, as a scalar
@@ -53,10 +54,29 @@ __device__ __forceinline__ seq_info seq_of(const paged_attn & A, int s) {
     return q;
 }
 
+// Few rows: the steps of a sequence's whole length for each of its tiles of `rows` rows and teams of heads; of more rows
+// than most, none (another launch's).
 __device__ __forceinline__ int steps_of(const seq_info & q) { return max((q.len + STEP - 1) / STEP, 1); }
+__device__ __forceinline__ int64_t split_units(const paged_attn & A, const seq_info & q, int rows) {
+    const int n = q.n * A.group;
+    return n > A.split_most ? 0 : (int64_t) ((n + rows - 1) / rows) * A.head_teams * steps_of(q);
+}
 
-__device__ __forceinline__ int64_t seq_units(const paged_attn & A, const seq_info & q, int rows) {
-    return (int64_t) ((q.n * A.group + rows - 1) / rows) * A.head_teams * steps_of(q);
+// Many: of each tile, the steps that its last token sees.
+__device__ __forceinline__ int tile_steps(const paged_attn & A, const seq_info & q, int rows, int tile) {
+    const int i = min((int) (((int64_t) (tile + 1) * rows - 1) / A.group), q.n - 1);
+    const int sees = min(q.last - (q.n - 1) + i + 1, q.len);
+    return max((sees + TILE_STEP - 1) / TILE_STEP, 1);
+}
+__device__ __forceinline__ int tiles_of(const paged_attn & A, const seq_info & q, int rows) {
+    const int64_t n = (int64_t) q.n * A.group;
+    return n < A.tile_least ? 0 : (int) ((n + rows - 1) / rows);
+}
+__device__ __forceinline__ int64_t tile_units(const paged_attn & A, const seq_info & q, int rows) {
+    const int tiles = tiles_of(A, q, rows);
+    int64_t sum = 0;
+    for (int k = 0; k < tiles; k++) sum += tile_steps(A, q, rows, k);
+    return sum * A.n_head_kv;
 }
 
 __device__ __forceinline__ int64_t wave_scan(int64_t v) {
@@ -176,19 +196,18 @@ template <int N> __device__ __forceinline__ float row_ror(float v) {
 
 // Few rows a sequence: a wave takes steps of one KV head by itself.
 //
-// Wide: the 16 columns of a tile are 16 rows (query, head), RT tiles of them. Narrow, for up to 16 / NB rows (4 for
+// Wide: the 16 columns of a tile are 16 rows (query, head). Narrow, for up to 16 / NB rows (4 for
 // heads of 96): a column is a row and a block. A lane takes its own block's sums of each product, scales them and
 // adds its neighbours', and forms p d for its own block only, which serves all blocks' products (a quarter of that
 // work where a KV head has four query heads).
 //
 // P16: pages of whole sixteens of rows, so that a load's 16 positions are on one page, found by scalar loads.
-template <int NB, int RT, bool NARROW, bool P16>
+template <int NB, bool NARROW, bool P16>
 __global__ __launch_bounds__(SPLIT_WG, NARROW ? 3 : 2) void paged_split_kernel(const paged_attn args) {
-    constexpr int D = NB * 32, COLS = NARROW ? (NB == 2 ? 8 : 4) : 16, ROWS = COLS * RT;
+    constexpr int D = NB * 32, RT = 1, COLS = NARROW ? (NB == 2 ? 8 : 4) : 16, ROWS = COLS;
     constexpr int QB = NARROW ? 1 : NB;               // blocks of a column's values: narrow, its own
     constexpr int LOADS = NB == 2 ? 1 : 2;            // 16-byte loads a lane of a step's K or V
     constexpr int SROW = STEP + 4;                    // scales of a block over a step's positions, in 32 bits
-    static_assert(!NARROW || RT == 1, "one tile");
     __shared__ __align__(16) uint8_t s_v[SPLIT_WG / WAVE][STEP * NB * 16];
     __shared__ __align__(16) float s_d[SPLIT_WG / WAVE][2][NB * SROW];
     const paged_attn & A = kernargs_prefetched(args);
@@ -206,10 +225,10 @@ __global__ __launch_bounds__(SPLIT_WG, NARROW ? 3 : 2) void paged_split_kernel(c
     int64_t u = 0, left;
     {
         // sequences by lanes, 64 at a time; of few, one look is enough
-        int64_t n = lane < A.n_seqs ? seq_units(A, seq_of(A, lane), ROWS) : 0, up = wave_scan(n), all = from_lane(up, WAVE - 1);
+        int64_t n = lane < A.n_seqs ? split_units(A, seq_of(A, lane), ROWS) : 0, up = wave_scan(n), all = from_lane(up, WAVE - 1);
         for (int s0 = WAVE; s0 < A.n_seqs; s0 += WAVE) {
             const int s = s0 + lane;
-            all += from_lane(wave_scan(s < A.n_seqs ? seq_units(A, seq_of(A, s), ROWS) : 0), WAVE - 1);
+            all += from_lane(wave_scan(s < A.n_seqs ? split_units(A, seq_of(A, s), ROWS) : 0), WAVE - 1);
         }
         P.deal(all, A.teams);
         if (team >= P.teams) return;
@@ -221,7 +240,7 @@ __global__ __launch_bounds__(SPLIT_WG, NARROW ? 3 : 2) void paged_split_kernel(c
         for (int s0 = WAVE; !past && s0 < A.n_seqs; s0 += WAVE) {
             before = from_lane(up, WAVE - 1);
             const int s = s0 + lane;
-            n = s < A.n_seqs ? seq_units(A, seq_of(A, s), ROWS) : 0;
+            n = s < A.n_seqs ? split_units(A, seq_of(A, s), ROWS) : 0;
             up = before + wave_scan(n);
             past = __ballot(up > u);
             seq = s0;
@@ -234,7 +253,7 @@ __global__ __launch_bounds__(SPLIT_WG, NARROW ? 3 : 2) void paged_split_kernel(c
     while (left > 0 && seq < A.n_seqs) {
         const seq_info Q = seq_of(A, seq);
         const int steps = steps_of(Q);
-        const int tiles = (Q.n * A.group + ROWS - 1) / ROWS;
+        const int tiles = Q.n * A.group > A.split_most ? 0 : (Q.n * A.group + ROWS - 1) / ROWS;
         if (u >= (int64_t) tiles * A.head_teams * steps) { seq++; u = 0; continue; }
         const int item = uniform(u < ((int64_t) 1 << 32) ? (int) ((uint32_t) u / (uint32_t) steps) : (int) (u / steps));
         const int step0 = (int) (u - (int64_t) item * steps);
@@ -607,69 +626,556 @@ __global__ __launch_bounds__(SPLIT_WG, NARROW ? 3 : 2) void paged_split_kernel(c
     }
 }
 
-// Rows whose steps several teams took: their parts joined, a workgroup a row, D / 4 threads a part.
-template <int NB, int ROWS>
+// ---- many rows a sequence: four waves share a step's operands ----
+//
+// A workgroup takes 64 RT rows of one KV head, a wave 16 RT of them, in steps of 64 positions. Wave b decodes block b of the
+// step's keys and values for all four: codes - 8 of K as A wants them, and V's values d (codes - 8) as two halves
+// (15 bits: exactly), so that p is split once for all blocks (three products: hi hi, lo hi, hi lo). V's scales are
+// taken times 2^s of each block, so that the largest so far is at 2^11 to 2^12; a scale that is not finite counts as 0, and
+// makes the results of the rows that see it NaN.
+template <int NB, int RT>
+__global__ __launch_bounds__(TILE_WG, RT == 1 ? 3 : 2) void paged_tile_kernel(const paged_attn args) {
+    constexpr int D = NB * 32, ROWS = 64 * RT;
+    constexpr int SROW = TILE_STEP + 4;
+    __shared__ __align__(16) u4 s_k[NB][4][WAVE];             // block, sixteen of positions, lane
+    __shared__ __align__(16) u4 s_v[NB][2][2][2][WAVE];       // block, 32 positions, half of the block, hi and lo, lane
+    __shared__ __align__(16) float s_kd[NB][SROW];
+    __shared__ __align__(16) _Float16 s_vd[NB][TILE_STEP];
+    __shared__ int s_shift[NB];
+    __shared__ uint64_t s_odd[NB], s_gone;                    // positions whose V scale is not finite; whose page is not there
+    const paged_attn & A = kernargs_prefetched(args);
+    const int lane = threadIdx.x % WAVE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
+    const int col = lane % 16, c = lane / 16;
+    const code_bits K;
+
+    plan P;
+    int seq = 0;
+    int64_t u = 0, left;
+    {
+        int64_t n = lane < A.n_seqs ? tile_units(A, seq_of(A, lane), ROWS) : 0, up = wave_scan(n), all = from_lane(up, WAVE - 1);
+        for (int s0 = WAVE; s0 < A.n_seqs; s0 += WAVE) {
+            const int s = s0 + lane;
+            all += from_lane(wave_scan(s < A.n_seqs ? tile_units(A, seq_of(A, s), ROWS) : 0), WAVE - 1);
+        }
+        P.deal(all, A.tile_teams);
+        if ((int) blockIdx.x >= P.teams) return;
+        u = P.begin(blockIdx.x);
+        left = P.begin(blockIdx.x + 1) - u;
+        if (left <= 0) return;
+        int64_t before = 0;
+        uint64_t past = __ballot(up > u);
+        for (int s0 = WAVE; !past && s0 < A.n_seqs; s0 += WAVE) {
+            before = from_lane(up, WAVE - 1);
+            const int s = s0 + lane;
+            n = s < A.n_seqs ? tile_units(A, seq_of(A, s), ROWS) : 0;
+            up = before + wave_scan(n);
+            past = __ballot(up > u);
+            seq = s0;
+        }
+        const int l = past ? __builtin_ctzll(past) : 0;
+        seq += l;
+        u -= from_lane(up - n, l);
+    }
+    // the tile of the sequence, and the unit in it (heads by steps)
+    int tile = 0;
+    {
+        const seq_info Q = seq_of(A, seq);
+        const int tiles = tiles_of(A, Q, ROWS);
+        for (int k0 = 0; k0 < tiles; k0 += WAVE) {
+            const int k = k0 + lane;
+            const int64_t n = k < tiles ? (int64_t) tile_steps(A, Q, ROWS, k) * A.n_head_kv : 0, up = wave_scan(n);
+            const uint64_t past = __ballot(up > u);
+            if (past) {
+                const int l = __builtin_ctzll(past);
+                tile = k0 + l;
+                u -= from_lane(up - n, l);
+                break;
+            }
+            u -= from_lane(up, WAVE - 1);
+        }
+    }
+
+    while (left > 0 && seq < A.n_seqs) {
+        const seq_info Q = seq_of(A, seq);
+        if (tile >= tiles_of(A, Q, ROWS)) { seq++; tile = 0; u = 0; continue; }
+        const int steps = tile_steps(A, Q, ROWS, tile);
+        if (u >= (int64_t) steps * A.n_head_kv) { tile++; u = 0; continue; }
+        const int head = uniform((int) ((uint32_t) u / (uint32_t) steps)), step0 = (int) u - head * steps;
+        const int step1 = (int) min((int64_t) steps, step0 + left);
+        u += step1 - step0;
+        left -= step1 - step0;
+
+        // ---- the step's operands: lane l of wave b takes block b of position l ----
+        const int32_t * table = A.pages + (int64_t) seq * A.pages_s;
+        const int64_t k_first = (int64_t) head * A.k_head + wave, v_first = (int64_t) head * A.v_head + wave;
+        const int n_pages = (int) min(A.n_pages, (int64_t) INT32_MAX), rows_page = A.page;
+        const int64_t k_page = A.k_page, k_pos = A.k_pos, v_page = A.v_page, v_pos = A.v_pos;
+        const bool decodes = wave < NB;
+        int page = -1;
+        auto page_of = [&](int step) {
+            const int pos = step * TILE_STEP + lane;
+            page = decodes && pos < Q.len && step < step1 ? table[page_index(A, pos)] : -1;
+        };
+        u4 kraw, vraw;
+        _Float16 kd, vd;
+        bool there;
+        auto load = [&](int step) {
+            const int pos = step * TILE_STEP + lane;
+            there = page >= 0 && page < n_pages;
+            const int off = pos - page_index(A, pos) * rows_page;
+            const int64_t kb = k_first + (there ? (int64_t) page * k_page + (int64_t) off * k_pos : 0);
+            const int64_t vb = v_first + (there ? (int64_t) page * v_page + (int64_t) off * v_pos : 0);
+            kraw = *(const u4 *) (A.kq + kb * 16);
+            vraw = *(const u4 *) (A.vq + vb * 16);
+            kd = ((const _Float16 *) A.kd)[kb];
+            vd = ((const _Float16 *) A.vd)[vb];
+        };
+        page_of(step0);
+
+        // ---- the wave's rows ----
+        h8 qh[RT][NB], ql[RT][NB];
+        float fac[RT], m[RT], l[RT];
+        int lim[RT];
+        f4 o[RT][NB][2];
+#pragma unroll
+        for (int t = 0; t < RT; t++) {
+            const int row = tile * ROWS + (wave * RT + t) * 16 + col;
+            const bool real = row < Q.n * A.group;
+            const int i = real ? row / A.group : 0, g = real ? row - i * A.group : 0;
+            const float * q = A.q + (int64_t) (Q.first + i) * A.q_t + (int64_t) (head * A.group + g) * A.q_h;
+            lim[t] = min(Q.last - (Q.n - 1) + (real ? i : Q.n - 1), Q.len - 1);
+            float v[NB][8], big = 0.0f;
+#pragma unroll
+            for (int b = 0; b < NB; b++) {
+                const float4 lo = load4(q + 32 * b + 4 * c), hi = load4(q + 32 * b + 16 + 4 * c);
+                const float w[8] = { lo.x, lo.z, hi.x, hi.z, lo.y, lo.w, hi.y, hi.w };
+#pragma unroll
+                for (int k = 0; k < 8; k++) {
+                    v[b][k] = real ? w[k] : 0.0f;
+                    big = fmaxf(big, fabsf(v[b][k]));
+                }
+            }
+            if (t == 0 && decodes) {
+                load(step0);
+                page_of(step0 + 1);
+            }
+            big = column_max(big);
+            const int e = big > 0.0f && big < INFINITY ? 14 - __builtin_amdgcn_frexp_expf(big) : 0;
+            const float sign = A.scale < 0.0f ? -1.0f : 1.0f;
+#pragma unroll
+            for (int b = 0; b < NB; b++) {
+#pragma unroll
+                for (int k = 0; k < 8; k++) {
+                    const float x = __builtin_amdgcn_ldexpf(v[b][k] * sign, e);
+                    qh[t][b][k] = (_Float16) x;
+                    ql[t][b][k] = (_Float16) (x - (float) qh[t][b][k]);
+                }
+            }
+            fac[t] = fabsf(A.scale) * LOG2E * __builtin_amdgcn_ldexpf(1.0f, -e);
+            m[t] = M_NONE;
+            l[t] = 0.0f;
+#pragma unroll
+            for (int b = 0; b < NB; b++) o[t][b][0] = o[t][b][1] = f4{ 0, 0, 0, 0 };
+        }
+        const int first_row = tile * ROWS + wave * RT * 16;
+        const int sure = min(Q.last - (Q.n - 1) + min(first_row / A.group, Q.n - 1), Q.len - 1);
+        int own_shift = 38, shift[NB];
+#pragma unroll
+        for (int b = 0; b < NB; b++) shift[b] = 38;
+
+        for (int step = step0; step < step1; step++) {
+            __syncthreads();                              // the operands before these are read
+            if (decodes) {
+                const bool finite = fabsf((float) vd) < INFINITY;
+                const float dv = there && finite ? fabsf((float) vd) : 0.0f;
+                if (__any(dv >= __builtin_amdgcn_ldexpf(1.0f, 12 - own_shift))) {
+                    const float big = wave_max(dv);
+                    own_shift = min(own_shift, 12 - __builtin_amdgcn_frexp_expf(big));
+                }
+                s_kd[wave][lane] = there ? (float) kd : 0.0f;
+                // scales of positions 16 t + 4 c + r side by side over t
+                s_vd[wave][(lane & 32) + ((lane >> 2) & 3) * 8 + (lane & 3) * 2 + ((lane >> 4) & 1)] =
+                    there && finite ? (_Float16) __builtin_amdgcn_ldexpf((float) vd, own_shift) : (_Float16) 0.0f;
+                const uint64_t odd = __ballot(there && !finite), gone = __ballot(step * TILE_STEP + lane < Q.len && !there);
+                if (lane == 0) {
+                    s_shift[wave] = own_shift;
+                    s_odd[wave] = odd;
+                    if (wave == 0) s_gone = gone;
+                }
+                // V's bytes where its values will be, read again by the transposing read
+                uint8_t * raw = (uint8_t *) &s_v[wave][0][0][0][0];
+                *(u4 *) (raw + lane * 16) = vraw;
+#pragma unroll
+                for (int k = 0; k < 4; k++) s_k[wave][lane / 16][k * 16 + col] = __builtin_bit_cast(u4, signed_of(kraw[k], K));
+                i2 codes[2];
+#pragma unroll
+                for (int hs = 0; hs < 2; hs++) {
+                    codes[hs] = __builtin_amdgcn_ds_read_tr4_b64_v2i32(
+                        (__attribute__((address_space(3))) i2 *) (raw + (32 * hs + 16 * ((col >> 2) & 1) + 4 * c + (col & 3)) * 16 + (col >> 3) * 8));
+                }
+                u4 d[2];
+#pragma unroll
+                for (int hs = 0; hs < 2; hs++) d[hs] = *(const u4 *) &s_vd[wave][32 * hs + c * 8];
+                // (these reads are before the writes: one wave's LDS operations keep their order)
+#pragma unroll
+                for (int hs = 0; hs < 2; hs++) {
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        const h8 a = signed_of(codes[hs][h], K), dd = __builtin_bit_cast(h8, d[hs]);
+                        const h8 hi = a * dd, lo = __builtin_elementwise_fma(a, dd, -hi);
+                        s_v[wave][hs][h][0][lane] = __builtin_bit_cast(u4, hi);
+                        s_v[wave][hs][h][1][lane] = __builtin_bit_cast(u4, lo);
+                    }
+                }
+                if (step + 1 < step1) {
+                    load(step + 1);
+                    page_of(step + 2);
+                }
+            }
+            __syncthreads();                              // the step's operands are there
+
+            uint64_t odd = 0;
+#pragma unroll
+            for (int b = 0; b < NB; b++) {
+                odd |= s_odd[b];
+                const int now = s_shift[b];
+                if (__any(now != shift[b])) {
+                    const float keep = __builtin_amdgcn_ldexpf(1.0f, now - shift[b]);
+                    shift[b] = now;
+#pragma unroll
+                    for (int x = 0; x < RT; x++) { o[x][b][0] *= keep; o[x][b][1] *= keep; }
+                }
+            }
+#pragma unroll 1
+            for (int hs = 0; hs < 2; hs++) {
+                const int at = step * TILE_STEP + 32 * hs;
+                f4 s[RT][2];
+#pragma unroll
+                for (int t = 0; t < 2; t++) {
+#pragma unroll
+                    for (int b = 0; b < NB; b++) {
+                        const h8 a = __builtin_bit_cast(h8, s_k[b][2 * hs + t][lane]);
+                        const f4 d = *(const f4 *) &s_kd[b][32 * hs + 16 * t + 4 * c];
+#pragma unroll
+                        for (int x = 0; x < RT; x++) {
+                            f4 acc = { 0, 0, 0, 0 };
+                            acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, qh[x][b], acc, 0, 0, 0);
+                            acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, ql[x][b], acc, 0, 0, 0);
+#pragma unroll
+                            for (int i = 0; i < 4; i++) s[x][t][i] = b == 0 ? acc[i] * d[i] : fmaf(acc[i], d[i], s[x][t][i]);
+                        }
+                    }
+                }
+                // positions on missing pages have scales of 0 but scores all the same: their rows' bits
+                const uint32_t missing = (uint32_t) (s_gone >> (32 * hs));
+                const bool edge = at + 31 > sure || missing;
+                uint32_t hidden[RT];
+                h8 ph[RT], pl[RT];
+#pragma unroll
+                for (int x = 0; x < RT; x++) {
+                    hidden[x] = 0;
+                    if (edge) {
+#pragma unroll
+                        for (int t = 0; t < 2; t++) {
+#pragma unroll
+                            for (int i = 0; i < 4; i++) {
+                                const int k = 16 * t + 4 * c + i;
+                                if (at + k > lim[x] || ((missing >> k) & 1)) {
+                                    s[x][t][i] = -INFINITY;
+                                    hidden[x] |= 1u << (4 * t + i);
+                                }
+                            }
+                        }
+                    }
+                    float top = -INFINITY;
+#pragma unroll
+                    for (int t = 0; t < 2; t++) {
+#pragma unroll
+                        for (int i = 0; i < 4; i++) top = fmaxf(top, s[x][t][i]);
+                    }
+                    top = column_max(top) * fac[x];
+                    if (__any(top > m[x])) {
+                        const float now = fmaxf(m[x], top), keep = exp2_hw(m[x] - now);
+                        m[x] = now;
+                        l[x] *= keep;
+#pragma unroll
+                        for (int b = 0; b < NB; b++) { o[x][b][0] *= keep; o[x][b][1] *= keep; }
+                    }
+                    // p times 2^15
+                    const float up = 15.0f - m[x];
+#pragma unroll
+                    for (int t = 0; t < 2; t++) {
+#pragma unroll
+                        for (int i = 0; i < 4; i++) s[x][t][i] = exp2_hw(fmaf(s[x][t][i], fac[x], up));
+                    }
+                    if (edge) {
+#pragma unroll
+                        for (int t = 0; t < 2; t++) {
+#pragma unroll
+                            for (int i = 0; i < 4; i++) if ((hidden[x] >> (4 * t + i)) & 1) s[x][t][i] = 0.0f;
+                        }
+                    }
+                    l[x] += ((s[x][0][0] + s[x][0][1]) + (s[x][0][2] + s[x][0][3])) + ((s[x][1][0] + s[x][1][1]) + (s[x][1][2] + s[x][1][3]));
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+#pragma unroll
+                        for (int t = 0; t < 2; t++) {
+                            ph[x][2 * i + t] = (_Float16) s[x][t][i];
+                            pl[x][2 * i + t] = (_Float16) (s[x][t][i] - (float) ph[x][2 * i + t]);
+                        }
+                    }
+                }
+                if (odd) {
+                    // a scale that is not finite at a position that the row sees
+#pragma unroll
+                    for (int b = 0; b < NB; b++) {
+                        const uint32_t bits = (uint32_t) (s_odd[b] >> (32 * hs));
+#pragma unroll
+                        for (int x = 0; x < RT; x++) {
+                            bool sees = false;
+#pragma unroll
+                            for (int t = 0; t < 2; t++) {
+#pragma unroll
+                                for (int i = 0; i < 4; i++) sees |= ((bits >> (16 * t + 4 * c + i)) & 1) && !((hidden[x] >> (4 * t + i)) & 1);
+                            }
+                            if (column_max(sees ? 1.0f : 0.0f) > 0.0f) o[x][b][0] = o[x][b][1] = f4{ NAN, NAN, NAN, NAN };
+                        }
+                    }
+                }
+#pragma unroll
+                for (int b = 0; b < NB; b++) {
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        const h8 hi = __builtin_bit_cast(h8, s_v[b][hs][h][0][lane]), lo = __builtin_bit_cast(h8, s_v[b][hs][h][1][lane]);
+#pragma unroll
+                        for (int x = 0; x < RT; x++) {
+                            o[x][b][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo, ph[x], o[x][b][h], 0, 0, 0);
+                            o[x][b][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, pl[x], o[x][b][h], 0, 0, 0);
+                            o[x][b][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, ph[x], o[x][b][h], 0, 0, 0);
+                        }
+                    }
+                }
+            }
+        }
+
+        // ---- the rows' results, or this run's part of them ----
+        const bool whole = step0 == 0 && step1 == steps;
+        const int64_t slot = ((int64_t) blockIdx.x * 2 + (step0 == 0)) * ROWS;
+#pragma unroll
+        for (int x = 0; x < RT; x++) {
+            const int at_row = (wave * RT + x) * 16 + col, row = tile * ROWS + at_row;
+            const float sum = column_sum(l[x]) * 0x1p-15f;
+            if (row >= Q.n * A.group) continue;
+            const int i = row / A.group, g = row - i * A.group;
+            const float inv = whole ? (sum > 0.0f ? 1.0f / sum : sum == 0.0f ? 0.0f : sum) : 1.0f;
+            float * out = whole ? A.out + ((int64_t) (Q.first + i) * A.n_head + head * A.group + g) * D
+                                : A.tile_part + (slot + at_row) * D;
+#pragma unroll
+            for (int b = 0; b < NB; b++) {
+                // (in two steps: 2^-(15 + shift) may be below the range where inv is large)
+                const float w = __builtin_amdgcn_ldexpf(inv, -15);
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    float r[4];
+#pragma unroll
+                    for (int k = 0; k < 4; k++) r[k] = __builtin_amdgcn_ldexpf(o[x][b][h][k], -shift[b]) * w;
+                    float * at = out + 32 * b + 8 * h + 2 * c;
+                    *(float2 *) at = make_float2(r[0], r[2]);
+                    *(float2 *) (at + 16) = make_float2(r[1], r[3]);
+                }
+            }
+            if (!whole && c == 0) A.tile_ml[slot + at_row] = make_float2(m[x], sum);
+        }
+    }
+}
+
+// parts of one row, four values of it: o = sum_k 2^(m_k - m) o_k, l likewise
+struct part_sum {
+    float m = M_NONE, l = 0.0f;
+    float4 o = make_float4(0, 0, 0, 0);
+    // parts from, from + by, .. up to last, four of them loaded at a time; at(k): row of part k
+    template <typename F>
+    __device__ __forceinline__ void add(const float * part, const float2 * part_ml, F at, int D, int e, int64_t from, int64_t last, int by) {
+        for (int64_t k0 = from; k0 <= last; k0 += 4 * by) {
+            float2 ml[4];
+            float4 v[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int64_t r = at(min(k0 + i * by, last));
+                ml[i] = part_ml[r];
+                v[i] = *(const float4 *) (part + r * D + 4 * e);
+            }
+            float now = m;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                if (k0 + i * by > last) ml[i] = make_float2(M_NONE, 0.0f);
+                now = fmaxf(now, ml[i].x);
+            }
+            const float was = exp2_hw(m - now);
+            l *= was;
+            o.x *= was;
+            o.y *= was;
+            o.z *= was;
+            o.w *= was;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                if (k0 + i * by > last) continue;
+                const float is = exp2_hw(ml[i].x - now);
+                l = fmaf(ml[i].y, is, l);
+                o.x = fmaf(v[i].x, is, o.x);
+                o.y = fmaf(v[i].y, is, o.y);
+                o.z = fmaf(v[i].z, is, o.z);
+                o.w = fmaf(v[i].w, is, o.w);
+            }
+            m = now;
+        }
+    }
+};
+
+// The same by teams: of many tokens few rows have parts. A workgroup looks at the item that its team ends in, and joins the
+// item's rows if the team began it and did not finish it.
+template <int NB, int SPLIT, int TILE>
+__global__ __launch_bounds__(256) void paged_join_teams_kernel(const paged_attn args) {
+    const paged_attn & A = kernargs_prefetched(args);
+    constexpr int D = NB * 32, PER = D / 4, GROUPS = 256 / PER, ROWS = SPLIT ? SPLIT : TILE;
+    const int lane = threadIdx.x % WAVE, t = threadIdx.x;
+    const int team = SPLIT ? A.team : 1, in_team = SPLIT ? (int) blockIdx.y : 0;
+    auto units = [&](int s) { return s >= A.n_seqs ? (int64_t) 0 : SPLIT ? split_units(A, seq_of(A, s), ROWS) : tile_units(A, seq_of(A, s), ROWS); };
+    int64_t all = 0;
+    for (int s0 = 0; s0 < A.n_seqs; s0 += WAVE) all += from_lane(wave_scan(units(s0 + lane)), WAVE - 1);
+    plan P;
+    P.deal(all, SPLIT ? A.teams : A.tile_teams);
+    const int64_t me = blockIdx.x;
+    if (me >= P.teams) return;
+    const int64_t begin = P.begin(me), end = P.begin(me + 1);
+    if (begin >= end) return;
+    int64_t u = end - 1, before = 0;
+    int seq = -1;
+    for (int s0 = 0; seq < 0 && s0 < A.n_seqs; s0 += WAVE) {
+        const int64_t n = units(s0 + lane), up = before + wave_scan(n);
+        const uint64_t past = __ballot(up > u);
+        if (past) {
+            const int l = __builtin_ctzll(past);
+            seq = s0 + l;
+            before = from_lane(up - n, l);
+        } else {
+            before = from_lane(up, WAVE - 1);
+        }
+    }
+    if (seq < 0) return;
+    const seq_info Q = seq_of(A, seq);
+    int tile = 0, head = 0, steps;
+    if (SPLIT) {
+        steps = steps_of(Q);
+        const int64_t item = (u - before) / steps;
+        tile = (int) (item / A.head_teams);
+        head = (int) (item - (int64_t) tile * A.head_teams) * team + in_team;
+        before += item * steps;
+    } else {
+        const int tiles = tiles_of(A, Q, ROWS);
+        for (int k0 = 0; k0 < tiles; k0 += WAVE) {
+            const int64_t n = k0 + lane < tiles ? (int64_t) tile_steps(A, Q, ROWS, k0 + lane) * A.n_head_kv : 0, up = before + wave_scan(n);
+            const uint64_t past = __ballot(up > u);
+            if (past) {
+                const int l = __builtin_ctzll(past);
+                tile = k0 + l;
+                before = from_lane(up - n, l);
+                break;
+            }
+            before = from_lane(up, WAVE - 1);
+        }
+        steps = tile_steps(A, Q, ROWS, tile);
+        head = (int) ((u - before) / steps);
+        before += (int64_t) head * steps;
+    }
+    if (before < begin || before + steps <= end) return;
+    const int64_t last = P.team_of(before + steps - 1);
+    const float * part = SPLIT ? A.part : A.tile_part;
+    const float2 * part_ml = SPLIT ? A.part_ml : A.tile_ml;
+    const int group = t / PER, e = t % PER, rows = min(ROWS, Q.n * A.group - tile * ROWS);
+    // TILE: rows over the grid's second dimension
+    for (int r = group + (SPLIT ? 0 : (int) blockIdx.y * GROUPS); group < GROUPS && r < rows; r += GROUPS * (SPLIT ? 1 : (int) gridDim.y)) {
+        part_sum S;
+        S.add(part, part_ml, [&](int64_t k) { return ((k * 2 + (k == me)) * team + in_team) * ROWS + r; }, D, e, me, last, 1);
+        const int row = tile * ROWS + r, i = row / A.group, g = row - i * A.group;
+        const float inv = S.l > 0.0f ? 1.0f / S.l : S.l == 0.0f ? 0.0f : S.l;
+        *(float4 *) (A.out + ((int64_t) (Q.first + i) * A.n_head + head * A.group + g) * D + 4 * e) =
+            make_float4(S.o.x * inv, S.o.y * inv, S.o.z * inv, S.o.w * inv);
+    }
+}
+
+// Rows whose steps several teams took: their parts joined, a workgroup a row, D / 4 threads a part. A row is a split
+// launch's (SPLIT rows a tile) or a tile launch's (TILE rows), by its sequence's rows.
+template <int NB, int SPLIT, int TILE>
 __global__ __launch_bounds__(256) void paged_join_kernel(const paged_attn args) {
     const paged_attn & A = kernargs_prefetched(args);
     constexpr int D = NB * 32, PER = D / 4, GROUPS = 256 / PER;
     __shared__ float4 s_o[GROUPS][PER];
     __shared__ float2 s_ml[GROUPS];
     const int token = blockIdx.x, head = blockIdx.y, t = threadIdx.x, lane = t % WAVE;
-    // the token's sequence, and the units before it
+    // the token's sequence, and the units before it in either line
     int seq = -1;
-    int64_t all = 0, begin = 0;
+    int64_t all_s = 0, all_t = 0, begin_s = 0, begin_t = 0;
     for (int s0 = 0; s0 < A.n_seqs; s0 += WAVE) {
         const int s = s0 + lane;
         bool mine = false;
-        int64_t n = 0;
+        int64_t ns = 0, nt = 0;
         if (s < A.n_seqs) {
             const seq_info q = seq_of(A, s);
             mine = token >= q.first && token < q.first + q.n;
-            n = seq_units(A, q, ROWS);
+            if (SPLIT) ns = split_units(A, q, SPLIT);
+            if (TILE) nt = tile_units(A, q, TILE);
         }
         const uint64_t b = __ballot(mine);
-        const int64_t up = wave_scan(n);
-        if (b && seq < 0) {
-            const int l = __builtin_ctzll(b);
-            seq = s0 + l;
-            begin = all + from_lane(up - n, l);
+        const int l = b ? __builtin_ctzll(b) : 0;
+        const bool first = b && seq < 0;
+        if (first) seq = s0 + l;
+        if (SPLIT) {
+            const int64_t up = wave_scan(ns);
+            if (first) begin_s = all_s + from_lane(up - ns, l);
+            all_s += from_lane(up, WAVE - 1);
         }
-        all += from_lane(up, WAVE - 1);
+        if (TILE) {
+            const int64_t up = wave_scan(nt);
+            if (first) begin_t = all_t + from_lane(up - nt, l);
+            all_t += from_lane(up, WAVE - 1);
+        }
     }
     if (seq < 0) return;
     const seq_info Q = seq_of(A, seq);
-    plan P;
-    P.deal(all, A.teams);
+    const bool tiled = TILE && (!SPLIT || (int64_t) Q.n * A.group >= A.tile_least);
     const int kvh = head / A.group, row = (token - Q.first) * A.group + head - kvh * A.group;
-    const int tile = row / ROWS, steps = steps_of(Q);
-    const int64_t a = begin + ((int64_t) tile * A.head_teams + kvh / A.team) * steps;
+    const int rows = tiled ? TILE : SPLIT, tile = row / rows, team = tiled ? 1 : A.team;
+    plan P;
+    P.deal(tiled ? all_t : all_s, tiled ? A.tile_teams : A.teams);
+    int64_t a;
+    int steps;
+    if (tiled) {
+        steps = tile_steps(A, Q, rows, tile);
+        a = begin_t + (int64_t) kvh * steps;
+        for (int k = 0; k < tile; k++) a += (int64_t) tile_steps(A, Q, rows, k) * A.n_head_kv;
+    } else {
+        steps = steps_of(Q);
+        a = begin_s + ((int64_t) tile * A.head_teams + kvh / team) * steps;
+    }
     const int64_t t0 = P.team_of(a), t1 = P.team_of(a + steps - 1);
     if (t0 == t1) return;                               // written whole
+    const float * part = tiled ? A.tile_part : A.part;
+    const float2 * part_ml = tiled ? A.tile_ml : A.part_ml;
     const int group = t / PER, e = t % PER;
-    float m = M_NONE, l = 0.0f;
-    float4 o = make_float4(0, 0, 0, 0);
+    part_sum S;
     if (group < GROUPS) {
-        for (int64_t k = t0 + group; k <= t1; k += GROUPS) {
-            const int64_t at = ((k * 2 + (k == t0)) * A.team + kvh % A.team) * ROWS + row - tile * ROWS;
-            const float2 ml = A.part_ml[at];
-            const float4 v = *(const float4 *) (A.part + at * D + 4 * e);
-            const float now = fmaxf(m, ml.x), was = exp2_hw(m - now), is = exp2_hw(ml.x - now);
-            l = l * was + ml.y * is;
-            o.x = o.x * was + v.x * is;
-            o.y = o.y * was + v.y * is;
-            o.z = o.z * was + v.z * is;
-            o.w = o.w * was + v.w * is;
-            m = now;
-        }
+        S.add(part, part_ml, [&](int64_t k) { return ((k * 2 + (k == t0)) * team + kvh % team) * rows + row - tile * rows; }, D, e, t0 + group, t1, GROUPS);
+        float m = S.m, l = S.l;
+        float4 o = S.o;
         s_o[group][e] = o;
         if (e == 0) s_ml[group] = make_float2(m, l);
     }
     __syncthreads();
     if (t >= PER) return;
-    float top = M_NONE;
+    float top = M_NONE, l = 0.0f;
     for (int k = 0; k < GROUPS; k++) top = fmaxf(top, s_ml[k].x);
-    l = 0.0f;
-    o = make_float4(0, 0, 0, 0);
+    float4 o = make_float4(0, 0, 0, 0);
     for (int k = 0; k < GROUPS; k++) {
         const float w = exp2_hw(s_ml[k].x - top);
         const float4 v = s_o[k][t];
@@ -683,57 +1189,86 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const paged_attn args) 
     *(float4 *) (A.out + ((int64_t) token * A.n_head + head) * D + 4 * t) = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
 }
 
-constexpr int SPLIT_WGS = 768;         // three workgroups of four waves a CU
-
-// rows of a tile: narrow, one or two of 16
-int split_rows(const paged_attn & A) {
+// Rows a sequence on average: up to 8 (of heads of 64) or 4 go narrow and up to 16 wide, a wave by itself; more in tiles of
+// 64. Past 64 in tiles of 128, and the sequences among them that have 16 or fewer by waves: a batch of prompts' parts and single
+// tokens.
+struct paged_ways { int split, tile; };      // rows of a tile, 0: no such launch
+paged_ways ways_of(const paged_attn & A) {
     const int narrow = A.D == 64 ? 8 : 4;
     const int64_t rows = (int64_t) A.n_tokens * A.group, per = A.n_seqs;
-    return rows <= narrow * per && A.group <= narrow ? narrow : rows <= 16 * per ? 16 : 32;
+    if (rows <= narrow * per && A.group <= narrow) return { narrow, 0 };
+    if (rows <= 16 * per) return { 16, 0 };
+    if (rows <= 64 * per) return { 0, 64 };
+    return { per > 1 ? 16 : 0, 128 };
 }
+// workgroups of four waves that a CU holds: more would run behind the first
+int split_wgs(int rows) { return rows < 16 ? 768 : 512; }
+int tile_wgs(int rows) { return rows == 64 ? 768 : 512; }
 
-template <int NB, int RT, bool NARROW>
+template <int NB, bool NARROW>
 void split(const paged_attn & A, hipStream_t st) {
-    constexpr int ROWS = NARROW ? (NB == 2 ? 8 : 4) : 16 * RT;
     // a sixteen of positions on one page, its rows within 32-bit offsets, and a row's number within 32 bits
     const int64_t reach = std::max(std::max(16 * 16 * std::max(A.k_pos, A.v_pos), std::max(A.k_page, A.v_page)), (A.n_pages * std::max(A.k_page, A.v_page) + 1) / 2);
-    if (A.page % 16 == 0 && reach <= INT32_MAX) launch(paged_split_kernel<NB, RT, NARROW, true>, dim3(SPLIT_WGS), dim3(SPLIT_WG), 0, st, A);
-    else launch(paged_split_kernel<NB, RT, NARROW, false>, dim3(SPLIT_WGS), dim3(SPLIT_WG), 0, st, A);
-    launch(paged_join_kernel<NB, ROWS>, dim3(A.n_tokens, A.n_head), dim3(256), 0, st, A);
+    const dim3 grid(split_wgs(NARROW ? 4 : 16));
+    if (A.page % 16 == 0 && reach <= INT32_MAX) launch(paged_split_kernel<NB, NARROW, true>, grid, dim3(SPLIT_WG), 0, st, A);
+    else launch(paged_split_kernel<NB, NARROW, false>, grid, dim3(SPLIT_WG), 0, st, A);
 }
 
 template <int NB>
-void split_by_rows(const paged_attn & A, int rows, hipStream_t st) {
-    if (rows < 16) split<NB, 1, true>(A, st);
-    else if (rows == 16) split<NB, 1, false>(A, st);
-    else split<NB, 2, false>(A, st);
+void attend(const paged_attn & A, const paged_ways & W, hipStream_t st) {
+    constexpr int narrow = NB == 2 ? 8 : 4;
+    if (W.tile == 64) launch(paged_tile_kernel<NB, 1>, dim3(tile_wgs(64)), dim3(TILE_WG), 0, st, A);
+    else if (W.tile == 128) launch(paged_tile_kernel<NB, 2>, dim3(tile_wgs(128)), dim3(TILE_WG), 0, st, A);
+    if (W.split == narrow) split<NB, true>(A, st);
+    else if (W.split == 16) split<NB, false>(A, st);
+    const dim3 grid(A.n_tokens, A.n_head);
+    if (W.tile && (int64_t) A.n_tokens * A.n_head > 4096) {
+        // (a row's workgroup takes 2 us even where it finds nothing to join)
+        if (W.tile == 64) launch(paged_join_teams_kernel<NB, 0, 64>, dim3(A.tile_teams, 2), dim3(256), 0, st, A);
+        else launch(paged_join_teams_kernel<NB, 0, 128>, dim3(A.tile_teams, 4), dim3(256), 0, st, A);
+        if (W.split) launch(paged_join_teams_kernel<NB, 16, 0>, dim3(A.teams, A.team), dim3(256), 0, st, A);
+        return;
+    }
+    if (W.split == narrow) launch(paged_join_kernel<NB, narrow, 0>, grid, dim3(256), 0, st, A);
+    else if (!W.tile) launch(paged_join_kernel<NB, 16, 0>, grid, dim3(256), 0, st, A);
+    else if (W.tile == 64) launch(paged_join_kernel<NB, 0, 64>, grid, dim3(256), 0, st, A);
+    else if (W.split) launch(paged_join_kernel<NB, 16, 128>, grid, dim3(256), 0, st, A);
+    else launch(paged_join_kernel<NB, 0, 128>, grid, dim3(256), 0, st, A);
 }
+
+// rows of parts: two a team of waves, or a workgroup
+int64_t split_rows(const paged_ways & W) { return W.split ? (int64_t) split_wgs(W.split) * (SPLIT_WG / WAVE) * 2 * W.split : 0; }
+int64_t tile_rows(const paged_ways & W) { return W.tile ? (int64_t) tile_wgs(W.tile) * 2 * W.tile : 0; }
 
 } // namespace
 
-// parts: two a wave
 int64_t paged_attn_scratch_bytes(const paged_attn & A) {
     if (A.n_tokens == 0 || A.n_seqs == 0 || A.n_head == 0) return 0;
-    const int64_t rows = (int64_t) SPLIT_WGS * (SPLIT_WG / WAVE) * 2 * split_rows(A);
-    return rows * (A.D * 4 + 8);
+    const paged_ways W = ways_of(A);
+    return (split_rows(W) + tile_rows(W)) * (A.D * 4 + 8);
 }
 
 void launch_paged_attn(paged_attn A, hipStream_t st) {
     if (A.n_tokens == 0 || A.n_seqs == 0 || A.n_head == 0) return;
+    const paged_ways W = ways_of(A);
     A.team = A.n_head_kv % 4 == 0 ? 4 : A.n_head_kv % 2 == 0 ? 2 : 1;
     A.team_bits = A.team / 2;
     A.head_teams = A.n_head_kv / A.team;
-    A.teams = SPLIT_WGS * (SPLIT_WG / WAVE) / A.team;
+    A.teams = W.split ? split_wgs(W.split) * (SPLIT_WG / WAVE) / A.team : 0;
+    A.tile_teams = W.tile ? tile_wgs(W.tile) : 0;
+    A.split_most = W.tile ? 16 : INT32_MAX;
+    A.tile_least = W.split ? 17 : 0;
     // pos / page as a product: exact below 2^31 (the multiplier is rounded up, by less than 2^-31 of it)
     int bits = 0;
     while ((1ll << bits) < A.page) bits++;
     A.page_shift = (1ll << bits) == A.page ? bits : bits - 1;
     A.page_mul = (1ll << bits) == A.page ? 0 : (uint32_t) (((uint64_t) 1 << (31 + bits)) / A.page + 1);
-    const int rows = split_rows(A);
     A.part = (float *) A.scratch;
-    A.part_ml = (float2 *) (A.part + (int64_t) A.teams * A.team * 2 * rows * A.D);
-    if (A.D == 64) split_by_rows<2>(A, rows, st);
-    else if (A.D == 96) split_by_rows<3>(A, rows, st);
-    else if (A.D == 128) split_by_rows<4>(A, rows, st);
+    A.part_ml = (float2 *) (A.part + split_rows(W) * A.D);
+    A.tile_part = (float *) (A.part_ml + split_rows(W));
+    A.tile_ml = (float2 *) (A.tile_part + tile_rows(W) * A.D);
+    if (A.D == 64) attend<2>(A, W, st);
+    else if (A.D == 96) attend<3>(A, W, st);
+    else if (A.D == 128) attend<4>(A, W, st);
     else HIP_ABORT("flash_attn_paged: heads of %d values", A.D);
 }

@@ -430,10 +430,10 @@ struct paged_attn {
     float scale;
     void * scratch;                  // paged_attn_scratch_bytes
     // set by launch_paged_attn
-    int team, team_bits, head_teams, teams, page_shift;
+    int team, team_bits, head_teams, teams, tile_teams, split_most, tile_least, page_shift;
     uint32_t page_mul;
-    float * part;
-    float2 * part_ml;
+    float * part, * tile_part;
+    float2 * part_ml, * tile_ml;
 };
 // Drafted tokens against probabilities (ggml_backend_hip_verify): rows as ggml row indices over ne[1..3]
 constexpr int VERIFY_SEGMENT = 2048;
