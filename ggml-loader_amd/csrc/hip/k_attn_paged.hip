@@ -27,7 +27,7 @@ typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
 constexpr int STEP = 32;               // positions of a step, few rows
 constexpr int TILE_STEP = 64;          // and many
-constexpr int SPLIT_WG = 256, TILE_WG = 256;
+constexpr int SPLIT_WG = 256;
 constexpr float M_NONE = -1.7e38f;     // the maximum of no scores: finite, so that differences are no NaN
 
 // a value that every lane holds, as a scalar
@@ -371,7 +371,7 @@ __global__ __launch_bounds__(SPLIT_WG, NARROW ? 3 : 2) void paged_split_kernel(c
             // rows that are not there see what the last one sees
             lim[t] = min(Q.last - (Q.n - 1) + (real ? i : Q.n - 1), Q.len - 1);
             float big = 0.0f;
-            auto values = [&](int b, float (&v)[8]) {
+            auto values_of = [&](int b, float (&v)[8]) {
                 const float4 lo = load4(q + 32 * b + 4 * c), hi = load4(q + 32 * b + 16 + 4 * c);
                 const float w[8] = { lo.x, lo.z, hi.x, hi.z, lo.y, lo.w, hi.y, hi.w };
 #pragma unroll
@@ -381,7 +381,7 @@ __global__ __launch_bounds__(SPLIT_WG, NARROW ? 3 : 2) void paged_split_kernel(c
             float v[8];
 #pragma unroll
             for (int b = 0; b < QB; b++) {
-                values(NARROW ? own : b, v);
+                values_of(NARROW ? own : b, v);
 #pragma unroll
                 for (int k = 0; k < 8; k++) big = fmaxf(big, fabsf(v[k]));
             }
@@ -401,7 +401,7 @@ __global__ __launch_bounds__(SPLIT_WG, NARROW ? 3 : 2) void paged_split_kernel(c
             const float sign = A.scale < 0.0f ? -1.0f : 1.0f;       // the factor of the sums is not negative
 #pragma unroll
             for (int b = 0; b < QB; b++) {
-                if (!NARROW) values(b, v);
+                if (!NARROW) values_of(b, v);
 #pragma unroll
                 for (int k = 0; k < 8; k++) {
                     const float x = __builtin_amdgcn_ldexpf(v[k] * sign, e);
@@ -626,16 +626,16 @@ __global__ __launch_bounds__(SPLIT_WG, NARROW ? 3 : 2) void paged_split_kernel(c
     }
 }
 
-// ---- many rows a sequence: four waves share a step's operands ----
+// ---- many rows a sequence: the waves of a workgroup share a step's operands ----
 //
-// A workgroup takes 64 RT rows of one KV head, a wave 16 RT of them, in steps of 64 positions. Wave b decodes block b of the
-// step's keys and values for all four: codes - 8 of K as A wants them, and V's values d (codes - 8) as two halves
-// (15 bits: exactly), so that p is split once for all blocks (three products: hi hi, lo hi, hi lo). V's scales are
-// taken times 2^s of each block, so that the largest so far is at 2^11 to 2^12; a scale that is not finite counts as 0, and
-// makes the results of the rows that see it NaN.
-template <int NB, int RT>
-__global__ __launch_bounds__(TILE_WG, RT == 1 ? 3 : 2) void paged_tile_kernel(const paged_attn args) {
-    constexpr int D = NB * 32, ROWS = 64 * RT;
+// A workgroup takes 64 or 128 rows of one KV head, a wave 16 of them, in steps of 64 positions. Each wave decodes a block of
+// the step's keys or values (of four waves, both) for all: codes - 8 of K as A wants them, and V's values
+// d (codes - 8) as two halves (15 bits: exactly), so that p is split once for all blocks (three products: hi hi,
+// lo hi, hi lo). V's scales are taken times 2^s of each block, so that the largest so far is at 2^11 to 2^12; a scale that
+// is not finite counts as 0, and makes the results of the rows that see it NaN.
+template <int NB, int WAVES>
+__global__ __launch_bounds__(WAVES * WAVE, WAVES == 8 ? 4 : 3) void paged_tile_kernel(const paged_attn args) {
+    constexpr int D = NB * 32, RT = 1, ROWS = 16 * WAVES;
     constexpr int SROW = TILE_STEP + 4;
     __shared__ __align__(16) u4 s_k[NB][4][WAVE];             // block, sixteen of positions, lane
     __shared__ __align__(16) u4 s_v[NB][2][2][2][WAVE];       // block, 32 positions, half of the block, hi and lo, lane
@@ -647,6 +647,11 @@ __global__ __launch_bounds__(TILE_WG, RT == 1 ? 3 : 2) void paged_tile_kernel(co
     const int lane = threadIdx.x % WAVE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
     const int col = lane % 16, c = lane / 16;
     const code_bits K;
+    const int block = wave & 3;                               // the wave's block: of K, of V, or of both
+    const bool keys = wave < NB, values = (WAVES == 4 ? wave : wave - 4) >= 0 && block < NB && (WAVES == 4 || wave >= 4);
+    const bool decodes = keys || values;
+    float one = 1.0f;                                         // a product with it takes an F16 operand as it is
+    asm("" : "+v"(one));
 
     plan P;
     int seq = 0;
@@ -707,28 +712,34 @@ __global__ __launch_bounds__(TILE_WG, RT == 1 ? 3 : 2) void paged_tile_kernel(co
 
         // ---- the step's operands: lane l of wave b takes block b of position l ----
         const int32_t * table = A.pages + (int64_t) seq * A.pages_s;
-        const int64_t k_first = (int64_t) head * A.k_head + wave, v_first = (int64_t) head * A.v_head + wave;
+        const int64_t k_first = (int64_t) head * A.k_head + block, v_first = (int64_t) head * A.v_head + block;
         const int n_pages = (int) min(A.n_pages, (int64_t) INT32_MAX), rows_page = A.page;
         const int64_t k_page = A.k_page, k_pos = A.k_pos, v_page = A.v_page, v_pos = A.v_pos;
-        const bool decodes = wave < NB;
         int page = -1;
         auto page_of = [&](int step) {
             const int pos = step * TILE_STEP + lane;
             page = decodes && pos < Q.len && step < step1 ? table[page_index(A, pos)] : -1;
         };
-        u4 kraw, vraw;
-        _Float16 kd, vd;
+        // (of eight waves, none has both)
+        u4 raw[WAVES == 8 ? 1 : 2];
+        uint16_t rd[WAVES == 8 ? 1 : 2];
+        u4 & kraw = raw[0], & vraw = raw[WAVES == 8 ? 0 : 1];
+        uint16_t & kd = rd[0], & vd = rd[WAVES == 8 ? 0 : 1];
         bool there;
         auto load = [&](int step) {
             const int pos = step * TILE_STEP + lane;
             there = page >= 0 && page < n_pages;
             const int off = pos - page_index(A, pos) * rows_page;
-            const int64_t kb = k_first + (there ? (int64_t) page * k_page + (int64_t) off * k_pos : 0);
-            const int64_t vb = v_first + (there ? (int64_t) page * v_page + (int64_t) off * v_pos : 0);
-            kraw = *(const u4 *) (A.kq + kb * 16);
-            vraw = *(const u4 *) (A.vq + vb * 16);
-            kd = ((const _Float16 *) A.kd)[kb];
-            vd = ((const _Float16 *) A.vd)[vb];
+            if (keys) {
+                const int64_t at = k_first + (there ? (int64_t) page * k_page + (int64_t) off * k_pos : 0);
+                kraw = *(const u4 *) (A.kq + at * 16);
+                kd = ((const uint16_t *) A.kd)[at];
+            }
+            if (values) {
+                const int64_t at = v_first + (there ? (int64_t) page * v_page + (int64_t) off * v_pos : 0);
+                vraw = *(const u4 *) (A.vq + at * 16);
+                vd = ((const uint16_t *) A.vd)[at];
+            }
         };
         page_of(step0);
 
@@ -785,37 +796,41 @@ __global__ __launch_bounds__(TILE_WG, RT == 1 ? 3 : 2) void paged_tile_kernel(co
 
         for (int step = step0; step < step1; step++) {
             __syncthreads();                              // the operands before these are read
-            if (decodes) {
-                const bool finite = fabsf((float) vd) < INFINITY;
-                const float dv = there && finite ? fabsf((float) vd) : 0.0f;
+            if (keys) {
+                s_kd[block][lane] = there ? (float) __builtin_bit_cast(_Float16, kd) : 0.0f;
+#pragma unroll
+                for (int k = 0; k < 4; k++) s_k[block][lane / 16][k * 16 + col] = __builtin_bit_cast(u4, signed_of(kraw[k], K));
+                const uint64_t gone = __ballot(step * TILE_STEP + lane < Q.len && !there);
+                if (wave == 0 && lane == 0) s_gone = gone;
+            }
+            if (values) {
+                const float dr = (float) __builtin_bit_cast(_Float16, vd);
+                const bool finite = fabsf(dr) < INFINITY;
+                const float dv = there && finite ? fabsf(dr) : 0.0f;
                 if (__any(dv >= __builtin_amdgcn_ldexpf(1.0f, 12 - own_shift))) {
                     const float big = wave_max(dv);
                     own_shift = min(own_shift, 12 - __builtin_amdgcn_frexp_expf(big));
                 }
-                s_kd[wave][lane] = there ? (float) kd : 0.0f;
                 // scales of positions 16 t + 4 c + r side by side over t
-                s_vd[wave][(lane & 32) + ((lane >> 2) & 3) * 8 + (lane & 3) * 2 + ((lane >> 4) & 1)] =
-                    there && finite ? (_Float16) __builtin_amdgcn_ldexpf((float) vd, own_shift) : (_Float16) 0.0f;
-                const uint64_t odd = __ballot(there && !finite), gone = __ballot(step * TILE_STEP + lane < Q.len && !there);
+                s_vd[block][(lane & 32) + ((lane >> 2) & 3) * 8 + (lane & 3) * 2 + ((lane >> 4) & 1)] =
+                    there && finite ? (_Float16) __builtin_amdgcn_ldexpf(dr, own_shift) : (_Float16) 0.0f;
+                const uint64_t odd = __ballot(there && !finite);
                 if (lane == 0) {
-                    s_shift[wave] = own_shift;
-                    s_odd[wave] = odd;
-                    if (wave == 0) s_gone = gone;
+                    s_shift[block] = own_shift;
+                    s_odd[block] = odd;
                 }
                 // V's bytes where its values will be, read again by the transposing read
-                uint8_t * raw = (uint8_t *) &s_v[wave][0][0][0][0];
-                *(u4 *) (raw + lane * 16) = vraw;
-#pragma unroll
-                for (int k = 0; k < 4; k++) s_k[wave][lane / 16][k * 16 + col] = __builtin_bit_cast(u4, signed_of(kraw[k], K));
+                uint8_t * bytes = (uint8_t *) &s_v[block][0][0][0][0];
+                *(u4 *) (bytes + lane * 16) = vraw;
                 i2 codes[2];
 #pragma unroll
                 for (int hs = 0; hs < 2; hs++) {
                     codes[hs] = __builtin_amdgcn_ds_read_tr4_b64_v2i32(
-                        (__attribute__((address_space(3))) i2 *) (raw + (32 * hs + 16 * ((col >> 2) & 1) + 4 * c + (col & 3)) * 16 + (col >> 3) * 8));
+                        (__attribute__((address_space(3))) i2 *) (bytes + (32 * hs + 16 * ((col >> 2) & 1) + 4 * c + (col & 3)) * 16 + (col >> 3) * 8));
                 }
                 u4 d[2];
 #pragma unroll
-                for (int hs = 0; hs < 2; hs++) d[hs] = *(const u4 *) &s_vd[wave][32 * hs + c * 8];
+                for (int hs = 0; hs < 2; hs++) d[hs] = *(const u4 *) &s_vd[block][32 * hs + c * 8];
                 // (these reads are before the writes: one wave's LDS operations keep their order)
 #pragma unroll
                 for (int hs = 0; hs < 2; hs++) {
@@ -823,23 +838,24 @@ __global__ __launch_bounds__(TILE_WG, RT == 1 ? 3 : 2) void paged_tile_kernel(co
                     for (int h = 0; h < 2; h++) {
                         const h8 a = signed_of(codes[hs][h], K), dd = __builtin_bit_cast(h8, d[hs]);
                         const h8 hi = a * dd, lo = __builtin_elementwise_fma(a, dd, -hi);
-                        s_v[wave][hs][h][0][lane] = __builtin_bit_cast(u4, hi);
-                        s_v[wave][hs][h][1][lane] = __builtin_bit_cast(u4, lo);
+                        s_v[block][hs][h][0][lane] = __builtin_bit_cast(u4, hi);
+                        s_v[block][hs][h][1][lane] = __builtin_bit_cast(u4, lo);
                     }
                 }
-                if (step + 1 < step1) {
-                    load(step + 1);
-                    page_of(step + 2);
-                }
+            }
+            if (decodes && step + 1 < step1) {
+                load(step + 1);
+                page_of(step + 2);
             }
             __syncthreads();                              // the step's operands are there
 
+            if (first_row >= Q.n * A.group) continue;     // no rows: the wave only decodes
             uint64_t odd = 0;
 #pragma unroll
             for (int b = 0; b < NB; b++) {
-                odd |= s_odd[b];
-                const int now = s_shift[b];
-                if (__any(now != shift[b])) {
+                odd |= (uint64_t) uniform((int64_t) s_odd[b]);
+                const int now = uniform(s_shift[b]);
+                if (now != shift[b]) {
                     const float keep = __builtin_amdgcn_ldexpf(1.0f, now - shift[b]);
                     shift[b] = now;
 #pragma unroll
@@ -852,6 +868,7 @@ __global__ __launch_bounds__(TILE_WG, RT == 1 ? 3 : 2) void paged_tile_kernel(co
                 f4 s[RT][2];
 #pragma unroll
                 for (int t = 0; t < 2; t++) {
+                    __builtin_amdgcn_sched_barrier(0);       // (16 reads at once would not leave their registers)
 #pragma unroll
                     for (int b = 0; b < NB; b++) {
                         const h8 a = __builtin_bit_cast(h8, s_k[b][2 * hs + t][lane]);
@@ -867,7 +884,7 @@ __global__ __launch_bounds__(TILE_WG, RT == 1 ? 3 : 2) void paged_tile_kernel(co
                     }
                 }
                 // positions on missing pages have scales of 0 but scores all the same: their rows' bits
-                const uint32_t missing = (uint32_t) (s_gone >> (32 * hs));
+                const uint32_t missing = (uint32_t) ((uint64_t) uniform((int64_t) s_gone) >> (32 * hs));
                 const bool edge = at + 31 > sure || missing;
                 uint32_t hidden[RT];
                 h8 ph[RT], pl[RT];
@@ -921,7 +938,7 @@ __global__ __launch_bounds__(TILE_WG, RT == 1 ? 3 : 2) void paged_tile_kernel(co
 #pragma unroll
                         for (int t = 0; t < 2; t++) {
                             ph[x][2 * i + t] = (_Float16) s[x][t][i];
-                            pl[x][2 * i + t] = (_Float16) (s[x][t][i] - (float) ph[x][2 * i + t]);
+                            pl[x][2 * i + t] = (_Float16) fmaf(s[x][t][i], one, -(float) ph[x][2 * i + t]);
                         }
                     }
                 }
@@ -944,6 +961,7 @@ __global__ __launch_bounds__(TILE_WG, RT == 1 ? 3 : 2) void paged_tile_kernel(co
                 }
 #pragma unroll
                 for (int b = 0; b < NB; b++) {
+                    if (b == 2) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                     for (int h = 0; h < 2; h++) {
                         const h8 hi = __builtin_bit_cast(h8, s_v[b][hs][h][0][lane]), lo = __builtin_bit_cast(h8, s_v[b][hs][h][1][lane]);
@@ -1201,7 +1219,7 @@ paged_ways ways_of(const paged_attn & A) {
     if (rows <= 64 * per) return { 0, 64 };
     return { per > 1 ? 16 : 0, 128 };
 }
-// workgroups of four waves that a CU holds: more would run behind the first
+// workgroups that the CUs hold at once: more would run behind the first
 int split_wgs(int rows) { return rows < 16 ? 768 : 512; }
 int tile_wgs(int rows) { return rows == 64 ? 768 : 512; }
 
@@ -1217,8 +1235,8 @@ void split(const paged_attn & A, hipStream_t st) {
 template <int NB>
 void attend(const paged_attn & A, const paged_ways & W, hipStream_t st) {
     constexpr int narrow = NB == 2 ? 8 : 4;
-    if (W.tile == 64) launch(paged_tile_kernel<NB, 1>, dim3(tile_wgs(64)), dim3(TILE_WG), 0, st, A);
-    else if (W.tile == 128) launch(paged_tile_kernel<NB, 2>, dim3(tile_wgs(128)), dim3(TILE_WG), 0, st, A);
+    if (W.tile == 64) launch(paged_tile_kernel<NB, 4>, dim3(tile_wgs(64)), dim3(4 * WAVE), 0, st, A);
+    else if (W.tile == 128) launch(paged_tile_kernel<NB, 8>, dim3(tile_wgs(128)), dim3(8 * WAVE), 0, st, A);
     if (W.split == narrow) split<NB, true>(A, st);
     else if (W.split == 16) split<NB, false>(A, st);
     const dim3 grid(A.n_tokens, A.n_head);
