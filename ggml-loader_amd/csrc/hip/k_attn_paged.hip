@@ -29,6 +29,10 @@ constexpr int STEP = 32;               // positions of a step, few rows
 constexpr int TILE_STEP = 64;          // and many
 constexpr int SPLIT_WG = 256;
 constexpr float M_NONE = -1.7e38f;     // the maximum of no scores: finite, so that differences are no NaN
+// The maximum that p = 2^(z - m) goes by follows the scores only where they pass it by 2^SLACK: with 16 rows, one of them
+// finds a new maximum in every second step, but such a one in every twentieth. What p's halves lose by it is their
+// range, from below 2^-38 of the largest to below 2^-34.
+constexpr int SLACK = 4;
 
 // a value that every lane holds, as a scalar
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
@@ -415,7 +419,7 @@ __global__ __launch_bounds__(SPLIT_WG, NARROW ? 3 : 2) void paged_split_kernel(c
 #pragma unroll
             for (int b = 0; b < NB; b++) o[t][b][0] = o[t][b][1] = f4{ 0, 0, 0, 0 };
         }
-        // p d is formed times 2^shift, so that the largest scale seen gives 2^14 to 2^15
+        // p d is formed times 2^shift, so that the largest scale seen gives 2^13 to 2^15 times the largest p
         int shift = 38;
         const int sure = Q.last - (Q.n - 1) + tile * ROWS / A.group;        // positions up to here are seen by all rows
 
@@ -492,9 +496,9 @@ __global__ __launch_bounds__(SPLIT_WG, NARROW ? 3 : 2) void paged_split_kernel(c
             }
             if (!P16) page_of(step + 2);
             // the largest scale of V so far
-            if (__any(dmax >= __builtin_amdgcn_ldexpf(1.0f, 15 - shift))) {
+            if (__any(dmax >= __builtin_amdgcn_ldexpf(1.0f, 15 - SLACK - shift))) {
                 const float big = wave_max(dmax);
-                const int now = min(shift, 14 - min(max(__builtin_amdgcn_frexp_expf(big < 65536.0f ? big : 65504.0f), -24), 16));
+                const int now = min(shift, 14 - SLACK - min(max(__builtin_amdgcn_frexp_expf(big < 65536.0f ? big : 65504.0f), -24), 16));
                 const float keep = __builtin_amdgcn_ldexpf(1.0f, now - shift);
                 shift = now;
 #pragma unroll
@@ -528,9 +532,9 @@ __global__ __launch_bounds__(SPLIT_WG, NARROW ? 3 : 2) void paged_split_kernel(c
 #pragma unroll
                     for (int i = 0; i < 4; i++) top = fmaxf(top, s[x][t][i]);
                 }
-                top = column_max(top) * fac[x];
-                if (__any(top > m[x])) {
-                    const float now = fmaxf(m[x], top), keep = exp2_hw(m[x] - now);
+                if (__any(top * fac[x] > m[x] + SLACK)) {
+                    top = column_max(top) * fac[x];
+                    const float now = top > m[x] + SLACK ? top : m[x], keep = exp2_hw(m[x] - now);
                     m[x] = now;
                     l[x] *= keep;
 #pragma unroll
@@ -636,7 +640,7 @@ __global__ __launch_bounds__(SPLIT_WG, NARROW ? 3 : 2) void paged_split_kernel(c
 template <int NB, int WAVES>
 __global__ __launch_bounds__(WAVES * WAVE, WAVES == 8 ? 4 : 3) void paged_tile_kernel(const paged_attn args) {
     constexpr int D = NB * 32, RT = 1, ROWS = 16 * WAVES;
-    constexpr int SROW = TILE_STEP + 4;
+    constexpr int SROW = TILE_STEP + 4, P_UP = 15 - SLACK;
     __shared__ __align__(16) u4 s_k[NB][4][WAVE];             // block, sixteen of positions, lane
     __shared__ __align__(16) u4 s_v[NB][2][2][2][WAVE];       // block, 32 positions, half of the block, hi and lo, lane
     __shared__ __align__(16) float s_kd[NB][SROW];
@@ -730,13 +734,18 @@ __global__ __launch_bounds__(WAVES * WAVE, WAVES == 8 ? 4 : 3) void paged_tile_k
             const int pos = step * TILE_STEP + lane;
             there = page >= 0 && page < n_pages;
             const int off = pos - page_index(A, pos) * rows_page;
+            // (a cache of 2^32 blocks is 64 GiB)
+            auto row = [&](int64_t per_page, int64_t per_pos) {
+                if (A.rows32) return (int64_t) (there ? (uint32_t) page * (uint32_t) per_page + (uint32_t) off * (uint32_t) per_pos : 0);
+                return there ? (int64_t) page * per_page + (int64_t) off * per_pos : 0;
+            };
             if (keys) {
-                const int64_t at = k_first + (there ? (int64_t) page * k_page + (int64_t) off * k_pos : 0);
+                const int64_t at = k_first + row(k_page, k_pos);
                 kraw = *(const u4 *) (A.kq + at * 16);
                 kd = ((const uint16_t *) A.kd)[at];
             }
             if (values) {
-                const int64_t at = v_first + (there ? (int64_t) page * v_page + (int64_t) off * v_pos : 0);
+                const int64_t at = v_first + row(v_page, v_pos);
                 vraw = *(const u4 *) (A.vq + at * 16);
                 vd = ((const uint16_t *) A.vd)[at];
             }
@@ -910,16 +919,16 @@ __global__ __launch_bounds__(WAVES * WAVE, WAVES == 8 ? 4 : 3) void paged_tile_k
 #pragma unroll
                         for (int i = 0; i < 4; i++) top = fmaxf(top, s[x][t][i]);
                     }
-                    top = column_max(top) * fac[x];
-                    if (__any(top > m[x])) {
-                        const float now = fmaxf(m[x], top), keep = exp2_hw(m[x] - now);
+                    if (__any(top * fac[x] > m[x] + SLACK)) {
+                        top = column_max(top) * fac[x];
+                        const float now = top > m[x] + SLACK ? top : m[x], keep = exp2_hw(m[x] - now);
                         m[x] = now;
                         l[x] *= keep;
 #pragma unroll
                         for (int b = 0; b < NB; b++) { o[x][b][0] *= keep; o[x][b][1] *= keep; }
                     }
-                    // p times 2^15
-                    const float up = 15.0f - m[x];
+                    // p times 2^P_UP, so that the largest is below 2^15
+                    const float up = (float) P_UP - m[x];
 #pragma unroll
                     for (int t = 0; t < 2; t++) {
 #pragma unroll
@@ -982,7 +991,7 @@ __global__ __launch_bounds__(WAVES * WAVE, WAVES == 8 ? 4 : 3) void paged_tile_k
 #pragma unroll
         for (int x = 0; x < RT; x++) {
             const int at_row = (wave * RT + x) * 16 + col, row = tile * ROWS + at_row;
-            const float sum = column_sum(l[x]) * 0x1p-15f;
+            const float sum = __builtin_amdgcn_ldexpf(column_sum(l[x]), -P_UP);
             if (row >= Q.n * A.group) continue;
             const int i = row / A.group, g = row - i * A.group;
             const float inv = whole ? (sum > 0.0f ? 1.0f / sum : sum == 0.0f ? 0.0f : sum) : 1.0f;
@@ -990,8 +999,8 @@ __global__ __launch_bounds__(WAVES * WAVE, WAVES == 8 ? 4 : 3) void paged_tile_k
                                 : A.tile_part + (slot + at_row) * D;
 #pragma unroll
             for (int b = 0; b < NB; b++) {
-                // (in two steps: 2^-(15 + shift) may be below the range where inv is large)
-                const float w = __builtin_amdgcn_ldexpf(inv, -15);
+                // (in two steps: 2^-(P_UP + shift) may be below the range where inv is large)
+                const float w = __builtin_amdgcn_ldexpf(inv, -P_UP);
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
                     float r[4];
@@ -1225,10 +1234,10 @@ int tile_wgs(int rows) { return rows == 64 ? 768 : 512; }
 
 template <int NB, bool NARROW>
 void split(const paged_attn & A, hipStream_t st) {
-    // a sixteen of positions on one page, its rows within 32-bit offsets, and a row's number within 32 bits
-    const int64_t reach = std::max(std::max(16 * 16 * std::max(A.k_pos, A.v_pos), std::max(A.k_page, A.v_page)), (A.n_pages * std::max(A.k_page, A.v_page) + 1) / 2);
+    // a sixteen of positions on one page, its rows within 32-bit offsets
+    const int64_t reach = 16 * 16 * std::max(A.k_pos, A.v_pos);
     const dim3 grid(split_wgs(NARROW ? 4 : 16));
-    if (A.page % 16 == 0 && reach <= INT32_MAX) launch(paged_split_kernel<NB, NARROW, true>, grid, dim3(SPLIT_WG), 0, st, A);
+    if (A.page % 16 == 0 && A.rows32 && reach <= INT32_MAX) launch(paged_split_kernel<NB, NARROW, true>, grid, dim3(SPLIT_WG), 0, st, A);
     else launch(paged_split_kernel<NB, NARROW, false>, grid, dim3(SPLIT_WG), 0, st, A);
 }
 
@@ -1276,6 +1285,9 @@ void launch_paged_attn(paged_attn A, hipStream_t st) {
     A.tile_teams = W.tile ? tile_wgs(W.tile) : 0;
     A.split_most = W.tile ? 16 : INT32_MAX;
     A.tile_least = W.split ? 17 : 0;
+    // a row's first block as a 32-bit number
+    const int64_t most = std::max({ A.k_page, A.v_page, A.k_pos * A.page, A.v_pos * A.page });
+    A.rows32 = most <= UINT32_MAX && A.n_pages <= (int64_t) UINT32_MAX / std::max<int64_t>(most, 1) - 1;
     // pos / page as a product: exact below 2^31 (the multiplier is rounded up, by less than 2^-31 of it)
     int bits = 0;
     while ((1ll << bits) < A.page) bits++;

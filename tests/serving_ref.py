@@ -65,9 +65,11 @@ def attention(q, k, v, pages, q_start, kv_len, scale):
     block, its scale) are off by less than 8 units of 32 bits of sum |q k|, and so is log2(e) times them; p = e^(s - m)
     is off by that and by 2 units more; a term p v by 4 (p d in two halves of 11 bits); sums in parts of at most 64 terms,
     then joined, by 64 + 40. Numerator and denominator both: 2 max_j(8 scale sum |q k| + 2) + 2 (4 + 104) units of
-    sum p |v| / sum p. What is absolute: p below 2^-126 ends the range of 32-bit floats, and a p d in two halves of 11
-    bits, scaled so that the largest is at 2^14, ends at 2^-25 (the smallest half), 2^-39 of the largest: each of the n
-    terms may lose 2^-38 max |v|, and sum p >= 1 divides it."""
+    sum p |v| / sum p. What is absolute: p below 2^-126 ends the range of 32-bit floats, and operands of the
+    products in two halves of 11 bits end at 2^-25, half the smallest F16. They are scaled so that the largest p (it may
+    be 2^4 times the one that is divided by) and the largest scale d make at most 2^15: where d's largest is at 2^9 or
+    more, a term p d c, |c| <= 8, may lose 2^-34 max |v|, max |v| = 8 max d, and a scale far below the largest of its kind
+    as much again: 2^-33 max |v| for each of the n terms, and sum p >= 1 divides it."""
     T, H, D = q.shape
     page, KV = k.shape[1:3]
     o, bound, listed = np.zeros(q.shape), np.zeros(q.shape), np.zeros(T, bool)
@@ -92,7 +94,7 @@ def attention(q, k, v, pages, q_start, kv_len, scale):
                 w = p / p.sum()
                 o[t, h] = w @ vh
                 most = (abs(scale) * (np.abs(kh) @ np.abs(qh))).max()
-                lost = see.sum() * 2.0 ** -38 * np.abs(vh).max()
+                lost = see.sum() * 2.0 ** -33 * np.abs(vv[see]).max()
                 bound[t, h] = U32 * (16 * most + 4 + 216) * (w @ np.abs(vh)) + lost
     return o, bound, listed
 
