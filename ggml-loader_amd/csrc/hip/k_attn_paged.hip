@@ -45,6 +45,12 @@ __device__ __forceinline__ int64_t from_lane(int64_t v, int l) {
     return (int64_t) (((uint64_t) hi << 32) | lo);
 }
 
+// x / d for 0 <= x < 2^31 as a product
+__device__ __forceinline__ int quotient(const paged_attn::divisor & d, int x) {
+    return d.mul ? (int) (__umulhi((uint32_t) x, d.mul) >> d.shift) : x >> d.shift;
+}
+__device__ __forceinline__ int page_index(const paged_attn & A, int pos) { return quotient(A.by_page, pos); }
+
 // ---- what each sequence asks for ----
 struct seq_info { int first, n, len, last; };   // tokens, positions in the table; the last token sees up to `last`
 
@@ -68,7 +74,7 @@ __device__ __forceinline__ int64_t split_units(const paged_attn & A, const seq_i
 
 // Many: of each tile, the steps that its last token sees.
 __device__ __forceinline__ int tile_steps(const paged_attn & A, const seq_info & q, int rows, int tile) {
-    const int i = min((int) (((int64_t) (tile + 1) * rows - 1) / A.group), q.n - 1);
+    const int i = min(quotient(A.by_group, (tile + 1) * rows - 1), q.n - 1);     // (rows are fewer than 2^30)
     const int sees = min(q.last - (q.n - 1) + i + 1, q.len);
     return max((sees + TILE_STEP - 1) / TILE_STEP, 1);
 }
@@ -118,9 +124,6 @@ struct plan {
     }
 };
 
-__device__ __forceinline__ int page_index(const paged_attn & A, int pos) {
-    return A.page_mul ? (int) (__umulhi((uint32_t) pos, A.page_mul) >> A.page_shift) : pos >> A.page_shift;
-}
 
 // ---- operands ----
 __device__ __forceinline__ h8 as_h8(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
@@ -370,7 +373,7 @@ __global__ __launch_bounds__(SPLIT_WG, NARROW ? 3 : 2) void paged_split_kernel(c
         for (int t = 0; t < RT; t++) {
             const int row = tile * ROWS + t * 16 + (NARROW ? col % COLS : col);
             const bool real = row < Q.n * A.group;
-            const int i = real ? row / A.group : 0, g = real ? row - i * A.group : 0;
+            const int i = real ? quotient(A.by_group, row) : 0, g = real ? row - i * A.group : 0;
             const float * q = A.q + (int64_t) (Q.first + i) * A.q_t + (int64_t) (head * A.group + g) * A.q_h;
             // rows that are not there see what the last one sees
             lim[t] = min(Q.last - (Q.n - 1) + (real ? i : Q.n - 1), Q.len - 1);
@@ -421,7 +424,7 @@ __global__ __launch_bounds__(SPLIT_WG, NARROW ? 3 : 2) void paged_split_kernel(c
         }
         // p d is formed times 2^shift, so that the largest scale seen gives 2^13 to 2^15 times the largest p
         int shift = 38;
-        const int sure = Q.last - (Q.n - 1) + tile * ROWS / A.group;        // positions up to here are seen by all rows
+        const int sure = Q.last - (Q.n - 1) + quotient(A.by_group, tile * ROWS);        // positions up to here are seen by all rows
 
         for (int step = step0; step < step1; step++) {
             const bool more = step + 1 < step1;
@@ -609,7 +612,7 @@ __global__ __launch_bounds__(SPLIT_WG, NARROW ? 3 : 2) void paged_split_kernel(c
             const int at_row = x * 16 + (NARROW ? col % COLS : col), row = tile * ROWS + at_row;
             const float sum = column_sum(l[x]);
             if (row >= Q.n * A.group || spare) continue;
-            const int i = row / A.group, g = row - i * A.group;
+            const int i = quotient(A.by_group, row), g = row - i * A.group;
             // no positions: 0; a NaN stays one
             const float inv = whole ? (sum > 0.0f ? 1.0f / sum : sum == 0.0f ? 0.0f : sum) : 1.0f;
             float * out = whole ? A.out + ((int64_t) (Q.first + i) * A.n_head + head * A.group + g) * D
@@ -761,7 +764,7 @@ __global__ __launch_bounds__(WAVES * WAVE, WAVES == 8 ? 4 : 3) void paged_tile_k
         for (int t = 0; t < RT; t++) {
             const int row = tile * ROWS + (wave * RT + t) * 16 + col;
             const bool real = row < Q.n * A.group;
-            const int i = real ? row / A.group : 0, g = real ? row - i * A.group : 0;
+            const int i = real ? quotient(A.by_group, row) : 0, g = real ? row - i * A.group : 0;
             const float * q = A.q + (int64_t) (Q.first + i) * A.q_t + (int64_t) (head * A.group + g) * A.q_h;
             lim[t] = min(Q.last - (Q.n - 1) + (real ? i : Q.n - 1), Q.len - 1);
             float v[NB][8], big = 0.0f;
@@ -798,7 +801,7 @@ __global__ __launch_bounds__(WAVES * WAVE, WAVES == 8 ? 4 : 3) void paged_tile_k
             for (int b = 0; b < NB; b++) o[t][b][0] = o[t][b][1] = f4{ 0, 0, 0, 0 };
         }
         const int first_row = tile * ROWS + wave * RT * 16;
-        const int sure = min(Q.last - (Q.n - 1) + min(first_row / A.group, Q.n - 1), Q.len - 1);
+        const int sure = min(Q.last - (Q.n - 1) + min(quotient(A.by_group, first_row), Q.n - 1), Q.len - 1);
         int own_shift = 38, shift[NB];
 #pragma unroll
         for (int b = 0; b < NB; b++) shift[b] = 38;
@@ -993,7 +996,7 @@ __global__ __launch_bounds__(WAVES * WAVE, WAVES == 8 ? 4 : 3) void paged_tile_k
             const int at_row = (wave * RT + x) * 16 + col, row = tile * ROWS + at_row;
             const float sum = __builtin_amdgcn_ldexpf(column_sum(l[x]), -P_UP);
             if (row >= Q.n * A.group) continue;
-            const int i = row / A.group, g = row - i * A.group;
+            const int i = quotient(A.by_group, row), g = row - i * A.group;
             const float inv = whole ? (sum > 0.0f ? 1.0f / sum : sum == 0.0f ? 0.0f : sum) : 1.0f;
             float * out = whole ? A.out + ((int64_t) (Q.first + i) * A.n_head + head * A.group + g) * D
                                 : A.tile_part + (slot + at_row) * D;
@@ -1124,7 +1127,7 @@ __global__ __launch_bounds__(256) void paged_join_teams_kernel(const paged_attn 
     for (int r = group + (SPLIT ? 0 : (int) blockIdx.y * GROUPS); group < GROUPS && r < rows; r += GROUPS * (SPLIT ? 1 : (int) gridDim.y)) {
         part_sum S;
         S.add(part, part_ml, [&](int64_t k) { return ((k * 2 + (k == me)) * team + in_team) * ROWS + r; }, D, e, me, last, 1);
-        const int row = tile * ROWS + r, i = row / A.group, g = row - i * A.group;
+        const int row = tile * ROWS + r, i = quotient(A.by_group, row), g = row - i * A.group;
         const float inv = S.l > 0.0f ? 1.0f / S.l : S.l == 0.0f ? 0.0f : S.l;
         *(float4 *) (A.out + ((int64_t) (Q.first + i) * A.n_head + head * A.group + g) * D + 4 * e) =
             make_float4(S.o.x * inv, S.o.y * inv, S.o.z * inv, S.o.w * inv);
@@ -1171,7 +1174,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const paged_attn args) 
     if (seq < 0) return;
     const seq_info Q = seq_of(A, seq);
     const bool tiled = TILE && (!SPLIT || (int64_t) Q.n * A.group >= A.tile_least);
-    const int kvh = head / A.group, row = (token - Q.first) * A.group + head - kvh * A.group;
+    const int kvh = quotient(A.by_group, head), row = (token - Q.first) * A.group + head - kvh * A.group;
     const int rows = tiled ? TILE : SPLIT, tile = row / rows, team = tiled ? 1 : A.team;
     plan P;
     P.deal(tiled ? all_t : all_s, tiled ? A.tile_teams : A.teams);
@@ -1251,8 +1254,8 @@ void attend(const paged_attn & A, const paged_ways & W, hipStream_t st) {
     const dim3 grid(A.n_tokens, A.n_head);
     if (W.tile && (int64_t) A.n_tokens * A.n_head > 4096) {
         // (a row's workgroup takes 2 us even where it finds nothing to join)
-        if (W.tile == 64) launch(paged_join_teams_kernel<NB, 0, 64>, dim3(A.tile_teams, 2), dim3(256), 0, st, A);
-        else launch(paged_join_teams_kernel<NB, 0, 128>, dim3(A.tile_teams, 4), dim3(256), 0, st, A);
+        if (W.tile == 64) launch(paged_join_teams_kernel<NB, 0, 64>, dim3(A.tile_teams, 4), dim3(256), 0, st, A);
+        else launch(paged_join_teams_kernel<NB, 0, 128>, dim3(A.tile_teams, 8), dim3(256), 0, st, A);
         if (W.split) launch(paged_join_teams_kernel<NB, 16, 0>, dim3(A.teams, A.team), dim3(256), 0, st, A);
         return;
     }
@@ -1288,11 +1291,15 @@ void launch_paged_attn(paged_attn A, hipStream_t st) {
     // a row's first block as a 32-bit number
     const int64_t most = std::max({ A.k_page, A.v_page, A.k_pos * A.page, A.v_pos * A.page });
     A.rows32 = most <= UINT32_MAX && A.n_pages <= (int64_t) UINT32_MAX / std::max<int64_t>(most, 1) - 1;
-    // pos / page as a product: exact below 2^31 (the multiplier is rounded up, by less than 2^-31 of it)
-    int bits = 0;
-    while ((1ll << bits) < A.page) bits++;
-    A.page_shift = (1ll << bits) == A.page ? bits : bits - 1;
-    A.page_mul = (1ll << bits) == A.page ? 0 : (uint32_t) (((uint64_t) 1 << (31 + bits)) / A.page + 1);
+    // exact below 2^31: the multiplier is rounded up, by less than 2^-31 of it
+    auto by = [](int d) {
+        int bits = 0;
+        while ((1ll << bits) < d) bits++;
+        const bool power = (1ll << bits) == d;
+        return paged_attn::divisor{ power ? 0 : (uint32_t) (((uint64_t) 1 << (31 + bits)) / d + 1), power ? bits : bits - 1 };
+    };
+    A.by_page = by(A.page);
+    A.by_group = by(A.group);
     A.part = (float *) A.scratch;
     A.part_ml = (float2 *) (A.part + split_rows(W) * A.D);
     A.tile_part = (float *) (A.part_ml + split_rows(W));

@@ -430,8 +430,8 @@ struct paged_attn {
     float scale;
     void * scratch;                  // paged_attn_scratch_bytes
     // set by launch_paged_attn
-    int team, team_bits, head_teams, teams, tile_teams, split_most, tile_least, rows32, page_shift;
-    uint32_t page_mul;
+    int team, team_bits, head_teams, teams, tile_teams, split_most, tile_least, rows32;
+    struct divisor { uint32_t mul; int shift; } by_page, by_group;
     float * part, * tile_part;
     float2 * part_ml, * tile_ml;
 };

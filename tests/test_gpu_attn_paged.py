@@ -102,6 +102,16 @@ def test_attention(hip, new, seen, H, KV, D, P):
     check(hip, draw(np.random.default_rng(sum(seen) + H + D), new, seen, H, KV, D, P))
 
 
+@pytest.mark.parametrize("new, seen, H, KV, D, P", [
+    ([300, 1, 40], [500, 300, 40], 32, 8, 64, 16), ([150, 2, 1, 1], [1100, 64, 700, 1], 32, 2, 128, 16), ([200], [200], 48, 16, 96, 10),
+    ([60, 50, 70], [64, 300, 70], 40, 40, 64, 64),
+])
+def test_attention_of_many_tokens(hip, new, seen, H, KV, D, P):
+    """Prompts' parts beside single tokens, joined by team."""
+    assert sum(new) * H > 4096
+    check(hip, draw(np.random.default_rng(sum(seen) + H + D), new, seen, H, KV, D, P))
+
+
 @pytest.mark.parametrize("order", ["heads", "odd"])
 @pytest.mark.parametrize("new, seen, D", [([1, 1], [90, 200], 128), ([6, 2], [70, 2], 96), ([80], [200], 64)])
 def test_attention_of_other_cache_layouts(hip, order, new, seen, D):
