@@ -38,6 +38,13 @@ __device__ __forceinline__ float rotated_f32(float a, float b, bool first, doubl
     return first ? a * c - b * s : a * s + b * c;
 }
 
+// a value's 16 bits as F16 or BF16
+__device__ __forceinline__ uint32_t bits16(int type, float v) {
+    if (type == GGML_TYPE_F16) return __half_as_ushort(__float2half_rn(as_f32(v)));
+    const uint32_t u = __float_as_uint(as_f32(v));
+    return (u & 0x7fffffffu) > 0x7f800000u ? (u >> 16) | 64u : (u + (0x7fffu + ((u >> 16) & 1u))) >> 16;
+}
+
 __device__ __forceinline__ int min8_dpp(int v) {
     v = min(v, dpp_i<0xB1>(v));
     v = min(v, dpp_i<0x4E>(v));
@@ -89,68 +96,68 @@ __device__ __forceinline__ void store_q8_0(const rows_job & J, int64_t block, co
     if (lane8 == 0) J.d[block] = nan ? __ushort_as_half(0x7e00) : __float2half_rn(as_f32(d));
 }
 
-__global__ __launch_bounds__(ROWS_WG) void rows_kernel(const rows_batch B) {
-    __shared__ double2 s_cs[ROWS_MAX_CS];
-    __shared__ int64_t s_at[ROWS_MAX_PER_WG];
-    __shared__ int s_dead[ROWS_MAX_PER_WG];
+// UNITS: pieces of 256 threads' values that a workgroup takes: of one row where rows are longer, else rows
+template <int UNITS>
+__global__ __launch_bounds__(ROWS_WG) void rows_kernel(const rows_batch args) {
+    __shared__ double2 s_cs[UNITS * ROWS_MAX_CS];
+    __shared__ int64_t s_at[UNITS * ROWS_MAX_PER_WG];
+    __shared__ int s_dead[UNITS * ROWS_MAX_PER_WG];
+    const rows_batch & B = kernargs_prefetched(args);
+    const int t = threadIdx.x;
     int j = 0;
 #pragma unroll
     for (int k = 1; k < ROWS_MAX_JOBS; k++) if (k < B.n_jobs && (int64_t) blockIdx.x >= B.job[k].first_wg) j = k;
     const rows_job & J = B.job[j];
-    const int t = threadIdx.x, wg = (int) (blockIdx.x - J.first_wg);
+    const int wg = (int) (blockIdx.x - J.first_wg);
     const int64_t i2 = blockIdx.y, i3 = blockIdx.z;
-    // the thread's row of the workgroup's, and its quad of values in it
-    int lr = 0, quad;
-    int64_t row0;
-    if (J.chunks > 1) {
-        row0 = wg / J.chunks;
-        quad = (wg % J.chunks) * ROWS_WG + t;
-    } else {
-        row0 = (int64_t) wg * J.per_wg;
-        lr = t / J.threads;
-        quad = t % J.threads;
-    }
-    const int n_rows = (int) min((int64_t) J.per_wg, J.rows - row0);
-    const int64_t row = J.row0 + row0 + min(lr, n_rows - 1);
-    const bool mine = lr < n_rows && quad * 4 < J.width;
-    const int e0 = mine ? quad * 4 : 0;
-
-    // the row's values, and the other values of their pairs
-    const char * src = J.src + row * J.s1 + i2 * J.s2 + i3 * J.s3;
-    const int head = e0 / J.head, w0 = e0 - head * J.head;
-    const float * x = (const float *) (src + head * J.s_head);
-    float own[4], other[4] = { 0, 0, 0, 0 };
-    const int n = min(4, J.width - e0);
+    // the workgroup's rows, and the thread's row and quad of values of each unit
+    const bool pieces = J.chunks > 1;
+    const int parts = (J.chunks + UNITS - 1) / UNITS, per = pieces ? 1 : UNITS * J.per_wg;
+    const int64_t row0 = pieces ? wg / parts : (int64_t) wg * per;
+    const int n_rows = (int) min((int64_t) per, J.rows - row0);
+    const int chunk0 = pieces ? (wg - (int) row0 * parts) * UNITS : 0, lr0 = pieces ? 0 : t / J.threads, quad0 = pieces ? t : t - lr0 * J.threads;
     const bool apart = J.rope && J.dist > 1;                      // pairs (i, i + dist), else neighbours
-    if (J.quads) {
-        const float4 a = load4(x + w0);
-        own[0] = a.x; own[1] = a.y; own[2] = a.z; own[3] = a.w;
-        if (apart && w0 < 2 * J.pairs) {
-            const float4 b = load4(x + (w0 < J.pairs ? w0 + J.dist : w0 - J.dist));
-            other[0] = b.x; other[1] = b.y; other[2] = b.z; other[3] = b.w;
-        }
-    } else {
+    auto row_of = [&](int u) { return pieces ? 0 : lr0 < J.per_wg ? u * J.per_wg + lr0 : n_rows; };
+    auto quad_of = [&](int u) { return pieces ? (chunk0 + u) * ROWS_WG + t : quad0; };
+    auto mine_of = [&](int u) { return row_of(u) < n_rows && quad_of(u) * 4 < J.width; };
+
+    // the rows' values, and the other values of their pairs
+    float own[UNITS][4], other[UNITS][4];
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int e = e0 + min(i, n - 1), h = e / J.head, w = e - h * J.head;
-            const float * xh = (const float *) (src + h * J.s_head);
-            own[i] = xh[w];
-            if (J.rope && w < 2 * J.pairs) other[i] = xh[apart ? (w < J.pairs ? w + J.dist : w - J.dist) : w ^ 1];
+    for (int u = 0; u < UNITS; u++) {
+        const int e0 = mine_of(u) ? quad_of(u) * 4 : 0;
+        const int64_t row = J.row0 + row0 + min(row_of(u), n_rows - 1);
+        const char * src = J.src + row * J.s1 + i2 * J.s2 + i3 * J.s3;
+        const int head = e0 / J.head, w0 = e0 - head * J.head;
+        const float * x = (const float *) (src + head * J.s_head);
+        const int n = min(4, J.width - e0);
+        if (J.quads) {
+            const float4 a = load4(x + w0);
+            own[u][0] = a.x; own[u][1] = a.y; own[u][2] = a.z; own[u][3] = a.w;
+            // (values that have no pair apart from them read their own again)
+            const float4 b = load4(x + (apart && w0 < 2 * J.pairs ? (w0 < J.pairs ? w0 + J.dist : w0 - J.dist) : w0));
+            other[u][0] = b.x; other[u][1] = b.y; other[u][2] = b.z; other[u][3] = b.w;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int e = e0 + min(i, n - 1), h = e / J.head, w = e - h * J.head;
+                const float * xh = (const float *) (src + h * J.s_head);
+                own[u][i] = xh[w];
+                other[u][i] = xh[J.rope && w < 2 * J.pairs ? (apart ? (w < J.pairs ? w + J.dist : w - J.dist) : w ^ 1) : w];
+            }
         }
     }
 
-    int64_t to = row;
+    const int64_t idx0 = J.row0 + (i2 % J.c_n2) * J.c2 + (i3 % J.c_n3) * J.c3;
     if (J.idx) {
         if (t < n_rows) {
-            s_at[t] = row_index(J, J.row0 + row0 + t + (i2 % J.c_n2) * J.c2 + (i3 % J.c_n3) * J.c3);
+            s_at[t] = row_index(J, idx0 + row0 + t);
             s_dead[t] = s_at[t] < 0 || s_at[t] >= J.to_rows;
         }
         __syncthreads();
-        to = s_at[min(lr, n_rows - 1)];
         // a later row of the pass with the same index
-        const int64_t base = J.row0 + (i2 % J.c_n2) * J.c2 + (i3 % J.c_n3) * J.c3;
         for (int64_t r = row0 + 1 + t; r < J.rows; r += ROWS_WG) {
-            const int64_t at = row_index(J, base + r);
+            const int64_t at = row_index(J, idx0 + r);
             for (int k = 0; k < n_rows && row0 + k < r; k++) if (at == s_at[k]) s_dead[k] = 1;
         }
     }
@@ -179,49 +186,54 @@ __global__ __launch_bounds__(ROWS_WG) void rows_kernel(const rows_batch B) {
     }
     if (J.idx || J.rope) __syncthreads();
 
-    const double2 * cs = s_cs + min(lr, n_rows - 1) * J.pairs;
-    float v[4];
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        v[i] = own[i];
-        if (!J.rope) continue;
-        const int w = J.quads ? w0 + i : (e0 + min(i, n - 1)) % J.head;
-        if (w >= 2 * J.pairs) continue;
-        const float mate = apart || !J.quads ? other[i] : own[i ^ 1];
-        const bool first = apart ? w < J.pairs : !(w & 1);
-        const double2 c = cs[apart ? (first ? w : w - J.dist) : w / 2];
-        const float a = first ? v[i] : mate, b = first ? mate : v[i];
-        v[i] = J.rope == ROWS_ROPE_MULTI ? rotated(a, b, first, c) : rotated_f32(a, b, first, c);
-    }
-
-    if (!mine || (J.idx && s_dead[lr])) return;
-    if (J.type == GGML_TYPE_Q4_0 || J.type == GGML_TYPE_Q8_0) {
-        const int64_t block = J.first_block + to * J.d1 + i2 * J.d2 + i3 * J.d3 + e0 / 32;
-        if (J.type == GGML_TYPE_Q4_0) store_q4_0(J, block, v, t % 8);
-        else store_q8_0(J, block, v, t % 8);
-        return;
-    }
-    char * out = J.dst + to * J.d1 + i2 * J.d2 + i3 * J.d3;
-    if (J.wide && n == 4) {
-        if (J.type == GGML_TYPE_F32) {
-            *(float4 *) (out + (int64_t) e0 * 4) = make_float4(v[0], v[1], v[2], v[3]);
-        } else {
-            uint16_t h[4];
+    for (int u = 0; u < UNITS; u++) {
+        const bool mine = mine_of(u);
+        const int lr = min(row_of(u), n_rows - 1), e0 = mine ? quad_of(u) * 4 : 0, n = min(4, J.width - e0), w0 = e0 % J.head;
+        const double2 * cs = s_cs + lr * J.pairs;
+        float v[4];
 #pragma unroll
-            for (int i = 0; i < 4; i++) st((char *) &h[i], J.type, v[i]);
-            *(uint2 *) (out + (int64_t) e0 * 2) = make_uint2(h[0] | (uint32_t) h[1] << 16, h[2] | (uint32_t) h[3] << 16);
+        for (int i = 0; i < 4; i++) {
+            v[i] = own[u][i];
+            if (!J.rope) continue;
+            const int w = J.quads ? w0 + i : (e0 + min(i, n - 1)) % J.head;
+            if (w >= 2 * J.pairs) continue;
+            const float mate = apart || !J.quads ? other[u][i] : own[u][i ^ 1];
+            const bool first = apart ? w < J.pairs : !(w & 1);
+            const double2 c = cs[apart ? (first ? w : w - J.dist) : w / 2];
+            const float a = first ? v[i] : mate, b = first ? mate : v[i];
+            v[i] = J.rope == ROWS_ROPE_MULTI ? rotated(a, b, first, c) : rotated_f32(a, b, first, c);
         }
-    } else {
-        const int size = J.type == GGML_TYPE_F32 ? 4 : 2;
+        if (!mine || (J.idx && s_dead[lr])) continue;
+        const int64_t to = J.idx ? s_at[lr] : J.row0 + row0 + lr;
+        if (J.type == GGML_TYPE_Q4_0 || J.type == GGML_TYPE_Q8_0) {
+            const int64_t block = J.first_block + to * J.d1 + i2 * J.d2 + i3 * J.d3 + e0 / 32;
+            if (J.type == GGML_TYPE_Q4_0) store_q4_0(J, block, v, t % 8);
+            else store_q8_0(J, block, v, t % 8);
+            continue;
+        }
+        char * out = J.dst + to * J.d1 + i2 * J.d2 + i3 * J.d3;
+        if (J.wide && n == 4) {
+            if (J.type == GGML_TYPE_F32) {
+                *(float4 *) (out + (int64_t) e0 * 4) = make_float4(v[0], v[1], v[2], v[3]);
+            } else {
+                uint32_t h[4];
 #pragma unroll
-        for (int i = 0; i < 4; i++) if (i < n) st(out + (int64_t) (e0 + i) * size, J.type, v[i]);
+                for (int i = 0; i < 4; i++) h[i] = bits16(J.type, v[i]);
+                *(uint2 *) (out + (int64_t) e0 * 2) = make_uint2(h[0] | h[1] << 16, h[2] | h[3] << 16);
+            }
+        } else {
+            const int size = J.type == GGML_TYPE_F32 ? 4 : 2;
+#pragma unroll
+            for (int i = 0; i < 4; i++) if (i < n) st(out + (int64_t) (e0 + i) * size, J.type, v[i]);
+        }
     }
 }
 
 } // namespace
 
-void rows_shape(rows_job & J) {
-    const int quads = (int) ((J.width + 3) / 4);
+static void rows_shape(rows_job & J) {
+    const int quads = (int) (((int64_t) J.width + 3) / 4);
     J.chunks = (quads + ROWS_WG - 1) / ROWS_WG;
     J.threads = J.chunks > 1 ? ROWS_WG : (quads + 7) / 8 * 8;
     J.per_wg = J.chunks > 1 ? 1 : ROWS_WG / J.threads;
@@ -231,24 +243,38 @@ void rows_shape(rows_job & J) {
     J.wide = ((uintptr_t) J.dst | (uintptr_t) J.d1 | (uintptr_t) J.d2 | (uintptr_t) J.d3) % size == 0;
 }
 
+static int64_t rows_wgs(const rows_job & J, int units) {
+    if (J.chunks > 1) return J.rows * ((J.chunks + units - 1) / units);
+    const int64_t per = (int64_t) units * J.per_wg;
+    return (J.rows + per - 1) / per;
+}
+
+static void launch_units(const rows_batch & B, int units, dim3 grid, hipStream_t st) {
+    if (units == 1) launch(rows_kernel<1>, grid, dim3(ROWS_WG), 0, st, B);
+    else launch(rows_kernel<4>, grid, dim3(ROWS_WG), 0, st, B);
+}
+
 // One launch for jobs of up to ROWS_PASS rows that have no third and fourth extent; else a job and a pass at a time.
+// Four units a workgroup where one would give more than ROWS_MANY: a token's cosines then serve four times the values,
+// or all threads form some.
+constexpr int64_t ROWS_MANY = 2048;
 void launch_rows(rows_batch & B, hipStream_t st) {
     bool together = true;
+    int64_t all = 0;
     for (int k = 0; k < B.n_jobs; k++) {
         rows_shape(B.job[k]);
         together = together && B.job[k].n2 == 1 && B.job[k].n3 == 1 && (!B.job[k].idx || B.job[k].rows <= ROWS_PASS);
+        all += rows_wgs(B.job[k], 1);
     }
-    auto wgs = [](const rows_job & J) { return J.chunks > 1 ? J.rows * J.chunks : (J.rows + J.per_wg - 1) / J.per_wg; };
-    if (together) {
-        int64_t all = 0;
-        for (int k = 0; k < B.n_jobs; k++) {
-            B.job[k].first_wg = all;
-            all += wgs(B.job[k]);
-        }
-        if (all > 0 && all <= INT32_MAX) {
-            launch(rows_kernel, dim3((unsigned) all), dim3(ROWS_WG), 0, st, B);
-            return;
-        }
+    const int units = all > ROWS_MANY ? 4 : 1;
+    all = 0;
+    for (int k = 0; k < B.n_jobs; k++) {
+        B.job[k].first_wg = all;
+        all += rows_wgs(B.job[k], units);
+    }
+    if (together && all <= INT32_MAX) {
+        if (all > 0) launch_units(B, units, dim3((unsigned) all), st);
+        return;
     }
     for (int k = 0; k < B.n_jobs; k++) {
         rows_batch one = B;
@@ -260,7 +286,7 @@ void launch_rows(rows_batch & B, hipStream_t st) {
         for (int64_t r = 0; r < n && J.n2 * J.n3 > 0; r += ROWS_PASS) {
             J.row0 = r;
             J.rows = std::min<int64_t>(ROWS_PASS, n - r);
-            launch(rows_kernel, dim3((unsigned) wgs(J), (unsigned) J.n2, (unsigned) J.n3), dim3(ROWS_WG), 0, st, one);
+            launch_units(one, units, dim3((unsigned) rows_wgs(J, units), (unsigned) J.n2, (unsigned) J.n3), st);
         }
     }
 }

@@ -410,7 +410,7 @@ struct rows_batch {
     // ROWS_ROPE_MULTI: each pair's turns per position and axis; what cosines and sines are multiplied by
     double scale;
     double turns[ROWS_MAX_PAIRS];
-    uint8_t axis[ROWS_MAX_PAIRS];
+    alignas(8) uint8_t axis[ROWS_MAX_PAIRS];
 };
 void launch_rows(rows_batch & B, hipStream_t st);
 
