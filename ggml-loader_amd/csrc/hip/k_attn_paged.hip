@@ -45,10 +45,6 @@ __device__ __forceinline__ int64_t from_lane(int64_t v, int l) {
     return (int64_t) (((uint64_t) hi << 32) | lo);
 }
 
-// x / d for 0 <= x < 2^31 as a product
-__device__ __forceinline__ int quotient(const paged_attn::divisor & d, int x) {
-    return d.mul ? (int) (__umulhi((uint32_t) x, d.mul) >> d.shift) : x >> d.shift;
-}
 __device__ __forceinline__ int page_index(const paged_attn & A, int pos) { return quotient(A.by_page, pos); }
 
 // ---- what each sequence asks for ----
@@ -1291,15 +1287,8 @@ void launch_paged_attn(paged_attn A, hipStream_t st) {
     // a row's first block as a 32-bit number
     const int64_t most = std::max({ A.k_page, A.v_page, A.k_pos * A.page, A.v_pos * A.page });
     A.rows32 = most <= UINT32_MAX && A.n_pages <= (int64_t) UINT32_MAX / std::max<int64_t>(most, 1) - 1;
-    // exact below 2^31: the multiplier is rounded up, by less than 2^-31 of it
-    auto by = [](int d) {
-        int bits = 0;
-        while ((1ll << bits) < d) bits++;
-        const bool power = (1ll << bits) == d;
-        return paged_attn::divisor{ power ? 0 : (uint32_t) (((uint64_t) 1 << (31 + bits)) / d + 1), power ? bits : bits - 1 };
-    };
-    A.by_page = by(A.page);
-    A.by_group = by(A.group);
+    A.by_page = divisor::by(A.page);
+    A.by_group = divisor::by(A.group);
     A.part = (float *) A.scratch;
     A.part_ml = (float2 *) (A.part + split_rows(W) * A.D);
     A.tile_part = (float *) (A.part_ml + split_rows(W));

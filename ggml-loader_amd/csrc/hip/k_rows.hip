@@ -9,8 +9,9 @@
 //
 // A thread holds four values of a row and its pair's other four (read twice, the second time from the
 // cache), eight threads one block of a quantized row; a workgroup 1024 values, whose tokens' cosines its
-// threads form once for all heads. Bound by launch and load latency for a few tokens (4096 tokens of 8 heads
-// of 128, K rotated and both into 4 bits: see the figures at launch_rows).
+// threads form once for all heads. Bound by launch and load latency for a few tokens (8 tokens' 12 rows of 128
+// rotated: 6 us with their launch); 2100 tokens of 28 + 4 heads of 128 rotate in 26 us, 3.3 TB/s; 4096 tokens of 8 heads
+// of 128, K rotated and both into 4 bits, take 25 us.
 //
 // Of rows with one index the last is stored: a workgroup looks its indices up among the later ones of its
 // pass (at most ROWS_PASS rows; passes follow one another on the stream).
@@ -29,13 +30,14 @@ __device__ __forceinline__ int64_t row_index(const rows_job & J, int64_t at) {
     return J.idx64 ? ((const int64_t *) J.idx)[at] : (int64_t) ((const int32_t *) J.idx)[at];
 }
 
-// value w of a head, rotated: a and b are the pair's values, first says whether w is the pair's first
-__device__ __forceinline__ float rotated(double a, double b, bool first, double2 cs) {
-    return (float) (first ? a * cs.x - b * cs.y : a * cs.y + b * cs.x);
+// A value of a pair, rotated: x cos -+ mate sin, minus for the pair's first. (In 32 bits the steps are rope_ext's, whose
+// second values add the products in the other order.)
+__device__ __forceinline__ float rotated(double x, double mate, bool first, double2 cs) {
+    return (float) fma(x, cs.x, (first ? -cs.y : cs.y) * mate);
 }
-__device__ __forceinline__ float rotated_f32(float a, float b, bool first, double2 cs) {
+__device__ __forceinline__ float rotated_f32(float x, float mate, bool first, double2 cs) {
     const float c = (float) cs.x, s = (float) cs.y;
-    return first ? a * c - b * s : a * s + b * c;
+    return x * c + mate * (first ? -s : s);
 }
 
 // a value's 16 bits as F16 or BF16
@@ -98,7 +100,7 @@ __device__ __forceinline__ void store_q8_0(const rows_job & J, int64_t block, co
 
 // UNITS: pieces of 256 threads' values that a workgroup takes: of one row where rows are longer, else rows
 template <int UNITS>
-__global__ __launch_bounds__(ROWS_WG) void rows_kernel(const rows_batch args) {
+__global__ __launch_bounds__(ROWS_WG, 4) void rows_kernel(const rows_batch args) {
     __shared__ double2 s_cs[UNITS * ROWS_MAX_CS];
     __shared__ int64_t s_at[UNITS * ROWS_MAX_PER_WG];
     __shared__ int s_dead[UNITS * ROWS_MAX_PER_WG];
@@ -123,20 +125,24 @@ __global__ __launch_bounds__(ROWS_WG) void rows_kernel(const rows_batch args) {
 
     // the rows' values, and the other values of their pairs
     float own[UNITS][4], other[UNITS][4];
+    int w0[UNITS];
 #pragma unroll
     for (int u = 0; u < UNITS; u++) {
         const int e0 = mine_of(u) ? quad_of(u) * 4 : 0;
         const int64_t row = J.row0 + row0 + min(row_of(u), n_rows - 1);
         const char * src = J.src + row * J.s1 + i2 * J.s2 + i3 * J.s3;
-        const int head = e0 / J.head, w0 = e0 - head * J.head;
+        const int head = J.rope ? quotient(J.by_head, e0) : 0;
+        w0[u] = e0 - head * J.head;
         const float * x = (const float *) (src + head * J.s_head);
         const int n = min(4, J.width - e0);
         if (J.quads) {
-            const float4 a = load4(x + w0);
+            const float4 a = load4(x + w0[u]);
             own[u][0] = a.x; own[u][1] = a.y; own[u][2] = a.z; own[u][3] = a.w;
-            // (values that have no pair apart from them read their own again)
-            const float4 b = load4(x + (apart && w0 < 2 * J.pairs ? (w0 < J.pairs ? w0 + J.dist : w0 - J.dist) : w0));
-            other[u][0] = b.x; other[u][1] = b.y; other[u][2] = b.z; other[u][3] = b.w;
+            if (apart) {
+                // (values that have no pair read their own again)
+                const float4 b = load4(x + (w0[u] < 2 * J.pairs ? (w0[u] < J.pairs ? w0[u] + J.dist : w0[u] - J.dist) : w0[u]));
+                other[u][0] = b.x; other[u][1] = b.y; other[u][2] = b.z; other[u][3] = b.w;
+            }
         } else {
 #pragma unroll
             for (int i = 0; i < 4; i++) {
@@ -155,10 +161,28 @@ __global__ __launch_bounds__(ROWS_WG) void rows_kernel(const rows_batch args) {
             s_dead[t] = s_at[t] < 0 || s_at[t] >= J.to_rows;
         }
         __syncthreads();
-        // a later row of the pass with the same index
-        for (int64_t r = row0 + 1 + t; r < J.rows; r += ROWS_WG) {
+        // a later row of the pass with the same index: of the workgroup's own, and of those behind them, whose lookups
+        // go eight at a time where they are many (a pass has fewer than 2^31 rows)
+        if (t < n_rows) {
+            for (int k = 0; k < t; k++) if (s_at[k] == s_at[t]) s_dead[k] = 1;
+        }
+        const int last = (int) J.rows - 1;
+        int r = (int) row0 + n_rows + t;
+        for (const bool many = last - r + t >= 8 * ROWS_WG; many && r <= last; r += 8 * ROWS_WG) {
+            int64_t at[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) at[i] = row_index(J, idx0 + min(r + i * ROWS_WG, last));
+            for (int k = 0; k < n_rows; k++) {
+                const int64_t mine = s_at[k];
+                bool same = false;
+#pragma unroll
+                for (int i = 0; i < 8; i++) same |= at[i] == mine;
+                if (same) s_dead[k] = 1;
+            }
+        }
+        for (; r <= last; r += ROWS_WG) {
             const int64_t at = row_index(J, idx0 + r);
-            for (int k = 0; k < n_rows && row0 + k < r; k++) if (at == s_at[k]) s_dead[k] = 1;
+            for (int k = 0; k < n_rows; k++) if (s_at[k] == at) s_dead[k] = 1;
         }
     }
     if (J.rope) {
@@ -189,20 +213,36 @@ __global__ __launch_bounds__(ROWS_WG) void rows_kernel(const rows_batch args) {
 #pragma unroll
     for (int u = 0; u < UNITS; u++) {
         const bool mine = mine_of(u);
-        const int lr = min(row_of(u), n_rows - 1), e0 = mine ? quad_of(u) * 4 : 0, n = min(4, J.width - e0), w0 = e0 % J.head;
-        const double2 * cs = s_cs + lr * J.pairs;
+        const int lr = min(row_of(u), n_rows - 1), e0 = mine ? quad_of(u) * 4 : 0, n = min(4, J.width - e0);
         float v[4];
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            v[i] = own[u][i];
-            if (!J.rope) continue;
-            const int w = J.quads ? w0 + i : (e0 + min(i, n - 1)) % J.head;
-            if (w >= 2 * J.pairs) continue;
-            const float mate = apart || !J.quads ? other[u][i] : own[u][i ^ 1];
-            const bool first = apart ? w < J.pairs : !(w & 1);
-            const double2 c = cs[apart ? (first ? w : w - J.dist) : w / 2];
-            const float a = first ? v[i] : mate, b = first ? mate : v[i];
-            v[i] = J.rope == ROWS_ROPE_MULTI ? rotated(a, b, first, c) : rotated_f32(a, b, first, c);
+        for (int i = 0; i < 4; i++) v[i] = own[u][i];
+        if (J.rope) {
+            const double2 * cs = s_cs + lr * J.pairs;
+            const bool multi = J.rope == ROWS_ROPE_MULTI;
+            if (J.quads) {
+                // a quad lies in one half of the pairs, in pairs of neighbours, or past them
+                if (w0[u] < 2 * J.pairs) {
+                    const bool first = w0[u] < J.pairs;
+                    const double2 * at = cs + (apart ? (first ? w0[u] : w0[u] - J.dist) : w0[u] / 2);
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const double2 c = at[apart ? i : i / 2];
+                        const float mate = apart ? other[u][i] : own[u][i ^ 1];
+                        const bool f = apart ? first : !(i & 1);
+                        v[i] = multi ? rotated(own[u][i], mate, f, c) : rotated_f32(own[u][i], mate, f, c);
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int w = (e0 + min(i, n - 1)) % J.head;
+                    if (w >= 2 * J.pairs) continue;
+                    const bool first = apart ? w < J.pairs : !(w & 1);
+                    const double2 c = cs[apart ? (first ? w : w - J.dist) : w / 2];
+                    v[i] = multi ? rotated(own[u][i], other[u][i], first, c) : rotated_f32(own[u][i], other[u][i], first, c);
+                }
+            }
         }
         if (!mine || (J.idx && s_dead[lr])) continue;
         const int64_t to = J.idx ? s_at[lr] : J.row0 + row0 + lr;
@@ -237,6 +277,7 @@ static void rows_shape(rows_job & J) {
     J.chunks = (quads + ROWS_WG - 1) / ROWS_WG;
     J.threads = J.chunks > 1 ? ROWS_WG : (quads + 7) / 8 * 8;
     J.per_wg = J.chunks > 1 ? 1 : ROWS_WG / J.threads;
+    J.by_head = divisor::by(std::max(J.head, 1));
     J.quads = J.width % 4 == 0 && J.head % 4 == 0 && (!J.rope || (J.dist > 1 ? J.pairs % 4 == 0 && J.dist % 4 == 0 : J.pairs % 2 == 0));
     if (J.type == GGML_TYPE_Q4_0 || J.type == GGML_TYPE_Q8_0) return;
     const int size = J.type == GGML_TYPE_F32 ? 16 : 8;

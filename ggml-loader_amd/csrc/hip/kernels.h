@@ -374,6 +374,21 @@ constexpr int64_t ROPE_TABLE_MIN_TOKENS = 16;   // RoPE jobs over at least this 
 // layer), formed once
 void launch_rope_table(const int32_t * pos, int64_t n_pos, const rope_params & p, const float * ff, float2 * out, hipStream_t st);
 
+// x / d for 0 <= x < 2^31 as a product: the multiplier is rounded up, by less than 2^-31 of it
+struct divisor {
+    uint32_t mul;
+    int shift;
+    static divisor by(int64_t d) {
+        int bits = 0;
+        while (((int64_t) 1 << bits) < d) bits++;
+        const bool power = ((int64_t) 1 << bits) == d;
+        return { power ? 0 : (uint32_t) (((uint64_t) 1 << (31 + bits)) / (uint64_t) d + 1), power ? bits : bits - 1 };
+    }
+};
+__device__ __forceinline__ int quotient(const divisor & d, int x) {
+    return d.mul ? (int) (__umulhi((uint32_t) x, d.mul) >> d.shift) : x >> d.shift;
+}
+
 // Rows of F32 values, rotated or not, into rows of dst (F32, F16, BF16, or the planes of Q8_0 / Q4_0): row r into row
 // idx[r], where that lies in [0, to_rows), or into row r without idx. A row is `width` values, heads of `head` at s_head.
 constexpr int ROWS_MAX_JOBS = 4;
@@ -401,6 +416,7 @@ struct rows_job {
     int64_t first_block, d1, d2, d3;
     // set by launch_rows
     int chunks, threads, per_wg, quads, wide;
+    divisor by_head;
     int64_t first_wg;
 };
 struct rows_batch {
