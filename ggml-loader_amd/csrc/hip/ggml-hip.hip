@@ -3394,12 +3394,12 @@ enum ggml_status ggml_backend_hip_verify(ggml_backend_t backend, const struct gg
         int64_t ns = 0, nd = 0;
         auto bytes = [](int64_t ns, int64_t nd) { return (size_t) ((nd + ns) * 8 + (ns + 1 + nd) * 4); };
         while (s0 + ns < n_seqs && ns < most && bytes(ns + 1, nd + n_drafted[s0 + ns]) <= UP_SMALL) nd += n_drafted[s0 + ns++];
-        const size_t parts = (size_t) (ns * segments) * sizeof(double2);
-        if (parts > d.lp_size) {
+        const size_t parts = (size_t) (ns * segments) * sizeof(double2), need = parts + (size_t) ns * sizeof(verify_head);
+        if (need > d.lp_size) {
             HIP_CHECK(hipStreamSynchronize(d.stream));
             drained(d);
             if (d.lp) HIP_CHECK(hipFree(d.lp));
-            d.lp_size = std::max(parts, (size_t) 1 << 20);
+            d.lp_size = std::max(need, (size_t) 1 << 20);
             HIP_CHECK(hipMalloc(&d.lp, d.lp_size));
         }
         uint8_t * slot = upload_slot(d, bytes(ns, nd));
@@ -3424,6 +3424,7 @@ enum ggml_status ggml_backend_hip_verify(ggml_backend_t backend, const struct gg
         L.n = (int) n; L.n_seqs = (int) ns; L.segments = (int) segments;
         L.first = first; L.tokens = st; L.u = su;
         L.parts = (double2 *) d.lp;
+        L.heads = (verify_head *) ((char *) d.lp + parts);
         L.out = area;
         launch_verify(L, d.stream);
         HIP_CHECK(hipStreamSynchronize(d.stream));

@@ -447,13 +447,18 @@ struct paged_attn {
     void * scratch;                  // paged_attn_scratch_bytes
     // set by launch_paged_attn
     int team, team_bits, head_teams, teams, tile_teams, split_most, tile_least, rows32;
-    struct divisor { uint32_t mul; int shift; } by_page, by_group;
+    divisor by_page, by_group;
     float * part, * tile_part;
     float2 * part_ml, * tile_ml;
 };
 // Drafted tokens against probabilities (ggml_backend_hip_verify): rows as ggml row indices over ne[1..3]
 constexpr int VERIFY_SEGMENT = 2048;
 struct verify_rows { const char * base; int64_t ne1, ne2, nb1, nb2, nb3; };
+struct verify_head {                 // where a sequence's token is drawn from
+    const float * p, * q;            // q: nullptr where nothing is taken off
+    double u;
+    int without;                     // the token without weight, or -1
+};
 struct verify_launch {
     verify_rows p, q;                // q.base: nullptr for drafts that are certain
     int64_t row0, seq0;              // drafted tokens and sequences before the launch's: q's row of token i is row0 + i
@@ -462,9 +467,11 @@ struct verify_launch {
     const int32_t * tokens;
     const double * u;
     double2 * parts;                 // [n_seqs][segments]
+    verify_head * heads;             // [n_seqs]
     int32_t * out;                   // (accepted, token) a sequence
+    int wide;                        // set by launch_verify
 };
-void launch_verify(const verify_launch & L, hipStream_t st);
+void launch_verify(verify_launch L, hipStream_t st);
 
 int64_t paged_attn_scratch_bytes(const paged_attn & A);
 void launch_paged_attn(paged_attn A, hipStream_t st);
