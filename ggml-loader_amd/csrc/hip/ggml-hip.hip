@@ -602,12 +602,13 @@ const char * flash_attn_paged_refusal(const ggml_tensor * n) {
     }
     const int64_t D = q->ne[0], H = q->ne[1], T = q->ne[2], KV = k->ne[1], P = k->ne[2], S = pages->ne[1];
     if (D != 64 && D != 96 && D != 128) return "flash_attn_paged: heads of 64, 96 or 128 values";
-    if (k->ne[0] != D || !ggml_are_same_shape(k, v) || KV < 1 || H % KV || P < 1) return "flash_attn_paged: the cache's extents do not fit";
+    if (k->ne[0] != D || !ggml_are_same_shape(k, v) || KV < 1 || H % KV || P < 1 || k->ne[3] < 1) return "flash_attn_paged: the cache's extents do not fit";
     if (!plain_rows(pages, GGML_TYPE_I32) || pages->ne[2] != 1 || pages->ne[3] != 1 || !i32_vector(start, S + 1) || !i32_vector(len, S)) {
         return "flash_attn_paged: I32 pages of each sequence, starts (one more than sequences) and lengths";
     }
     if (n->type != GGML_TYPE_F32 || !ggml_is_contiguous(n) || !has_shape(n, D, H, T, 1)) return "flash_attn_paged: the result's extent does not fit";
-    if (S > PAGED_MAX_SEQS || T > PAGED_MAX_TOKENS || H > PAGED_MAX_HEADS || P > INT_MAX / 2 || pages->ne[0] > INT_MAX / 2 / P) {
+    if (S > PAGED_MAX_SEQS || T > PAGED_MAX_TOKENS || H > PAGED_MAX_HEADS || P > INT_MAX / 2 || pages->ne[0] > INT_MAX / 2 / P ||
+        (pages->ne[0] * P + 31) / 32 > INT_MAX / KV) {
         return "flash_attn_paged: too many sequences, tokens, heads or positions";
     }
     return nullptr;

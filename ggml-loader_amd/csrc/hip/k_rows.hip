@@ -275,7 +275,7 @@ __global__ __launch_bounds__(ROWS_WG, 4) void rows_kernel(const rows_batch args)
 static void rows_shape(rows_job & J) {
     const int quads = (int) (((int64_t) J.width + 3) / 4);
     J.chunks = (quads + ROWS_WG - 1) / ROWS_WG;
-    J.threads = J.chunks > 1 ? ROWS_WG : (quads + 7) / 8 * 8;
+    J.threads = J.chunks > 1 ? ROWS_WG : std::max((quads + 7) / 8 * 8, 8);
     J.per_wg = J.chunks > 1 ? 1 : ROWS_WG / J.threads;
     J.by_head = divisor::by(std::max(J.head, 1));
     J.quads = J.width % 4 == 0 && J.head % 4 == 0 && (!J.rope || (J.dist > 1 ? J.pairs % 4 == 0 && J.dist % 4 == 0 : J.pairs % 2 == 0));
@@ -285,6 +285,7 @@ static void rows_shape(rows_job & J) {
 }
 
 static int64_t rows_wgs(const rows_job & J, int units) {
+    if (J.width == 0) return 0;
     if (J.chunks > 1) return J.rows * ((J.chunks + units - 1) / units);
     const int64_t per = (int64_t) units * J.per_wg;
     return (J.rows + per - 1) / per;
@@ -324,7 +325,7 @@ void launch_rows(rows_batch & B, hipStream_t st) {
         rows_job & J = one.job[0];
         J.first_wg = 0;
         const int64_t n = J.rows;
-        for (int64_t r = 0; r < n && J.n2 * J.n3 > 0; r += ROWS_PASS) {
+        for (int64_t r = 0; r < n && J.width > 0 && J.n2 * J.n3 > 0; r += ROWS_PASS) {
             J.row0 = r;
             J.rows = std::min<int64_t>(ROWS_PASS, n - r);
             launch_units(one, units, dim3((unsigned) rows_wgs(J, units), (unsigned) J.n2, (unsigned) J.n3), st);

@@ -324,7 +324,7 @@ GGML_API struct ggml_tensor * ggml_rope_multi(struct ggml_context * ctx, struct 
 // Row r of b into row c[r] of a, converted to a's type (F32, F16, BF16, Q8_0, Q4_0: blocks as ggml_quantize_chunk forms
 // them); returns a view of a. b: F32 [a->ne[0], n, a->ne[2], a->ne[3]]; c: I32 or I64 [n, c2, c3], c2 dividing a->ne[2] and
 // c3 a->ne[3] (used again over them). A row whose index is outside [0, a->ne[1]) is not stored; of rows with one index the
-// last is. A Q4_0 block that holds a NaN gets a NaN scale.
+// last is. A Q4_0 or Q8_0 block that holds a NaN gets a NaN scale.
 GGML_API struct ggml_tensor * ggml_set_rows(struct ggml_context * ctx, struct ggml_tensor * a, struct ggml_tensor * b, struct ggml_tensor * c);
 // Causal attention of the new tokens of several sequences over a cache on pages. q: F32 [d, n_head, n_tokens], rotated, the
 // sequences' tokens one after another: sequence s has tokens q_start[s] .. q_start[s + 1] - 1 (q_start: I32 [n_seqs + 1]), the

@@ -300,3 +300,59 @@ def test_append_in_order_with_what_reads_the_cache(hip):
     want[[0, 2, 3, 4]] = x.reshape(4, 128)
     assert np.array_equal(got[1], fill.ravel())
     assert np.array_equal(got[4], want.ravel())
+
+
+@pytest.mark.parametrize("how", ["several", "neox"])
+@pytest.mark.parametrize("T", [1, 3, 40])
+def test_append_of_normed_keys(hip, how, T):
+    """Queries and keys normed by head before they turn, values added to a bias: bits as without fusion."""
+    rng = np.random.default_rng(T)
+    x, w, bias = (rng.standard_normal(s).astype(np.float32) for s in ((T, 8, 64), 64, (T, 128)))
+    idx = rng.permutation(T + 3)[:T].astype(np.int64)
+    pos = positions(rng, T, 5000)
+    got = []
+    for fused in (True, False):
+        gl.libs()["hip"].ggml_backend_hip_set_fusion(hip, fused)
+        with Graph(mem=1 << 20) as g:
+            rows, tw = g.tensor(gl.F32, 64, 8, T, data=x), g.tensor(gl.F32, 64, data=w)
+            p = g.tensor(gl.I32, 4 * T, data=pos) if how == "several" else g.tensor(gl.I32, T, data=pos[0])
+            to = g.tensor(gl.I64, T, data=idx)
+            kc, vc = (g.tensor(gl.Q4_0, 128, T + 3, data=quantize(np.zeros((T + 3, 128), np.float32), gl.Q4_0)) for _ in "kv")
+
+            def normed(n, at):
+                a = g.mul(g.rms_norm(g.cont_3d(g.view_3d(rows, 64, n, T, 256, 2048, 256 * at), 64, n, T), 1e-6), tw)
+                return multi(g, a, p, 64, (8, 12, 12, 0), ref.MROPE) if how == "several" else \
+                    g.rope_ext(a, p, None, 64, gl.ROPE_NEOX, 0, 1e4, 1.0, 0.0, 1.0, 32.0, 1.0)
+            q, k = normed(4, 0), normed(2, 4)
+            v = g.add(g.cont_2d(g.view_3d(rows, 64, 2, T, 256, 2048, 256 * 6), 128, T), g.tensor(gl.F32, 128, T, data=bias))
+            res = g.compute(hip, [q, g.set_rows(kc, g.reshape_2d(k, 128, T), to), g.set_rows(vc, v, to)])
+            got.append((res[0], raw(g, kc), raw(g, vc)))
+    gl.libs()["hip"].ggml_backend_hip_set_fusion(hip, True)
+    for a, b in zip(*got):
+        assert np.array_equal(a.view(np.uint8), b.view(np.uint8))
+    cache = quantize(np.zeros((T + 3, 128), np.float32), gl.Q4_0).view(np.uint8).reshape(T + 3, -1).copy()
+    values = x[:, 6:].reshape(T, 128) + bias
+    assert np.array_equal(got[0][2], expected(cache, values, idx, gl.Q4_0).ravel())
+
+
+def test_rows_of_nothing(hip):
+    """No heads, no tokens, no rows, no values."""
+    with Graph(mem=1 << 20) as g:
+        some = g.tensor(gl.F32, 64, 2, 3, data=np.ones((3, 2, 64), np.float32))
+        pos = g.tensor(gl.I32, 12, data=np.zeros(12, np.int32))
+        a = multi(g, g.tensor(gl.F32, 64, 0, 3), pos, 64, (8, 12, 12, 0), ref.MROPE)
+        b = multi(g, g.tensor(gl.F32, 64, 2, 0), g.tensor(gl.I32, 0), 64, (8, 12, 12, 0), ref.MROPE)
+        c = multi(g, some, pos, 64, (8, 12, 12, 0), ref.MROPE)
+        cache = g.tensor(gl.F16, 64, 5, data=np.ones((5, 64), np.float16))
+        d = g.set_rows(cache, g.tensor(gl.F32, 64, 0), g.tensor(gl.I64, 0))
+        e = g.set_rows(g.tensor(gl.F32, 0, 5), g.tensor(gl.F32, 0, 3), g.tensor(gl.I64, 3, data=np.arange(3)))
+        f = g.set_rows(g.tensor(gl.F32, 64, 5, 0), g.tensor(gl.F32, 64, 3, 0), g.tensor(gl.I64, 3, data=np.arange(3)))
+        core, gf = g.core, g.core.ggml_new_graph(g.ctx)
+        for t in (a, b, c, d, e, f):
+            core.ggml_set_output(t)
+            core.ggml_build_forward_expand(gf, t)
+        g.buf = core.ggml_backend_alloc_ctx_tensors(g.ctx, hip)
+        for t, x in g.inputs:
+            core.ggml_backend_tensor_set(t, x.ctypes.data, 0, x.nbytes)
+        assert core.ggml_backend_graph_compute(hip, gf) == 0
+        assert (g.read(c) == 1).all() and (g.read(cache, np.float16) == 1).all()

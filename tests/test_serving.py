@@ -122,6 +122,23 @@ def test_flash_attn_paged_refuses(name, ne, t):
         assert refusal(paged(g, **{name: g.tensor(t, *ne)}))
 
 
+def test_flash_attn_paged_refuses_a_cache_without_pages_and_tables_of_too_many_positions():
+    with Graph(mem=1 << 20) as g:
+        assert refusal(paged(g, k=g.tensor(gl.Q4_0, 64, 2, 16, 0), v=g.tensor(gl.Q4_0, 64, 2, 16, 0)))
+        t = g.tensor(gl.Q4_0, 64 * 64, 1)
+        k = g.view_4d(t, 64, 64, 1, 1, 36, 36 * 64, 36 * 64, 0)                     # 64 heads, a position a page
+        q = g.tensor(gl.F32, 64, 64, 6)
+        for most, ok in ((1 << 29, True), ((1 << 30) - 32, True), (1 << 30, False)):
+            n = paged(g, q=q, k=k, v=k, pages=g.tensor(gl.I32, most, 2))
+            assert (refusal(n) is None) == ok
+        t = g.tensor(gl.Q4_0, 64 * 1024, 1)
+        k = g.view_4d(t, 64, 1024, 1, 1, 36, 36 * 1024, 36 * 1024, 0)
+        q = g.tensor(gl.F32, 64, 1024, 6)
+        for most, ok in ((1 << 25, True), (1 << 26, False), (1 << 29, False)):
+            n = paged(g, q=q, k=k, v=k, pages=g.tensor(gl.I32, most, 2))
+            assert (refusal(n) is None) == ok
+
+
 def test_flash_attn_paged_refuses_missing_operands_and_strides():
     with Graph(mem=1 << 20) as g:
         for name in ("pages", "start", "seen", "k", "v"):
