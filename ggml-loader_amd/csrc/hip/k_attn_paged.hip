@@ -78,13 +78,6 @@ __device__ __forceinline__ int tiles_of(const paged_attn & A, const seq_info & q
     const int64_t n = (int64_t) q.n * A.group;
     return n < A.tile_least ? 0 : (int) ((n + rows - 1) / rows);
 }
-__device__ __forceinline__ int64_t tile_units(const paged_attn & A, const seq_info & q, int rows) {
-    const int tiles = tiles_of(A, q, rows);
-    int64_t sum = 0;
-    for (int k = 0; k < tiles; k++) sum += tile_steps(A, q, rows, k);
-    return sum * A.n_head_kv;
-}
-
 __device__ __forceinline__ int64_t wave_scan(int64_t v) {
     const int lane = threadIdx.x % WAVE;
 #pragma unroll
@@ -93,6 +86,29 @@ __device__ __forceinline__ int64_t wave_scan(int64_t v) {
         if (lane >= k) v += o;
     }
     return v;
+}
+
+// The units of sequence s0 + lane: by each lane over its tiles, or where one has more than three times as many as there are
+// sequences, by the whole wave over each sequence's (a prompt of 8192 tokens in 256 tiles: 13 us by a lane).
+__device__ __forceinline__ int64_t tile_units(const paged_attn & A, int s0, int rows) {
+    const int lane = threadIdx.x % WAVE, n = min(A.n_seqs - s0, WAVE);
+    seq_info q{ 0, 0, 0, 0 };
+    if (lane < n) q = seq_of(A, s0 + lane);
+    const int tiles = lane < n ? tiles_of(A, q, rows) : 0;
+    int64_t sum = 0;
+    if (!__any(tiles > 3 * n)) {
+        for (int k = 0; k < tiles; k++) sum += tile_steps(A, q, rows, k);
+        return sum * A.n_head_kv;
+    }
+    for (int i = 0; i < n; i++) {
+        const seq_info one{ 0, __builtin_amdgcn_readlane(q.n, i), __builtin_amdgcn_readlane(q.len, i), __builtin_amdgcn_readlane(q.last, i) };
+        const int all = __builtin_amdgcn_readlane(tiles, i);
+        int64_t mine = 0;
+        for (int k = lane; k < all; k += WAVE) mine += tile_steps(A, one, rows, k);
+        mine = from_lane(wave_scan(mine), WAVE - 1);
+        if (lane == i) sum = mine;
+    }
+    return sum * A.n_head_kv;
 }
 
 // All sequences' tiles, heads and steps in one line of units; teams (of A.team waves, a KV head each) take equal
@@ -660,11 +676,8 @@ __global__ __launch_bounds__(WAVES * WAVE, WAVES == 8 ? 4 : 3) void paged_tile_k
     int seq = 0;
     int64_t u = 0, left;
     {
-        int64_t n = lane < A.n_seqs ? tile_units(A, seq_of(A, lane), ROWS) : 0, up = wave_scan(n), all = from_lane(up, WAVE - 1);
-        for (int s0 = WAVE; s0 < A.n_seqs; s0 += WAVE) {
-            const int s = s0 + lane;
-            all += from_lane(wave_scan(s < A.n_seqs ? tile_units(A, seq_of(A, s), ROWS) : 0), WAVE - 1);
-        }
+        int64_t n = tile_units(A, 0, ROWS), up = wave_scan(n), all = from_lane(up, WAVE - 1);
+        for (int s0 = WAVE; s0 < A.n_seqs; s0 += WAVE) all += from_lane(wave_scan(tile_units(A, s0, ROWS)), WAVE - 1);
         P.deal(all, A.tile_teams);
         if ((int) blockIdx.x >= P.teams) return;
         u = P.begin(blockIdx.x);
@@ -674,8 +687,7 @@ __global__ __launch_bounds__(WAVES * WAVE, WAVES == 8 ? 4 : 3) void paged_tile_k
         uint64_t past = __ballot(up > u);
         for (int s0 = WAVE; !past && s0 < A.n_seqs; s0 += WAVE) {
             before = from_lane(up, WAVE - 1);
-            const int s = s0 + lane;
-            n = s < A.n_seqs ? tile_units(A, seq_of(A, s), ROWS) : 0;
+            n = tile_units(A, s0, ROWS);
             up = before + wave_scan(n);
             past = __ballot(up > u);
             seq = s0;
@@ -1019,21 +1031,21 @@ __global__ __launch_bounds__(WAVES * WAVE, WAVES == 8 ? 4 : 3) void paged_tile_k
 struct part_sum {
     float m = M_NONE, l = 0.0f;
     float4 o = make_float4(0, 0, 0, 0);
-    // parts from, from + by, .. up to last, eight of them loaded at a time; at(k): row of part k
-    template <typename F>
+    // parts from, from + by, .. up to last, N of them loaded at a time; at(k): row of part k
+    template <int N, typename F>
     __device__ __forceinline__ void add(const float * part, const float2 * part_ml, F at, int D, int e, int64_t from, int64_t last, int by) {
-        for (int64_t k0 = from; k0 <= last; k0 += 8 * by) {
-            float2 ml[8];
-            float4 v[8];
+        for (int64_t k0 = from; k0 <= last; k0 += N * by) {
+            float2 ml[N];
+            float4 v[N];
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
+            for (int i = 0; i < N; i++) {
                 const int64_t r = at(min(k0 + i * by, last));
                 ml[i] = part_ml[r];
                 v[i] = *(const float4 *) (part + r * D + 4 * e);
             }
             float now = m;
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
+            for (int i = 0; i < N; i++) {
                 if (k0 + i * by > last) ml[i] = make_float2(M_NONE, 0.0f);
                 now = fmaxf(now, ml[i].x);
             }
@@ -1044,7 +1056,7 @@ struct part_sum {
             o.z *= was;
             o.w *= was;
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
+            for (int i = 0; i < N; i++) {
                 if (k0 + i * by > last) continue;
                 const float is = exp2_hw(ml[i].x - now);
                 l = fmaf(ml[i].y, is, l);
@@ -1058,76 +1070,101 @@ struct part_sum {
     }
 };
 
-// The same by teams: of many tokens few rows have parts. A workgroup looks at the item that its team ends in, and joins the
-// item's rows if the team began it and did not finish it.
-template <int NB, int SPLIT, int TILE>
-__global__ __launch_bounds__(256) void paged_join_teams_kernel(const paged_attn args) {
-    const paged_attn & A = kernargs_prefetched(args);
-    constexpr int D = NB * 32, PER = D / 4, GROUPS = 256 / PER, ROWS = SPLIT ? SPLIT : TILE;
-    const int lane = threadIdx.x % WAVE, t = threadIdx.x;
-    const int team = SPLIT ? A.team : 1, in_team = SPLIT ? (int) blockIdx.y : 0;
-    auto units = [&](int s) { return s >= A.n_seqs ? (int64_t) 0 : SPLIT ? split_units(A, seq_of(A, s), ROWS) : tile_units(A, seq_of(A, s), ROWS); };
-    int64_t all = 0;
-    for (int s0 = 0; s0 < A.n_seqs; s0 += WAVE) all += from_lane(wave_scan(units(s0 + lane)), WAVE - 1);
+// The same by teams: of many tokens few rows have parts. A workgroup looks at the item that its team ends in (its first wave
+// does, for all), and joins the item's rows if the team began it and did not finish it. in_team: the team's wave, or of
+// TILE's rows the sixteens that it starts with, `by` apart.
+struct item_parts { int seq, tile, head; int64_t last; };
+template <int SPLIT, int TILE>
+__device__ __forceinline__ bool parts_of(const paged_attn & A, int64_t me, int in_team, item_parts & I) {
+    constexpr int ROWS = SPLIT ? SPLIT : TILE;
+    const int lane = threadIdx.x % WAVE;
+    auto units = [&](int s0) {
+        if (!SPLIT) return tile_units(A, s0, ROWS);
+        return s0 + lane < A.n_seqs ? split_units(A, seq_of(A, s0 + lane), ROWS) : (int64_t) 0;
+    };
+    int64_t n = units(0), up = wave_scan(n), all = from_lane(up, WAVE - 1);
+    for (int s0 = WAVE; s0 < A.n_seqs; s0 += WAVE) all += from_lane(wave_scan(units(s0)), WAVE - 1);
     plan P;
     P.deal(all, SPLIT ? A.teams : A.tile_teams);
-    const int64_t me = blockIdx.x;
-    if (me >= P.teams) return;
+    if (me >= P.teams) return false;
     const int64_t begin = P.begin(me), end = P.begin(me + 1);
-    if (begin >= end) return;
-    int64_t u = end - 1, before = 0;
-    int seq = -1;
-    for (int s0 = 0; seq < 0 && s0 < A.n_seqs; s0 += WAVE) {
-        const int64_t n = units(s0 + lane), up = before + wave_scan(n);
-        const uint64_t past = __ballot(up > u);
-        if (past) {
-            const int l = __builtin_ctzll(past);
-            seq = s0 + l;
-            before = from_lane(up - n, l);
-        } else {
-            before = from_lane(up, WAVE - 1);
-        }
+    if (begin >= end) return false;
+    const int64_t u = end - 1;
+    uint64_t past = __ballot(up > u);
+    int s0 = 0;
+    while (!past && s0 + WAVE < A.n_seqs) {
+        s0 += WAVE;
+        n = units(s0);
+        up = from_lane(up, WAVE - 1) + wave_scan(n);
+        past = __ballot(up > u);
     }
-    if (seq < 0) return;
-    const seq_info Q = seq_of(A, seq);
-    int tile = 0, head = 0, steps;
+    if (!past) return false;
+    I.seq = s0 + __builtin_ctzll(past);
+    int64_t before = from_lane(up - n, __builtin_ctzll(past));
+    const seq_info Q = seq_of(A, I.seq);
+    auto over = [](int64_t a, int b) { return a < ((int64_t) 1 << 32) ? (int) ((uint32_t) a / (uint32_t) b) : (int) (a / b); };
+    int steps;
     if (SPLIT) {
         steps = steps_of(Q);
-        const int64_t item = (u - before) / steps;
-        tile = (int) (item / A.head_teams);
-        head = (int) (item - (int64_t) tile * A.head_teams) * team + in_team;
-        before += item * steps;
+        const int item = over(u - before, steps);
+        I.tile = item / A.head_teams;
+        I.head = (item - I.tile * A.head_teams) * A.team + in_team;
+        before += (int64_t) item * steps;
     } else {
         const int tiles = tiles_of(A, Q, ROWS);
+        I.tile = 0;
         for (int k0 = 0; k0 < tiles; k0 += WAVE) {
-            const int64_t n = k0 + lane < tiles ? (int64_t) tile_steps(A, Q, ROWS, k0 + lane) * A.n_head_kv : 0, up = before + wave_scan(n);
-            const uint64_t past = __ballot(up > u);
+            n = k0 + lane < tiles ? (int64_t) tile_steps(A, Q, ROWS, k0 + lane) * A.n_head_kv : 0;
+            up = before + wave_scan(n);
+            past = __ballot(up > u);
             if (past) {
-                const int l = __builtin_ctzll(past);
-                tile = k0 + l;
-                before = from_lane(up - n, l);
+                I.tile = k0 + __builtin_ctzll(past);
+                before = from_lane(up - n, __builtin_ctzll(past));
                 break;
             }
             before = from_lane(up, WAVE - 1);
         }
-        steps = tile_steps(A, Q, ROWS, tile);
-        head = (int) ((u - before) / steps);
-        before += (int64_t) head * steps;
+        steps = tile_steps(A, Q, ROWS, I.tile);
+        I.head = over(u - before, steps);
+        before += (int64_t) I.head * steps;
     }
-    if (before < begin || before + steps <= end) return;
-    const int64_t last = P.team_of(before + steps - 1);
+    if (before < begin || before + steps <= end) return false;
+    I.last = P.team_of(before + steps - 1);
+    return true;
+}
+template <int NB, int SPLIT, int TILE>
+__device__ __forceinline__ void join_team(const paged_attn & A, int64_t me, int in_team, int by) {
+    constexpr int D = NB * 32, PER = D / 4, GROUPS = 256 / PER, ROWS = SPLIT ? SPLIT : TILE;
+    __shared__ item_parts s_item;
+    __shared__ bool s_any;
+    const int t = threadIdx.x;
+    if (t < WAVE) {
+        item_parts I;
+        const bool any = parts_of<SPLIT, TILE>(A, me, in_team, I);
+        if (t == 0) { s_any = any; s_item = I; }
+    }
+    __syncthreads();
+    if (!s_any) return;
+    const item_parts I = s_item;
+    const seq_info Q = seq_of(A, I.seq);
     const float * part = SPLIT ? A.part : A.tile_part;
     const float2 * part_ml = SPLIT ? A.part_ml : A.tile_ml;
-    const int group = t / PER, e = t % PER, rows = min(ROWS, Q.n * A.group - tile * ROWS);
-    // TILE: rows over the grid's second dimension
-    for (int r = group + (SPLIT ? 0 : (int) blockIdx.y * GROUPS); group < GROUPS && r < rows; r += GROUPS * (SPLIT ? 1 : (int) gridDim.y)) {
+    const int group = t / PER, e = t % PER, rows = min(ROWS, Q.n * A.group - I.tile * ROWS), team = SPLIT ? A.team : 1;
+    for (int r = group + (SPLIT ? 0 : in_team * GROUPS); group < GROUPS && r < rows; r += GROUPS * (SPLIT ? 1 : by)) {
         part_sum S;
-        S.add(part, part_ml, [&](int64_t k) { return ((k * 2 + (k == me)) * team + in_team) * ROWS + r; }, D, e, me, last, 1);
-        const int row = tile * ROWS + r, i = quotient(A.by_group, row), g = row - i * A.group;
+        S.add<4>(part, part_ml, [&](int64_t k) { return ((k * 2 + (k == me)) * team + (SPLIT ? in_team : 0)) * ROWS + r; }, D, e, me, I.last, 1);
+        const int row = I.tile * ROWS + r, i = quotient(A.by_group, row), g = row - i * A.group;
         const float inv = S.l > 0.0f ? 1.0f / S.l : S.l == 0.0f ? 0.0f : S.l;
-        *(float4 *) (A.out + ((int64_t) (Q.first + i) * A.n_head + head * A.group + g) * D + 4 * e) =
+        *(float4 *) (A.out + ((int64_t) (Q.first + i) * A.n_head + I.head * A.group + g) * D + 4 * e) =
             make_float4(S.o.x * inv, S.o.y * inv, S.o.z * inv, S.o.w * inv);
     }
+}
+// BY workgroups a tile launch's team, and (SPLIT) one a wave of a split launch's behind them
+template <int NB, int SPLIT, int TILE, int BY>
+__global__ __launch_bounds__(256) void paged_join_teams_kernel(const paged_attn args) {
+    const paged_attn & A = kernargs_prefetched(args);
+    if ((int) blockIdx.y < BY) join_team<NB, 0, TILE>(A, blockIdx.x, blockIdx.y, BY);
+    else if (SPLIT) join_team<NB, SPLIT ? SPLIT : 16, 0>(A, blockIdx.x, blockIdx.y - BY, 0);
 }
 
 // Rows whose steps several teams took: their parts joined, a workgroup a row (or COLS columns of it), COLS / 4 threads
@@ -1151,8 +1188,8 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const paged_attn args) 
             const seq_info q = seq_of(A, s);
             mine = token >= q.first && token < q.first + q.n;
             if (SPLIT) ns = split_units(A, q, SPLIT);
-            if (TILE) nt = tile_units(A, q, TILE);
         }
+        if (TILE) nt = tile_units(A, s0, TILE);
         const uint64_t b = __ballot(mine);
         const int l = b ? __builtin_ctzll(b) : 0;
         const bool first = b && seq < 0;
@@ -1192,7 +1229,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const paged_attn args) 
     const int group = t / PER, e = t % PER, e0 = COLS < D ? (int) blockIdx.z * PER : 0;
     part_sum S;
     if (group < GROUPS) {
-        S.add(part, part_ml, [&](int64_t k) { return ((k * 2 + (k == t0)) * team + kvh % team) * rows + row - tile * rows; }, D, e0 + e, t0 + group, t1, GROUPS);
+        S.add<COLS < D ? 8 : 4>(part, part_ml, [&](int64_t k) { return ((k * 2 + (k == t0)) * team + kvh % team) * rows + row - tile * rows; }, D, e0 + e, t0 + group, t1, GROUPS);
         if (COLS < D) {                                 // a wave's groups first
 #pragma unroll
             for (int k = PER; k < WAVE; k *= 2) {
@@ -1255,6 +1292,7 @@ void split(const paged_attn & A, hipStream_t st) {
 }
 
 constexpr int64_t JOIN_FEW = 512;
+constexpr int JOIN_BY = 4;
 template <int NB>
 void attend(const paged_attn & A, const paged_ways & W, hipStream_t st) {
     constexpr int narrow = NB == 2 ? 8 : 4;
@@ -1265,9 +1303,10 @@ void attend(const paged_attn & A, const paged_ways & W, hipStream_t st) {
     const dim3 grid(A.n_tokens, A.n_head);
     if (W.tile && (int64_t) A.n_tokens * A.n_head > 4096) {
         // (a row's workgroup takes 2 us even where it finds nothing to join)
-        if (W.tile == 64) launch(paged_join_teams_kernel<NB, 0, 64>, dim3(A.tile_teams, 4), dim3(256), 0, st, A);
-        else launch(paged_join_teams_kernel<NB, 0, 128>, dim3(A.tile_teams, 8), dim3(256), 0, st, A);
-        if (W.split) launch(paged_join_teams_kernel<NB, 16, 0>, dim3(A.teams, A.team), dim3(256), 0, st, A);
+        const int most = std::max(A.teams, A.tile_teams);
+        if (W.tile == 64) launch(paged_join_teams_kernel<NB, 0, 64, 4>, dim3(A.tile_teams, 4), dim3(256), 0, st, A);
+        else if (W.split) launch(paged_join_teams_kernel<NB, 16, 128, JOIN_BY>, dim3(most, JOIN_BY + A.team), dim3(256), 0, st, A);
+        else launch(paged_join_teams_kernel<NB, 0, 128, JOIN_BY>, dim3(A.tile_teams, JOIN_BY), dim3(256), 0, st, A);
         return;
     }
     // Of few rows, whose parts are many, a workgroup joins 32 columns: one sequence of 30000 positions, 32 heads of 128,

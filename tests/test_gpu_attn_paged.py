@@ -112,6 +112,16 @@ def test_attention_of_many_tokens(hip, new, seen, H, KV, D, P):
     check(hip, draw(np.random.default_rng(sum(seen) + H + D), new, seen, H, KV, D, P))
 
 
+@pytest.mark.parametrize("D", [64, 96])
+def test_attention_of_many_tokens_of_many_sequences(hip, D):
+    """More sequences than lanes, one of them longer than the others together."""
+    rng = np.random.default_rng(70 + D)
+    new = rng.integers(0, 50, 70)
+    new[66] = 900
+    seen = new + rng.integers(0, 60, 70)
+    check(hip, draw(rng, [int(n) for n in new], [int(n) for n in seen], 4, 1, D, 16))
+
+
 @pytest.mark.parametrize("order", ["heads", "odd"])
 @pytest.mark.parametrize("new, seen, D", [([1, 1], [90, 200], 128), ([6, 2], [70, 2], 96), ([80], [200], 64)])
 def test_attention_of_other_cache_layouts(hip, order, new, seen, D):
