@@ -89,7 +89,7 @@ __device__ __forceinline__ int64_t wave_scan(int64_t v) {
 }
 
 // The units of sequence s0 + lane: by each lane over its tiles, or where one has more than three times as many as there are
-// sequences, by the whole wave over each sequence's (a prompt of 8192 tokens in 256 tiles: 13 us by a lane).
+// sequences, by the whole wave over each sequence's (a prompt of 8192 tokens in 256 tiles, 32 heads: 1.77 ms for 1.79).
 __device__ __forceinline__ int64_t tile_units(const paged_attn & A, int s0, int rows) {
     const int lane = threadIdx.x % WAVE, n = min(A.n_seqs - s0, WAVE);
     seq_info q{ 0, 0, 0, 0 };
@@ -1266,9 +1266,11 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const paged_attn args) 
     *(float4 *) (A.out + ((int64_t) token * A.n_head + head) * D + 4 * (e0 + t)) = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
 }
 
-// Rows a sequence on average: up to 8 (of heads of 64) or 4 go narrow and up to 16 wide, a wave by itself; more in tiles of
-// 64. Past 64 in tiles of 128, and the sequences among them that have 16 or fewer by waves: a batch of prompts' parts and single
-// tokens.
+// Rows a sequence on average. Up to 8 (of heads of 64) or 4 go narrow (32 sequences of 4096 positions, 32 heads over 8 of
+// 128: 43 us, wide 50), up to 16 wide, a wave by itself (3 tokens each of 16 such sequences: 37 us, in tiles of 64 53), more
+// in tiles: of 64, and of 128 where there are many (8 sequences' 50 tokens 119 us in tiles of 64 and 123 of 128, 150 254 and
+// 227, one's 200 71 and 90). Past 64 rows the sequences among them that have 16 or fewer go by waves: 31 single tokens beside
+// a prompt of 700 109 us, 319 all in tiles; what it costs where there are none is two launches' 8 us.
 struct paged_ways { int split, tile; };      // rows of a tile, 0: no such launch
 paged_ways ways_of(const paged_attn & A) {
     const int narrow = A.D == 64 ? 8 : 4;
@@ -1276,7 +1278,7 @@ paged_ways ways_of(const paged_attn & A) {
     if (rows <= narrow * per && A.group <= narrow) return { narrow, 0 };
     if (rows <= 16 * per) return { 16, 0 };
     if (rows <= 64 * per) return { 0, 64 };
-    return { per > 1 ? 16 : 0, 128 };
+    return { per > 1 ? 16 : 0, (int64_t) A.n_tokens * A.n_head <= 24576 ? 64 : 128 };
 }
 // workgroups that the CUs hold at once: more would run behind the first
 int split_wgs(int rows) { return rows < 16 ? 768 : 512; }
@@ -1292,7 +1294,7 @@ void split(const paged_attn & A, hipStream_t st) {
 }
 
 constexpr int64_t JOIN_FEW = 512;
-constexpr int JOIN_BY = 4;
+constexpr int JOIN_BY = 4, JOIN_MANY = 4096;
 template <int NB>
 void attend(const paged_attn & A, const paged_ways & W, hipStream_t st) {
     constexpr int narrow = NB == 2 ? 8 : 4;
@@ -1301,10 +1303,12 @@ void attend(const paged_attn & A, const paged_ways & W, hipStream_t st) {
     if (W.split == narrow) split<NB, true>(A, st);
     else if (W.split == 16) split<NB, false>(A, st);
     const dim3 grid(A.n_tokens, A.n_head);
-    if (W.tile && (int64_t) A.n_tokens * A.n_head > 4096) {
-        // (a row's workgroup takes 2 us even where it finds nothing to join)
+    // By teams, where rows are many: 250 tokens of 32 heads over 250 positions 28 us with all launches, by rows 40, whose
+    // workgroups take 2 us even where they find nothing to join; 200 tokens over 4000 positions, with more parts, 90 and 81.
+    if (W.tile && ((int64_t) A.n_tokens * A.n_head > JOIN_MANY || W.tile == 128)) {
         const int most = std::max(A.teams, A.tile_teams);
-        if (W.tile == 64) launch(paged_join_teams_kernel<NB, 0, 64, 4>, dim3(A.tile_teams, 4), dim3(256), 0, st, A);
+        if (W.tile == 64 && W.split) launch(paged_join_teams_kernel<NB, 16, 64, JOIN_BY>, dim3(most, JOIN_BY + A.team), dim3(256), 0, st, A);
+        else if (W.tile == 64) launch(paged_join_teams_kernel<NB, 0, 64, JOIN_BY>, dim3(A.tile_teams, JOIN_BY), dim3(256), 0, st, A);
         else if (W.split) launch(paged_join_teams_kernel<NB, 16, 128, JOIN_BY>, dim3(most, JOIN_BY + A.team), dim3(256), 0, st, A);
         else launch(paged_join_teams_kernel<NB, 0, 128, JOIN_BY>, dim3(A.tile_teams, JOIN_BY), dim3(256), 0, st, A);
         return;
@@ -1312,18 +1316,17 @@ void attend(const paged_attn & A, const paged_ways & W, hipStream_t st) {
     // Of few rows, whose parts are many, a workgroup joins 32 columns: one sequence of 30000 positions, 32 heads of 128,
     // 21.8 us with both launches for 28.4 by rows; of 16 sequences (2048 such workgroups) by rows 18.6 for 22.9.
     constexpr int D = NB * 32;
-    if (W.tile < 128 && (int64_t) A.n_tokens * A.n_head * NB <= JOIN_FEW) {
+    if (!(W.split && W.tile) && (int64_t) A.n_tokens * A.n_head * NB <= JOIN_FEW) {
         const dim3 columns(A.n_tokens, A.n_head, NB);
         if (W.split == narrow) launch(paged_join_kernel<NB, narrow, 0, 32>, columns, dim3(256), 0, st, A);
-        else if (!W.tile) launch(paged_join_kernel<NB, 16, 0, 32>, columns, dim3(256), 0, st, A);
+        else if (W.split) launch(paged_join_kernel<NB, 16, 0, 32>, columns, dim3(256), 0, st, A);
         else launch(paged_join_kernel<NB, 0, 64, 32>, columns, dim3(256), 0, st, A);
         return;
     }
     if (W.split == narrow) launch(paged_join_kernel<NB, narrow, 0, D>, grid, dim3(256), 0, st, A);
     else if (!W.tile) launch(paged_join_kernel<NB, 16, 0, D>, grid, dim3(256), 0, st, A);
-    else if (W.tile == 64) launch(paged_join_kernel<NB, 0, 64, D>, grid, dim3(256), 0, st, A);
-    else if (W.split) launch(paged_join_kernel<NB, 16, 128, D>, grid, dim3(256), 0, st, A);
-    else launch(paged_join_kernel<NB, 0, 128, D>, grid, dim3(256), 0, st, A);
+    else if (W.split) launch(paged_join_kernel<NB, 16, 64, D>, grid, dim3(256), 0, st, A);
+    else launch(paged_join_kernel<NB, 0, 64, D>, grid, dim3(256), 0, st, A);
 }
 
 // rows of parts: two a team of waves, or a workgroup
