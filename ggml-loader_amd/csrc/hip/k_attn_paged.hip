@@ -12,6 +12,12 @@
 // The rows of z land in the registers as o's operand B wants them, so p never leaves its lane.
 // K's dwords are exchanged between lanes so that a lane has the four values of a block that its k-index
 // wants; V passes through LDS, whose transposing read gives a lane one value's codes at 16 positions.
+//
+// Few rows are bound by the vector unit's issue (decoding, exponentials, p's halves: 366 instructions a step of 32
+// positions): 32 sequences of up to 16384 positions, 24 heads over 8 of 128, 53 us, 3.2 TB/s of the cache, where a copy
+// reaches 4.7; a single sequence by latency (4113 positions, 32 heads over 8: 8 us and 5 for the join). Many rows are bound by
+// the matrix and the vector units, which take turns on a SIMD: parts of 700 tokens of two prompts over 8192 positions,
+// 32 heads over 8 of 128, 407 us, 363 TFLOP/s of the formula's products, five matrix products for each two of it.
 #include "kernels.h"
 #include "ssm_ops.h"
 
@@ -1303,8 +1309,9 @@ void attend(const paged_attn & A, const paged_ways & W, hipStream_t st) {
     if (W.split == narrow) split<NB, true>(A, st);
     else if (W.split == 16) split<NB, false>(A, st);
     const dim3 grid(A.n_tokens, A.n_head);
-    // By teams, where rows are many: 250 tokens of 32 heads over 250 positions 28 us with all launches, by rows 40, whose
-    // workgroups take 2 us even where they find nothing to join; 200 tokens over 4000 positions, with more parts, 90 and 81.
+    // By teams, where rows are many: of 32 heads over 8 of 128, 250 tokens over 250 positions take 25 us with all launches, and
+    // joined by rows, whose workgroups take 2 us even where they find nothing to join, 41; 60 tokens over 4000, with few rows
+    // and many parts, 75 and 45.
     if (W.tile && ((int64_t) A.n_tokens * A.n_head > JOIN_MANY || W.tile == 128)) {
         const int most = std::max(A.teams, A.tile_teams);
         if (W.tile == 64 && W.split) launch(paged_join_teams_kernel<NB, 16, 64, JOIN_BY>, dim3(most, JOIN_BY + A.team), dim3(256), 0, st, A);

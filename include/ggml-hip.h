@@ -31,7 +31,7 @@ GGML_API ggml_backend_buffer_type_t ggml_backend_hip_buffer_type(int device);
 
 // ggml_backend_graph_compute without any device allocation: no counterpart in the reference; for
 // callers that cannot allocate (serving loops, harnesses that forbid hipMalloc). The kernels'
-// scratch (attention scores and partials, quantized activations, expert groups, argmax parts, scans'
+// scratch (attention scores and partials, a paged attention's parts (up to 98 MiB), quantized activations, expert groups, argmax parts, scans'
 // prepared operands and segment states: ggml_backend_hip_scan_scratch of the largest scan)
 // comes from a file-scope device array of GGML_HIP_STATIC_SCRATCH_BYTES that every GPU the
 // library runs on holds until the process ends; the graph's tensors are the caller's as with
