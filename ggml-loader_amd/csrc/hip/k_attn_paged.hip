@@ -17,7 +17,7 @@
 // positions): 32 sequences of up to 16384 positions, 24 heads over 8 of 128, 53 us, 3.2 TB/s of the cache, where a copy
 // reaches 4.7; a single sequence by latency (4113 positions, 32 heads over 8: 8 us and 5 for the join). Many rows are bound by
 // the matrix and the vector units, which take turns on a SIMD: parts of 700 tokens of two prompts over 8192 positions,
-// 32 heads over 8 of 128, 407 us, 363 TFLOP/s of the formula's products, five matrix products for each two of it.
+// 32 heads over 8 of 128, 402 us, 367 TFLOP/s of the formula's products, five matrix products for each two of it.
 #include "kernels.h"
 #include "ssm_ops.h"
 
