@@ -9,8 +9,8 @@
 //
 // A thread holds four values of a row and its pair's other four (read twice, the second time from the
 // cache), eight threads one block of a quantized row; a workgroup 1024 values, whose tokens' cosines its
-// threads form once for all heads. Bound by launch and load latency for a few tokens (8 tokens' 12 rows of 128
-// rotated: 6 us with their launch); 2100 tokens of 28 + 4 heads of 128 rotate in 26 us, 3.3 TB/s; 4096 tokens of 8 heads
+// threads form once for all heads. Bound by launch and load latency for a few tokens (16 tokens' 40 heads of 128
+// rotated: 6 us with their launch); 2100 tokens of 32 + 8 heads of 128 rotate in 26 us, 3.3 TB/s; 4096 tokens of 8 heads
 // of 128, K rotated and both into 4 bits, take 25 us.
 //
 // Of rows with one index the last is stored: a workgroup looks its indices up among the later ones of its
@@ -297,8 +297,9 @@ static void launch_units(const rows_batch & B, int units, dim3 grid, hipStream_t
 }
 
 // One launch for jobs of up to ROWS_PASS rows that have no third and fourth extent; else a job and a pass at a time.
-// Four units a workgroup where one would give more than ROWS_MANY: a token's cosines then serve four times the values,
-// or all threads form some.
+// Four units a workgroup where one would give more than ROWS_MANY workgroups: a token's cosines and the search for equal
+// indices then serve four times the values (2100 tokens of 40 heads of 128 rotate in 26 us, by one unit in 38); of few tokens
+// one, so that all CUs have some (96 tokens' append into F16 5.5 us, by four 9.2).
 constexpr int64_t ROWS_MANY = 2048;
 void launch_rows(rows_batch & B, hipStream_t st) {
     bool together = true;

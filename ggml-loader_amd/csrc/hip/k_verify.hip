@@ -13,6 +13,8 @@
 // adds up its weights, and one a sequence looks for the segment, and in it for the token. (The last segment's
 // workgroup to end could do that: but to make its sums visible to it every workgroup writes its die's cache back,
 // 130 us for 64 sequences of 128256 tokens.)
+// Bound by latency: 4.7 + 2.8 + 3.8 us for one sequence of 151936 tokens, 7 + 10.4 + 4.3 for 64 of 128256 (66 MB of
+// probabilities at 6.3 TB/s, out of the memory-side cache), of calls of 28 and 38.
 #include "kernels.h"
 
 #include <algorithm>

@@ -137,6 +137,24 @@ def test_verify_follows_a_graph(hip):
     assert np.array_equal(got[0], want[0]) and np.array_equal(got[1], want[1])
 
 
+@pytest.mark.parametrize("V, off, pitch", [(2052, 0, 2052), (2052, 1, 2053), (2052, 2, 2056), (4096, 4, 4101), (4098, 4, 4104)])
+def test_verify_rows_at_any_place(hip, V, off, pitch):
+    """Rows at 16 bytes and elsewhere, in planes of two and four extents."""
+    rng = np.random.default_rng(V + off)
+    d = draw(rng, [3, 0, 2, 1, 2], V)
+    with Graph(mem=1 << 20) as g:
+        views = []
+        for rows, planes in ((d["p"], (13, 1)), (d["q"], (2, 4))):
+            wide = np.full((len(rows) * pitch + 8), np.nan, np.float32)
+            wide[off:off + len(rows) * pitch].reshape(-1, pitch)[:, :V] = rows
+            t = g.tensor(gl.F32, wide.size, data=wide)
+            views.append(g.view_3d(t, V, *planes, pitch * 4, planes[0] * pitch * 4, off * 4))
+        g.compute(hip, [])
+        got = gl.hip_verify(hip, views[0], d["drafted"], d["tokens"], d["u"], draft_probs=views[1])
+    want = ref.verify(d["p"], d["q"], d["drafted"], d["tokens"], d["u"])
+    assert np.array_equal(got[0], want[0]) and np.array_equal(got[1], want[1])
+
+
 def test_verify_refuses(hip):
     d = draw(np.random.default_rng(7), [2, 1], 100)
     g, p, q = tensors(hip, d)
