@@ -13,8 +13,8 @@
 // K's dwords are exchanged between lanes so that a lane has the four values of a block that its k-index
 // wants; V passes through LDS, whose transposing read gives a lane one value's codes at 16 positions.
 //
-// Few rows are bound by the vector unit's issue (decoding, exponentials, p's halves: 366 instructions a step of 32
-// positions): 32 sequences of up to 16384 positions, 24 heads over 8 of 128, 53 us, 3.2 TB/s of the cache, where a copy
+// Few rows are bound by the vector unit's issue (decoding, exponentials, p's halves: some 360 instructions a step of 32
+// positions): 32 sequences of up to 16384 positions, 24 heads over 8 of 128, 52.5 us, 3.2 TB/s of the cache, where a copy
 // reaches 4.7; a single sequence by latency (4113 positions, 32 heads over 8: 8 us and 5 for the join). Many rows are bound by
 // the matrix and the vector units, which take turns on a SIMD: parts of 700 tokens of two prompts over 8192 positions,
 // 32 heads over 8 of 128, 402 us, 367 TFLOP/s of the formula's products, five matrix products for each two of it.
