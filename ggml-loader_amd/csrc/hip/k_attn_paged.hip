@@ -62,7 +62,7 @@ __device__ __forceinline__ seq_info seq_of(const paged_attn & A, int s) {
     q.first = min(max(a, 0), A.n_tokens);
     q.n = min(max(b, q.first), A.n_tokens) - q.first;
     q.len = min(max(kv, 0), A.max_pages * A.page);
-    q.last = kv - 1;
+    q.last = max(kv, 0) - 1;
     return q;
 }
 
@@ -442,7 +442,8 @@ __global__ __launch_bounds__(SPLIT_WG, NARROW ? 3 : 2) void paged_split_kernel(c
         }
         // p d is formed times 2^shift, so that the largest scale seen gives 2^13 to 2^15 times the largest p
         int shift = 38;
-        const int sure = Q.last - (Q.n - 1) + quotient(A.by_group, tile * ROWS);        // positions up to here are seen by all rows
+        // positions up to here are seen by all rows (a length may be past the table)
+        const int sure = min(Q.last - (Q.n - 1) + quotient(A.by_group, tile * ROWS), Q.len - 1);
 
         for (int step = step0; step < step1; step++) {
             const bool more = step + 1 < step1;

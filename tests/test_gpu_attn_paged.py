@@ -162,6 +162,22 @@ def test_attention_of_bad_pages_and_bounds(hip, new):
     check(hip, d)
 
 
+@pytest.mark.parametrize("new, H, KV, D, P, n", [
+    ([1], 8, 1, 64, 8, 5), ([1, 1], 4, 4, 96, 7, 3), ([1], 8, 2, 128, 16, 3), ([1], 8, 2, 128, 1, 33),          # few rows, narrow
+    ([1], 16, 1, 64, 16, 5), ([2, 1], 24, 3, 96, 16, 1), ([1], 32, 4, 128, 48, 1),                              # wide, on pages of sixteens
+    ([2, 3], 8, 2, 128, 7, 6), ([1], 9, 1, 64, 100, 1),                                                         # wide, on others
+    ([1, 100], 8, 2, 64, 8, 5), ([1, 2, 150], 8, 2, 128, 16, 3), ([40], 8, 2, 96, 16, 5),                       # beside tiles, in tiles
+])
+def test_attention_of_lengths_past_the_table(hip, new, H, KV, D, P, n):
+    """Lengths are cut to a table that is full of pages, also where it ends inside a step of positions."""
+    d = draw(np.random.default_rng(n * P + H), new, [n * P] * len(new), H, KV, D, P)
+    d["pages"] = np.ascontiguousarray(d["pages"][:, :n])
+    check(hip, d)
+    for seen in (n * P + 1, n * P + 40, 1000, 2 ** 31 - 1, -2 ** 31):
+        d["seen"][:] = seen
+        check(hip, d)
+
+
 def test_attention_of_values_at_the_edges(hip):
     """Scores that leave all weight on one position, equal scores, queries and scales of any size; infinities and NaN in
     places that are masked, or on pages of others."""
