@@ -519,8 +519,15 @@ __global__ __launch_bounds__(SPLIT_WG, NARROW ? 3 : 2) void paged_split_kernel(c
             if (!P16) page_of(step + 2);
             // the largest scale of V so far
             if (__any(dmax >= __builtin_amdgcn_ldexpf(1.0f, 15 - SLACK - shift))) {
-                const float big = wave_max(dmax);
-                const int now = min(shift, 14 - SLACK - min(max(__builtin_amdgcn_frexp_expf(big < 65536.0f ? big : 65504.0f), -24), 16));
+                // of those that are finite (others make the rows that see them NaN, and cost the rest no bits); 2^-24, the
+                // smallest F16, where none is
+                float big = 0x1p-24f;
+#pragma unroll
+                for (int b = 0; b < NB; b++) {
+                    const float d = fabsf(s_d[wave][1][b * SROW + dpos]);
+                    if (d < INFINITY) big = fmaxf(big, d);
+                }
+                const int now = min(shift, 14 - SLACK - __builtin_amdgcn_frexp_expf(wave_max(big)));
                 const float keep = __builtin_amdgcn_ldexpf(1.0f, now - shift);
                 shift = now;
 #pragma unroll

@@ -222,6 +222,21 @@ def test_attention_keeps_later_positions_out(hip):
         assert (np.abs(got[:-1] - want[:-1]) <= bound[:-1]).all()
 
 
+@pytest.mark.parametrize("new, H, D", [([2], 4, 64), ([2], 2, 128), ([3], 1, 96), ([5], 4, 128), ([4], 3, 64), ([80], 4, 128)])
+@pytest.mark.parametrize("bad", [np.inf, -np.inf, np.nan])
+def test_attention_of_scales_that_are_not_finite_later(hip, new, H, D, bad):
+    """A scale of V that is no number reaches the token that sees it, and costs the others, of small values, no bits."""
+    d = draw(np.random.default_rng(D + H), new, [100], H, 1, D, 16)
+    raw = d["v"].reshape(*d["v_values"].shape[:3], -1, 18)
+    raw[..., :2].view(np.float16)[:] *= np.float16(2.0 ** -9)
+    d["v_values"] = dequantize(d["v"], gl.Q4_0, d["v_values"].size).reshape(d["v_values"].shape)
+    want, bound, _ = ref.attention(d["q"], d["k_values"], d["v_values"], d["pages"], d["start"], d["seen"], d["scale"])
+    raw[d["pages"][0, 99 // 16], 99 % 16, :, :, :2] = np.array([bad], np.float16).view(np.uint8)
+    got = computed(hip, d)
+    assert not np.isfinite(got[-1]).any()
+    assert (np.abs(got[:-1] - want[:-1]) <= bound[:-1]).all()
+
+
 def test_attention_of_a_long_cache(hip):
     """Blocks past 2^31 bytes and rows past 2^32 values of the cache: pages at its far end."""
     D, KV, P = 128, 8, 64
