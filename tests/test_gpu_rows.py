@@ -302,6 +302,38 @@ def test_append_in_order_with_what_reads_the_cache(hip):
     assert np.array_equal(got[4], want.ravel())
 
 
+@pytest.mark.parametrize("how", ["several", "neox", "normal"])
+@pytest.mark.parametrize("T, KV, D, moved", [(60, 2, 64, True), (300, 8, 128, True), (5, 30, 96, False), (40, 17, 96, False), (3, 24, 80, True)])
+def test_rows_of_the_cache_itself(hip, how, T, KV, D, moved):
+    """A cache's rows turned further and stored in it again, moved or where they were (heads across the border of what a
+    workgroup reads): bits as without fusion, and all rows read before one is stored."""
+    rng = np.random.default_rng(T + KV)
+    rows, W = T + 7, KV * D
+    fill, pos = rng.standard_normal((rows, W)).astype(np.float32), positions(rng, T, 5000)
+    idx = (rng.permutation(rows)[:T] if moved else np.arange(3, T + 3)).astype(np.int64)
+    got = []
+    for fused in (True, False):
+        gl.libs()["hip"].ggml_backend_hip_set_fusion(hip, fused)
+        with Graph(mem=1 << 20) as g:
+            cache = g.tensor(gl.F32, W, rows, data=fill)
+            x = g.view_3d(cache, D, KV, T, D * 4, W * 4, 3 * W * 4)
+            if how == "several":
+                k = multi(g, x, g.tensor(gl.I32, 4 * T, data=pos), D, (D // 8, D // 8, D // 4, 0), ref.MROPE)
+            else:
+                k = g.rope_ext(x, g.tensor(gl.I32, T, data=pos[0]), None, D, gl.ROPE_NORMAL if how == "normal" else gl.ROPE_NEOX,
+                               0, 1e4, 1.0, 0.0, 1.0, 32.0, 1.0)
+            out = g.set_rows(cache, g.reshape_2d(k, W, T), g.tensor(gl.I64, T, data=idx))
+            res = g.compute(hip, out if fused else [out, k])
+            got.append((g.read(cache).reshape(rows, W), None if fused else res[1].reshape(T, W)))
+    gl.libs()["hip"].ggml_backend_hip_set_fusion(hip, True)
+    turned = got[1][1]
+    if how == "several":
+        near(turned, *ref.rope(fill[3:T + 3].reshape(T, KV, D), pos, D, (D // 8, D // 8, D // 4, 0), ref.MROPE, 1e6))
+    want = fill.copy()
+    want[idx] = turned
+    assert np.array_equal(got[0][0], want) and np.array_equal(got[1][0], want)
+
+
 @pytest.mark.parametrize("how", ["several", "neox"])
 @pytest.mark.parametrize("T", [1, 3, 40])
 def test_append_of_normed_keys(hip, how, T):
