@@ -1622,6 +1622,13 @@ private:
         return u;
     }
 
+    // a rope_ext whose pairs, rows and batches a launch of rows holds (others are op_rope's)
+    static bool rows_take(const ggml_tensor * n) {
+        const int n_dims = n->op_params[1];
+        return n_dims >= 2 && n_dims % 2 == 0 && n_dims <= n->ne[0] && n_dims / 2 <= ROWS_MAX_CS && n->ne[0] <= INT_MAX / 4 &&
+               n->ne[1] <= INT_MAX / 4 / n->ne[0] && n->ne[3] <= 65535;
+    }
+
     // Rotations of several axes and rows stored by index from node i on, with the rotations between them, as one
     // launch: nodes whose inputs are final and none of which touches another's memory; a rotation that only a set_rows
     // reads is stored by it. False where node i is a rope_ext that no such node goes with.
@@ -1649,6 +1656,7 @@ private:
                 reads = { n->src[0], n->src[1] };
             } else {
                 if (n->src[0]->type != GGML_TYPE_F32 || n->type != GGML_TYPE_F32 || n->src[0]->nb[0] != 4) return false;
+                if (n->op == GGML_OP_ROPE && !rows_take(n)) return false;
                 for (int k = 0; k < 3; k++) {
                     if (!n->src[k]) continue;
                     if (!ready(n->src[k])) return false;

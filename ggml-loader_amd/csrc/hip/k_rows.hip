@@ -24,7 +24,6 @@ namespace {
 
 constexpr int ROWS_WG = 256;
 constexpr int ROWS_MAX_PER_WG = 32;               // rows of 8 threads
-constexpr int ROWS_MAX_CS = 512;                  // rows x pairs of a workgroup: a row has at least pairs / 2 threads
 
 __device__ __forceinline__ int64_t row_index(const rows_job & J, int64_t at) {
     return J.idx64 ? ((const int64_t *) J.idx)[at] : (int64_t) ((const int32_t *) J.idx)[at];
@@ -273,6 +272,7 @@ __global__ __launch_bounds__(ROWS_WG, 4) void rows_kernel(const rows_batch args)
 } // namespace
 
 static void rows_shape(rows_job & J) {
+    if (J.rope && (J.pairs > ROWS_MAX_CS || J.pairs * 2 > J.head)) HIP_ABORT("rows: %d pairs of heads of %d values", J.pairs, J.head);
     const int quads = (int) (((int64_t) J.width + 3) / 4);
     J.chunks = (quads + ROWS_WG - 1) / ROWS_WG;
     J.threads = J.chunks > 1 ? ROWS_WG : std::max((quads + 7) / 8 * 8, 8);

@@ -392,7 +392,8 @@ __device__ __forceinline__ int quotient(const divisor & d, int x) {
 // Rows of F32 values, rotated or not, into rows of dst (F32, F16, BF16, or the planes of Q8_0 / Q4_0): row r into row
 // idx[r], where that lies in [0, to_rows), or into row r without idx. A row is `width` values, heads of `head` at s_head.
 constexpr int ROWS_MAX_JOBS = 4;
-constexpr int ROWS_MAX_PAIRS = 128;
+constexpr int ROWS_MAX_PAIRS = 128;               // of a rotation of several axes
+constexpr int ROWS_MAX_CS = 512;                  // rows x pairs of a workgroup: a row has at least pairs / 2 threads, or all
 constexpr int64_t ROWS_PASS = 8192;
 enum { ROWS_ROPE_NONE = 0, ROWS_ROPE_MULTI = 1, ROWS_ROPE_EXT = 2 };
 struct rows_job {

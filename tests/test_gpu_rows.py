@@ -367,6 +367,30 @@ def test_append_of_normed_keys(hip, how, T):
     assert np.array_equal(got[0][2], expected(cache, values, idx, gl.Q4_0).ravel())
 
 
+@pytest.mark.parametrize("D, n_dims", [(1024, 1024), (1028, 1026), (1100, 1030), (2048, 2048), (4096, 3000)])
+@pytest.mark.parametrize("T", [2, 40])
+def test_append_of_wide_heads(hip, D, n_dims, T):
+    """Rotations of up to and past the pairs that a workgroup holds, beside rows stored by index: bits as without fusion."""
+    rng = np.random.default_rng(D + T)
+    x, pos = rng.standard_normal((T, 2, D)).astype(np.float32), rng.integers(0, 5000, T).astype(np.int32)
+    idx = rng.permutation(T + 3)[:T].astype(np.int32)
+    got = []
+    for fused in (True, False):
+        gl.libs()["hip"].ggml_backend_hip_set_fusion(hip, fused)
+        with Graph(mem=1 << 20) as g:
+            a, p, c = g.tensor(gl.F32, D, 2, T, data=x), g.tensor(gl.I32, T, data=pos), g.tensor(gl.I32, T, data=idx)
+            kc, vc = (g.tensor(gl.F16, 2 * D, T + 3, data=np.zeros((T + 3, 2 * D), np.float16)) for _ in "kv")
+            q, k = (g.rope_ext(a, p, None, n_dims, mode, 0, 1e4, 1.0, 0.0, 1.0, 32.0, 1.0) for mode in (gl.ROPE_NORMAL, gl.ROPE_NEOX))
+            res = g.compute(hip, [q, g.set_rows(kc, g.reshape_2d(k, 2 * D, T), c), g.set_rows(vc, g.reshape_2d(a, 2 * D, T), c)])
+            got.append((res[0], raw(g, kc), raw(g, vc)))
+    gl.libs()["hip"].ggml_backend_hip_set_fusion(hip, True)
+    for a, b in zip(*got):
+        assert np.array_equal(a.view(np.uint8), b.view(np.uint8))
+    want = np.zeros((T + 3, 2 * D), np.float16)
+    want[idx] = x.reshape(T, -1)
+    assert np.array_equal(got[0][2], want.view(np.uint8).ravel())
+
+
 def test_rows_of_nothing(hip):
     """No heads, no tokens, no rows, no values."""
     with Graph(mem=1 << 20) as g:
