@@ -153,8 +153,8 @@ __global__ __launch_bounds__(ROWS_WG, 4) void rows_kernel(const rows_batch args)
         }
     }
 
-    const int64_t idx0 = J.row0 + (i2 % J.c_n2) * J.c2 + (i3 % J.c_n3) * J.c3;
     if (J.idx) {
+        const int64_t idx0 = J.row0 + (i2 % J.c_n2) * J.c2 + (i3 % J.c_n3) * J.c3;
         if (t < n_rows) {
             s_at[t] = row_index(J, idx0 + row0 + t);
             s_dead[t] = s_at[t] < 0 || s_at[t] >= J.to_rows;
