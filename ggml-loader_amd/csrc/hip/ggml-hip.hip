@@ -700,6 +700,10 @@ bool graph_refused(const ggml_cgraph * g, int device) {
             if (!why && n->op == GGML_OP_SET_ROWS && (overlap(n->src[2], n->src[0]) || overlap(n->src[2], n->src[1]))) {
                 why = "set_rows: the rows share memory with what is stored into them";
             }
+            // written while other runs of the same rows, and rows, still read
+            for (int k = 0; !why && n->op == GGML_OP_FLASH_ATTN_PAGED && k < 6; k++) {
+                if (overlap(n, n->src[k])) why = "flash_attn_paged: the result shares memory with an operand";
+            }
         }
         if (!why) continue;
         fprintf(stderr, "ggml-hip: %s (node '%s')\n", why, n->name);

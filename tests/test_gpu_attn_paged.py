@@ -280,3 +280,23 @@ def test_attention_in_the_static_scratch(hip):
             core.ggml_build_forward_expand(gf, n)
             assert h.ggml_backend_hip_graph_compute_static(hip, gf) == 0
             assert np.array_equal(want.view(np.uint32), g.read(n).view(np.uint32))
+
+
+def test_attention_refuses_shared_memory(hip):
+    """A result over its queries, its cache or its lengths is refused before anything runs."""
+    d = draw(np.random.default_rng(10), [1, 6], [30, 50], 8, 2, 64, 16)
+    core = gl.libs()["core"]
+    with Graph(mem=1 << 20) as g:
+        n = node(g, d)
+        want = g.compute(hip, n)
+        gf = core.ggml_new_graph(g.ctx)
+        core.ggml_build_forward_expand(gf, n)
+        own = n.contents.data
+        for k in range(6):
+            n.contents.data = n.contents.src[k].contents.data
+            assert core.ggml_backend_graph_compute(hip, gf) != 0
+        n.contents.data = n.contents.src[0].contents.data + d["q"].nbytes - 4          # its last value alone
+        assert core.ggml_backend_graph_compute(hip, gf) != 0
+        n.contents.data = own
+        assert core.ggml_backend_graph_compute(hip, gf) == 0
+        assert np.array_equal(want.view(np.uint32), g.read(n).view(np.uint32))
