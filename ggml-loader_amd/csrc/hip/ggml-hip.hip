@@ -672,6 +672,12 @@ bool overlap(const ggml_tensor * a, const ggml_tensor * b) {
     return x.b < y.e && y.b < x.e;
 }
 
+// a rotation over its own rows, whose workgroups each have whole heads
+bool turns_in_place(const ggml_tensor * n) {
+    const ggml_tensor * a = n->src[0];
+    return n->data == a->data && ggml_is_contiguous(a) && (a->ne[0] * a->ne[1] <= ROWS_PIECE || ROWS_PIECE % a->ne[0] == 0);
+}
+
 // memory that the device's kernels can read and write: for tensors that a caller placed without a buffer
 bool on_device(const void * p, int device) {
     hipPointerAttribute_t a{};
@@ -699,6 +705,9 @@ bool graph_refused(const ggml_cgraph * g, int device) {
             // stored while others are still read
             if (!why && n->op == GGML_OP_SET_ROWS && (overlap(n->src[2], n->src[0]) || overlap(n->src[2], n->src[1]))) {
                 why = "set_rows: the rows share memory with what is stored into them";
+            }
+            for (int k = 0; !why && n->op == GGML_OP_ROPE_MULTI && k < 3; k++) {
+                if (n->src[k] && overlap(n, n->src[k]) && !(k == 0 && turns_in_place(n))) why = "rope_multi: the result shares memory with an operand";
             }
             // written while other runs of the same rows, and rows, still read
             for (int k = 0; !why && n->op == GGML_OP_FLASH_ATTN_PAGED && k < 6; k++) {
@@ -1626,9 +1635,11 @@ private:
         return u;
     }
 
-    // a rope_ext whose pairs, rows and batches a launch of rows holds (others are op_rope's)
+    // a rope_ext whose pairs, rows and batches a launch of rows holds, and that is not over its own operands (others are
+    // op_rope's)
     static bool rows_take(const ggml_tensor * n) {
         const int n_dims = n->op_params[1];
+        for (int k = 0; k < 3; k++) if (n->src[k] && overlap(n, n->src[k])) return false;
         return n_dims >= 2 && n_dims % 2 == 0 && n_dims <= n->ne[0] && n_dims / 2 <= ROWS_MAX_CS && n->ne[0] <= INT_MAX / 4 &&
                n->ne[1] <= INT_MAX / 4 / n->ne[0] && n->ne[3] <= 65535;
     }

@@ -22,7 +22,7 @@
 
 namespace {
 
-constexpr int ROWS_WG = 256;
+constexpr int ROWS_WG = ROWS_PIECE / 4;
 constexpr int ROWS_MAX_PER_WG = 32;               // rows of 8 threads
 
 __device__ __forceinline__ int64_t row_index(const rows_job & J, int64_t at) {

@@ -394,6 +394,7 @@ __device__ __forceinline__ int quotient(const divisor & d, int x) {
 constexpr int ROWS_MAX_JOBS = 4;
 constexpr int ROWS_MAX_PAIRS = 128;               // of a rotation of several axes
 constexpr int ROWS_MAX_CS = 512;                  // rows x pairs of a workgroup: a row has at least pairs / 2 threads, or all
+constexpr int ROWS_PIECE = 1024;                  // values of a longer row that a workgroup has read before it writes any, or several such
 constexpr int64_t ROWS_PASS = 8192;
 enum { ROWS_ROPE_NONE = 0, ROWS_ROPE_MULTI = 1, ROWS_ROPE_EXT = 2 };
 struct rows_job {

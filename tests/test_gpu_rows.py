@@ -391,6 +391,71 @@ def test_append_of_wide_heads(hip, D, n_dims, T):
     assert np.array_equal(got[0][2], want.view(np.uint8).ravel())
 
 
+@pytest.mark.parametrize("T, H, D", [(7, 5, 96), (3, 40, 64), (2, 9, 128)])
+def test_rope_multi_in_place(hip, T, H, D):
+    """Over its own rows, where a workgroup has whole heads: bits as into other memory."""
+    rng = np.random.default_rng(T)
+    x, pos = rng.standard_normal((T, H, D)).astype(np.float32), positions(rng, T)
+    core = gl.libs()["core"]
+    with Graph(mem=1 << 20) as g:
+        a = g.tensor(gl.F32, D, H, T, data=x)
+        n = multi(g, a, g.tensor(gl.I32, 4 * T, data=pos), D, (D // 8, D // 8, D // 4, 0), ref.MROPE)
+        want = g.compute(hip, n)
+        n.contents.data = a.contents.data
+        gf = core.ggml_new_graph(g.ctx)
+        core.ggml_build_forward_expand(gf, n)
+        assert core.ggml_backend_graph_compute(hip, gf) == 0
+        assert np.array_equal(want.view(np.uint32), g.read(a).view(np.uint32))
+
+
+def test_rope_multi_refuses_shared_memory(hip):
+    """Over parts of its rows, its positions or its factors, or its rows where a head goes over two workgroups."""
+    core = gl.libs()["core"]
+    with Graph(mem=1 << 20) as g:
+        a, f = g.tensor(gl.F32, 96, 40, 6, data=np.ones((6, 40, 96), np.float32)), g.tensor(gl.F32, 48, data=np.ones(48, np.float32))
+        p = g.tensor(gl.I32, 24, data=np.arange(24, dtype=np.int32))
+        n = multi(g, g.view_3d(a, 96, 40, 5, 384, 384 * 40, 0), g.view_1d(p, 20, 0), 96, (16, 16, 16, 0), ref.MROPE, ff=f)
+        g.compute(hip, n)
+        gf = core.ggml_new_graph(g.ctx)
+        core.ggml_build_forward_expand(gf, n)
+        own = n.contents.data
+        for at in (a.contents.data, a.contents.data + 96 * 40 * 4, p.contents.data, f.contents.data):
+            n.contents.data = at
+            assert core.ggml_backend_graph_compute(hip, gf) != 0
+        n.contents.data = own
+        assert core.ggml_backend_graph_compute(hip, gf) == 0
+
+
+@pytest.mark.parametrize("D, H", [(96, 40), (64, 3)])
+def test_rope_in_place_beside_rows(hip, D, H):
+    """A rope_ext over its own rows, before rows stored by index: bits as without fusion."""
+    rng = np.random.default_rng(D)
+    T, core = 30, gl.libs()["core"]
+    x, v = (rng.standard_normal((T, H, D)).astype(np.float32) for _ in "kv")
+    pos, idx = rng.integers(0, 5000, T).astype(np.int32), rng.permutation(T + 2)[:T].astype(np.int32)
+    got = []
+    for fused in (True, False):
+        gl.libs()["hip"].ggml_backend_hip_set_fusion(hip, fused)
+        with Graph(mem=1 << 20) as g:
+            a, b, p, c = g.tensor(gl.F32, D, H, T, data=x), g.tensor(gl.F32, D * H, T, data=v), g.tensor(gl.I32, T, data=pos), g.tensor(gl.I32, T, data=idx)
+            cache = g.tensor(gl.F32, D * H, T + 2, data=np.zeros((T + 2, D * H), np.float32))
+            k = g.rope_ext(a, p, None, D, gl.ROPE_NEOX, 0, 1e4, 1.0, 0.0, 1.0, 32.0, 1.0)
+            s = g.set_rows(cache, b, c)
+            g.compute(hip, [])
+            gf = core.ggml_new_graph(g.ctx)
+            for n in (k, s):
+                core.ggml_set_output(n)
+                core.ggml_build_forward_expand(gf, n)
+            k.contents.data = a.contents.data
+            assert core.ggml_backend_graph_compute(hip, gf) == 0
+            got.append((g.read(a), g.read(cache)))
+    gl.libs()["hip"].ggml_backend_hip_set_fusion(hip, True)
+    assert all(np.array_equal(*pair) for pair in zip(*got))
+    want = np.zeros((T + 2, D * H), np.float32)
+    want[idx] = v.reshape(T, -1)
+    assert np.array_equal(got[0][1].reshape(want.shape), want)
+
+
 def test_rows_of_nothing(hip):
     """No heads, no tokens, no rows, no values."""
     with Graph(mem=1 << 20) as g:
