@@ -122,6 +122,31 @@ def test_attention_of_many_tokens_of_many_sequences(hip, D):
     check(hip, draw(rng, [int(n) for n in new], [int(n) for n in seen], 4, 1, D, 16))
 
 
+@pytest.mark.parametrize("new, seen, H, KV, D, P", [
+    ([25], [180], 1000, 1, 64, 16), ([26], [26], 1024, 8, 96, 10), ([200], [270], 128, 16, 128, 16), ([26], [90], 1000, 4, 128, 7),
+    ([500, 1, 310, 3, 0], [560, 300, 310, 70, 9], 32, 8, 64, 64), ([20, 1, 9], [150, 40, 33], 840, 20, 96, 16),
+    ([410, 2, 1, 400, 1], [500, 400, 1, 400, 129], 32, 4, 128, 24),
+])
+def test_attention_of_prompts(hip, new, seen, H, KV, D, P):
+    """Tiles of 128 rows, beside sequences of few rows and without: last tiles in part, a missing page, scales of V that
+    are no numbers at positions that no token sees, and at the last that one does."""
+    assert sum(new) * H > 24576 and sum(new) * (H // KV) > 64 * len(new)
+    d = draw(np.random.default_rng(sum(seen) + D), new, seen, H, KV, D, P)
+    if seen[0] > new[0] + 2 * P:
+        d["pages"][0, 1] = -1
+    want, bound, _ = ref.attention(d["q"], d["k_values"], d["v_values"], d["pages"], d["start"], d["seen"], d["scale"])
+    last, row = d["pages"][0, (seen[0] - 1) // P], (seen[0] - 1) % P
+    raw = d["v"].reshape(*d["v_values"].shape[:3], -1, 18)
+    raw[last, row + 1:, :, :, :2] = np.array([np.nan], np.float16).view(np.uint8)
+    off = np.abs(computed(hip, d) - want)
+    assert (off <= bound).all(), (off - bound).max()
+    raw[last, row, :, :, :2] = np.array([np.inf], np.float16).view(np.uint8)
+    got = computed(hip, d)
+    others = np.arange(len(got)) != new[0] - 1
+    assert not np.isfinite(got[new[0] - 1]).any()
+    assert (np.abs(got - want)[others] <= bound[others]).all()
+
+
 @pytest.mark.parametrize("order", ["heads", "odd"])
 @pytest.mark.parametrize("new, seen, D", [([1, 1], [90, 200], 128), ([6, 2], [70, 2], 96), ([80], [200], 64)])
 def test_attention_of_other_cache_layouts(hip, order, new, seen, D):
