@@ -4,8 +4,8 @@
 //   o = sum_j e^(z_j - m) v_j / sum_j e^(z_j - m),  z_j = scale q . k_j,  m = max_j z_j,
 // with k_j = d (c - 8) for each block of 32 codes c under one scale d, and v_j likewise.
 //
-// Both products run on the F16 matrix cores without losing bits of the 32-bit operands: the codes are
-// small integers, exact in F16, and the other operand goes in as two halves (22 bits, two products).
+// Both products run on the F16 matrix cores: the codes are small integers, exact in F16, and the other operand goes in
+// as two halves (two products), which hold 22 of its 24 bits.
 //   z: A = codes - 8 of 16 positions, B = 16 rows (query, head) of one KV head, a block of 32 values at a time;
 //      the block's sum times the block's scale, in 32 bits.
 //   o: A = codes - 8 of 16 values' columns at 32 positions, B = p d, with the scale of each position's block.
@@ -13,11 +13,21 @@
 // K's dwords are exchanged between lanes so that a lane has the four values of a block that its k-index
 // wants; V passes through LDS, whose transposing read gives a lane one value's codes at 16 positions.
 //
-// Few rows are bound by the vector unit's issue (decoding, exponentials, p's halves: some 360 instructions a step of 32
-// positions): 32 sequences of up to 16384 positions, 24 heads over 8 of 128, 52.5 us, 3.2 TB/s of the cache, where a copy
-// reaches 4.7; a single sequence by latency (4113 positions, 32 heads over 8: 8 us and 5 for the join). Many rows are bound by
-// the matrix and the vector units, which take turns on a SIMD: parts of 700 tokens of two prompts over 8192 positions,
-// 32 heads over 8 of 128, 402 us, 367 TFLOP/s of the formula's products, five matrix products for each two of it.
+// What has fewer bits than a sum of 32-bit products (half the smallest F16, 2^-25, is where halves end):
+//   q: 22 bits, of values below 2^-16 of their row's largest fewer, none below 2^-38 of it;
+//   few rows: p d, 22 bits, fewer below 2^-12 of the largest finite scale d that the wave has met (at positions that its
+//     rows see or not), none below 2^-34 of it;
+//   many: p, 22 bits, fewer below 2^-14, none below 2^-36; V in all its 15 bits, but for scales below 2^-25 of the largest
+//     so far in the same place of their heads; of the four products of halves the least, at most 2^-22 p |v|, is left out.
+// Errors against 64 bits are 2e-7 to 8e-7 of the output; the formula in 32-bit steps has 5e-7 to 2e-6.
+//
+// Few rows: 32 sequences of up to 16384 positions, 24 heads over 8 of 128, 52.4 us, 3.2 TB/s of the cache, where a copy
+// reaches 4.7. Of the first launch's cycles (46 us) the vector unit has 57 % (decoding, exponentials, p's halves: some 360
+// instructions a step of 32 positions), the matrix cores 15 and LDS 18; the rest is waiting, with three waves a SIMD. A
+// single sequence is bound by latency (4113 positions, 32 heads over 8: 8 us and 5 for the join). Many rows: parts of 700
+// tokens of two prompts over 8192 positions, 32 heads over 8 of 128, 402 us, 367 TFLOP/s of the formula's products, five
+// matrix products for each two of it. The matrix cores have 38 % of the cycles, the vector unit 50, LDS 41: none is full, and
+// a step's reads, products and exponentials follow one another within a wave.
 #include "kernels.h"
 #include "ssm_ops.h"
 
@@ -1285,6 +1295,10 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const paged_attn args) 
 // in tiles: of 64, and of 128 where there are many (8 sequences' 50 tokens 119 us in tiles of 64 and 123 of 128, 150 254 and
 // 227, one's 200 71 and 90). Past 64 rows the sequences among them that have 16 or fewer go by waves: 31 single tokens beside
 // a prompt of 700 109 us, 319 all in tiles; what it costs where there are none is two launches' 8 us.
+// The lengths are the device's, so the average is all that the host knows of a mixture, and below 64 rows it chooses badly
+// where a prompt's part is among many single tokens. Over 4000 positions, 32 heads over 8, the part's and the tokens' nodes by
+// themselves for one of both: 31 tokens and 512 161 us for 170 (by waves and in tiles), 34 and 512 164 for 207 and 48 and
+// 512 176 for 239 (all in tiles), 199 and 500 357 for 438 (all by waves).
 struct paged_ways { int split, tile; };      // rows of a tile, 0: no such launch
 paged_ways ways_of(const paged_attn & A) {
     const int narrow = A.D == 64 ? 8 : 4;

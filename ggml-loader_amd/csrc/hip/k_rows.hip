@@ -11,7 +11,8 @@
 // cache), eight threads one block of a quantized row; a workgroup 1024 values, whose tokens' cosines its
 // threads form once for all heads. Bound by launch and load latency for a few tokens (16 tokens' 40 heads of 128
 // rotated: 6 us with their launch); 2100 tokens of 32 + 8 heads of 128 rotate in 26 us, 3.3 TB/s; 4096 tokens of 8 heads
-// of 128, K rotated and both into 4 bits, take 25 us.
+// of 128, K rotated and both into 4 bits, take 25 us in two rounds of workgroups (34 KB of LDS and 128 registers: four a CU), whose
+// waves wait for 55 % of their cycles: loads, indices, cosines and stores follow one another.
 //
 // Of rows with one index the last is stored: a workgroup looks its indices up among the later ones of its
 // pass (at most ROWS_PASS rows; passes follow one another on the stream).

@@ -332,7 +332,8 @@ GGML_API struct ggml_tensor * ggml_set_rows(struct ggml_context * ctx, struct gg
 // position j of sequence s is row j % page_size of page pages[j / page_size, s] (pages: I32 [max_pages, n_seqs]). Head h reads
 // KV head h / (n_head / n_head_kv). Result: F32 [d, n_head, n_tokens], o = sum_j softmax_j(scale q . k_j) v_j over the positions
 // up to the token's own. A token without positions gets zeros. Tokens of no sequence keep what the result's memory held.
-// Positions on a page outside [0, n_pages) do not exist; kv_len is cut to the table, q_start to the tokens.
+// Positions on a page outside [0, n_pages) do not exist; kv_len is cut to the table, q_start to the tokens. The result shares no
+// memory with an operand.
 GGML_API struct ggml_tensor * ggml_flash_attn_paged(struct ggml_context * ctx, struct ggml_tensor * q, struct ggml_tensor * k,
         struct ggml_tensor * v, struct ggml_tensor * pages, struct ggml_tensor * q_start, struct ggml_tensor * kv_len, float scale);
 
