@@ -673,7 +673,7 @@ __global__ __launch_bounds__(SPLIT_WG, NARROW ? 3 : 2) void paged_split_kernel(c
 //
 // A workgroup takes 64 or 128 rows of one KV head, a wave 16 of them, in steps of 64 positions. Each wave decodes a block of
 // the step's keys or values (of four waves, both) for all: codes - 8 of K as A wants them, and V's values
-// d (codes - 8) as two halves (15 bits: exactly), so that p is split once for all blocks (three products: hi hi,
+// d (codes - 8) as two halves (15 bits: exact but for the smallest scales), so that p is split once for all blocks (three products: hi hi,
 // lo hi, hi lo). V's scales are taken times 2^s of each block, so that the largest so far is at 2^11 to 2^12; a scale that
 // is not finite counts as 0, and makes the results of the rows that see it NaN.
 template <int NB, int WAVES>
