@@ -1681,8 +1681,9 @@ private:
                 const bool wm = multi, we = ext;
                 if (!rows_rotated(B, J, n, multi, ext)) return false;
                 stored = rows_stored(j);
-                // (rows of the cache itself, moved or turned in place: read before any of them is stored)
-                for (const ggml_tensor * t : reads) if (stored >= 0 && overlap(t, g_->nodes[stored])) stored = -1;
+                // (rows of the cache itself, moved or turned in place: read before any of them is stored; and a rotation over
+                // its own rows, which others may read, is written)
+                for (const ggml_tensor * t : reads) if (stored >= 0 && (overlap(t, g_->nodes[stored]) || overlap(t, n))) stored = -1;
                 if (stored >= 0) {
                     const ggml_tensor * r = g_->nodes[stored];
                     std::vector<int> inside = members;

@@ -408,6 +408,33 @@ def test_rope_multi_in_place(hip, T, H, D):
         assert np.array_equal(want.view(np.uint32), g.read(a).view(np.uint32))
 
 
+def test_rope_multi_in_place_is_written(hip):
+    """Over its own rows, stored by index and read by another node through the rows' own tensor: bits as without fusion."""
+    rng = np.random.default_rng(1)
+    x, pos, core = rng.standard_normal((5, 3, 64)).astype(np.float32), positions(rng, 5), gl.libs()["core"]
+    got = []
+    for fused in (True, False):
+        gl.libs()["hip"].ggml_backend_hip_set_fusion(hip, fused)
+        with Graph(mem=1 << 20) as g:
+            a, c = g.tensor(gl.F32, 64, 3, 5, data=x), g.tensor(gl.I32, 5, data=np.array([4, 2, 0, 1, 3], np.int32))
+            cache = g.tensor(gl.F32, 192, 5, data=np.zeros((5, 192), np.float32))
+            k = multi(g, a, g.tensor(gl.I32, 20, data=pos), 64, (8, 8, 16, 0), ref.MROPE)
+            s, y = g.set_rows(cache, g.reshape_2d(k, 192, 5), c), g.scale(a, 1.0)
+            g.compute(hip, [])
+            gf = core.ggml_new_graph(g.ctx)
+            for n in (s, y):
+                core.ggml_set_output(n)
+                core.ggml_build_forward_expand(gf, n)
+            k.contents.data = a.contents.data
+            s.contents.src[0].contents.data = a.contents.data
+            assert core.ggml_backend_graph_compute(hip, gf) == 0
+            got.append((g.read(y).reshape(5, 192), g.read(cache).reshape(5, 192)))
+    gl.libs()["hip"].ggml_backend_hip_set_fusion(hip, True)
+    assert all(np.array_equal(*pair) for pair in zip(*got))
+    near(got[0][0], *(v.reshape(5, 192) for v in ref.rope(x, pos, 64, (8, 8, 16, 0), ref.MROPE, 1e6)))
+    assert np.array_equal(got[0][1][[4, 2, 0, 1, 3]], got[0][0])
+
+
 def test_rope_multi_refuses_shared_memory(hip):
     """Over parts of its rows, its positions or its factors, or its rows where a head goes over two workgroups."""
     core = gl.libs()["core"]
